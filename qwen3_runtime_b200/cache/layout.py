@@ -20,6 +20,22 @@ from dataclasses import dataclass
 from .manager import GroupSpec
 
 
+def four_bit_groups(head_dim: int) -> int:
+    """Groups of channels of a head that is held in 4 bits: the fewest equal ones of at most 64 channels, each of whole words of 8."""
+    words = head_dim // 8
+    return next(g for g in range(-(-head_dim // 64), words + 1) if words % g == 0)
+
+
+def four_bit_token_bytes(head_dim: int) -> int:
+    """Bytes of one token's key and value of one head: 4 bits a number, a bfloat16 scale and minimum a group."""
+    return head_dim + 8 * four_bit_groups(head_dim)
+
+
+def four_bit_page_bytes(head_dim: int, page_size: int) -> int:
+    """Bytes of one page and kv head (the layout: csrc/four_bit.cuh)."""
+    return -(-page_size * four_bit_token_bytes(head_dim) // 16) * 16
+
+
 @dataclass(frozen=True)
 class KVLayerSpec:
     """``value_dim``: values have a size of their own (None: the keys' ``head_dim``); keys and values

@@ -9,6 +9,7 @@ kernel does not support; they never substitute another code path silently.
 
 from __future__ import annotations
 
+import copy
 import ctypes
 import functools
 import math
@@ -16,6 +17,7 @@ from ctypes import c_float, c_int, c_long, c_void_p
 
 import torch
 
+from ..cache.layout import four_bit_page_bytes, four_bit_token_bytes
 from . import build
 
 _CODES = {1: "unsupported size or option", 2: "CUDA launch failed", 3: "bad argument"}
@@ -232,6 +234,23 @@ _SIGNATURES = {
         "q3_chunk_attention_decode": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                       c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                       c_int, c_float, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p],
+    },
+    "cache_4bit": {
+        "q3_store_4bit": [c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p,
+                          c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int,
+                          c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+        "q3_unpack_4bit": [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
+                           c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+        "q3_evict_4bit": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int,
+                          c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
+    },
+    "attention_4bit": {
+        "q3_decode_attention_4bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
+                                     c_int, c_void_p, c_void_p],
+        "q3_attention_mass_4bit": [c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
+                                   c_void_p],
     },
     "gemm_f32": {
         "q3_gemm_f32": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
@@ -2063,6 +2082,250 @@ class CudaOps:
                    _ptr(tickets), _ptr(longest), keep_first, _ptr(sink), _ptr(gate),
                    gate.stride(0) if gate is not None else 0, float(softcap or 0.0))
         return out
+
+    # ---- a cache in 4 bits (csrc/four_bit.cuh says how a page is laid out and how values are rounded) ----------------------
+    EVICT_KEYS = 49152  # tokens of a sequence whose keys one block sorts in shared memory; longer ones use scratch
+
+    def _check_4bit(self, what, pages, num_kv_heads, head_dim, page_size, block_table=None, kv_lens=None, layers=False):
+        if head_dim % 16 or not 16 <= head_dim <= 256 or page_size < 1 or num_kv_heads < 1:
+            raise KernelError(f"{what}: head sizes are multiples of 16 up to 256, pages and heads at least one "
+                              f"(got head_dim={head_dim}, page_size={page_size}, num_kv_heads={num_kv_heads})")
+        shape = (num_kv_heads, four_bit_page_bytes(head_dim, page_size))
+        if (pages.dtype != torch.uint8 or pages.dim() not in ((3, 4) if layers else (3,)) or tuple(pages.shape[-2:]) != shape
+                or not pages.is_contiguous()):
+            raise KernelError(f"{what}: pages are dense uint8 [pages, {shape[0]}, {shape[1]}], got {pages.dtype} {tuple(pages.shape)}")
+        self._check_here(what, pages)
+        if block_table is not None:
+            if (block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous()
+                    or block_table.shape[1] < 1):
+                raise KernelError(f"{what}: the block table is dense int32 [sequences, pages], at least one page wide")
+            self._check_here(what, block_table)
+        if kv_lens is not None:
+            if kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous() or kv_lens.numel() < (block_table.shape[0]):
+                raise KernelError(f"{what}: lengths are dense int32, one per row of the block table")
+            self._check_here(what, kv_lens)
+
+    def _check_here(self, what, *tensors):
+        for t in tensors:
+            if t is not None and (not t.is_cuda or t.device.index != self._device_index):
+                raise KernelError(f"{what}: this kernel table launches on cuda:{self._device_index}, a tensor is on {t.device}")
+
+    def _check_cells(self, what, t, dtype, pages, page_size):
+        """Sums and places: one number per (page, kv head, token)."""
+        if t is not None:
+            if t.dtype != dtype or t.shape != (*pages.shape[:-1], page_size) or not t.is_contiguous():
+                raise KernelError(f"{what}: sums are float32 and places int32, dense {tuple(pages.shape[:-1]) + (page_size,)}, "
+                                  f"got {t.dtype} {tuple(t.shape)}")
+            self._check_here(what, t)
+
+    def qk_norm_rope_store_4bit(self, qkv, *, num_heads, num_kv_heads, head_dim, q_weight, k_weight, eps, cos, sin, positions,
+                                token_seq, block_table, pages, page_size, write_kv=True, pairing="half", q_out=None, slots=None,
+                                mass=None, places=None):
+        """:meth:`qk_norm_rope_store` for a cache in 4 bits: per-head q/k norm, rotation, and the write of k and v into ``pages``
+        (uint8 ``[pages, kv heads, four_bit_page_bytes(head_dim, page_size)]``).  Queries go to ``q_out`` ``[T, num_heads *
+        head_dim]``, or are changed in place.  ``slots`` (int32 ``[T]``): each token's place in its sequence's cache, where that is
+        not its position (tokens were evicted).  ``mass`` / ``places`` (float32 / int32 ``[pages, kv heads, page_size]``): what
+        eviction goes by; the written tokens' sums become zero, their places their positions."""
+        what = "qk_norm_rope_store_4bit"
+        T = qkv.shape[0]
+        code = _dtype_code(qkv.dtype)
+        self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table)
+        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < (num_heads + (2 * num_kv_heads if write_kv else 0)) * head_dim:
+            raise KernelError(f"{what}: the projection is [tokens, heads * head_dim] with unit-stride rows")
+        q_out = qkv if q_out is None else q_out
+        if (q_out.dtype != qkv.dtype or q_out.dim() != 2 or q_out.shape[0] != T or q_out.shape[1] < num_heads * head_dim
+                or (T and q_out.stride(1) != 1)):
+            raise KernelError(f"{what}: queries go to [tokens, heads * head_dim] of the projection's type, unit-stride rows")
+        for t, name in ((positions, "positions"), (token_seq, "token_seq"), (slots, "slots")):
+            if t is not None and (t.dtype != torch.int32 or t.numel() != T or not t.is_contiguous()):
+                raise KernelError(f"{what}: {name} are dense int32, one per token")
+        for w in (q_weight, k_weight):
+            if w is not None and (w.dtype != torch.float32 or w.numel() != head_dim or not w.is_contiguous()):
+                raise KernelError(f"{what}: norm weights are dense float32 vectors of head_dim")
+        if (cos is None) != (sin is None):
+            raise KernelError(f"{what}: cos and sin come together")
+        if cos is not None and (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < 1 or 2 * cos.shape[1] > head_dim
+                                or cos.dtype != torch.float32 or sin.dtype != torch.float32
+                                or not cos.is_contiguous() or not sin.is_contiguous()):
+            raise KernelError(f"{what}: rotation tables are dense float32 [positions, pairs] of one shape, at least one position")
+        self._check_cells(what, mass, torch.float32, pages, page_size)
+        self._check_cells(what, places, torch.int32, pages, page_size)
+        self._check_here(what, qkv, q_out, positions, token_seq, slots, q_weight, k_weight, cos, sin)
+        if self.timing is not None:
+            e = qkv.element_size()
+            self._costs(T * (2 * num_heads + 2 * num_kv_heads) * head_dim * e + T * num_kv_heads * four_bit_token_bytes(head_dim))
+        self._call("cache_4bit", "q3_store_4bit", what, code, _ptr(qkv), qkv.stride(0), _ptr(q_out), q_out.stride(0), num_heads,
+                   num_kv_heads, head_dim, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
+                   cos.shape[1] if cos is not None else 0, cos.shape[0] if cos is not None else 0, _ptr(positions), _ptr(slots),
+                   _ptr(token_seq), _ptr(block_table), block_table.shape[1], block_table.shape[0], _ptr(pages), pages.shape[0],
+                   page_size, T, int(bool(write_kv)), self.PAIRINGS[pairing], _ptr(mass), _ptr(places),
+                   _ptr(self._error_word(qkv.device)))
+        return q_out
+
+    def unpack_4bit(self, pages, *, num_kv_heads, head_dim, page_size, block_table, kv_lens, max_kv_len, dtype):
+        """Keys and values of the sequences' first ``max_kv_len`` tokens as wide pages ``[sequences * n, kv heads, page_size, head_dim]``
+        of ``dtype``, ``n = ceil(max_kv_len / page_size)`` pages per sequence in order; zero behind a sequence's last token."""
+        what = "unpack_4bit"
+        self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens)
+        B, n = block_table.shape[0], -(-int(max_kv_len) // page_size)
+        if n > block_table.shape[1] or max_kv_len < 0:
+            raise KernelError(f"{what}: max_kv_len={max_kv_len} does not fit a block table of {block_table.shape[1]} pages")
+        k, v = (torch.empty((B * n, num_kv_heads, page_size, head_dim), dtype=dtype, device=pages.device) for _ in range(2))
+        self._unpack_4bit(pages, block_table, kv_lens, int(max_kv_len), None, B, n, k, v, None, page_size)
+        return k, v
+
+    def _unpack_4bit(self, pages, block_table, kv_lens, max_len, cu, count, width, k, v, table, page_size):
+        G, D = k.shape[1], k.shape[3]
+        if self.timing is not None:
+            self._costs(2 * k.numel() * k.element_size() + count * width * G * four_bit_page_bytes(D, page_size))
+        self._call("cache_4bit", "q3_unpack_4bit", "unpack_4bit", _dtype_code(k.dtype), _ptr(pages), pages.shape[0], G, D, page_size,
+                   _ptr(block_table), block_table.shape[1], _ptr(kv_lens), block_table.shape[0], max_len, _ptr(cu), count, width,
+                   int(table is None), _ptr(k), _ptr(v), _ptr(table))
+
+    def paged_attention_4bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, block_table, out, page_size, scale, step,
+                             window=None, decode_slices=None, lse=None):
+        """:meth:`paged_attention` over a cache in 4 bits.  A sequence's tokens are the first ``kv_lens`` places of its cache and the
+        step's tokens the last of them (``step.kv_lens`` and ``step.host_kv_lens`` count places: without evicted tokens, positions).
+        Single tokens of bfloat16 heads of 64, 128 or 256 read the numbers as they are (csrc/attention_4bit.cu); portions of prompts,
+        float32 and other head sizes have their sequences' pages unpacked once and go through the kernels for wide pages.
+        ``lse`` (float32 ``[T, heads]``, steps of single tokens of those sizes): gets the logarithm of each row's sum."""
+        what = "paged_attention_4bit"
+        _dtype_code(out.dtype)
+        T, D, G, H = out.shape[0], head_dim, num_kv_heads, num_heads
+        self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens)
+        if H % G or q.dtype != out.dtype or out.stride(1) != 1 or out.shape[1] != H * D or out.stride(0) != H * D:
+            raise KernelError(f"{what}: out is dense [tokens, heads * head_dim] of the queries' type, heads a multiple of kv heads")
+        self._check_here(what, q, out, lse)
+        max_len = min(step.captured_width * page_size or step.max_kv_len, block_table.shape[1] * page_size)
+        if step.max_kv_len > block_table.shape[1] * page_size:
+            raise KernelError(f"{what}: {step.max_kv_len} tokens do not fit a block table of {block_table.shape[1]} pages")
+        fast = (out.dtype == torch.bfloat16 and D in (64, 128, 256) and H // G <= 16 and q_stride % 8 == 0 and q.data_ptr() % 16 == 0
+                and out.data_ptr() % 8 == 0)
+        if lse is not None and not (fast and step.decode_only):
+            raise KernelError(f"{what}: log sums come from steps of single tokens in bfloat16, head sizes 64, 128 and 256")
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (T, H) or not lse.is_contiguous()):
+            raise KernelError(f"{what}: log sums are dense float32 [tokens, heads]")
+        if fast and step.decode_only:
+            return self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, None, step.num_seqs, max_len,
+                                     decode_slices or self.decode_slices_4bit(step.host_kv_lens, G, D, window), out, page_size, scale,
+                                     window, step.kv_longest, lse)
+        wide = dict(num_heads=H, num_kv_heads=G, head_dim=D, token_seq=step.token_seq, positions=step.positions, out=out,
+                    page_size=page_size, scale=scale, window=window)
+        n = -(-max_len // page_size)
+        split = fast and D != 256  # prompts apart from single tokens
+        cu = step.host_cu_seqlens
+        count = sum(cu[b + 1] - cu[b] > 1 for b in range(step.num_seqs)) if split else step.num_seqs
+        if split and step.num_single:
+            singles = [kv for b, kv in enumerate(step.host_kv_lens) if cu[b + 1] - cu[b] == 1]
+            self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, step.single_seqs, step.num_single, max(singles),
+                              self.decode_slices_4bit(singles, G, D, window), out, page_size, scale, window, None, None)
+        if not count:
+            return out
+        k, v = (torch.empty((count * n, G, page_size, D), dtype=out.dtype, device=out.device) for _ in range(2))
+        table = torch.empty((block_table.shape[0], n), dtype=torch.int32, device=out.device)
+        self._unpack_4bit(pages, block_table, step.kv_lens, max_len, step.cu_seqlens if split else None, count, n, k, v, table, page_size)
+        if split:
+            step = copy.copy(step)
+            step.single_seqs, step.num_single = None, 0
+        elif step.captured_width:
+            step = copy.copy(step)
+            step.captured_width = n
+        # the wide kernels number a token by its place: kv_lens and cu_seqlens say it, or for the general kernel `positions`
+        return self.paged_attention(q, q_stride, k_pages=k, v_pages=v, block_table=table, step=step, **wide)
+
+    DECODE_4BIT_BLOCKS_PER_SM = {64: 6, 128: 4, 256: 2}
+
+    def decode_slices_4bit(self, kv_lens, num_kv_heads, head_dim, window) -> int:
+        """Into how many slices the longest of these sequences' keys are cut by decode attention over a cache in 4 bits."""
+        tiles = [-(-min(n, window or n) // 64) for n in kv_lens if n > 0]
+        if not tiles:
+            return 1
+        slots = self.DECODE_4BIT_BLOCKS_PER_SM[head_dim] * self.SM_COUNT
+        per = max(1, -(-sum(tiles) * num_kv_heads // slots))
+        return max(1, min(64, -(-max(tiles) // per)))
+
+    def _decode_4bit(self, q, q_stride, H, G, D, pages, block_table, step, seq_list, num_seqs, max_len, slices, out, page_size, scale,
+                     window, longest, lse):
+        mid_o = mid_lse = None
+        if slices > 1:
+            mid_o = torch.empty((num_seqs, H, slices, D), dtype=torch.float32, device=out.device)
+            mid_lse = torch.empty((num_seqs, H, slices), dtype=torch.float32, device=out.device)
+            self.launches += 1
+        if self.timing is not None:
+            singles = [kv for b, kv in enumerate(step.host_kv_lens) if step.host_cu_seqlens[b + 1] - step.host_cu_seqlens[b] == 1]
+            self._costs(sum(singles) * G * four_bit_token_bytes(D) + 4 * num_seqs * H * D, 4 * H * D * sum(singles))
+        self._call("attention_4bit", "q3_decode_attention_4bit", "paged_attention_decode_4bit", _ptr(q), q_stride, _ptr(pages),
+                   pages.shape[0], _ptr(block_table), block_table.shape[1], _ptr(step.kv_lens), _ptr(step.cu_seqlens), _ptr(seq_list),
+                   _ptr(out), _ptr(mid_o), _ptr(mid_lse), _ptr(lse), num_seqs, H, G, D, page_size, float(scale), int(window or 0),
+                   slices, max_len, _ptr(longest))
+        return out
+
+    def attention_mass_4bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, mass, block_table, page_size, scale, step,
+                            observe=None, lse=None):
+        """Adds to ``mass`` (float32 ``[pages, kv heads, page_size]``) the softmax weights that every sequence's last ``observe`` tokens
+        of the step (None: all of them) give to its cached tokens, summed over the query heads of a kv head.  ``lse``: the rows' log
+        sums, when :meth:`paged_attention_4bit` has written them for this step.  A page belongs to one sequence."""
+        what = "attention_mass_4bit"
+        code = _dtype_code(q.dtype)
+        self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, step.kv_lens)
+        self._check_cells(what, mass, torch.float32, pages, page_size)
+        self._check_here(what, q)
+        T = step.num_tokens
+        if num_heads % num_kv_heads or q_stride % 8 or q.data_ptr() % 16:
+            raise KernelError(f"{what}: heads are a multiple of kv heads, rows of queries begin at multiples of 16 bytes")
+        if observe is not None and observe < 1:
+            raise KernelError(f"{what}: observe at least one token, or None for all")
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (T, num_heads) or not lse.is_contiguous()):
+            raise KernelError(f"{what}: log sums are dense float32 [tokens, heads]")
+        max_len = min(step.captured_width * page_size or step.max_kv_len, block_table.shape[1] * page_size)
+        observe = int(min(observe or 1 << 30, 1 << 30))
+        cu = step.host_cu_seqlens
+        counts = [min(observe, cu[b + 1] - cu[b]) for b in range(step.num_seqs)]
+        have, part, slices = lse is not None, None, 1
+        if not have:
+            lse = torch.empty((T, num_heads), dtype=torch.float32, device=q.device)
+            # about two blocks of 32 rows an SM, at least 128 keys a slice
+            blocks = num_kv_heads * sum(-(-n * (num_heads // num_kv_heads) // 32) for n in counts)
+            slices = max(1, min(16, 2 * self.SM_COUNT // max(1, blocks), max_len // 128))
+            if slices > 1:
+                part = torch.empty((T, num_heads, slices, 2), dtype=torch.float32, device=q.device)
+        if self.timing is not None:
+            seen = sum(n * kv - n * (n - 1) // 2 for n, kv in zip(counts, step.host_kv_lens))
+            self._costs(sum(step.host_kv_lens) * num_kv_heads * (four_bit_token_bytes(head_dim) // 2 + 8), 2 * num_heads * head_dim * seen)
+        self._call("attention_4bit", "q3_attention_mass_4bit", what, code, _ptr(q), q_stride, _ptr(pages), pages.shape[0],
+                   _ptr(block_table), block_table.shape[1], _ptr(step.kv_lens), _ptr(step.cu_seqlens), _ptr(mass), _ptr(lse), int(have),
+                   _ptr(part), slices, step.num_seqs, num_heads, num_kv_heads, head_dim, page_size, float(scale), max_len, observe,
+                   max(counts, default=0))
+
+    def evict_4bit(self, *, pages, mass, places, block_table, kv_lens, max_kv_len, keep, first, recent, num_kv_heads, head_dim,
+                   page_size):
+        """Cuts every sequence that holds more than ``keep`` tokens to ``keep``, per kv head: the positions below ``first`` and the last
+        ``recent`` ones stay, and of the others those with the largest ``mass`` (equal sums: the lower place).  Kept tokens behind the
+        first ``keep`` places fill the holes in front, in order; ``mass`` and ``places`` move along.  What lies behind ``keep`` afterwards
+        is nobody's.  ``max_kv_len``: no sequence is longer.  ``pages``, ``mass`` and ``places`` may have a first axis of layers, all of
+        one block table."""
+        what = "evict_4bit"
+        self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens, layers=True)
+        self._check_cells(what, mass, torch.float32, pages, page_size)
+        self._check_cells(what, places, torch.int32, pages, page_size)
+        if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+            raise KernelError(f"{what}: keep at least one token, and no fewer than first + recent (got {keep}, {first}, {recent})")
+        max_kv_len = int(max_kv_len)
+        if max_kv_len > block_table.shape[1] * page_size:
+            raise KernelError(f"{what}: max_kv_len={max_kv_len} does not fit a block table of {block_table.shape[1]} pages")
+        if max_kv_len <= keep:
+            return
+        layers = pages.shape[0] if pages.dim() == 4 else 1
+        B, cap = block_table.shape[0], min(int(keep), max_kv_len - int(keep))
+        pairs = layers * B * num_kv_heads
+        lists = torch.empty(pairs * (1 + 2 * cap), dtype=torch.int32, device=pages.device)
+        spill = torch.empty(pairs * max_kv_len, dtype=torch.int32, device=pages.device) if max_kv_len > self.EVICT_KEYS else None
+        if self.timing is not None:
+            self._costs(pairs * (8 * max_kv_len + 2 * cap * (four_bit_token_bytes(head_dim) + 8)))
+        self.launches += 1  # choose, then move
+        self._call("cache_4bit", "q3_evict_4bit", what, _ptr(pages), layers, pages.shape[-3], num_kv_heads, head_dim, page_size,
+                   _ptr(mass), _ptr(places), _ptr(block_table), block_table.shape[1], _ptr(kv_lens), B, max_kv_len, int(keep),
+                   int(first), int(recent), cap, _ptr(spill), _ptr(lists))
 
     # ---- matrix products ----------------------------------------------------------------
     def linear(self, x, weight, out=None, out_dtype=None, partial_sums=False, bias=None):
