@@ -1,37 +1,63 @@
 // Attention over a cache in 4 bits (layout: four_bit.cuh): decode attention in bfloat16, and the sums of attention weights per cached
 // token that eviction goes by.
 //
-// Numbers never leave 4 bits before the registers: a 32-bit word of 8 of them becomes four pairs of bfloat16 by a shift and a
-// (x & 0x000F000F) | 0x43004300 each, which is 128 + n exactly, and the scale, the minimum and the 128 are applied to sums:
-//   scores   K (16 keys) x Q^T (8 queries) on mma.sync m16n8k16, one accumulator per group g of channels that starts at
-//            -128 * sum_c q_c:     score = sum_g  s_g * acc_g + z_g * sum_(c in g) q_c
-//   results  V^T (16 channels) x P^T: P^T is the transposed score tile (movmatrix), times the tokens' scales per group, rounded to
-//            w_t = bf16(p_t s_t); what is the same for all channels of a group joins as three more products with constant rows:
-//              o_c = sum_t w_t (128 + n_tc)  -  136 sum_t w_t  +  sum_t p_t (z_t + 8 s_t)
-//            so that the rounding of w weighs on n - 8, which is as small as the values about their middle, and not on n (taken off
-//            as 128 with sum_t p_t z_t alone, results were 0.003 to 0.005 off, relative; so 0.0023, of which 0.0017 is the result's own
-//            rounding).
+// Numbers stay in 4 bits up to the registers, and what all channels of a group share is applied to sums:
+// A number n = 0 .. 15 in the low bits of a bfloat16 is n * 2^-133 (subnormal), and four bits further up 16 n * 2^-133 (subnormal up to 7,
+// the lowest exponent from 8 on: both have the same step).  mma.sync takes subnormal operands exactly, so a word of 8 numbers becomes
+// four operands by four masks and one shift, x & 0x000F000F, x & 0x00F000F0 and the same of x >> 8, and the other operand brings the
+// power of two that lifts the products into float32's range:
+//   scores   K (16 keys) x Q^T (8 queries) on mma.sync m16n8k16, one accumulator per group g of channels; a query row times 2^S, its
+//            largest near 2^110:
+//              score = sum_g  s_g 2^(133 - S) acc_g + z_g sum_(c in g) q_c
+//   results  V^T (16 channels) x P^T.  P^T is the score tile times the tokens' scales, w_t = bf16(p_t s_t) 2^T, transposed by movmatrix;
+//            T follows the largest scale seen, as the softmax follows the largest score:
+//              o_c = 2^(133 - T) (sum_t w_t n_tc - sum_t 8 w_t) + sum_t p_t (z_t + 8 s_t)
+//            The second sum is one more product with constant rows, the third runs in float32.  The one rounding of a weight thus
+//            weighs on n - 8, as small as the values about their middle (with w_t n_tc and z_t alone results were twice as far off).
+// (Numbers as 1 + n / 16, a shift and a mask each, took 118 us where this takes 73, eight sequences of 17,000 to 32,768 tokens, 64 heads
+// over 8 of 128; as 8-bit floats, whose byte n is n * 2^-9 without any conversion, 137: mma.sync converts those by instructions.)
 // Keys as the product's 16 rows and the kv head's queries as its 8 columns: a group of up to 8 query heads wastes nothing (the other way
 // round, 16 rows of queries, computes twice as much, and the conversion would meet half as many values per instruction).
+#include <type_traits>
+
+#include "async_tiles.cuh"
 #include "four_bit.cuh"
 #include "mma_tiles.cuh"
+
+#define Q3_ERR_WAIT_4BIT 21
 
 namespace {
 
 constexpr float MINUS_BIG = -1e30f;  // of a row that has seen nothing: a hidden key's score is -inf and weighs 2^(-inf - MINUS_BIG) = 0
 constexpr float LN_2 = 0.6931471805599453f;
 
-template <int J> __device__ __forceinline__ uint32_t pair_of(uint32_t w) {  // numbers J and J + 4 of a word, plus 128, as two bfloat16
-  return ((w >> (4 * J)) & 0x000F000Fu) | 0x43004300u;
+// Numbers J and J + 4 of a word `w` (`high`: w >> 8), or number J of two tokens whose halves were put side by side, as two bfloat16:
+// times 2^-133 (J even) or 2^-129 (J odd).
+template <int J> __device__ __forceinline__ uint32_t tiny_of(uint32_t w, uint32_t high) {
+  return (J < 2 ? w : high) & (J & 1 ? 0x00F000F0u : 0x000F000Fu);
 }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&y);
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
+// Numbers J and J + 4 of a word (or number J of two tokens whose halves were put side by side) as two bfloat16 1 + n / 16.
+template <int J> __device__ __forceinline__ uint32_t sixteenths_of(uint32_t w) {
+  const uint32_t x = J == 0 ? w << 3 : w >> (4 * J - 3 > 0 ? 4 * J - 3 : 0);
+  return (x & 0x00780078u) | 0x3F803F80u;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(a));
   return y;
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // 2^x to 2 units in the last place; below 2^-126 zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// c[16 x 8] = a[16 x 16] b[16 x 8]: a sum's first product
+__device__ __forceinline__ void mma_bf16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
@@ -47,7 +73,7 @@ template <int D> struct Head {
   static constexpr int WORDS = D / 32;     // words of a row that a lane holds
   static constexpr int ROW = D / 2;        // bytes of a row of codes
   static constexpr int PAR = 4 * G;
-  static constexpr int STAGE = 16 * (D + 2 * PAR);  // bytes of 16 tokens' keys and values
+  static constexpr int TILE = 16 * (D + 2 * PAR);  // bytes of 16 tokens' keys and values
   // word j of lane l: which group, and which 8 channels of it
   static __device__ __forceinline__ int group(int j) { return D == 64 ? 0 : j % G; }
   static __device__ __forceinline__ int index(int j, int l) {
@@ -85,23 +111,73 @@ template <int D> __device__ __forceinline__ void query_sums(float (&sum)[Head<D>
   for (int g = 0; g < Head<D>::G; ++g) sum[g][0] = c[g][0], sum[g][1] = c[g][1];
 }
 
+// The queries for the tiny numbers: as load_query's fragments, times 2^S, the channels that meet 2^-129 a 16th of it.  `undo`: what the sums
+// are to be multiplied by, for columns 2 (lane % 4) and + 1; `sum`: the channels' sums per group, both times the scores' scale.
+template <int D> __device__ __forceinline__ void load_query_tiny(uint32_t (&b)[Head<D>::WORDS][4], float (&undo)[2], float (&sum)[Head<D>::G][2],
+                                                                 const bf16* row, float scale_log2, int lane) {
+  using H = Head<D>;
+  float v[H::WORDS][8], top = 0.f, part[H::G];
+#pragma unroll
+  for (int g = 0; g < H::G; ++g) part[g] = 0.f;
+#pragma unroll
+  for (int j = 0; j < H::WORDS; ++j) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+    if (row) load8(row + 64 * H::group(j) + 8 * H::index(j, lane & 3), v[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      top = fmaxf(top, fabsf(v[j][e]));
+      part[H::group(j)] += v[j][e];
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+#pragma unroll
+    for (int g = 0; g < H::G; ++g) part[g] += __shfl_xor_sync(0xffffffffu, part[g], d);
+  }
+  // S = 110 less the largest's exponent; 120 at most (smaller rows need no more), and an infinite row stays infinite
+  const int S = min(120, 237 - (int)(__float_as_uint(top) >> 23));
+  const float even = power_of_two(S), odd = power_of_two(S - 4);
+#pragma unroll
+  for (int j = 0; j < H::WORDS; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[j][e] = pack_bf16(v[j][e] * (e & 1 ? odd : even), v[j][e + 4] * (e & 1 ? odd : even));
+  // (scores beyond 2^100 of rows beyond 2^104 come out too small, and still tell one key from all others)
+  const float back = scale_log2 * power_of_two(min(120, 133 - S));
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int from = 4 * (2 * (lane & 3) + c);
+    undo[c] = __shfl_sync(0xffffffffu, back, from);
+#pragma unroll
+    for (int g = 0; g < H::G; ++g) sum[g][c] = __shfl_sync(0xffffffffu, part[g], from) * scale_log2;
+  }
+}
+
 // ---- decode attention -------------------------------------------------------------------------------------------------------------
 // Grid (slice, kv head, sequence): a block takes one slice of one sequence's keys for one kv head and the query heads that read it; each of
-// its 4 warps takes every fourth 16 keys, with a ring of its own that cp.async fills (no barrier in the loop) and a softmax of its own;
-// the warps are joined at the end, the slices by whoever reads the partial results (merge kernel).
+// its 4 warps takes every fourth 32 keys, with a ring of its own and a softmax of its own (no barrier in the loop), and the warps are
+// joined at the end.  Where the launch leaves SMs idle, up to 16 slices are the blocks of a cluster, which read each other's results in shared
+// memory; else they go through global memory and a second kernel (a B200 holds 45 clusters of 11 of these blocks at a
+// time, 495 of the 592 blocks that it holds otherwise).
+//   BULK   page sizes that are a multiple of 16: a tile is 16 tokens of one page, brought by one bulk copy (16 tokens a page) or four
+//          that a lane asks for.  Rows behind the slice's end come along and are masked.
+//   else   any page size: cp.async token by token, what is not there is zero.
+// What bounds it: instructions.  16 tokens of 128 channels, 2304 bytes, take 100 clocks of an SM to stream; their shifts and logic run at 2
+// a clock, 128 of them for the conversion alone.
 constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
-constexpr int STEP = 16;  // keys a warp takes at a time
-constexpr int STAGES = 4;
+constexpr int STEP = 16;            // keys of a tile
+constexpr int TILES = 2;            // tiles that a warp takes at a time: what is asked and counted once for both costs half
+constexpr int ROUND = STEP * TILES * WARPS;
+constexpr int STAGES = 3;
+constexpr int MOST_CLUSTER = 16;
 
-// Rows of values are read by tokens 2l, 2l + 1 (lane % 4 = l) in pieces of lane / 4: places that let the lanes of one request hit different banks.
-template <int D> __device__ __forceinline__ int value_place(int t, int chunk) {
-  if (D == 64) return ((t & 8) + (t & 1) * 4 + ((t >> 1) & 3)) * 32 + chunk * 16;
-  if (D == 128) return (t >> 1) * 128 + (((t & 1) ^ ((t >> 1) & 1)) * 64) + (chunk ^ (((t >> 2) & 1) << 1)) * 16;
-  return t * 128 + (chunk ^ (((t >> 1) & 3) << 1)) * 16;
-}
-template <int D> __device__ __forceinline__ int key_place(int t, int chunk) {
-  return t * Head<D>::ROW + (D == 256 ? chunk ^ ((t & 1) << 2) : chunk) * 16;
+// Which token is row r of a tile (r < 8; row r + 8 is token + 8).  Any order will do, as keys and values agree on it; these let the rows
+// that one shared-memory access meets lie in different banks (D = 128: values two-way at worst).
+template <int D> __device__ __forceinline__ int token_of(int r) {
+  const int l = r >> 1;
+  return r & 1 ? 4 + (D == 64 ? (l + 2) & 3 : l ^ 1) : l;
 }
 
 struct Decode {
@@ -116,248 +192,354 @@ struct Decode {
   int nq, nkv, ps, window, splits, max_len;
   float scale_log2;
   const int* longest;
+  int* error_word;
 };
 
-// Keys per slice, the same for all sequences of the launch: the longest sequence's keys over the slices asked for, in whole rounds of the
-// block.  A shorter sequence has fewer slices.
-__device__ __forceinline__ int slice_keys(const Decode& a) {
-  int longest = a.longest ? min(*a.longest, a.max_len) : a.max_len;
-  if (a.window > 0) longest = min(longest, a.window);
-  const int per = (longest + a.splits - 1) / a.splits;
-  return max(64, (per + 63) & ~63);
-}
+// Slices are cut from the first visible key, rounded down to a tile (BULK: a tile lies in one page).  Keys per slice, the same for all
+// sequences of the launch: the longest sequence's keys over the slices asked for, in whole rounds of the block.  A shorter sequence has
+// fewer slices.
+struct Slice {
+  int kv_len, lo, begin, end, per;
+  __device__ __forceinline__ Slice(const Decode& a, int seq, int split) {
+    kv_len = min(a.kv_lens[seq], a.max_len);
+    lo = a.window > 0 ? max(0, kv_len - a.window) : 0;
+    int longest = a.longest ? min(*a.longest, a.max_len) : a.max_len;
+    if (a.window > 0) longest = min(longest, a.window + STEP - 1);
+    per = max(ROUND, ((longest + a.splits - 1) / a.splits + ROUND - 1) / ROUND * ROUND);
+    begin = (lo & ~(STEP - 1)) + split * per;
+    end = min(kv_len, begin + per);
+  }
+  __device__ __forceinline__ int count(const Decode& a) const {  // slices that have keys
+    return min(a.splits, max(0, kv_len - (lo & ~(STEP - 1)) + per - 1) / per);
+  }
+};
 
-template <int D, int NT>
-__global__ void __launch_bounds__(THREADS) decode_4bit_kernel(Decode a) {
+template <int D, int NT> constexpr int decode_blocks() { return D == 64 ? (NT == 1 ? 5 : 4) : D == 128 ? (NT == 1 ? 4 : 2) : NT == 1 ? 2 : 1; }
+
+template <int D, int NT, bool BULK, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_4bit_kernel(Decode a) {
   using H = Head<D>;
+  constexpr int QS = 8 * NT, PITCH = D + 4;
   extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) uint64_t bars[WARPS][STAGES];
   const int split = blockIdx.x, kvh = blockIdx.y, slot = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, l = lane & 3;
   const int R = a.nq / a.nkv;
+  if (BULK) {
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i) mbar_init(smem_addr(&bars[warp][i]), TILES);
+      mbar_init_fence();
+    }
+    __syncwarp();
+  }
   pdl_wait();
   const int seq = a.seq_list ? a.seq_list[slot] : slot;
-  const int kv_len = min(a.kv_lens[seq], a.max_len), tok = a.cu_seqlens[seq];
-  const int lo = a.window > 0 ? max(0, kv_len - a.window) : 0;
-  const int per = slice_keys(a);
-  const int begin = lo + split * per, end = min(kv_len, begin + per);
+  const Slice sl(a, seq, split);
+  const int tok = a.cu_seqlens[seq], begin = sl.begin, end = sl.end;
   const long out_row = (long)tok * a.nq + kvh * R;
-  if (begin >= end) {
+  if (!CLUSTER && begin >= end) {
     pdl_launch_dependents();
-    if (split == 0) {  // no key at all
-      if (a.splits > 1) {
-        if (tid < R) a.mid_lse[((long)slot * a.nq + kvh * R + tid) * a.splits] = -INFINITY;
-      } else {
-        for (int i = tid; i < R * D; i += THREADS) a.out[out_row * D + i] = __float2bfloat16_rn(0.f);
-        if (a.lse && tid < R) a.lse[out_row + tid] = -INFINITY;
-      }
+    if (a.splits == 1) {  // no key at all
+      for (int i = tid; i < R * D; i += THREADS) a.out[out_row * D + i] = __float2bfloat16_rn(0.f);
+      if (a.lse && tid < R) a.lse[out_row + tid] = -INFINITY;
     }
     return;
   }
   const Q4Page L(D, H::G, a.ps);
   const int* bt = a.block_table + (long)seq * a.max_pages;
-  unsigned char* ring = smem + warp * STAGES * H::STAGE;
-  const int steps = (end - begin + STEP * WARPS - 1) / (STEP * WARPS);
+  constexpr int STAGE = TILES * H::TILE;
+  unsigned char* ring = smem + warp * STAGES * STAGE;
 
-  // A lane copies half of the pieces of token lane / 2 of the 16.  The page is looked up a step ahead: the copies' addresses wait for it.
-  auto look_up = [&](int i) {
-    const int key = begin + (i * WARPS + warp) * STEP + (lane >> 1);
-    return key < end ? bt[key / a.ps] : -1;
-  };
-  auto load_step = [&](int i, int page) {
-    unsigned char* st = ring + (i % STAGES) * H::STAGE;
-    const int t = lane >> 1, key = begin + (i * WARPS + warp) * STEP + t;
-    const bool valid = page >= 0 && page < a.num_pages;  // (a page that was given back reads as zeros, like what lies behind the slice)
-    const unsigned char* rec = a.pages + ((long)(valid ? page : 0) * a.nkv + kvh) * L.record;
-    const int row = valid ? key % a.ps : 0;
-    constexpr int CH = H::ROW / 16;  // pieces of a row: 2, 4 or 8
+  // The token that this lane copies (BULK: lanes 0 and 1, a tile's first), as page of the sequence and row, moved on by a round at a time.
+  // Its page is looked up a step before the copy, whose address waits for it.
+  const unsigned char* head = a.pages + kvh * L.record;
+  const uint32_t page_bytes = (uint32_t)(a.nkv * L.record);
+  int at = begin + warp * STEP * TILES + (BULK ? STEP * lane : lane), at_page = at / a.ps, at_row = at - at_page * a.ps;
+  const int go_pages = ROUND / a.ps, go_rows = ROUND - go_pages * a.ps;
+  auto look_up = [&]() { return at < end ? bt[at_page] : -1; };
+  int page = -1;
+  if (!BULK || lane < TILES) page = look_up();
+  const uint32_t ring_at = smem_addr(ring) + (BULK ? lane * H::TILE : (lane >> 4) * H::TILE), bar_at = smem_addr(&bars[warp][0]);
+  auto load_step = [&](int stage) {  // the token looked up last; then the next is
+    if (BULK && lane >= TILES) return;
+    const uint32_t dst = ring_at + stage * STAGE;
+    const bool valid = (uint32_t)page < (uint32_t)a.num_pages;
+    const unsigned char* rec = head + (unsigned long long)(uint32_t)(valid ? page : 0) * page_bytes;
+    if (BULK) {  // each lane arrives once, with the bytes that it asks for
+      const uint32_t bar = bar_at + 8 * stage;
+      mbar_expect_tx(bar, valid ? H::TILE : 0);
+      if (valid) {
+        if (a.ps == STEP) {
+          bulk_copy(dst, rec, H::TILE, bar);
+        } else {
+          bulk_copy(dst, rec + at_row * H::ROW, STEP * H::ROW, bar);
+          bulk_copy(dst + STEP * H::ROW, rec + L.values + at_row * H::ROW, STEP * H::ROW, bar);
+          bulk_copy(dst + 2 * STEP * H::ROW, rec + L.kpar + at_row * H::PAR, STEP * H::PAR, bar);
+          bulk_copy(dst + 2 * STEP * H::ROW + STEP * H::PAR, rec + L.vpar + at_row * H::PAR, STEP * H::PAR, bar);
+        }
+      }
+    } else {
+      const unsigned char* src = rec + (valid ? at_row : 0) * H::ROW;
 #pragma unroll
-    for (int c = 0; c < CH / 2; ++c) {
-      const int chunk = (lane & 1) * (CH / 2) + c;
-      cp_async16(smem_u32(st + key_place<D>(t, chunk)), rec + (long)row * H::ROW + 16 * chunk, valid ? 16 : 0);
-      cp_async16(smem_u32(st + STEP * H::ROW + value_place<D>(t, chunk)), rec + L.values + (long)row * H::ROW + 16 * chunk, valid ? 16 : 0);
+      for (int c = 0; c < H::ROW / 16; ++c) {
+        cp_async16(dst + (lane & 15) * H::ROW + 16 * c, src + 16 * c, valid ? 16 : 0);
+        cp_async16(dst + (STEP + (lane & 15)) * H::ROW + 16 * c, src + L.values + 16 * c, valid ? 16 : 0);
+      }
+      const uint32_t par = dst + 2 * STEP * H::ROW + (lane & 15) * H::PAR;
+      src = rec + L.kpar + (valid ? at_row : 0) * H::PAR;
+      const long vpar = L.vpar - L.kpar;
+      if (D == 64) cp_async4(par, src, valid ? 4 : 0), cp_async4(par + STEP * H::PAR, src + vpar, valid ? 4 : 0);
+      if (D == 128) cp_async8(par, src, valid ? 8 : 0), cp_async8(par + STEP * H::PAR, src + vpar, valid ? 8 : 0);
+      if (D == 256) cp_async16(par, src, valid ? 16 : 0), cp_async16(par + STEP * H::PAR, src + vpar, valid ? 16 : 0);
+      cp_async_commit();
     }
-    const uint32_t par = smem_u32(st + 2 * STEP * H::ROW + (lane & 1) * STEP * H::PAR + t * H::PAR);
-    const unsigned char* src = rec + (lane & 1 ? L.vpar : L.kpar) + (long)row * H::PAR;
-    if (D == 64) cp_async4(par, src, valid ? 4 : 0);
-    if (D == 128) cp_async8(par, src, valid ? 8 : 0);
-    if (D == 256) cp_async16(par, src, valid ? 16 : 0);
+    at += ROUND, at_page += go_pages, at_row += go_rows;
+    if (at_row >= a.ps) at_row -= a.ps, ++at_page;
+    page = look_up();
   };
-  int next[STAGES - 1];
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) next[i] = look_up(i);
-  int ahead = look_up(STAGES - 1);
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    load_step(i, next[i]);
-    cp_async_commit();
-  }
+  for (int i = 0; i < STAGES - 1; ++i) load_step(i);
 
-  uint32_t qf[NT][H::WORDS][4];
-  float qsum[NT][H::G][2];
+  uint32_t q[NT][H::WORDS][4];
+  float qsum[NT][H::G][2], undo[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int h = 8 * n + r;
-    load_query<D>(qf[n], h < R ? a.q + (long)tok * a.q_stride + (long)(kvh * R + h) * D : nullptr, lane);
-    query_sums<D>(qsum[n], qf[n]);
+    load_query_tiny<D>(q[n], undo[n], qsum[n], h < R ? a.q + (long)tok * a.q_stride + (long)(kvh * R + h) * D : nullptr, a.scale_log2, lane);
   }
-  float o[NT][H::G][4][4], oz[NT][H::G][4], m[NT][2], sum[NT][2];
+  // o: sums of w n (times 2^-133, odd j 2^-129); oz: of -8 w (2^-133); oc: of p (z + 8 s), this lane's share; all of 16 p in place of p.
+  // lift = 2^T is set so that the largest scale seen lies in 2^100 .. 2^115, beyond which it is set anew.
+  float o[NT][H::G][4][4], oz[NT][H::G][4], oc[NT][H::G][2], m[NT][2], sum[NT][2];
+  float most_scale = -1.f, lift = 1.f;
+  int T = 0;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m[n][0] = m[n][1] = MINUS_BIG;
     sum[n][0] = sum[n][1] = 0.f;
 #pragma unroll
-    for (int g = 0; g < H::G; ++g)
+    for (int g = 0; g < H::G; ++g) {
+      oc[n][g][0] = oc[n][g][1] = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         oz[n][g][e] = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[n][g][j][e] = 0.f;
       }
+    }
   }
+  uint32_t eight[4];  // -8 * 2^-133, kept in registers: as a constant it is built anew for every product
+#pragma unroll
+  for (int e = 0; e < 4; ++e) asm volatile("mov.b32 %0, 0x80088008;" : "=r"(eight[e]));
+  const int tr = token_of<D>(r);
+  const int k_at = tr * H::ROW + (D == 64 ? 8 * l : 16 * l), par_at = 2 * STEP * H::ROW + tr * H::PAR;
+  const int va_at = (STEP + token_of<D>(2 * l)) * H::ROW + (D / 16) * r, vb_at = (STEP + token_of<D>(2 * l + 1)) * H::ROW + (D / 16) * r;
 
-  for (int i = 0; i < steps; ++i) {
-    cp_async_wait<STAGES - 2>();
-    __syncwarp();
-    const unsigned char* st = ring + (i % STAGES) * Head<D>::STAGE;
-    const int base = begin + (i * WARPS + warp) * STEP;
-    if (base < end) {
-      const unsigned char* par_k = st + 2 * STEP * H::ROW;
-      const unsigned char* par_v = par_k + STEP * H::PAR;
-      // ---- scores of 16 keys
+  int stage = 0;
+  uint32_t parity = 0;
+  // WHOLE: every key of both tiles is visible
+  auto take = [&](auto whole_tiles, const unsigned char* st, int base) {
+    constexpr bool WHOLE = decltype(whole_tiles)::value;
+    float x[TILES][NT][4];
+    uint32_t vp[TILES][2][H::G];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      const unsigned char* tile = st + t * H::TILE;
       uint32_t kw[2][H::WORDS], kp[2][H::G];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int t = r + 8 * half;
+        const unsigned char *kr = tile + k_at + 8 * half * H::ROW, *pr = tile + par_at + 8 * half * H::PAR;
         if constexpr (D == 64) {
-          *reinterpret_cast<uint2*>(&kw[half][0]) = *reinterpret_cast<const uint2*>(st + t * H::ROW + 8 * l);
-          kp[half][0] = *reinterpret_cast<const uint32_t*>(par_k + t * 4);
+          *reinterpret_cast<uint2*>(&kw[half][0]) = *reinterpret_cast<const uint2*>(kr);
+          kp[half][0] = *reinterpret_cast<const uint32_t*>(pr);
+          vp[t][half][0] = *reinterpret_cast<const uint32_t*>(pr + STEP * H::PAR);
         } else if constexpr (D == 128) {
-          *reinterpret_cast<uint4*>(&kw[half][0]) = *reinterpret_cast<const uint4*>(st + key_place<D>(t, l));
-          *reinterpret_cast<uint2*>(&kp[half][0]) = *reinterpret_cast<const uint2*>(par_k + t * 8);
+          *reinterpret_cast<uint4*>(&kw[half][0]) = *reinterpret_cast<const uint4*>(kr);
+          *reinterpret_cast<uint2*>(&kp[half][0]) = *reinterpret_cast<const uint2*>(pr);
+          *reinterpret_cast<uint2*>(&vp[t][half][0]) = *reinterpret_cast<const uint2*>(pr + STEP * H::PAR);
         } else {
-          *reinterpret_cast<uint4*>(&kw[half][0]) = *reinterpret_cast<const uint4*>(st + key_place<D>(t, l));
-          *reinterpret_cast<uint4*>(&kw[half][4]) = *reinterpret_cast<const uint4*>(st + key_place<D>(t, l + 4));
-          *reinterpret_cast<uint4*>(&kp[half][0]) = *reinterpret_cast<const uint4*>(par_k + t * 16);
+          *reinterpret_cast<uint4*>(&kw[half][0]) = *reinterpret_cast<const uint4*>(kr);
+          *reinterpret_cast<uint4*>(&kw[half][4]) = *reinterpret_cast<const uint4*>(kr + 64);
+          *reinterpret_cast<uint4*>(&kp[half][0]) = *reinterpret_cast<const uint4*>(pr);
+          *reinterpret_cast<uint4*>(&vp[t][half][0]) = *reinterpret_cast<const uint4*>(pr + STEP * H::PAR);
         }
       }
       float acc[NT][H::G][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int g = 0; g < H::G; ++g) {
-          acc[n][g][0] = acc[n][g][2] = -128.f * qsum[n][g][0];
-          acc[n][g][1] = acc[n][g][3] = -128.f * qsum[n][g][1];
-        }
-#pragma unroll
       for (int j = 0; j < H::WORDS; ++j) {
-        const uint32_t a0[4] = {pair_of<0>(kw[0][j]), pair_of<0>(kw[1][j]), pair_of<1>(kw[0][j]), pair_of<1>(kw[1][j])};
-        const uint32_t a1[4] = {pair_of<2>(kw[0][j]), pair_of<2>(kw[1][j]), pair_of<3>(kw[0][j]), pair_of<3>(kw[1][j])};
+        const uint32_t w0 = kw[0][j], w1 = kw[1][j], u0 = w0 >> 8, u1 = w1 >> 8;
+        const uint32_t a0[4] = {tiny_of<0>(w0, u0), tiny_of<0>(w1, u1), tiny_of<1>(w0, u0), tiny_of<1>(w1, u1)};
+        const uint32_t a1[4] = {tiny_of<2>(w0, u0), tiny_of<2>(w1, u1), tiny_of<3>(w0, u0), tiny_of<3>(w1, u1)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma_bf16(acc[n][H::group(j)], a0, qf[n][j][0], qf[n][j][1]);
-          mma_bf16(acc[n][H::group(j)], a1, qf[n][j][2], qf[n][j][3]);
+          if (j < H::G)  // the words of the groups come in turn: the first of each starts its sum
+            mma_bf16_first(acc[n][H::group(j)], a0, q[n][j][0], q[n][j][1]);
+          else
+            mma_bf16(acc[n][H::group(j)], a0, q[n][j][0], q[n][j][1]);
+          mma_bf16(acc[n][H::group(j)], a1, q[n][j][2], q[n][j][3]);
         }
       }
-      const bool in0 = base + r < end, in1 = base + r + 8 < end;
-      uint32_t p[NT][2];
+      bool in[2] = {true, true};
+      if (!WHOLE) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int key = base + t * STEP + tr + 8 * half;
+          in[half] = key < end && key >= sl.lo;
+#pragma unroll
+          for (int g = 0; g < H::G; ++g)
+            if (!in[half]) kp[half][g] = vp[t][half][g] = 0;  // rows that are nobody's may hold anything
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        float(&y)[4] = x[t][n];
 #pragma unroll
         for (int g = 0; g < H::G; ++g) {
-          const float s0 = q4_s(kp[0][g]), z0 = q4_z(kp[0][g]), s1 = q4_s(kp[1][g]), z1 = q4_z(kp[1][g]);
-          x[0] += s0 * acc[n][g][0] + z0 * qsum[n][g][0];
-          x[1] += s0 * acc[n][g][1] + z0 * qsum[n][g][1];
-          x[2] += s1 * acc[n][g][2] + z1 * qsum[n][g][0];
-          x[3] += s1 * acc[n][g][3] + z1 * qsum[n][g][1];
+          const float s0 = q4_s(kp[0][g]), s1 = q4_s(kp[1][g]);
+          y[0] = g ? y[0] + s0 * acc[n][g][0] : s0 * acc[n][g][0];
+          y[1] = g ? y[1] + s0 * acc[n][g][1] : s0 * acc[n][g][1];
+          y[2] = g ? y[2] + s1 * acc[n][g][2] : s1 * acc[n][g][2];
+          y[3] = g ? y[3] + s1 * acc[n][g][3] : s1 * acc[n][g][3];
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = (e < 2 ? in0 : in1) ? x[e] * a.scale_log2 : -INFINITY;
-        // the maximum moves only when it would be passed by a factor of 2^8: a weight is 2^8 at most, which float32 sums do not mind
-        const bool far = fmaxf(x[0], x[2]) > m[n][0] + 8.f || fmaxf(x[1], x[3]) > m[n][1] + 8.f;
-        if (__any_sync(0xffffffffu, far)) {
+        for (int e = 0; e < 4; ++e) y[e] *= undo[n][e & 1];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(m[n][c], fmaxf(x[c], x[c + 2]));
+        for (int g = 0; g < H::G; ++g) {
+          const float z0 = q4_z(kp[0][g]), z1 = q4_z(kp[1][g]);
+          y[0] += z0 * qsum[n][g][0];
+          y[1] += z0 * qsum[n][g][1];
+          y[2] += z1 * qsum[n][g][0];
+          y[3] += z1 * qsum[n][g][1];
+        }
+        if (!WHOLE) {
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float f = exp2f(m[n][c] - top);
-            m[n][c] = top;
-            sum[n][c] *= f;
+          for (int e = 0; e < 4; ++e) y[e] = in[e >> 1] ? y[e] : -INFINITY;
+        }
+      }
+    }
+    // The maximum moves only when it would be passed by a factor of 2^8 (a weight is 2^8 at most, which float32 sums do not mind), the
+    // lift when a scale would leave its range; hardly ever after the first tiles.
+    float top[NT][2], scale = 0.f;
+    bool far = false;
 #pragma unroll
-            for (int g = 0; g < H::G; ++g) {
-              oz[n][g][c] *= f, oz[n][g][c + 2] *= f;
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) o[n][g][j][c] *= f, o[n][g][j][c + 2] *= f;
-            }
+      for (int g = 0; g < H::G; ++g) scale = fmaxf(scale, fmaxf(q4_s(vp[t][0][g]), q4_s(vp[t][1][g])));
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        top[n][c] = fmaxf(fmaxf(x[0][n][c], x[0][n][c + 2]), fmaxf(x[1][n][c], x[1][n][c + 2]));
+        far = far || top[n][c] > m[n][c] + 8.f;
+      }
+    if (__any_sync(0xffffffffu, far || scale > most_scale)) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) scale = fmaxf(scale, __shfl_xor_sync(0xffffffffu, scale, d));
+      float down = 1.f;
+      if (scale > most_scale) {
+        const int now = min(120, 227 - (int)(__float_as_uint(scale) >> 23));  // 100 less its exponent
+        down = most_scale < 0.f ? 1.f : power_of_two(max(-126, now - T));
+        T = now;
+        lift = power_of_two(T);
+        most_scale = power_of_two(min(127, 115 - T));
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float now = fmaxf(m[n][c], top[n][c]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+          const float f = exp2_fast(m[n][c] - now), fd = f * down;
+          m[n][c] = now;
+          sum[n][c] *= f;
+#pragma unroll
+          for (int g = 0; g < H::G; ++g) {
+            oc[n][g][c] *= f, oz[n][g][c] *= fd, oz[n][g][c + 2] *= fd;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][g][j][c] *= fd, o[n][g][j][c + 2] *= fd;
           }
         }
+    }
+    uint32_t w[TILES][NT][H::G][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = exp2f(x[e] - m[n][e & 1]);
-        sum[n][0] += x[0] + x[2];
-        sum[n][1] += x[1] + x[3];
-        // weights are rounded to bfloat16 for the product, as everywhere in this engine's 16-bit attention
-        p[n][0] = transposed(pack_bf16(x[0], x[1]));
-        p[n][1] = transposed(pack_bf16(x[2], x[3]));
+    for (int n = 0; n < NT; ++n) {
+      const float off[2] = {4.f - m[n][0], 4.f - m[n][1]};
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        float(&y)[4] = x[t][n];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = exp2_fast(y[e] + off[e & 1]);
+        sum[n][0] += y[0] + y[2];
+        sum[n][1] += y[1] + y[3];
+#pragma unroll
+        for (int g = 0; g < H::G; ++g) {
+          const float s0 = q4_s(vp[t][0][g]), s1 = q4_s(vp[t][1][g]);
+          const float c0 = q4_z(vp[t][0][g]) + 8.f * s0, c1 = q4_z(vp[t][1][g]) + 8.f * s1;
+          oc[n][g][0] += y[0] * c0 + y[2] * c1;
+          oc[n][g][1] += y[1] * c0 + y[3] * c1;
+          // weight times scale is rounded to bfloat16 for the product, as weights are everywhere in this engine's 16-bit attention
+          const float l0 = s0 * lift, l1 = s1 * lift;
+          w[t][n][g][0] = transposed(pack_bf16(y[0] * l0, y[1] * l0));
+          w[t][n][g][1] = transposed(pack_bf16(y[2] * l1, y[3] * l1));
+        }
       }
-      // ---- results: tokens 2l, 2l + 1, 2l + 8, 2l + 9
-      uint32_t vw[4][H::G], vp[4][H::G];
+    }
+    // ---- results: of each tile the tokens of rows 2l, 2l + 1, 2l + 8, 2l + 9
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      const unsigned char* tile = st + t * H::TILE;
+      uint32_t vw[4][H::G];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int t = 2 * l + (e & 1) + 8 * (e >> 1);
-        const unsigned char* vs = st + STEP * H::ROW;
-        if constexpr (D == 64) {
-          vw[e][0] = *reinterpret_cast<const uint32_t*>(vs + value_place<D>(t, r >> 2) + 4 * (r & 3));
-          vp[e][0] = *reinterpret_cast<const uint32_t*>(par_v + t * 4);
-        } else if constexpr (D == 128) {
-          *reinterpret_cast<uint2*>(&vw[e][0]) = *reinterpret_cast<const uint2*>(vs + value_place<D>(t, r >> 1) + 8 * (r & 1));
-          *reinterpret_cast<uint2*>(&vp[e][0]) = *reinterpret_cast<const uint2*>(par_v + t * 8);
-        } else {
-          *reinterpret_cast<uint4*>(&vw[e][0]) = *reinterpret_cast<const uint4*>(vs + value_place<D>(t, r));
-          *reinterpret_cast<uint4*>(&vp[e][0]) = *reinterpret_cast<const uint4*>(par_v + t * 16);
-        }
+        const unsigned char* vr = tile + (e & 1 ? vb_at : va_at) + 8 * (e >> 1) * H::ROW;
+        if constexpr (D == 64) vw[e][0] = *reinterpret_cast<const uint32_t*>(vr);
+        if constexpr (D == 128) *reinterpret_cast<uint2*>(&vw[e][0]) = *reinterpret_cast<const uint2*>(vr);
+        if constexpr (D == 256) *reinterpret_cast<uint4*>(&vw[e][0]) = *reinterpret_cast<const uint4*>(vr);
       }
 #pragma unroll
       for (int g = 0; g < H::G; ++g) {
         const uint32_t lo0 = __byte_perm(vw[0][g], vw[1][g], 0x5410), hi0 = __byte_perm(vw[0][g], vw[1][g], 0x7632);
         const uint32_t lo1 = __byte_perm(vw[2][g], vw[3][g], 0x5410), hi1 = __byte_perm(vw[2][g], vw[3][g], 0x7632);
-        const uint32_t s0 = __byte_perm(vp[0][g], vp[1][g], 0x5410), z0 = __byte_perm(vp[0][g], vp[1][g], 0x7632);
-        const uint32_t s1 = __byte_perm(vp[2][g], vp[3][g], 0x5410), z1 = __byte_perm(vp[2][g], vp[3][g], 0x7632);
-        const uint32_t az[4] = {z0, z0, z1, z1};
-        const __nv_bfloat162 eight = __floats2bfloat162_rn(8.f, 8.f);
-        const uint32_t e0 = mul_bf16x2(s0, *reinterpret_cast<const uint32_t*>(&eight)), e1 = mul_bf16x2(s1, *reinterpret_cast<const uint32_t*>(&eight));
-        const uint32_t as[4] = {e0, e0, e1, e1};
-        const uint32_t off[4] = {0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u};  // -136
-        const uint32_t v0[4] = {pair_of<0>(lo0), pair_of<0>(hi0), pair_of<0>(lo1), pair_of<0>(hi1)};
-        const uint32_t v1[4] = {pair_of<1>(lo0), pair_of<1>(hi0), pair_of<1>(lo1), pair_of<1>(hi1)};
-        const uint32_t v2[4] = {pair_of<2>(lo0), pair_of<2>(hi0), pair_of<2>(lo1), pair_of<2>(hi1)};
-        const uint32_t v3[4] = {pair_of<3>(lo0), pair_of<3>(hi0), pair_of<3>(lo1), pair_of<3>(hi1)};
+        const uint32_t lu0 = lo0 >> 8, hu0 = hi0 >> 8, lu1 = lo1 >> 8, hu1 = hi1 >> 8;
+        const uint32_t v0[4] = {tiny_of<0>(lo0, lu0), tiny_of<0>(hi0, hu0), tiny_of<0>(lo1, lu1), tiny_of<0>(hi1, hu1)};
+        const uint32_t v1[4] = {tiny_of<1>(lo0, lu0), tiny_of<1>(hi0, hu0), tiny_of<1>(lo1, lu1), tiny_of<1>(hi1, hu1)};
+        const uint32_t v2[4] = {tiny_of<2>(lo0, lu0), tiny_of<2>(hi0, hu0), tiny_of<2>(lo1, lu1), tiny_of<2>(hi1, hu1)};
+        const uint32_t v3[4] = {tiny_of<3>(lo0, lu0), tiny_of<3>(hi0, hu0), tiny_of<3>(lo1, lu1), tiny_of<3>(hi1, hu1)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint32_t w0 = mul_bf16x2(p[n][0], s0), w1 = mul_bf16x2(p[n][1], s1);
-          mma_bf16(oz[n][g], az, p[n][0], p[n][1]);
-          mma_bf16(oz[n][g], as, p[n][0], p[n][1]);
-          mma_bf16(oz[n][g], off, w0, w1);
-          mma_bf16(o[n][g][0], v0, w0, w1);
-          mma_bf16(o[n][g][1], v1, w0, w1);
-          mma_bf16(o[n][g][2], v2, w0, w1);
-          mma_bf16(o[n][g][3], v3, w0, w1);
+          mma_bf16(oz[n][g], eight, w[t][n][g][0], w[t][n][g][1]);
+          mma_bf16(o[n][g][0], v0, w[t][n][g][0], w[t][n][g][1]);
+          mma_bf16(o[n][g][1], v1, w[t][n][g][0], w[t][n][g][1]);
+          mma_bf16(o[n][g][2], v2, w[t][n][g][0], w[t][n][g][1]);
+          mma_bf16(o[n][g][3], v3, w[t][n][g][0], w[t][n][g][1]);
         }
       }
     }
+  };
+  for (int base = begin + warp * STEP * TILES; base < end; base += ROUND) {
+    if (BULK)
+      mbar_wait_report(bar_at + 8 * stage, parity, a.error_word, Q3_ERR_WAIT_4BIT);
+    else
+      cp_async_wait<STAGES - 2>();
     __syncwarp();
-    load_step(i + STAGES - 1, ahead);
-    ahead = look_up(i + STAGES);
-    cp_async_commit();
+    const unsigned char* st = ring + stage * STAGE;
+    if (base + STEP * TILES <= end && base >= sl.lo)  // (of one mind over the warp)
+      take(std::true_type(), st, base);
+    else
+      take(std::false_type(), st, base);
+    __syncwarp();
+    load_step(stage ? stage - 1 : STAGES - 1);
+    if (++stage == STAGES) stage = 0, parity ^= 1;
   }
   pdl_launch_dependents();
 
   // ---- the warps' results: [warp][query][D + 4] and [warp][query][2] over the rings
-  asm volatile("cp.async.wait_all;\n" ::);
+  if (!BULK) asm volatile("cp.async.wait_all;\n" ::);
   __syncthreads();
-  constexpr int QS = 8 * NT, PITCH = D + 4;
   float* ow = reinterpret_cast<float*>(smem);
   float* ml = ow + WARPS * QS * PITCH;
+  float* part = ml + WARPS * QS * 2;  // CLUSTER: [query][D], then [query][2]
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -365,19 +547,24 @@ __global__ void __launch_bounds__(THREADS) decode_4bit_kernel(Decode a) {
       const int h = 8 * n + 2 * l + c;
       float total = sum[n][c];
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+      for (int d = 4; d < 32; d <<= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, d);
+#pragma unroll
+        for (int g = 0; g < H::G; ++g) oc[n][g][c] += __shfl_xor_sync(0xffffffffu, oc[n][g][c], d);
+      }
       if (r == 0) {
         ml[(warp * QS + h) * 2] = m[n][c];
         ml[(warp * QS + h) * 2 + 1] = total;
       }
       float* row = ow + (warp * QS + h) * PITCH;
+      const float up = power_of_two(69 - T), up_odd = up * 0.0625f;  // 2^(133 - T) in two steps
 #pragma unroll
       for (int g = 0; g < H::G; ++g) {
-        const float add = oz[n][g][c];
-        *reinterpret_cast<float4*>(row + 64 * g + 8 * r) =
-            make_float4(o[n][g][0][c] + add, o[n][g][1][c] + add, o[n][g][2][c] + add, o[n][g][3][c] + add);
-        *reinterpret_cast<float4*>(row + 64 * g + 8 * r + 4) =
-            make_float4(o[n][g][0][c + 2] + add, o[n][g][1][c + 2] + add, o[n][g][2][c + 2] + add, o[n][g][3][c + 2] + add);
+        const float base = oz[n][g][c] * 0x1p64f * up + oc[n][g][c];
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = o[n][g][e & 3][c + (e >> 2) * 2] * 0x1p64f * (e & 1 ? up_odd : up) + base;
+        store8(row + 64 * g + 8 * r, y);
       }
     }
   }
@@ -390,27 +577,65 @@ __global__ void __launch_bounds__(THREADS) decode_4bit_kernel(Decode a) {
     float den = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      const float f = exp2f(ml[(w * QS + h) * 2] - top);
+      const float f = exp2_fast(ml[(w * QS + h) * 2] - top);
       den += f * ml[(w * QS + h) * 2 + 1];
       const float4 v = *reinterpret_cast<const float4*>(ow + (w * QS + h) * PITCH + d);
       y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
     }
-    const float lse2 = top + log2f(den);
-    if (a.splits > 1) {
-      const long at = ((long)slot * a.nq + kvh * R + h) * a.splits + split;
-      *reinterpret_cast<float4*>(a.mid_o + at * D + d) = make_float4(y[0] / den, y[1] / den, y[2] / den, y[3] / den);
-      if (d == 0) a.mid_lse[at] = lse2;
+    if (CLUSTER) {
+      *reinterpret_cast<float4*>(part + h * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+      if (d == 0) part[QS * D + 2 * h] = top, part[QS * D + 2 * h + 1] = den;
+    } else if (a.splits > 1) {
+      const long where = ((long)slot * a.nq + kvh * R + h) * a.splits + split;
+      *reinterpret_cast<float4*>(a.mid_o + where * D + d) = make_float4(y[0] / den, y[1] / den, y[2] / den, y[3] / den);
+      if (d == 0) a.mid_lse[where] = top + log2f(den) - 4.f;
     } else {
       uint2 packed;
       packed.x = pack_bf16(y[0] / den, y[1] / den);
       packed.y = pack_bf16(y[2] / den, y[3] / den);
       *reinterpret_cast<uint2*>(a.out + (out_row + h) * D + d) = packed;
-      if (a.lse && d == 0) a.lse[out_row + h] = lse2 * LN_2;
+      if (a.lse && d == 0) a.lse[out_row + h] = (top + log2f(den) - 4.f) * LN_2;
     }
+  }
+  if (CLUSTER) {  // every block of the cluster joins a share of the rows, slices in order
+    cluster_sync_all();
+    const uint32_t part_at = smem_addr(part), ml_at = smem_addr(part + QS * D);
+    const int count = sl.count(a);
+    for (int u = split * THREADS + tid; u < R * (D / 4); u += a.splits * THREADS) {
+      const int h = u / (D / 4), d = 4 * (u % (D / 4));
+      float2 t[MOST_CLUSTER];
+      float4 v[MOST_CLUSTER];
+#pragma unroll
+      for (int s = 0; s < MOST_CLUSTER; ++s)
+        if (s < count) {
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(t[s].x), "=f"(t[s].y) : "r"(map_to_cta(ml_at + 8 * h, s)));
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
+                       : "r"(map_to_cta(part_at + 4 * (h * D + d), s)));
+        }
+      float top = MINUS_BIG, den = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < MOST_CLUSTER; ++s)
+        if (s < count) top = fmaxf(top, t[s].x);
+#pragma unroll
+      for (int s = 0; s < MOST_CLUSTER; ++s)
+        if (s < count) {
+          const float f = exp2_fast(t[s].x - top);
+          den += f * t[s].y;
+          y[0] += f * v[s].x, y[1] += f * v[s].y, y[2] += f * v[s].z, y[3] += f * v[s].w;
+        }
+      const float inv = count > 0 ? 1.f / den : 0.f;
+      uint2 packed;
+      packed.x = pack_bf16(y[0] * inv, y[1] * inv);
+      packed.y = pack_bf16(y[2] * inv, y[3] * inv);
+      *reinterpret_cast<uint2*>(a.out + (out_row + h) * D + d) = packed;
+      if (a.lse && d == 0) a.lse[out_row + h] = count > 0 ? (top + log2f(den) - 4.f) * LN_2 : -INFINITY;
+    }
+    cluster_sync_all();  // a block's results are read until here
   }
 }
 
-// Slices of a (sequence, head), in order: a warp per head.
+// Slices of a (sequence, head), in order: a warp per head, four slices' loads in flight.
 template <int D> __global__ void __launch_bounds__(THREADS) merge_4bit_kernel(Decode a, int heads) {
   pdl_wait();
   pdl_launch_dependents();
@@ -418,21 +643,21 @@ template <int D> __global__ void __launch_bounds__(THREADS) merge_4bit_kernel(De
   if (item >= heads) return;
   const int slot = item / a.nq, h = item - slot * a.nq;
   const int seq = a.seq_list ? a.seq_list[slot] : slot;
-  const int kv_len = min(a.kv_lens[seq], a.max_len), tok = a.cu_seqlens[seq];
-  const int lo = a.window > 0 ? max(0, kv_len - a.window) : 0;
-  const int per = slice_keys(a);
-  const int slices = min(a.splits, (kv_len - lo + per - 1) / per);
+  const int tok = a.cu_seqlens[seq];
+  const int slices = Slice(a, seq, 0).count(a);
   const float* lses = a.mid_lse + (long)item * a.splits;
   const float* os = a.mid_o + (long)item * a.splits * D;
   float top = MINUS_BIG;
-  for (int s = 0; s < slices; ++s) top = fmaxf(top, lses[s]);
-  float den = 0.f, y[D / 128 > 0 ? D / 128 : 1][4] = {};
-  constexpr int PER = D / 4 < 32 ? D / 4 : 32;
+  for (int s = lane; s < slices; s += 32) top = fmaxf(top, lses[s]);
+  top = warp_max(top);
+  constexpr int C = D >= 128 ? D / 128 : 1, PER = D / 4 < 32 ? D / 4 : 32;
+  float den = 0.f, y[C][4] = {};
+#pragma unroll 4
   for (int s = 0; s < slices; ++s) {
-    const float f = exp2f(lses[s] - top);
+    const float f = exp2_fast(lses[s] - top);
     den += f;
 #pragma unroll
-    for (int c = 0; c < (D >= 128 ? D / 128 : 1); ++c)
+    for (int c = 0; c < C; ++c)
       if (lane < PER) {
         const float4 v = *reinterpret_cast<const float4*>(os + (long)s * D + 128 * c + 4 * lane);
         y[c][0] += f * v.x, y[c][1] += f * v.y, y[c][2] += f * v.z, y[c][3] += f * v.w;
@@ -441,7 +666,7 @@ template <int D> __global__ void __launch_bounds__(THREADS) merge_4bit_kernel(De
   const float inv = slices > 0 ? 1.f / den : 0.f;
   bf16* row = a.out + ((long)tok * a.nq + h) * D;
 #pragma unroll
-  for (int c = 0; c < (D >= 128 ? D / 128 : 1); ++c)
+  for (int c = 0; c < C; ++c)
     if (lane < PER) {
       uint2 packed;
       packed.x = pack_bf16(y[c][0] * inv, y[c][1] * inv);
@@ -451,23 +676,49 @@ template <int D> __global__ void __launch_bounds__(THREADS) merge_4bit_kernel(De
   if (a.lse && lane == 0) a.lse[(long)tok * a.nq + h] = slices > 0 ? (top + log2f(den)) * LN_2 : -INFINITY;
 }
 
-template <int D, int NT> int launch_decode(const Decode& a, int num_seqs, cudaStream_t stream) {
-  constexpr int ring = WARPS * STAGES * Head<D>::STAGE;
-  constexpr int joined = WARPS * 8 * NT * (D + 4 + 2) * 4;
+template <int D, int NT, bool BULK, bool CLUSTER> int launch_decode_as(const Decode& a, int num_seqs, cudaStream_t stream) {
+  constexpr int ring = WARPS * STAGES * TILES * Head<D>::TILE;
+  constexpr int joined = (WARPS * 8 * NT * (D + 4 + 2) + (CLUSTER ? 8 * NT * (D + 2) : 0)) * 4;
   constexpr int smem = ring > joined ? ring : joined;
+  auto kernel = decode_4bit_kernel<D, NT, BULK, CLUSTER>;
   static bool once[Q3_MAX_DEVICES];
   const int dev = q3_current_device();
   if (!once[dev]) {
-    if (cudaFuncSetAttribute(decode_4bit_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return Q3_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return Q3_ERR_LAUNCH;
+    if (CLUSTER && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return Q3_ERR_LAUNCH;
     once[dev] = true;
   }
-  cudaError_t err = launch_pdl(decode_4bit_kernel<D, NT>, dim3(a.splits, a.nkv, num_seqs), dim3(THREADS), smem, stream, a);
-  if (err == cudaSuccess && a.splits > 1) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.splits, a.nkv, num_seqs);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (CLUSTER) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.splits;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (q3_pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (err == cudaSuccess && !CLUSTER && a.splits > 1) {
     const int heads = num_seqs * a.nq;
     err = launch_pdl(merge_4bit_kernel<D>, dim3((heads + WARPS - 1) / WARPS), dim3(THREADS), 0, stream, a, heads);
   }
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
+}
+template <int D, int NT> int launch_decode(const Decode& a, int num_seqs, cudaStream_t stream) {
+  const bool bulk = a.ps % STEP == 0, cluster = a.splits > 1 && !a.mid_o;
+  if (bulk) return cluster ? launch_decode_as<D, NT, true, true>(a, num_seqs, stream) : launch_decode_as<D, NT, true, false>(a, num_seqs, stream);
+  return cluster ? launch_decode_as<D, NT, false, true>(a, num_seqs, stream) : launch_decode_as<D, NT, false, false>(a, num_seqs, stream);
 }
 
 // ---- sums of attention weights -----------------------------------------------------------------------------------------------------
@@ -476,11 +727,6 @@ template <int D, int NT> int launch_decode(const Decode& a, int num_seqs, cudaSt
 // (token, head of the group), token by token; the scores' tiles are those of decode attention, with the numbers as 1 + n / 16: what
 // has to be taken off the sums is then no larger than they are, and the sums keep float32's precision (with 128 + n seven bits of it go).
 // A cached token's sum belongs to one lane: no atomics, the same bits every time.
-template <int J> __device__ __forceinline__ uint32_t sixteenths_of(uint32_t w) {
-  const uint32_t x = J == 0 ? w << 3 : w >> (4 * J - 3 > 0 ? 4 * J - 3 : 0);
-  return (x & 0x00780078u) | 0x3F803F80u;
-}
-
 struct Mass {
   const bf16* q;
   int q_stride;
@@ -856,17 +1102,17 @@ Q3_EXPORT int q3_attention_mass_4bit(int dtype, const void* q, int q_stride, con
 Q3_EXPORT int q3_decode_attention_4bit(const void* q, int q_stride, const void* pages, int num_pages, const int* block_table, int max_pages,
                                        const int* kv_lens, const int* cu_seqlens, const int* seq_list, void* out, float* mid_o,
                                        float* mid_lse, float* lse, int num_seqs, int nq, int nkv, int D, int ps, float scale, int window,
-                                       int splits, int max_len, const int* longest, cudaStream_t stream) {
-  if (!q || !pages || !block_table || !kv_lens || !cu_seqlens || !out || nq < 1 || nkv < 1 || nq % nkv || ps < 1 || splits < 1 ||
-      (splits > 1 && (!mid_o || !mid_lse)) || max_len > (long)max_pages * ps)
+                                       int splits, int max_len, const int* longest, int* error_word, cudaStream_t stream) {
+  if (!q || !pages || !block_table || !kv_lens || !cu_seqlens || !out || nq < 1 || nkv < 1 || nq % nkv || !q4_sizes_ok(D, ps) || splits < 1 ||
+      !error_word || (splits > MOST_CLUSTER && !mid_o) || (mid_o && !mid_lse) || max_len > (long)max_pages * ps)
     return Q3_ERR_ARGUMENT;
   const int R = nq / nkv;
   if (R > 16 || q_stride % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(pages) & 15) ||
-      (reinterpret_cast<uintptr_t>(out) & 7) || num_seqs > 65535 || nkv > 65535)
+      (reinterpret_cast<uintptr_t>(out) & 7) || num_seqs > 65535 || nkv > 65535 || Q4Page(D, q4_groups(D), ps).record * nkv > 0x7fffffffL)
     return Q3_ERR_UNSUPPORTED;
   if (num_seqs < 1) return Q3_OK;
   Decode a{(const bf16*)q, q_stride, (const unsigned char*)pages, num_pages, block_table, kv_lens, cu_seqlens, seq_list, max_pages,
-           (bf16*)out, mid_o, mid_lse, lse, nq, nkv, ps, window, splits, max_len, scale * LOG2_E, longest};
+           (bf16*)out, mid_o, mid_lse, lse, nq, nkv, ps, window, splits, max_len, scale * LOG2_E, longest, error_word};
   if (D == 64) return R <= 8 ? launch_decode<64, 1>(a, num_seqs, stream) : launch_decode<64, 2>(a, num_seqs, stream);
   if (D == 128) return R <= 8 ? launch_decode<128, 1>(a, num_seqs, stream) : launch_decode<128, 2>(a, num_seqs, stream);
   if (D == 256) return R <= 8 ? launch_decode<256, 1>(a, num_seqs, stream) : launch_decode<256, 2>(a, num_seqs, stream);

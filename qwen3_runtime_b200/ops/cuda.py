@@ -247,7 +247,7 @@ _SIGNATURES = {
     "attention_4bit": {
         "q3_decode_attention_4bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
-                                     c_int, c_void_p, c_void_p],
+                                     c_int, c_void_p, c_void_p, c_void_p],
         "q3_attention_mass_4bit": [c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
                                    c_void_p],
@@ -2233,11 +2233,11 @@ class CudaOps:
         # the wide kernels number a token by its place: kv_lens and cu_seqlens say it, or for the general kernel `positions`
         return self.paged_attention(q, q_stride, k_pages=k, v_pages=v, block_table=table, step=step, **wide)
 
-    DECODE_4BIT_BLOCKS_PER_SM = {64: 6, 128: 4, 256: 2}
+    DECODE_4BIT_BLOCKS_PER_SM = {64: 5, 128: 4, 256: 2}
 
     def decode_slices_4bit(self, kv_lens, num_kv_heads, head_dim, window) -> int:
         """Into how many slices the longest of these sequences' keys are cut by decode attention over a cache in 4 bits."""
-        tiles = [-(-min(n, window or n) // 64) for n in kv_lens if n > 0]
+        tiles = [-(-min(n, window or n) // 128) for n in kv_lens if n > 0]
         if not tiles:
             return 1
         slots = self.DECODE_4BIT_BLOCKS_PER_SM[head_dim] * self.SM_COUNT
@@ -2247,7 +2247,7 @@ class CudaOps:
     def _decode_4bit(self, q, q_stride, H, G, D, pages, block_table, step, seq_list, num_seqs, max_len, slices, out, page_size, scale,
                      window, longest, lse):
         mid_o = mid_lse = None
-        if slices > 1:
+        if slices > 16 or slices * G * num_seqs > self.SM_COUNT:  # else the blocks of a cluster join them
             mid_o = torch.empty((num_seqs, H, slices, D), dtype=torch.float32, device=out.device)
             mid_lse = torch.empty((num_seqs, H, slices), dtype=torch.float32, device=out.device)
             self.launches += 1
@@ -2257,7 +2257,7 @@ class CudaOps:
         self._call("attention_4bit", "q3_decode_attention_4bit", "paged_attention_decode_4bit", _ptr(q), q_stride, _ptr(pages),
                    pages.shape[0], _ptr(block_table), block_table.shape[1], _ptr(step.kv_lens), _ptr(step.cu_seqlens), _ptr(seq_list),
                    _ptr(out), _ptr(mid_o), _ptr(mid_lse), _ptr(lse), num_seqs, H, G, D, page_size, float(scale), int(window or 0),
-                   slices, max_len, _ptr(longest))
+                   slices, max_len, _ptr(longest), _ptr(self._error_word(out.device)))
         return out
 
     def attention_mass_4bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, mass, block_table, page_size, scale, step,

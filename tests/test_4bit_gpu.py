@@ -3,8 +3,7 @@ go wrong.
 
 Tolerances.  u = 2^-8 is half a step of bfloat16 relative to the value.  A decoded row rounds each weight times scale once (u s|n - 8| p)
 and each weight once (u |z + 8 s| p) -- together at most 2 u p (|z + 8 s| + s |n - 8|) -- and the result once (u |o|).  A score is a sum of D
-products whose float32 sums carry the numbers with 128 added: it is off by at most ``score_error`` below, which moves a weight by a factor
-of exp(2 error).  Prompts read keys and values rounded to bfloat16 (u each) and round the weights and the result (u each)."""
+products in float32: it is off by at most ``score_error`` below, which moves a weight by a factor of exp(2 error).  Prompts read keys and values rounded to bfloat16 (u each) and round the weights and the result (u each)."""
 
 import math
 
@@ -35,9 +34,9 @@ def queries(T, H, D, seed, dtype=BF16, extra=0):
     return torch.randn((T, H * D + extra), generator=g).to(dtype)
 
 
-def score_error(q, cache, b, scale, base=128.0):
-    """Bound of a score's error ``[T, H]``: D additions of float32 to sums of |q| s (16 + base), whatever their order, and 2^-17 of the
-    largest |q| where queries are held as sums of two 8-bit numbers."""
+def score_error(q, cache, b, scale, base=0.0):
+    """Bound of a score's error ``[T, H]``: D additions of float32 to sums of |q| s (16 + base) -- ``base`` 16 where numbers are summed as
+    1 + n / 16 -- whatever their order, and 2^-17 of the largest |q| where queries are held as sums of two 8-bit floats."""
     H, D = q.shape[1:]
     s = cache.k[b][1].double().nan_to_num().amax()
     z = cache.k[b][2].double().abs().nan_to_num().amax()
