@@ -37,11 +37,6 @@ template <int J> __device__ __forceinline__ uint32_t tiny_of(uint32_t w, uint32_
   return (J < 2 ? w : high) & (J & 1 ? 0x00F000F0u : 0x000F000Fu);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
-// Numbers J and J + 4 of a word (or number J of two tokens whose halves were put side by side) as two bfloat16 1 + n / 16.
-template <int J> __device__ __forceinline__ uint32_t sixteenths_of(uint32_t w) {
-  const uint32_t x = J == 0 ? w << 3 : w >> (4 * J - 3 > 0 ? 4 * J - 3 : 0);
-  return (x & 0x00780078u) | 0x3F803F80u;
-}
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(a));
@@ -81,37 +76,8 @@ template <int D> struct Head {
   }
 };
 
-// The queries' side of the scores: B fragments (n = lane / 4: the query, k: the channels that word j's pairs stand for).
-// b[j][0..3]: of word j, channels (0, 4), (1, 5), (2, 6), (3, 7) of its eight.
-template <int D> __device__ __forceinline__ void load_query(uint32_t (&b)[Head<D>::WORDS][4], const bf16* row, int lane) {
-#pragma unroll
-  for (int j = 0; j < Head<D>::WORDS; ++j) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row) v = *reinterpret_cast<const uint4*>(row + 64 * Head<D>::group(j) + 8 * Head<D>::index(j, lane & 3));
-    // v: channels (0,1) (2,3) (4,5) (6,7)
-    b[j][0] = __byte_perm(v.x, v.z, 0x5410);
-    b[j][1] = __byte_perm(v.x, v.z, 0x7632);
-    b[j][2] = __byte_perm(v.y, v.w, 0x5410);
-    b[j][3] = __byte_perm(v.y, v.w, 0x7632);
-  }
-}
-
-// Sums of the queries' channels per group, in the accumulators' layout (columns 2 (lane % 4), + 1): a product with ones.
-template <int D> __device__ __forceinline__ void query_sums(float (&sum)[Head<D>::G][2], const uint32_t (&b)[Head<D>::WORDS][4]) {
-  const uint32_t one[4] = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-  float c[Head<D>::G][4];
-#pragma unroll
-  for (int g = 0; g < Head<D>::G; ++g) c[g][0] = c[g][1] = c[g][2] = c[g][3] = 0.f;
-#pragma unroll
-  for (int j = 0; j < Head<D>::WORDS; ++j) {
-    mma_bf16(c[Head<D>::group(j)], one, b[j][0], b[j][1]);
-    mma_bf16(c[Head<D>::group(j)], one, b[j][2], b[j][3]);
-  }
-#pragma unroll
-  for (int g = 0; g < Head<D>::G; ++g) sum[g][0] = c[g][0], sum[g][1] = c[g][1];
-}
-
-// The queries for the tiny numbers: as load_query's fragments, times 2^S, the channels that meet 2^-129 a 16th of it.  `undo`: what the sums
+// The queries' side of the scores: B fragments (n = lane / 4: the query, k: the channels that word j's pairs stand for; b[j][0..3]: of word j,
+// channels (0, 4), (1, 5), (2, 6), (3, 7) of its eight), times 2^S, the channels that meet 2^-129 a 16th of it.  `undo`: what the sums
 // are to be multiplied by, for columns 2 (lane % 4) and + 1; `sum`: the channels' sums per group, both times the scores' scale.
 template <int D> __device__ __forceinline__ void load_query_tiny(uint32_t (&b)[Head<D>::WORDS][4], float (&undo)[2], float (&sum)[Head<D>::G][2],
                                                                  const bf16* row, float scale_log2, int lane) {
@@ -722,11 +688,14 @@ template <int D, int NT> int launch_decode(const Decode& a, int num_seqs, cudaSt
 }
 
 // ---- sums of attention weights -----------------------------------------------------------------------------------------------------
-// mass[key] += sum over a sequence's last `observe` tokens and the query heads of the kv head of 2^(score - log sum of the row).  Three
-// kernels: the rows' log sums (left out when the attention has them), their slices joined, and the columns' sums.  Rows are
-// (token, head of the group), token by token; the scores' tiles are those of decode attention, with the numbers as 1 + n / 16: what
-// has to be taken off the sums is then no larger than they are, and the sums keep float32's precision (with 128 + n seven bits of it go).
-// A cached token's sum belongs to one lane: no atomics, the same bits every time.
+// mass[key] += sum over a sequence's last `observe` tokens and the query heads of the kv head of 2^(score - log sum of the row).  Rows are
+// (token, head of the group), token by token; the scores' tiles are those of decode attention.  A cached token's sum belongs to one warp's
+// lane: no atomics, the same bits every time.
+//   few rows (up to 16: single tokens)  mass_few_kernel: the queries stay in registers, keys stream past them, 16 a warp at a time, the next
+//                                       ones' bytes on their way; reads half of what the attention reads.
+//   more                                mass_rows_kernel: the rows' log sums, keys cut into slices so that all SMs have some (left out
+//                                       where the attention has them); mass_columns_kernel: a warp keeps 16 keys and goes through the
+//                                       rows, which the block has turned into operands in shared memory.
 struct Mass {
   const bf16* q;
   int q_stride;
@@ -736,82 +705,105 @@ struct Mass {
   int max_pages, nq, nkv, ps, max_len, observe, slices, num_seqs;
   float scale_log2;
   float* lse;    // [tokens][nq], natural logarithms
-  float2* part;  // [tokens][nq][slices]: maximum and sum
+  float2* part;  // null (the log sums are in lse), or [tokens][nq][slices]: maximum and sum
   float* mass;
 };
 
-template <int D> struct KeyTile {  // 16 keys as A fragments
-  uint32_t a[Head<D>::WORDS][2][4];
-  float s[2][Head<D>::G], z[2][Head<D>::G];  // 16 * scale, minimum
-  // rows of keys first + r and first + r + 8; what is not there is zero
-  __device__ __forceinline__ void load(const Mass& m, const Q4Page& L, const int* bt, int kvh, int first, int end, int lane) {
+constexpr int ROWS_STEP = STEP * WARPS;  // keys of a block at a time
+
+template <int D> struct KeyBytes {  // what a lane holds of 16 keys as they are stored
+  uint32_t w[2][Head<D>::WORDS], p[2][Head<D>::G];
+  // rows of keys first + r and first + r + 8; what is not there is zero.  `page`, `row`: where they lie
+  __device__ __forceinline__ void load(const Mass& m, const Q4Page& L, int kvh, const int (&page)[2], const int (&row)[2], int lane) {
     using H = Head<D>;
-    const int r = lane >> 2, l = lane & 3;
-    uint32_t w[2][H::WORDS], p[2][H::G];
+    const int l = lane & 3;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int key = first + r + 8 * half;
-      int page = key < end ? bt[key / m.ps] : -1;
-      const bool valid = page >= 0 && page < m.num_pages;
 #pragma unroll
       for (int j = 0; j < H::WORDS; ++j) w[half][j] = 0;
 #pragma unroll
       for (int g = 0; g < H::G; ++g) p[half][g] = 0;
-      if (valid) {
-        const unsigned char* rec = m.pages + ((long)page * m.nkv + kvh) * L.record;
-        const unsigned char* row = rec + (long)(key % m.ps) * H::ROW;
-        const unsigned char* par = rec + L.kpar + (long)(key % m.ps) * H::PAR;
+      if ((uint32_t)page[half] < (uint32_t)m.num_pages) {
+        const unsigned char* rec = m.pages + ((long)page[half] * m.nkv + kvh) * L.record;
+        const unsigned char* codes = rec + (long)row[half] * H::ROW;
+        const unsigned char* par = rec + L.kpar + (long)row[half] * H::PAR;
         if constexpr (D == 64) {
-          *reinterpret_cast<uint2*>(&w[half][0]) = *reinterpret_cast<const uint2*>(row + 8 * l);
+          *reinterpret_cast<uint2*>(&w[half][0]) = *reinterpret_cast<const uint2*>(codes + 8 * l);
           p[half][0] = *reinterpret_cast<const uint32_t*>(par);
         } else if constexpr (D == 128) {
-          *reinterpret_cast<uint4*>(&w[half][0]) = *reinterpret_cast<const uint4*>(row + 16 * l);
+          *reinterpret_cast<uint4*>(&w[half][0]) = *reinterpret_cast<const uint4*>(codes + 16 * l);
           *reinterpret_cast<uint2*>(&p[half][0]) = *reinterpret_cast<const uint2*>(par);
         } else {
-          *reinterpret_cast<uint4*>(&w[half][0]) = *reinterpret_cast<const uint4*>(row + 16 * l);
-          *reinterpret_cast<uint4*>(&w[half][4]) = *reinterpret_cast<const uint4*>(row + 16 * (l + 4));
+          *reinterpret_cast<uint4*>(&w[half][0]) = *reinterpret_cast<const uint4*>(codes + 16 * l);
+          *reinterpret_cast<uint4*>(&w[half][4]) = *reinterpret_cast<const uint4*>(codes + 16 * (l + 4));
           *reinterpret_cast<uint4*>(&p[half][0]) = *reinterpret_cast<const uint4*>(par);
         }
       }
     }
+  }
+};
+
+template <int D> struct KeyTile {  // 16 keys as A fragments
+  uint32_t a[Head<D>::WORDS][2][4];
+  float s[2][Head<D>::G], z[2][Head<D>::G];
+  __device__ __forceinline__ void load(const Mass& m, const Q4Page& L, const int* bt, int kvh, int first, int end, int lane) {
+    int page[2], row[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int key = first + (lane >> 2) + 8 * half, i = key / m.ps;
+      page[half] = key < end ? bt[i] : -1;
+      row[half] = key - i * m.ps;
+    }
+    KeyBytes<D> bytes;
+    bytes.load(m, L, kvh, page, row, lane);
+    take(bytes);
+  }
+  __device__ __forceinline__ void take(const KeyBytes<D>& b) {
+    using H = Head<D>;
+    const auto& w = b.w;
+    const auto& p = b.p;
 #pragma unroll
     for (int g = 0; g < H::G; ++g) {
-      s[0][g] = 16.f * q4_s(p[0][g]), s[1][g] = 16.f * q4_s(p[1][g]);
+      s[0][g] = q4_s(p[0][g]), s[1][g] = q4_s(p[1][g]);
       z[0][g] = q4_z(p[0][g]), z[1][g] = q4_z(p[1][g]);
     }
 #pragma unroll
     for (int j = 0; j < H::WORDS; ++j) {
-      a[j][0][0] = sixteenths_of<0>(w[0][j]), a[j][0][1] = sixteenths_of<0>(w[1][j]);
-      a[j][0][2] = sixteenths_of<1>(w[0][j]), a[j][0][3] = sixteenths_of<1>(w[1][j]);
-      a[j][1][0] = sixteenths_of<2>(w[0][j]), a[j][1][1] = sixteenths_of<2>(w[1][j]);
-      a[j][1][2] = sixteenths_of<3>(w[0][j]), a[j][1][3] = sixteenths_of<3>(w[1][j]);
+      const uint32_t w0 = w[0][j], w1 = w[1][j], u0 = w0 >> 8, u1 = w1 >> 8;
+      a[j][0][0] = tiny_of<0>(w0, u0), a[j][0][1] = tiny_of<0>(w1, u1), a[j][0][2] = tiny_of<1>(w0, u0), a[j][0][3] = tiny_of<1>(w1, u1);
+      a[j][1][0] = tiny_of<2>(w0, u0), a[j][1][1] = tiny_of<2>(w1, u1), a[j][1][2] = tiny_of<3>(w0, u0), a[j][1][3] = tiny_of<3>(w1, u1);
     }
   }
   // scores (times scale, in powers of two): x[0], x[1] of key r and queries 2l, 2l + 1; x[2], x[3] of key r + 8
-  __device__ __forceinline__ void scores(float (&x)[4], const uint32_t (&q)[Head<D>::WORDS][4], const float (&qsum)[Head<D>::G][2],
-                                         float scale_log2) const {
+  __device__ __forceinline__ void scores(float (&x)[4], const uint32_t (&q)[Head<D>::WORDS][4], const float (&undo)[2],
+                                         const float (&qsum)[Head<D>::G][2]) const {
     using H = Head<D>;
     float acc[H::G][4];
 #pragma unroll
-    for (int g = 0; g < H::G; ++g) {
-      acc[g][0] = acc[g][2] = -qsum[g][0];
-      acc[g][1] = acc[g][3] = -qsum[g][1];
-    }
-#pragma unroll
     for (int j = 0; j < H::WORDS; ++j) {
-      mma_bf16(acc[H::group(j)], a[j][0], q[j][0], q[j][1]);
+      if (j < H::G)
+        mma_bf16_first(acc[H::group(j)], a[j][0], q[j][0], q[j][1]);
+      else
+        mma_bf16(acc[H::group(j)], a[j][0], q[j][0], q[j][1]);
       mma_bf16(acc[H::group(j)], a[j][1], q[j][2], q[j][3]);
     }
     x[0] = x[1] = x[2] = x[3] = 0.f;
 #pragma unroll
     for (int g = 0; g < H::G; ++g) {
-      x[0] += s[0][g] * acc[g][0] + z[0][g] * qsum[g][0];
-      x[1] += s[0][g] * acc[g][1] + z[0][g] * qsum[g][1];
-      x[2] += s[1][g] * acc[g][2] + z[1][g] * qsum[g][0];
-      x[3] += s[1][g] * acc[g][3] + z[1][g] * qsum[g][1];
+      x[0] += s[0][g] * acc[g][0];
+      x[1] += s[0][g] * acc[g][1];
+      x[2] += s[1][g] * acc[g][2];
+      x[3] += s[1][g] * acc[g][3];
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] *= scale_log2;
+    for (int e = 0; e < 4; ++e) x[e] *= undo[e & 1];
+#pragma unroll
+    for (int g = 0; g < H::G; ++g) {
+      x[0] += z[0][g] * qsum[g][0];
+      x[1] += z[0][g] * qsum[g][1];
+      x[2] += z[1][g] * qsum[g][0];
+      x[3] += z[1][g] * qsum[g][1];
+    }
   }
 };
 
@@ -842,13 +834,13 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS) mass_rows_ke
   const Q4Page L(D, H::G, a.ps);
   const int* bt = a.block_table + (long)seq * a.max_pages;
   uint32_t q[NT][H::WORDS][4];
-  float qsum[NT][H::G][2], m[NT][2], sum[NT][2];
+  float qsum[NT][H::G][2], undo[NT][2], m[NT][2], sum[NT][2];
   int sees[NT][2];  // the last key that the row's token sees
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int row = row0 + 8 * n + r, i = row / R;
-    load_query<D>(q[n], i < rows.count ? a.q + (long)(rows.first + i) * a.q_stride + (long)(kvh * R + row % R) * D : nullptr, lane);
-    query_sums<D>(qsum[n], q[n]);
+    load_query_tiny<D>(q[n], undo[n], qsum[n], i < rows.count ? a.q + (long)(rows.first + i) * a.q_stride + (long)(kvh * R + row % R) * D : nullptr,
+                       a.scale_log2, lane);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       m[n][c] = MINUS_BIG, sum[n][c] = 0.f;
@@ -861,7 +853,7 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS) mass_rows_ke
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float x[4];
-      k.scores(x, q[n], qsum[n], a.scale_log2);
+      k.scores(x, q[n], undo[n], qsum[n]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float x0 = first + r <= sees[n][c] ? x[c] : -INFINITY, x1 = first + r + 8 <= sees[n][c] ? x[c + 2] : -INFINITY;
@@ -894,31 +886,118 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS) mass_rows_ke
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) den += joined[w][tid].y * exp2f(joined[w][tid].x - top);
     const long at = (long)(rows.first + row / R) * a.nq + kvh * R + row % R;
-    if (a.slices > 1)
+    if (a.part)
       a.part[at * a.slices + slice] = make_float2(top, den);
     else
       a.lse[at] = (top + log2f(den)) * LN_2;
   }
 }
 
-__global__ void mass_join_kernel(Mass a) {  // grid (blocks over observed rows, sequence)
-  pdl_wait();
-  pdl_launch_dependents();
-  const Rows rows(a, blockIdx.y);
-  const int u = blockIdx.x * blockDim.x + threadIdx.x;
-  if (u >= rows.count * a.nq) return;
-  const long at = (long)rows.first * a.nq + u;
+// The log sum of a row in powers of two: as the attention wrote it, or its slices joined.
+__device__ __forceinline__ float row_log2(const Mass& a, long at) {
+  if (!a.part) return a.lse[at] * LOG2_E;
   float top = MINUS_BIG, den = 0.f;
   for (int s = 0; s < a.slices; ++s) top = fmaxf(top, a.part[at * a.slices + s].x);
   for (int s = 0; s < a.slices; ++s) {
     const float2 y = a.part[at * a.slices + s];
     den += y.y * exp2f(y.x - top);
   }
-  a.lse[at] = (top + log2f(den)) * LN_2;
+  return top + log2f(den);
 }
 
-// Column sums: grid (blocks of 64 MT keys, kv head, sequence); a warp keeps 16 MT keys in registers and goes through the rows.
-template <int D, int MT> __global__ void __launch_bounds__(THREADS) mass_columns_kernel(Mass a) {
+// Column sums of many rows: grid (blocks of 16 * COLUMN_WARPS keys, kv head, sequence).
+constexpr int COLUMN_WARPS = 8;
+constexpr int COLUMN_TILES = 8;  // tiles of 8 rows in shared memory at a time
+
+template <int D> struct RowTile {  // 8 rows as operands, as each lane reads them
+  uint32_t q[Head<D>::WORDS][32][4];
+  float undo[32][2], sums[Head<D>::G][32][2], lse2[32][2];
+  int sees[32][2];
+};
+
+template <int D> __global__ void __launch_bounds__(32 * COLUMN_WARPS) mass_columns_kernel(Mass a) {
+  using H = Head<D>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  RowTile<D>* tiles = reinterpret_cast<RowTile<D>*>(smem);
+  pdl_wait();
+  pdl_launch_dependents();
+  const int seq = blockIdx.z, kvh = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, l = lane & 3, R = a.nq / a.nkv;
+  const Rows rows(a, seq);
+  const int kv_len = rows.before + rows.count;
+  const int block_first = blockIdx.x * COLUMN_WARPS * STEP, first = block_first + warp * STEP;
+  if (block_first >= kv_len || rows.count == 0) return;
+  const Q4Page L(D, H::G, a.ps);
+  const int* bt = a.block_table + (long)seq * a.max_pages;
+  KeyTile<D> k;
+  k.load(a, L, bt, kvh, first, kv_len, lane);
+  float total[2] = {0.f, 0.f};
+  // rows of tokens that see none of the block's keys are left out
+  const int start = max(0, block_first - rows.before) * R & ~7, stop = rows.count * R;
+  for (int portion = start; portion < stop; portion += 8 * COLUMN_TILES) {
+    __syncthreads();
+    for (int n = warp; n < COLUMN_TILES && portion + 8 * n < stop; n += COLUMN_WARPS) {
+      RowTile<D>& t = tiles[n];
+      uint32_t q[H::WORDS][4];
+      float undo[2], sums[H::G][2];
+      const int own = portion + 8 * n + r, own_i = own / R;
+      load_query_tiny<D>(q, undo, sums,
+                         own_i < rows.count ? a.q + (long)(rows.first + own_i) * a.q_stride + (long)(kvh * R + own % R) * D : nullptr,
+                         a.scale_log2, lane);
+#pragma unroll
+      for (int j = 0; j < H::WORDS; ++j) *reinterpret_cast<uint4*>(t.q[j][lane]) = make_uint4(q[j][0], q[j][1], q[j][2], q[j][3]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int row = portion + 8 * n + 2 * l + c, i = row / R;
+        const bool is = i < rows.count;
+        t.undo[lane][c] = undo[c];
+#pragma unroll
+        for (int g = 0; g < H::G; ++g) t.sums[g][lane][c] = sums[g][c];
+        t.lse2[lane][c] = is ? row_log2(a, (long)(rows.first + i) * a.nq + kvh * R + row % R) : 0.f;
+        t.sees[lane][c] = is ? rows.before + i : -1;
+      }
+    }
+    __syncthreads();
+    if (first >= kv_len) continue;
+    for (int n = 0; n < COLUMN_TILES && portion + 8 * n < stop; ++n) {
+      const RowTile<D>& t = tiles[n];
+      uint32_t q[H::WORDS][4];
+      float sums[H::G][2];
+#pragma unroll
+      for (int j = 0; j < H::WORDS; ++j) {
+        const uint4 v = *reinterpret_cast<const uint4*>(t.q[j][lane]);
+        q[j][0] = v.x, q[j][1] = v.y, q[j][2] = v.z, q[j][3] = v.w;
+      }
+      const float2 undo2 = *reinterpret_cast<const float2*>(t.undo[lane]), lse2 = *reinterpret_cast<const float2*>(t.lse2[lane]);
+      const int2 sees = *reinterpret_cast<const int2*>(t.sees[lane]);
+#pragma unroll
+      for (int g = 0; g < H::G; ++g) sums[g][0] = t.sums[g][lane][0], sums[g][1] = t.sums[g][lane][1];
+      const float undo[2] = {undo2.x, undo2.y};
+      float x[4];
+      k.scores(x, q, undo, sums);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = first + r + 8 * (e >> 1);
+        total[e >> 1] += key <= (e & 1 ? sees.y : sees.x) ? exp2f(x[e] - (e & 1 ? lse2.y : lse2.x)) : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float y = total[half];
+    y += __shfl_xor_sync(0xffffffffu, y, 1);
+    y += __shfl_xor_sync(0xffffffffu, y, 2);
+    const int key = first + r + 8 * half;
+    if (l == 0 && key < kv_len) {
+      const int page = bt[key / a.ps];
+      if (page >= 0 && page < a.num_pages) a.mass[((long)page * a.nkv + kvh) * a.ps + key % a.ps] += y;
+    }
+  }
+}
+
+// Few rows: grid (slice, kv head, sequence); a warp takes every fourth 16 keys of the slice.  Two tiles are on their way while one is
+// worked on: the first one's bytes, and the pages of the second, whose bytes wait for them.  NT tiles of 8 rows.
+template <int D, int NT> __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 4) mass_few_kernel(Mass a) {
   using H = Head<D>;
   pdl_wait();
   pdl_launch_dependents();
@@ -926,59 +1005,87 @@ template <int D, int MT> __global__ void __launch_bounds__(THREADS) mass_columns
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, l = lane & 3, R = a.nq / a.nkv;
   const Rows rows(a, seq);
   const int kv_len = rows.before + rows.count;
-  const int first = (blockIdx.x * WARPS + warp) * STEP * MT;
-  if (first >= kv_len || rows.count == 0) return;
+  const int per = ((a.max_len + (int)gridDim.x - 1) / (int)gridDim.x + ROWS_STEP - 1) / ROWS_STEP * ROWS_STEP;
+  const int begin = blockIdx.x * per, end = min(kv_len, begin + per);
+  if (begin >= end || rows.count == 0) return;
   const Q4Page L(D, H::G, a.ps);
   const int* bt = a.block_table + (long)seq * a.max_pages;
-  KeyTile<D> k[MT];
+  // this lane's two keys of the tile to come: page of the sequence and row, moved on by a step of the block at a time
+  int at_page[2], row[2];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) k[t].load(a, L, bt, kvh, first + STEP * t, kv_len, lane);
-  float total[MT][2];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) total[t][0] = total[t][1] = 0.f;
-  // rows of tokens that see none of these keys are left out
-  const int start = max(0, first - rows.before) * R;
-  for (int row0 = start & ~7; row0 < rows.count * R; row0 += 8) {
-    uint32_t q[H::WORDS][4];
-    float qsum[H::G][2];
-    {
-      const int row = row0 + r, i = row / R;
-      load_query<D>(q, i < rows.count ? a.q + (long)(rows.first + i) * a.q_stride + (long)(kvh * R + row % R) * D : nullptr, lane);
-      query_sums<D>(qsum, q);
-    }
-    float lse2[2];
-    int sees[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int row = row0 + 2 * l + c, i = row / R;
-      const bool is = i < rows.count;
-      lse2[c] = is ? a.lse[(long)(rows.first + i) * a.nq + kvh * R + row % R] * LOG2_E : 0.f;
-      sees[c] = is ? rows.before + i : -1;
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      float x[4];
-      k[t].scores(x, q, qsum, a.scale_log2);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = first + STEP * t + r + 8 * (e >> 1);
-        total[t][e >> 1] += key <= sees[e & 1] ? exp2f(x[e] - lse2[e & 1]) : 0.f;
-      }
-    }
+  for (int half = 0; half < 2; ++half) {
+    const int key = begin + warp * STEP + r + 8 * half;
+    at_page[half] = key / a.ps, row[half] = key - at_page[half] * a.ps;
   }
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
+  const int go_pages = ROWS_STEP / a.ps, go_rows = ROWS_STEP - go_pages * a.ps;
+  int page[2], next_row[2];
+  auto look_up = [&](int first) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      float y = total[t][half];
-      y += __shfl_xor_sync(0xffffffffu, y, 1);
-      y += __shfl_xor_sync(0xffffffffu, y, 2);
-      const int key = first + STEP * t + r + 8 * half;
-      if (l == 0 && key < kv_len) {
-        const int page = bt[key / a.ps];
-        if (page >= 0 && page < a.num_pages) a.mass[((long)page * a.nkv + kvh) * a.ps + key % a.ps] += y;
+      page[half] = first + r + 8 * half < end ? bt[at_page[half]] : -1;
+      next_row[half] = row[half];
+      at_page[half] += go_pages, row[half] += go_rows;
+      if (row[half] >= a.ps) row[half] -= a.ps, ++at_page[half];
+    }
+  };
+  KeyBytes<D> bytes;
+  float* cell[2];
+  float old[2];
+  auto fetch = [&]() {  // the bytes and sums of the keys looked up last
+    bytes.load(a, L, kvh, page, next_row, lane);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const bool own = l == 0 && (uint32_t)page[half] < (uint32_t)a.num_pages;
+      cell[half] = own ? a.mass + ((long)page[half] * a.nkv + kvh) * a.ps + next_row[half] : nullptr;
+      old[half] = own ? *cell[half] : 0.f;
+    }
+  };
+  int first = begin + warp * STEP;
+  look_up(first);
+  uint32_t q[NT][H::WORDS][4];
+  float qsum[NT][H::G][2], undo[NT][2], lse2[NT][2];
+  int sees[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int own = 8 * n + r, own_i = own / R;
+    load_query_tiny<D>(q[n], undo[n], qsum[n],
+                       own_i < rows.count ? a.q + (long)(rows.first + own_i) * a.q_stride + (long)(kvh * R + own % R) * D : nullptr, a.scale_log2, lane);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int at = 8 * n + 2 * l + c, i = at / R;
+      const bool is = i < rows.count;
+      lse2[n][c] = is ? row_log2(a, (long)(rows.first + i) * a.nq + kvh * R + at % R) : 0.f;
+      sees[n][c] = is ? rows.before + i : -1;
+    }
+  }
+  fetch();
+  look_up(first + ROWS_STEP);
+  for (; first < end; first += ROWS_STEP) {
+    KeyTile<D> k;
+    k.take(bytes);
+    float* const mine[2] = {cell[0], cell[1]};
+    const float was[2] = {old[0], old[1]};
+    fetch();
+    look_up(first + 2 * ROWS_STEP);
+    float total[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float x[4];
+      k.scores(x, q[n], undo[n], qsum[n]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = first + r + 8 * (e >> 1);
+        total[e >> 1] += key <= sees[n][e & 1] ? exp2f(x[e] - lse2[n][e & 1]) : 0.f;
       }
     }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float y = total[half];
+      y += __shfl_xor_sync(0xffffffffu, y, 1);
+      y += __shfl_xor_sync(0xffffffffu, y, 2);
+      if (mine[half]) *mine[half] = was[half] + y;
+    }
+  }
 }
 
 // float32, and head sizes that the tiles do not take: the same sums on the FMA pipes.
@@ -1047,17 +1154,27 @@ template <typename T> __global__ void mass_columns_general_kernel(Mass a, const 
   if (rows.count) a.mass[((long)page * a.nkv + kvh) * a.ps + key % a.ps] += total;
 }
 
-template <int D, int NT, int MT> int launch_mass(const Mass& a, bool want_rows, int most_tokens, cudaStream_t stream) {
+template <int D, int NT> int launch_mass(const Mass& a, bool want_rows, int most_tokens, int few_slices, cudaStream_t stream) {
   const int rows = most_tokens * (a.nq / a.nkv);
   cudaError_t err = cudaSuccess;
-  if (want_rows) {
+  if (want_rows)
     err = launch_pdl(mass_rows_kernel<D, NT>, dim3(a.slices, (rows + 8 * NT - 1) / (8 * NT), a.num_seqs * a.nkv), dim3(THREADS), 0, stream, a);
-    if (err == cudaSuccess && a.slices > 1)
-      err = launch_pdl(mass_join_kernel, dim3((most_tokens * a.nq + 127) / 128, a.num_seqs), dim3(128), 0, stream, a);
+  if (err != cudaSuccess) return Q3_ERR_LAUNCH;
+  if (rows <= 16) {
+    const dim3 grid(few_slices, a.nkv, a.num_seqs);
+    err = rows <= 8 ? launch_pdl(mass_few_kernel<D, 1>, grid, dim3(THREADS), 0, stream, a)
+                    : launch_pdl(mass_few_kernel<D, 2>, grid, dim3(THREADS), 0, stream, a);
+  } else {
+    constexpr int KEYS = COLUMN_WARPS * STEP;
+    constexpr int smem = COLUMN_TILES * sizeof(RowTile<D>);
+    static bool once[Q3_MAX_DEVICES];
+    const int dev = q3_current_device();
+    if (!once[dev]) {
+      if (cudaFuncSetAttribute(mass_columns_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return Q3_ERR_LAUNCH;
+      once[dev] = true;
+    }
+    err = launch_pdl(mass_columns_kernel<D>, dim3((a.max_len + KEYS - 1) / KEYS, a.nkv, a.num_seqs), dim3(32 * COLUMN_WARPS), smem, stream, a);
   }
-  constexpr int KEYS = WARPS * STEP * MT;
-  if (err == cudaSuccess)
-    err = launch_pdl(mass_columns_kernel<D, MT>, dim3((a.max_len + KEYS - 1) / KEYS, a.nkv, a.num_seqs), dim3(THREADS), 0, stream, a);
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
 }
 
@@ -1067,9 +1184,9 @@ template <int D, int NT, int MT> int launch_mass(const Mass& a, bool want_rows, 
 Q3_EXPORT int q3_attention_mass_4bit(int dtype, const void* q, int q_stride, const void* pages, int num_pages, const int* block_table,
                                      int max_pages, const int* kv_lens, const int* cu_seqlens, float* mass, float* lse, int have_lse,
                                      void* part, int slices, int num_seqs, int nq, int nkv, int D, int ps, float scale, int max_len,
-                                     int observe, int most_tokens, cudaStream_t stream) {
+                                     int observe, int most_tokens, int few_slices, cudaStream_t stream) {
   if (!q || !pages || !block_table || !kv_lens || !cu_seqlens || !mass || !lse || nq < 1 || nkv < 1 || nq % nkv || !q4_sizes_ok(D, ps) ||
-      slices < 1 || (slices > 1 && !part) || observe < 1 || max_len > (long)max_pages * ps)
+      slices < 1 || few_slices < 1 || (slices > 1 && !part) || observe < 1 || max_len > (long)max_pages * ps)
     return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
   if (num_seqs < 1 || most_tokens < 1 || max_len < 1) return Q3_OK;
@@ -1077,12 +1194,12 @@ Q3_EXPORT int q3_attention_mass_4bit(int dtype, const void* q, int q_stride, con
       (long)num_seqs * nkv > 65535 || nq > 65535)
     return Q3_ERR_UNSUPPORTED;
   Mass a{(const bf16*)q, q_stride, (const unsigned char*)pages, num_pages, block_table, kv_lens, cu_seqlens, max_pages, nq, nkv, ps,
-         max_len, observe, slices, num_seqs, scale * LOG2_E, lse, (float2*)part, mass};
+         max_len, observe, slices, num_seqs, scale * LOG2_E, lse, have_lse || slices == 1 ? nullptr : (float2*)part, mass};
   if (dtype == Q3_DTYPE_BF16 && (D == 64 || D == 128 || D == 256)) {
     if ((long)most_tokens * (nq / nkv) > 65535L * 16) return Q3_ERR_UNSUPPORTED;
-    if (D == 64) return launch_mass<64, 4, 2>(a, !have_lse, most_tokens, stream);
-    if (D == 128) return launch_mass<128, 4, 2>(a, !have_lse, most_tokens, stream);
-    return launch_mass<256, 2, 1>(a, !have_lse, most_tokens, stream);
+    if (D == 64) return launch_mass<64, 4>(a, !have_lse, most_tokens, few_slices, stream);
+    if (D == 128) return launch_mass<128, 4>(a, !have_lse, most_tokens, few_slices, stream);
+    return launch_mass<256, 2>(a, !have_lse, most_tokens, few_slices, stream);
   }
   const int G = q4_groups(D);
   cudaError_t err = cudaSuccess;

@@ -1,9 +1,10 @@
 // The cache in 4 bits (layout and rounding: four_bit.cuh): what writes it, what reads it back, and what drops tokens from it.
 //
-// * store:  per-head q/k RMSNorm, rotation, and the write of keys and values in 4 bits, as rope_kv.cu does it for wide pages: the same
-//           float32 arithmetic in the same order, so queries have the same bits.
+// * store:  per-head q/k RMSNorm, rotation, and the write of keys and values in 4 bits, as rope_kv.cu does it for wide pages.
 // * unpack: a step's sequences as pages of bfloat16 or float32, one after the other, for the attention over prompts.
 // * evict:  see evict_select_kernel.
+#include <limits.h>
+
 #include "four_bit.cuh"
 #include "rotary.cuh"
 
@@ -37,8 +38,20 @@ __device__ __forceinline__ bool store_place(const Store& a, int t, int nkv, int 
 }
 
 // Head sizes 16, 32, 64, 128, 256 with the rotation over the whole head (or none): D / 16 threads per (token, head); thread c owns
-// channels [8c, 8c + 8) and [D/2 + 8c, D/2 + 8c + 8), which are one word of 4-bit numbers each.  Limited by the bytes of the projection
-// and of the queries; the divisions of the rounding hide behind them.
+// channels [8c, 8c + 8) and [D/2 + 8c, D/2 + 8c + 8), which are one word of 4-bit numbers each.  What bounds it is the bytes of the projection
+// and of the queries.
+//
+// A key near the border between two numbers falls on either side by float32's last bit.  So that it falls where a float32 statement of
+// norm and rotation in PyTorch puts it, heads of 128 and 256 sum their squares four neighbours at a time and then by halves, and products
+// and sums are rounded one by one (14 keys of 59 million fell elsewhere with fused products and another order).
+__device__ __forceinline__ float quad_of_squares(const float* v) {
+  return __fadd_rn(__fadd_rn(__fadd_rn(__fmul_rn(v[0], v[0]), __fmul_rn(v[1], v[1])), __fmul_rn(v[2], v[2])), __fmul_rn(v[3], v[3]));
+}
+__device__ __forceinline__ void turn_rounded(float& a, float& b, float cs, float sn) {
+  const float x = a, y = b;
+  a = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
+  b = __fadd_rn(__fmul_rn(y, cs), __fmul_rn(x, sn));
+}
 template <typename T>
 __global__ void store_4bit_vec_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, int nq, int nkv, int D, int G, int tph_shift,
                                       Store a) {
@@ -65,10 +78,20 @@ __global__ void store_4bit_vec_kernel(const T* qkv, int row_stride, T* q_out, in
   }
   const bool is_v = hi >= nq + nkv, is_q = hi < nq;
   const float* w = is_q ? a.q_w : a.k_w;
-  float ss = 0.f;
+  float ss;
+  if (D >= 128) {
+    float even = __fadd_rn(quad_of_squares(v0), quad_of_squares(v1)), odd = __fadd_rn(quad_of_squares(v0 + 4), quad_of_squares(v1 + 4));
+    for (int o = tph >> 1; o > 0; o >>= 1) {
+      even = __fadd_rn(even, __shfl_xor_sync(0xffffffffu, even, o));
+      odd = __fadd_rn(odd, __shfl_xor_sync(0xffffffffu, odd, o));
+    }
+    ss = __fadd_rn(even, odd);
+  } else {
+    ss = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) ss += v0[e] * v0[e] + v1[e] * v1[e];
-  for (int o = tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    for (int e = 0; e < 8; ++e) ss += v0[e] * v0[e] + v1[e] * v1[e];
+    for (int o = tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  }
   bool turned = true;
   if (!is_v) {
     if (w) {
@@ -87,7 +110,17 @@ __global__ void store_4bit_vec_kernel(const T* qkv, int row_stride, T* q_out, in
         if (live && a.error_word && c == 0) atomicExch(a.error_word, Q3_ERR_POSITION);
         turned = false;
       } else {
-        rotate_chunks(v0, v1, a.cos_t + (long)p * half, a.sin_t + (long)p * half, c, half, a.pairing);
+        const Angles y = load_angles(a.cos_t + (long)p * half, a.sin_t + (long)p * half, c, half, a.pairing);
+        if (!a.pairing) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) turn_rounded(v0[e], v1[e], y.cs[e], y.sn[e]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            turn_rounded(v0[2 * j], v0[2 * j + 1], y.cs[j], y.sn[j]);
+            turn_rounded(v1[2 * j], v1[2 * j + 1], y.cs[4 + j], y.sn[4 + j]);
+          }
+        }
       }
     }
   }
@@ -98,7 +131,8 @@ __global__ void store_4bit_vec_kernel(const T* qkv, int row_stride, T* q_out, in
       store8(y + half + 8 * c, v1);
     }
   }
-  // (all lanes take part in the reductions: heads of queries and keys may share a warp)
+  if (__all_sync(0xffffffffu, !live || is_q)) return;
+  // (else all lanes take part in the reductions: heads of queries and keys may share a warp)
   float lo0 = v0[0], hi0 = v0[0], lo1 = v1[0], hi1 = v1[0], nan0 = 0.f, nan1 = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -222,45 +256,99 @@ __global__ void store_4bit_kernel(const T* qkv, int row_stride, T* q_out, int q_
 }
 
 // ---- back to wide pages -------------------------------------------------------------------------------------------------------------
-// Block: one page of one sequence and kv head.  out page index: sequence's row * width + its page; rows behind the sequence's last token
-// are zero, and pages behind it too (fill) or left alone (not fill).  `cu_seqlens` (may be null): only sequences that bring more than
-// one token count, in order; `table_out` [num_seqs][width] then gets where their pages went.
-template <typename T>
-__global__ void unpack_4bit_kernel(const unsigned char* __restrict__ pages, int num_pages, int nkv, int D, int G, int ps,
-                                   const int* __restrict__ block_table, int max_pages, const int* __restrict__ kv_lens, int num_seqs,
-                                   int max_len, const int* __restrict__ cu_seqlens, int width, int fill, T* __restrict__ k_out,
-                                   T* __restrict__ v_out, int* __restrict__ table_out) {
+// Out page: sequence's row * width + its page; rows behind the sequence's last token are zero, and pages behind it too (fill) or left alone
+// (not fill).  `cu_seqlens` (may be null): only sequences that bring more than one token count, in order; `table_out` [num_seqs][width]
+// then gets where their pages went.
+struct Unpack {
+  const unsigned char* pages;
+  int num_pages, nkv, ps;
+  const int *block_table, *kv_lens, *cu_seqlens;
+  int max_pages, num_seqs, max_len, width, fill;
+  int* table_out;
+  // the sequence that stands at place `z`; -1: none.  Called by whole warps.
+  __device__ __forceinline__ int sequence(int z) const {
+    if (!cu_seqlens) return z;
+    for (int base = 0; base < num_seqs; base += 32) {
+      const int s = base + (threadIdx.x & 31);
+      const uint32_t found = __ballot_sync(0xffffffffu, s < num_seqs && cu_seqlens[s + 1] - cu_seqlens[s] > 1);
+      if (z < __popc(found)) return base + __fns(found, 0, z + 1);
+      z -= __popc(found);
+    }
+    return -1;
+  }
+};
+
+// Head sizes 64, 128, 256: a warp per (page, kv head), 8 lanes a row.  Lane r of a row reads word r of every group and writes 8 channels of
+// each, so that the 8 lanes' writes are one piece.  All of a page's loads (16 tokens: 8 of up to 16 bytes) are under way before the
+// first is used: what bounds it is the bytes written, as long as enough warps have theirs under way.
+template <typename T, int D> __global__ void __launch_bounds__(256) unpack_4bit_rows_kernel(Unpack a, T* __restrict__ k_out, T* __restrict__ v_out) {
+  constexpr int G = D / 64, AT_ONCE = 8;
   pdl_wait();
   pdl_launch_dependents();
-  const int i = blockIdx.x, kvh = blockIdx.y;
-  int seq = blockIdx.z;
-  if (cu_seqlens) {  // the blockIdx.z-th of the sequences with more than one token
-    int want = blockIdx.z, base = 0;
-    seq = -1;
-    for (; base < num_seqs; base += 32) {
-      const int s = base + (threadIdx.x & 31);
-      const bool is = s < num_seqs && cu_seqlens[s + 1] - cu_seqlens[s] > 1;
-      const uint32_t found = __ballot_sync(0xffffffffu, is);
-      if (want < __popc(found)) {
-        seq = base + __fns(found, 0, want + 1);
-        break;
+  const int lane = threadIdx.x & 31, r = lane & 7;
+  const long item = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int kvh = (int)(item % a.nkv), i = (int)(item / a.nkv);
+  if (i >= a.width) return;
+  const int seq = a.sequence(blockIdx.y);
+  if (seq < 0) return;
+  const int place = blockIdx.y * a.width + i;
+  if (a.table_out && kvh == 0 && lane == 0) a.table_out[(long)seq * a.width + i] = place;
+  const int page = i < a.max_pages ? a.block_table[(long)seq * a.max_pages + i] : -1;
+  int rows = min(max(min(a.kv_lens[seq], a.max_len) - i * a.ps, 0), a.ps);
+  if (page < 0 || page >= a.num_pages) rows = 0;
+  if (rows == 0 && !a.fill) return;
+  const Q4Page L(D, G, a.ps);
+  const unsigned char* rec = a.pages + ((long)max(page, 0) * a.nkv + kvh) * L.record;
+  const long out_base = ((long)place * a.nkv + kvh) * a.ps * D;
+  for (int first = lane >> 3; first < 2 * a.ps; first += 4 * AT_ONCE) {  // rows of keys, then of values
+    uint32_t code[AT_ONCE][G], par[AT_ONCE][G];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int at = first + 4 * u, is_v = at >= a.ps, row = at - is_v * a.ps;
+#pragma unroll
+      for (int g = 0; g < G; ++g) code[u][g] = par[u][g] = 0;
+      if (at < 2 * a.ps && row < rows) {
+        const unsigned char *c = rec + (is_v ? L.values : 0) + (long)row * (D / 2) + 4 * G * r, *p = rec + (is_v ? L.vpar : L.kpar) + (long)row * 4 * G;
+        if constexpr (D == 64) code[u][0] = *reinterpret_cast<const uint32_t*>(c), par[u][0] = *reinterpret_cast<const uint32_t*>(p);
+        if constexpr (D == 128)
+          *reinterpret_cast<uint2*>(code[u]) = *reinterpret_cast<const uint2*>(c), *reinterpret_cast<uint2*>(par[u]) = *reinterpret_cast<const uint2*>(p);
+        if constexpr (D == 256)
+          *reinterpret_cast<uint4*>(code[u]) = *reinterpret_cast<const uint4*>(c), *reinterpret_cast<uint4*>(par[u]) = *reinterpret_cast<const uint4*>(p);
       }
-      want -= __popc(found);
     }
-    if (seq < 0) return;
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int at = first + 4 * u, is_v = at >= a.ps, row = at - is_v * a.ps;
+      if (at >= 2 * a.ps) break;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float s = q4_s(par[u][g]), z = q4_z(par[u][g]);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = z + (float)((code[u][g] >> (4 * e)) & 15u) * s;
+        store8((is_v ? v_out : k_out) + out_base + (long)row * D + 64 * g + 8 * r, v);
+      }
+    }
   }
-  const int len = min(kv_lens[seq], max_len);
-  const int place = blockIdx.z * width + i;
-  if (table_out && kvh == 0 && threadIdx.x == 0) table_out[(long)seq * width + i] = place;
-  int rows = min(max(len - i * ps, 0), ps);
-  int page = -1;
-  if (rows > 0 && i < max_pages) page = block_table[(long)seq * max_pages + i];
-  if (page < 0 || page >= num_pages) rows = 0;
-  if (rows == 0 && !fill) return;
-  const Q4Page L(D, G, ps);
-  const unsigned char* rec = pages + ((long)max(page, 0) * nkv + kvh) * L.record;
-  const int words = D / 8, size_words = words / G;
-  const long out_base = ((long)place * nkv + kvh) * ps * D;
+}
+
+// Other sizes: a block per (page, kv head), a thread per word.
+template <typename T> __global__ void unpack_4bit_kernel(Unpack a, int D, int G, T* __restrict__ k_out, T* __restrict__ v_out) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int i = blockIdx.x / a.nkv, kvh = blockIdx.x % a.nkv;
+  const int seq = a.sequence(blockIdx.y);
+  if (seq < 0) return;
+  const int place = blockIdx.y * a.width + i;
+  if (a.table_out && kvh == 0 && threadIdx.x == 0) a.table_out[(long)seq * a.width + i] = place;
+  const int page = i < a.max_pages ? a.block_table[(long)seq * a.max_pages + i] : -1;
+  int rows = min(max(min(a.kv_lens[seq], a.max_len) - i * a.ps, 0), a.ps);
+  if (page < 0 || page >= a.num_pages) rows = 0;
+  if (rows == 0 && !a.fill) return;
+  const Q4Page L(D, G, a.ps);
+  const unsigned char* rec = a.pages + ((long)max(page, 0) * a.nkv + kvh) * L.record;
+  const int words = D / 8, size_words = words / G, ps = a.ps;
+  const long out_base = ((long)place * a.nkv + kvh) * ps * D;
   for (int u = threadIdx.x; u < 2 * ps * words; u += blockDim.x) {
     const int is_v = u >= ps * words;
     const int at = u - is_v * ps * words;
@@ -281,15 +369,32 @@ __global__ void unpack_4bit_kernel(const unsigned char* __restrict__ pages, int 
   }
 }
 
+template <typename T> cudaError_t launch_unpack(const Unpack& a, int count, int D, T* k_out, T* v_out, cudaStream_t stream) {
+  const long items = (long)a.width * a.nkv;
+  if (D == 64 || D == 128 || D == 256) {
+    const dim3 grid((unsigned)((items + 7) / 8), (unsigned)count);
+    if (D == 64) return launch_pdl(unpack_4bit_rows_kernel<T, 64>, grid, dim3(256), 0, stream, a, k_out, v_out);
+    if (D == 128) return launch_pdl(unpack_4bit_rows_kernel<T, 128>, grid, dim3(256), 0, stream, a, k_out, v_out);
+    return launch_pdl(unpack_4bit_rows_kernel<T, 256>, grid, dim3(256), 0, stream, a, k_out, v_out);
+  }
+  return launch_pdl(unpack_4bit_kernel<T>, dim3((unsigned)items, (unsigned)count), dim3(a.ps * D / 8 >= 256 ? 256 : 128), 0, stream, a, D,
+                    q4_groups(D), k_out, v_out);
+}
+
 // ---- eviction -------------------------------------------------------------------------------------------------------------------------
 // Per (layer, sequence, kv head) that holds more than `keep` tokens: which tokens stay, and who fills whose place.  Stay: positions below
 // `first`, the last `recent` positions, and of the others those with the largest sums until `keep` are found (equal sums: the lower
 // place; NaN counts as the largest).  The tokens that go leave holes among the first `keep` places, which the tokens that stay from
 // behind `keep` fill, both in order: nothing that stays in front moves, and no token's source is another's goal, so the moves are
 // independent of each other.
-// One block: order-preserving keys in shared memory (or scratch when they are too many), the threshold by four passes of a histogram
-// over 8 bits, then both lists by scans.  Limited by the latency of these passes (few blocks) or by reading sums and positions.
+// One block: order-preserving keys in shared memory (or scratch when they are too many), the threshold by three passes of a histogram over
+// 11, 11 and 10 bits (with 8 bits the first pass meets a sum's exponent alone, and counters collide), then both lists in order: a thread
+// owns neighbouring places, an odd number of them, so that threads read different banks.  What bounds it is the latency of these steps.
 constexpr int EVICT_THREADS = 1024;
+constexpr int EVICT_BINS = 2048;
+constexpr int EVICT_KEYS = 49152;           // that one block holds in shared memory; more go through scratch
+constexpr int EVICT_PLACES = 24576;         // up to here the positions fit beside them, and are read once
+constexpr int EVICT_TOGETHER = 512;         // as many moves at most are made by the block that chose them: no second kernel
 
 __device__ __forceinline__ int block_scan(int v, int* total, int* red) {  // exclusive sum over the block; red: 33 ints
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -320,157 +425,231 @@ __device__ __forceinline__ int block_scan(int v, int* total, int* red) {  // exc
 
 struct Evict {
   const int *block_table, *kv_lens;
-  int max_pages, num_pages, num_seqs, nkv, ps, keep, first, recent, cap, max_len;
+  int max_pages, num_pages, num_seqs, nkv, ps, ps_shift, keep, first, recent, cap, max_len;
+  unsigned char* pages;
+  int D, G, wide;
   float* mass;
   int* places;
   uint32_t* spill;  // null, or [pairs][max_len]: the keys when they do not fit shared memory
   int* lists;       // [pairs][1 + 2 cap]: how many, holes, movers
 };
 
+// Page and row of a place (pages of a power of two take no division).
+struct EvictRow {
+  int page, row;
+  __device__ __forceinline__ EvictRow(const Evict& a, const int* bt, int slot) {
+    const int i = a.ps_shift >= 0 ? slot >> a.ps_shift : slot / a.ps;
+    row = slot - i * a.ps;
+    page = bt[i];
+    if ((uint32_t)page >= (uint32_t)a.num_pages) page = -1;
+  }
+};
+
+// The rows of one (layer, sequence, kv head) that move: a group of 8 lanes takes four tokens at a time, so that their places, pages and
+// bytes are looked up side by side.  Rows whose codes are whole pieces of 16 bytes go in those, others in words.
+__device__ __forceinline__ void evict_move(const Evict& a, const int* list, int count, const int* bt, long layer_heads, int kvh, int group, int groups) {
+  constexpr int AT_ONCE = 4;
+  const Q4Page L(a.D, a.G, a.ps);
+  const int lane = threadIdx.x & 7;
+  for (int first = group * AT_ONCE; first < count; first += groups * AT_ONCE) {
+    int to[AT_ONCE], from[AT_ONCE], tr[AT_ONCE], fr[AT_ONCE];
+    long th[AT_ONCE], fh[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const bool is = first + u < count;
+      to[u] = is ? list[1 + first + u] : -1;
+      from[u] = is ? list[1 + a.cap + first + u] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      if (to[u] < 0) continue;
+      const EvictRow t(a, bt, to[u]), f(a, bt, from[u]);
+      tr[u] = t.row, fr[u] = f.row;
+      th[u] = layer_heads + (long)t.page * a.nkv + kvh, fh[u] = layer_heads + (long)f.page * a.nkv + kvh;
+      if (t.page < 0 || f.page < 0) to[u] = -1;
+    }
+    // parameters, sum and position: one word of each by lanes 0 .. 2 G + 1, the rest of them (more than three groups) below
+    uint32_t word[AT_ONCE];
+    uint4 piece[AT_ONCE];
+    const int pieces = L.half / 16;  // of the key's codes, then as many of the value's
+    auto word_at = [&](int v, long h, int row) -> uint32_t* {
+      if (v >= 2 * a.G) return reinterpret_cast<uint32_t*>(v == 2 * a.G ? (void*)a.mass : (void*)a.places) + h * a.ps + row;
+      const int is_v = v >= a.G;
+      return reinterpret_cast<uint32_t*>(a.pages + h * L.record + (is_v ? L.vpar : L.kpar) + (long)row * L.par + 4 * (v - is_v * a.G));
+    };
+    auto piece_at = [&](int v, long h, int row) -> uint4* {
+      const int is_v = v >= pieces;
+      return reinterpret_cast<uint4*>(a.pages + h * L.record + (is_v ? L.values : 0) + (long)row * L.half + 16 * (v - is_v * pieces));
+    };
+    const bool first_piece = a.wide && lane < 2 * pieces, first_word = lane < 2 * a.G + 2;
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+      if (to[u] >= 0) {
+        if (first_piece) piece[u] = *piece_at(lane, fh[u], fr[u]);
+        if (first_word) word[u] = *word_at(lane, fh[u], fr[u]);
+      }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+      if (to[u] >= 0) {
+        if (first_piece) *piece_at(lane, th[u], tr[u]) = piece[u];
+        if (first_word) *word_at(lane, th[u], tr[u]) = word[u];
+      }
+    for (int u = 0; u < AT_ONCE; ++u) {  // what 8 lanes do not do at once
+      if (to[u] < 0) continue;
+      for (int v = lane + 8; v < 2 * a.G + 2; v += 8) *word_at(v, th[u], tr[u]) = *word_at(v, fh[u], fr[u]);
+      if (a.wide) {
+        for (int v = lane + 8; v < 2 * pieces; v += 8) *piece_at(v, th[u], tr[u]) = *piece_at(v, fh[u], fr[u]);
+      } else {
+        const int words = L.half / 4;
+        for (int v = lane; v < 2 * words; v += 8) {
+          const int is_v = v >= words;
+          const long sec = (is_v ? L.values : 0) + 4 * (v - is_v * words);
+          *reinterpret_cast<uint32_t*>(a.pages + th[u] * L.record + sec + (long)tr[u] * L.half) =
+              *reinterpret_cast<const uint32_t*>(a.pages + fh[u] * L.record + sec + (long)fr[u] * L.half);
+        }
+      }
+    }
+  }
+}
+
 __global__ void __launch_bounds__(EVICT_THREADS, 1) evict_select_kernel(Evict a) {
   extern __shared__ uint32_t keys_s[];
-  __shared__ int hist[256], red[33], s_newest, s_digit, s_left;
+  __shared__ int bins[EVICT_BINS], red[33], s_newest, s_digit, s_left;
   pdl_wait();
   pdl_launch_dependents();
   const int kvh = blockIdx.x, seq = blockIdx.y, layer = blockIdx.z;
   const long pair = ((long)layer * a.num_seqs + seq) * a.nkv + kvh;
   int* list = a.lists + pair * (1 + 2 * (long)a.cap);
-  const int n = min(a.kv_lens[seq], a.max_len), tid = threadIdx.x;
+  const int n = min(a.kv_lens[seq], a.max_len), tid = threadIdx.x, lane = tid & 31;
+  constexpr int threads = EVICT_THREADS;
   if (n <= a.keep) {
     if (tid == 0) list[0] = 0;
     return;
   }
   uint32_t* keys = a.spill ? a.spill + pair * a.max_len : keys_s;
+  int* place_s = reinterpret_cast<int*>(keys_s) + a.max_len;
+  const bool kept_places = a.max_len <= EVICT_PLACES;
   const int* bt = a.block_table + (long)seq * a.max_pages;
-  const long layer_cells = (long)layer * a.num_pages * a.nkv * a.ps;
-  auto cell = [&](int slot) -> long {
-    const int page = bt[slot / a.ps];
-    return page < 0 || page >= a.num_pages ? -1 : layer_cells + ((long)page * a.nkv + kvh) * a.ps + slot % a.ps;
-  };
+  const long layer_heads = (long)layer * a.num_pages * a.nkv;
   if (tid == 0) s_newest = -1;
+  for (int i = tid; i < EVICT_BINS; i += threads) bins[i] = 0;
   __syncthreads();
   int newest = -1;
-  for (int i = tid; i < n; i += EVICT_THREADS) {
-    const long c = cell(i);
-    const int place = c < 0 ? -1 : a.places[c];
-    newest = max(newest, place);
-    const float m = c < 0 ? -INFINITY : a.mass[c] + 0.f;  // (minus zero is zero)
+  auto put = [&](int i, bool there, float sum, int place) {
+    newest = max(newest, there ? place : -1);
+    const float m = there ? sum + 0.f : -INFINITY;  // (minus zero is zero)
     uint32_t key = __float_as_uint(m);
     key = m != m ? 0xFFFFFFFEu : (key & 0x80000000u) ? ~key : key | 0x80000000u;
-    keys[i] = c >= 0 && place < a.first ? 0xFFFFFFFFu : key;
+    keys[i] = there && place < a.first ? 0xFFFFFFFFu : key;
+    if (kept_places) place_s[i] = there ? place : INT_MIN;
+  };
+  if (a.ps % 4 == 0) {  // four neighbours lie in one page
+    for (int i = 4 * tid; i < n; i += 4 * threads) {
+      const EvictRow at(a, bt, i);
+      float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
+      int4 p = make_int4(0, 0, 0, 0);
+      if (at.page >= 0) {
+        const long c = (layer_heads + (long)at.page * a.nkv + kvh) * a.ps + at.row;
+        m = *reinterpret_cast<const float4*>(a.mass + c);
+        p = *reinterpret_cast<const int4*>(a.places + c);
+      }
+      put(i, at.page >= 0, m.x, p.x);
+      if (i + 1 < n) put(i + 1, at.page >= 0, m.y, p.y);
+      if (i + 2 < n) put(i + 2, at.page >= 0, m.z, p.z);
+      if (i + 3 < n) put(i + 3, at.page >= 0, m.w, p.w);
+    }
+  } else {
+    for (int i = tid; i < n; i += threads) {
+      const EvictRow at(a, bt, i);
+      const long c = (layer_heads + (long)at.page * a.nkv + kvh) * a.ps + at.row;
+      put(i, at.page >= 0, at.page >= 0 ? a.mass[c] : 0.f, at.page >= 0 ? a.places[c] : 0);
+    }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) newest = max(newest, __shfl_xor_sync(0xffffffffu, newest, o));
-  if ((tid & 31) == 0) atomicMax(&s_newest, newest);
+  newest = __reduce_max_sync(0xffffffffu, newest);
+  if (lane == 0) atomicMax(&s_newest, newest);
   __syncthreads();
   newest = s_newest;
-  for (int i = tid; i < n; i += EVICT_THREADS) {
-    const long c = cell(i);
-    if (c >= 0 && a.places[c] > newest - a.recent) keys[i] = 0xFFFFFFFFu;
-  }
-  // the keep-th largest key
+  // the keep-th largest key; the first pass makes the newest positions' keys on its way
   uint32_t prefix = 0, mask = 0;
   int left = a.keep;  // how many of those that share the prefix stay
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += EVICT_THREADS)
-      if ((keys[i] & mask) == prefix) atomicAdd(&hist[(keys[i] >> shift) & 255], 1);
-    __syncthreads();
-    if (tid < 32) {  // from the largest digit down: lane l holds digits 255 - 8 l .. 248 - 8 l
-      int own = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) own += hist[255 - 8 * tid - e];
-      int sum = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, sum, o);
-        if (tid >= o) sum += y;
-      }
-      int before = sum - own;
-      if (before < left && left <= sum) {
-        for (int e = 0; e < 8; ++e) {
-          const int d = 255 - 8 * tid - e;
-          if (before + hist[d] >= left) {
-            s_digit = d;
-            s_left = left - before;
-            break;
-          }
-          before += hist[d];
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < n; i += threads) {
+      uint32_t key = keys[i];
+      if (pass == 0 && a.recent > 0) {
+        int place;
+        if (kept_places) {
+          place = place_s[i];
+        } else {
+          const EvictRow at(a, bt, i);
+          place = at.page < 0 ? INT_MIN : a.places[(layer_heads + (long)at.page * a.nkv + kvh) * a.ps + at.row];
         }
+        if (place > newest - a.recent && place != INT_MIN) keys[i] = key = 0xFFFFFFFFu;
+      }
+      if ((key & mask) == prefix) atomicAdd(&bins[(key >> shift) & ((1 << bits) - 1)], 1);
+    }
+    __syncthreads();
+    // from the largest digit down: thread t holds `per_bin` of them, the first EVICT_BINS - 1 - t * per_bin
+    const int per_bin = EVICT_BINS / threads;
+    int own = 0, all;
+    for (int e = 0; e < per_bin; ++e) own += bins[EVICT_BINS - 1 - tid * per_bin - e];
+    int before = block_scan(own, &all, red);
+    if (before < left && left <= before + own) {
+      for (int e = 0; e < per_bin; ++e) {
+        const int d = EVICT_BINS - 1 - tid * per_bin - e;
+        if (before + bins[d] >= left) {
+          s_digit = d;
+          s_left = left - before;
+          break;
+        }
+        before += bins[d];
       }
     }
     __syncthreads();
     prefix |= (uint32_t)s_digit << shift;
-    mask |= 255u << shift;
+    mask |= ((1u << bits) - 1) << shift;
     left = s_left;
+    for (int i = tid; i < EVICT_BINS; i += threads) bins[i] = 0;
+    __syncthreads();
   }
   // holes in front, movers behind, in order; of the keys equal to the threshold the first `left` stay
-  int ties = 0, holes = 0, movers = 0;
-  for (int base = 0; base < n; base += EVICT_THREADS) {
-    const int i = base + tid;
-    const uint32_t key = i < n ? keys[i] : 0;
-    const bool tie = i < n && key == prefix;
-    int t_all, f_all;
-    const int rank = ties + block_scan(tie, &t_all, red);
-    const bool stays = i < n && (key > prefix || (tie && rank < left));
-    const bool hole = i < n && i < a.keep && !stays, mover = i >= a.keep && stays;
-    const int at = block_scan((hole ? 1 : 0) | (mover ? 1 << 16 : 0), &f_all, red);  // (at most 1024 of each)
-    if (hole) list[1 + holes + (at & 0xFFFF)] = i;
-    if (mover) list[1 + a.cap + movers + (at >> 16)] = i;
-    ties += t_all;
-    holes += f_all & 0xFFFF;
-    movers += f_all >> 16;
+  const int per = ((n + threads - 1) / threads) | 1;
+  const int begin = min(n, tid * per), end = min(n, begin + per);
+  int ties = 0, all;
+  for (int i = begin; i < end; ++i) ties += keys[i] == prefix;
+  const int ties_before = block_scan(ties, &all, red);
+  auto walk = [&](auto&& hole, auto&& mover) {
+    int rank = ties_before;
+    for (int i = begin; i < end; ++i) {
+      const uint32_t key = keys[i];
+      const bool stays = key > prefix || (key == prefix && rank < left);
+      rank += key == prefix;
+      if (i < a.keep && !stays) hole(i);
+      if (i >= a.keep && stays) mover(i);
+    }
+  };
+  int holes = 0, movers = 0, count;
+  walk([&](int) { ++holes; }, [&](int) { ++movers; });
+  // (there are as many of the one as of the other, so the movers' total is the holes')
+  holes = block_scan(holes, &count, red);
+  movers = block_scan(movers, &count, red);
+  walk([&](int i) { list[1 + holes++] = i; }, [&](int i) { list[1 + a.cap + movers++] = i; });
+  if (a.cap <= EVICT_TOGETHER) {
+    __syncthreads();  // (orders the block's writes of the list, too)
+    evict_move(a, list, count, bt, layer_heads, kvh, tid >> 3, threads >> 3);
+  } else if (tid == 0) {
+    list[0] = count;
   }
-  if (tid == 0) list[0] = min(holes, movers);
 }
 
-// Moves rows: a group of 8 lanes per moved token; codes in pieces of 16 bytes, parameters in words.
-__global__ void evict_move_kernel(Evict a, unsigned char* pages, int D, int G) {
+__global__ void __launch_bounds__(256) evict_move_kernel(Evict a) {
   pdl_wait();
   pdl_launch_dependents();
   const int kvh = blockIdx.y % a.nkv, seq = blockIdx.y / a.nkv, layer = blockIdx.z;
   const long pair = ((long)layer * a.num_seqs + seq) * a.nkv + kvh;
   const int* list = a.lists + pair * (1 + 2 * (long)a.cap);
-  const int count = list[0];
-  const Q4Page L(D, G, a.ps);
-  const int* bt = a.block_table + (long)seq * a.max_pages;
-  const long layer_heads = (long)layer * a.num_pages * a.nkv;
-  const int lane = threadIdx.x & 7, per_block = blockDim.x >> 3;
-  const bool wide = L.half % 16 == 0;
-  for (int m = blockIdx.x * per_block + (threadIdx.x >> 3); m < count; m += gridDim.x * per_block) {
-    const int to = list[1 + m], from = list[1 + a.cap + m];
-    const int tp = bt[to / a.ps], fp = bt[from / a.ps];
-    if (tp < 0 || fp < 0 || tp >= a.num_pages || fp >= a.num_pages) continue;
-    const long th = layer_heads + (long)tp * a.nkv + kvh, fh = layer_heads + (long)fp * a.nkv + kvh;
-    const int tr = to % a.ps, fr = from % a.ps;
-    unsigned char *dst = pages + th * L.record, *src = pages + fh * L.record;
-    if (wide) {
-      const int pieces = L.half / 16;
-      for (int u = lane; u < 2 * pieces; u += 8) {
-        const int is_v = u >= pieces;
-        const long sec = is_v ? L.values : 0, off = 16 * (u - is_v * pieces);
-        *reinterpret_cast<uint4*>(dst + sec + (long)tr * L.half + off) = *reinterpret_cast<const uint4*>(src + sec + (long)fr * L.half + off);
-      }
-    } else {
-      const int words = L.half / 4;
-      for (int u = lane; u < 2 * words; u += 8) {
-        const int is_v = u >= words;
-        const long sec = is_v ? L.values : 0, off = 4 * (u - is_v * words);
-        *reinterpret_cast<uint32_t*>(dst + sec + (long)tr * L.half + off) =
-            *reinterpret_cast<const uint32_t*>(src + sec + (long)fr * L.half + off);
-      }
-    }
-    for (int u = lane; u < 2 * G; u += 8) {
-      const int is_v = u >= G;
-      const long sec = is_v ? L.vpar : L.kpar, off = 4 * (u - is_v * G);
-      *reinterpret_cast<uint32_t*>(dst + sec + (long)tr * L.par + off) =
-          *reinterpret_cast<const uint32_t*>(src + sec + (long)fr * L.par + off);
-    }
-    if (lane == 0) a.mass[th * a.ps + tr] = a.mass[fh * a.ps + fr];
-    if (lane == 1) a.places[th * a.ps + tr] = a.places[fh * a.ps + fr];
-  }
+  evict_move(a, list, list[0], a.block_table + (long)seq * a.max_pages, (long)layer * a.num_pages * a.nkv, kvh,
+             blockIdx.x * (blockDim.x >> 3) + (threadIdx.x >> 3), gridDim.x * (blockDim.x >> 3));
 }
 
 inline bool q4_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -525,52 +704,45 @@ Q3_EXPORT int q3_unpack_4bit(int dtype, const void* pages, int num_pages, int nk
   if (!pages || !block_table || !kv_lens || !k_out || !v_out || nkv < 1 || max_pages < 1 || !q4_sizes_ok(D, ps)) return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
   if (count < 1 || width < 1) return Q3_OK;
-  if (nkv > 65535 || count > 65535) return Q3_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)width, (unsigned)nkv, (unsigned)count);
-  const int G = q4_groups(D);
-  const int threads = ps * D / 8 >= 256 ? 256 : 128;
-  const cudaError_t err =
-      dtype == Q3_DTYPE_F32
-          ? launch_pdl(unpack_4bit_kernel<float>, grid, dim3(threads), 0, stream, (const unsigned char*)pages, num_pages, nkv, D, G, ps,
-                       block_table, max_pages, kv_lens, num_seqs, max_len, cu_seqlens, width, fill, (float*)k_out, (float*)v_out, table_out)
-          : launch_pdl(unpack_4bit_kernel<bf16>, grid, dim3(threads), 0, stream, (const unsigned char*)pages, num_pages, nkv, D, G, ps,
-                       block_table, max_pages, kv_lens, num_seqs, max_len, cu_seqlens, width, fill, (bf16*)k_out, (bf16*)v_out, table_out);
+  if (count > 65535) return Q3_ERR_UNSUPPORTED;
+  if ((long)width * nkv > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
+  const Unpack a{(const unsigned char*)pages, num_pages, nkv, ps, block_table, kv_lens, cu_seqlens, max_pages, num_seqs, max_len, width, fill,
+                 table_out};
+  const cudaError_t err = dtype == Q3_DTYPE_F32 ? launch_unpack(a, count, D, (float*)k_out, (float*)v_out, stream)
+                                                : launch_unpack(a, count, D, (bf16*)k_out, (bf16*)v_out, stream);
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
 }
 
-// Keys that one block holds in shared memory; above, `spill` is needed.
-#define Q3_EVICT_KEYS 49152
-
-Q3_EXPORT int q3_evict_4bit_keys() { return Q3_EVICT_KEYS; }
-
+// `lists`: [layers * sequences * kv heads][1 + 2 cap] ints; `spill`: the same times max_len, for more than EVICT_KEYS tokens.
 Q3_EXPORT int q3_evict_4bit(void* pages, int num_layers, int num_pages, int nkv, int D, int ps, float* mass, int* places,
                             const int* block_table, int max_pages, const int* kv_lens, int num_seqs, int max_len, int keep, int first,
                             int recent, int cap, void* spill, int* lists, cudaStream_t stream) {
   if (!pages || !mass || !places || !block_table || !kv_lens || !lists || nkv < 1 || max_pages < 1 || !q4_sizes_ok(D, ps))
     return Q3_ERR_ARGUMENT;
   if (keep < 1 || first < 0 || recent < 0 || (long)first + recent > keep || cap < 1 || max_len > (long)max_pages * ps) return Q3_ERR_ARGUMENT;
-  if (max_len > Q3_EVICT_KEYS && !spill) return Q3_ERR_ARGUMENT;
+  if (max_len > EVICT_KEYS && !spill) return Q3_ERR_ARGUMENT;
   if (num_seqs < 1 || num_layers < 1 || max_len <= keep) return Q3_OK;
+  if (cap < (keep < max_len - keep ? keep : max_len - keep)) return Q3_ERR_ARGUMENT;
   if (num_seqs > 65535 || num_layers > 65535 || (long)num_seqs * nkv > 65535) return Q3_ERR_UNSUPPORTED;
-  Evict a{block_table, kv_lens, max_pages, num_pages, num_seqs, nkv, ps, keep, first, recent, cap, max_len, mass, places,
-          max_len > Q3_EVICT_KEYS ? (uint32_t*)spill : nullptr, lists};
+  int shift = 0;
+  while ((1 << shift) < ps) ++shift;
+  Evict a{block_table, kv_lens, max_pages, num_pages, num_seqs, nkv, ps, (1 << shift) == ps ? shift : -1, keep, first, recent, cap, max_len,
+          (unsigned char*)pages, D, q4_groups(D), (D / 2) % 16 == 0, mass, places, max_len > EVICT_KEYS ? (uint32_t*)spill : nullptr, lists};
   static bool once[Q3_MAX_DEVICES];
   const int dev = q3_current_device();
   if (!once[dev]) {
-    if (cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * Q3_EVICT_KEYS) != cudaSuccess)
+    if (cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * EVICT_KEYS) != cudaSuccess)
       return Q3_ERR_LAUNCH;
     once[dev] = true;
   }
-  const size_t smem = a.spill ? 0 : 4 * (size_t)max_len;
+  const size_t smem = a.spill ? 0 : (max_len <= EVICT_PLACES ? 8 : 4) * (size_t)max_len;
   cudaError_t err = launch_pdl(evict_select_kernel, dim3(nkv, num_seqs, num_layers), dim3(EVICT_THREADS), smem, stream, a);
   if (err != cudaSuccess) return Q3_ERR_LAUNCH;
-  const int G = q4_groups(D);
+  if (cap <= EVICT_TOGETHER) return Q3_OK;
+  // 128 tokens a block at a time, about eight blocks an SM
   const long pairs = (long)num_seqs * nkv * num_layers;
-  // 32 tokens a block at a time, about eight blocks an SM
-  long chunks = (cap + 31) / 32, most = (148 * 8 + pairs - 1) / pairs;
+  long chunks = (cap + 127) / 128, most = (148 * 8 + pairs - 1) / pairs;
   if (chunks > most) chunks = most;
-  if (chunks < 1) chunks = 1;
-  err = launch_pdl(evict_move_kernel, dim3((unsigned)chunks, (unsigned)(num_seqs * nkv), (unsigned)num_layers), dim3(256), 0, stream, a,
-                   (unsigned char*)pages, D, G);
+  err = launch_pdl(evict_move_kernel, dim3((unsigned)chunks, (unsigned)(num_seqs * nkv), (unsigned)num_layers), dim3(256), 0, stream, a);
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
 }

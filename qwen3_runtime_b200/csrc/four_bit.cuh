@@ -57,14 +57,23 @@ __device__ __forceinline__ Q4Scale q4_scale(float lo, float hi, float poison) {
   }
   return y;
 }
-__device__ __forceinline__ uint32_t q4_code(float x, const Q4Scale& y) {
-  if (!(y.s > 0.f)) return 0;  // one value all over, or NaN
-  return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x - y.z, y.s)), 0.f), 15.f);
-}
+// (x - z) / s for several x: with y = 1 / s rounded to nearest, q = x y and its remainder x - q s (exact in one fused step), q + remainder * y
+// is the rounded quotient (Markstein, IBM J. Res. Dev. 34, 1990), as long as nothing leaves the range of normal numbers.
 __device__ __forceinline__ uint32_t q4_word(const float (&x)[8], const Q4Scale& y) {
   uint32_t w = 0;
+  if (!(y.s > 0.f)) return 0;  // one value all over, or NaN
+  if (y.s > 0x1p-90f && y.s < 0x1p90f) {
+    const float inv = __frcp_rn(y.s);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w |= q4_code(x[e], y) << (4 * e);
+    for (int e = 0; e < 8; ++e) {
+      const float d = x[e] - y.z, q = d * inv;
+      const float n = rintf(fmaf(fmaf(-q, y.s, d), inv, q));
+      w |= (uint32_t)fminf(fmaxf(n, 0.f), 15.f) << (4 * e);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[e] - y.z, y.s)), 0.f), 15.f) << (4 * e);
+  }
   return w;
 }
 __device__ __forceinline__ float q4_s(uint32_t word) { return __uint_as_float(word << 16); }

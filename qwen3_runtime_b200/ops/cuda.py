@@ -250,7 +250,7 @@ _SIGNATURES = {
                                      c_int, c_void_p, c_void_p, c_void_p],
         "q3_attention_mass_4bit": [c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
-                                   c_void_p],
+                                   c_int, c_void_p],
     },
     "gemm_f32": {
         "q3_gemm_f32": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
@@ -484,6 +484,14 @@ def chunk_segment(cu, H, D, Dv, sms, seg) -> int:
         if best is None or cost < best:
             best, found = cost, seg
     return found
+
+
+@functools.lru_cache(maxsize=None)
+def _four_bit_record(head_dim: int, page_size: int) -> int:
+    """Bytes of a page's record; 0 for sizes that do not exist."""
+    if head_dim % 16 or not 16 <= head_dim <= 256 or page_size < 1:
+        return 0
+    return four_bit_page_bytes(head_dim, page_size)
 
 
 class CudaOps:
@@ -2086,28 +2094,24 @@ class CudaOps:
     # ---- a cache in 4 bits (csrc/four_bit.cuh says how a page is laid out and how values are rounded) ----------------------
     EVICT_KEYS = 49152  # tokens of a sequence whose keys one block sorts in shared memory; longer ones use scratch
 
-    def _check_4bit(self, what, pages, num_kv_heads, head_dim, page_size, block_table=None, kv_lens=None, layers=False):
-        if head_dim % 16 or not 16 <= head_dim <= 256 or page_size < 1 or num_kv_heads < 1:
+    def _check_4bit(self, what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens=None, layers=False):
+        record = _four_bit_record(head_dim, page_size)
+        if not record or num_kv_heads < 1:
             raise KernelError(f"{what}: head sizes are multiples of 16 up to 256, pages and heads at least one "
                               f"(got head_dim={head_dim}, page_size={page_size}, num_kv_heads={num_kv_heads})")
-        shape = (num_kv_heads, four_bit_page_bytes(head_dim, page_size))
-        if (pages.dtype != torch.uint8 or pages.dim() not in ((3, 4) if layers else (3,)) or tuple(pages.shape[-2:]) != shape
-                or not pages.is_contiguous()):
-            raise KernelError(f"{what}: pages are dense uint8 [pages, {shape[0]}, {shape[1]}], got {pages.dtype} {tuple(pages.shape)}")
-        self._check_here(what, pages)
-        if block_table is not None:
-            if (block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous()
-                    or block_table.shape[1] < 1):
-                raise KernelError(f"{what}: the block table is dense int32 [sequences, pages], at least one page wide")
-            self._check_here(what, block_table)
-        if kv_lens is not None:
-            if kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous() or kv_lens.numel() < (block_table.shape[0]):
-                raise KernelError(f"{what}: lengths are dense int32, one per row of the block table")
-            self._check_here(what, kv_lens)
+        dims = pages.dim()
+        if (pages.dtype != torch.uint8 or (dims != 3 and not (layers and dims == 4)) or pages.size(-1) != record
+                or pages.size(-2) != num_kv_heads or not pages.is_contiguous()):
+            raise KernelError(f"{what}: pages are dense uint8 [pages, {num_kv_heads}, {record}], got {pages.dtype} {tuple(pages.shape)}")
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous() or block_table.size(1) < 1:
+            raise KernelError(f"{what}: the block table is dense int32 [sequences, pages], at least one page wide")
+        if kv_lens is not None and (kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous() or kv_lens.numel() < block_table.size(0)):
+            raise KernelError(f"{what}: lengths are dense int32, one per row of the block table")
+        self._check_here(what, pages, block_table, kv_lens)
 
     def _check_here(self, what, *tensors):
         for t in tensors:
-            if t is not None and (not t.is_cuda or t.device.index != self._device_index):
+            if t is not None and t.get_device() != self._device_index:
                 raise KernelError(f"{what}: this kernel table launches on cuda:{self._device_index}, a tensor is on {t.device}")
 
     def _check_cells(self, what, t, dtype, pages, page_size):
@@ -2190,25 +2194,29 @@ class CudaOps:
         float32 and other head sizes have their sequences' pages unpacked once and go through the kernels for wide pages.
         ``lse`` (float32 ``[T, heads]``, steps of single tokens of those sizes): gets the logarithm of each row's sum."""
         what = "paged_attention_4bit"
-        _dtype_code(out.dtype)
-        T, D, G, H = out.shape[0], head_dim, num_kv_heads, num_heads
+        T, D, G, H, dtype = out.size(0), head_dim, num_kv_heads, num_heads, out.dtype
         self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens)
-        if H % G or q.dtype != out.dtype or out.stride(1) != 1 or out.shape[1] != H * D or out.stride(0) != H * D:
+        if H % G or q.dtype != dtype or out.dim() != 2 or out.size(1) != H * D or not out.is_contiguous():
             raise KernelError(f"{what}: out is dense [tokens, heads * head_dim] of the queries' type, heads a multiple of kv heads")
+        if q.dim() != 2 or q.size(0) < T or q.size(1) < H * D or q_stride < H * D or T != step.num_tokens:
+            raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step")
         self._check_here(what, q, out, lse)
-        max_len = min(step.captured_width * page_size or step.max_kv_len, block_table.shape[1] * page_size)
-        if step.max_kv_len > block_table.shape[1] * page_size:
-            raise KernelError(f"{what}: {step.max_kv_len} tokens do not fit a block table of {block_table.shape[1]} pages")
-        fast = (out.dtype == torch.bfloat16 and D in (64, 128, 256) and H // G <= 16 and q_stride % 8 == 0 and q.data_ptr() % 16 == 0
+        room = block_table.size(1) * page_size
+        if step.max_kv_len > room or step.num_seqs > block_table.size(0):
+            raise KernelError(f"{what}: {step.num_seqs} sequences of up to {step.max_kv_len} tokens do not fit a block table of "
+                              f"{block_table.size(0)} x {block_table.size(1)} pages")
+        max_len = min(step.captured_width * page_size, room) if step.captured_width else step.max_kv_len
+        fast = (dtype == torch.bfloat16 and D in (64, 128, 256) and H // G <= 16 and q_stride % 8 == 0 and q.data_ptr() % 16 == 0
                 and out.data_ptr() % 8 == 0)
         if lse is not None and not (fast and step.decode_only):
             raise KernelError(f"{what}: log sums come from steps of single tokens in bfloat16, head sizes 64, 128 and 256")
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (T, H) or not lse.is_contiguous()):
+        if lse is not None and (lse.dtype != torch.float32 or lse.dim() != 2 or lse.size(0) != T or lse.size(1) != H or not lse.is_contiguous()):
             raise KernelError(f"{what}: log sums are dense float32 [tokens, heads]")
         if fast and step.decode_only:
             return self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, None, step.num_seqs, max_len,
                                      decode_slices or self.decode_slices_4bit(step.host_kv_lens, G, D, window), out, page_size, scale,
                                      window, step.kv_longest, lse)
+        _dtype_code(dtype)
         wide = dict(num_heads=H, num_kv_heads=G, head_dim=D, token_seq=step.token_seq, positions=step.positions, out=out,
                     page_size=page_size, scale=scale, window=window)
         n = -(-max_len // page_size)
@@ -2237,26 +2245,29 @@ class CudaOps:
 
     def decode_slices_4bit(self, kv_lens, num_kv_heads, head_dim, window) -> int:
         """Into how many slices the longest of these sequences' keys are cut by decode attention over a cache in 4 bits."""
-        tiles = [-(-min(n, window or n) // 128) for n in kv_lens if n > 0]
-        if not tiles:
+        longest, total, count = max(kv_lens, default=0), sum(kv_lens), len(kv_lens)
+        if window:
+            longest, total = min(longest, window + 15), min(total, count * (window + 15))
+        if longest < 1:
             return 1
         slots = self.DECODE_4BIT_BLOCKS_PER_SM[head_dim] * self.SM_COUNT
-        per = max(1, -(-sum(tiles) * num_kv_heads // slots))
-        return max(1, min(64, -(-max(tiles) // per)))
+        per = max(1, -(-(total + 64 * count) * num_kv_heads // (128 * slots)))  # rounds of 128 keys a block
+        return max(1, min(64, -(-longest // (128 * per))))
 
     def _decode_4bit(self, q, q_stride, H, G, D, pages, block_table, step, seq_list, num_seqs, max_len, slices, out, page_size, scale,
                      window, longest, lse):
         mid_o = mid_lse = None
-        if slices > 16 or slices * G * num_seqs > self.SM_COUNT:  # else the blocks of a cluster join them
-            mid_o = torch.empty((num_seqs, H, slices, D), dtype=torch.float32, device=out.device)
-            mid_lse = torch.empty((num_seqs, H, slices), dtype=torch.float32, device=out.device)
+        if slices > 16 or (slices > 1 and slices * G * num_seqs > self.SM_COUNT):  # else the blocks of a cluster join them
+            mid = torch.empty(num_seqs * H * slices * (D + 1), dtype=torch.float32, device=out.device)
+            mid_o = mid.data_ptr()
+            mid_lse = mid_o + 4 * num_seqs * H * slices * D
             self.launches += 1
         if self.timing is not None:
             singles = [kv for b, kv in enumerate(step.host_kv_lens) if step.host_cu_seqlens[b + 1] - step.host_cu_seqlens[b] == 1]
             self._costs(sum(singles) * G * four_bit_token_bytes(D) + 4 * num_seqs * H * D, 4 * H * D * sum(singles))
         self._call("attention_4bit", "q3_decode_attention_4bit", "paged_attention_decode_4bit", _ptr(q), q_stride, _ptr(pages),
                    pages.shape[0], _ptr(block_table), block_table.shape[1], _ptr(step.kv_lens), _ptr(step.cu_seqlens), _ptr(seq_list),
-                   _ptr(out), _ptr(mid_o), _ptr(mid_lse), _ptr(lse), num_seqs, H, G, D, page_size, float(scale), int(window or 0),
+                   _ptr(out), mid_o, mid_lse, _ptr(lse), num_seqs, H, G, D, page_size, float(scale), int(window or 0),
                    slices, max_len, _ptr(longest), _ptr(self._error_word(out.device)))
         return out
 
@@ -2273,14 +2284,24 @@ class CudaOps:
         T = step.num_tokens
         if num_heads % num_kv_heads or q_stride % 8 or q.data_ptr() % 16:
             raise KernelError(f"{what}: heads are a multiple of kv heads, rows of queries begin at multiples of 16 bytes")
+        if q.dim() != 2 or q.size(0) < T or q.size(1) < num_heads * head_dim or q_stride < num_heads * head_dim:
+            raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step")
         if observe is not None and observe < 1:
             raise KernelError(f"{what}: observe at least one token, or None for all")
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (T, num_heads) or not lse.is_contiguous()):
+        if lse is not None and (lse.dtype != torch.float32 or lse.dim() != 2 or lse.size(0) != T or lse.size(1) != num_heads or not lse.is_contiguous()):
             raise KernelError(f"{what}: log sums are dense float32 [tokens, heads]")
-        max_len = min(step.captured_width * page_size or step.max_kv_len, block_table.shape[1] * page_size)
+        room = block_table.size(1) * page_size
+        if step.max_kv_len > room or step.num_seqs > block_table.size(0):
+            raise KernelError(f"{what}: {step.num_seqs} sequences of up to {step.max_kv_len} tokens do not fit a block table of "
+                              f"{block_table.size(0)} x {block_table.size(1)} pages")
+        max_len = min(step.captured_width * page_size, room) if step.captured_width else step.max_kv_len
         observe = int(min(observe or 1 << 30, 1 << 30))
-        cu = step.host_cu_seqlens
-        counts = [min(observe, cu[b + 1] - cu[b]) for b in range(step.num_seqs)]
+        if step.decode_only:
+            counts, most = [1] * step.num_seqs, 1
+        else:
+            cu = step.host_cu_seqlens
+            counts = [min(observe, cu[b + 1] - cu[b]) for b in range(step.num_seqs)]
+            most = max(counts, default=0)
         have, part, slices = lse is not None, None, 1
         if not have:
             lse = torch.empty((T, num_heads), dtype=torch.float32, device=q.device)
@@ -2289,13 +2310,15 @@ class CudaOps:
             slices = max(1, min(16, 2 * self.SM_COUNT // max(1, blocks), max_len // 128))
             if slices > 1:
                 part = torch.empty((T, num_heads, slices, 2), dtype=torch.float32, device=q.device)
+        # few rows: blocks of at least 128 keys, about four an SM for the sequences' keys together
+        total = sum(step.host_kv_lens) * num_kv_heads
+        few = max(1, min(-(-max_len // 128), -(-max_len * 4 * self.SM_COUNT // max(1, total))))
         if self.timing is not None:
             seen = sum(n * kv - n * (n - 1) // 2 for n, kv in zip(counts, step.host_kv_lens))
             self._costs(sum(step.host_kv_lens) * num_kv_heads * (four_bit_token_bytes(head_dim) // 2 + 8), 2 * num_heads * head_dim * seen)
         self._call("attention_4bit", "q3_attention_mass_4bit", what, code, _ptr(q), q_stride, _ptr(pages), pages.shape[0],
                    _ptr(block_table), block_table.shape[1], _ptr(step.kv_lens), _ptr(step.cu_seqlens), _ptr(mass), _ptr(lse), int(have),
-                   _ptr(part), slices, step.num_seqs, num_heads, num_kv_heads, head_dim, page_size, float(scale), max_len, observe,
-                   max(counts, default=0))
+                   _ptr(part), slices, step.num_seqs, num_heads, num_kv_heads, head_dim, page_size, float(scale), max_len, observe, most, few)
 
     def evict_4bit(self, *, pages, mass, places, block_table, kv_lens, max_kv_len, keep, first, recent, num_kv_heads, head_dim,
                    page_size):

@@ -199,8 +199,12 @@ def test_norm_and_rotation_are_those_of_the_wide_cache(ops, dtype, D, rot, pairi
     before = qkv.clone()
     ops.qk_norm_rope_store_4bit(qkv, pages=pages, q_out=q, **args)
     assert torch.equal(qkv, before), "with q_out the projection stays as it is"
-    err = (q.float() - wide[:, : H * D]).abs()
-    assert bool((err <= (2 * U if dtype == BF16 else 2.0 ** -20) * wide[:, : H * D].abs().clamp(min=1e-3)).all())
+    # a turned element is a difference of two products, each at most the pair's length, which turning keeps and which is at most
+    # sqrt(2) times the head's largest element: the two ways round those products and the norm (a few units of 2^-24), and store the
+    # result rounded to its own type
+    want = wide[:, : H * D].view(T, H, D)
+    err = (q.float().view(T, H, D) - want).abs()
+    assert bool((err <= 2.0 ** -20 * 2 ** 0.5 * want.abs().amax(-1, keepdim=True) + (U * want.abs() if dtype == BF16 else 0)).all())
     k, v = ops.unpack_4bit(pages, num_kv_heads=G, head_dim=D, page_size=page, block_table=table, kv_lens=pos[-1:] + 1, max_kv_len=T, dtype=F32)
     used = -(-T // page)
     for got, src in ((k, kp), (v, vp)):
