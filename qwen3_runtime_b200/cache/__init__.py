@@ -1,3 +1,3 @@
-from .manager import FREED, CacheError, CacheManager, GroupSpec, PageAllocator, RequestCache, SlotAllocator
+from .manager import FREED, CacheError, CacheManager, GroupSpec, PageAllocator, RequestCache, SlotAllocator, TokenBudget
 
-__all__ = ["FREED", "CacheError", "CacheManager", "GroupSpec", "PageAllocator", "RequestCache", "SlotAllocator"]
+__all__ = ["FREED", "CacheError", "CacheManager", "GroupSpec", "PageAllocator", "RequestCache", "SlotAllocator", "TokenBudget"]

@@ -43,7 +43,10 @@ class KVLayerSpec:
     ``keep_first``: with a window, the sequence's first ``keep_first`` tokens stay readable as well.
     ``chunk``: a token reads only the keys of its own chunk of that many tokens (counted from the sequence's
     first token); pages wholly before the current chunk are given back.  A tuple of chunk sizes: several layers read
-    this one's keys, each under chunks of its own; a page is given back when none of them needs it any more."""
+    this one's keys, each under chunks of its own; a page is given back when none of them needs it any more.
+    ``bits`` 4: keys and values are held in 4 bits, one byte tensor ``[layers, pages + 1, kv_heads, four_bit_page_bytes]``
+    (csrc/four_bit.cuh).  ``sums``: beside them each token's summed attention weight and its position, float32 and int32
+    ``[layers, pages + 1, kv_heads, page_size]``, for requests that are cut to a budget of tokens."""
 
     num_kv_heads: int
     head_dim: int
@@ -51,6 +54,8 @@ class KVLayerSpec:
     value_dim: int | None = None
     keep_first: int = 0
     chunk: int | tuple[int, ...] | None = None
+    bits: int | None = None
+    sums: bool = False
 
     @property
     def split(self) -> bool:
@@ -89,8 +94,8 @@ def kept_for_readers(cache_id, own, others: list):
         return own
     specs = [own, *others]
     if (not all(isinstance(s, KVLayerSpec) for s in specs)
-            or any((s.num_kv_heads, s.head_dim, s.value_dim or s.head_dim)
-                   != (own.num_kv_heads, own.head_dim, own.value_dim or own.head_dim) for s in specs)):
+            or any((s.num_kv_heads, s.head_dim, s.value_dim or s.head_dim, s.bits, s.sums)
+                   != (own.num_kv_heads, own.head_dim, own.value_dim or own.head_dim, own.bits, own.sums) for s in specs)):
         raise ValueError(f"a run entry reads cache layer {cache_id} whose layout differs from its own")
     window = chunk = None
     keep_first = 0
@@ -99,7 +104,8 @@ def kept_for_readers(cache_id, own, others: list):
         chunk = chunk[0] if len(chunk) == 1 else chunk
     elif all(s.window for s in specs):
         window, keep_first = max(s.window for s in specs), max(s.keep_first for s in specs)
-    return KVLayerSpec(own.num_kv_heads, own.head_dim, window, value_dim=own.value_dim, keep_first=keep_first, chunk=chunk)
+    return KVLayerSpec(own.num_kv_heads, own.head_dim, window, value_dim=own.value_dim, keep_first=keep_first, chunk=chunk,
+                       bits=own.bits, sums=own.sums)
 
 
 @dataclass(frozen=True)
@@ -164,6 +170,8 @@ class CacheLayout:
             s = g.layer_spec
             if isinstance(s, LatentLayerSpec):
                 out.append(len(g.cache_ids) * s.width * page_size * dtype_bytes)
+            elif s.bits == 4:
+                out.append(len(g.cache_ids) * s.num_kv_heads * (four_bit_page_bytes(s.head_dim, page_size) + 8 * page_size * s.sums))
             else:
                 per_token = s.num_kv_heads * (s.head_dim + (s.value_dim or s.head_dim))
                 out.append(len(g.cache_ids) * per_token * page_size * dtype_bytes)

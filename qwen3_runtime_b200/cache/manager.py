@@ -70,6 +70,32 @@ class GroupSpec:
         return self.window or (max(self.chunks) if self.chunks else None)
 
 
+@dataclass(frozen=True)
+class TokenBudget:
+    """Requests keep at most ``keep`` tokens in the cache, each kv head its own: the sequence's ``first`` ones, the last ``recent`` and of
+    the others those that were given the most attention (csrc/cache_4bit.cu).  A request is cut when it holds more than ``keep + slack``.
+    ``observe``: how many last tokens of a prompt's portion give weight (a decoded token always does)."""
+
+    keep: int
+    first: int = 4
+    recent: int | None = None  # None: half of what is kept
+    slack: int | None = None  # None: an eighth of what is kept
+    observe: int = 32
+
+    def __post_init__(self) -> None:
+        if self.keep < 1:
+            raise ValueError("a token budget keeps at least one token")
+        object.__setattr__(self, "first", min(self.first, self.keep) if self.first == 4 else self.first)
+        if self.recent is None:
+            object.__setattr__(self, "recent", min(self.keep // 2, self.keep - self.first))
+        if self.slack is None:
+            object.__setattr__(self, "slack", self.keep // 8)
+        if self.first < 0 or self.recent < 0 or self.first + self.recent > self.keep:
+            raise ValueError(f"a token budget of {self.keep} cannot keep {self.first} first and {self.recent} last tokens")
+        if self.slack < 0 or self.observe < 1:
+            raise ValueError("a token budget needs slack >= 0 and observe >= 1")
+
+
 class PageAllocator:
     """Page ids ``0..num_pages-1`` with a first-in first-out free list and owner checks."""
 
@@ -141,10 +167,16 @@ class RequestCache:
     num_computed: int = 0  # tokens whose keys/values/state are in the cache
     num_reserved: int = 0  # tokens for which pages are reserved (>= num_computed)
     needs_state_reset: bool = True  # its slot must be zeroed before its next step
+    num_evicted: int = 0  # tokens that a budget has dropped: token p lies at place p - num_evicted or was moved, or is gone
     closed: bool = field(default=False, repr=False)
     # int32 copies of ``tables`` kept in step with them, so that a step's block tables are
     # filled with array copies instead of per-element conversions
     table_arrays: list = field(default_factory=list, repr=False)
+
+    @property
+    def held(self) -> int:
+        """Tokens whose keys and values the cache still holds."""
+        return self.num_computed - self.num_evicted
 
     def table_array(self, paged_index: int) -> np.ndarray:
         """The block table of one paged group as an int32 array (a view; do not keep it)."""
@@ -162,9 +194,13 @@ class RequestCache:
 
 
 class CacheManager:
-    def __init__(self, groups: list[GroupSpec], page_size: int, num_pages: int | list[int], num_slots: int):
+    def __init__(self, groups: list[GroupSpec], page_size: int, num_pages: int | list[int], num_slots: int,
+                 budget: TokenBudget | None = None):
         if page_size < 1:
             raise ValueError("page_size must be positive")
+        if budget is not None and any(g.kind in ("window", "chunk") for g in groups):
+            raise ValueError("a token budget cuts groups that keep every key; windows and chunks give back their own pages")
+        self.budget = budget
         self.groups = list(groups)
         self.page_size = page_size
         self.paged_groups = [i for i, g in enumerate(self.groups) if g.paged]
@@ -190,6 +226,8 @@ class CacheManager:
 
     def fits_at_all(self, num_tokens: int) -> bool:
         """Could a request of this many tokens ever be held, with the pool otherwise empty?"""
+        if self.budget is not None:  # cut after every step, and a portion is trimmed to what fits: one token more than the budget will do
+            num_tokens = min(num_tokens, self.budget.keep + self.budget.slack + 1)
         need = self.pages_for(num_tokens)
         return all(need <= a.num_pages for a in self.allocators)
 
@@ -201,12 +239,12 @@ class CacheManager:
         n = limit
         for table, alloc in zip(rc.tables, self.allocators):
             capacity = (len(table) + alloc.num_free) * self.page_size
-            n = min(n, capacity - rc.num_computed)
+            n = min(n, capacity - rc.held)
         return max(0, n)
 
     def new_pages_needed(self, rc: RequestCache, num_tokens: int) -> list[int]:
         """Pages that :meth:`reserve` would take from each paged group's pool for these tokens."""
-        need = self.pages_for(rc.num_computed + num_tokens)
+        need = self.pages_for(rc.held + num_tokens)
         return [max(0, need - len(table)) for table in rc.tables]
 
     def can_reserve(self, rc: RequestCache, num_tokens: int) -> bool:
@@ -229,7 +267,7 @@ class CacheManager:
         if not self.can_reserve(rc, num_tokens):
             raise CacheError("page pool exhausted")
         end = rc.num_computed + num_tokens
-        need = self.pages_for(end)
+        need = self.pages_for(end - rc.num_evicted)
         for pi, (table, alloc) in enumerate(zip(rc.tables, self.allocators)):
             while len(table) < need:
                 rc._append_page(pi, alloc.allocate())
@@ -260,12 +298,27 @@ class CacheManager:
                     table[idx] = FREED
                     rc.table_arrays[self.paged_groups.index(gi)][idx] = FREED
 
+    def over_budget(self, rc: RequestCache) -> bool:
+        return self.budget is not None and rc.held > self.budget.keep + self.budget.slack
+
+    def cut(self, rc: RequestCache) -> None:
+        """Record that the request was cut to its budget; give back the pages behind what is kept (and what is reserved)."""
+        self._check_open(rc)
+        if self.budget is None or rc.held <= self.budget.keep:
+            raise CacheError("there is nothing to cut")
+        rc.num_evicted = rc.num_computed - self.budget.keep
+        need = self.pages_for(rc.num_reserved - rc.num_evicted)
+        for table, alloc in zip(rc.tables, self.allocators):
+            while len(table) > need:
+                alloc.release(table.pop())
+
     def reset(self, rc: RequestCache) -> None:
         """Give back every page and forget what was computed (preemption by recompute)."""
         self._check_open(rc)
         self._release_pages(rc)
         rc.num_computed = 0
         rc.num_reserved = 0
+        rc.num_evicted = 0
         rc.needs_state_reset = True
 
     def close(self, rc: RequestCache) -> None:

@@ -6,7 +6,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .layout import CacheLayout, KVLayerSpec, LatentLayerSpec, StateLayerSpec, flatten_specs
+from .layout import CacheLayout, KVLayerSpec, LatentLayerSpec, StateLayerSpec, flatten_specs, four_bit_page_bytes
 
 
 @dataclass
@@ -22,6 +22,9 @@ class CacheLayerView:
     state: torch.Tensor | None  # [slots + 1, *shape]
     writes: bool = True
     latent_pages: torch.Tensor | None = None  # [pages + 1, page_size, width] (a latent group)
+    packed_pages: torch.Tensor | None = None  # uint8 [pages + 1, kv_heads, bytes of a page] (a group held in 4 bits)
+    mass: torch.Tensor | None = None  # float32 [pages + 1, kv_heads, page_size]: summed attention weights (a group with sums)
+    places: torch.Tensor | None = None  # int32, the same shape: positions
 
 
 class CacheStorage:
@@ -40,8 +43,16 @@ class CacheStorage:
         self.scratch_page = tuple(self.num_pages)
         self.scratch_slot = num_slots
         self.tensors: list[torch.Tensor] = []
+        self.sums: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}  # group -> (summed weights, positions)
         for gi, g in enumerate(layout.groups):
             s = g.layer_spec
+            if isinstance(s, KVLayerSpec) and s.bits == 4:
+                shape = (len(g.cache_ids), self.num_pages[layout.paged_groups.index(gi)] + 1, s.num_kv_heads)
+                self.tensors.append(torch.zeros((*shape, four_bit_page_bytes(s.head_dim, page_size)), dtype=torch.uint8, device=device))
+                if s.sums:
+                    self.sums[gi] = (torch.zeros((*shape, page_size), dtype=torch.float32, device=device),
+                                     torch.zeros((*shape, page_size), dtype=torch.int32, device=device))
+                continue
             if isinstance(s, KVLayerSpec) and s.split:  # keys and values of unlike sizes: a tensor each
                 pages = self.num_pages[layout.paged_groups.index(gi)]
                 shape = (len(g.cache_ids), pages + 1, s.num_kv_heads, page_size)
@@ -80,6 +91,11 @@ class CacheStorage:
         if isinstance(t, tuple):
             return CacheLayerView(gi, self.layout.paged_groups.index(gi), self.page_size, g.spec.window,
                                   t[0][li], t[1][li], None, writes)
+        if g.spec.paged and getattr(g.layer_spec, "bits", None) == 4:
+            mass, places = self.sums.get(gi, (None, None))
+            return CacheLayerView(gi, self.layout.paged_groups.index(gi), self.page_size, g.spec.window, None, None, None, writes,
+                                  packed_pages=t[li], mass=None if mass is None else mass[li],
+                                  places=None if places is None else places[li])
         if g.spec.paged and isinstance(g.layer_spec, LatentLayerSpec):
             return CacheLayerView(gi, self.layout.paged_groups.index(gi), self.page_size, g.spec.window,
                                   None, None, None, writes, latent_pages=t[li])
@@ -114,6 +130,8 @@ class CacheStorage:
         if pages and isinstance(t, tuple):
             for part in t:
                 part[:, torch.tensor(pages, dtype=torch.long, device=part.device)] = value
+        elif pages and getattr(self.layout.groups[gi].layer_spec, "bits", None) == 4:
+            t[:, torch.tensor(pages, dtype=torch.long, device=t.device)] = 255  # parameters that are not numbers
         elif pages and isinstance(self.layout.groups[gi].layer_spec, LatentLayerSpec):
             t[:, torch.tensor(pages, dtype=torch.long, device=t.device)] = value
         elif pages:
@@ -121,4 +139,5 @@ class CacheStorage:
 
     def nbytes(self) -> int:
         flat = [x for t in self.tensors for x in (t if isinstance(t, tuple) else (t,))]
+        flat += [x for pair in self.sums.values() for x in pair]
         return sum(t.numel() * t.element_size() for t in flat)

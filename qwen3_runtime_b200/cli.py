@@ -39,6 +39,10 @@ def _generate(argv: list[str]) -> int:
     parser.add_argument("--seed", type=int, default=None, help="sampling seed")
     parser.add_argument("--block-size", type=int, default=16)
     parser.add_argument("--num-kv-blocks", type=int, default=None)
+    parser.add_argument("--kv-bits", type=int, default=None, choices=[4],
+                        help="hold keys and values in 4 bits. Default: in the compute dtype.")
+    parser.add_argument("--token-budget", type=int, default=None,
+                        help="cached tokens that a request keeps (needs --kv-bits 4): its first, its last and the most attended")
     parser.add_argument("--max-num-seqs", type=int, default=1)
     parser.add_argument("--max-num-batched-tokens", type=int, default=2048)
     args = parser.parse_args(argv)
@@ -50,7 +54,8 @@ def _generate(argv: list[str]) -> int:
     engine = build_engine(args.model, max_num_seqs=args.max_num_seqs,
                           max_num_batched_tokens=args.max_num_batched_tokens, block_size=args.block_size,
                           dtype=args.dtype, num_kv_blocks=args.num_kv_blocks, cuda_graph=args.cuda_graph,
-                          pin_path=args.pin_path, run_ahead=args.run_ahead)
+                          pin_path=args.pin_path, run_ahead=args.run_ahead, kv_bits=args.kv_bits,
+                          token_budget=args.token_budget)
     sampling = SamplingParams(temperature=args.temperature, top_p=args.top_p, top_k=args.top_k, min_p=args.min_p,
                               seed=args.seed)
     out = engine.generate(args.prompt_tokens, max_tokens=args.max_tokens, sampling=sampling)

@@ -75,7 +75,7 @@ class BatchBuilder:
         change.  Updates the kept image of the buffer and copies it; False if the step is not
         such a continuation (the caller then packs it in full)."""
         last = self._last_decode
-        if (last is None or last["device_buffer"] is not device_buffer or len(entries) != len(last["caches"])
+        if (last is None or self.cache.budget is not None or last["device_buffer"] is not device_buffer or len(entries) != len(last["caches"])
                 or last["key"] != (pad_to, table_width, scratch_page, scratch_slot)):
             return False
         for e, c in zip(entries, last["caches"]):
@@ -186,8 +186,10 @@ class BatchBuilder:
         rows: list[int] = []
         # section offsets inside the int32 buffer (each 4-int aligned => 16-byte aligned)
         off, sections = 0, {}
+        budget = self.cache.budget is not None
         for name, size in (("ids", T), ("pos", T), ("seq", T), ("cu", B + 1), ("kv", B), ("kvmax", 1), ("slot", B),
-                           ("rows", T), ("single", B), *[(f"bt{g}", B * width) for g in range(n_paged)]):
+                           ("rows", T), ("single", B), *([("place", T)] if budget else []),
+                           *[(f"bt{g}", B * width) for g in range(n_paged)]):
             sections[name] = (off, size)
             off += _round_up(size, 4)
         host, dev = self._buffers(off)
@@ -208,7 +210,8 @@ class BatchBuilder:
         lens_np = np.asarray(lens, dtype=np.int32)
         cu[0] = 0
         np.cumsum(lens_np, out=cu[1:B_real + 1])
-        kv[:B_real] = starts + lens_np
+        evicted = np.fromiter((e.cache.num_evicted for e in entries), dtype=np.int32, count=B_real)
+        kv[:B_real] = starts - evicted + lens_np
         slot[:B_real] = np.fromiter((e.cache.slot for e in entries), dtype=np.int32, count=B_real)
         if T_real == B_real:  # every entry brings one token
             pos[:T_real] = starts
@@ -216,6 +219,9 @@ class BatchBuilder:
         else:
             seq[:T_real] = np.repeat(np.arange(B_real, dtype=np.int32), lens_np)
             pos[:T_real] = np.arange(T_real, dtype=np.int32) - np.repeat(cu[:B_real] - starts, lens_np)
+        if budget:
+            sec("place")[:T_real] = pos[:T_real] - np.repeat(evicted, lens_np)
+            sec("place")[T_real:] = 0
         for e, first in zip(entries, cu[:B_real].tolist()):
             if e.want:
                 rows.extend(first + w for w in e.want)
@@ -271,6 +277,6 @@ class BatchBuilder:
             logit_rows=dsec("rows", R), num_logit_rows=R,
             max_query_len=max(lens, default=1), max_kv_len=int(kv[:B].max()),
             decode_only=all(n == 1 for n in lens),
-            single_seqs=dsec("single", len(singles)), num_single=len(singles),
+            single_seqs=dsec("single", len(singles)), num_single=len(singles), places=dsec("place") if budget else None,
             host_cu_seqlens=[int(x) for x in cu], host_kv_lens=[int(x) for x in kv[:B]],
         )

@@ -10,9 +10,9 @@ from pathlib import Path
 
 import torch
 
-from ..cache.manager import CacheManager
+from ..cache.manager import CacheManager, TokenBudget
 from ..cache.storage import CacheStorage
-from ..config.engine_config import EngineConfig, canonical_dtype
+from ..config.engine_config import EngineConfig, canonical_cache, canonical_dtype
 from ..config.registry import architecture_for_config, load_config, read_config_json
 from ..parts.base import BuildContext
 from ..parts.model import DecoderModel
@@ -30,12 +30,22 @@ def default_ops(groups=None):
     return CudaOps(groups)
 
 
-def build_model(config, source, *, dtype: str = "bfloat16", device="cuda", ops=None) -> DecoderModel:
-    """A loaded :class:`DecoderModel` for a typed config and a tensor source."""
+def build_model(config, source, *, dtype: str = "bfloat16", device="cuda", ops=None, kv_bits: int | None = None,
+                token_budget: TokenBudget | None = None) -> DecoderModel:
+    """A loaded :class:`DecoderModel` for a typed config and a tensor source.  ``kv_bits`` 4: keys and values are held in 4 bits;
+    ``token_budget``: requests are cut to that many cached tokens.  A model with a part that cannot do so is refused."""
+    kv_bits, token_budget = canonical_cache(kv_bits, token_budget)
     arch = architecture_for_config(config)
     ops = ops if ops is not None else default_ops()
-    ctx = BuildContext(dtype=_TORCH_DTYPE[canonical_dtype(dtype)], device=torch.device(device), ops=ops)
+    ctx = BuildContext(dtype=_TORCH_DTYPE[canonical_dtype(dtype)], device=torch.device(device), ops=ops, kv_bits=kv_bits,
+                       kv_budget=token_budget)
     model = DecoderModel(arch.build_spec(config), ctx)
+    if kv_bits is not None:
+        for group in model.cache_layout().groups:
+            if getattr(group.layer_spec, "bits", None) != kv_bits and (group.spec.paged or token_budget is not None):
+                raise ValueError(f"{arch.name}: a layer's cache ({group.layer_spec}) cannot be held in {kv_bits} bits"
+                                 + (" and cut to a budget" if token_budget is not None else "")
+                                 + "; the paged_attention mixer's can")
     if hasattr(ops, "prepare"):
         ops.prepare(model.kernel_groups())
     load_into(model, source)
@@ -43,7 +53,7 @@ def build_model(config, source, *, dtype: str = "bfloat16", device="cuda", ops=N
 
 
 def load_model(model_dir: str | Path, *, dtype: str = "bfloat16", device="cuda", ops=None,
-               pin_path: str | Path | None = None):
+               pin_path: str | Path | None = None, kv_bits: int | None = None, token_budget: TokenBudget | None = None):
     """``(model, typed config, raw config.json)`` from a folder with config.json and safetensors.
     ``pin_path``: a config.json that the folder's model has to match (checked before any weight
     is read)."""
@@ -51,7 +61,7 @@ def load_model(model_dir: str | Path, *, dtype: str = "bfloat16", device="cuda",
     source = SafetensorsDir(model_dir)
     if hasattr(config, "with_tensor_shapes"):  # sizes that config.json leaves to the stored tensors
         config = config.with_tensor_shapes(source.shape)
-    model = build_model(config, source, dtype=dtype, device=device, ops=ops)
+    model = build_model(config, source, dtype=dtype, device=device, ops=ops, kv_bits=kv_bits, token_budget=token_budget)
     return model, config, read_config_json(model_dir)
 
 
@@ -94,7 +104,7 @@ def build_runtime(model: DecoderModel, *, max_positions: int | None = None, bloc
         counts = layout.pages_for_budget(kv_budget, block_size, dtype_bytes, max_num_seqs=max_num_seqs,
                                          max_step_tokens=max_num_batched_tokens)
         num_kv_blocks = [max(32, n) for n in counts]
-    cache = CacheManager(layout.group_specs, block_size, num_kv_blocks, max_num_seqs)
+    cache = CacheManager(layout.group_specs, block_size, num_kv_blocks, max_num_seqs, budget=ctx.kv_budget)
     storage = CacheStorage(layout, block_size, num_kv_blocks, max_num_seqs, ctx.dtype, ctx.device)
     runner = ModelRunner(model, cache, storage, max_positions=max_positions, cuda_graph=cuda_graph)
     return Runtime(model, cache, storage, runner, max_positions)
@@ -113,15 +123,23 @@ def build_engine(model_dir: str | Path | None = None, *, max_num_seqs: int = 8, 
                  kv_budget: int | None = None, cuda_graph: bool | None = None, eos_token_id: int | None = None,
                  device="cuda", ops=None, model: DecoderModel | None = None, config=None,
                  max_positions: int | None = None, pin_path: str | Path | None = None,
-                 run_ahead: bool = True, kv_memory_fraction: float = 0.85) -> Engine:
+                 run_ahead: bool = True, kv_memory_fraction: float = 0.85, kv_bits: int | None = None,
+                 token_budget: TokenBudget | int | None = None) -> Engine:
     """An :class:`Engine` for a model folder (or an already built ``model``; its ``config`` is
-    kept on the engine for the caller's reference only)."""
+    kept on the engine for the caller's reference only).  ``kv_bits`` and ``token_budget`` (a number: the tokens to keep): as for
+    :func:`build_model`; a model that is built already has its own."""
     dtype = canonical_dtype(dtype)
+    kv_bits, token_budget = canonical_cache(kv_bits, token_budget)
+    if model is not None:
+        if (kv_bits, token_budget) not in ((None, None), (model.ctx.kv_bits, model.ctx.kv_budget)):
+            raise ValueError("the model was built for another cache: give kv_bits and token_budget to build_model")
+        kv_bits, token_budget = model.ctx.kv_bits, model.ctx.kv_budget
     raw: dict = {}
     if model is None:
         if model_dir is None:
             raise ValueError("give a model folder or a built model")
-        model, config, raw = load_model(model_dir, dtype=dtype, device=device, ops=ops, pin_path=pin_path)
+        model, config, raw = load_model(model_dir, dtype=dtype, device=device, ops=ops, pin_path=pin_path, kv_bits=kv_bits,
+                                        token_budget=token_budget)
     if cuda_graph is None:
         cuda_graph = model.ctx.device.type == "cuda"
     if eos_token_id is None:
@@ -132,7 +150,7 @@ def build_engine(model_dir: str | Path | None = None, *, max_num_seqs: int = 8, 
     cfg = EngineConfig(block_size=block_size, num_kv_blocks=min(rt.cache.num_pages) if rt.cache.num_pages else None,
                        max_num_seqs=max_num_seqs, max_num_batched_tokens=max_num_batched_tokens,
                        eos_token_id=eos_token_id, cuda_graph=bool(cuda_graph), dtype=dtype, run_ahead=bool(run_ahead),
-                       kv_memory_fraction=kv_memory_fraction)
+                       kv_memory_fraction=kv_memory_fraction, kv_bits=kv_bits, token_budget=token_budget)
     engine = Engine(cfg, rt.runner, rt.cache, Sampler(model.ops, model.ctx.device))
     engine.runtime = rt
     engine.model_config = config

@@ -60,7 +60,7 @@ class DecodeGraphs:
         need = max((len(t) for e in entries for t in e.cache.tables), default=1)
         width = max(8, 1 << (max(need, 1) - 1).bit_length())
         # what the parts' kernels choose from the lengths of the moment is part of the key
-        choices = self.runner.model.step_choices([e.cache.num_computed + 1 for e in entries])
+        choices = self.runner.model.step_choices([e.cache.held + 1 for e in entries])
         key = (bucket, width, tuple(sorted(choices.items())))
         cap = self.captured.get(key)
         if cap is None:
@@ -92,7 +92,7 @@ class DecodeGraphs:
         bucket, width = key[:2]
         r = self.runner
         n_paged = len(r.cache.paged_groups)
-        meta = torch.zeros(8 * bucket + 64 + n_paged * bucket * width, dtype=torch.int32, device=r.device)
+        meta = torch.zeros(9 * bucket + 68 + n_paged * bucket * width, dtype=torch.int32, device=r.device)
         cap = _Captured(torch.cuda.CUDAGraph(), meta, None)
         step = self._fill(cap, [], bucket, width)
         step.captured_width = width

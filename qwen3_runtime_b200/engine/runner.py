@@ -66,5 +66,35 @@ class ModelRunner:
             logits = logits if logits.numel() else None
         for e in entries:
             self.cache.commit(e.cache, len(e.tokens))
+        if self.cache.budget is not None:
+            self.cut([e.cache for e in entries if self.cache.over_budget(e.cache)])
         self.num_steps += 1
         return logits
+
+    def cut(self, requests) -> None:
+        """Cut requests that hold more tokens than the budget allows: all layers at once, each kv head by its own sums.  What the
+        next step reads lies in front; the pages behind it go back to the pool (later work on the stream comes after the moves)."""
+        if not requests:
+            return
+        budget, page_size = self.cache.budget, self.cache.page_size
+        width = max(len(t) for rc in requests for t in rc.tables)
+        count, n_paged = len(requests), len(self.cache.paged_groups)
+        host = torch.zeros((n_paged * count * width + count,), dtype=torch.int32, pin_memory=self.builder.pin)
+        image = host.numpy()
+        tables = image[: n_paged * count * width].reshape(n_paged, count, width)
+        for g in range(n_paged):
+            tables[g] = self.storage.scratch_page[g]
+            for b, rc in enumerate(requests):
+                tables[g, b, : len(rc.tables[g])] = rc.table_array(g)
+        image[n_paged * count * width:] = [rc.held for rc in requests]
+        dev = host.to(self.device, non_blocking=True)
+        lens = dev[n_paged * count * width:]
+        for g, gi in enumerate(self.cache.paged_groups):
+            spec = self.storage.layout.groups[gi].layer_spec
+            mass, places = self.storage.sums[gi]
+            self.model.ops.evict_4bit(
+                pages=self.storage.tensors[gi], mass=mass, places=places, kv_lens=lens, max_kv_len=max(rc.held for rc in requests),
+                block_table=dev[g * count * width:(g + 1) * count * width].view(count, width), keep=budget.keep, first=budget.first,
+                recent=budget.recent, num_kv_heads=spec.num_kv_heads, head_dim=spec.head_dim, page_size=page_size)
+        for rc in requests:
+            self.cache.cut(rc)

@@ -29,7 +29,8 @@ class LLM:
                  architecture: str | None = None, max_num_seqs: int = 4, max_num_batched_tokens: int = 256,
                  seed: int = 0, dtype: str = "bfloat16", **factory_kwargs):
         """``model=None``: random weights (``seed``) for ``config``, or for the tiny configuration
-        that the registered ``architecture`` (default: the first registered) offers."""
+        that the registered ``architecture`` (default: the first registered) offers.  ``kv_bits=4`` holds keys and values in 4
+        bits, ``token_budget`` (a number or a ``TokenBudget``) cuts requests to that many cached tokens."""
         self.tokenizer = tokenizer
         common = dict(max_num_seqs=max_num_seqs, max_num_batched_tokens=max_num_batched_tokens, dtype=dtype)
         if model is not None:
@@ -43,7 +44,8 @@ class LLM:
             config = arch.tiny_config()
         weights = DictSource(random_state(config, seed, std=0.2))
         built = build_model(config, weights, dtype=dtype, device=factory_kwargs.get("device", "cuda"),
-                            ops=factory_kwargs.get("ops"))
+                            ops=factory_kwargs.get("ops"), kv_bits=factory_kwargs.pop("kv_bits", None),
+                            token_budget=factory_kwargs.pop("token_budget", None))
         factory_kwargs.setdefault("block_size", 4)
         factory_kwargs.setdefault("num_kv_blocks", 64)
         self.engine = build_engine(model=built, config=config, **common, **factory_kwargs)

@@ -2241,6 +2241,12 @@ class CudaOps:
         # the wide kernels number a token by its place: kv_lens and cu_seqlens say it, or for the general kernel `positions`
         return self.paged_attention(q, q_stride, k_pages=k, v_pages=v, block_table=table, step=step, **wide)
 
+    @staticmethod
+    def decode_4bit_ok(q, num_heads, num_kv_heads, head_dim) -> bool:
+        """Whether single tokens with these queries read the 4-bit numbers as they are (and can have their log sums)."""
+        return (q.dtype == torch.bfloat16 and head_dim in (64, 128, 256) and num_heads // num_kv_heads <= 16 and q.stride(0) % 8 == 0
+                and q.data_ptr() % 16 == 0)
+
     DECODE_4BIT_BLOCKS_PER_SM = {64: 5, 128: 4, 256: 2}
 
     def decode_slices_4bit(self, kv_lens, num_kv_heads, head_dim, window) -> int:

@@ -8,6 +8,7 @@ Parity: qwen3_runtime/models/qwen3.py:62-127 and attention/pytorch.py:18-47.
 
 from __future__ import annotations
 
+import copy
 import math
 
 import torch
@@ -29,9 +30,13 @@ class PagedAttention(Part):
         self.qk_norm_eps = spec.get("qk_norm_eps")
         self.window = spec.get("window") or None
         self.scale = float(spec.get("scale") or 1.0 / math.sqrt(self.head_dim))
-        self._slices_choice = ("decode_slices", self.num_kv_heads, self.head_dim, self.window)
+        self.four_bit = ctx.kv_bits == 4
+        self.budget = ctx.kv_budget
+        self._slices_choice = ("decode_slices_4bit" if self.four_bit else "decode_slices", self.num_kv_heads, self.head_dim, self.window)
         if self.num_heads % self.num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
+        if self.budget is not None and self.window:
+            raise ValueError("a token budget cuts layers that keep every key: this one has a window of its own")
         if self.head_dim % 16 or self.head_dim > 256:
             raise ValueError(
                 f"head_dim={self.head_dim} is not supported: the attention kernels take multiples of 16 up to 256")
@@ -79,6 +84,8 @@ class PagedAttention(Part):
 
     def kernel_groups(self):
         groups = ["rope_kv", "attention_generic", *product_groups(self.ctx), *self.position.kernel_groups()]
+        if self.four_bit:
+            groups += ["cache_4bit", "attention_4bit"]
         if self.ctx.dtype == torch.bfloat16:
             # the specialised attention kernels that this head size can reach (ops.paged_attention)
             group = self.num_heads // self.num_kv_heads
@@ -92,13 +99,15 @@ class PagedAttention(Part):
 
     def step_choosers(self):
         """Into how many slices the split-KV decode kernel cuts the longest sequence's keys."""
-        model = getattr(self.ops, "decode_slices_for", None)
+        model = getattr(self.ops, "decode_slices_4bit" if self.four_bit else "decode_slices_for", None)
         if model is None or self.ctx.dtype != torch.bfloat16 or self.head_dim not in (64, 128, 256):
             return {}
         nkv, D, window = self.num_kv_heads, self.head_dim, self.window
         return {self._slices_choice: lambda kv_lens: model(kv_lens, nkv, D, window)}
 
     def cache_spec(self):
+        if self.four_bit:
+            return KVLayerSpec(self.num_kv_heads, self.head_dim, self.window, bits=4, sums=self.budget is not None)
         return KVLayerSpec(self.num_kv_heads, self.head_dim, self.window)
 
     def position_limit(self):
@@ -118,6 +127,9 @@ class PagedAttention(Part):
         ctx_out = torch.empty((T, self.q_size), dtype=h.dtype, device=h.device)
         eps = self.qk_norm_eps if self.qk_norm_eps is not None else 0.0
         slices = step.choices.get(self._slices_choice)
+        if self.four_bit:
+            self._attend_4bit(qkv, ctx_out, step, cache, block_table, eps, cos, sin, slices)
+            return self._project_out(ctx_out)
         fusable = getattr(ops, "decode_new_token_ok", None)
         if (fusable is not None and step.decode_only and cache.writes
                 and fusable(qkv, num_heads=self.num_heads, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,
@@ -147,6 +159,31 @@ class PagedAttention(Part):
             token_seq=step.token_seq, positions=step.positions, out=ctx_out, page_size=cache.page_size,
             scale=self.scale, window=self.window, step=step, **({"decode_slices": slices} if slices else {}))
         return self._project_out(ctx_out)
+
+    def _attend_4bit(self, qkv, out, step: StepContext, cache, block_table, eps, cos, sin, slices) -> None:
+        """Norm, rotation, cache write and attention over a cache in 4 bits; under a token budget the weights that the step's
+        tokens give are added to their keys' sums."""
+        ops = self.ops
+        sizes = dict(num_heads=self.num_heads, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim, pages=cache.packed_pages,
+                     block_table=block_table, page_size=cache.page_size)
+        ops.qk_norm_rope_store_4bit(
+            qkv, q_weight=self.q_norm_weight, k_weight=self.k_norm_weight, eps=eps, cos=cos, sin=sin, positions=step.positions,
+            token_seq=step.token_seq, write_kv=cache.writes, pairing=self.pairing, slots=step.places,
+            mass=cache.mass if cache.writes else None, places=cache.places if cache.writes else None, **sizes)
+        if step.places is not None:  # from here on tokens are counted by their places
+            held = step.extras.get("by_place")
+            if held is None:
+                held = step.extras["by_place"] = copy.copy(step)
+                held.positions = step.places
+            step = held
+        lse = None
+        if cache.mass is not None and step.decode_only and ops.decode_4bit_ok(qkv, self.num_heads, self.num_kv_heads, self.head_dim):
+            lse = torch.empty((out.shape[0], self.num_heads), dtype=torch.float32, device=out.device)
+        ops.paged_attention_4bit(qkv, qkv.stride(0), out=out, scale=self.scale, window=self.window, step=step, decode_slices=slices,
+                                 lse=lse, **sizes)
+        if cache.mass is not None:
+            ops.attention_mass_4bit(qkv, qkv.stride(0), mass=cache.mass, scale=self.scale, step=step, observe=self.budget.observe,
+                                    lse=lse, **sizes)
 
     def _project_out(self, ctx_out: torch.Tensor) -> torch.Tensor:
         if self.o_bias_vec is not None:

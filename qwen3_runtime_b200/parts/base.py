@@ -42,6 +42,8 @@ class BuildContext:
     device: torch.device
     ops: Any  # the kernel table (qwen3_runtime_b200.ops.cuda.CudaOps in production)
     shared: dict = field(default_factory=dict)  # tables shared between parts (e.g. rotary cos/sin)
+    kv_bits: int | None = None  # 4: keys and values are held in 4 bits (parts that can; the factory refuses the others)
+    kv_budget: Any = None  # a TokenBudget: each cached token's attention weights are summed beside it
 
 
 @dataclass
@@ -54,7 +56,7 @@ class StepContext:
     positions: torch.Tensor  # [T] absolute position of each token in its sequence
     token_seq: torch.Tensor  # [T] row of the batch (sequence) each token belongs to
     cu_seqlens: torch.Tensor  # [B + 1] first token of each sequence in the packed batch
-    kv_lens: torch.Tensor  # [B] tokens in the cache after this step
+    kv_lens: torch.Tensor  # [B] tokens in the cache after this step (under a token budget: those that are still held)
     state_slots: torch.Tensor  # [B] fixed-size state slot of each sequence
     block_tables: list[torch.Tensor]  # per paged cache group: [B, max_pages]
     logit_rows: torch.Tensor  # [R] packed rows whose logits are wanted
@@ -65,6 +67,8 @@ class StepContext:
     kv_longest: torch.Tensor | None = None  # [1] the largest of kv_lens, on the device
     single_seqs: torch.Tensor | None = None  # [num_single] sequences that bring exactly one token
     num_single: int = 0
+    # Under a token budget: [T] each token's place among the tokens that its sequence still holds (its position otherwise)
+    places: torch.Tensor | None = None
     # host copies (lists) for parts that need them without a device read
     host_cu_seqlens: list[int] = field(default_factory=list)
     host_kv_lens: list[int] = field(default_factory=list)

@@ -194,3 +194,18 @@ def evict(mass, place, keep, first, recent):
     movers = [i for i in stays if i >= keep]
     kept = set(stays)
     return [i if i in kept else movers.pop(0) for i in range(keep)]
+
+
+def values_of(pages, D, page):
+    """What whole records ``[.., bytes]`` stand for: keys and values ``[.., page, D]`` in float32, by tensors."""
+    G, half, par = groups(D), D // 2, 4 * groups(D)
+    out = []
+    for which in range(2):
+        code = pages[..., which * page * half:(which + 1) * page * half].unflatten(-1, (page, half))
+        n = torch.stack([code & 15, code >> 4], -1).flatten(-2)  # [.., page, D] in the order of words
+        n = n.unflatten(-1, (-1, G, 8)).transpose(-3, -2).flatten(-3).float()
+        base = 2 * page * half + which * page * par
+        sz = pages[..., base:base + page * par].contiguous().view(torch.bfloat16).float().unflatten(-1, (page, G, 2))
+        s, z = (x.repeat_interleave(D // G, -1) for x in (sz[..., 0], sz[..., 1]))
+        out.append(z + n * s)
+    return out
