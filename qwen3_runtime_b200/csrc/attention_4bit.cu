@@ -79,17 +79,24 @@ template <int D> struct Head {
 // The queries' side of the scores: B fragments (n = lane / 4: the query, k: the channels that word j's pairs stand for; b[j][0..3]: of word j,
 // channels (0, 4), (1, 5), (2, 6), (3, 7) of its eight), times 2^S, the channels that meet 2^-129 a 16th of it.  `undo`: what the sums
 // are to be multiplied by, for columns 2 (lane % 4) and + 1; `sum`: the channels' sums per group, both times the scores' scale.
-template <int D> __device__ __forceinline__ void load_query_tiny(uint32_t (&b)[Head<D>::WORDS][4], float (&undo)[2], float (&sum)[Head<D>::G][2],
-                                                                 const bf16* row, float scale_log2, int lane) {
+template <int D> __device__ __forceinline__ void fetch_query(uint4 (&raw)[Head<D>::WORDS], const bf16* row, int lane) {
+#pragma unroll
+  for (int j = 0; j < Head<D>::WORDS; ++j) {
+    raw[j] = make_uint4(0, 0, 0, 0);
+    if (row) raw[j] = *reinterpret_cast<const uint4*>(row + 64 * Head<D>::group(j) + 8 * Head<D>::index(j, lane & 3));
+  }
+}
+template <int D> __device__ __forceinline__ void take_query(uint32_t (&b)[Head<D>::WORDS][4], float (&undo)[2], float (&sum)[Head<D>::G][2],
+                                                            const uint4 (&raw)[Head<D>::WORDS], float scale_log2, int lane) {
   using H = Head<D>;
   float v[H::WORDS][8], top = 0.f, part[H::G];
 #pragma unroll
   for (int g = 0; g < H::G; ++g) part[g] = 0.f;
 #pragma unroll
   for (int j = 0; j < H::WORDS; ++j) {
+    const uint32_t word[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-    if (row) load8(row + 64 * H::group(j) + 8 * H::index(j, lane & 3), v[j]);
+    for (int e = 0; e < 4; ++e) v[j][2 * e] = __uint_as_float(word[e] << 16), v[j][2 * e + 1] = __uint_as_float(word[e] & 0xFFFF0000u);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       top = fmaxf(top, fabsf(v[j][e]));
@@ -118,6 +125,12 @@ template <int D> __device__ __forceinline__ void load_query_tiny(uint32_t (&b)[H
 #pragma unroll
     for (int g = 0; g < H::G; ++g) sum[g][c] = __shfl_sync(0xffffffffu, part[g], from) * scale_log2;
   }
+}
+template <int D> __device__ __forceinline__ void load_query_tiny(uint32_t (&b)[Head<D>::WORDS][4], float (&undo)[2], float (&sum)[Head<D>::G][2],
+                                                                 const bf16* row, float scale_log2, int lane) {
+  uint4 raw[Head<D>::WORDS];
+  fetch_query<D>(raw, row, lane);
+  take_query<D>(b, undo, sum, raw, scale_log2, lane);
 }
 
 // ---- decode attention -------------------------------------------------------------------------------------------------------------
@@ -201,8 +214,9 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_4bit_k
   }
   pdl_wait();
   const int seq = a.seq_list ? a.seq_list[slot] : slot;
+  const int tok = a.cu_seqlens[seq];
   const Slice sl(a, seq, split);
-  const int tok = a.cu_seqlens[seq], begin = sl.begin, end = sl.end;
+  const int begin = sl.begin, end = sl.end;
   const long out_row = (long)tok * a.nq + kvh * R;
   if (!CLUSTER && begin >= end) {
     pdl_launch_dependents();
@@ -264,16 +278,18 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_4bit_k
     if (at_row >= a.ps) at_row -= a.ps, ++at_page;
     page = look_up();
   };
+  // the queries' rows are on their way together with the first pages
+  uint4 raw[NT][H::WORDS];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    fetch_query<D>(raw[n], 8 * n + r < R ? a.q + (long)tok * a.q_stride + (long)(kvh * R + 8 * n + r) * D : nullptr, lane);
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) load_step(i);
 
   uint32_t q[NT][H::WORDS][4];
   float qsum[NT][H::G][2], undo[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int h = 8 * n + r;
-    load_query_tiny<D>(q[n], undo[n], qsum[n], h < R ? a.q + (long)tok * a.q_stride + (long)(kvh * R + h) * D : nullptr, a.scale_log2, lane);
-  }
+  for (int n = 0; n < NT; ++n) take_query<D>(q[n], undo[n], qsum[n], raw[n], a.scale_log2, lane);
   // o: sums of w n (times 2^-133, odd j 2^-129); oz: of -8 w (2^-133); oc: of p (z + 8 s), this lane's share; all of 16 p in place of p.
   // lift = 2^T is set so that the largest scale seen lies in 2^100 .. 2^115, beyond which it is set anew.
   float o[NT][H::G][4][4], oz[NT][H::G][4], oc[NT][H::G][2], m[NT][2], sum[NT][2];
@@ -917,7 +933,7 @@ template <int D> struct RowTile {  // 8 rows as operands, as each lane reads the
 
 template <int D> __global__ void __launch_bounds__(32 * COLUMN_WARPS) mass_columns_kernel(Mass a) {
   using H = Head<D>;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   RowTile<D>* tiles = reinterpret_cast<RowTile<D>*>(smem);
   pdl_wait();
   pdl_launch_dependents();
@@ -1178,6 +1194,210 @@ template <int D, int NT> int launch_mass(const Mass& a, bool want_rows, int most
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
 }
 
+// ---- attention in general -----------------------------------------------------------------------------------------------------------------
+// float32, and bfloat16 tokens whose head size or group the tiles above do not take: a block of 256 threads takes a (token, kv head, up to 8
+// of its query heads); 64 keys at a time come to shared memory as they are stored, four threads make a key's scores, a warp a head's
+// weights, a thread a channel's results.  Sums are float32 on the FMA pipes, in an order that depends on the keys' places alone: tiles
+// begin at multiples of 64, slices of 1024 keys have a softmax of their own and are joined in order, by the same block or, where the
+// launch leaves SMs idle, by a second kernel from what one block a slice has left -- the same bits, however a sequence is cut into steps
+// and batched with others.
+constexpr int GEN_THREADS = 256;
+constexpr int GEN_TILE = 64;
+constexpr int GEN_SLICE = 1024;
+constexpr int GEN_HEADS = 8;
+
+struct General {
+  const unsigned char* pages;
+  int num_pages;
+  const int *block_table, *token_seq, *places;
+  int max_pages, num_seqs, nq, nkv, D, G, ps, window, slices;
+  long q_stride;
+  float scale_log2;
+  float *mid_o, *mid_ml;  // slices > 0: [tokens][nq][slices][D] and [tokens][nq][slices][2]
+};
+
+// (m, l, o) <- its join with another's; o and b are unnormalised
+__device__ __forceinline__ void join_slices(float& m, float& l, float& o, float bm, float bl, float bo) {
+  const float top = fmaxf(m, bm), fa = exp2f(m - top), fb = exp2f(bm - top);
+  m = top;
+  l = l * fa + bl * fb;
+  o = o * fa + bo * fb;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(GEN_THREADS) general_4bit_kernel(General a, const T* __restrict__ q, T* __restrict__ out) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int R = a.nq / a.nkv, chunks = (R + GEN_HEADS - 1) / GEN_HEADS;
+  const int t = blockIdx.x, kvh = blockIdx.y / chunks, h0 = kvh * R + (blockIdx.y % chunks) * GEN_HEADS;
+  const int heads = min(GEN_HEADS, kvh * R + R - h0);
+  const int D = a.D, G = a.G, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Q4Page L(D, G, a.ps);
+  float* q_s = reinterpret_cast<float*>(smem);                   // [8][D]
+  float* p_s = q_s + GEN_HEADS * D;                              // [8][64]
+  float* f_s = p_s + GEN_HEADS * GEN_TILE;                       // [8]: what the results so far shrink by; then the slice's maximum and sum
+  float* v_s = f_s + 32;                                         // [groups of threads][8][D] at the end of a slice, else the tile's bytes
+  unsigned char* k_s = reinterpret_cast<unsigned char*>(v_s);    // [64][half + par] of keys, then of values
+  const int pitch = L.half + L.par, words = pitch / 4;
+  const int seq = a.token_seq[t], place = a.places[t];
+  const bool there = seq >= 0 && seq < a.num_seqs && place >= 0 && place / a.ps < a.max_pages;
+  const int last = there ? place : -1, lo = a.window > 0 ? max(0, last - a.window + 1) : 0;
+  const int* bt = a.block_table + (long)(there ? seq : 0) * a.max_pages;
+  for (int i = tid; i < heads * D; i += GEN_THREADS) q_s[i] = to_f32(q[t * a.q_stride + (long)h0 * D + i]) * a.scale_log2;
+  // a thread owns channel c of the keys g, g + parts, g + 2 parts ... of each tile
+  const int parts = GEN_THREADS / D, c = tid % D, part = tid / D;
+  const bool owner = part < parts;
+  const int c_group = c / (D / G), c_in = c % (D / G), c_byte = 4 * ((c_in / 8) * G + c_group) + (c_in % 8) / 2, c_shift = 4 * (c_in % 2);
+  float M[GEN_HEADS], S[GEN_HEADS], O[GEN_HEADS];
+#pragma unroll
+  for (int h = 0; h < GEN_HEADS; ++h) M[h] = MINUS_BIG, S[h] = 0.f, O[h] = 0.f;
+  const int slice0 = a.slices > 0 ? blockIdx.z : lo / GEN_SLICE, slice1 = a.slices > 0 ? blockIdx.z : last / GEN_SLICE;
+  for (int slice = slice0; slice <= slice1 && last >= 0; ++slice) {
+    const int begin = max(lo, slice * GEN_SLICE) / GEN_TILE * GEN_TILE, end = min(last + 1, (slice + 1) * GEN_SLICE);
+    float o[GEN_HEADS];
+#pragma unroll
+    for (int h = 0; h < GEN_HEADS; ++h) o[h] = 0.f;
+    float m = MINUS_BIG, l = 0.f;  // warp h: of head h, the same in every lane
+    for (int base = begin; base < end; base += GEN_TILE) {
+      __syncthreads();
+      for (int i = tid; i < 2 * GEN_TILE * words; i += GEN_THREADS) {
+        const int row = i / words, w = i - row * words, is_v = row >= GEN_TILE, key = base + row - is_v * GEN_TILE;
+        uint32_t x = 0;
+        if (key >= lo && key < end) {
+          const int pi = key / a.ps, page = bt[pi], pr = key - pi * a.ps;
+          if ((uint32_t)page < (uint32_t)a.num_pages) {
+            const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
+            const bool par = 4 * w >= L.half;
+            x = *reinterpret_cast<const uint32_t*>(rec + (par ? (is_v ? L.vpar : L.kpar) + (long)pr * L.par + 4 * w - L.half
+                                                               : (is_v ? L.values : 0) + (long)pr * L.half + 4 * w));
+          }
+        }
+        reinterpret_cast<uint32_t*>(k_s)[i] = x;
+      }
+      __syncthreads();
+      {  // four threads a key, each every fourth word; 8 channels of a word in order, the four threads' sums in pairs
+        const int key = tid >> 2, sub = tid & 3;
+        const uint32_t* row = reinterpret_cast<const uint32_t*>(k_s + key * pitch);
+        const uint32_t* par = reinterpret_cast<const uint32_t*>(k_s + key * pitch + L.half);
+        float x[GEN_HEADS];
+#pragma unroll
+        for (int h = 0; h < GEN_HEADS; ++h) x[h] = 0.f;
+        for (int w = sub; w < D / 8; w += 4) {
+          const uint32_t code = row[w];
+          const int g = w % G, first = g * (D / G) + 8 * (w / G);
+          const float s = q4_s(par[g]), z = q4_z(par[g]);
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = z + (float)((code >> (4 * e)) & 15u) * s;
+#pragma unroll
+          for (int h = 0; h < GEN_HEADS; ++h)
+            if (h < heads) {
+              const float4 qa = *reinterpret_cast<const float4*>(q_s + h * D + first), qb = *reinterpret_cast<const float4*>(q_s + h * D + first + 4);
+              x[h] = fmaf(qa.x, v[0], x[h]), x[h] = fmaf(qa.y, v[1], x[h]), x[h] = fmaf(qa.z, v[2], x[h]), x[h] = fmaf(qa.w, v[3], x[h]);
+              x[h] = fmaf(qb.x, v[4], x[h]), x[h] = fmaf(qb.y, v[5], x[h]), x[h] = fmaf(qb.z, v[6], x[h]), x[h] = fmaf(qb.w, v[7], x[h]);
+            }
+        }
+        const bool seen = base + key >= lo && base + key < end;
+#pragma unroll
+        for (int h = 0; h < GEN_HEADS; ++h) {
+          x[h] += __shfl_xor_sync(0xffffffffu, x[h], 1);
+          x[h] += __shfl_xor_sync(0xffffffffu, x[h], 2);
+          if (sub == (h & 3) && h < heads) p_s[h * GEN_TILE + key] = seen ? x[h] : -INFINITY;
+        }
+      }
+      __syncthreads();
+      if (warp < heads) {
+        const float x0 = p_s[warp * GEN_TILE + lane], x1 = p_s[warp * GEN_TILE + 32 + lane];
+        const float top = fmaxf(m, warp_max(fmaxf(x0, x1))), f = exp2f(m - top);
+        const float p0 = exp2f(x0 - top), p1 = exp2f(x1 - top);
+        p_s[warp * GEN_TILE + lane] = p0, p_s[warp * GEN_TILE + 32 + lane] = p1;
+        l = l * f + warp_sum(p0 + p1);
+        m = top;
+        if (lane == 0) f_s[warp] = f;
+      }
+      __syncthreads();
+      if (owner) {
+#pragma unroll
+        for (int h = 0; h < GEN_HEADS; ++h)
+          if (h < heads) o[h] *= f_s[h];
+        const unsigned char* rows = k_s + GEN_TILE * pitch;
+        for (int key = part; key < GEN_TILE; key += parts) {
+          const unsigned char* row = rows + key * pitch;
+          const uint32_t par = *reinterpret_cast<const uint32_t*>(row + L.half + 4 * c_group);
+          const float v = q4_z(par) + (float)((row[c_byte] >> c_shift) & 15) * q4_s(par);
+#pragma unroll
+          for (int h = 0; h < GEN_HEADS; ++h)
+            if (h < heads) o[h] = fmaf(p_s[h * GEN_TILE + key], v, o[h]);
+        }
+      }
+    }
+    // the threads' shares of a channel, in order; then the slice joins what came before it
+    __syncthreads();
+    if (owner) {
+#pragma unroll
+      for (int h = 0; h < GEN_HEADS; ++h)
+        if (h < heads) v_s[(part * GEN_HEADS + h) * D + c] = o[h];
+    }
+    if (warp < heads && lane == 0) f_s[8 + 2 * warp] = m, f_s[9 + 2 * warp] = l;
+    __syncthreads();
+    if (owner && part == 0) {
+#pragma unroll
+      for (int h = 0; h < GEN_HEADS; ++h)
+        if (h < heads) {
+          float y = v_s[h * D + c];
+          for (int g = 1; g < parts; ++g) y += v_s[(g * GEN_HEADS + h) * D + c];
+          join_slices(M[h], S[h], O[h], f_s[8 + 2 * h], f_s[9 + 2 * h], y);
+        }
+    }
+  }
+  if (owner && part == 0) {
+#pragma unroll
+    for (int h = 0; h < GEN_HEADS; ++h)
+      if (h < heads) {
+        if (a.slices > 0) {
+          const long at = ((long)t * a.nq + h0 + h) * a.slices + blockIdx.z;
+          a.mid_o[at * D + c] = O[h];
+          if (c == 0) a.mid_ml[2 * at] = M[h], a.mid_ml[2 * at + 1] = S[h];
+        } else {
+          out[((long)t * a.nq + h0 + h) * D + c] = from_f32<T>(last >= 0 ? O[h] / S[h] : 0.f);
+        }
+      }
+  }
+}
+
+// One block per (token, head): joins the slices in order, a thread per channel.
+template <typename T> __global__ void general_4bit_merge_kernel(General a, T* __restrict__ out) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const long at = blockIdx.x;
+  const int place = a.places[at / a.nq], lo = a.window > 0 ? max(0, place - a.window + 1) : 0;
+  for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
+    float M = MINUS_BIG, S = 0.f, O = 0.f;
+    for (int s = lo / GEN_SLICE; s <= place / GEN_SLICE && s < a.slices; ++s)
+      join_slices(M, S, O, a.mid_ml[2 * (at * a.slices + s)], a.mid_ml[2 * (at * a.slices + s) + 1], a.mid_o[(at * a.slices + s) * a.D + c]);
+    out[at * a.D + c] = from_f32<T>(place >= 0 ? O / S : 0.f);
+  }
+}
+
+template <typename T> int launch_general(const General& a, const T* q, T* out, int tokens, cudaStream_t stream) {
+  const Q4Page L(a.D, a.G, a.ps);
+  const int R = a.nq / a.nkv, chunks = (R + GEN_HEADS - 1) / GEN_HEADS, parts = GEN_THREADS / a.D;
+  const int tile = 2 * GEN_TILE * (L.half + L.par), shares = parts * GEN_HEADS * a.D * 4;
+  const int smem = (GEN_HEADS * (a.D + GEN_TILE) + 32) * 4 + (tile > shares ? tile : shares);
+  static bool once[Q3_MAX_DEVICES];
+  const int dev = q3_current_device();
+  if (!once[dev]) {
+    if (cudaFuncSetAttribute(general_4bit_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != cudaSuccess) return Q3_ERR_LAUNCH;
+    once[dev] = true;
+  }
+  cudaError_t err = launch_pdl(general_4bit_kernel<T>, dim3(tokens, a.nkv * chunks, a.slices > 0 ? a.slices : 1), dim3(GEN_THREADS), smem, stream,
+                               a, q, out);
+  if (err == cudaSuccess && a.slices > 0)
+    err = launch_pdl(general_4bit_merge_kernel<T>, dim3((unsigned)((long)tokens * a.nq)), dim3(a.D <= 128 ? 128 : 256), 0, stream, a, out);
+  return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
+}
+
 }  // namespace
 
 // `lse` holds the observed rows' log sums (have_lse) or is scratch for them; `part` [tokens][nq][slices] pairs of floats when slices > 1.
@@ -1234,4 +1454,24 @@ Q3_EXPORT int q3_decode_attention_4bit(const void* q, int q_stride, const void* 
   if (D == 128) return R <= 8 ? launch_decode<128, 1>(a, num_seqs, stream) : launch_decode<128, 2>(a, num_seqs, stream);
   if (D == 256) return R <= 8 ? launch_decode<256, 1>(a, num_seqs, stream) : launch_decode<256, 2>(a, num_seqs, stream);
   return Q3_ERR_UNSUPPORTED;
+}
+
+// `slices` 0: a block goes through all of a token's keys; else mid_o [tokens][nq][slices][D] and mid_ml [tokens][nq][slices][2] are given and
+// slices * 1024 covers the longest sequence.
+Q3_EXPORT int q3_general_attention_4bit(int dtype, const void* q, long q_stride, const void* pages, int num_pages, const int* block_table,
+                                        int max_pages, int num_seqs, const int* token_seq, const int* places, void* out, float* mid_o,
+                                        float* mid_ml, int slices, int tokens, int nq, int nkv, int D, int ps, float scale, int window,
+                                        cudaStream_t stream) {
+  if (!q || !pages || !block_table || !token_seq || !places || !out || nq < 1 || nkv < 1 || nq % nkv || !q4_sizes_ok(D, ps) || max_pages < 1 ||
+      slices < 0 || (slices > 0 && (!mid_o || !mid_ml)))
+    return Q3_ERR_ARGUMENT;
+  if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
+  if (tokens < 1) return Q3_OK;
+  if ((long)nkv * ((nq / nkv + GEN_HEADS - 1) / GEN_HEADS) > 65535 || slices > 65535 || (long)tokens * nq > 0x7fffffffL ||
+      (reinterpret_cast<uintptr_t>(pages) & 15))
+    return Q3_ERR_UNSUPPORTED;
+  General a{(const unsigned char*)pages, num_pages, block_table, token_seq, places, max_pages, num_seqs, nq, nkv, D, q4_groups(D), ps, window,
+            slices, q_stride, scale * LOG2_E, mid_o, mid_ml};
+  return dtype == Q3_DTYPE_F32 ? launch_general(a, (const float*)q, (float*)out, tokens, stream)
+                               : launch_general(a, (const bf16*)q, (bf16*)out, tokens, stream);
 }

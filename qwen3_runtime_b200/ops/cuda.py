@@ -248,6 +248,8 @@ _SIGNATURES = {
         "q3_decode_attention_4bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
                                      c_int, c_void_p, c_void_p, c_void_p],
+        "q3_general_attention_4bit": [c_int, c_void_p, c_long, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
         "q3_attention_mass_4bit": [c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
                                    c_int, c_void_p],
@@ -2131,37 +2133,39 @@ class CudaOps:
         not its position (tokens were evicted).  ``mass`` / ``places`` (float32 / int32 ``[pages, kv heads, page_size]``): what
         eviction goes by; the written tokens' sums become zero, their places their positions."""
         what = "qk_norm_rope_store_4bit"
-        T = qkv.shape[0]
-        code = _dtype_code(qkv.dtype)
-        self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table)
-        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < (num_heads + (2 * num_kv_heads if write_kv else 0)) * head_dim:
+        T, D, dtype = qkv.size(0), head_dim, qkv.dtype
+        self._check_4bit(what, pages, num_kv_heads, D, page_size, block_table)
+        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.size(1) < (num_heads + (2 * num_kv_heads if write_kv else 0)) * D:
             raise KernelError(f"{what}: the projection is [tokens, heads * head_dim] with unit-stride rows")
-        q_out = qkv if q_out is None else q_out
-        if (q_out.dtype != qkv.dtype or q_out.dim() != 2 or q_out.shape[0] != T or q_out.shape[1] < num_heads * head_dim
+        if q_out is None:
+            q_out = qkv
+        elif (q_out.dtype != dtype or q_out.dim() != 2 or q_out.size(0) != T or q_out.size(1) < num_heads * D
                 or (T and q_out.stride(1) != 1)):
             raise KernelError(f"{what}: queries go to [tokens, heads * head_dim] of the projection's type, unit-stride rows")
-        for t, name in ((positions, "positions"), (token_seq, "token_seq"), (slots, "slots")):
+        for t in (positions, token_seq, slots):
             if t is not None and (t.dtype != torch.int32 or t.numel() != T or not t.is_contiguous()):
-                raise KernelError(f"{what}: {name} are dense int32, one per token")
+                raise KernelError(f"{what}: positions, token_seq and slots are dense int32, one per token")
         for w in (q_weight, k_weight):
-            if w is not None and (w.dtype != torch.float32 or w.numel() != head_dim or not w.is_contiguous()):
+            if w is not None and (w.dtype != torch.float32 or w.numel() != D or not w.is_contiguous()):
                 raise KernelError(f"{what}: norm weights are dense float32 vectors of head_dim")
-        if (cos is None) != (sin is None):
-            raise KernelError(f"{what}: cos and sin come together")
-        if cos is not None and (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < 1 or 2 * cos.shape[1] > head_dim
-                                or cos.dtype != torch.float32 or sin.dtype != torch.float32
-                                or not cos.is_contiguous() or not sin.is_contiguous()):
-            raise KernelError(f"{what}: rotation tables are dense float32 [positions, pairs] of one shape, at least one position")
-        self._check_cells(what, mass, torch.float32, pages, page_size)
-        self._check_cells(what, places, torch.int32, pages, page_size)
+        rot_half = max_pos = 0
+        if cos is not None or sin is not None:
+            if cos is None or sin is None:
+                raise KernelError(f"{what}: cos and sin come together")
+            if (cos.dim() != 2 or cos.shape != sin.shape or cos.size(0) < 1 or 2 * cos.size(1) > D or cos.dtype != torch.float32
+                    or sin.dtype != torch.float32 or not cos.is_contiguous() or not sin.is_contiguous()):
+                raise KernelError(f"{what}: rotation tables are dense float32 [positions, pairs] of one shape, at least one position")
+            max_pos, rot_half = cos.size(0), cos.size(1)
+        if mass is not None or places is not None:
+            self._check_cells(what, mass, torch.float32, pages, page_size)
+            self._check_cells(what, places, torch.int32, pages, page_size)
         self._check_here(what, qkv, q_out, positions, token_seq, slots, q_weight, k_weight, cos, sin)
         if self.timing is not None:
             e = qkv.element_size()
             self._costs(T * (2 * num_heads + 2 * num_kv_heads) * head_dim * e + T * num_kv_heads * four_bit_token_bytes(head_dim))
-        self._call("cache_4bit", "q3_store_4bit", what, code, _ptr(qkv), qkv.stride(0), _ptr(q_out), q_out.stride(0), num_heads,
-                   num_kv_heads, head_dim, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
-                   cos.shape[1] if cos is not None else 0, cos.shape[0] if cos is not None else 0, _ptr(positions), _ptr(slots),
-                   _ptr(token_seq), _ptr(block_table), block_table.shape[1], block_table.shape[0], _ptr(pages), pages.shape[0],
+        self._call("cache_4bit", "q3_store_4bit", what, _dtype_code(dtype), _ptr(qkv), qkv.stride(0), _ptr(q_out), q_out.stride(0),
+                   num_heads, num_kv_heads, D, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin), rot_half, max_pos,
+                   _ptr(positions), _ptr(slots), _ptr(token_seq), _ptr(block_table), block_table.size(1), block_table.size(0), _ptr(pages), pages.size(0),
                    page_size, T, int(bool(write_kv)), self.PAIRINGS[pairing], _ptr(mass), _ptr(places),
                    _ptr(self._error_word(qkv.device)))
         return q_out
@@ -2190,8 +2194,9 @@ class CudaOps:
                              window=None, decode_slices=None, lse=None):
         """:meth:`paged_attention` over a cache in 4 bits.  A sequence's tokens are the first ``kv_lens`` places of its cache and the
         step's tokens the last of them (``step.kv_lens`` and ``step.host_kv_lens`` count places: without evicted tokens, positions).
-        Single tokens of bfloat16 heads of 64, 128 or 256 read the numbers as they are (csrc/attention_4bit.cu); portions of prompts,
-        float32 and other head sizes have their sequences' pages unpacked once and go through the kernels for wide pages.
+        Single tokens of bfloat16 heads of 64, 128 or 256 read the numbers as they are, on the tensor cores; float32, and single tokens
+        of other sizes, on the FMA pipes (csrc/attention_4bit.cu).  bfloat16 portions of prompts have their sequences' pages unpacked
+        once (values rounded to bfloat16) and go through the kernels for wide pages.  ``step.positions`` are places here.
         ``lse`` (float32 ``[T, heads]``, steps of single tokens of those sizes): gets the logarithm of each row's sum."""
         what = "paged_attention_4bit"
         T, D, G, H, dtype = out.size(0), head_dim, num_kv_heads, num_heads, out.dtype
@@ -2214,32 +2219,55 @@ class CudaOps:
             raise KernelError(f"{what}: log sums are dense float32 [tokens, heads]")
         if fast and step.decode_only:
             return self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, None, step.num_seqs, max_len,
-                                     decode_slices or self.decode_slices_4bit(step.host_kv_lens, G, D, window), out, page_size, scale,
+                                     decode_slices or self.decode_slices_4bit(step.host_kv_lens, G, D, window, H // G), out, page_size, scale,
                                      window, step.kv_longest, lse)
-        _dtype_code(dtype)
-        wide = dict(num_heads=H, num_kv_heads=G, head_dim=D, token_seq=step.token_seq, positions=step.positions, out=out,
-                    page_size=page_size, scale=scale, window=window)
+        if dtype == torch.float32 or (step.decode_only and not fast):
+            return self._general_4bit(q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window)
+        # portions of prompts (and single tokens beside them): their sequences' pages unpacked, the kernels for wide pages
         n = -(-max_len // page_size)
-        split = fast and D != 256  # prompts apart from single tokens
+        split = fast and D != 256  # prompts apart from single tokens, which are decoded as they are
         cu = step.host_cu_seqlens
         count = sum(cu[b + 1] - cu[b] > 1 for b in range(step.num_seqs)) if split else step.num_seqs
         if split and step.num_single:
             singles = [kv for b, kv in enumerate(step.host_kv_lens) if cu[b + 1] - cu[b] == 1]
             self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, step.single_seqs, step.num_single, max(singles),
-                              self.decode_slices_4bit(singles, G, D, window), out, page_size, scale, window, None, None)
+                              self.decode_slices_4bit(singles, G, D, window, H // G), out, page_size, scale, window, None, None)
         if not count:
             return out
-        k, v = (torch.empty((count * n, G, page_size, D), dtype=out.dtype, device=out.device) for _ in range(2))
+        k, v = (torch.empty((count * n, G, page_size, D), dtype=dtype, device=out.device) for _ in range(2))
         table = torch.empty((block_table.shape[0], n), dtype=torch.int32, device=out.device)
         self._unpack_4bit(pages, block_table, step.kv_lens, max_len, step.cu_seqlens if split else None, count, n, k, v, table, page_size)
+        step = copy.copy(step)
         if split:
-            step = copy.copy(step)
             step.single_seqs, step.num_single = None, 0
-        elif step.captured_width:
-            step = copy.copy(step)
-            step.captured_width = n
         # the wide kernels number a token by its place: kv_lens and cu_seqlens say it, or for the general kernel `positions`
-        return self.paged_attention(q, q_stride, k_pages=k, v_pages=v, block_table=table, step=step, **wide)
+        return self.paged_attention(q, q_stride, num_heads=H, num_kv_heads=G, head_dim=D, k_pages=k, v_pages=v, block_table=table,
+                                    token_seq=step.token_seq, positions=step.positions, out=out, page_size=page_size, scale=scale,
+                                    window=window, step=step)
+
+    GENERAL_SLICE = 1024  # keys with a softmax of their own (csrc/attention_4bit.cu)
+
+    def _general_4bit(self, q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window):
+        code, T = _dtype_code(out.dtype), out.size(0)
+        for t in (step.token_seq, step.positions):
+            if t.dtype != torch.int32 or t.numel() < T or not t.is_contiguous():
+                raise KernelError("paged_attention_4bit: token_seq and positions are dense int32, one per token")
+        self._check_here("paged_attention_4bit", step.token_seq, step.positions)
+        slices, mid_o, mid_ml = -(-max_len // self.GENERAL_SLICE), None, None
+        blocks = T * G * -(-(H // G) // 8)
+        if slices < 2 or blocks >= 4 * self.SM_COUNT:  # enough blocks without: each goes through all slices
+            slices = 0
+        else:
+            mid_o = torch.empty((T, H, slices, D), dtype=torch.float32, device=out.device)
+            mid_ml = torch.empty((T, H, slices, 2), dtype=torch.float32, device=out.device)
+            self.launches += 1
+        if self.timing is not None:
+            self._costs(*self._attention_cost(step, H, G, D, out))
+        self._call("attention_4bit", "q3_general_attention_4bit", "paged_attention_general_4bit", code, _ptr(q), q_stride, _ptr(pages),
+                   pages.shape[0], _ptr(block_table), block_table.shape[1], block_table.shape[0], _ptr(step.token_seq),
+                   _ptr(step.positions), _ptr(out), _ptr(mid_o), _ptr(mid_ml), slices, T, H, G, D, page_size, float(scale),
+                   int(window or 0))
+        return out
 
     @staticmethod
     def decode_4bit_ok(q, num_heads, num_kv_heads, head_dim) -> bool:
@@ -2247,23 +2275,64 @@ class CudaOps:
         return (q.dtype == torch.bfloat16 and head_dim in (64, 128, 256) and num_heads // num_kv_heads <= 16 and q.stride(0) % 8 == 0
                 and q.data_ptr() % 16 == 0)
 
-    DECODE_4BIT_BLOCKS_PER_SM = {64: 5, 128: 4, 256: 2}
+    # blocks of decode attention over 4-bit numbers that an SM holds, by head size: up to 8 query heads a kv head, and more
+    DECODE_4BIT_BLOCKS_PER_SM = {64: (5, 4), 128: (4, 2), 256: (2, 1)}
 
-    def decode_slices_4bit(self, kv_lens, num_kv_heads, head_dim, window) -> int:
-        """Into how many slices the longest of these sequences' keys are cut by decode attention over a cache in 4 bits."""
-        longest, total, count = max(kv_lens, default=0), sum(kv_lens), len(kv_lens)
-        if window:
-            longest, total = min(longest, window + 15), min(total, count * (window + 15))
-        if longest < 1:
+    def decode_slices_4bit(self, kv_lens, num_kv_heads, head_dim, window=None, group=1) -> int:
+        """Into how many slices the longest of these sequences' keys are cut by decode attention over a cache in 4 bits (a shorter
+        sequence is cut into fewer of that length); negative: they are joined by a second kernel and not by the blocks of a cluster."""
+        cap = window + 15 if window else 1 << 30
+        rounds = tuple(-(-min(n, cap) // 128) for n in kv_lens)  # a block takes 128 keys at a time
+        key = ("4bit", num_kv_heads, head_dim, group > 8, rounds)
+        slices = self._slices_cache.get(key)
+        if slices is None:
+            if len(self._slices_cache) > 8192:
+                self._slices_cache.clear()
+            slices = self._slices_cache[key] = self._decode_slices_4bit(rounds, num_kv_heads, head_dim, group > 8)
+        return slices
+
+    def _decode_slices_4bit(self, rounds, num_kv_heads, head_dim, wide) -> int:
+        """Times in us, fitted to a sweep of 1 to 64 slices over 20 batches of 1 to 128 sequences of 64 to 32,769 tokens on a B200: the choice
+        is 4 % slower than the best one on average, 14 % at worst.  A round of 128 keys of 128 channels takes a block 1.15 alone and
+        0.66 for every block on its SM (groups of more than 8 heads 1.69 times as much), a block's beginning and end as much as 2.23
+        rounds, of which the SM notices 1.66 where other blocks go on meanwhile; the last blocks end apart by a share of their length.
+        A second kernel joins slices in 2.7 and more; clusters do so for nothing, but take a fifth longer, and all have to run at once."""
+        longest = max(rounds, default=0)
+        if longest < 2:
             return 1
-        slots = self.DECODE_4BIT_BLOCKS_PER_SM[head_dim] * self.SM_COUNT
-        per = max(1, -(-(total + 64 * count) * num_kv_heads // (128 * slots)))  # rounds of 128 keys a block
-        return max(1, min(64, -(-longest // (128 * per))))
+        sms, per_sm = self.SM_COUNT, self.DECODE_4BIT_BLOCKS_PER_SM[head_dim][int(wide)]
+        slots, unit, pairs = sms * per_sm, head_dim / 128 * (1.69 if wide else 1.0), len(rounds) * num_kv_heads
+        best, best_cost, seen = 1, math.inf, 0
+        for s in range(1, min(64, longest) + 1):
+            per = -(-longest // s)
+            if per == seen:  # more slices of the same length: none
+                continue
+            seen = per
+            blocks = num_kv_heads * sum(-(-r // per) for r in rounds)
+            if blocks > slots:
+                cost = 0.66 * unit * ((num_kv_heads * sum(rounds) + 1.66 * blocks) / sms + 0.08 * per * per_sm)
+            else:
+                cost = (per + 2.23) * unit * max(1.15, 0.66 * min(per_sm, math.ceil(blocks / sms)))
+            if s > 1:
+                cost += 2.7 + 0.28 * s
+            if cost < best_cost:
+                best, best_cost = -s if s > 1 else 1, cost
+            if 1 < s <= self._most_clustered(head_dim, wide) and s * pairs <= slots:
+                cost = 1.21 * (per + 2.23) * unit * max(1.15, 0.66 * min(per_sm, math.ceil(0.86 * blocks / sms))) + 0.14
+                if cost < best_cost:
+                    best, best_cost = s, cost
+        return best
+
+    @staticmethod
+    def _most_clustered(head_dim, wide) -> int:
+        """Slices that the blocks of one cluster join (blocks that fill an SM: no more than any cluster may have)."""
+        return 8 if head_dim == 256 and wide else 16
 
     def _decode_4bit(self, q, q_stride, H, G, D, pages, block_table, step, seq_list, num_seqs, max_len, slices, out, page_size, scale,
                      window, longest, lse):
         mid_o = mid_lse = None
-        if slices > 16 or (slices > 1 and slices * G * num_seqs > self.SM_COUNT):  # else the blocks of a cluster join them
+        joined, slices = slices < 0 or slices > self._most_clustered(D, H // G > 8), abs(slices)
+        if joined and slices > 1:
             mid = torch.empty(num_seqs * H * slices * (D + 1), dtype=torch.float32, device=out.device)
             mid_o = mid.data_ptr()
             mid_lse = mid_o + 4 * num_seqs * H * slices * D

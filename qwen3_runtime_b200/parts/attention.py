@@ -32,7 +32,8 @@ class PagedAttention(Part):
         self.scale = float(spec.get("scale") or 1.0 / math.sqrt(self.head_dim))
         self.four_bit = ctx.kv_bits == 4
         self.budget = ctx.kv_budget
-        self._slices_choice = ("decode_slices_4bit" if self.four_bit else "decode_slices", self.num_kv_heads, self.head_dim, self.window)
+        self._slices_choice = (("decode_slices_4bit", self.num_kv_heads, self.head_dim, self.window, self.num_heads // self.num_kv_heads)
+                               if self.four_bit else ("decode_slices", self.num_kv_heads, self.head_dim, self.window))
         if self.num_heads % self.num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         if self.budget is not None and self.window:
@@ -102,8 +103,8 @@ class PagedAttention(Part):
         model = getattr(self.ops, "decode_slices_4bit" if self.four_bit else "decode_slices_for", None)
         if model is None or self.ctx.dtype != torch.bfloat16 or self.head_dim not in (64, 128, 256):
             return {}
-        nkv, D, window = self.num_kv_heads, self.head_dim, self.window
-        return {self._slices_choice: lambda kv_lens: model(kv_lens, nkv, D, window)}
+        sizes = self._slices_choice[1:]
+        return {self._slices_choice: lambda kv_lens: model(kv_lens, *sizes)}
 
     def cache_spec(self):
         if self.four_bit:

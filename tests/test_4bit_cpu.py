@@ -176,3 +176,20 @@ def test_tensors_on_another_device_are_refused():
     table = Table()
     with pytest.raises(KernelError, match="launches on cuda:0"):
         cuda.CudaOps._check_here(table, "x", torch.zeros(1))
+
+
+def test_slices_of_decode_attention():
+    """At least one, no more than the longest sequence has rounds of 128 keys; a launch that fills the device is not cut further, one that
+    leaves it idle is; clusters only where all their blocks run at once; asked again, the answer is kept."""
+    table = Table()
+    table._slices_cache = {}
+    for lens in ([1], [128], [129], [513], [4097] * 8, [32768], [1024] * 64, [512] * 128, [65 + 83 * i for i in range(48)]):
+        for G, D, group in ((8, 128, 4), (8, 64, 2), (2, 256, 8), (1, 128, 16), (1, 256, 16)):
+            s = table.decode_slices_4bit(lens, G, D, None, group)
+            slots = 148 * table.DECODE_4BIT_BLOCKS_PER_SM[D][int(group > 8)]
+            assert 1 <= abs(s) <= min(64, -(-max(lens) // 128)) and s != -1
+            assert s < 0 or s == 1 or (s <= table._most_clustered(D, group > 8) and s * len(lens) * G <= slots)
+            assert s == table.decode_slices_4bit(lens, G, D, None, group)
+    assert table.decode_slices_4bit([1024] * 64, 8, 128) == 1 and table.decode_slices_4bit([1], 8, 128) == 1
+    assert table.decode_slices_4bit([32768], 8, 128) < -16 and 8 <= table.decode_slices_4bit([4097], 8, 128) <= 16
+    assert table.decode_slices_4bit([32768], 8, 128, 100) == 1 and table.decode_slices_4bit([], 8, 128) == 1

@@ -253,7 +253,7 @@ def test_positions_outside_the_tables_write_nothing_and_are_reported(ops):
 
 @pytest.mark.parametrize("H,G,D,page", [(8, 2, 128, 16), (4, 4, 128, 16), (16, 2, 128, 32), (12, 1, 128, 16), (16, 1, 64, 16), (2, 2, 64, 8),
                                         (6, 2, 256, 16), (16, 1, 256, 64), (8, 2, 128, 5), (8, 2, 64, 24), (5, 1, 128, 48), (8, 1, 256, 3)])
-@pytest.mark.parametrize("slices", [None, 1, 3, 9, 40])
+@pytest.mark.parametrize("slices", [None, 1, 3, -3, 8, 9, 16, 40])
 def test_decoded_tokens(ops, H, G, D, page, slices):
     lens = [1, 2, 15, 16, 17, 63, 64, 65, 200, 611]
     c = p4.Cache(lens, G, D, page, seed=H + D, k_scale=1.5)
@@ -286,7 +286,7 @@ def test_a_long_cache(ops):
     lens = [20011, 9000]
     c = p4.Cache(lens, 1, 128, 16, seed=5, k_scale=2.0)
     q = queries(2, 4, 128, 3)
-    for slices in (None, 1, 64):
+    for slices in (None, 1, 16, -16, 64):
         got, lse = attend(ops, c, q, [1, 1], lens, 4, 128 ** -0.5, lse=True, slices=slices)
         check_rows(got, q.view(-1, 4, 128), c, [1, 1], lens, 128 ** -0.5)
 
