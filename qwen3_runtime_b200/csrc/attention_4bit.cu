@@ -152,6 +152,27 @@ constexpr int ROUND = STEP * TILES * WARPS;
 constexpr int STAGES = 3;
 constexpr int MOST_CLUSTER = 16;
 
+// A step's barrier, when the first look finds its bytes still on their way; called by whole warps, which leave it of one mind.  Bounded:
+// false after the limit.  The warp then asks for nothing more (the barrier has its arrivals, and must not be given others), waits for what
+// it has in flight (wait_for_copies) and goes on to the block's end; the error word says that the result is invalid.
+__device__ __noinline__ bool wait_for_tiles(uint32_t bar, uint32_t parity, int* error_word) {
+  const long long start = clock64();
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    if (__any_sync(0xffffffffu, clock64() - start > Q3_WAIT_LIMIT_CYCLES)) {
+      atomicExch(error_word, Q3_ERR_WAIT_4BIT);
+      return false;
+    }
+  }
+  return true;
+}
+// The steps that are asked for and not yet taken, from `stage` on (bounded).
+__device__ __noinline__ void wait_for_copies(uint32_t bars, int stage, uint32_t parity) {
+  for (int i = 0; i < STAGES - 1; ++i) {
+    mbar_wait_drain(bars + 8 * stage, parity);
+    if (++stage == STAGES) stage = 0, parity ^= 1;
+  }
+}
+
 // Which token is row r of a tile (r < 8; row r + 8 is token + 8).  Any order will do, as keys and values agree on it; these let the rows
 // that one shared-memory access meets lie in different banks (D = 128: values two-way at worst).
 template <int D> __device__ __forceinline__ int token_of(int r) {
@@ -249,7 +270,11 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_4bit_k
     if (BULK) {  // each lane arrives once, with the bytes that it asks for
       const uint32_t bar = bar_at + 8 * stage;
       mbar_expect_tx(bar, valid ? H::TILE : 0);
+#ifdef Q3_TEST_WITHHOLD_A_BOX  // (a test build leaves the second tiles out: the stages never fill, a wait runs out)
+      if (valid && lane == 0) {
+#else
       if (valid) {
+#endif
         if (a.ps == STEP) {
           bulk_copy(dst, rec, H::TILE, bar);
         } else {
@@ -500,10 +525,14 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_4bit_k
     }
   };
   for (int base = begin + warp * STEP * TILES; base < end; base += ROUND) {
-    if (BULK)
-      mbar_wait_report(bar_at + 8 * stage, parity, a.error_word, Q3_ERR_WAIT_4BIT);
-    else
+    if (BULK) {
+      if (!__all_sync(0xffffffffu, mbar_try_wait(bar_at + 8 * stage, parity)) && !wait_for_tiles(bar_at + 8 * stage, parity, a.error_word)) {
+        wait_for_copies(bar_at, stage, parity);
+        break;
+      }
+    } else {
       cp_async_wait<STAGES - 2>();
+    }
     __syncwarp();
     const unsigned char* st = ring + stage * STAGE;
     if (base + STEP * TILES <= end && base >= sl.lo)  // (of one mind over the warp)
