@@ -2101,19 +2101,21 @@ class CudaOps:
         if not record or num_kv_heads < 1:
             raise KernelError(f"{what}: head sizes are multiples of 16 up to 256, pages and heads at least one "
                               f"(got head_dim={head_dim}, page_size={page_size}, num_kv_heads={num_kv_heads})")
-        dims = pages.dim()
-        if (pages.dtype != torch.uint8 or (dims != 3 and not (layers and dims == 4)) or pages.size(-1) != record
-                or pages.size(-2) != num_kv_heads or not pages.is_contiguous()):
-            raise KernelError(f"{what}: pages are dense uint8 [pages, {num_kv_heads}, {record}], got {pages.dtype} {tuple(pages.shape)}")
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous() or block_table.size(1) < 1:
+        shape, table = pages.shape, block_table.shape  # (each read of a tensor's fields costs: once)
+        if (pages.dtype != torch.uint8 or (len(shape) != 3 and not (layers and len(shape) == 4)) or shape[-1] != record
+                or shape[-2] != num_kv_heads or not pages.is_contiguous()):
+            raise KernelError(f"{what}: pages are dense uint8 [pages, {num_kv_heads}, {record}], got {pages.dtype} {tuple(shape)}")
+        if block_table.dtype != torch.int32 or len(table) != 2 or not block_table.is_contiguous() or table[1] < 1:
             raise KernelError(f"{what}: the block table is dense int32 [sequences, pages], at least one page wide")
-        if kv_lens is not None and (kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous() or kv_lens.numel() < block_table.size(0)):
+        if kv_lens is not None and (kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous() or kv_lens.numel() < table[0]):
             raise KernelError(f"{what}: lengths are dense int32, one per row of the block table")
         self._check_here(what, pages, block_table, kv_lens)
+        return shape, table
 
     def _check_here(self, what, *tensors):
+        here = self._device_index
         for t in tensors:
-            if t is not None and t.get_device() != self._device_index:
+            if t is not None and t.get_device() != here:
                 raise KernelError(f"{what}: this kernel table launches on cuda:{self._device_index}, a tensor is on {t.device}")
 
     def _check_cells(self, what, t, dtype, pages, page_size):
@@ -2133,15 +2135,17 @@ class CudaOps:
         not its position (tokens were evicted).  ``mass`` / ``places`` (float32 / int32 ``[pages, kv heads, page_size]``): what
         eviction goes by; the written tokens' sums become zero, their places their positions."""
         what = "qk_norm_rope_store_4bit"
-        T, D, dtype = qkv.size(0), head_dim, qkv.dtype
-        self._check_4bit(what, pages, num_kv_heads, D, page_size, block_table)
-        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.size(1) < (num_heads + (2 * num_kv_heads if write_kv else 0)) * D:
+        D, dtype, shape, stride = head_dim, qkv.dtype, qkv.shape, qkv.stride()
+        (num_pages, *_), (num_seqs, max_pages) = self._check_4bit(what, pages, num_kv_heads, D, page_size, block_table)
+        if len(shape) != 2 or stride[1] != 1 or shape[1] < (num_heads + (2 * num_kv_heads if write_kv else 0)) * D:
             raise KernelError(f"{what}: the projection is [tokens, heads * head_dim] with unit-stride rows")
+        T, q_stride = shape[0], stride[0]
         if q_out is None:
             q_out = qkv
-        elif (q_out.dtype != dtype or q_out.dim() != 2 or q_out.size(0) != T or q_out.size(1) < num_heads * D
-                or (T and q_out.stride(1) != 1)):
-            raise KernelError(f"{what}: queries go to [tokens, heads * head_dim] of the projection's type, unit-stride rows")
+        else:
+            shape, stride = q_out.shape, q_out.stride()
+            if (q_out.dtype != dtype or len(shape) != 2 or shape[0] != T or shape[1] < num_heads * D or (T and stride[1] != 1)):
+                raise KernelError(f"{what}: queries go to [tokens, heads * head_dim] of the projection's type, unit-stride rows")
         for t in (positions, token_seq, slots):
             if t is not None and (t.dtype != torch.int32 or t.numel() != T or not t.is_contiguous()):
                 raise KernelError(f"{what}: positions, token_seq and slots are dense int32, one per token")
@@ -2152,10 +2156,11 @@ class CudaOps:
         if cos is not None or sin is not None:
             if cos is None or sin is None:
                 raise KernelError(f"{what}: cos and sin come together")
-            if (cos.dim() != 2 or cos.shape != sin.shape or cos.size(0) < 1 or 2 * cos.size(1) > D or cos.dtype != torch.float32
+            shape = cos.shape
+            if (len(shape) != 2 or shape != sin.shape or shape[0] < 1 or 2 * shape[1] > D or cos.dtype != torch.float32
                     or sin.dtype != torch.float32 or not cos.is_contiguous() or not sin.is_contiguous()):
                 raise KernelError(f"{what}: rotation tables are dense float32 [positions, pairs] of one shape, at least one position")
-            max_pos, rot_half = cos.size(0), cos.size(1)
+            max_pos, rot_half = shape
         if mass is not None or places is not None:
             self._check_cells(what, mass, torch.float32, pages, page_size)
             self._check_cells(what, places, torch.int32, pages, page_size)
@@ -2163,10 +2168,10 @@ class CudaOps:
         if self.timing is not None:
             e = qkv.element_size()
             self._costs(T * (2 * num_heads + 2 * num_kv_heads) * head_dim * e + T * num_kv_heads * four_bit_token_bytes(head_dim))
-        self._call("cache_4bit", "q3_store_4bit", what, _dtype_code(dtype), _ptr(qkv), qkv.stride(0), _ptr(q_out), q_out.stride(0),
+        self._call("cache_4bit", "q3_store_4bit", what, _dtype_code(dtype), qkv.data_ptr(), q_stride, q_out.data_ptr(), stride[0],
                    num_heads, num_kv_heads, D, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin), rot_half, max_pos,
-                   _ptr(positions), _ptr(slots), _ptr(token_seq), _ptr(block_table), block_table.size(1), block_table.size(0), _ptr(pages), pages.size(0),
-                   page_size, T, int(bool(write_kv)), self.PAIRINGS[pairing], _ptr(mass), _ptr(places),
+                   _ptr(positions), _ptr(slots), _ptr(token_seq), block_table.data_ptr(), max_pages, num_seqs, pages.data_ptr(),
+                   num_pages, page_size, T, int(bool(write_kv)), self.PAIRINGS[pairing], _ptr(mass), _ptr(places),
                    _ptr(self._error_word(qkv.device)))
         return q_out
 
@@ -2174,21 +2179,23 @@ class CudaOps:
         """Keys and values of the sequences' first ``max_kv_len`` tokens as wide pages ``[sequences * n, kv heads, page_size, head_dim]``
         of ``dtype``, ``n = ceil(max_kv_len / page_size)`` pages per sequence in order; zero behind a sequence's last token."""
         what = "unpack_4bit"
-        self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens)
-        B, n = block_table.shape[0], -(-int(max_kv_len) // page_size)
-        if n > block_table.shape[1] or max_kv_len < 0:
-            raise KernelError(f"{what}: max_kv_len={max_kv_len} does not fit a block table of {block_table.shape[1]} pages")
-        k, v = (torch.empty((B * n, num_kv_heads, page_size, head_dim), dtype=dtype, device=pages.device) for _ in range(2))
+        _, (B, width) = self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens)
+        n = -(-int(max_kv_len) // page_size)
+        if n > width or max_kv_len < 0:
+            raise KernelError(f"{what}: max_kv_len={max_kv_len} does not fit a block table of {width} pages")
+        k = torch.empty((B * n, num_kv_heads, page_size, head_dim), dtype=dtype, device=pages.device)
+        v = torch.empty_like(k)
         self._unpack_4bit(pages, block_table, kv_lens, int(max_kv_len), None, B, n, k, v, None, page_size)
         return k, v
 
     def _unpack_4bit(self, pages, block_table, kv_lens, max_len, cu, count, width, k, v, table, page_size):
-        G, D = k.shape[1], k.shape[3]
+        _, G, _, D = k.shape
+        num_seqs, max_pages = block_table.shape
         if self.timing is not None:
             self._costs(2 * k.numel() * k.element_size() + count * width * G * four_bit_page_bytes(D, page_size))
-        self._call("cache_4bit", "q3_unpack_4bit", "unpack_4bit", _dtype_code(k.dtype), _ptr(pages), pages.shape[0], G, D, page_size,
-                   _ptr(block_table), block_table.shape[1], _ptr(kv_lens), block_table.shape[0], max_len, _ptr(cu), count, width,
-                   int(table is None), _ptr(k), _ptr(v), _ptr(table))
+        self._call("cache_4bit", "q3_unpack_4bit", "unpack_4bit", _dtype_code(k.dtype), pages.data_ptr(), pages.shape[0], G, D, page_size,
+                   block_table.data_ptr(), max_pages, _ptr(kv_lens), num_seqs, max_len, _ptr(cu), count, width,
+                   int(table is None), k.data_ptr(), v.data_ptr(), _ptr(table))
 
     def paged_attention_4bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, block_table, out, page_size, scale, step,
                              window=None, decode_slices=None, lse=None):
@@ -2199,17 +2206,18 @@ class CudaOps:
         once (values rounded to bfloat16) and go through the kernels for wide pages.  ``step.positions`` are places here.
         ``lse`` (float32 ``[T, heads]``, steps of single tokens of those sizes): gets the logarithm of each row's sum."""
         what = "paged_attention_4bit"
-        T, D, G, H, dtype = out.size(0), head_dim, num_kv_heads, num_heads, out.dtype
-        self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens)
-        if H % G or q.dtype != dtype or out.dim() != 2 or out.size(1) != H * D or not out.is_contiguous():
+        D, G, H, dtype, shape, rows = head_dim, num_kv_heads, num_heads, out.dtype, q.shape, out.shape
+        _, (table_rows, max_pages) = self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens)
+        if H % G or q.dtype != dtype or len(rows) != 2 or rows[1] != H * D or not out.is_contiguous():
             raise KernelError(f"{what}: out is dense [tokens, heads * head_dim] of the queries' type, heads a multiple of kv heads")
-        if q.dim() != 2 or q.size(0) < T or q.size(1) < H * D or q_stride < H * D or T != step.num_tokens:
+        T = rows[0]
+        if len(shape) != 2 or shape[0] < T or shape[1] < H * D or q_stride < H * D or T != step.num_tokens:
             raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step")
         self._check_here(what, q, out, lse)
-        room = block_table.size(1) * page_size
-        if step.max_kv_len > room or step.num_seqs > block_table.size(0):
+        room = max_pages * page_size
+        if step.max_kv_len > room or step.num_seqs > table_rows:
             raise KernelError(f"{what}: {step.num_seqs} sequences of up to {step.max_kv_len} tokens do not fit a block table of "
-                              f"{block_table.size(0)} x {block_table.size(1)} pages")
+                              f"{table_rows} x {max_pages} pages")
         max_len = min(step.captured_width * page_size, room) if step.captured_width else step.max_kv_len
         fast = (dtype == torch.bfloat16 and D in (64, 128, 256) and H // G <= 16 and q_stride % 8 == 0 and q.data_ptr() % 16 == 0
                 and out.data_ptr() % 8 == 0)
