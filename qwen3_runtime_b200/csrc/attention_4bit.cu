@@ -735,9 +735,10 @@ template <int D, int NT> int launch_decode(const Decode& a, int num_seqs, cudaSt
 // ---- sums of attention weights -----------------------------------------------------------------------------------------------------
 // mass[key] += sum over a sequence's last `observe` tokens and the query heads of the kv head of 2^(score - log sum of the row).  Rows are
 // (token, head of the group), token by token; the scores' tiles are those of decode attention.  A cached token's sum belongs to one warp's
-// lane: no atomics, the same bits every time.
+// lane: no atomics, the same bits every time.  Sums are float32; a weight is 2^x to 2 units in the last place (2^-22 of itself).
 //   few rows (up to 16: single tokens)  mass_few_kernel: the queries stay in registers, keys stream past them, 16 a warp at a time, the next
-//                                       ones' bytes on their way; reads half of what the attention reads.
+//                                       ones' bytes on their way; reads half of what the attention reads.  Instructions bound it: 96,700
+//                                       tokens of 8 kv heads of 128 channels in 29 us (2.0 TB/s); with two tiles on their way no less.
 //   more                                mass_rows_kernel: the rows' log sums, keys cut into slices so that all SMs have some (left out
 //                                       where the attention has them); mass_columns_kernel: a warp keeps 16 keys and goes through the
 //                                       rows, which the block has turned into operands in shared memory.
@@ -783,6 +784,42 @@ template <int D> struct KeyBytes {  // what a lane holds of 16 keys as they are 
           *reinterpret_cast<uint4*>(&w[half][4]) = *reinterpret_cast<const uint4*>(codes + 16 * (l + 4));
           *reinterpret_cast<uint4*>(&p[half][0]) = *reinterpret_cast<const uint4*>(par);
         }
+      }
+    }
+  }
+};
+
+// Sixteen keys of one page (page sizes that are multiples of 16): one place for all of them.
+template <int D> struct PageKeys {
+  long code_at, par_at;  // this lane's first bytes in a tile
+  __device__ __forceinline__ PageKeys(const Q4Page& L, int lane)
+      : code_at((lane >> 2) * Head<D>::ROW + (D == 64 ? 8 : 16) * (lane & 3)), par_at(L.kpar + (lane >> 2) * Head<D>::PAR) {}
+  __device__ __forceinline__ void load(KeyBytes<D>& b, const Mass& m, const Q4Page& L, int kvh, int page, int row) const {
+    using H = Head<D>;
+    if ((uint32_t)page >= (uint32_t)m.num_pages) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int j = 0; j < H::WORDS; ++j) b.w[half][j] = 0;
+#pragma unroll
+        for (int g = 0; g < H::G; ++g) b.p[half][g] = 0;
+      }
+      return;
+    }
+    const unsigned char* rec = m.pages + ((long)page * m.nkv + kvh) * L.record;
+    const unsigned char *codes = rec + ((long)row * H::ROW + code_at), *par = rec + ((long)row * H::PAR + par_at);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if constexpr (D == 64) {
+        *reinterpret_cast<uint2*>(&b.w[half][0]) = *reinterpret_cast<const uint2*>(codes + 8 * half * H::ROW);
+        b.p[half][0] = *reinterpret_cast<const uint32_t*>(par + 8 * half * H::PAR);
+      } else if constexpr (D == 128) {
+        *reinterpret_cast<uint4*>(&b.w[half][0]) = *reinterpret_cast<const uint4*>(codes + 8 * half * H::ROW);
+        *reinterpret_cast<uint2*>(&b.p[half][0]) = *reinterpret_cast<const uint2*>(par + 8 * half * H::PAR);
+      } else {
+        *reinterpret_cast<uint4*>(&b.w[half][0]) = *reinterpret_cast<const uint4*>(codes + 8 * half * H::ROW);
+        *reinterpret_cast<uint4*>(&b.w[half][4]) = *reinterpret_cast<const uint4*>(codes + 8 * half * H::ROW + 64);
+        *reinterpret_cast<uint4*>(&b.p[half][0]) = *reinterpret_cast<const uint4*>(par + 8 * half * H::PAR);
       }
     }
   }
@@ -903,7 +940,7 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS) mass_rows_ke
       for (int c = 0; c < 2; ++c) {
         const float x0 = first + r <= sees[n][c] ? x[c] : -INFINITY, x1 = first + r + 8 <= sees[n][c] ? x[c + 2] : -INFINITY;
         const float top = fmaxf(m[n][c], fmaxf(x0, x1));
-        sum[n][c] = sum[n][c] * exp2f(m[n][c] - top) + exp2f(x0 - top) + exp2f(x1 - top);
+        sum[n][c] = sum[n][c] * exp2_fast(m[n][c] - top) + exp2_fast(x0 - top) + exp2_fast(x1 - top);
         m[n][c] = top;
       }
     }
@@ -917,7 +954,7 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS) mass_rows_ke
       for (int d = 4; d < 32; d <<= 1) {
         const float om = __shfl_xor_sync(0xffffffffu, m[n][c], d), os = __shfl_xor_sync(0xffffffffu, sum[n][c], d);
         const float top = fmaxf(m[n][c], om);
-        sum[n][c] = sum[n][c] * exp2f(m[n][c] - top) + os * exp2f(om - top);
+        sum[n][c] = sum[n][c] * exp2_fast(m[n][c] - top) + os * exp2_fast(om - top);
         m[n][c] = top;
       }
       if (r == 0) joined[warp][8 * n + 2 * l + c] = make_float2(m[n][c], sum[n][c]);
@@ -929,7 +966,7 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS) mass_rows_ke
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) top = fmaxf(top, joined[w][tid].x);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) den += joined[w][tid].y * exp2f(joined[w][tid].x - top);
+    for (int w = 0; w < WARPS; ++w) den += joined[w][tid].y * exp2_fast(joined[w][tid].x - top);
     const long at = (long)(rows.first + row / R) * a.nq + kvh * R + row % R;
     if (a.part)
       a.part[at * a.slices + slice] = make_float2(top, den);
@@ -945,7 +982,7 @@ __device__ __forceinline__ float row_log2(const Mass& a, long at) {
   for (int s = 0; s < a.slices; ++s) top = fmaxf(top, a.part[at * a.slices + s].x);
   for (int s = 0; s < a.slices; ++s) {
     const float2 y = a.part[at * a.slices + s];
-    den += y.y * exp2f(y.x - top);
+    den += y.y * exp2_fast(y.x - top);
   }
   return top + log2f(den);
 }
@@ -1023,7 +1060,7 @@ template <int D> __global__ void __launch_bounds__(32 * COLUMN_WARPS) mass_colum
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = first + r + 8 * (e >> 1);
-        total[e >> 1] += key <= (e & 1 ? sees.y : sees.x) ? exp2f(x[e] - (e & 1 ? lse2.y : lse2.x)) : 0.f;
+        total[e >> 1] += key <= (e & 1 ? sees.y : sees.x) ? exp2_fast(x[e] - (e & 1 ? lse2.y : lse2.x)) : 0.f;
       }
     }
   }
@@ -1042,7 +1079,8 @@ template <int D> __global__ void __launch_bounds__(32 * COLUMN_WARPS) mass_colum
 
 // Few rows: grid (slice, kv head, sequence); a warp takes every fourth 16 keys of the slice.  Two tiles are on their way while one is
 // worked on: the first one's bytes, and the pages of the second, whose bytes wait for them.  NT tiles of 8 rows.
-template <int D, int NT> __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 4) mass_few_kernel(Mass a) {
+// WHOLE: page sizes that are multiples of 16, so that a tile's keys lie in one page and have one lookup (29 us; a lookup a key takes 33).
+template <int D, int NT, bool WHOLE> __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 4) mass_few_kernel(Mass a) {
   using H = Head<D>;
   pdl_wait();
   pdl_launch_dependents();
@@ -1055,33 +1093,39 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS, D == 256 ? 2
   if (begin >= end || rows.count == 0) return;
   const Q4Page L(D, H::G, a.ps);
   const int* bt = a.block_table + (long)seq * a.max_pages;
-  // this lane's two keys of the tile to come: page of the sequence and row, moved on by a step of the block at a time
-  int at_page[2], row[2];
+  // this lane's two keys of the tile to come (or the whole tile): page of the sequence and row, moved on by a step of the block at a time
+  constexpr int PLACES = WHOLE ? 1 : 2;
+  int at_page[PLACES], row[PLACES];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int key = begin + warp * STEP + r + 8 * half;
+  for (int half = 0; half < PLACES; ++half) {
+    const int key = begin + warp * STEP + (WHOLE ? 0 : r + 8 * half);
     at_page[half] = key / a.ps, row[half] = key - at_page[half] * a.ps;
   }
   const int go_pages = ROWS_STEP / a.ps, go_rows = ROWS_STEP - go_pages * a.ps;
-  int page[2], next_row[2];
+  int page[PLACES], next_row[PLACES];
   auto look_up = [&](int first) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      page[half] = first + r + 8 * half < end ? bt[at_page[half]] : -1;
+    for (int half = 0; half < PLACES; ++half) {
+      page[half] = first + (WHOLE ? 0 : r + 8 * half) < end ? bt[at_page[half]] : -1;
       next_row[half] = row[half];
       at_page[half] += go_pages, row[half] += go_rows;
       if (row[half] >= a.ps) row[half] -= a.ps, ++at_page[half];
     }
   };
+  const PageKeys<D> tile(L, lane);
   KeyBytes<D> bytes;
   float* cell[2];
   float old[2];
-  auto fetch = [&]() {  // the bytes and sums of the keys looked up last
-    bytes.load(a, L, kvh, page, next_row, lane);
+  auto fetch = [&](int first) {  // the bytes and sums of the keys looked up last
+    if constexpr (WHOLE)
+      tile.load(bytes, a, L, kvh, page[0], next_row[0]);
+    else
+      bytes.load(a, L, kvh, page, next_row, lane);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const bool own = l == 0 && (uint32_t)page[half] < (uint32_t)a.num_pages;
-      cell[half] = own ? a.mass + ((long)page[half] * a.nkv + kvh) * a.ps + next_row[half] : nullptr;
+      const int at = WHOLE ? 0 : half;
+      const bool own = l == 0 && (uint32_t)page[at] < (uint32_t)a.num_pages && (!WHOLE || first + r + 8 * half < end);
+      cell[half] = own ? a.mass + ((long)page[at] * a.nkv + kvh) * a.ps + next_row[at] + (WHOLE ? r + 8 * half : 0) : nullptr;
       old[half] = own ? *cell[half] : 0.f;
     }
   };
@@ -1103,14 +1147,14 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS, D == 256 ? 2
       sees[n][c] = is ? rows.before + i : -1;
     }
   }
-  fetch();
+  fetch(first);
   look_up(first + ROWS_STEP);
   for (; first < end; first += ROWS_STEP) {
     KeyTile<D> k;
     k.take(bytes);
     float* const mine[2] = {cell[0], cell[1]};
     const float was[2] = {old[0], old[1]};
-    fetch();
+    fetch(first + ROWS_STEP);
     look_up(first + 2 * ROWS_STEP);
     float total[2] = {0.f, 0.f};
 #pragma unroll
@@ -1120,7 +1164,7 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS, D == 256 ? 2
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = first + r + 8 * (e >> 1);
-        total[e >> 1] += key <= sees[n][e & 1] ? exp2f(x[e] - lse2[n][e & 1]) : 0.f;
+        total[e >> 1] += key <= sees[n][e & 1] ? exp2_fast(x[e] - lse2[n][e & 1]) : 0.f;
       }
     }
 #pragma unroll
@@ -1207,8 +1251,12 @@ template <int D, int NT> int launch_mass(const Mass& a, bool want_rows, int most
   if (err != cudaSuccess) return Q3_ERR_LAUNCH;
   if (rows <= 16) {
     const dim3 grid(few_slices, a.nkv, a.num_seqs);
-    err = rows <= 8 ? launch_pdl(mass_few_kernel<D, 1>, grid, dim3(THREADS), 0, stream, a)
-                    : launch_pdl(mass_few_kernel<D, 2>, grid, dim3(THREADS), 0, stream, a);
+    if (a.ps % STEP == 0)
+      err = rows <= 8 ? launch_pdl(mass_few_kernel<D, 1, true>, grid, dim3(THREADS), 0, stream, a)
+                      : launch_pdl(mass_few_kernel<D, 2, true>, grid, dim3(THREADS), 0, stream, a);
+    else
+      err = rows <= 8 ? launch_pdl(mass_few_kernel<D, 1, false>, grid, dim3(THREADS), 0, stream, a)
+                      : launch_pdl(mass_few_kernel<D, 2, false>, grid, dim3(THREADS), 0, stream, a);
   } else {
     constexpr int KEYS = COLUMN_WARPS * STEP;
     constexpr int smem = COLUMN_TILES * sizeof(RowTile<D>);

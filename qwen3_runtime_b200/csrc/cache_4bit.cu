@@ -5,6 +5,8 @@
 // * evict:  see evict_select_kernel.
 #include <limits.h>
 
+#include <type_traits>
+
 #include "four_bit.cuh"
 #include "rotary.cuh"
 
@@ -38,8 +40,9 @@ __device__ __forceinline__ bool store_place(const Store& a, int t, int nkv, int 
 }
 
 // Head sizes 16, 32, 64, 128, 256 with the rotation over the whole head (or none): D / 16 threads per (token, head); thread c owns
-// channels [8c, 8c + 8) and [D/2 + 8c, D/2 + 8c + 8), which are one word of 4-bit numbers each.  What bounds it is the bytes of the projection
-// and of the queries.
+// channels [8c, 8c + 8) and [D/2 + 8c, D/2 + 8c + 8), which are one word of 4-bit numbers each.  The floor is the bytes of the projection
+// and of the queries; what bounds it is instructions, 415 for four heads of 128 channels: 3,258 tokens of 32 + 8 heads take 24 us, 2.9 TB/s.
+// Weights and angles asked for ahead of the squares' sum cost more in registers than they hide (26 us), three heads a thread more again (41).
 //
 // A key near the border between two numbers falls on either side by float32's last bit.  So that it falls where a float32 statement of
 // norm and rotation in PyTorch puts it, heads of 128 and 256 sum their squares four neighbours at a time and then by halves, and products
@@ -52,10 +55,15 @@ __device__ __forceinline__ void turn_rounded(float& a, float& b, float cs, float
   a = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
   b = __fadd_rn(__fmul_rn(y, cs), __fmul_rn(x, sn));
 }
-template <typename T>
-__global__ void store_4bit_vec_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, int nq, int nkv, int D, int G, int tph_shift,
-                                      Store a) {
-  const int tph = 1 << tph_shift;
+__device__ __forceinline__ float least_or_nan(float x, float y) {
+  float z;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+// KNOWN: the head size where the compiler knows it, else 0.
+template <typename T, int KNOWN>
+__global__ void store_4bit_vec_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, int nq, int nkv, int size, Store a) {
+  const int D = KNOWN ? KNOWN : size, G = q4_groups(D), tph = D / 16, tph_shift = 31 - __clz(tph);
   const int heads = a.write_kv ? nq + 2 * nkv : nq;
   pdl_wait();
   pdl_launch_dependents();
@@ -81,6 +89,7 @@ __global__ void store_4bit_vec_kernel(const T* qkv, int row_stride, T* q_out, in
   float ss;
   if (D >= 128) {
     float even = __fadd_rn(quad_of_squares(v0), quad_of_squares(v1)), odd = __fadd_rn(quad_of_squares(v0 + 4), quad_of_squares(v1 + 4));
+#pragma unroll
     for (int o = tph >> 1; o > 0; o >>= 1) {
       even = __fadd_rn(even, __shfl_xor_sync(0xffffffffu, even, o));
       odd = __fadd_rn(odd, __shfl_xor_sync(0xffffffffu, odd, o));
@@ -133,23 +142,22 @@ __global__ void store_4bit_vec_kernel(const T* qkv, int row_stride, T* q_out, in
   }
   if (__all_sync(0xffffffffu, !live || is_q)) return;
   // (else all lanes take part in the reductions: heads of queries and keys may share a warp)
-  float lo0 = v0[0], hi0 = v0[0], lo1 = v1[0], hi1 = v1[0], nan0 = 0.f, nan1 = 0.f;
+  float lo0 = v0[0], hi0 = v0[0], lo1 = v1[0], hi1 = v1[0];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo0 = fminf(lo0, v0[e]), hi0 = fmaxf(hi0, v0[e]), nan0 += v0[e] * 0.f;
-    lo1 = fminf(lo1, v1[e]), hi1 = fmaxf(hi1, v1[e]), nan1 += v1[e] * 0.f;
+  for (int e = 1; e < 8; ++e) {
+    lo0 = least_or_nan(lo0, v0[e]), hi0 = fmaxf(hi0, v0[e]);
+    lo1 = least_or_nan(lo1, v1[e]), hi1 = fmaxf(hi1, v1[e]);
   }
-  if (G == 1) {  // both words lie in the one group
-    lo0 = lo1 = fminf(lo0, lo1), hi0 = hi1 = fmaxf(hi0, hi1), nan0 = nan1 = nan0 + nan1;
-  }
-  const int lanes = G == 1 ? tph : 8;  // of one group
+  if (G == 1) lo0 = least_or_nan(lo0, lo1), hi0 = fmaxf(hi0, hi1);  // both words lie in the one group
+  const int lanes = G == 1 ? tph : 8;                               // of one group
+#pragma unroll
   for (int o = lanes >> 1; o > 0; o >>= 1) {
-    lo0 = fminf(lo0, __shfl_xor_sync(0xffffffffu, lo0, o));
+    lo0 = least_or_nan(lo0, __shfl_xor_sync(0xffffffffu, lo0, o));
     hi0 = fmaxf(hi0, __shfl_xor_sync(0xffffffffu, hi0, o));
-    nan0 += __shfl_xor_sync(0xffffffffu, nan0, o);
-    lo1 = fminf(lo1, __shfl_xor_sync(0xffffffffu, lo1, o));
-    hi1 = fmaxf(hi1, __shfl_xor_sync(0xffffffffu, hi1, o));
-    nan1 += __shfl_xor_sync(0xffffffffu, nan1, o);
+    if (G > 1) {
+      lo1 = least_or_nan(lo1, __shfl_xor_sync(0xffffffffu, lo1, o));
+      hi1 = fmaxf(hi1, __shfl_xor_sync(0xffffffffu, hi1, o));
+    }
   }
   if (!live || is_q || !turned) return;
   const int kvh = is_v ? hi - nq - nkv : hi - nq;
@@ -158,7 +166,7 @@ __global__ void store_4bit_vec_kernel(const T* qkv, int row_stride, T* q_out, in
   int row;
   long cell;
   if (!store_place(a, t, nkv, kvh, L.record, &rec, &row, &cell)) return;
-  const Q4Scale y0 = q4_scale(lo0, hi0, nan0), y1 = q4_scale(lo1, hi1, nan1);
+  const Q4Scale y0 = q4_scale(lo0, hi0), y1 = G == 1 ? y0 : q4_scale(lo1, hi1);
   uint32_t* code = reinterpret_cast<uint32_t*>(rec + (is_v ? L.values : 0) + (long)row * L.half);
   uint32_t* par = reinterpret_cast<uint32_t*>(rec + (is_v ? L.vpar : L.kpar) + (long)row * L.par);
   // group and index in it of the two words
@@ -240,7 +248,7 @@ __global__ void store_4bit_kernel(const T* qkv, int row_stride, T* q_out, int q_
       lo = fminf(lo, v), high = fmaxf(high, v), nan += v * 0.f;
     }
     lo = -warp_max(-lo), high = warp_max(high), nan = warp_sum(nan);
-    const Q4Scale y = q4_scale(lo, high, nan);
+    const Q4Scale y = q4_scale(lo + nan, high);
     if (lane < size / 8) {
       float v[8];
 #pragma unroll
@@ -673,15 +681,24 @@ Q3_EXPORT int q3_store_4bit(int dtype, const void* qkv, int row_stride, void* q_
                    q4_aligned(qkv) && q4_aligned(q_out) && q4_aligned(q_w) && q4_aligned(k_w) && q4_aligned(cos_t) && q4_aligned(sin_t);
   cudaError_t err;
   if (vec) {
-    int shift = 0;
-    while ((1 << shift) < tph) ++shift;
     const int threads = 128, per_token = (write_kv ? nq + 2 * nkv : nq) * tph;
     const dim3 grid((unsigned)num_tokens, (unsigned)((per_token + threads - 1) / threads));
     if (grid.y > 65535) return Q3_ERR_UNSUPPORTED;
-    err = dtype == Q3_DTYPE_F32 ? launch_pdl(store_4bit_vec_kernel<float>, grid, dim3(threads), 0, stream, (const float*)qkv, row_stride,
-                                             (float*)q_out, q_stride, nq, nkv, D, G, shift, a)
-                                : launch_pdl(store_4bit_vec_kernel<bf16>, grid, dim3(threads), 0, stream, (const bf16*)qkv, row_stride,
-                                             (bf16*)q_out, q_stride, nq, nkv, D, G, shift, a);
+    auto launch = [&](auto known) {
+      constexpr int K = decltype(known)::value;
+      err = dtype == Q3_DTYPE_F32 ? launch_pdl(store_4bit_vec_kernel<float, K>, grid, dim3(threads), 0, stream, (const float*)qkv, row_stride,
+                                               (float*)q_out, q_stride, nq, nkv, D, a)
+                                  : launch_pdl(store_4bit_vec_kernel<bf16, K>, grid, dim3(threads), 0, stream, (const bf16*)qkv, row_stride,
+                                               (bf16*)q_out, q_stride, nq, nkv, D, a);
+    };
+    if (D == 64)
+      launch(std::integral_constant<int, 64>());
+    else if (D == 128)
+      launch(std::integral_constant<int, 128>());
+    else if (D == 256)
+      launch(std::integral_constant<int, 256>());
+    else
+      launch(std::integral_constant<int, 0>());
     return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
   }
   constexpr int WARPS = 4;
