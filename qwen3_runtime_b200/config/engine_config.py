@@ -29,7 +29,9 @@ def canonical_cache(kv_bits, token_budget):
     if kv_bits is not None and (isinstance(kv_bits, bool) or kv_bits != 4):
         raise ValueError(f"kv_bits must be 4 (or None: keys and values in the compute dtype), got {kv_bits!r}")
     if token_budget is not None and not isinstance(token_budget, TokenBudget):
-        token_budget = TokenBudget(int(token_budget))
+        if isinstance(token_budget, bool) or not isinstance(token_budget, int):
+            raise ValueError(f"token_budget must be a number of tokens or a TokenBudget, got {token_budget!r}")
+        token_budget = TokenBudget(token_budget)
     if token_budget is not None and kv_bits is None:
         raise ValueError("a token budget needs kv_bits=4: the weights are summed by the attention over a cache in 4 bits")
     return kv_bits, token_budget

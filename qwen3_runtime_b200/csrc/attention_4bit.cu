@@ -1482,11 +1482,11 @@ Q3_EXPORT int q3_attention_mass_4bit(int dtype, const void* q, int q_stride, con
                                      int max_pages, const int* kv_lens, const int* cu_seqlens, float* mass, float* lse, int have_lse,
                                      void* part, int slices, int num_seqs, int nq, int nkv, int D, int ps, float scale, int max_len,
                                      int observe, int most_tokens, int few_slices, cudaStream_t stream) {
+  if (num_seqs < 1 || most_tokens < 1 || max_len < 1) return Q3_OK;
   if (!q || !pages || !block_table || !kv_lens || !cu_seqlens || !mass || !lse || nq < 1 || nkv < 1 || nq % nkv || !q4_sizes_ok(D, ps) ||
       slices < 1 || few_slices < 1 || (slices > 1 && !part) || observe < 1 || max_len > (long)max_pages * ps)
     return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
-  if (num_seqs < 1 || most_tokens < 1 || max_len < 1) return Q3_OK;
   if (q_stride % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(pages) & 15) ||
       (long)num_seqs * nkv > 65535 || nq > 65535)
     return Q3_ERR_UNSUPPORTED;
@@ -1517,6 +1517,7 @@ Q3_EXPORT int q3_decode_attention_4bit(const void* q, int q_stride, const void* 
                                        const int* kv_lens, const int* cu_seqlens, const int* seq_list, void* out, float* mid_o,
                                        float* mid_lse, float* lse, int num_seqs, int nq, int nkv, int D, int ps, float scale, int window,
                                        int splits, int max_len, const int* longest, int* error_word, cudaStream_t stream) {
+  if (num_seqs < 1) return Q3_OK;
   if (!q || !pages || !block_table || !kv_lens || !cu_seqlens || !out || nq < 1 || nkv < 1 || nq % nkv || !q4_sizes_ok(D, ps) || splits < 1 ||
       !error_word || (splits > MOST_CLUSTER && !mid_o) || (mid_o && !mid_lse) || max_len > (long)max_pages * ps)
     return Q3_ERR_ARGUMENT;
@@ -1524,7 +1525,6 @@ Q3_EXPORT int q3_decode_attention_4bit(const void* q, int q_stride, const void* 
   if (R > 16 || q_stride % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(pages) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 7) || num_seqs > 65535 || nkv > 65535 || Q4Page(D, q4_groups(D), ps).record * nkv > 0x7fffffffL)
     return Q3_ERR_UNSUPPORTED;
-  if (num_seqs < 1) return Q3_OK;
   Decode a{(const bf16*)q, q_stride, (const unsigned char*)pages, num_pages, block_table, kv_lens, cu_seqlens, seq_list, max_pages,
            (bf16*)out, mid_o, mid_lse, lse, nq, nkv, ps, window, splits, max_len, scale * LOG2_E, longest, error_word};
   if (D == 64) return R <= 8 ? launch_decode<64, 1>(a, num_seqs, stream) : launch_decode<64, 2>(a, num_seqs, stream);
@@ -1539,11 +1539,11 @@ Q3_EXPORT int q3_general_attention_4bit(int dtype, const void* q, long q_stride,
                                         int max_pages, int num_seqs, const int* token_seq, const int* places, void* out, float* mid_o,
                                         float* mid_ml, int slices, int tokens, int nq, int nkv, int D, int ps, float scale, int window,
                                         cudaStream_t stream) {
+  if (tokens < 1) return Q3_OK;
   if (!q || !pages || !block_table || !token_seq || !places || !out || nq < 1 || nkv < 1 || nq % nkv || !q4_sizes_ok(D, ps) || max_pages < 1 ||
       slices < 0 || (slices > 0 && (!mid_o || !mid_ml)))
     return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
-  if (tokens < 1) return Q3_OK;
   if ((long)nkv * ((nq / nkv + GEN_HEADS - 1) / GEN_HEADS) > 65535 || slices > 65535 || (long)tokens * nq > 0x7fffffffL ||
       (reinterpret_cast<uintptr_t>(pages) & 15))
     return Q3_ERR_UNSUPPORTED;

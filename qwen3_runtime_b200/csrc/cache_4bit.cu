@@ -435,7 +435,7 @@ struct Evict {
   const int *block_table, *kv_lens;
   int max_pages, num_pages, num_seqs, nkv, ps, ps_shift, keep, first, recent, cap, max_len;
   unsigned char* pages;
-  int D, G, wide;
+  int D, G, wide, fours;  // rows of codes in pieces of 16 bytes; sums and positions in fours
   float* mass;
   int* places;
   uint32_t* spill;  // null, or [pairs][max_len]: the keys when they do not fit shared memory
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(EVICT_THREADS, 1) evict_select_kernel(Evict a)
     keys[i] = there && place < a.first ? 0xFFFFFFFFu : key;
     if (kept_places) place_s[i] = there ? place : INT_MIN;
   };
-  if (a.ps % 4 == 0) {  // four neighbours lie in one page
+  if (a.fours) {  // four neighbours lie in one page, at a multiple of 16 bytes
     for (int i = 4 * tid; i < n; i += 4 * threads) {
       const EvictRow at(a, bt, i);
       float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -669,11 +669,12 @@ Q3_EXPORT int q3_store_4bit(int dtype, const void* qkv, int row_stride, void* q_
                             const int* positions, const int* slots, const int* token_seq, const int* block_table, int max_pages,
                             int num_seqs, void* pages, int num_pages, int ps, int num_tokens, int write_kv, int pairing, float* mass,
                             int* places, int* error_word, cudaStream_t stream) {
+  if (num_tokens < 1) return Q3_OK;  // (tensors of nothing have no address)
   if (!qkv || !q_out || !positions || nq < 1 || nkv < 1 || pairing < 0 || pairing > 1 || !q4_sizes_ok(D, ps)) return Q3_ERR_ARGUMENT;
   if (cos_t && (max_pos < 1 || !sin_t || rot_half < 1 || 2 * rot_half > D)) return Q3_ERR_ARGUMENT;
   if (write_kv && (!token_seq || !block_table || !pages || max_pages < 1)) return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
-  if (num_tokens == 0) return Q3_OK;
+  if (write_kv && !q4_aligned(pages)) return Q3_ERR_UNSUPPORTED;
   Store a{q_w, k_w, cos_t, sin_t, eps, rot_half, max_pos, pairing, positions, slots, token_seq, block_table,
           max_pages, num_pages, num_seqs, ps, write_kv, (unsigned char*)pages, mass, places, error_word};
   const int G = q4_groups(D), tph = D / 16;
@@ -718,10 +719,10 @@ Q3_EXPORT int q3_store_4bit(int dtype, const void* qkv, int row_stride, void* q_
 Q3_EXPORT int q3_unpack_4bit(int dtype, const void* pages, int num_pages, int nkv, int D, int ps, const int* block_table, int max_pages,
                              const int* kv_lens, int num_seqs, int max_len, const int* cu_seqlens, int count, int width, int fill,
                              void* k_out, void* v_out, int* table_out, cudaStream_t stream) {
+  if (count < 1 || width < 1) return Q3_OK;
   if (!pages || !block_table || !kv_lens || !k_out || !v_out || nkv < 1 || max_pages < 1 || !q4_sizes_ok(D, ps)) return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
-  if (count < 1 || width < 1) return Q3_OK;
-  if (count > 65535) return Q3_ERR_UNSUPPORTED;
+  if (count > 65535 || !q4_aligned(pages) || !q4_aligned(k_out) || !q4_aligned(v_out)) return Q3_ERR_UNSUPPORTED;
   if ((long)width * nkv > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
   const Unpack a{(const unsigned char*)pages, num_pages, nkv, ps, block_table, kv_lens, cu_seqlens, max_pages, num_seqs, max_len, width, fill,
                  table_out};
@@ -734,17 +735,17 @@ Q3_EXPORT int q3_unpack_4bit(int dtype, const void* pages, int num_pages, int nk
 Q3_EXPORT int q3_evict_4bit(void* pages, int num_layers, int num_pages, int nkv, int D, int ps, float* mass, int* places,
                             const int* block_table, int max_pages, const int* kv_lens, int num_seqs, int max_len, int keep, int first,
                             int recent, int cap, void* spill, int* lists, cudaStream_t stream) {
+  if (num_seqs < 1 || num_layers < 1 || max_len <= keep) return Q3_OK;
   if (!pages || !mass || !places || !block_table || !kv_lens || !lists || nkv < 1 || max_pages < 1 || !q4_sizes_ok(D, ps))
     return Q3_ERR_ARGUMENT;
   if (keep < 1 || first < 0 || recent < 0 || (long)first + recent > keep || cap < 1 || max_len > (long)max_pages * ps) return Q3_ERR_ARGUMENT;
   if (max_len > EVICT_KEYS && !spill) return Q3_ERR_ARGUMENT;
-  if (num_seqs < 1 || num_layers < 1 || max_len <= keep) return Q3_OK;
   if (cap < (keep < max_len - keep ? keep : max_len - keep)) return Q3_ERR_ARGUMENT;
-  if (num_seqs > 65535 || num_layers > 65535 || (long)num_seqs * nkv > 65535) return Q3_ERR_UNSUPPORTED;
+  if (num_seqs > 65535 || num_layers > 65535 || (long)num_seqs * nkv > 65535 || !q4_aligned(pages)) return Q3_ERR_UNSUPPORTED;
   int shift = 0;
   while ((1 << shift) < ps) ++shift;
   Evict a{block_table, kv_lens, max_pages, num_pages, num_seqs, nkv, ps, (1 << shift) == ps ? shift : -1, keep, first, recent, cap, max_len,
-          (unsigned char*)pages, D, q4_groups(D), (D / 2) % 16 == 0, mass, places, max_len > EVICT_KEYS ? (uint32_t*)spill : nullptr, lists};
+          (unsigned char*)pages, D, q4_groups(D), (D / 2) % 16 == 0, ps % 4 == 0 && q4_aligned(mass) && q4_aligned(places), mass, places, max_len > EVICT_KEYS ? (uint32_t*)spill : nullptr, lists};
   static bool once[Q3_MAX_DEVICES];
   const int dev = q3_current_device();
   if (!once[dev]) {

@@ -2103,8 +2103,9 @@ class CudaOps:
                               f"(got head_dim={head_dim}, page_size={page_size}, num_kv_heads={num_kv_heads})")
         shape, table = pages.shape, block_table.shape  # (each read of a tensor's fields costs: once)
         if (pages.dtype != torch.uint8 or (len(shape) != 3 and not (layers and len(shape) == 4)) or shape[-1] != record
-                or shape[-2] != num_kv_heads or not pages.is_contiguous()):
-            raise KernelError(f"{what}: pages are dense uint8 [pages, {num_kv_heads}, {record}], got {pages.dtype} {tuple(shape)}")
+                or shape[-2] != num_kv_heads or not pages.is_contiguous() or pages.data_ptr() & 15):
+            raise KernelError(f"{what}: pages are dense uint8 [pages, {num_kv_heads}, {record}] that begin at a multiple of 16 bytes, "
+                              f"got {pages.dtype} {tuple(shape)}")
         if block_table.dtype != torch.int32 or len(table) != 2 or not block_table.is_contiguous() or table[1] < 1:
             raise KernelError(f"{what}: the block table is dense int32 [sequences, pages], at least one page wide")
         if kv_lens is not None and (kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous() or kv_lens.numel() < table[0]):
@@ -2201,8 +2202,8 @@ class CudaOps:
                              window=None, decode_slices=None, lse=None):
         """:meth:`paged_attention` over a cache in 4 bits.  A sequence's tokens are the first ``kv_lens`` places of its cache and the
         step's tokens the last of them (``step.kv_lens`` and ``step.host_kv_lens`` count places: without evicted tokens, positions).
-        Single tokens of bfloat16 heads of 64, 128 or 256 read the numbers as they are, on the tensor cores; float32, and single tokens
-        of other sizes, on the FMA pipes (csrc/attention_4bit.cu).  bfloat16 portions of prompts have their sequences' pages unpacked
+        Single tokens of bfloat16 heads of 64, 128 or 256 read the numbers as they are, on the tensor cores; float32, single tokens
+        of other sizes, and rows that do not begin at 16 bytes, on the FMA pipes (csrc/attention_4bit.cu).  bfloat16 portions of prompts have their sequences' pages unpacked
         once (values rounded to bfloat16) and go through the kernels for wide pages.  ``step.positions`` are places here.
         ``lse`` (float32 ``[T, heads]``, steps of single tokens of those sizes): gets the logarithm of each row's sum."""
         what = "paged_attention_4bit"
@@ -2211,8 +2212,9 @@ class CudaOps:
         if H % G or q.dtype != dtype or len(rows) != 2 or rows[1] != H * D or not out.is_contiguous():
             raise KernelError(f"{what}: out is dense [tokens, heads * head_dim] of the queries' type, heads a multiple of kv heads")
         T = rows[0]
-        if len(shape) != 2 or shape[0] < T or shape[1] < H * D or q_stride < H * D or T != step.num_tokens:
-            raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step")
+        if (len(shape) != 2 or shape[0] < T or shape[1] < H * D or q_stride < H * D or T != step.num_tokens
+                or q.stride() != (q_stride if shape[0] > 1 else q.stride(0), 1)):
+            raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step, q_stride apart")
         self._check_here(what, q, out, lse)
         room = max_pages * page_size
         if step.max_kv_len > room or step.num_seqs > table_rows:
@@ -2229,7 +2231,8 @@ class CudaOps:
             return self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, None, step.num_seqs, max_len,
                                      decode_slices or self.decode_slices_4bit(step.host_kv_lens, G, D, window, H // G), out, page_size, scale,
                                      window, step.kv_longest, lse)
-        if dtype == torch.float32 or (step.decode_only and not fast):
+        aligned = q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0  # what the kernels for wide pages go by
+        if dtype == torch.float32 or (step.decode_only and not fast) or not aligned:
             return self._general_4bit(q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window)
         # portions of prompts (and single tokens beside them): their sequences' pages unpacked, the kernels for wide pages
         n = -(-max_len // page_size)
@@ -2367,8 +2370,9 @@ class CudaOps:
         T = step.num_tokens
         if num_heads % num_kv_heads or q_stride % 8 or q.data_ptr() % 16:
             raise KernelError(f"{what}: heads are a multiple of kv heads, rows of queries begin at multiples of 16 bytes")
-        if q.dim() != 2 or q.size(0) < T or q.size(1) < num_heads * head_dim or q_stride < num_heads * head_dim:
-            raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step")
+        if (q.dim() != 2 or q.size(0) < T or q.size(1) < num_heads * head_dim or q_stride < num_heads * head_dim
+                or q.stride() != (q_stride if q.size(0) > 1 else q.stride(0), 1)):
+            raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step, q_stride apart")
         if observe is not None and observe < 1:
             raise KernelError(f"{what}: observe at least one token, or None for all")
         if lse is not None and (lse.dtype != torch.float32 or lse.dim() != 2 or lse.size(0) != T or lse.size(1) != num_heads or not lse.is_contiguous()):
@@ -2408,7 +2412,7 @@ class CudaOps:
         """Cuts every sequence that holds more than ``keep`` tokens to ``keep``, per kv head: the positions below ``first`` and the last
         ``recent`` ones stay, and of the others those with the largest ``mass`` (equal sums: the lower place).  Kept tokens behind the
         first ``keep`` places fill the holes in front, in order; ``mass`` and ``places`` move along.  What lies behind ``keep`` afterwards
-        is nobody's.  ``max_kv_len``: no sequence is longer.  ``pages``, ``mass`` and ``places`` may have a first axis of layers, all of
+        is nobody's.  A page belongs to one sequence.  ``max_kv_len``: no sequence is longer.  ``pages``, ``mass`` and ``places`` may have a first axis of layers, all of
         one block table."""
         what = "evict_4bit"
         self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens, layers=True)

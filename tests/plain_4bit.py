@@ -153,9 +153,9 @@ def step_of(new, lens, page, device="cuda", captured_width=0):
     dev = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
     singles = [b for b, n in enumerate(new) if n == 1]
     return SimpleNamespace(
-        num_tokens=cu[-1], num_seqs=len(new), cu_seqlens=dev(cu), kv_lens=dev(list(lens)), kv_longest=dev([max(lens)]),
+        num_tokens=cu[-1], num_seqs=len(new), cu_seqlens=dev(cu), kv_lens=dev(list(lens)), kv_longest=dev([max(lens, default=0)]),
         token_seq=dev([b for b, n in enumerate(new) for _ in range(n)]),
-        positions=dev([L - n + i for n, L in zip(new, lens) for i in range(n)]), max_query_len=max(new), max_kv_len=max(lens),
+        positions=dev([L - n + i for n, L in zip(new, lens) for i in range(n)]), max_query_len=max(new, default=0), max_kv_len=max(lens, default=0),
         decode_only=all(n == 1 for n in new), single_seqs=dev(singles), num_single=len(singles), host_cu_seqlens=cu,
         host_kv_lens=list(lens), captured_width=captured_width, choices={})
 

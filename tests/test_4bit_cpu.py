@@ -125,7 +125,9 @@ def attention_args(new=(1, 1), lens=(20, 3), H=4, G=2, D=128, page=16, dtype=tor
     (dict(dtype=torch.float32, lse=torch.zeros((2, 4))), "log sums come from"), (dict(pages=cache(page=8)), "dense uint8"),
     (dict(block_table=i32([[0], [1]])), "do not fit"), (dict(block_table=i32([[0, 1]])), "do not fit"),
     (dict(q=torch.zeros((1, 512), dtype=torch.bfloat16)), "a row per token"), (dict(q=torch.zeros((2, 504), dtype=torch.bfloat16)), "a row per token"),
-    (dict(q_stride=504), "a row per token")])
+    (dict(q_stride=504), "a row per token"), (dict(q_stride=1024), "a row per token"),
+    (dict(q=torch.zeros((2, 1024), dtype=torch.bfloat16)[:, ::2], q_stride=1024), "a row per token"),
+    (dict(pages=torch.zeros(cache().numel() + 1, dtype=torch.uint8)[1:].view(cache().shape)), "multiple of 16 bytes")])
 def test_attention_that_is_refused(ops, change, match):
     args = attention_args(**change)
     with pytest.raises(KernelError, match=match):
@@ -136,6 +138,7 @@ def test_attention_that_is_refused(ops, change, match):
 @pytest.mark.parametrize("change,match", [
     (dict(mass=torch.zeros((4, 2, 8))), "sums"), (dict(mass=torch.zeros((4, 2, 16)).double()), "sums"), (dict(observe=0), "observe"),
     (dict(lse=torch.zeros((2, 5))), "log sums"), (dict(num_heads=5), "multiple"), (dict(q_stride=516), "16 bytes"),
+    (dict(q_stride=520), "a row per token"),
     (dict(q=torch.zeros((1, 512), dtype=torch.bfloat16)), "a row per token"), (dict(block_table=i32([[0, 1]])), "do not fit")])
 def test_sums_that_are_refused(ops, change, match):
     args = {**attention_args(), "mass": torch.zeros((4, 2, 16)), **change}

@@ -34,14 +34,13 @@ def queries(T, H, D, seed, dtype=BF16, extra=0):
     return torch.randn((T, H * D + extra), generator=g).to(dtype)
 
 
-def score_error(q, cache, b, scale, base=0.0):
-    """Bound of a score's error ``[T, H]``: D additions of float32 to sums of |q| s (16 + base) -- ``base`` 16 where numbers are summed as
-    1 + n / 16 -- whatever their order, and 2^-17 of the largest |q| where queries are held as sums of two 8-bit floats."""
-    H, D = q.shape[1:]
+def score_error(q, cache, b, scale):
+    """Bound of a score's error ``[T, H]``: D additions of float32 to sums of |q| s n, n at most 15, and of |q z|, whatever their order."""
+    D = q.shape[2]
     s = cache.k[b][1].double().nan_to_num().amax()
     z = cache.k[b][2].double().abs().nan_to_num().amax()
     total = q.double().abs().sum(-1)
-    return scale * (2.0 ** -23 * (D + 8) * total * (s * (16 + base) + z) + D * 15 * s * q.double().abs().amax(-1) * 2.0 ** -17)
+    return scale * 2.0 ** -23 * (D + 8) * total * (s * 16 + z)
 
 
 def attend(ops, c, q, new, lens, H, scale, *, window=None, lse=False, slices=None, dtype=BF16, table=None, step=None):
@@ -397,7 +396,7 @@ def check_mass(got, q, c, new, lens, scale, observe, start=None, dtype=BF16, tim
     tol = want.abs() * 2.0 ** -23
     t = 0
     for b, (n, L) in enumerate(zip(new, lens)):
-        err = float(score_error(q[t:t + n], c, b, scale, base=16.0).max()) + 2.0 ** -20 * 12
+        err = float(score_error(q[t:t + n], c, b, scale).max()) + 2.0 ** -20 * 12
         w = weights[b][max(0, n - (observe or n)):].view(-1, c.G, R, L).sum((0, 2)) * times  # [G, L]
         for j in range(L):
             at = (int(c.table[b, j // c.page]), slice(None), j % c.page)
@@ -632,3 +631,140 @@ def test_a_cache_that_is_written_attended_summed_and_cut(ops):
     for h in range(G):
         want = torch.tensor([r[3] for r in rows[h]], dtype=torch.float64)
         assert bool(((m[h] - want).abs() <= 1e-4 * want).all())
+
+
+@pytest.mark.parametrize("page,D", [(48, 128), (80, 64), (160, 128), (256, 256), (67, 128)])
+def test_pages_larger_than_what_a_block_takes_at_a_time(ops, page, D):
+    """A block's next keys lie in the same page, or further on than one page behind."""
+    H, G, lens = 8, 2, [1, 47, 48, 161, 700]
+    c = p4.Cache(lens, G, D, page, seed=page)
+    q = queries(len(lens), H, D, 5)
+    rows, new = q.view(-1, H, D), [1] * len(lens)
+    for slices in (None, 3, -3):
+        got, lse = attend(ops, c, q, new, lens, H, D ** -0.5, lse=True, slices=slices)
+        check_rows(got, rows, c, new, lens, D ** -0.5)
+        check_mass(mass_of(ops, c, q, new, lens, H, D ** -0.5, 1, lse=lse.cuda()), rows, c, new, lens, D ** -0.5, 1)
+    check_mass(mass_of(ops, c, q, new, lens, H, D ** -0.5, 1), rows, c, new, lens, D ** -0.5, 1)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 1, 20]])
+@pytest.mark.parametrize("shift,extra", [(0, 4), (1, 0), (1, 3), (4, 8)])
+def test_rows_of_queries_that_begin_anywhere(ops, new, shift, extra):
+    """``shift`` elements behind a multiple of 16 bytes, rows ``extra`` elements apart."""
+    H, G, D, lens = 8, 2, 128, [9, 40, 33]
+    c = p4.Cache(lens, G, D, 16, seed=3)
+    q = queries(sum(new), H, D, 4)
+    T, width = q.shape[0], H * D + extra
+    dev = torch.zeros(shift + T * width, dtype=BF16, device="cuda")[shift:].view(T, width)
+    dev[:, : H * D] = q.cuda()
+    out = torch.zeros(2 + T * H * D, dtype=BF16, device="cuda")[2:].view(T, H * D) if shift == 1 else torch.zeros_like(q, device="cuda")
+    ops.paged_attention_4bit(dev, width, num_heads=H, pages=c.pages.cuda(), block_table=c.table.cuda(), out=out, scale=D ** -0.5,
+                             step=p4.step_of(new, lens, 16), **sizes(c))
+    check_rows(out.cpu().view(T, H, D), q.view(T, H, D), c, new, lens, D ** -0.5, wide=True)
+
+
+@pytest.mark.parametrize("slices", [1, 4, -4])
+def test_sequences_without_keys(ops, slices):
+    """Length zero: results are zero, log sums minus infinity, no sum moves; the others are as ever."""
+    H, G, D, lens, page = 8, 2, 128, [20, 700, 31], 16
+    c = p4.Cache(lens, G, D, page, seed=6)
+    q = queries(3, H, D, 5)
+    step = p4.step_of([1] * 3, lens, page)
+    step.kv_lens[0] = 0
+    got, lse = attend(ops, c, q, [1] * 3, lens, H, D ** -0.5, lse=True, slices=slices, step=step)
+    assert bool((got[0] == 0).all()) and bool((lse[0] == -math.inf).all())
+    whole = attend(ops, c, q, [1] * 3, lens, H, D ** -0.5, slices=slices)
+    assert torch.equal(got[1:], whole[1:])
+    for sums in (lse.cuda(), None):
+        mass = torch.zeros((c.pages.shape[0], G, page), device="cuda")
+        ops.attention_mass_4bit(q.cuda(), H * D, num_heads=H, pages=c.pages.cuda(), mass=mass, block_table=c.table.cuda(), scale=D ** -0.5,
+                                step=step, lse=sums, **sizes(c))
+        assert bool((mass[c.table[0, :2].long().cuda()] == 0).all()) and abs(float(mass.sum()) - 2 * H) < 1e-2
+
+
+def test_two_streams_at_once(ops):
+    """Unequal steps under way together, each with workspaces of its own."""
+    H, G, D = 8, 2, 128
+    caches = [p4.Cache([5000, 1200], G, D, 16, seed=1), p4.Cache([3000, 64, 900], G, D, 16, seed=2)]
+    made, alone = [], []
+    for i, c in enumerate(caches):
+        q = queries(len(c.lens), H, D, i)
+        made.append((c, q.cuda(), c.pages.cuda(), c.table.cuda(), p4.step_of([1] * len(c.lens), c.lens, 16), torch.cuda.Stream()))
+        alone.append(attend(ops, c, q, [1] * len(c.lens), c.lens, H, D ** -0.5, slices=-9))
+    outs = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, (c, q, pages, table, step, stream) in enumerate(made):
+            with torch.cuda.stream(stream):
+                out = torch.empty_like(q)
+                ops.paged_attention_4bit(q, H * D, num_heads=H, pages=pages, block_table=table, out=out, scale=D ** -0.5, step=step,
+                                         decode_slices=-9, **sizes(c))
+                outs[i].append(out)
+    torch.cuda.synchronize()
+    for got, want in zip(outs, alone):
+        assert all(torch.equal(x.cpu().view(want.shape), want) for x in got)
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("keep", [40, 700])
+def test_a_captured_eviction(ops, keep, shift):
+    """Replayed with other lengths, some within the budget; sums and positions that do not begin at 16 bytes."""
+    G, D, page, lens = 2, 64, 16, [1500, 64, 900]
+    c = p4.Cache(lens, G, D, page, seed=9)
+    g = torch.Generator().manual_seed(1)
+    shape = (c.pages.shape[0], G, page)
+    count = shape[0] * G * page
+    mass = torch.rand(shape, generator=g)
+    places = torch.full(shape, -1, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        for j in range(n):
+            places[int(c.table[b, j // page]), :, j % page] = j
+    dev = [c.pages.cuda(), torch.zeros(count + shift, device="cuda")[shift:].view(shape),
+           torch.zeros(count + shift, dtype=torch.int32, device="cuda")[shift:].view(shape)]
+    table, kv_lens = c.table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    run = lambda: ops.evict_4bit(pages=dev[0], mass=dev[1], places=dev[2], block_table=table, kv_lens=kv_lens, max_kv_len=1500,  # noqa: E731
+                                 keep=keep, first=4, recent=10, **sizes(c))
+    graph = torch.cuda.CUDAGraph()
+    run()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        run()
+    for now in (lens, [keep + 1, 20, 0], [1499, 64, keep]):
+        for d, x in zip(dev, (c.pages, mass, places)):
+            d.copy_(x)
+        kv_lens.copy_(torch.tensor(now, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        for b, n in enumerate(now):
+            rows = c.table[b].long()
+            for h in range(G):
+                m, p = (x[rows, h].flatten()[:n].tolist() for x in (mass, places))
+                src = p4.evict(m, p, keep, 4, 10) if n > keep else list(range(n))
+                assert dev[2].cpu()[rows, h].flatten()[: len(src)].tolist() == [p[i] for i in src]
+                assert dev[1].cpu()[rows, h].flatten()[: len(src)].tolist() == [m[i] for i in src]
+
+
+def test_steps_of_nothing(ops):
+    G, D, page = 2, 128, 16
+    c = p4.Cache([20], G, D, page)
+    pages, table = c.pages.cuda(), c.table.cuda()
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    qkv = torch.zeros((0, (4 + 2 * G) * D), dtype=BF16, device="cuda")
+    ops.qk_norm_rope_store_4bit(qkv, num_heads=4, q_weight=None, k_weight=None, eps=0.0, cos=None, sin=None, positions=none, token_seq=none,
+                                block_table=table, pages=pages, **sizes(c))
+    k, v = ops.unpack_4bit(pages, block_table=table, kv_lens=torch.tensor([20], dtype=torch.int32, device="cuda"), max_kv_len=0, dtype=BF16, **sizes(c))
+    assert k.shape == v.shape == (0, G, page, D)
+    k, v = ops.unpack_4bit(pages, block_table=table[:0], kv_lens=none, max_kv_len=20, dtype=BF16, **sizes(c))
+    assert k.shape == v.shape == (0, G, page, D)
+    torch.cuda.synchronize()
+    assert torch.equal(pages.cpu(), c.pages)
+    for dtype in (BF16, F32):
+        step, q = p4.step_of([], [], page), torch.zeros((0, 4 * D), dtype=dtype, device="cuda")
+        out, mass = torch.empty_like(q), torch.zeros((pages.shape[0], G, page), device="cuda")
+        args = dict(num_heads=4, pages=pages, block_table=table[:0], scale=1.0, step=step, **sizes(c))
+        ops.paged_attention_4bit(q, 4 * D, out=out, **args)
+        ops.attention_mass_4bit(q, 4 * D, mass=mass, **args)
+    ops.evict_4bit(pages=pages, mass=mass, places=torch.zeros_like(mass, dtype=torch.int32), block_table=table[:0], kv_lens=none, max_kv_len=20,
+                   keep=4, first=0, recent=0, **sizes(c))
+    torch.cuda.synchronize()
+    assert torch.equal(pages.cpu(), c.pages) and not bool(mass.any())

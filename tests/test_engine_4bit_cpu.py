@@ -141,3 +141,11 @@ def test_build_model_takes_the_number_of_tokens():
     cfg = TINY["A"]["config"]
     model = build_model(cfg, DictSource(random_state(cfg, 0)), dtype="float32", device=DEV, ops=OPS, kv_bits=4, token_budget=64)
     assert model.ctx.kv_budget == TokenBudget(64)
+
+
+def test_a_budget_is_a_number_of_tokens():
+    for budget in (True, 1.5, "100"):
+        with pytest.raises(ValueError, match="number of tokens"):
+            EngineConfig(kv_bits=4, token_budget=budget)
+    with pytest.raises(ValueError, match="at least one"):
+        EngineConfig(kv_bits=4, token_budget=0)
