@@ -2204,7 +2204,8 @@ class CudaOps:
         step's tokens the last of them (``step.kv_lens`` and ``step.host_kv_lens`` count places: without evicted tokens, positions).
         Single tokens of bfloat16 heads of 64, 128 or 256 read the numbers as they are, on the tensor cores; float32, single tokens
         of other sizes, and rows that do not begin at 16 bytes, on the FMA pipes (csrc/attention_4bit.cu).  bfloat16 portions of prompts have their sequences' pages unpacked
-        once (values rounded to bfloat16) and go through the kernels for wide pages.  ``step.positions`` are places here.
+        once (values rounded to bfloat16) and go through the kernels for wide pages.  ``step.positions`` are places here.  A table entry that is no page is read nowhere; the rows of a
+        sequence that sees such a token are undefined, the others are not.
         ``lse`` (float32 ``[T, heads]``, steps of single tokens of those sizes): gets the logarithm of each row's sum."""
         what = "paged_attention_4bit"
         D, G, H, dtype, shape, rows = head_dim, num_kv_heads, num_heads, out.dtype, q.shape, out.shape

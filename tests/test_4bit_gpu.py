@@ -682,6 +682,29 @@ def test_sequences_without_keys(ops, slices):
         assert bool((mass[c.table[0, :2].long().cuda()] == 0).all()) and abs(float(mass.sum()) - 2 * H) < 1e-2
 
 
+@pytest.mark.parametrize("page", [16, 32, 5])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 20]])
+def test_entries_that_are_no_pages_are_read_nowhere(ops, page, new):
+    H, G, D, lens = 8, 2, 128, [90, 70, 60]
+    c = p4.Cache(lens, G, D, page, seed=3)
+    q = queries(sum(new), H, D, 4)
+    table = c.table.clone()
+    table[0, 0], table[0, 1] = -7, c.pages.shape[0]
+    for slices in (1, 3):
+        got, whole = (attend(ops, c, q, new, lens, H, D ** -0.5, table=t, slices=slices) for t in (table, c.table))
+        assert torch.equal(got[new[0]:], whole[new[0]:])
+    step, dev = p4.step_of(new, lens, page), q.cuda()
+    masses = []
+    for t in (table, c.table):
+        masses.append(torch.zeros((c.pages.shape[0], G, page), device="cuda"))
+        ops.attention_mass_4bit(dev, H * D, num_heads=H, pages=c.pages.cuda(), mass=masses[-1], block_table=t.cuda(), scale=D ** -0.5, step=step,
+                                **sizes(c))
+    others = c.table[1:].flatten().long().unique()
+    others = others[~torch.isin(others, c.table[0].long())].cuda()
+    assert torch.equal(masses[0][others], masses[1][others])
+    assert bool((masses[0][c.table[0, :2].long().cuda()] == 0).all()), "what the table does not name is left alone"
+
+
 def test_two_streams_at_once(ops):
     """Unequal steps under way together, each with workspaces of its own."""
     H, G, D = 8, 2, 128
