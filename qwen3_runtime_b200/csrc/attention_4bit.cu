@@ -1273,15 +1273,19 @@ template <int D, int NT> int launch_mass(const Mass& a, bool want_rows, int most
 
 // ---- attention in general -----------------------------------------------------------------------------------------------------------------
 // float32, and bfloat16 tokens whose head size or group the tiles above do not take: a block of 256 threads takes a (token, kv head, up to 8
-// of its query heads); 64 keys at a time come to shared memory as they are stored, four threads make a key's scores, a warp a head's
-// weights, a thread a channel's results.  Sums are float32 on the FMA pipes, in an order that depends on the keys' places alone: tiles
-// begin at multiples of 64, slices of 1024 keys have a softmax of their own and are joined in order, by the same block or, where the
-// launch leaves SMs idle, by a second kernel from what one block a slice has left -- the same bits, however a sequence is cut into steps
-// and batched with others.
+// of its query heads); 64 keys at a time come to shared memory as they are stored, the next ones while these are worked on; four threads
+// make a key's scores, a warp a head's weights, a thread two channels' results.  Sums are float32 on the FMA pipes, in an order that
+// depends on the keys' places alone: tiles begin at multiples of 64, slices of 256 keys have a softmax of their own and are joined in
+// order, by the same block or, where the launch leaves SMs idle, by a second kernel from what one block a slice has left -- the same bits,
+// however a sequence is cut into steps and batched with others.  What bounds it is instructions.  Slices of 512, 256, 128 keys, in us
+// (16 heads over 4 of 64, float32): 21 tokens behind up to 320 keys 20, 20, 16; 8 behind 4,096 35, 38, 44; one behind 32,768 40, 48, 63;
+// a prompt of 512 134, 139, 148.  (A tile brought without looking ahead, a division a word, a thread a channel: 35, 62, 75 and 227 at 512.)
 constexpr int GEN_THREADS = 256;
 constexpr int GEN_TILE = 64;
-constexpr int GEN_SLICE = 1024;
+constexpr int GEN_SLICE = 256;
 constexpr int GEN_HEADS = 8;
+// bytes of a token's codes and parameters in shared memory
+__host__ __device__ __forceinline__ int general_pitch(const Q4Page& L) { return (int)(L.half + L.par + 7) & ~7; }
 
 struct General {
   const unsigned char* pages;
@@ -1291,14 +1295,15 @@ struct General {
   long q_stride;
   float scale_log2;
   float *mid_o, *mid_ml;  // slices > 0: [tokens][nq][slices][D] and [tokens][nq][slices][2]
+  int tiles_at;           // byte of shared memory
 };
 
-// (m, l, o) <- its join with another's; o and b are unnormalised
+// (m, l, o) <- its join with another's; o and b are unnormalised.  The fused steps are named, so that both kernels round alike.
 __device__ __forceinline__ void join_slices(float& m, float& l, float& o, float bm, float bl, float bo) {
   const float top = fmaxf(m, bm), fa = exp2f(m - top), fb = exp2f(bm - top);
   m = top;
-  l = l * fa + bl * fb;
-  o = o * fa + bo * fb;
+  l = __fmaf_rn(l, fa, __fmul_rn(bl, fb));
+  o = __fmaf_rn(o, fa, __fmul_rn(bo, fb));
 }
 
 template <typename T>
@@ -1312,51 +1317,65 @@ __global__ void __launch_bounds__(GEN_THREADS) general_4bit_kernel(General a, co
   const int D = a.D, G = a.G, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Q4Page L(D, G, a.ps);
   float* q_s = reinterpret_cast<float*>(smem);                   // [8][D]
-  float* p_s = q_s + GEN_HEADS * D;                              // [8][64]
+  float* x_s = q_s + GEN_HEADS * D;                              // [8][64] scores
+  float* p_s = x_s + GEN_HEADS * GEN_TILE;                       // [64][8] weights
   float* f_s = p_s + GEN_HEADS * GEN_TILE;                       // [8]: what the results so far shrink by; then the slice's maximum and sum
-  float* v_s = f_s + 32;                                         // [groups of threads][8][D] at the end of a slice, else the tile's bytes
-  unsigned char* k_s = reinterpret_cast<unsigned char*>(v_s);    // [64][half + par] of keys, then of values
-  const int pitch = L.half + L.par, words = pitch / 4;
+  float* v_s = f_s + 32;                                         // [groups of threads][8][D] at the end of a slice
+  unsigned char* k_s = smem + a.tiles_at;                        // two tiles: 64 rows of keys' codes and parameters, then of values
+  const int pitch = general_pitch(L), bytes = 2 * GEN_TILE * pitch;
   const int seq = a.token_seq[t], place = a.places[t];
   const bool there = seq >= 0 && seq < a.num_seqs && place >= 0 && place / a.ps < a.max_pages;
   const int last = there ? place : -1, lo = a.window > 0 ? max(0, last - a.window + 1) : 0;
   const int* bt = a.block_table + (long)(there ? seq : 0) * a.max_pages;
   for (int i = tid; i < heads * D; i += GEN_THREADS) q_s[i] = to_f32(q[t * a.q_stride + (long)h0 * D + i]) * a.scale_log2;
-  // a thread owns channel c of the keys g, g + parts, g + 2 parts ... of each tile
-  const int parts = GEN_THREADS / D, c = tid % D, part = tid / D;
+  // a thread owns channels c and c + 1, which share a byte, of the keys g, g + parts, g + 2 parts ... of each tile
+  const int parts = 2 * GEN_THREADS / D, c = 2 * (tid % (D / 2)), part = tid / (D / 2);
   const bool owner = part < parts;
-  const int c_group = c / (D / G), c_in = c % (D / G), c_byte = 4 * ((c_in / 8) * G + c_group) + (c_in % 8) / 2, c_shift = 4 * (c_in % 2);
-  float M[GEN_HEADS], S[GEN_HEADS], O[GEN_HEADS];
+  const int c_group = c / (D / G), c_in = c % (D / G), c_byte = 4 * ((c_in / 8) * G + c_group) + (c_in % 8) / 2;
+  // two threads bring a row (64 of keys, then 64 of values), 8 bytes of codes or a group's parameters in turn, a tile ahead of its use, into
+  // two buffers in turn; what is not there is zero
+  const int my_row = tid & (2 * GEN_TILE - 1), my_half = tid >> 7, my_v = my_row >= GEN_TILE;
+  auto fetch = [&](int base, int stop) {
+    const int key = base + (my_row & (GEN_TILE - 1));
+    const unsigned char *codes = a.pages, *pars = a.pages;
+    int there = 0;
+    if (key >= lo && key < stop) {
+      const int pi = key / a.ps, page = bt[pi];
+      if ((uint32_t)page < (uint32_t)a.num_pages) {
+        const long pr = key - pi * a.ps;
+        const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
+        codes = rec + (my_v ? L.values : 0) + pr * L.half;
+        pars = rec + (my_v ? L.vpar : L.kpar) + pr * L.par;
+        there = 1;
+      }
+    }
+    const uint32_t dst = smem_addr(k_s) + (base / GEN_TILE & 1) * bytes + my_row * pitch;
+    for (int at = 8 * my_half; at < L.half; at += 16) cp_async8(dst + at, codes + at * there, 8 * there);
+    for (int at = 4 * my_half; at < L.par; at += 8) cp_async4(dst + L.half + at, pars + at * there, 4 * there);
+    cp_async_commit();
+  };
+  float M[GEN_HEADS], S[GEN_HEADS], O[GEN_HEADS][2];
 #pragma unroll
-  for (int h = 0; h < GEN_HEADS; ++h) M[h] = MINUS_BIG, S[h] = 0.f, O[h] = 0.f;
+  for (int h = 0; h < GEN_HEADS; ++h) M[h] = MINUS_BIG, S[h] = 0.f, O[h][0] = O[h][1] = 0.f;
   const int slice0 = a.slices > 0 ? blockIdx.z : lo / GEN_SLICE, slice1 = a.slices > 0 ? blockIdx.z : last / GEN_SLICE;
+  const int stop = min(last + 1, (slice1 + 1) * GEN_SLICE);
+  fetch(max(lo, slice0 * GEN_SLICE) / GEN_TILE * GEN_TILE, stop);
   for (int slice = slice0; slice <= slice1 && last >= 0; ++slice) {
     const int begin = max(lo, slice * GEN_SLICE) / GEN_TILE * GEN_TILE, end = min(last + 1, (slice + 1) * GEN_SLICE);
-    float o[GEN_HEADS];
+    float o[GEN_HEADS][2];
 #pragma unroll
-    for (int h = 0; h < GEN_HEADS; ++h) o[h] = 0.f;
+    for (int h = 0; h < GEN_HEADS; ++h) o[h][0] = o[h][1] = 0.f;
     float m = MINUS_BIG, l = 0.f;  // warp h: of head h, the same in every lane
     for (int base = begin; base < end; base += GEN_TILE) {
       __syncthreads();
-      for (int i = tid; i < 2 * GEN_TILE * words; i += GEN_THREADS) {
-        const int row = i / words, w = i - row * words, is_v = row >= GEN_TILE, key = base + row - is_v * GEN_TILE;
-        uint32_t x = 0;
-        if (key >= lo && key < end) {
-          const int pi = key / a.ps, page = bt[pi], pr = key - pi * a.ps;
-          if ((uint32_t)page < (uint32_t)a.num_pages) {
-            const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
-            const bool par = 4 * w >= L.half;
-            x = *reinterpret_cast<const uint32_t*>(rec + (par ? (is_v ? L.vpar : L.kpar) + (long)pr * L.par + 4 * w - L.half
-                                                               : (is_v ? L.values : 0) + (long)pr * L.half + 4 * w));
-          }
-        }
-        reinterpret_cast<uint32_t*>(k_s)[i] = x;
-      }
+      fetch(base + GEN_TILE, stop);
+      cp_async_wait<1>();
       __syncthreads();
+      const unsigned char* tile = k_s + (base / GEN_TILE & 1) * bytes;
       {  // four threads a key, each every fourth word; 8 channels of a word in order, the four threads' sums in pairs
         const int key = tid >> 2, sub = tid & 3;
-        const uint32_t* row = reinterpret_cast<const uint32_t*>(k_s + key * pitch);
-        const uint32_t* par = reinterpret_cast<const uint32_t*>(k_s + key * pitch + L.half);
+        const uint32_t* row = reinterpret_cast<const uint32_t*>(tile + key * pitch);
+        const uint32_t* par = reinterpret_cast<const uint32_t*>(tile + key * pitch + L.half);
         float x[GEN_HEADS];
 #pragma unroll
         for (int h = 0; h < GEN_HEADS; ++h) x[h] = 0.f;
@@ -1380,15 +1399,15 @@ __global__ void __launch_bounds__(GEN_THREADS) general_4bit_kernel(General a, co
         for (int h = 0; h < GEN_HEADS; ++h) {
           x[h] += __shfl_xor_sync(0xffffffffu, x[h], 1);
           x[h] += __shfl_xor_sync(0xffffffffu, x[h], 2);
-          if (sub == (h & 3) && h < heads) p_s[h * GEN_TILE + key] = seen ? x[h] : -INFINITY;
+          if (sub == (h & 3) && h < heads) x_s[h * GEN_TILE + key] = seen ? x[h] : -INFINITY;
         }
       }
       __syncthreads();
       if (warp < heads) {
-        const float x0 = p_s[warp * GEN_TILE + lane], x1 = p_s[warp * GEN_TILE + 32 + lane];
+        const float x0 = x_s[warp * GEN_TILE + lane], x1 = x_s[warp * GEN_TILE + 32 + lane];
         const float top = fmaxf(m, warp_max(fmaxf(x0, x1))), f = exp2f(m - top);
         const float p0 = exp2f(x0 - top), p1 = exp2f(x1 - top);
-        p_s[warp * GEN_TILE + lane] = p0, p_s[warp * GEN_TILE + 32 + lane] = p1;
+        p_s[GEN_HEADS * lane + warp] = p0, p_s[GEN_HEADS * (lane + 32) + warp] = p1;
         l = l * f + warp_sum(p0 + p1);
         m = top;
         if (lane == 0) f_s[warp] = f;
@@ -1397,15 +1416,18 @@ __global__ void __launch_bounds__(GEN_THREADS) general_4bit_kernel(General a, co
       if (owner) {
 #pragma unroll
         for (int h = 0; h < GEN_HEADS; ++h)
-          if (h < heads) o[h] *= f_s[h];
-        const unsigned char* rows = k_s + GEN_TILE * pitch;
+          if (h < heads) o[h][0] *= f_s[h], o[h][1] *= f_s[h];
+        const unsigned char* rows = tile + GEN_TILE * pitch;
         for (int key = part; key < GEN_TILE; key += parts) {
           const unsigned char* row = rows + key * pitch;
-          const uint32_t par = *reinterpret_cast<const uint32_t*>(row + L.half + 4 * c_group);
-          const float v = q4_z(par) + (float)((row[c_byte] >> c_shift) & 15) * q4_s(par);
+          const uint32_t par = *reinterpret_cast<const uint32_t*>(row + L.half + 4 * c_group), code = row[c_byte];
+          const float v0 = q4_z(par) + (float)(code & 15) * q4_s(par), v1 = q4_z(par) + (float)(code >> 4) * q4_s(par);
+          float w[GEN_HEADS];
+          *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(p_s + GEN_HEADS * key);
+          if (heads > 4) *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(p_s + GEN_HEADS * key + 4);
 #pragma unroll
           for (int h = 0; h < GEN_HEADS; ++h)
-            if (h < heads) o[h] = fmaf(p_s[h * GEN_TILE + key], v, o[h]);
+            if (h < heads) o[h][0] = fmaf(w[h], v0, o[h][0]), o[h][1] = fmaf(w[h], v1, o[h][1]);
         }
       }
     }
@@ -1414,7 +1436,7 @@ __global__ void __launch_bounds__(GEN_THREADS) general_4bit_kernel(General a, co
     if (owner) {
 #pragma unroll
       for (int h = 0; h < GEN_HEADS; ++h)
-        if (h < heads) v_s[(part * GEN_HEADS + h) * D + c] = o[h];
+        if (h < heads) *reinterpret_cast<float2*>(v_s + (part * GEN_HEADS + h) * D + c) = make_float2(o[h][0], o[h][1]);
     }
     if (warp < heads && lane == 0) f_s[8 + 2 * warp] = m, f_s[9 + 2 * warp] = l;
     __syncthreads();
@@ -1422,22 +1444,29 @@ __global__ void __launch_bounds__(GEN_THREADS) general_4bit_kernel(General a, co
 #pragma unroll
       for (int h = 0; h < GEN_HEADS; ++h)
         if (h < heads) {
-          float y = v_s[h * D + c];
-          for (int g = 1; g < parts; ++g) y += v_s[(g * GEN_HEADS + h) * D + c];
-          join_slices(M[h], S[h], O[h], f_s[8 + 2 * h], f_s[9 + 2 * h], y);
+          float2 y = *reinterpret_cast<const float2*>(v_s + h * D + c);
+          for (int g = 1; g < parts; ++g) {
+            const float2 z = *reinterpret_cast<const float2*>(v_s + (g * GEN_HEADS + h) * D + c);
+            y.x += z.x, y.y += z.y;
+          }
+          float m = M[h], l = S[h];
+          join_slices(m, l, O[h][0], f_s[8 + 2 * h], f_s[9 + 2 * h], y.x);
+          join_slices(M[h], S[h], O[h][1], f_s[8 + 2 * h], f_s[9 + 2 * h], y.y);
         }
     }
   }
+  cp_async_wait<0>();  // (the tile behind the last one: zeros)
   if (owner && part == 0) {
 #pragma unroll
     for (int h = 0; h < GEN_HEADS; ++h)
       if (h < heads) {
         if (a.slices > 0) {
           const long at = ((long)t * a.nq + h0 + h) * a.slices + blockIdx.z;
-          a.mid_o[at * D + c] = O[h];
+          a.mid_o[at * D + c] = O[h][0], a.mid_o[at * D + c + 1] = O[h][1];
           if (c == 0) a.mid_ml[2 * at] = M[h], a.mid_ml[2 * at + 1] = S[h];
         } else {
-          out[((long)t * a.nq + h0 + h) * D + c] = from_f32<T>(last >= 0 ? O[h] / S[h] : 0.f);
+          T* y = out + ((long)t * a.nq + h0 + h) * D + c;
+          y[0] = from_f32<T>(last >= 0 ? O[h][0] / S[h] : 0.f), y[1] = from_f32<T>(last >= 0 ? O[h][1] / S[h] : 0.f);
         }
       }
   }
@@ -1451,17 +1480,29 @@ template <typename T> __global__ void general_4bit_merge_kernel(General a, T* __
   const int place = a.places[at / a.nq], lo = a.window > 0 ? max(0, place - a.window + 1) : 0;
   for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
     float M = MINUS_BIG, S = 0.f, O = 0.f;
-    for (int s = lo / GEN_SLICE; s <= place / GEN_SLICE && s < a.slices; ++s)
-      join_slices(M, S, O, a.mid_ml[2 * (at * a.slices + s)], a.mid_ml[2 * (at * a.slices + s) + 1], a.mid_o[(at * a.slices + s) * a.D + c]);
+    const int stop = place >= 0 ? min(place / GEN_SLICE + 1, a.slices) : 0;
+    for (int s0 = lo / GEN_SLICE; s0 < stop; s0 += 8) {  // eight slices' loads at a time
+      float m[8], l[8], o[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (s0 + u < stop) {
+          const long i = at * a.slices + s0 + u;
+          m[u] = a.mid_ml[2 * i], l[u] = a.mid_ml[2 * i + 1], o[u] = a.mid_o[i * a.D + c];
+        }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (s0 + u < stop) join_slices(M, S, O, m[u], l[u], o[u]);
+    }
     out[at * a.D + c] = from_f32<T>(place >= 0 ? O / S : 0.f);
   }
 }
 
-template <typename T> int launch_general(const General& a, const T* q, T* out, int tokens, cudaStream_t stream) {
+template <typename T> int launch_general(General a, const T* q, T* out, int tokens, cudaStream_t stream) {
   const Q4Page L(a.D, a.G, a.ps);
-  const int R = a.nq / a.nkv, chunks = (R + GEN_HEADS - 1) / GEN_HEADS, parts = GEN_THREADS / a.D;
-  const int tile = 2 * GEN_TILE * (L.half + L.par), shares = parts * GEN_HEADS * a.D * 4;
-  const int smem = (GEN_HEADS * (a.D + GEN_TILE) + 32) * 4 + (tile > shares ? tile : shares);
+  const int R = a.nq / a.nkv, chunks = (R + GEN_HEADS - 1) / GEN_HEADS, parts = 2 * GEN_THREADS / a.D;
+  const int tiles_at = ((GEN_HEADS * (a.D + 2 * GEN_TILE) + 32 + parts * GEN_HEADS * a.D) * 4 + 15) & ~15;
+  a.tiles_at = tiles_at;
+  const int smem = tiles_at + 2 * 2 * GEN_TILE * general_pitch(L);
   static bool once[Q3_MAX_DEVICES];
   const int dev = q3_current_device();
   if (!once[dev]) {
@@ -1534,7 +1575,7 @@ Q3_EXPORT int q3_decode_attention_4bit(const void* q, int q_stride, const void* 
 }
 
 // `slices` 0: a block goes through all of a token's keys; else mid_o [tokens][nq][slices][D] and mid_ml [tokens][nq][slices][2] are given and
-// slices * 1024 covers the longest sequence.
+// slices * 256 covers the longest sequence.
 Q3_EXPORT int q3_general_attention_4bit(int dtype, const void* q, long q_stride, const void* pages, int num_pages, const int* block_table,
                                         int max_pages, int num_seqs, const int* token_seq, const int* places, void* out, float* mid_o,
                                         float* mid_ml, int slices, int tokens, int nq, int nkv, int D, int ps, float scale, int window,

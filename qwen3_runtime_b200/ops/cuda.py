@@ -2257,7 +2257,7 @@ class CudaOps:
                                     token_seq=step.token_seq, positions=step.positions, out=out, page_size=page_size, scale=scale,
                                     window=window, step=step)
 
-    GENERAL_SLICE = 1024  # keys with a softmax of their own (csrc/attention_4bit.cu)
+    GENERAL_SLICE = 256  # keys with a softmax of their own (csrc/attention_4bit.cu)
 
     def _general_4bit(self, q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window):
         code, T = _dtype_code(out.dtype), out.size(0)
@@ -2267,7 +2267,8 @@ class CudaOps:
         self._check_here("paged_attention_4bit", step.token_seq, step.positions)
         slices, mid_o, mid_ml = -(-max_len // self.GENERAL_SLICE), None, None
         blocks = T * G * -(-(H // G) // 8)
-        if slices < 2 or blocks >= 4 * self.SM_COUNT:  # enough blocks without: each goes through all slices
+        # enough blocks without, or more to keep of the slices than 256 MB: each block goes through all slices (the same bits)
+        if slices < 2 or blocks >= 4 * self.SM_COUNT or T * H * slices * D > 1 << 26:
             slices = 0
         else:
             mid_o = torch.empty((T, H, slices, D), dtype=torch.float32, device=out.device)

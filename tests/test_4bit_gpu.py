@@ -791,3 +791,17 @@ def test_steps_of_nothing(ops):
                    keep=4, first=0, recent=0, **sizes(c))
     torch.cuda.synchronize()
     assert torch.equal(pages.cpu(), c.pages) and not bool(mass.any())
+
+
+@pytest.mark.parametrize("D,dtype", [(64, F32), (80, BF16), (208, F32)])
+def test_slices_joined_by_a_block_or_by_a_second_kernel(ops, D, dtype):
+    """The same bits either way: a token alone (a block a slice), and among so many that each block goes through its token's slices."""
+    H, G, lens = 4, 2, [700, 1100] + [3] * 400
+    c = p4.Cache(lens, G, D, 16, seed=D)
+    q = queries(len(lens), H, D, 4, dtype)
+    got = attend(ops, c, q, [1] * len(lens), lens, H, D ** -0.5, dtype=dtype)
+    few = attend(ops, c, q[:2], [1, 1], lens[:2], H, D ** -0.5, dtype=dtype, table=c.table[:2])
+    assert torch.equal(got[:2], few)
+    two = p4.Cache.__new__(p4.Cache)
+    two.__dict__.update(c.__dict__)
+    check_rows(got[:2], q[:2].view(2, H, D), two, [1, 1], lens[:2], D ** -0.5, wide=True, dtype=dtype)
