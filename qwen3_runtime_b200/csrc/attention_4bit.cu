@@ -787,6 +787,17 @@ template <int D> struct KeyBytes {  // what a lane holds of 16 keys as they are 
       }
     }
   }
+  // keys first + r and first + r + 8 of a sequence, as far as they lie in front of `end`
+  __device__ __forceinline__ void load_at(const Mass& m, const Q4Page& L, const int* bt, int kvh, int first, int end, int lane) {
+    int page[2], row[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int key = first + (lane >> 2) + 8 * half, i = key / m.ps;
+      page[half] = key < end ? bt[i] : -1;
+      row[half] = key - i * m.ps;
+    }
+    load(m, L, kvh, page, row, lane);
+  }
 };
 
 // Sixteen keys of one page (page sizes that are multiples of 16): one place for all of them.
@@ -828,18 +839,6 @@ template <int D> struct PageKeys {
 template <int D> struct KeyTile {  // 16 keys as A fragments
   uint32_t a[Head<D>::WORDS][2][4];
   float s[2][Head<D>::G], z[2][Head<D>::G];
-  __device__ __forceinline__ void load(const Mass& m, const Q4Page& L, const int* bt, int kvh, int first, int end, int lane) {
-    int page[2], row[2];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int key = first + (lane >> 2) + 8 * half, i = key / m.ps;
-      page[half] = key < end ? bt[i] : -1;
-      row[half] = key - i * m.ps;
-    }
-    KeyBytes<D> bytes;
-    bytes.load(m, L, kvh, page, row, lane);
-    take(bytes);
-  }
   __device__ __forceinline__ void take(const KeyBytes<D>& b) {
     using H = Head<D>;
     const auto& w = b.w;
@@ -929,9 +928,12 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS) mass_rows_ke
       sees[n][c] = min(end - 1, rows.before + (row0 + 8 * n + 2 * l + c) / R);
     }
   }
+  KeyBytes<D> bytes;
+  bytes.load_at(a, L, bt, kvh, begin + STEP * warp, end, lane);
   for (int first = begin + STEP * warp; first < end; first += STEP * WARPS) {
     KeyTile<D> k;
-    k.load(a, L, bt, kvh, first, end, lane);
+    k.take(bytes);
+    bytes.load_at(a, L, bt, kvh, first + STEP * WARPS, end, lane);  // (on its way while this tile is worked on)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float x[4];
@@ -979,10 +981,17 @@ template <int D, int NT> __global__ void __launch_bounds__(THREADS) mass_rows_ke
 __device__ __forceinline__ float row_log2(const Mass& a, long at) {
   if (!a.part) return a.lse[at] * LOG2_E;
   float top = MINUS_BIG, den = 0.f;
-  for (int s = 0; s < a.slices; ++s) top = fmaxf(top, a.part[at * a.slices + s].x);
-  for (int s = 0; s < a.slices; ++s) {
-    const float2 y = a.part[at * a.slices + s];
-    den += y.y * exp2_fast(y.x - top);
+  for (int s = 0; s < a.slices; s += 8) {  // eight loads at a time
+    float2 y[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) y[u] = s + u < a.slices ? a.part[at * a.slices + s + u] : make_float2(MINUS_BIG, 0.f);
+    float now = top;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) now = fmaxf(now, y[u].x);
+    den *= exp2_fast(top - now);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) den += y[u].y * exp2_fast(y[u].x - now);
+    top = now;
   }
   return top + log2f(den);
 }
@@ -1012,7 +1021,11 @@ template <int D> __global__ void __launch_bounds__(32 * COLUMN_WARPS) mass_colum
   const Q4Page L(D, H::G, a.ps);
   const int* bt = a.block_table + (long)seq * a.max_pages;
   KeyTile<D> k;
-  k.load(a, L, bt, kvh, first, kv_len, lane);
+  {
+    KeyBytes<D> bytes;
+    bytes.load_at(a, L, bt, kvh, first, kv_len, lane);
+    k.take(bytes);
+  }
   float total[2] = {0.f, 0.f};
   // rows of tokens that see none of the block's keys are left out
   const int start = max(0, block_first - rows.before) * R & ~7, stop = rows.count * R;
