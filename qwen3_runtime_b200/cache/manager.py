@@ -74,7 +74,8 @@ class GroupSpec:
 class TokenBudget:
     """Requests keep at most ``keep`` tokens in the cache, each kv head its own: the sequence's ``first`` ones, the last ``recent`` and of
     the others those that were given the most attention (csrc/cache_4bit.cu).  A request is cut when it holds more than ``keep + slack``.
-    ``observe``: how many last tokens of a prompt's portion give weight (a decoded token always does)."""
+    ``observe``: how many last tokens of a prompt's portion give weight (a decoded token always does).  What goes depends on how a prompt
+    was cut into portions, so a request that was preempted and recomputed may go on with other tokens."""
 
     keep: int
     first: int = 4
