@@ -41,8 +41,9 @@ __device__ __forceinline__ bool store_place(const Store& a, int t, int nkv, int 
 
 // Head sizes 16, 32, 64, 128, 256 with the rotation over the whole head (or none): D / 16 threads per (token, head); thread c owns
 // channels [8c, 8c + 8) and [D/2 + 8c, D/2 + 8c + 8), which are one word of 4-bit numbers each.  The floor is the bytes of the projection
-// and of the queries; what bounds it is instructions, 415 for four heads of 128 channels: 3,258 tokens of 32 + 8 heads take 24 us, 2.9 TB/s.
-// Weights and angles asked for ahead of the squares' sum cost more in registers than they hide (26 us), three heads a thread more again (41).
+// and of the queries; 3,258 tokens of 32 + 8 heads of 128 take 24 us, 2.9 TB/s.  What bounds it: schedulers issue in 0.7 of their clocks, and
+// the rest waits for loads.  One side alone gives nothing: two numbers an instruction (24), angles asked for into L1 (25) or into registers
+// ahead of the squares' sum (26), three heads a thread (41), blocks of 64 to 256 threads (24 to 28).
 //
 // A key near the border between two numbers falls on either side by float32's last bit.  So that it falls where a float32 statement of
 // norm and rotation in PyTorch puts it, heads of 128 and 256 sum their squares four neighbours at a time and then by halves, and products
