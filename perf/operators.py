@@ -271,7 +271,9 @@ def _run_own(s):
         return (q, *ops.unpack_4bit(s["pages"], block_table=s["table"], kv_lens=s["lens"], max_kv_len=max(s["kv"]), dtype=qkv.dtype, **sizes))
     step, scale = _step(s), D ** -0.5
     out = torch.empty((T, H * D), dtype=qkv.dtype, device=DEV)
-    lse = torch.empty((T, H), dtype=torch.float32, device=DEV) if case["kind"] == "mass" and step.decode_only else None
+    lse = None
+    if case["kind"] == "mass" and step.decode_only and ops.decode_4bit_ok(qkv, H, case["kv_heads"], D):  # (other sizes have no log sums)
+        lse = torch.empty((T, H), dtype=torch.float32, device=DEV)
     ops.paged_attention_4bit(qkv, qkv.stride(0), num_heads=H, pages=s["pages"], block_table=s["table"], out=out, scale=scale,
                              window=case.get("window") or None, step=step, lse=lse, **sizes)
     if case["kind"] == "attention":
