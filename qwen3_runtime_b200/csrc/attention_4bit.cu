@@ -1309,6 +1309,11 @@ struct General {
   float scale_log2;
   float *mid_o, *mid_ml;  // slices > 0: [tokens][nq][slices][D] and [tokens][nq][slices][2]
   int tiles_at;           // byte of shared memory
+  // the last key that token t sees; -1: none (it belongs to no sequence, or its place lies outside the table), and its row is zero
+  __device__ __forceinline__ int last_key(long t) const {
+    const int seq = token_seq[t], place = places[t];
+    return seq >= 0 && seq < num_seqs && place >= 0 && place / ps < max_pages ? place : -1;
+  }
 };
 
 // (m, l, o) <- its join with another's; o and b are unnormalised.  The fused steps are named, so that both kernels round alike.
@@ -1336,10 +1341,8 @@ __global__ void __launch_bounds__(GEN_THREADS) general_4bit_kernel(General a, co
   float* v_s = f_s + 32;                                         // [groups of threads][8][D] at the end of a slice
   unsigned char* k_s = smem + a.tiles_at;                        // two tiles: 64 rows of keys' codes and parameters, then of values
   const int pitch = general_pitch(L), bytes = 2 * GEN_TILE * pitch;
-  const int seq = a.token_seq[t], place = a.places[t];
-  const bool there = seq >= 0 && seq < a.num_seqs && place >= 0 && place / a.ps < a.max_pages;
-  const int last = there ? place : -1, lo = a.window > 0 ? max(0, last - a.window + 1) : 0;
-  const int* bt = a.block_table + (long)(there ? seq : 0) * a.max_pages;
+  const int last = a.last_key(t), lo = a.window > 0 ? max(0, last - a.window + 1) : 0;
+  const int* bt = a.block_table + (long)(last >= 0 ? a.token_seq[t] : 0) * a.max_pages;
   for (int i = tid; i < heads * D; i += GEN_THREADS) q_s[i] = to_f32(q[t * a.q_stride + (long)h0 * D + i]) * a.scale_log2;
   // a thread owns channels c and c + 1, which share a byte, of the keys g, g + parts, g + 2 parts ... of each tile
   const int parts = 2 * GEN_THREADS / D, c = 2 * (tid % (D / 2)), part = tid / (D / 2);
@@ -1490,10 +1493,10 @@ template <typename T> __global__ void general_4bit_merge_kernel(General a, T* __
   pdl_wait();
   pdl_launch_dependents();
   const long at = blockIdx.x;
-  const int place = a.places[at / a.nq], lo = a.window > 0 ? max(0, place - a.window + 1) : 0;
+  const int last = a.last_key(at / a.nq), lo = a.window > 0 ? max(0, last - a.window + 1) : 0;
   for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
     float M = MINUS_BIG, S = 0.f, O = 0.f;
-    const int stop = place >= 0 ? min(place / GEN_SLICE + 1, a.slices) : 0;
+    const int stop = last >= 0 ? min(last / GEN_SLICE + 1, a.slices) : 0;
     for (int s0 = lo / GEN_SLICE; s0 < stop; s0 += 8) {  // eight slices' loads at a time
       float m[8], l[8], o[8];
 #pragma unroll
@@ -1506,7 +1509,7 @@ template <typename T> __global__ void general_4bit_merge_kernel(General a, T* __
       for (int u = 0; u < 8; ++u)
         if (s0 + u < stop) join_slices(M, S, O, m[u], l[u], o[u]);
     }
-    out[at * a.D + c] = from_f32<T>(place >= 0 ? O / S : 0.f);
+    out[at * a.D + c] = from_f32<T>(last >= 0 ? O / S : 0.f);
   }
 }
 
