@@ -28,7 +28,8 @@
 
 namespace {
 
-constexpr float MINUS_BIG = -1e30f;  // of a row that has seen nothing: a hidden key's score is -inf and weighs 2^(-inf - MINUS_BIG) = 0
+// The maximum of a row that has seen nothing: no score lies below it, and a hidden key's, -inf, weighs 2^(-inf - MINUS_BIG) = 0.
+constexpr float MINUS_BIG = -3.402823466e+38f;
 constexpr float LN_2 = 0.6931471805599453f;
 
 // Numbers J and J + 4 of a word `w` (`high`: w >> 8), or number J of two tokens whose halves were put side by side, as two bfloat16:
@@ -735,7 +736,9 @@ template <int D, int NT> int launch_decode(const Decode& a, int num_seqs, cudaSt
 // ---- sums of attention weights -----------------------------------------------------------------------------------------------------
 // mass[key] += sum over a sequence's last `observe` tokens and the query heads of the kv head of 2^(score - log sum of the row).  Rows are
 // (token, head of the group), token by token; the scores' tiles are those of decode attention.  A cached token's sum belongs to one warp's
-// lane: no atomics, the same bits every time.  Sums are float32; a weight is 2^x to 2 units in the last place (2^-22 of itself).
+// lane: no atomics, the same bits every time.  Sums are float32; a weight is 2^x to 2 units in the last place (2^-22 of itself), and the
+// log sum that is taken off, a float32 too, is good to 2^-23 of the row's scores: beyond some 2^20 weights are no more than a guess, but
+// no sum gets more than one for each row.
 //   few rows (up to 16: single tokens)  mass_few_kernel: the queries stay in registers, keys stream past them, 16 a warp at a time, the next
 //                                       ones' bytes on their way; reads half of what the attention reads.  Instructions bound it: 96,700
 //                                       tokens of 8 kv heads of 128 channels in 29 us (2.0 TB/s); with two tiles on their way no less.
@@ -899,6 +902,8 @@ struct Rows {
     before = kv_len - count;
   }
 };
+
+__device__ __forceinline__ float at_most(float y, int rows) { return y > (float)rows ? (float)rows : y; }  // (what is no number stays none)
 
 // Log sums: grid (slice, block of 8 NT rows, sequence x kv head); a warp takes every fourth 16 keys of the slice.
 template <int D, int NT> __global__ void __launch_bounds__(THREADS) mass_rows_kernel(Mass a) {
@@ -1082,6 +1087,7 @@ template <int D> __global__ void __launch_bounds__(32 * COLUMN_WARPS) mass_colum
     float y = total[half];
     y += __shfl_xor_sync(0xffffffffu, y, 1);
     y += __shfl_xor_sync(0xffffffffu, y, 2);
+    y = at_most(y, rows.count * R);
     const int key = first + r + 8 * half;
     if (l == 0 && key < kv_len) {
       const int page = bt[key / a.ps];
@@ -1185,7 +1191,7 @@ template <int D, int NT, bool WHOLE> __global__ void __launch_bounds__(THREADS, 
       float y = total[half];
       y += __shfl_xor_sync(0xffffffffu, y, 1);
       y += __shfl_xor_sync(0xffffffffu, y, 2);
-      if (mine[half]) *mine[half] = was[half] + y;
+      if (mine[half]) *mine[half] = was[half] + at_most(y, rows.count * R);
     }
   }
 }
@@ -1253,7 +1259,7 @@ template <typename T> __global__ void mass_columns_general_kernel(Mass a, const 
       const float x = score_of(q + t * a.q_stride + (long)h * D, rec, L, key % a.ps, D, G) * a.scale_log2;
       total += exp2f(x - a.lse[t * a.nq + h] * LOG2_E);
     }
-  if (rows.count) a.mass[((long)page * a.nkv + kvh) * a.ps + key % a.ps] += total;
+  if (rows.count) a.mass[((long)page * a.nkv + kvh) * a.ps + key % a.ps] += at_most(total, rows.count * R);
 }
 
 template <int D, int NT> int launch_mass(const Mass& a, bool want_rows, int most_tokens, int few_slices, cudaStream_t stream) {

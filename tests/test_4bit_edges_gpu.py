@@ -2,6 +2,8 @@
 sums.  The tolerances are those of tests/test_4bit_gpu.py."""
 
 
+import math
+
 import pytest
 import torch
 
@@ -30,3 +32,44 @@ def test_a_token_without_a_place_is_zero(ops, copies, dtype, D, window):  # noqa
     step.positions[2], step.positions[3] = table.shape[1] * 16, -2
     got = t4.attend(ops, c, q, new, lens * copies, H, D ** -0.5, step=step, **args)
     assert bool((got[:4] == 0).all()) and torch.equal(got[4:], want[4:])
+
+
+@pytest.mark.parametrize("H,G,D,dtype,slices", [(8, 2, 128, BF16, 1), (8, 2, 128, BF16, 3), (8, 2, 128, BF16, -3), (8, 1, 64, BF16, 2),
+                                                (4, 2, 256, BF16, -2), (4, 2, 80, BF16, None), (4, 2, 64, F32, None), (4, 1, 128, F32, None)])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_scores_that_all_lie_far_from_zero(ops, H, G, D, dtype, slices, sign):  # noqa: F811
+    """All scores of a row near -10^33 (or 10^33): the largest takes the row, as it does anywhere else.  A score is off by 2^-23 (D + 8) of
+    the row's largest product sum (``score_error``); here the best key is twice as far from the next as two such errors, so it weighs one."""
+    lens, scale = [70, 700], D ** -0.5
+
+    def mutate(b, k, v):
+        k.abs_()
+        k *= sign * 1e16
+        k[:, 33] *= 0.5 if sign < 0 else 2.0  # (the best key of most rows)
+
+    c = p4.Cache(lens, G, D, 16, seed=D, mutate=mutate)
+    q = (t4.queries(2, H, D, 3, F32).abs() * 1e17).to(dtype)
+    rows = q.view(2, H, D)
+    log_sums = dtype == BF16 and D in (64, 128, 256)
+    got = t4.attend(ops, c, q, [1, 1], lens, H, scale, dtype=dtype, lse=log_sums, slices=slices)
+    got, lse = got if log_sums else (got, None)
+    for b in range(2):
+        k, v = c.values(b)
+        err = t4.score_error(rows[b:b + 1], c, b, scale)[0]
+        num, s, z = (x.double() for x in c.v[b])
+        s, z = s.repeat_interleave(D // s.shape[-1], -1), z.repeat_interleave(D // z.shape[-1], -1)
+        spread = (z + 8 * s).abs() + s * (num - 8).abs()
+        for h in range(H):
+            x = (k[h // (H // G)] @ rows[b, h].double()) * scale
+            best, next_best = x.topk(2).values.tolist()
+            j = int(x.argmax())
+            assert best - next_best > 4 * float(err[h])
+            want = v[h // (H // G), j]
+            tol = 2.0 ** -22 * spread[h // (H // G), j] if dtype == F32 else (2 * t4.U + 2.0 ** -14) * spread[h // (H // G), j] + t4.U * want.abs()
+            assert bool(((got[b, h].double() - want).abs() <= tol).all()), (b, h)
+            if log_sums:
+                assert abs(float(lse[b, h]) - best) <= float(err[h]) + 2.0 ** -20 * abs(best)
+    # a log sum of such rows is known to 2^-23 of itself only: sums stay within what the rows can give, none is lost to infinity
+    for given in {None, lse}:
+        mass = t4.mass_of(ops, c, q, [1, 1], lens, H, scale, 1, lse=None if given is None else given.cuda())
+        assert bool((mass >= 0).all()) and bool((mass <= H // G).all()) and math.isfinite(float(mass.sum()))
