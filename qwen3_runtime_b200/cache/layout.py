@@ -182,6 +182,12 @@ class CacheLayout:
         (qwen3_runtime/engine/memory.py:8-10)."""
         return sum(self.page_bytes(1, dtype_bytes))
 
+    def unpacked_bytes(self, tokens: int) -> int:
+        """Bytes that the attention over prompts of one layer takes to unpack a request of that many tokens from 4 bits (keys and values in
+        bfloat16; the layers' turns come one after the other); a window reaches over part of it."""
+        specs = [g.layer_spec for g in self.groups if getattr(g.layer_spec, "bits", None) == 4]
+        return max((4 * s.num_kv_heads * s.head_dim * tokens for s in specs), default=0)
+
     def pages_for_budget(self, budget_bytes: int, page_size: int, dtype_bytes: int, *,
                          max_num_seqs: int | None = None, max_step_tokens: int | None = None) -> list[int]:
         """Pages for each paged group that together fit in ``budget_bytes``

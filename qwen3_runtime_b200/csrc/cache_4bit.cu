@@ -265,25 +265,74 @@ __global__ void store_4bit_kernel(const T* qkv, int row_stride, T* q_out, int q_
 }
 
 // ---- back to wide pages -------------------------------------------------------------------------------------------------------------
-// Out page: sequence's row * width + its page; rows behind the sequence's last token are zero, and pages behind it too (fill) or left alone
-// (not fill).  `cu_seqlens` (may be null): only sequences that bring more than one token count, in order; `table_out` [num_seqs][width]
-// then gets where their pages went.
+// Two forms.  Without `cu_seqlens`, sequence z's page i goes to page z * width + i, rows behind its last token are zero, and whole pages behind
+// it too.  With it, the attention over prompts reads the pages: only sequences that bring at least `least` tokens count, and of each
+// only the pages that its first new token's window reaches up to the last token's; they lie one after the other, `count` pages in all, and
+// `table_out` [num_seqs][width] says where (entries that nobody asks for name a page of the same sequence, never none).
 struct Unpack {
   const unsigned char* pages;
   int num_pages, nkv, ps;
   const int *block_table, *kv_lens, *cu_seqlens;
-  int max_pages, num_seqs, max_len, width, fill;
+  int max_pages, num_seqs, max_len, least, window, count, width;
   int* table_out;
-  // the sequence that stands at place `z`; -1: none.  Called by whole warps.
-  __device__ __forceinline__ int sequence(int z) const {
-    if (!cu_seqlens) return z;
-    for (int base = 0; base < num_seqs; base += 32) {
-      const int s = base + (threadIdx.x & 31);
-      const uint32_t found = __ballot_sync(0xffffffffu, s < num_seqs && cu_seqlens[s + 1] - cu_seqlens[s] > 1);
-      if (z < __popc(found)) return base + __fns(found, 0, z + 1);
-      z -= __popc(found);
+};
+
+// Page `p` of the output (of a launch whose second axis is the sequences, without `cu_seqlens`).  Called by whole warps.
+struct UnpackPage {
+  int seq, i, first, last;  // the sequence (-1: none), its page, and the first and last of its pages that count
+  __device__ __forceinline__ UnpackPage(const Unpack& a, int p) : seq(-1), i(0), first(0), last(a.width - 1) {
+    if (!a.cu_seqlens) {
+      seq = blockIdx.y, i = p;
+      return;
     }
-    return -1;
+    if (p >= a.count) return;
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base < a.num_seqs; base += 32) {
+      int skip = 0, n = 0;
+      if (base + lane < a.num_seqs) {
+        const int tokens = a.cu_seqlens[base + lane + 1] - a.cu_seqlens[base + lane], len = min(a.kv_lens[base + lane], a.max_len);
+        if (tokens >= a.least && len > 0) {
+          if (a.window > 0) skip = max(0, len - tokens - a.window + 1) / a.ps;
+          n = (len + a.ps - 1) / a.ps - skip;
+        }
+      }
+      int sum = n;  // pages up to and with this lane's sequence
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      const uint32_t reach = __ballot_sync(0xffffffffu, sum > p);
+      if (reach) {
+        const int from = __ffs(reach) - 1;
+        seq = base + from;
+        first = __shfl_sync(0xffffffffu, skip, from);
+        last = first + __shfl_sync(0xffffffffu, n, from) - 1;
+        i = last - (__shfl_sync(0xffffffffu, sum, from) - 1 - p);
+        return;
+      }
+      p -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  // what the table says of this page, and of those in front of the first and behind the last; by one warp a page
+  __device__ __forceinline__ void name(const Unpack& a, int p) const {
+    if (!a.table_out) return;
+    int* row = a.table_out + (long)seq * a.width;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0 && i < a.width) row[i] = p;
+    if (i == first)
+      for (int j = lane; j < min(first, a.width); j += 32) row[j] = p;
+    if (i == last)
+      for (int j = last + 1 + lane; j < a.width; j += 32) row[j] = p;
+  }
+  // where its bytes lie, and how many rows of it count
+  __device__ __forceinline__ int rows(const Unpack& a, int* page) const {
+    *page = i < a.max_pages ? a.block_table[(long)seq * a.max_pages + i] : -1;
+    if (*page < 0 || *page >= a.num_pages) {
+      *page = 0;
+      return 0;
+    }
+    return min(max(min(a.kv_lens[seq], a.max_len) - i * a.ps, 0), a.ps);
   }
 };
 
@@ -296,18 +345,16 @@ template <typename T, int D> __global__ void __launch_bounds__(256) unpack_4bit_
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, r = lane & 7;
   const long item = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int kvh = (int)(item % a.nkv), i = (int)(item / a.nkv);
-  if (i >= a.width) return;
-  const int seq = a.sequence(blockIdx.y);
-  if (seq < 0) return;
-  const int place = blockIdx.y * a.width + i;
-  if (a.table_out && kvh == 0 && lane == 0) a.table_out[(long)seq * a.width + i] = place;
-  const int page = i < a.max_pages ? a.block_table[(long)seq * a.max_pages + i] : -1;
-  int rows = min(max(min(a.kv_lens[seq], a.max_len) - i * a.ps, 0), a.ps);
-  if (page < 0 || page >= a.num_pages) rows = 0;
-  if (rows == 0 && !a.fill) return;
+  const int kvh = (int)(item % a.nkv), p = (int)(item / a.nkv);
+  if (p >= (a.cu_seqlens ? a.count : a.width)) return;
+  const UnpackPage at_page(a, p);
+  if (at_page.seq < 0) return;
+  const int place = a.cu_seqlens ? p : blockIdx.y * a.width + p;
+  if (kvh == 0) at_page.name(a, place);
+  int page;
+  const int rows = at_page.rows(a, &page);
   const Q4Page L(D, G, a.ps);
-  const unsigned char* rec = a.pages + ((long)max(page, 0) * a.nkv + kvh) * L.record;
+  const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
   const long out_base = ((long)place * a.nkv + kvh) * a.ps * D;
   for (int first = lane >> 3; first < 2 * a.ps; first += 4 * AT_ONCE) {  // rows of keys, then of values
     uint32_t code[AT_ONCE][G], par[AT_ONCE][G];
@@ -345,17 +392,15 @@ template <typename T, int D> __global__ void __launch_bounds__(256) unpack_4bit_
 template <typename T> __global__ void unpack_4bit_kernel(Unpack a, int D, int G, T* __restrict__ k_out, T* __restrict__ v_out) {
   pdl_wait();
   pdl_launch_dependents();
-  const int i = blockIdx.x / a.nkv, kvh = blockIdx.x % a.nkv;
-  const int seq = a.sequence(blockIdx.y);
-  if (seq < 0) return;
-  const int place = blockIdx.y * a.width + i;
-  if (a.table_out && kvh == 0 && threadIdx.x == 0) a.table_out[(long)seq * a.width + i] = place;
-  const int page = i < a.max_pages ? a.block_table[(long)seq * a.max_pages + i] : -1;
-  int rows = min(max(min(a.kv_lens[seq], a.max_len) - i * a.ps, 0), a.ps);
-  if (page < 0 || page >= a.num_pages) rows = 0;
-  if (rows == 0 && !a.fill) return;
+  const int p = blockIdx.x / a.nkv, kvh = blockIdx.x % a.nkv;
+  const UnpackPage at_page(a, p);
+  if (at_page.seq < 0) return;
+  const int place = a.cu_seqlens ? p : blockIdx.y * a.width + p;
+  if (kvh == 0 && threadIdx.x < 32) at_page.name(a, place);
+  int page;
+  const int rows = at_page.rows(a, &page);
   const Q4Page L(D, G, a.ps);
-  const unsigned char* rec = a.pages + ((long)max(page, 0) * a.nkv + kvh) * L.record;
+  const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
   const int words = D / 8, size_words = words / G, ps = a.ps;
   const long out_base = ((long)place * a.nkv + kvh) * ps * D;
   for (int u = threadIdx.x; u < 2 * ps * words; u += blockDim.x) {
@@ -378,15 +423,16 @@ template <typename T> __global__ void unpack_4bit_kernel(Unpack a, int D, int G,
   }
 }
 
-template <typename T> cudaError_t launch_unpack(const Unpack& a, int count, int D, T* k_out, T* v_out, cudaStream_t stream) {
-  const long items = (long)a.width * a.nkv;
+template <typename T> cudaError_t launch_unpack(const Unpack& a, int D, T* k_out, T* v_out, cudaStream_t stream) {
+  const long items = (long)(a.cu_seqlens ? a.count : a.width) * a.nkv;
+  const unsigned sequences = a.cu_seqlens ? 1 : a.num_seqs;
   if (D == 64 || D == 128 || D == 256) {
-    const dim3 grid((unsigned)((items + 7) / 8), (unsigned)count);
+    const dim3 grid((unsigned)((items + 7) / 8), sequences);
     if (D == 64) return launch_pdl(unpack_4bit_rows_kernel<T, 64>, grid, dim3(256), 0, stream, a, k_out, v_out);
     if (D == 128) return launch_pdl(unpack_4bit_rows_kernel<T, 128>, grid, dim3(256), 0, stream, a, k_out, v_out);
     return launch_pdl(unpack_4bit_rows_kernel<T, 256>, grid, dim3(256), 0, stream, a, k_out, v_out);
   }
-  return launch_pdl(unpack_4bit_kernel<T>, dim3((unsigned)items, (unsigned)count), dim3(a.ps * D / 8 >= 256 ? 256 : 128), 0, stream, a, D,
+  return launch_pdl(unpack_4bit_kernel<T>, dim3((unsigned)items, sequences), dim3(a.ps * D / 8 >= 256 ? 256 : 128), 0, stream, a, D,
                     q4_groups(D), k_out, v_out);
 }
 
@@ -717,18 +763,20 @@ Q3_EXPORT int q3_store_4bit(int dtype, const void* qkv, int row_stride, void* q_
   return q3_launch_status();
 }
 
+// `cu_seqlens` null: num_seqs * width pages are written; else `count` pages (struct Unpack).
 Q3_EXPORT int q3_unpack_4bit(int dtype, const void* pages, int num_pages, int nkv, int D, int ps, const int* block_table, int max_pages,
-                             const int* kv_lens, int num_seqs, int max_len, const int* cu_seqlens, int count, int width, int fill,
+                             const int* kv_lens, int num_seqs, int max_len, const int* cu_seqlens, int least, int window, int count, int width,
                              void* k_out, void* v_out, int* table_out, cudaStream_t stream) {
-  if (count < 1 || width < 1) return Q3_OK;
+  if (num_seqs < 1 || width < 1 || (cu_seqlens && count < 1)) return Q3_OK;
   if (!pages || !block_table || !kv_lens || !k_out || !v_out || nkv < 1 || max_pages < 1 || !q4_sizes_ok(D, ps)) return Q3_ERR_ARGUMENT;
+  if (cu_seqlens && (!table_out || least < 1)) return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
-  if (count > 65535 || !q4_aligned(pages) || !q4_aligned(k_out) || !q4_aligned(v_out)) return Q3_ERR_UNSUPPORTED;
-  if ((long)width * nkv > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
-  const Unpack a{(const unsigned char*)pages, num_pages, nkv, ps, block_table, kv_lens, cu_seqlens, max_pages, num_seqs, max_len, width, fill,
-                 table_out};
-  const cudaError_t err = dtype == Q3_DTYPE_F32 ? launch_unpack(a, count, D, (float*)k_out, (float*)v_out, stream)
-                                                : launch_unpack(a, count, D, (bf16*)k_out, (bf16*)v_out, stream);
+  if ((!cu_seqlens && num_seqs > 65535) || !q4_aligned(pages) || !q4_aligned(k_out) || !q4_aligned(v_out)) return Q3_ERR_UNSUPPORTED;
+  if ((long)(cu_seqlens ? count : width) * nkv > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
+  const Unpack a{(const unsigned char*)pages, num_pages, nkv, ps, block_table, kv_lens, cu_seqlens, max_pages, num_seqs, max_len, least, window,
+                 count, width, table_out};
+  const cudaError_t err = dtype == Q3_DTYPE_F32 ? launch_unpack(a, D, (float*)k_out, (float*)v_out, stream)
+                                                : launch_unpack(a, D, (bf16*)k_out, (bf16*)v_out, stream);
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
 }
 

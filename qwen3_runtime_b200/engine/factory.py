@@ -79,6 +79,20 @@ class Runtime:
 UNLIMITED_POSITIONS = 1 << 30  # a model none of whose parts limits the positions
 
 
+def beside_unpacked(total: int, layout, block_size: int, longest: int, at_once: int, max_num_seqs: int,
+                    max_num_batched_tokens: int | None) -> int:
+    """What of ``total`` bytes the pages of a cache in 4 bits can have when the steps' attention over prompts unpacks its sequences beside
+    them: ``at_once`` bytes at a time, or one request of ``longest`` tokens if that is more; never more than the pages hold."""
+
+    def room(pages_bytes: int) -> int:
+        counts = layout.pages_for_budget(pages_bytes, block_size, 2, max_num_seqs=max_num_seqs, max_step_tokens=max_num_batched_tokens)
+        held = max(counts, default=0) * block_size
+        return max(min(at_once, layout.unpacked_bytes(held)), layout.unpacked_bytes(min(longest, held)))
+
+    left = total * total // (total + room(total))  # fewer pages hold shorter requests: where that is the limit, both shrink alike
+    return min(left, total - room(left))
+
+
 def build_runtime(model: DecoderModel, *, max_positions: int | None = None, block_size: int,
                   num_kv_blocks: int | list[int] | None, max_num_seqs: int, cuda_graph: bool = False,
                   kv_budget: int | None = None, kv_memory_fraction: float = 0.85,
@@ -86,7 +100,8 @@ def build_runtime(model: DecoderModel, *, max_positions: int | None = None, bloc
     """Cache and step function for a loaded model.  ``max_positions`` defaults to what the
     model's own parts can serve (the shortest position table among them).  ``num_kv_blocks``:
     pages of every paged group, one count per paged group, or None to size the pools from
-    ``kv_budget`` bytes (default: ``kv_memory_fraction`` of the free device memory)."""
+    ``kv_budget`` bytes (default: ``kv_memory_fraction`` of the free device memory; for a cache in 4 bits what prompts unpack
+    from it is kept free of that)."""
     if max_positions is None:
         max_positions = model.position_limit() or UNLIMITED_POSITIONS
     layout = model.cache_layout()
@@ -99,6 +114,12 @@ def build_runtime(model: DecoderModel, *, max_positions: int | None = None, bloc
             else:
                 free, _total = torch.cuda.mem_get_info(ctx.device)
                 kv_budget = int(free * kv_memory_fraction)
+                if ctx.kv_bits == 4 and ctx.dtype == torch.bfloat16:
+                    longest = max_positions
+                    if ctx.kv_budget is not None and max_num_batched_tokens is not None:
+                        longest = min(longest, ctx.kv_budget.keep + ctx.kv_budget.slack + max_num_batched_tokens)
+                    kv_budget = beside_unpacked(kv_budget, layout, block_size, longest, getattr(ctx.ops, "UNPACK_BYTES", 0), max_num_seqs,
+                                                max_num_batched_tokens)
         elif kv_budget <= 0:
             raise ValueError(f"kv_budget must be positive, got {kv_budget!r}")
         counts = layout.pages_for_budget(kv_budget, block_size, dtype_bytes, max_num_seqs=max_num_seqs,

@@ -240,7 +240,7 @@ _SIGNATURES = {
                           c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int,
                           c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
         "q3_unpack_4bit": [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
-                           c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+                           c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
         "q3_evict_4bit": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int,
                           c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     },
@@ -486,6 +486,35 @@ def chunk_segment(cu, H, D, Dv, sms, seg) -> int:
         if best is None or cost < best:
             best, found = cost, seg
     return found
+
+
+def unpacked_pages_4bit(cu, kv_lens, page_size, window=None, least=1, exact=True) -> list:
+    """Pages that attention over prompts reads of each sequence of a step (tokens ``cu[b]`` to ``cu[b + 1] - 1``, ``kv_lens[b]`` keys): from
+    the first that its first new token's window reaches to the last; none of a sequence that brings fewer than ``least`` tokens.  Not
+    ``exact``: as many as any shorter length asks for, too."""
+    counts = []
+    for b, kv in enumerate(kv_lens):
+        new, pages = cu[b + 1] - cu[b], -(-kv // page_size)
+        if window and exact:
+            pages -= max(0, kv - new - window + 1) // page_size
+        elif window:
+            pages = min(pages, -(-(new + window) // page_size) + 1)
+        counts.append(pages if new >= least else 0)
+    return counts
+
+
+def runs_within(counts, limit) -> list:
+    """Neighbours whose counts sum to ``limit`` at most, as ``(first, end)``; a larger one alone.  Those that count nothing go along with
+    their neighbours, and a run of nothing is left out."""
+    runs, first, total = [], 0, 0
+    for i, n in enumerate(counts):
+        if n and total and total + n > limit:
+            runs.append((first, i))
+            first, total = i, 0
+        total += n
+    if total:
+        runs.append((first, len(counts)))
+    return runs
 
 
 @functools.lru_cache(maxsize=None)
@@ -2186,17 +2215,11 @@ class CudaOps:
             raise KernelError(f"{what}: max_kv_len={max_kv_len} does not fit a block table of {width} pages")
         k = torch.empty((B * n, num_kv_heads, page_size, head_dim), dtype=dtype, device=pages.device)
         v = torch.empty_like(k)
-        self._unpack_4bit(pages, block_table, kv_lens, int(max_kv_len), None, B, n, k, v, None, page_size)
-        return k, v
-
-    def _unpack_4bit(self, pages, block_table, kv_lens, max_len, cu, count, width, k, v, table, page_size):
-        _, G, _, D = k.shape
-        num_seqs, max_pages = block_table.shape
         if self.timing is not None:
-            self._costs(2 * k.numel() * k.element_size() + count * width * G * four_bit_page_bytes(D, page_size))
-        self._call("cache_4bit", "q3_unpack_4bit", "unpack_4bit", _dtype_code(k.dtype), pages.data_ptr(), pages.shape[0], G, D, page_size,
-                   block_table.data_ptr(), max_pages, _ptr(kv_lens), num_seqs, max_len, _ptr(cu), count, width,
-                   int(table is None), k.data_ptr(), v.data_ptr(), _ptr(table))
+            self._costs(2 * k.numel() * k.element_size() + B * n * num_kv_heads * four_bit_page_bytes(head_dim, page_size))
+        self._call("cache_4bit", "q3_unpack_4bit", what, _dtype_code(dtype), pages.data_ptr(), pages.shape[0], num_kv_heads, head_dim,
+                   page_size, block_table.data_ptr(), width, _ptr(kv_lens), B, int(max_kv_len), None, 0, 0, 0, n, k.data_ptr(), v.data_ptr(), None)
+        return k, v
 
     def paged_attention_4bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, block_table, out, page_size, scale, step,
                              window=None, decode_slices=None, lse=None):
@@ -2236,26 +2259,59 @@ class CudaOps:
         if dtype == torch.float32 or (step.decode_only and not fast) or not aligned:
             return self._general_4bit(q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window)
         # portions of prompts (and single tokens beside them): their sequences' pages unpacked, the kernels for wide pages
-        n = -(-max_len // page_size)
         split = fast and D != 256  # prompts apart from single tokens, which are decoded as they are
         cu = step.host_cu_seqlens
-        count = sum(cu[b + 1] - cu[b] > 1 for b in range(step.num_seqs)) if split else step.num_seqs
         if split and step.num_single:
             singles = [kv for b, kv in enumerate(step.host_kv_lens) if cu[b + 1] - cu[b] == 1]
             self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, step.single_seqs, step.num_single, max(singles),
                               self.decode_slices_4bit(singles, G, D, window, H // G), out, page_size, scale, window, None, None)
-        if not count:
-            return out
-        k, v = (torch.empty((count * n, G, page_size, D), dtype=dtype, device=out.device) for _ in range(2))
-        table = torch.empty((block_table.shape[0], n), dtype=torch.int32, device=out.device)
-        self._unpack_4bit(pages, block_table, step.kv_lens, max_len, step.cu_seqlens if split else None, count, n, k, v, table, page_size)
-        step = copy.copy(step)
+        exact = not step.captured_width and len(step.host_kv_lens) >= step.num_seqs  # (else the lengths are those of the moment, up to max_len)
+        lens = list(step.host_kv_lens[:step.num_seqs]) if exact else [max_len] * step.num_seqs
+        counts = unpacked_pages_4bit(cu, lens, page_size, window, 2 if split else 1, exact)
+        total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * page_size * D)
+        if total <= limit:
+            runs = [(0, len(counts), total)] if total else []
+        else:
+            runs = [(first, end, sum(counts[first:end])) for first, end in runs_within(counts, limit)]
+        for first, end, count in runs:
+            longest = max([n for n, c in zip(lens[first:end], counts[first:end]) if c])
+            self._prompts_4bit(q, q_stride, H, G, D, pages, block_table, step, first, end, count, longest, split, out, page_size, scale, window)
+        return out
+
+    # Keys and values that a step's attention over prompts unpacks at a time, in bytes: sequences beyond it are taken in turn (one that needs
+    # more by itself is taken alone).
+    UNPACK_BYTES = 1 << 30
+
+    def _prompts_4bit(self, q, q_stride, H, G, D, pages, block_table, step, first, end, count, longest, split, out, page_size, scale, window):
+        """Attention of the step's sequences ``first .. end - 1``, whose ``count`` pages are unpacked for it (none of those has more than
+        ``longest`` keys)."""
+        cu, t0, t1 = step.host_cu_seqlens, step.host_cu_seqlens[first], step.host_cu_seqlens[end]
+        part = copy.copy(step)
+        if (first, end) != (0, step.num_seqs):  # a step of these sequences alone, counted from zero
+            single = [b for b in range(step.num_seqs) if cu[b + 1] - cu[b] == 1]
+            here = [i for i, b in enumerate(single) if first <= b < end]
+            part.num_tokens, part.num_seqs, part.num_single = t1 - t0, end - first, len(here)
+            part.host_cu_seqlens, part.host_kv_lens = [c - t0 for c in cu[first:end + 1]], step.host_kv_lens[first:end]
+            part.max_query_len, part.max_kv_len = max(b - a for a, b in zip(cu[first:end], cu[first + 1:end + 1])), longest
+            part.cu_seqlens, part.kv_lens = step.cu_seqlens[first:end + 1] - t0, step.kv_lens[first:end]
+            part.token_seq, part.positions = step.token_seq[t0:t1] - first, step.positions[t0:t1]
+            part.single_seqs = step.single_seqs[here[0]:here[-1] + 1] - first if here else None
+            q, out, block_table = q[t0:t1], out[t0:t1], block_table[first:end]
         if split:
-            step.single_seqs, step.num_single = None, 0
+            part.single_seqs, part.num_single = None, 0
+        k = torch.empty((count, G, page_size, D), dtype=out.dtype, device=out.device)
+        v = torch.empty_like(k)
+        width = -(-longest // page_size)
+        table = torch.empty((part.num_seqs, width), dtype=torch.int32, device=out.device)
+        if self.timing is not None:
+            self._costs(2 * k.numel() * k.element_size() + count * G * four_bit_page_bytes(D, page_size))
+        self._call("cache_4bit", "q3_unpack_4bit", "unpack_4bit", _dtype_code(k.dtype), _ptr(pages), pages.shape[0], G, D, page_size,
+                   _ptr(block_table), block_table.shape[1], _ptr(part.kv_lens), part.num_seqs, longest, _ptr(part.cu_seqlens),
+                   2 if split else 1, int(window or 0), count, width, k.data_ptr(), v.data_ptr(), _ptr(table))
         # the wide kernels number a token by its place: kv_lens and cu_seqlens say it, or for the general kernel `positions`
-        return self.paged_attention(q, q_stride, num_heads=H, num_kv_heads=G, head_dim=D, k_pages=k, v_pages=v, block_table=table,
-                                    token_seq=step.token_seq, positions=step.positions, out=out, page_size=page_size, scale=scale,
-                                    window=window, step=step)
+        self.paged_attention(q, q_stride, num_heads=H, num_kv_heads=G, head_dim=D, k_pages=k, v_pages=v, block_table=table,
+                             token_seq=part.token_seq, positions=part.positions, out=out, page_size=page_size, scale=scale,
+                             window=window, step=part)
 
     GENERAL_SLICE = 256  # keys with a softmax of their own (csrc/attention_4bit.cu)
 
