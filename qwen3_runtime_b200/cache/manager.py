@@ -78,7 +78,7 @@ class TokenBudget:
     was cut into portions, so a request that was preempted and recomputed may go on with other tokens."""
 
     keep: int
-    first: int = 4
+    first: int | None = None  # None: 4, or all that are kept if those are fewer
     recent: int | None = None  # None: half of what is kept
     slack: int | None = None  # None: an eighth of what is kept
     observe: int = 32
@@ -86,7 +86,8 @@ class TokenBudget:
     def __post_init__(self) -> None:
         if self.keep < 1:
             raise ValueError("a token budget keeps at least one token")
-        object.__setattr__(self, "first", min(self.first, self.keep) if self.first == 4 else self.first)
+        if self.first is None:
+            object.__setattr__(self, "first", min(4, self.keep))
         if self.recent is None:
             object.__setattr__(self, "recent", min(self.keep // 2, self.keep - self.first))
         if self.slack is None:
