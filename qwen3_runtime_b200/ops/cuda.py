@@ -2124,6 +2124,7 @@ class CudaOps:
 
     # ---- a cache in 4 bits (csrc/four_bit.cuh says how a page is laid out and how values are rounded) ----------------------
     EVICT_KEYS = 49152  # tokens of a sequence whose keys one block sorts in shared memory; longer ones use scratch
+    EVICT_TOGETHER = 512  # moves that the choosing kernel makes itself; more have a kernel of their own
 
     def _check_4bit(self, what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens=None, layers=False):
         record = _four_bit_record(head_dim, page_size)
@@ -2455,6 +2456,7 @@ class CudaOps:
             slices = max(1, min(16, 2 * self.SM_COUNT // max(1, blocks), max_len // 128))
             if slices > 1:
                 part = torch.empty((T, num_heads, slices, 2), dtype=torch.float32, device=q.device)
+            self.launches += 1  # the log sums' kernel
         # few rows: blocks of at least 128 keys, about four an SM for the sequences' keys together
         total = sum(step.host_kv_lens) * num_kv_heads
         few = max(1, min(-(-max_len // 128), -(-max_len * 4 * self.SM_COUNT // max(1, total))))
@@ -2490,7 +2492,7 @@ class CudaOps:
         spill = torch.empty(pairs * max_kv_len, dtype=torch.int32, device=pages.device) if max_kv_len > self.EVICT_KEYS else None
         if self.timing is not None:
             self._costs(pairs * (8 * max_kv_len + 2 * cap * (four_bit_token_bytes(head_dim) + 8)))
-        self.launches += 1  # choose, then move
+        self.launches += int(cap > self.EVICT_TOGETHER)  # choose, then move
         self._call("cache_4bit", "q3_evict_4bit", what, _ptr(pages), layers, pages.shape[-3], num_kv_heads, head_dim, page_size,
                    _ptr(mass), _ptr(places), _ptr(block_table), block_table.shape[1], _ptr(kv_lens), B, max_kv_len, int(keep),
                    int(first), int(recent), cap, _ptr(spill), _ptr(lists))
