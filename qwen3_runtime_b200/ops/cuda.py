@@ -2417,10 +2417,12 @@ class CudaOps:
         return out
 
     def attention_mass_4bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, mass, block_table, page_size, scale, step,
-                            observe=None, lse=None):
+                            observe=None, lse=None, slice_keys=None):
         """Adds to ``mass`` (float32 ``[pages, kv heads, page_size]``) the softmax weights that every sequence's last ``observe`` tokens
         of the step (None: all of them) give to its cached tokens, summed over the query heads of a kv head.  ``lse``: the rows' log
-        sums, when :meth:`paged_attention_4bit` has written them for this step.  A page belongs to one sequence."""
+        sums, when :meth:`paged_attention_4bit` has written them for this step.  A page belongs to one sequence.  ``slice_keys``
+        (:meth:`mass_slice_keys_4bit`): keys that a block takes where a sequence has few rows, for a captured step, whose lengths
+        are not known when it is captured; results do not depend on it."""
         what = "attention_mass_4bit"
         code = _dtype_code(q.dtype)
         self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, step.kv_lens)
@@ -2457,15 +2459,19 @@ class CudaOps:
             if slices > 1:
                 part = torch.empty((T, num_heads, slices, 2), dtype=torch.float32, device=q.device)
             self.launches += 1  # the log sums' kernel
-        # few rows: blocks of at least 128 keys, about four an SM for the sequences' keys together
-        total = sum(step.host_kv_lens) * num_kv_heads
-        few = max(1, min(-(-max_len // 128), -(-max_len * 4 * self.SM_COUNT // max(1, total))))
+        few = max(1, -(-max_len // (slice_keys or self.mass_slice_keys_4bit(step.host_kv_lens, num_kv_heads))))
         if self.timing is not None:
             seen = sum(n * kv - n * (n - 1) // 2 for n, kv in zip(counts, step.host_kv_lens))
             self._costs(sum(step.host_kv_lens) * num_kv_heads * (four_bit_token_bytes(head_dim) // 2 + 8), 2 * num_heads * head_dim * seen)
         self._call("attention_4bit", "q3_attention_mass_4bit", what, code, _ptr(q), q_stride, _ptr(pages), pages.shape[0],
                    _ptr(block_table), block_table.shape[1], _ptr(step.kv_lens), _ptr(step.cu_seqlens), _ptr(mass), _ptr(lse), int(have),
                    _ptr(part), slices, step.num_seqs, num_heads, num_kv_heads, head_dim, page_size, float(scale), max_len, observe, most, few)
+
+    def mass_slice_keys_4bit(self, kv_lens, num_kv_heads) -> int:
+        """Keys that a block of the sums of few rows takes, for sequences of these lengths: at least 128, and four blocks an SM or up to twice as
+        many for all keys together (a power of two, so that captured steps of like lengths share their graph)."""
+        per = sum(kv_lens) * num_kv_heads // (4 * self.SM_COUNT)
+        return max(128, 1 << max(0, per.bit_length() - 1))
 
     def evict_4bit(self, *, pages, mass, places, block_table, kv_lens, max_kv_len, keep, first, recent, num_kv_heads, head_dim,
                    page_size):

@@ -34,6 +34,7 @@ class PagedAttention(Part):
         self.budget = ctx.kv_budget
         self._slices_choice = (("decode_slices_4bit", self.num_kv_heads, self.head_dim, self.window, self.num_heads // self.num_kv_heads)
                                if self.four_bit else ("decode_slices", self.num_kv_heads, self.head_dim, self.window))
+        self._sums_choice = ("mass_slice_keys_4bit", self.num_kv_heads)
         if self.num_heads % self.num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         if self.budget is not None and self.window:
@@ -99,12 +100,17 @@ class PagedAttention(Part):
         return groups
 
     def step_choosers(self):
-        """Into how many slices the split-KV decode kernel cuts the longest sequence's keys."""
+        """Into how many slices the split-KV decode kernel cuts the longest sequence's keys, and under a token budget how many keys a block
+        takes for their sums."""
         model = getattr(self.ops, "decode_slices_4bit" if self.four_bit else "decode_slices_for", None)
         if model is None or self.ctx.dtype != torch.bfloat16 or self.head_dim not in (64, 128, 256):
             return {}
         sizes = self._slices_choice[1:]
-        return {self._slices_choice: lambda kv_lens: model(kv_lens, *sizes)}
+        choosers = {self._slices_choice: lambda kv_lens: model(kv_lens, *sizes)}
+        if self.budget is not None:
+            heads = self.num_kv_heads
+            choosers[self._sums_choice] = lambda kv_lens: self.ops.mass_slice_keys_4bit(kv_lens, heads)
+        return choosers
 
     def cache_spec(self):
         if self.four_bit:
@@ -183,8 +189,9 @@ class PagedAttention(Part):
         ops.paged_attention_4bit(qkv, qkv.stride(0), out=out, scale=self.scale, window=self.window, step=step, decode_slices=slices,
                                  lse=lse, **sizes)
         if cache.mass is not None:
+            keys = step.choices.get(self._sums_choice)
             ops.attention_mass_4bit(qkv, qkv.stride(0), mass=cache.mass, scale=self.scale, step=step, observe=self.budget.observe,
-                                    lse=lse, **sizes)
+                                    lse=lse, **({"slice_keys": keys} if keys else {}), **sizes)
 
     def _project_out(self, ctx_out: torch.Tensor) -> torch.Tensor:
         if self.o_bias_vec is not None:
