@@ -73,3 +73,21 @@ def test_scores_that_all_lie_far_from_zero(ops, H, G, D, dtype, slices, sign):  
     for given in {None, lse}:
         mass = t4.mass_of(ops, c, q, [1, 1], lens, H, scale, 1, lse=None if given is None else given.cuda())
         assert bool((mass >= 0).all()) and bool((mass <= H // G).all()) and math.isfinite(float(mass.sum()))
+
+
+@pytest.mark.parametrize("H,G,D,dtype", [(8, 2, 128, BF16), (8, 2, 64, BF16), (4, 2, 256, BF16), (20, 4, 80, BF16), (20, 1, 128, BF16), (4, 2, 16, BF16),
+                                         (6, 2, 240, BF16), (8, 2, 128, F32), (4, 2, 80, F32)])
+def test_single_tokens_from_attention_to_sums(ops, H, G, D, dtype):  # noqa: F811
+    """As a layer under a token budget calls them: log sums are asked for where the decode kernel has them, elsewhere the sums make their own."""
+    lens, page = [1, 16, 100, 333], 16
+    c = p4.Cache(lens, G, D, page, seed=D)
+    q = t4.queries(len(lens), H, D, 6, dtype)
+    rows, new, scale = q.view(-1, H, D), [1] * len(lens), D ** -0.5
+    ok = ops.decode_4bit_ok(q.cuda(), H, G, D)
+    assert ok == (dtype == BF16 and D in (64, 128, 256) and H // G <= 16)
+    got = t4.attend(ops, c, q, new, lens, H, scale, dtype=dtype, lse=ok)
+    got, lse = got if ok else (got, None)
+    t4.check_rows(got, rows, c, new, lens, scale, wide=not ok, dtype=dtype)
+    start = torch.rand((c.pages.shape[0], G, page), generator=torch.Generator().manual_seed(1))
+    mass = t4.mass_of(ops, c, q, new, lens, H, scale, 1, lse=None if lse is None else lse.cuda(), start=start)
+    t4.check_mass(mass, rows, c, new, lens, scale, 1, start=start, dtype=dtype)
