@@ -45,9 +45,10 @@ __device__ __forceinline__ bool store_place(const Store& a, int t, int nkv, int 
 // the rest waits for loads.  One side alone gives nothing: two numbers an instruction (24), angles asked for into L1 (25) or into registers
 // ahead of the squares' sum (26), three heads a thread (41), blocks of 64 to 256 threads (24 to 28).
 //
-// A key near the border between two numbers falls on either side by float32's last bit.  So that it falls where a float32 statement of
-// norm and rotation in PyTorch puts it, heads of 128 and 256 sum their squares four neighbours at a time and then by halves, and products
-// and sums are rounded one by one (14 keys of 59 million fell elsewhere with fused products and another order).
+// A key near the border between two numbers falls on either side by float32's last bit.  So that it falls where element-wise float32
+// operations put it that anybody can repeat, heads of 128 and 256 sum their squares in a stated order, four neighbours at a time and then
+// by halves, and products and sums are rounded one by one (with fused products and another order 14 keys of 59 million fell elsewhere).
+// Heads of 16, 32 and 64 add fused squares, as the general form below does.
 __device__ __forceinline__ float quad_of_squares(const float* v) {
   return __fadd_rn(__fadd_rn(__fadd_rn(__fmul_rn(v[0], v[0]), __fmul_rn(v[1], v[1])), __fmul_rn(v[2], v[2])), __fmul_rn(v[3], v[3]));
 }

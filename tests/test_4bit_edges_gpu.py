@@ -91,3 +91,57 @@ def test_single_tokens_from_attention_to_sums(ops, H, G, D, dtype):  # noqa: F81
     start = torch.rand((c.pages.shape[0], G, page), generator=torch.Generator().manual_seed(1))
     mass = t4.mass_of(ops, c, q, new, lens, H, scale, 1, lse=None if lse is None else lse.cuda(), start=start)
     t4.check_mass(mass, rows, c, new, lens, scale, 1, start=start, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [128, 256])
+def test_the_order_of_a_writes_sums(ops, dtype, D):  # noqa: F811
+    """Heads of 128 and 256, number for number: squares are summed four neighbours at a time, then eight channels of either half of the head
+    with their counterparts, then by halves; products and sums of norm and rotation are rounded one by one.  Stated here by element-wise
+    operations, which leave no order open."""
+    H, G, page, T = 3, 2, 16, 400
+    g = torch.Generator().manual_seed(D)
+    qkv = torch.randn((T, (H + 2 * G) * D), generator=g).to(dtype).cuda()
+    qw, kw = ((1 + 0.1 * torch.randn(D, generator=g)).cuda() for _ in range(2))
+    angle = torch.arange(T)[:, None] * 1e4 ** (-torch.arange(0, D, 2) / D)
+    cos, sin = angle.cos().contiguous().cuda(), angle.sin().contiguous().cuda()
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    table = torch.randperm(T // page, generator=g).int()[None].cuda()
+    pages = torch.zeros((T // page, G, p4.page_bytes(D, page)), dtype=torch.uint8, device="cuda")
+    q = torch.empty((T, H * D), dtype=dtype, device="cuda")
+    ops.qk_norm_rope_store_4bit(qkv, num_heads=H, num_kv_heads=G, head_dim=D, q_weight=qw, k_weight=kw, eps=1e-6, cos=cos, sin=sin, positions=pos,
+                                token_seq=torch.zeros_like(pos), block_table=table, pages=pages, page_size=page, q_out=q)
+    x = qkv.float().view(T, -1, D)
+    square = (x * x).unflatten(-1, (-1, 4))
+    fours = square[..., 0] + square[..., 1]
+    fours = fours + square[..., 2]
+    fours = fours + square[..., 3]  # [T, heads, D / 4]: of channels 4i .. 4i + 3
+    first, second = fours.chunk(2, -1)
+    lanes = (first + second).unflatten(-1, (-1, 2))  # of each eight channels of a half: their first four, their last four
+    while lanes.shape[-2] > 1:
+        low, high = lanes.chunk(2, -2)
+        lanes = low + high
+    mean = (lanes[..., 0, 0] + lanes[..., 0, 1])[..., None] / D
+    y = x * torch.rsqrt(mean + 1e-6)
+    for rows, weight, name in ((y[:, :H], qw, "q"), (y[:, H:H + G], kw, "k")):
+        a, b = (rows * weight).chunk(2, -1)
+        c, s = cos[:, None], sin[:, None]
+        left, right = a * c, b * s
+        top = left - right
+        left, right = b * c, a * s
+        turned = torch.cat([top, left + right], -1)
+        if name == "q":
+            assert torch.equal(q.view(T, H, D), turned.to(dtype))
+        else:
+            keys = turned
+    got = pages[table[0].long()]
+    half, par = D // 2, 4 * p4.groups(D)
+    for which, rows in enumerate((keys, x[:, H + G:])):
+        n, scale, low = p4.quantise(rows.transpose(0, 1).reshape(G * T, D).cpu())
+        words = n.view(G, T, p4.groups(D), -1, 8).transpose(2, 3).reshape(G, T, D)
+        code = (words[..., 0::2] | (words[..., 1::2] << 4)).to(torch.uint8)
+        params = torch.stack([scale, low], -1).reshape(G, T, -1).contiguous().view(torch.uint8)
+        have = got[:, :, which * page * half:(which + 1) * page * half].reshape(-1, G, page, half).transpose(0, 1).reshape(G, T, half)
+        base = 2 * page * half + which * page * par
+        have_par = got[:, :, base:base + page * par].reshape(-1, G, page, par).transpose(0, 1).reshape(G, T, par)
+        assert torch.equal(have.cpu(), code) and torch.equal(have_par.cpu(), params)
