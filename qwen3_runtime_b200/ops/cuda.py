@@ -9,7 +9,6 @@ kernel does not support; they never substitute another code path silently.
 
 from __future__ import annotations
 
-import copy
 import ctypes
 import functools
 import math
@@ -2149,6 +2148,12 @@ class CudaOps:
             if t is not None and t.get_device() != here:
                 raise KernelError(f"{what}: this kernel table launches on cuda:{self._device_index}, a tensor is on {t.device}")
 
+    def _check_step_4bit(self, what, cu, count, *others):
+        """``cu`` of ``count`` numbers, and whatever else of a call lies on the device."""
+        if cu.dtype != torch.int32 or cu.numel() < count or not cu.is_contiguous():
+            raise KernelError(f"{what}: cu_seqlens is dense int32, one more than there are sequences")
+        self._check_here(what, cu, *others)
+
     def _check_cells(self, what, t, dtype, pages, page_size):
         """Sums and places: one number per (page, kv head, token)."""
         if t is not None:
@@ -2240,7 +2245,7 @@ class CudaOps:
         if (len(shape) != 2 or shape[0] < T or shape[1] < H * D or q_stride < H * D or T != step.num_tokens
                 or q.stride() != (q_stride if shape[0] > 1 else q.stride(0), 1)):
             raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step, q_stride apart")
-        self._check_here(what, q, out, lse)
+        self._check_step_4bit(what, step.cu_seqlens, step.num_seqs + 1, q, out, lse, step.kv_longest)
         room = max_pages * page_size
         if step.max_kv_len > room or step.num_seqs > table_rows:
             raise KernelError(f"{what}: {step.num_seqs} sequences of up to {step.max_kv_len} tokens do not fit a block table of "
@@ -2253,6 +2258,9 @@ class CudaOps:
         if lse is not None and (lse.dtype != torch.float32 or lse.dim() != 2 or lse.size(0) != T or lse.size(1) != H or not lse.is_contiguous()):
             raise KernelError(f"{what}: log sums are dense float32 [tokens, heads]")
         if fast and step.decode_only:
+            longest = step.kv_longest
+            if longest is not None and (longest.dtype != torch.int32 or longest.numel() < 1):
+                raise KernelError(f"{what}: kv_longest is one int32")
             return self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, None, step.num_seqs, max_len,
                                      decode_slices or self.decode_slices_4bit(step.host_kv_lens, G, D, window, H // G), out, page_size, scale,
                                      window, step.kv_longest, lse)
@@ -2261,6 +2269,11 @@ class CudaOps:
             return self._general_4bit(q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window)
         # portions of prompts (and single tokens beside them): their sequences' pages unpacked, the kernels for wide pages
         split = fast and D != 256  # prompts apart from single tokens, which are decoded as they are
+        singles = step.single_seqs
+        if (singles is None and step.num_single) or (singles is not None and (
+                singles.dtype != torch.int32 or singles.numel() < step.num_single or not singles.is_contiguous())):
+            raise KernelError(f"{what}: single_seqs is dense int32, one per sequence that brings one token")
+        self._check_here(what, singles)
         cu = step.host_cu_seqlens
         if split and step.num_single:
             singles = [kv for b, kv in enumerate(step.host_kv_lens) if cu[b + 1] - cu[b] == 1]
@@ -2287,7 +2300,8 @@ class CudaOps:
         """Attention of the step's sequences ``first .. end - 1``, whose ``count`` pages are unpacked for it (none of those has more than
         ``longest`` keys)."""
         cu, t0, t1 = step.host_cu_seqlens, step.host_cu_seqlens[first], step.host_cu_seqlens[end]
-        part = copy.copy(step)
+        part = type(step).__new__(type(step))
+        part.__dict__.update(step.__dict__)  # (copy.copy takes five times as long)
         if (first, end) != (0, step.num_seqs):  # a step of these sequences alone, counted from zero
             single = [b for b in range(step.num_seqs) if cu[b + 1] - cu[b] == 1]
             here = [i for i, b in enumerate(single) if first <= b < end]
@@ -2410,10 +2424,10 @@ class CudaOps:
         if self.timing is not None:
             singles = [kv for b, kv in enumerate(step.host_kv_lens) if step.host_cu_seqlens[b + 1] - step.host_cu_seqlens[b] == 1]
             self._costs(sum(singles) * G * four_bit_token_bytes(D) + 4 * num_seqs * H * D, 4 * H * D * sum(singles))
-        self._call("attention_4bit", "q3_decode_attention_4bit", "paged_attention_decode_4bit", _ptr(q), q_stride, _ptr(pages),
-                   pages.shape[0], _ptr(block_table), block_table.shape[1], _ptr(step.kv_lens), _ptr(step.cu_seqlens), _ptr(seq_list),
-                   _ptr(out), mid_o, mid_lse, _ptr(lse), num_seqs, H, G, D, page_size, float(scale), int(window or 0),
-                   slices, max_len, _ptr(longest), _ptr(self._error_word(out.device)))
+        self._call("attention_4bit", "q3_decode_attention_4bit", "paged_attention_decode_4bit", q.data_ptr(), q_stride, pages.data_ptr(),
+                   pages.shape[0], block_table.data_ptr(), block_table.shape[1], step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(),
+                   _ptr(seq_list), out.data_ptr(), mid_o, mid_lse, _ptr(lse), num_seqs, H, G, D, page_size, float(scale), int(window or 0),
+                   slices, max_len, _ptr(longest), self._error_word(out.device).data_ptr())
         return out
 
     def attention_mass_4bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, mass, block_table, page_size, scale, step,
@@ -2427,7 +2441,7 @@ class CudaOps:
         code = _dtype_code(q.dtype)
         self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, step.kv_lens)
         self._check_cells(what, mass, torch.float32, pages, page_size)
-        self._check_here(what, q)
+        self._check_step_4bit(what, step.cu_seqlens, step.num_seqs + 1, q, lse)
         T = step.num_tokens
         if num_heads % num_kv_heads or q_stride % 8 or q.data_ptr() % 16:
             raise KernelError(f"{what}: heads are a multiple of kv heads, rows of queries begin at multiples of 16 bytes")
