@@ -76,3 +76,23 @@ def test_short_portions_beside_a_long_request_take_what_they_hold(ops, new, H, G
     assert torch.cuda.max_memory_allocated() - before <= own + 32 * count * 4 + (16 << 20)
     assert bool((out == 0).all())
     ops.raise_if_kernel_error()
+
+
+def test_a_pool_sized_from_free_memory_leaves_room(tmp_path):
+    """Pages and what prompts unpack beside them stay within the share of the free memory that the cache is given, and the engine runs."""
+    import engine_4bit_cases as ec
+    from helpers import TINY, random_ids
+    from qwen3_runtime_b200.ops.cuda import CudaOps
+
+    ops = CudaOps()
+    torch.cuda.empty_cache()
+    free, _total = torch.cuda.mem_get_info()
+    share = 0.01
+    eng = ec.engine(tmp_path, "E", "bfloat16", ops, "cuda", pages=None, kv_memory_fraction=share)
+    layout, page = eng.runner.storage.layout, TINY["E"]["page_size"]
+    held = eng.cache.num_pages[0] * page
+    longest = min(held, eng.runtime.max_positions)
+    room = max(min(ops.UNPACK_BYTES, layout.unpacked_bytes(held)), layout.unpacked_bytes(longest))
+    assert 0.5 * share * free < eng.runner.storage.nbytes() + room <= share * free + (64 << 20)
+    assert len(eng.generate(random_ids(TINY["E"]["config"].vocab_size, 40, 1), max_tokens=4)) == 4
+    ops.raise_if_kernel_error()
