@@ -46,7 +46,7 @@ class EngineConfig:
     eos_token_id: int | None = None
     cuda_graph: bool = True  # replay captured decode steps
     dtype: str = "bfloat16"
-    kv_memory_fraction: float = 0.85  # share of free device memory given to the pages
+    kv_memory_fraction: float = 0.85  # share of free device memory given to the pages (in 4 bits: and to what prompts unpack of them)
     run_ahead: bool = True  # put the next decode step on the device before reading this one's tokens
     kv_bits: int | None = None  # 4: keys and values are held in 4 bits; None: in the compute dtype
     token_budget: TokenBudget | None = None  # requests are cut to that many cached tokens (or a number: the tokens to keep)

@@ -2231,9 +2231,11 @@ class CudaOps:
                              window=None, decode_slices=None, lse=None):
         """:meth:`paged_attention` over a cache in 4 bits.  A sequence's tokens are the first ``kv_lens`` places of its cache and the
         step's tokens the last of them (``step.kv_lens`` and ``step.host_kv_lens`` count places: without evicted tokens, positions).
-        Single tokens of bfloat16 heads of 64, 128 or 256 read the numbers as they are, on the tensor cores; float32, single tokens
-        of other sizes, and rows that do not begin at 16 bytes, on the FMA pipes (csrc/attention_4bit.cu).  bfloat16 portions of prompts have their sequences' pages unpacked
-        once (values rounded to bfloat16) and go through the kernels for wide pages.  ``step.positions`` are places here.  A table entry that is no page is read nowhere; the rows of a
+        Single tokens of bfloat16 heads of 64, 128 or 256 (up to 16 query heads a kv head) read the numbers as they are, on the tensor cores;
+        float32, single tokens of other sizes, and rows that do not begin at 16 bytes, on the FMA pipes (csrc/attention_4bit.cu).  bfloat16
+        portions of prompts have their sequences' pages unpacked once (values rounded to bfloat16; at most ``UNPACK_BYTES`` at a time, or one
+        sequence) and go through the kernels for wide pages; so do the single tokens beside them, but for heads of 64 and 128, whose numbers
+        are read as they are there too.  ``step.positions`` are places here.  A table entry that is no page is read nowhere; the rows of a
         sequence that sees such a token are undefined, the others are not.
         ``lse`` (float32 ``[T, heads]``, steps of single tokens of those sizes): gets the logarithm of each row's sum."""
         what = "paged_attention_4bit"
@@ -2376,8 +2378,9 @@ class CudaOps:
         return slices
 
     def _decode_slices_4bit(self, rounds, num_kv_heads, head_dim, wide) -> int:
-        """Times in us, fitted to a sweep of 1 to 64 slices over 20 batches of 1 to 128 sequences of 64 to 32,769 tokens on a B200: the choice
-        is 4 % slower than the best one on average, 14 % at worst.  A round of 128 keys of 128 channels takes a block 1.15 alone and
+        """Times in us, fitted to a sweep of 1 to 64 slices over 20 batches of 1 to 128 sequences of 64 to 32,769 tokens on a B200, 17 of them with
+        heads of 128: there the choice is 4 % slower than the best one on average, 14 % at worst.  Sizes of 64 and 256 scale the same
+        constants, and are 7 to 11 % slower than the best on average, 26 to 74 % at worst (12 batches for each of six sizes and groups).  A round of 128 keys of 128 channels takes a block 1.15 alone and
         0.66 for every block on its SM (groups of more than 8 heads 1.69 times as much), a block's beginning and end as much as 2.23
         rounds, of which the SM notices 1.66 where other blocks go on meanwhile; the last blocks end apart by a share of their length.
         A second kernel joins slices in 2.7 and more; clusters do so for nothing, but take a fifth longer, and all have to run at once."""
@@ -2434,7 +2437,7 @@ class CudaOps:
                             observe=None, lse=None, slice_keys=None):
         """Adds to ``mass`` (float32 ``[pages, kv heads, page_size]``) the softmax weights that every sequence's last ``observe`` tokens
         of the step (None: all of them) give to its cached tokens, summed over the query heads of a kv head.  ``lse``: the rows' log
-        sums, when :meth:`paged_attention_4bit` has written them for this step.  A page belongs to one sequence.  ``slice_keys``
+        sums, when :meth:`paged_attention_4bit` has written them for this step (without a window: the weights are those over all keys).  A page belongs to one sequence.  ``slice_keys``
         (:meth:`mass_slice_keys_4bit`): keys that a block takes where a sequence has few rows, for a captured step, whose lengths
         are not known when it is captured; results do not depend on it."""
         what = "attention_mass_4bit"
