@@ -2277,12 +2277,12 @@ class CudaOps:
             raise KernelError(f"{what}: single_seqs is dense int32, one per sequence that brings one token")
         self._check_here(what, singles)
         cu = step.host_cu_seqlens
-        if split and step.num_single:
-            singles = [kv for b, kv in enumerate(step.host_kv_lens) if cu[b + 1] - cu[b] == 1]
-            self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, step.single_seqs, step.num_single, max(singles),
-                              self.decode_slices_4bit(singles, G, D, window, H // G), out, page_size, scale, window, None, None)
         exact = not step.captured_width and len(step.host_kv_lens) >= step.num_seqs  # (else the lengths are those of the moment, up to max_len)
         lens = list(step.host_kv_lens[:step.num_seqs]) if exact else [max_len] * step.num_seqs
+        if split and step.num_single:
+            own = [kv for b, kv in enumerate(lens) if cu[b + 1] - cu[b] == 1]
+            self._decode_4bit(q, q_stride, H, G, D, pages, block_table, step, singles, step.num_single, max(own),
+                              self.decode_slices_4bit(own, G, D, window, H // G), out, page_size, scale, window, None, None)
         counts = unpacked_pages_4bit(cu, lens, page_size, window, 2 if split else 1, exact)
         total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * page_size * D)
         if total <= limit:

@@ -41,7 +41,7 @@ def test_sequences_in_turn(ops, H, G, D, page, window):  # noqa: F811
 @pytest.mark.parametrize("D,page,window", [(128, 16, None), (128, 16, 40), (80, 5, 40)])
 def test_lengths_of_the_moment(ops, D, page, window):  # noqa: F811
     """A step that says how far its lengths may reach, or names none on the host: the device's lengths count, and no page is missing."""
-    H, G, new, lens = 4, 2, [9, 20, 3], [100, 20, 61]
+    H, G, new, lens = 4, 2, [9, 1, 20, 3, 1], [100, 70, 20, 61, 1]
     c = p4.Cache(lens, G, D, page, seed=1, width=-(-200 // page))
     q = t4.queries(sum(new), H, D, 2)
     want = t4.attend(ops, c, q, new, lens, H, D ** -0.5, window=window)
@@ -51,7 +51,39 @@ def test_lengths_of_the_moment(ops, D, page, window):  # noqa: F811
             setattr(step, name, x)
         got = t4.attend(ops, c, q, new, lens, H, D ** -0.5, window=window, step=step)
         t4.check_rows(got, q.view(-1, H, D), c, new, lens, D ** -0.5, window=window, wide=True)
-        assert torch.equal(got, want)
+        cu = step.host_cu_seqlens
+        many = [t for b, n in enumerate(new) if n > 1 for t in range(cu[b], cu[b + 1])]
+        assert torch.equal(got[many], want[many]), "(single tokens: other slices)"
+
+
+@pytest.mark.parametrize("D", [128, 64, 256])
+def test_a_captured_step_of_portions_and_single_tokens(ops, D):  # noqa: F811
+    """Captured while its sequences are short, replayed when they are longer, up to the table that it was captured for."""
+    H, G, page, new, short, long = 8, 2, 16, [1, 20, 1, 3], [5, 20, 9, 3], [250, 60, 140, 256]
+    c = p4.Cache(long, G, D, page, seed=D, width=16)
+    q = t4.queries(sum(new), H, D, 2)
+    step = p4.step_of(new, short, page, captured_width=16)
+    dev, pages, table, out = q.cuda(), c.pages.cuda(), c.table.cuda(), torch.zeros((sum(new), H * D), dtype=BF16, device="cuda")
+
+    def run():
+        ops.paged_attention_4bit(dev, H * D, num_heads=H, pages=pages, block_table=table, out=out, scale=D ** -0.5, step=step, **t4.sizes(c))
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for lens in (long, [n + 2 for n in short]):
+        now = p4.step_of(new, lens, page)
+        for name in ("kv_lens", "positions", "kv_longest"):
+            getattr(step, name).copy_(getattr(now, name))
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.raise_if_kernel_error()
+        cut = p4.Cache.__new__(p4.Cache)
+        cut.__dict__.update(c.__dict__)
+        cut.k, cut.v = ([[x[:, :n] for x in y] for y, n in zip(z, lens)] for z in (c.k, c.v))
+        t4.check_rows(out.cpu().view(-1, H, D), q.view(-1, H, D), cut, new, lens, D ** -0.5, wide=True)
 
 
 @pytest.mark.parametrize("new", [[1] + [20] * 31, [20] * 32])
