@@ -36,6 +36,16 @@ def four_bit_page_bytes(head_dim: int, page_size: int) -> int:
     return -(-page_size * four_bit_token_bytes(head_dim) // 16) * 16
 
 
+def eight_bit_page_bytes(head_dim: int, page_size: int) -> int:
+    """Bytes of one page and kv head held in 8 bits: a byte a number, and the page's two scales (the layout: csrc/eight_bit.cuh)."""
+    return 2 * page_size * head_dim + 16
+
+
+def packed_page_bytes(bits: int, head_dim: int, page_size: int) -> int:
+    """Bytes of one page and kv head held in 4 or 8 bits."""
+    return (four_bit_page_bytes if bits == 4 else eight_bit_page_bytes)(head_dim, page_size)
+
+
 @dataclass(frozen=True)
 class KVLayerSpec:
     """``value_dim``: values have a size of their own (None: the keys' ``head_dim``); keys and values
@@ -44,8 +54,8 @@ class KVLayerSpec:
     ``chunk``: a token reads only the keys of its own chunk of that many tokens (counted from the sequence's
     first token); pages wholly before the current chunk are given back.  A tuple of chunk sizes: several layers read
     this one's keys, each under chunks of its own; a page is given back when none of them needs it any more.
-    ``bits`` 4: keys and values are held in 4 bits, one byte tensor ``[layers, pages + 1, kv_heads, four_bit_page_bytes]``
-    (csrc/four_bit.cuh).  ``sums``: beside them each token's summed attention weight and its position, float32 and int32
+    ``bits`` 4 or 8: keys and values are held in so many bits, one byte tensor ``[layers, pages + 1, kv_heads, packed_page_bytes]``
+    (csrc/four_bit.cuh, csrc/eight_bit.cuh).  ``sums`` (in 4 bits): beside them each token's summed attention weight and its position, float32 and int32
     ``[layers, pages + 1, kv_heads, page_size]``, for requests that are cut to a budget of tokens."""
 
     num_kv_heads: int
@@ -170,8 +180,8 @@ class CacheLayout:
             s = g.layer_spec
             if isinstance(s, LatentLayerSpec):
                 out.append(len(g.cache_ids) * s.width * page_size * dtype_bytes)
-            elif s.bits == 4:
-                out.append(len(g.cache_ids) * s.num_kv_heads * (four_bit_page_bytes(s.head_dim, page_size) + 8 * page_size * s.sums))
+            elif s.bits:
+                out.append(len(g.cache_ids) * s.num_kv_heads * (packed_page_bytes(s.bits, s.head_dim, page_size) + 8 * page_size * s.sums))
             else:
                 per_token = s.num_kv_heads * (s.head_dim + (s.value_dim or s.head_dim))
                 out.append(len(g.cache_ids) * per_token * page_size * dtype_bytes)
@@ -183,9 +193,9 @@ class CacheLayout:
         return sum(self.page_bytes(1, dtype_bytes))
 
     def unpacked_bytes(self, tokens: int) -> int:
-        """Bytes that the attention over prompts of one layer takes to unpack a request of that many tokens from 4 bits (keys and values in
+        """Bytes that the attention over prompts of one layer takes to unpack a request of that many tokens from 4 or 8 bits (keys and values in
         bfloat16; the layers' turns come one after the other); a window reaches over part of it."""
-        specs = [g.layer_spec for g in self.groups if getattr(g.layer_spec, "bits", None) == 4]
+        specs = [g.layer_spec for g in self.groups if getattr(g.layer_spec, "bits", None)]
         return max((4 * s.num_kv_heads * s.head_dim * tokens for s in specs), default=0)
 
     def pages_for_budget(self, budget_bytes: int, page_size: int, dtype_bytes: int, *,

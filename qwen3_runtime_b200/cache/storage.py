@@ -6,7 +6,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .layout import CacheLayout, KVLayerSpec, LatentLayerSpec, StateLayerSpec, flatten_specs, four_bit_page_bytes
+from .layout import CacheLayout, KVLayerSpec, LatentLayerSpec, StateLayerSpec, flatten_specs, packed_page_bytes
 
 
 @dataclass
@@ -22,7 +22,7 @@ class CacheLayerView:
     state: torch.Tensor | None  # [slots + 1, *shape]
     writes: bool = True
     latent_pages: torch.Tensor | None = None  # [pages + 1, page_size, width] (a latent group)
-    packed_pages: torch.Tensor | None = None  # uint8 [pages + 1, kv_heads, bytes of a page] (a group held in 4 bits)
+    packed_pages: torch.Tensor | None = None  # uint8 [pages + 1, kv_heads, bytes of a page] (a group held in 4 or 8 bits)
     mass: torch.Tensor | None = None  # float32 [pages + 1, kv_heads, page_size]: summed attention weights (a group with sums)
     places: torch.Tensor | None = None  # int32, the same shape: positions
 
@@ -46,9 +46,10 @@ class CacheStorage:
         self.sums: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}  # group -> (summed weights, positions)
         for gi, g in enumerate(layout.groups):
             s = g.layer_spec
-            if isinstance(s, KVLayerSpec) and s.bits == 4:
+            if isinstance(s, KVLayerSpec) and s.bits:
                 shape = (len(g.cache_ids), self.num_pages[layout.paged_groups.index(gi)] + 1, s.num_kv_heads)
-                self.tensors.append(torch.zeros((*shape, four_bit_page_bytes(s.head_dim, page_size)), dtype=torch.uint8, device=device))
+                self.tensors.append(torch.zeros((*shape, packed_page_bytes(s.bits, s.head_dim, page_size)), dtype=torch.uint8,
+                                                device=device))
                 if s.sums:
                     self.sums[gi] = (torch.zeros((*shape, page_size), dtype=torch.float32, device=device),
                                      torch.zeros((*shape, page_size), dtype=torch.int32, device=device))
@@ -91,7 +92,7 @@ class CacheStorage:
         if isinstance(t, tuple):
             return CacheLayerView(gi, self.layout.paged_groups.index(gi), self.page_size, g.spec.window,
                                   t[0][li], t[1][li], None, writes)
-        if g.spec.paged and getattr(g.layer_spec, "bits", None) == 4:
+        if g.spec.paged and getattr(g.layer_spec, "bits", None):
             mass, places = self.sums.get(gi, (None, None))
             return CacheLayerView(gi, self.layout.paged_groups.index(gi), self.page_size, g.spec.window, None, None, None, writes,
                                   packed_pages=t[li], mass=None if mass is None else mass[li],
@@ -130,8 +131,8 @@ class CacheStorage:
         if pages and isinstance(t, tuple):
             for part in t:
                 part[:, torch.tensor(pages, dtype=torch.long, device=part.device)] = value
-        elif pages and getattr(self.layout.groups[gi].layer_spec, "bits", None) == 4:
-            t[:, torch.tensor(pages, dtype=torch.long, device=t.device)] = 255  # parameters that are not numbers
+        elif pages and getattr(self.layout.groups[gi].layer_spec, "bits", None):
+            t[:, torch.tensor(pages, dtype=torch.long, device=t.device)] = 255  # parameters, in 8 bits codes too, that are not numbers
         elif pages and isinstance(self.layout.groups[gi].layer_spec, LatentLayerSpec):
             t[:, torch.tensor(pages, dtype=torch.long, device=t.device)] = value
         elif pages:

@@ -39,8 +39,8 @@ def _generate(argv: list[str]) -> int:
     parser.add_argument("--seed", type=int, default=None, help="sampling seed")
     parser.add_argument("--block-size", type=int, default=16)
     parser.add_argument("--num-kv-blocks", type=int, default=None)
-    parser.add_argument("--kv-bits", type=int, default=None, choices=[4],
-                        help="hold keys and values in 4 bits. Default: in the compute dtype.")
+    parser.add_argument("--kv-bits", type=int, default=None, choices=[4, 8],
+                        help="hold keys and values in 4 or 8 bits. Default: in the compute dtype.")
     parser.add_argument("--token-budget", type=int, default=None,
                         help="cached tokens that a request keeps (needs --kv-bits 4): its first, its last and the most attended")
     parser.add_argument("--max-num-seqs", type=int, default=1)

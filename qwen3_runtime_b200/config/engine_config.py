@@ -25,14 +25,14 @@ def canonical_dtype(name: str) -> str:
 
 
 def canonical_cache(kv_bits, token_budget):
-    """``(kv_bits, TokenBudget | None)`` of what was given: 4 or None, and a budget or the number of tokens to keep."""
-    if kv_bits is not None and (isinstance(kv_bits, bool) or kv_bits != 4):
-        raise ValueError(f"kv_bits must be 4 (or None: keys and values in the compute dtype), got {kv_bits!r}")
+    """``(kv_bits, TokenBudget | None)`` of what was given: 4, 8 or None, and a budget or the number of tokens to keep."""
+    if kv_bits is not None and (isinstance(kv_bits, bool) or kv_bits not in (4, 8)):
+        raise ValueError(f"kv_bits must be 4 or 8 (or None: keys and values in the compute dtype), got {kv_bits!r}")
     if token_budget is not None and not isinstance(token_budget, TokenBudget):
         if isinstance(token_budget, bool) or not isinstance(token_budget, int):
             raise ValueError(f"token_budget must be a number of tokens or a TokenBudget, got {token_budget!r}")
         token_budget = TokenBudget(token_budget)
-    if token_budget is not None and kv_bits is None:
+    if token_budget is not None and kv_bits != 4:
         raise ValueError("a token budget needs kv_bits=4: the weights are summed by the attention over a cache in 4 bits")
     return kv_bits, token_budget
 
@@ -46,9 +46,9 @@ class EngineConfig:
     eos_token_id: int | None = None
     cuda_graph: bool = True  # replay captured decode steps
     dtype: str = "bfloat16"
-    kv_memory_fraction: float = 0.85  # share of free device memory given to the pages (in 4 bits: and to what prompts unpack of them)
+    kv_memory_fraction: float = 0.85  # share of free device memory given to the pages (in 4 and 8 bits: and to what prompts unpack of them)
     run_ahead: bool = True  # put the next decode step on the device before reading this one's tokens
-    kv_bits: int | None = None  # 4: keys and values are held in 4 bits; None: in the compute dtype
+    kv_bits: int | None = None  # 4 or 8: keys and values are held in so many bits; None: in the compute dtype
     token_budget: TokenBudget | None = None  # requests are cut to that many cached tokens (or a number: the tokens to keep)
 
     def __post_init__(self) -> None:

@@ -49,14 +49,6 @@ __device__ __forceinline__ bool store_place(const Store& a, int t, int nkv, int 
 // operations put it that anybody can repeat, heads of 128 and 256 sum their squares in a stated order, four neighbours at a time and then
 // by halves, and products and sums are rounded one by one (with fused products and another order 14 keys of 59 million fell elsewhere).
 // Heads of 16, 32 and 64 add fused squares, as the general form below does.
-__device__ __forceinline__ float quad_of_squares(const float* v) {
-  return __fadd_rn(__fadd_rn(__fadd_rn(__fmul_rn(v[0], v[0]), __fmul_rn(v[1], v[1])), __fmul_rn(v[2], v[2])), __fmul_rn(v[3], v[3]));
-}
-__device__ __forceinline__ void turn_rounded(float& a, float& b, float cs, float sn) {
-  const float x = a, y = b;
-  a = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
-  b = __fadd_rn(__fmul_rn(y, cs), __fmul_rn(x, sn));
-}
 __device__ __forceinline__ float least_or_nan(float x, float y) {
   float z;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));

@@ -47,3 +47,14 @@ __device__ __forceinline__ void rotate_chunks(float (&a)[8], float (&b)[8], cons
                                               const float* __restrict__ sin_row, int c, int half, int pairing) {
   rotate_by(a, b, load_angles(cos_row, sin_row, c, half, pairing), pairing);
 }
+
+// For rows that are rounded to few bits afterwards: squares summed four neighbours at a time and then by halves, products and sums
+// rounded one by one, so that anybody can repeat which side of a border a value falls on (cache_4bit.cu, cache_8bit.cu).
+__device__ __forceinline__ float quad_of_squares(const float* v) {
+  return __fadd_rn(__fadd_rn(__fadd_rn(__fmul_rn(v[0], v[0]), __fmul_rn(v[1], v[1])), __fmul_rn(v[2], v[2])), __fmul_rn(v[3], v[3]));
+}
+__device__ __forceinline__ void turn_rounded(float& a, float& b, float cs, float sn) {
+  const float x = a, y = b;
+  a = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
+  b = __fadd_rn(__fmul_rn(y, cs), __fmul_rn(x, sn));
+}

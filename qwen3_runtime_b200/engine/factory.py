@@ -32,11 +32,13 @@ def default_ops(groups=None):
 
 def build_model(config, source, *, dtype: str = "bfloat16", device="cuda", ops=None, kv_bits: int | None = None,
                 token_budget: TokenBudget | None = None) -> DecoderModel:
-    """A loaded :class:`DecoderModel` for a typed config and a tensor source.  ``kv_bits`` 4: keys and values are held in 4 bits;
+    """A loaded :class:`DecoderModel` for a typed config and a tensor source.  ``kv_bits`` 4 or 8: keys and values are held in so many bits;
     ``token_budget``: requests are cut to that many cached tokens.  A model with a part that cannot do so is refused."""
     kv_bits, token_budget = canonical_cache(kv_bits, token_budget)
     arch = architecture_for_config(config)
     ops = ops if ops is not None else default_ops()
+    if kv_bits == 8 and not hasattr(ops, "paged_attention_8bit"):
+        raise ValueError(f"kv_bits=8: the kernel table {getattr(ops, 'name', type(ops).__name__)!r} has no attention over a cache in 8 bits")
     ctx = BuildContext(dtype=_TORCH_DTYPE[canonical_dtype(dtype)], device=torch.device(device), ops=ops, kv_bits=kv_bits,
                        kv_budget=token_budget)
     model = DecoderModel(arch.build_spec(config), ctx)
@@ -81,7 +83,7 @@ UNLIMITED_POSITIONS = 1 << 30  # a model none of whose parts limits the position
 
 def beside_unpacked(total: int, layout, block_size: int, longest: int, at_once: int, max_num_seqs: int,
                     max_num_batched_tokens: int | None) -> int:
-    """What of ``total`` bytes the pages of a cache in 4 bits can have when the steps' attention over prompts unpacks its sequences beside
+    """What of ``total`` bytes the pages of a cache in 4 or 8 bits can have when the steps' attention over prompts unpacks its sequences beside
     them: ``at_once`` bytes at a time, or one request of ``longest`` tokens if that is more; never more than the pages hold."""
 
     def room(pages_bytes: int) -> int:
@@ -100,7 +102,7 @@ def build_runtime(model: DecoderModel, *, max_positions: int | None = None, bloc
     """Cache and step function for a loaded model.  ``max_positions`` defaults to what the
     model's own parts can serve (the shortest position table among them).  ``num_kv_blocks``:
     pages of every paged group, one count per paged group, or None to size the pools from
-    ``kv_budget`` bytes (default: ``kv_memory_fraction`` of the free device memory; for a cache in 4 bits what prompts unpack
+    ``kv_budget`` bytes (default: ``kv_memory_fraction`` of the free device memory; for a cache in 4 or 8 bits what prompts unpack
     from it is kept free of that)."""
     if max_positions is None:
         max_positions = model.position_limit() or UNLIMITED_POSITIONS
@@ -114,7 +116,7 @@ def build_runtime(model: DecoderModel, *, max_positions: int | None = None, bloc
             else:
                 free, _total = torch.cuda.mem_get_info(ctx.device)
                 kv_budget = int(free * kv_memory_fraction)
-                if ctx.kv_bits == 4 and ctx.dtype == torch.bfloat16:
+                if ctx.kv_bits is not None and ctx.dtype == torch.bfloat16:
                     longest = max_positions
                     if ctx.kv_budget is not None and max_num_batched_tokens is not None:
                         longest = min(longest, ctx.kv_budget.keep + ctx.kv_budget.slack + max_num_batched_tokens)

@@ -29,8 +29,8 @@ class LLM:
                  architecture: str | None = None, max_num_seqs: int = 4, max_num_batched_tokens: int = 256,
                  seed: int = 0, dtype: str = "bfloat16", **factory_kwargs):
         """``model=None``: random weights (``seed``) for ``config``, or for the tiny configuration
-        that the registered ``architecture`` (default: the first registered) offers.  ``kv_bits=4`` holds keys and values in 4
-        bits, ``token_budget`` (a number or a ``TokenBudget``) cuts requests to that many cached tokens."""
+        that the registered ``architecture`` (default: the first registered) offers.  ``kv_bits=8`` or ``4`` holds keys and
+        values in so many bits, ``token_budget`` (with 4; a number or a ``TokenBudget``) cuts requests to that many cached tokens."""
         self.tokenizer = tokenizer
         common = dict(max_num_seqs=max_num_seqs, max_num_batched_tokens=max_num_batched_tokens, dtype=dtype)
         if model is not None:

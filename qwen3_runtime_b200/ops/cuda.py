@@ -16,7 +16,7 @@ from ctypes import c_float, c_int, c_long, c_void_p
 
 import torch
 
-from ..cache.layout import four_bit_page_bytes, four_bit_token_bytes
+from ..cache.layout import eight_bit_page_bytes, four_bit_page_bytes, four_bit_token_bytes
 from . import build
 
 _CODES = {1: "unsupported size or option", 2: "CUDA launch failed", 3: "bad argument"}
@@ -253,6 +253,20 @@ _SIGNATURES = {
                                    c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
                                    c_int, c_void_p],
     },
+    "cache_8bit": {
+        "q3_store_8bit": [c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p,
+                          c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int,
+                          c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+        "q3_unpack_8bit": [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
+                           c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    },
+    "attention_8bit": {
+        "q3_decode_attention_8bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int,
+                                     c_void_p, c_void_p, c_void_p],
+        "q3_general_attention_8bit": [c_int, c_void_p, c_long, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
+    },
     "gemm_f32": {
         "q3_gemm_f32": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
         "q3_gemm_f32_split_segments": [c_int, c_int],
@@ -487,17 +501,18 @@ def chunk_segment(cu, H, D, Dv, sms, seg) -> int:
     return found
 
 
-def unpacked_pages_4bit(cu, kv_lens, page_size, window=None, least=1, exact=True) -> list:
+def unpacked_pages_4bit(cu, kv_lens, page_size, window=None, least=1, exact=True, keep_first=0) -> list:
     """Pages that attention over prompts reads of each sequence of a step (tokens ``cu[b]`` to ``cu[b + 1] - 1``, ``kv_lens[b]`` keys): from
-    the first that its first new token's window reaches to the last; none of a sequence that brings fewer than ``least`` tokens.  Not
+    the first that its first new token's window reaches to the last, and those of its first ``keep_first`` tokens; none of a sequence that brings fewer than ``least`` tokens.  Not
     ``exact``: as many as any shorter length asks for, too."""
     counts = []
     for b, kv in enumerate(kv_lens):
         new, pages = cu[b + 1] - cu[b], -(-kv // page_size)
         if window and exact:
-            pages -= max(0, kv - new - window + 1) // page_size
+            before = max(0, kv - new - window + 1) // page_size
+            pages -= before - min(before, -(-keep_first // page_size))
         elif window:
-            pages = min(pages, -(-(new + window) // page_size) + 1)
+            pages = min(pages, -(-(new + window) // page_size) + 1 + -(-keep_first // page_size))
         counts.append(pages if new >= least else 0)
     return counts
 
@@ -522,6 +537,14 @@ def _four_bit_record(head_dim: int, page_size: int) -> int:
     if head_dim % 16 or not 16 <= head_dim <= 256 or page_size < 1:
         return 0
     return four_bit_page_bytes(head_dim, page_size)
+
+
+@functools.lru_cache(maxsize=None)
+def _eight_bit_record(head_dim: int, page_size: int) -> int:
+    """The same of a page in 8 bits."""
+    if head_dim % 16 or not 16 <= head_dim <= 256 or not 1 <= page_size < 1 << 23:
+        return 0
+    return eight_bit_page_bytes(head_dim, page_size)
 
 
 class CudaOps:
@@ -2125,8 +2148,8 @@ class CudaOps:
     EVICT_KEYS = 49152  # tokens of a sequence whose keys one block sorts in shared memory; longer ones use scratch
     EVICT_TOGETHER = 512  # moves that the choosing kernel makes itself; more have a kernel of their own
 
-    def _check_4bit(self, what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens=None, layers=False):
-        record = _four_bit_record(head_dim, page_size)
+    def _check_4bit(self, what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens=None, layers=False, record_of=_four_bit_record):
+        record = record_of(head_dim, page_size)
         if not record or num_kv_heads < 1:
             raise KernelError(f"{what}: head sizes are multiples of 16 up to 256, pages and heads at least one "
                               f"(got head_dim={head_dim}, page_size={page_size}, num_kv_heads={num_kv_heads})")
@@ -2298,9 +2321,10 @@ class CudaOps:
     # more by itself is taken alone).
     UNPACK_BYTES = 1 << 30
 
-    def _prompts_4bit(self, q, q_stride, H, G, D, pages, block_table, step, first, end, count, longest, split, out, page_size, scale, window):
+    def _prompts_4bit(self, q, q_stride, H, G, D, pages, block_table, step, first, end, count, longest, split, out, page_size, scale, window,
+                      keep_first=None):
         """Attention of the step's sequences ``first .. end - 1``, whose ``count`` pages are unpacked for it (none of those has more than
-        ``longest`` keys)."""
+        ``longest`` keys).  ``keep_first``: a number for a cache in 8 bits, None for one in 4."""
         cu, t0, t1 = step.host_cu_seqlens, step.host_cu_seqlens[first], step.host_cu_seqlens[end]
         part = type(step).__new__(type(step))
         part.__dict__.update(step.__dict__)  # (copy.copy takes five times as long)
@@ -2321,14 +2345,15 @@ class CudaOps:
         width = -(-longest // page_size)
         table = torch.empty((part.num_seqs, width), dtype=torch.int32, device=out.device)
         if self.timing is not None:
-            self._costs(2 * k.numel() * k.element_size() + count * G * four_bit_page_bytes(D, page_size))
-        self._call("cache_4bit", "q3_unpack_4bit", "unpack_4bit", _dtype_code(k.dtype), _ptr(pages), pages.shape[0], G, D, page_size,
+            self._costs(2 * k.numel() * k.element_size() + count * pages.shape[-1] * G)
+        bits, kept = ("4bit", ()) if keep_first is None else ("8bit", (keep_first,))
+        self._call(f"cache_{bits}", f"q3_unpack_{bits}", f"unpack_{bits}", _dtype_code(k.dtype), _ptr(pages), pages.shape[0], G, D, page_size,
                    _ptr(block_table), block_table.shape[1], _ptr(part.kv_lens), part.num_seqs, longest, _ptr(part.cu_seqlens),
-                   2 if split else 1, int(window or 0), count, width, k.data_ptr(), v.data_ptr(), _ptr(table))
+                   2 if split else 1, int(window or 0), *kept, count, width, k.data_ptr(), v.data_ptr(), _ptr(table))
         # the wide kernels number a token by its place: kv_lens and cu_seqlens say it, or for the general kernel `positions`
         self.paged_attention(q, q_stride, num_heads=H, num_kv_heads=G, head_dim=D, k_pages=k, v_pages=v, block_table=table,
                              token_seq=part.token_seq, positions=part.positions, out=out, page_size=page_size, scale=scale,
-                             window=window, step=part)
+                             window=window, keep_first=keep_first, step=part)
 
     GENERAL_SLICE = 256  # keys with a softmax of their own (csrc/attention_4bit.cu)
 
@@ -2519,6 +2544,237 @@ class CudaOps:
         self._call("cache_4bit", "q3_evict_4bit", what, _ptr(pages), layers, pages.shape[-3], num_kv_heads, head_dim, page_size,
                    _ptr(mass), _ptr(places), _ptr(block_table), block_table.shape[1], _ptr(kv_lens), B, max_kv_len, int(keep),
                    int(first), int(recent), cap, _ptr(spill), _ptr(lists))
+
+    # ---- a cache in 8 bits (csrc/eight_bit.cuh says how a page is laid out and how values are rounded) ----------------------
+    def qk_norm_rope_store_8bit(self, qkv, *, num_heads, num_kv_heads, head_dim, q_weight, k_weight, eps, cos, sin, step, block_table, pages,
+                                page_size, write_kv=True, pairing="half", q_out=None):
+        """:meth:`qk_norm_rope_store` for a cache in 8 bits: per-head q/k norm, rotation by ``step.positions``, and the write of k and v into
+        ``pages`` (uint8 ``[pages, kv heads, eight_bit_page_bytes(head_dim, page_size)]``).  A sequence's new tokens are the last of its
+        ``step.kv_lens`` places, so what its last page held before is known: it goes on under a scale that grows when it has to (a page that
+        gets its first token starts anew).  A page belongs to one sequence; tokens whose place or page lies outside the table or
+        the pages are written nowhere.  Queries go to ``q_out`` ``[T, num_heads * head_dim]``, or are changed in place."""
+        what = "qk_norm_rope_store_8bit"
+        D, dtype, shape, stride = head_dim, qkv.dtype, qkv.shape, qkv.stride()
+        (num_pages, *_), (num_seqs, max_pages) = self._check_4bit(what, pages, num_kv_heads, D, page_size, block_table, step.kv_lens,
+                                                                  record_of=_eight_bit_record)
+        if len(shape) != 2 or stride[1] != 1 or shape[1] < (num_heads + (2 * num_kv_heads if write_kv else 0)) * D:
+            raise KernelError(f"{what}: the projection is [tokens, heads * head_dim] with unit-stride rows")
+        T, q_stride, seqs = shape[0], stride[0], step.num_seqs
+        if T != step.num_tokens or seqs > num_seqs:
+            raise KernelError(f"{what}: the projection has a row per token of the step, the block table a row per sequence "
+                              f"(got {T} and {num_seqs} for {step.num_tokens} and {seqs})")
+        if q_out is None:
+            q_out = qkv
+        else:
+            shape, stride = q_out.shape, q_out.stride()
+            if (q_out.dtype != dtype or len(shape) != 2 or shape[0] != T or shape[1] < num_heads * D or (T and stride[1] != 1)):
+                raise KernelError(f"{what}: queries go to [tokens, heads * head_dim] of the projection's type, unit-stride rows")
+        positions = step.positions
+        if positions.dtype != torch.int32 or positions.numel() < T or not positions.is_contiguous():
+            raise KernelError(f"{what}: positions are dense int32, one per token")
+        for w in (q_weight, k_weight):
+            if w is not None and (w.dtype != torch.float32 or w.numel() != D or not w.is_contiguous()):
+                raise KernelError(f"{what}: norm weights are dense float32 vectors of head_dim")
+        rot_half = max_pos = 0
+        if cos is not None or sin is not None:
+            if cos is None or sin is None:
+                raise KernelError(f"{what}: cos and sin come together")
+            shape = cos.shape
+            if (len(shape) != 2 or shape != sin.shape or shape[0] < 1 or 2 * shape[1] > D or cos.dtype != torch.float32
+                    or sin.dtype != torch.float32 or not cos.is_contiguous() or not sin.is_contiguous()):
+                raise KernelError(f"{what}: rotation tables are dense float32 [positions, pairs] of one shape, at least one position")
+            max_pos, rot_half = shape
+        self._check_step_4bit(what, step.cu_seqlens, seqs + 1, qkv, q_out, positions, q_weight, k_weight, cos, sin)
+        units, most_new = self._written_pages(what, step, page_size) if write_kv else (0, 1)
+        if self.timing is not None:
+            e = qkv.element_size()
+            self._costs(T * (2 * num_heads + 2 * num_kv_heads) * D * e + 2 * T * num_kv_heads * D)
+        self._call("cache_8bit", "q3_store_8bit", what, _dtype_code(dtype), qkv.data_ptr(), q_stride, q_out.data_ptr(), stride[0],
+                   num_heads, num_kv_heads, D, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin), rot_half, max_pos,
+                   positions.data_ptr(), step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(), block_table.data_ptr(), max_pages, seqs,
+                   pages.data_ptr(), num_pages, page_size, T, units, most_new, int(step.decode_only), self.PAIRINGS[pairing],
+                   _ptr(self._error_word(qkv.device)))
+        return q_out
+
+    @staticmethod
+    def _written_pages(what, step, page_size):
+        """Pages that get tokens, at most, and the most tokens that a sequence brings: known from how many each brings, so that a captured
+        step holds for all lengths."""
+        if step.decode_only:
+            if step.num_tokens != step.num_seqs:
+                raise KernelError(f"{what}: a step of single tokens has as many tokens as sequences")
+            return step.num_seqs, 1
+        found = step.extras.get(("written_pages", page_size))
+        if found is None:
+            cu = step.host_cu_seqlens
+            if len(cu) <= step.num_seqs or cu[0] != 0 or cu[step.num_seqs] != step.num_tokens:
+                raise KernelError(f"{what}: host_cu_seqlens are the sequences' first tokens and the number of all")
+            news = [cu[b + 1] - cu[b] for b in range(step.num_seqs)]
+            units = sum((n + page_size - 2) // page_size + 1 for n in news if n > 0)
+            found = step.extras[("written_pages", page_size)] = (units, max([1, *news]))
+        return found
+
+    def unpack_8bit(self, pages, *, num_kv_heads, head_dim, page_size, block_table, kv_lens, max_kv_len, dtype):
+        """Keys and values of the sequences' first ``max_kv_len`` tokens as wide pages ``[sequences * n, kv heads, page_size, head_dim]``
+        of ``dtype``, ``n = ceil(max_kv_len / page_size)`` pages per sequence in order; zero behind a sequence's last token.  Exact."""
+        what = "unpack_8bit"
+        _, (B, width) = self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens, record_of=_eight_bit_record)
+        n = -(-int(max_kv_len) // page_size)
+        if n > width or max_kv_len < 0:
+            raise KernelError(f"{what}: max_kv_len={max_kv_len} does not fit a block table of {width} pages")
+        k = torch.empty((B * n, num_kv_heads, page_size, head_dim), dtype=dtype, device=pages.device)
+        v = torch.empty_like(k)
+        if self.timing is not None:
+            self._costs(2 * k.numel() * k.element_size() + B * n * num_kv_heads * eight_bit_page_bytes(head_dim, page_size))
+        self._call("cache_8bit", "q3_unpack_8bit", what, _dtype_code(dtype), pages.data_ptr(), pages.shape[0], num_kv_heads, head_dim,
+                   page_size, block_table.data_ptr(), width, _ptr(kv_lens), B, int(max_kv_len), None, 0, 0, 0, 0, n, k.data_ptr(), v.data_ptr(),
+                   None)
+        return k, v
+
+    def paged_attention_8bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, block_table, out, page_size, scale, step,
+                             window=None, keep_first=0, decode_slices=None):
+        """:meth:`paged_attention` over a cache in 8 bits; ``window``: a token sees that many tokens up to itself; ``keep_first``: with a window,
+        the sequence's first tokens as well.  A sequence's tokens are the first ``kv_lens`` places of its cache and the step's tokens the last
+        of them; ``step.positions`` are places here.  Single tokens of bfloat16 heads of 64, 128 or 256 (up to 16 query heads a kv head)
+        read the codes as they are, on the tensor cores; float32, single tokens of other sizes, and rows that do not begin at 16
+        bytes, on the FMA pipes (csrc/attention_8bit.cu).  bfloat16 portions of prompts have their sequences' pages unpacked once (exactly; at
+        most ``UNPACK_BYTES`` at a time, or one sequence) and go through the kernels for wide pages; so do the single tokens beside them,
+        but for heads of 64 and 128, whose codes are read as they are there too.  A table entry that is no page is read nowhere; the rows
+        of a sequence that sees such a token are undefined, the others are not."""
+        what = "paged_attention_8bit"
+        D, G, H, dtype, shape, rows = head_dim, num_kv_heads, num_heads, out.dtype, q.shape, out.shape
+        _, (table_rows, max_pages) = self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens, record_of=_eight_bit_record)
+        window, keep_first = int(window or 0), int(keep_first or 0)
+        if window < 0 or keep_first < 0 or window + keep_first > 1 << 30:
+            raise KernelError(f"{what}: a window and the first tokens are no fewer than none (got {window}, {keep_first})")
+        keep_first = keep_first if window else 0
+        if H < 1 or H % G or q.dtype != dtype or len(rows) != 2 or rows[1] != H * D or not out.is_contiguous():
+            raise KernelError(f"{what}: out is dense [tokens, heads * head_dim] of the queries' type, heads a multiple of kv heads")
+        T = rows[0]
+        if (len(shape) != 2 or shape[0] < T or shape[1] < H * D or q_stride < H * D or T != step.num_tokens
+                or q.stride() != (q_stride if shape[0] > 1 else q.stride(0), 1)):
+            raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step, q_stride apart")
+        longest = step.kv_longest
+        self._check_step_4bit(what, step.cu_seqlens, step.num_seqs + 1, q, out, longest)
+        room = max_pages * page_size
+        if step.max_kv_len > room or step.num_seqs > table_rows:
+            raise KernelError(f"{what}: {step.num_seqs} sequences of up to {step.max_kv_len} tokens do not fit a block table of "
+                              f"{table_rows} x {max_pages} pages")
+        max_len = min(step.captured_width * page_size, room) if step.captured_width else step.max_kv_len
+        fast = (dtype == torch.bfloat16 and D in (64, 128, 256) and H // G <= 16 and q_stride % 8 == 0 and q.data_ptr() % 16 == 0
+                and out.data_ptr() % 8 == 0)
+        if fast and step.decode_only:
+            if longest is not None and (longest.dtype != torch.int32 or longest.numel() < 1):
+                raise KernelError(f"{what}: kv_longest is one int32")
+            return self._decode_8bit(q, q_stride, H, G, D, pages, block_table, step, None, step.num_seqs, max_len,
+                                     decode_slices or self.decode_slices_8bit(step.host_kv_lens, G, D, window, H // G, keep_first), out,
+                                     page_size, scale, window, keep_first, longest)
+        aligned = q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0  # what the kernels for wide pages go by
+        if dtype == torch.float32 or (step.decode_only and not fast) or not aligned:
+            return self._general_8bit(q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window, keep_first)
+        # portions of prompts (and single tokens beside them): their sequences' pages unpacked, the kernels for wide pages
+        split = fast and D != 256  # prompts apart from single tokens, which are decoded as they are
+        singles = step.single_seqs
+        if (singles is None and step.num_single) or (singles is not None and (
+                singles.dtype != torch.int32 or singles.numel() < step.num_single or not singles.is_contiguous())):
+            raise KernelError(f"{what}: single_seqs is dense int32, one per sequence that brings one token")
+        self._check_here(what, singles)
+        cu = step.host_cu_seqlens
+        exact = not step.captured_width and len(step.host_kv_lens) >= step.num_seqs  # (else the lengths are those of the moment, up to max_len)
+        lens = list(step.host_kv_lens[:step.num_seqs]) if exact else [max_len] * step.num_seqs
+        if split and step.num_single:
+            own = [kv for b, kv in enumerate(lens) if cu[b + 1] - cu[b] == 1]
+            self._decode_8bit(q, q_stride, H, G, D, pages, block_table, step, singles, step.num_single, max(own),
+                              self.decode_slices_8bit(own, G, D, window, H // G, keep_first), out, page_size, scale, window, keep_first, None)
+        counts = unpacked_pages_4bit(cu, lens, page_size, window, 2 if split else 1, exact, keep_first)
+        total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * page_size * D)
+        if total <= limit:
+            runs = [(0, len(counts), total)] if total else []
+        else:
+            runs = [(first, end, sum(counts[first:end])) for first, end in runs_within(counts, limit)]
+        for first, end, count in runs:
+            most = max([n for n, c in zip(lens[first:end], counts[first:end]) if c])
+            self._prompts_4bit(q, q_stride, H, G, D, pages, block_table, step, first, end, count, most, split, out, page_size, scale, window,
+                               keep_first)
+        return out
+
+    def _general_8bit(self, q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window, keep_first):
+        code, T = _dtype_code(out.dtype), out.size(0)
+        for t in (step.token_seq, step.positions):
+            if t.dtype != torch.int32 or t.numel() < T or not t.is_contiguous():
+                raise KernelError("paged_attention_8bit: token_seq and positions are dense int32, one per token")
+        self._check_here("paged_attention_8bit", step.token_seq, step.positions)
+        slices, mid_o, mid_ml = -(-max_len // self.GENERAL_SLICE), None, None
+        blocks = T * G * -(-(H // G) // 8)
+        # enough blocks without, or more to keep of the slices than 256 MB: each block goes through all slices (the same bits)
+        if slices < 2 or blocks >= 4 * self.SM_COUNT or T * H * slices * D > 1 << 26:
+            slices = 0
+        else:
+            mid_o = torch.empty((T, H, slices, D), dtype=torch.float32, device=out.device)
+            mid_ml = torch.empty((T, H, slices, 2), dtype=torch.float32, device=out.device)
+            self.launches += 1
+        if self.timing is not None:
+            self._costs(*self._attention_cost(step, H, G, D, out))
+        self._call("attention_8bit", "q3_general_attention_8bit", "paged_attention_general_8bit", code, _ptr(q), q_stride, _ptr(pages),
+                   pages.shape[0], _ptr(block_table), block_table.shape[1], block_table.shape[0], _ptr(step.token_seq),
+                   _ptr(step.positions), _ptr(out), _ptr(mid_o), _ptr(mid_ml), slices, T, H, G, D, page_size, float(scale), window, keep_first)
+        return out
+
+    # blocks of decode attention over 8-bit numbers that an SM holds, by head size
+    DECODE_8BIT_BLOCKS_PER_SM = {64: 4, 128: 2, 256: 2}
+
+    def decode_slices_8bit(self, kv_lens, num_kv_heads, head_dim, window=None, group=1, keep_first=0) -> int:
+        """Into how many slices the longest of these sequences' keys are cut by decode attention over a cache in 8 bits (a shorter
+        sequence is cut into fewer of that length); negative: they are joined by a second kernel and not by the blocks of a cluster."""
+        cap = window + 15 + -(-keep_first // 16) * 16 if window else 1 << 30
+        unit = 64 if head_dim == 256 else 128  # keys that a block takes at a time
+        rounds = tuple(-(-min(n, cap) // unit) for n in kv_lens)
+        key = ("8bit", num_kv_heads, head_dim, group > 8, rounds)
+        slices = self._slices_cache.get(key)
+        if slices is None:
+            if len(self._slices_cache) > 8192:
+                self._slices_cache.clear()
+            slices = self._slices_cache[key] = self._decode_slices_8bit(rounds, num_kv_heads, head_dim, group > 8)
+        return slices
+
+    def _decode_slices_8bit(self, rounds, num_kv_heads, head_dim, wide) -> int:
+        longest = max(rounds, default=0)
+        if longest < 2:
+            return 1
+        slots, pairs = self.SM_COUNT * self.DECODE_8BIT_BLOCKS_PER_SM[head_dim], len(rounds) * num_kv_heads
+        best, best_cost, seen = 1, math.inf, 0
+        for s in range(1, min(64, longest) + 1):
+            per = -(-longest // s)
+            if per == seen:  # more slices of the same length: none
+                continue
+            seen = per
+            blocks = num_kv_heads * sum(-(-r // per) for r in rounds)
+            waves = max(1.0, blocks / slots)
+            cost = (per + 2.0) * (math.ceil(waves) if waves < 4 else waves + 0.5) + 0.3 * s + (3.0 if s > 1 else 0.0)
+            if cost < best_cost:
+                best, best_cost = -s if s > 1 else 1, cost
+            if 1 < s <= 16 and s * pairs <= slots and cost - 2.5 < best_cost:
+                best, best_cost = s, cost - 2.5
+        return best
+
+    def _decode_8bit(self, q, q_stride, H, G, D, pages, block_table, step, seq_list, num_seqs, max_len, slices, out, page_size, scale,
+                     window, keep_first, longest):
+        mid_o = mid_lse = None
+        joined, slices = slices < 0 or slices > 16, abs(slices)  # 16 blocks a cluster at most
+        if joined and slices > 1:
+            mid = torch.empty(num_seqs * H * slices * (D + 1), dtype=torch.float32, device=out.device)
+            mid_o = mid.data_ptr()
+            mid_lse = mid_o + 4 * num_seqs * H * slices * D
+            self.launches += 1
+        if self.timing is not None:
+            singles = [kv for b, kv in enumerate(step.host_kv_lens) if step.host_cu_seqlens[b + 1] - step.host_cu_seqlens[b] == 1]
+            seen = sum(min(kv, window + keep_first) if window else kv for kv in singles)
+            self._costs(seen * 2 * G * D + 4 * num_seqs * H * D, 4 * H * D * seen)
+        self._call("attention_8bit", "q3_decode_attention_8bit", "paged_attention_decode_8bit", q.data_ptr(), q_stride, pages.data_ptr(),
+                   pages.shape[0], block_table.data_ptr(), block_table.shape[1], step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(),
+                   _ptr(seq_list), out.data_ptr(), mid_o, mid_lse, num_seqs, H, G, D, page_size, float(scale), window, keep_first,
+                   slices, max_len, _ptr(longest), self._error_word(out.device).data_ptr())
+        return out
 
     # ---- matrix products ----------------------------------------------------------------
     def linear(self, x, weight, out=None, out_dtype=None, partial_sums=False, bias=None):

@@ -30,10 +30,10 @@ class PagedAttention(Part):
         self.qk_norm_eps = spec.get("qk_norm_eps")
         self.window = spec.get("window") or None
         self.scale = float(spec.get("scale") or 1.0 / math.sqrt(self.head_dim))
-        self.four_bit = ctx.kv_bits == 4
+        self.bits = ctx.kv_bits  # of the cache: 4, 8, or None for the compute dtype
         self.budget = ctx.kv_budget
-        self._slices_choice = (("decode_slices_4bit", self.num_kv_heads, self.head_dim, self.window, self.num_heads // self.num_kv_heads)
-                               if self.four_bit else ("decode_slices", self.num_kv_heads, self.head_dim, self.window))
+        self._slices_choice = ((f"decode_slices_{self.bits}bit", self.num_kv_heads, self.head_dim, self.window, self.num_heads // self.num_kv_heads)
+                               if self.bits else ("decode_slices", self.num_kv_heads, self.head_dim, self.window))
         self._sums_choice = ("mass_slice_keys_4bit", self.num_kv_heads)
         if self.num_heads % self.num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
@@ -86,8 +86,8 @@ class PagedAttention(Part):
 
     def kernel_groups(self):
         groups = ["rope_kv", "attention_generic", *product_groups(self.ctx), *self.position.kernel_groups()]
-        if self.four_bit:
-            groups += ["cache_4bit", "attention_4bit"]
+        if self.bits:
+            groups += [f"cache_{self.bits}bit", f"attention_{self.bits}bit"]
         if self.ctx.dtype == torch.bfloat16:
             # the specialised attention kernels that this head size can reach (ops.paged_attention)
             group = self.num_heads // self.num_kv_heads
@@ -102,7 +102,7 @@ class PagedAttention(Part):
     def step_choosers(self):
         """Into how many slices the split-KV decode kernel cuts the longest sequence's keys, and under a token budget how many keys a block
         takes for their sums."""
-        model = getattr(self.ops, "decode_slices_4bit" if self.four_bit else "decode_slices_for", None)
+        model = getattr(self.ops, f"decode_slices_{self.bits}bit" if self.bits else "decode_slices_for", None)
         if model is None or self.ctx.dtype != torch.bfloat16 or self.head_dim not in (64, 128, 256):
             return {}
         sizes = self._slices_choice[1:]
@@ -113,8 +113,8 @@ class PagedAttention(Part):
         return choosers
 
     def cache_spec(self):
-        if self.four_bit:
-            return KVLayerSpec(self.num_kv_heads, self.head_dim, self.window, bits=4, sums=self.budget is not None)
+        if self.bits:
+            return KVLayerSpec(self.num_kv_heads, self.head_dim, self.window, bits=self.bits, sums=self.budget is not None)
         return KVLayerSpec(self.num_kv_heads, self.head_dim, self.window)
 
     def position_limit(self):
@@ -134,8 +134,9 @@ class PagedAttention(Part):
         ctx_out = torch.empty((T, self.q_size), dtype=h.dtype, device=h.device)
         eps = self.qk_norm_eps if self.qk_norm_eps is not None else 0.0
         slices = step.choices.get(self._slices_choice)
-        if self.four_bit:
-            self._attend_4bit(qkv, ctx_out, step, cache, block_table, eps, cos, sin, slices)
+        if self.bits:
+            attend = self._attend_4bit if self.bits == 4 else self._attend_8bit
+            attend(qkv, ctx_out, step, cache, block_table, eps, cos, sin, slices)
             return self._project_out(ctx_out)
         fusable = getattr(ops, "decode_new_token_ok", None)
         if (fusable is not None and step.decode_only and cache.writes
@@ -192,6 +193,14 @@ class PagedAttention(Part):
             keys = step.choices.get(self._sums_choice)
             ops.attention_mass_4bit(qkv, qkv.stride(0), mass=cache.mass, scale=self.scale, step=step, observe=self.budget.observe,
                                     lse=lse, **({"slice_keys": keys} if keys else {}), **sizes)
+
+    def _attend_8bit(self, qkv, out, step: StepContext, cache, block_table, eps, cos, sin, slices) -> None:
+        """Norm, rotation, cache write and attention over a cache in 8 bits."""
+        sizes = dict(num_heads=self.num_heads, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim, pages=cache.packed_pages,
+                     block_table=block_table, page_size=cache.page_size)
+        self.ops.qk_norm_rope_store_8bit(qkv, q_weight=self.q_norm_weight, k_weight=self.k_norm_weight, eps=eps, cos=cos, sin=sin, step=step,
+                                         write_kv=cache.writes, pairing=self.pairing, **sizes)
+        self.ops.paged_attention_8bit(qkv, qkv.stride(0), out=out, scale=self.scale, window=self.window, step=step, decode_slices=slices, **sizes)
 
     def _project_out(self, ctx_out: torch.Tensor) -> torch.Tensor:
         if self.o_bias_vec is not None:

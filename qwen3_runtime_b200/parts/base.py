@@ -42,7 +42,7 @@ class BuildContext:
     device: torch.device
     ops: Any  # the kernel table (qwen3_runtime_b200.ops.cuda.CudaOps in production)
     shared: dict = field(default_factory=dict)  # tables shared between parts (e.g. rotary cos/sin)
-    kv_bits: int | None = None  # 4: keys and values are held in 4 bits (parts that can; the factory refuses the others)
+    kv_bits: int | None = None  # 4 or 8: keys and values are held in so many bits (parts that can; the factory refuses the others)
     kv_budget: Any = None  # a TokenBudget: each cached token's attention weights are summed beside it
 
 
