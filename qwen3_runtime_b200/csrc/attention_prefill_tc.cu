@@ -1,7 +1,9 @@
 // Causal attention of prompt portions on the 5th-generation tensor cores: S = Q K^T and O += P V are tcgen05.mma
-// with accumulators in tensor memory; Q, K and V tiles arrive by TMA (128-byte swizzle).  bfloat16; three forms:
+// with accumulators in tensor memory; Q, K and V tiles arrive by TMA (128-byte swizzle).  bfloat16; four forms:
 //   PAGED    heads of 128 over the paged cache, straight from the QKV buffer and the pages (group size a divisor of 128,
 //            page size 8/16/32/64); options: a chunked mask, turned values, sinks;
+//   FIRST    the same under a window whose tokens see the sequence's first ones as well: the tiles of those come in front, and the ones
+//            between them and the window are left out;
 //   MAPS     differential attention: a head is two maps of 64 side by side in its 128 columns, over one value of 128;
 //            options: a chunked mask or a window;
 //   DENSE    keys of 192 = 128 of the head's own + 64 shared by the heads, values of 128, one key head per query head,
@@ -52,7 +54,7 @@
 
 namespace {
 
-enum { PAGED = 0, MAPS = 1, DENSE = 2 };
+enum { PAGED = 0, MAPS = 1, DENSE = 2, FIRST = 3 };
 constexpr int D = 128;  // value size, and query/key size of PAGED and of both maps together
 constexpr int BLOCK_M = 128;
 constexpr int BLOCK_N = 64;
@@ -84,6 +86,7 @@ struct Params {
   const int* kv_base;             // DENSE: key j of sequence s is row kv_base[s] + j
   float lambda, eps, out_scale;   // MAPS
   int* error_word;
+  int keep_first;                 // FIRST: keys that every token sees, whatever its window
 };
 
 // 2^x in one instruction (exp2f adds range fix-ups around the same instruction; results
@@ -220,13 +223,17 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
     const int p_first = base_pos + (MODE == MAPS ? 1 : 2) * s_item[1] * BLOCK_M / G;
     const int k_lo = chunk > 0 ? p_first / chunk * chunk : (window > 0 ? max(0, p_first - window + 1) : 0);
     const int tile0 = k_lo / BLOCK_N;
+    // FIRST: tiles 0 .. firsts - 1 and those from tile0 on; `skip` of them lie between
+    const int keep = MODE == FIRST ? p.keep_first : 0;
+    const int firsts = MODE == FIRST ? min((keep + BLOCK_N - 1) / BLOCK_N, tile0) : 0, skip = tile0 - firsts;
+    auto tile_at = [&](int j) { return MODE == FIRST ? j + (j >= firsts ? skip : 0) : tile0 + j; };
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       row0[x] = (MODE == MAPS ? s_item[1] : 2 * s_item[1] + x) * BLOCK_M;
       const bool live = row0[x] < rows;
       const int last_row = min(rows, row0[x] + BLOCK_M) - 1;
       p_max[x] = live ? base_pos + last_row / G : -1;
-      tiles[x] = live ? p_max[x] / BLOCK_N + 1 - tile0 : 0;
+      tiles[x] = live ? p_max[x] / BLOCK_N + 1 - skip : 0;
     }
     const int num_tiles = max(tiles[0], tiles[1]);  // B lies after A, so this is B's count when B exists
     const int p_last = max(p_max[0], p_max[1]);
@@ -257,8 +264,9 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       const uint32_t dst0 = smem_addr(part < 2 ? k_s : v_s) + half * HALF_KV;
       const CUtensorMap* map = MODE == DENSE || part < 2 ? &tmap_k : &tmap_v;
       auto page_of = [&](int j) -> int {  // pages of tile j that exist in the block table (the rest of the tile is masked)
-        const int pi = (tile0 + j) * pages_per_tile + lane;
-        const bool in = lane < pages_per_tile && j < num_tiles && pi < max_pages && pi * ps <= p_last && (pi + 1) * ps > k_lo;
+        const int pi = tile_at(j) * pages_per_tile + lane;
+        const bool in = lane < pages_per_tile && j < num_tiles && pi < max_pages && pi * ps <= p_last &&
+                        ((pi + 1) * ps > k_lo || (MODE == FIRST && pi * ps < keep));
         return in ? bt[pi] : -1;
       };
       int next = MODE == DENSE ? 0 : page_of(0);
@@ -391,7 +399,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       // are scheduled as one run of instructions.
       auto step = [&](int j, auto edge) -> bool {
         constexpr bool EDGE = decltype(edge)::value;
-        const int key0 = (tile0 + j) * BLOCK_N;
+        const int key0 = tile_at(j) * BLOCK_N;
         if (!wait(bar(BAR_S_FULL + x), j & 1, &abort_flag)) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t sa[32], sb[32];
@@ -412,8 +420,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
           if (key0 < lo) {  // keys of an earlier chunk, or before the window
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
-              if (key0 + c < lo) sa[c] = 0xff800000u;
-              if (key0 + 32 + c < lo) sb[c] = 0xff800000u;
+              if (key0 + c < lo && (MODE != FIRST || key0 + c >= keep)) sa[c] = 0xff800000u;
+              if (key0 + 32 + c < lo && (MODE != FIRST || key0 + 32 + c >= keep)) sb[c] = 0xff800000u;
             }
           }
         }
@@ -473,7 +481,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
             const int vst = j % KV_STAGES;
             if (!wait(bar(BAR_V_FULL + vst), (j / KV_STAGES) & 1, &abort_flag)) return false;
             const int vrow = r & 63, half = r >> 6;
-            if (key0 + vrow > p_last || key0 + vrow < k_lo) {
+            if (key0 + vrow > p_last || (key0 + vrow < k_lo && (MODE != FIRST || key0 + vrow >= keep))) {
               uint4* dst = reinterpret_cast<uint4*>(v_s + vst * V_BYTES + half * HALF_KV + vrow * 128);
 #pragma unroll
               for (int ch = 0; ch < 8; ++ch) dst[ch] = make_uint4(0, 0, 0, 0);
@@ -494,8 +502,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       // masks only is the longest of its sequence: 32 heads over 8, 500 tokens behind 3000, 78 us; so 64.)
       int whole0 = 1, whole1 = 0;  // such tiles behind the first one
       if (row0[x] < rows) {
-        whole0 = max(1, (max(lo_last, k_lo) + BLOCK_N - 1) / BLOCK_N - tile0);
-        whole1 = min(my_tiles, (pos_first + 1) / BLOCK_N - tile0);
+        whole0 = max(1, (max(lo_last, k_lo) + BLOCK_N - 1) / BLOCK_N - skip);
+        whole1 = min(my_tiles, (pos_first + 1) / BLOCK_N - skip);
       }
       bool ok = true;
       for (int j = 0; j < my_tiles && ok; ++j) {
@@ -682,6 +690,26 @@ Q3_EXPORT int q3_paged_attention_prefill_tc(const void* q, int q_stride, int num
   const Params p = {block_table, max_pages, kv_lens, cu_seqlens, (bf16*)out, num_seqs, num_work, nq, nkv, ps,
                     scale * LOG2_E, skip_single, chunk, 0, turns, sinks, nullptr, 0.f, 0.f, 0.f, error_word};
   return launch<PAGED>(tq, tk, tv, tq, p, stream);
+}
+
+// The same under a window: a token sees the last `window` keys up to itself, and the sequence's first `keep_first`.
+Q3_EXPORT int q3_window_attention_prefill_tc(const void* q, int q_stride, int num_tokens, const void* kpages, const void* vpages,
+                                             long num_rows_kv, const int* block_table, int max_pages, const int* kv_lens,
+                                             const int* cu_seqlens, void* out, int num_seqs, int num_work, int nq, int nkv, int head_dim,
+                                             int ps, float scale, int skip_single, int window, int keep_first, int* error_word,
+                                             cudaStream_t stream) {
+  if (!q || !kpages || !vpages || !block_table || !kv_lens || !cu_seqlens || !out || window < 1 || keep_first < 0) return Q3_ERR_ARGUMENT;
+  if (nq < 1 || nkv < 1 || nq % nkv) return Q3_ERR_ARGUMENT;
+  if (head_dim != D || !paged_ok(q, q_stride, kpages, vpages, nq, nkv, ps) || ((uintptr_t)out & 15)) return Q3_ERR_UNSUPPORTED;
+  if (num_work == 0) return Q3_OK;
+  CUtensorMap tq, tk, tv;
+  if (!q_map(&tq, q, D, nq, num_tokens, q_stride, nq / nkv) ||
+      !q3_bf16_map(&tk, kpages, num_rows_kv, D, D, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
+      !q3_bf16_map(&tv, vpages, num_rows_kv, D, D, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
+    return Q3_ERR_LAUNCH;
+  const Params p = {block_table, max_pages, kv_lens, cu_seqlens, (bf16*)out, num_seqs, num_work, nq, nkv, ps, scale * LOG2_E, skip_single, 0,
+                    window, nullptr, nullptr, nullptr, 0.f, 0.f, 0.f, error_word, keep_first};
+  return launch<FIRST>(tq, tk, tv, tq, p, stream);
 }
 
 // Differential attention of every sequence of the step: query head h is [map 1 (64) | map 2 (64)] at column h * 128, key

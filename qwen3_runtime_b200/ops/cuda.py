@@ -219,6 +219,9 @@ _SIGNATURES = {
         "q3_paged_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, ctypes.c_long, c_void_p, c_int,
                                           c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                                           c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+        "q3_window_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_long, c_void_p, c_int, c_void_p, c_void_p,
+                                           c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p,
+                                           c_void_p],
         "q3_diff_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_long, c_void_p, c_int, c_void_p,
                                          c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
                                          c_float, c_float, c_float, c_void_p, c_void_p],
@@ -2350,6 +2353,17 @@ class CudaOps:
         self._call(f"cache_{bits}", f"q3_unpack_{bits}", f"unpack_{bits}", _dtype_code(k.dtype), _ptr(pages), pages.shape[0], G, D, page_size,
                    _ptr(block_table), block_table.shape[1], _ptr(part.kv_lens), part.num_seqs, longest, _ptr(part.cu_seqlens),
                    2 if split else 1, int(window or 0), *kept, count, width, k.data_ptr(), v.data_ptr(), _ptr(table))
+        if (keep_first is not None and window and split and D == 128 and 128 % (H // G) == 0 and page_size in (8, 16, 32, 64)
+                and self.prefill_attention == "tcgen05"):
+            news = [b - a for a, b in zip(part.host_cu_seqlens, part.host_cu_seqlens[1:])]
+            pairs = sum(-(-(-(-n * H // G // 128)) // 2) for n in news if n > 1)  # two blocks of 128 rows an item
+            if self.timing is not None:
+                self._costs(*self._attention_cost(part, H, G, D, out, prompts=True))
+            self._call("attention_prefill_tc", "q3_window_attention_prefill_tc", "paged_attention_prefill_window", q.data_ptr(), q_stride,
+                       q.shape[0], k.data_ptr(), v.data_ptr(), count * G * page_size, table.data_ptr(), width, part.kv_lens.data_ptr(),
+                       part.cu_seqlens.data_ptr(), out.data_ptr(), part.num_seqs, pairs, H, G, D, page_size, float(scale), 1, window,
+                       keep_first, self._error_word(out.device).data_ptr())
+            return
         # the wide kernels number a token by its place: kv_lens and cu_seqlens say it, or for the general kernel `positions`
         self.paged_attention(q, q_stride, num_heads=H, num_kv_heads=G, head_dim=D, k_pages=k, v_pages=v, block_table=table,
                              token_seq=part.token_seq, positions=part.positions, out=out, page_size=page_size, scale=scale,

@@ -95,7 +95,7 @@ class PagedAttention(Part):
                 groups.append("attention_decode")
             if self.head_dim in (64, 128) and group <= 16:
                 groups.append("attention_prefill")
-            if self.head_dim == 128 and not self.window and 128 % group == 0:
+            if self.head_dim == 128 and (not self.window or self.bits == 8) and 128 % group == 0:
                 groups.append("attention_prefill_tc")
         return groups
 
