@@ -595,18 +595,43 @@ template <int D> __global__ void __launch_bounds__(THREADS) merge_8bit_kernel(De
     }
 }
 
-template <int D, int NT, bool BULK, bool CLUSTER> int launch_decode_as(const Decode& a, int num_seqs, cudaStream_t stream) {
+template <int D, int NT, bool BULK, bool CLUSTER> constexpr int decode_smem() {
   constexpr int ring = WARPS * STAGES * Head<D>::TILES * (2 * STEP * D + (BULK ? 16 : 8 * STEP));
   constexpr int joined = (WARPS * 8 * NT * (D + 4 + 2) + (CLUSTER ? 8 * NT * (D + 2) : 0)) * 4;
-  constexpr int smem = ring > joined ? ring : joined;
+  return ring > joined ? ring : joined;
+}
+template <int D, int NT, bool BULK, bool CLUSTER> bool decode_ready() {
   auto kernel = decode_8bit_kernel<D, NT, BULK, CLUSTER>;
   static bool once[Q3_MAX_DEVICES];
   const int dev = q3_current_device();
   if (!once[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return Q3_ERR_LAUNCH;
-    if (CLUSTER && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return Q3_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem<D, NT, BULK, CLUSTER>()) != cudaSuccess) return false;
+    if (CLUSTER && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
     once[dev] = true;
   }
+  return true;
+}
+// Clusters of `size` blocks that the device holds at a time (which SMs lie together differs between devices).
+template <int D, int NT> int decode_clusters(int size) {
+  if (!decode_ready<D, NT, true, true>()) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = decode_smem<D, NT, true, true>();
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int count = 0;
+  return cudaOccupancyMaxActiveClusters(&count, decode_8bit_kernel<D, NT, true, true>, &cfg) == cudaSuccess ? count : 0;
+}
+
+template <int D, int NT, bool BULK, bool CLUSTER> int launch_decode_as(const Decode& a, int num_seqs, cudaStream_t stream) {
+  constexpr int smem = decode_smem<D, NT, BULK, CLUSTER>();
+  auto kernel = decode_8bit_kernel<D, NT, BULK, CLUSTER>;
+  if (!decode_ready<D, NT, BULK, CLUSTER>()) return Q3_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.splits, a.nkv, num_seqs);
   cfg.blockDim = dim3(THREADS);
@@ -915,6 +940,15 @@ Q3_EXPORT int q3_decode_attention_8bit(const void* q, int q_stride, const void* 
   if (D == 128) return R <= 8 ? launch_decode<128, 1>(a, num_seqs, stream) : launch_decode<128, 2>(a, num_seqs, stream);
   if (D == 256) return R <= 8 ? launch_decode<256, 1>(a, num_seqs, stream) : launch_decode<256, 2>(a, num_seqs, stream);
   return Q3_ERR_UNSUPPORTED;
+}
+
+// How many clusters of `size` blocks of decode attention run at a time, for groups of up to 8 query heads or (wide) more; 0: not known.
+Q3_EXPORT int q3_decode_clusters_8bit(int D, int wide, int size) {
+  if (size < 1 || size > MOST_CLUSTER) return 0;
+  if (D == 64) return wide ? decode_clusters<64, 2>(size) : decode_clusters<64, 1>(size);
+  if (D == 128) return wide ? decode_clusters<128, 2>(size) : decode_clusters<128, 1>(size);
+  if (D == 256) return wide ? decode_clusters<256, 2>(size) : decode_clusters<256, 1>(size);
+  return 0;
 }
 
 // `slices` 0: a block goes through all of a token's keys; else mid_o [tokens][nq][slices][D] and mid_ml [tokens][nq][slices][2] are given and

@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+from collections import Counter
 from ctypes import c_float, c_int, c_long, c_void_p
 
 import torch
@@ -267,6 +268,7 @@ _SIGNATURES = {
         "q3_decode_attention_8bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int,
                                      c_void_p, c_void_p, c_void_p],
+        "q3_decode_clusters_8bit": [c_int, c_int, c_int],
         "q3_general_attention_8bit": [c_int, c_void_p, c_long, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                       c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
     },
@@ -2734,15 +2736,21 @@ class CudaOps:
                    _ptr(step.positions), _ptr(out), _ptr(mid_o), _ptr(mid_ml), slices, T, H, G, D, page_size, float(scale), window, keep_first)
         return out
 
-    # blocks of decode attention over 8-bit numbers that an SM holds, by head size
+    # Blocks of decode attention over 8-bit numbers that an SM holds, by head size; and what its cost model takes (see there), by head size and
+    # whether a kv head has more than 8 query heads.
     DECODE_8BIT_BLOCKS_PER_SM = {64: 4, 128: 2, 256: 2}
+    DECODE_8BIT_COSTS = {
+        (64, False): (0.81, 0.33, 2.6, 1.8, 0.45, 1.16), (64, True): (0.92, 0.56, 0.3, 1.2, 0.0, 1.09),
+        (128, False): (0.89, 0.57, 2.9, 2.8, 0.62, 1.14), (128, True): (1.11, 0.70, 4.0, 4.0, 0.56, 1.08),
+        (256, False): (0.86, 0.54, 5.2, 5.1, 0.86, 1.08), (256, True): (1.13, 0.75, 0.0, 5.5, 0.0, 1.06),
+    }
 
     def decode_slices_8bit(self, kv_lens, num_kv_heads, head_dim, window=None, group=1, keep_first=0) -> int:
         """Into how many slices the longest of these sequences' keys are cut by decode attention over a cache in 8 bits (a shorter
         sequence is cut into fewer of that length); negative: they are joined by a second kernel and not by the blocks of a cluster."""
         cap = window + 15 + -(-keep_first // 16) * 16 if window else 1 << 30
         unit = 64 if head_dim == 256 else 128  # keys that a block takes at a time
-        rounds = tuple(-(-min(n, cap) // unit) for n in kv_lens)
+        rounds = tuple([-(-n // unit) if n < cap else -(-cap // unit) for n in kv_lens])
         key = ("8bit", num_kv_heads, head_dim, group > 8, rounds)
         slices = self._slices_cache.get(key)
         if slices is None:
@@ -2752,24 +2760,42 @@ class CudaOps:
         return slices
 
     def _decode_slices_8bit(self, rounds, num_kv_heads, head_dim, wide) -> int:
+        """Times in us, fitted to a sweep of 1 to 64 slices over 212 batches of 1 to 128 sequences of 20 to 131,072 tokens (7 head counts and sizes) on
+        a B200: the choice is 2 to 5 % slower than the best one on average (heads of 64 in wide groups 8 %), 26 % at worst.  A round of keys takes
+        a block `alone` on its SM, and `shared` for every block there; a block's beginning and end as much as `ends` rounds, of which an SM
+        notices `ends_shared` where other blocks go on meanwhile; the last blocks end apart by a share `tail` of their length.  A second kernel
+        joins slices in 2.1 and more; clusters do so for less, but take `clustered` times as long, and all have to run at once."""
         longest = max(rounds, default=0)
         if longest < 2:
             return 1
-        slots, pairs = self.SM_COUNT * self.DECODE_8BIT_BLOCKS_PER_SM[head_dim], len(rounds) * num_kv_heads
+        alone, shared, ends, ends_shared, tail, clustered = self.DECODE_8BIT_COSTS[head_dim, wide]
+        sms, per_sm, pairs, total = self.SM_COUNT, self.DECODE_8BIT_BLOCKS_PER_SM[head_dim], len(rounds) * num_kv_heads, num_kv_heads * sum(rounds)
         best, best_cost, seen = 1, math.inf, 0
+        lengths = Counter(rounds).items()  # (many are alike)
         for s in range(1, min(64, longest) + 1):
             per = -(-longest // s)
             if per == seen:  # more slices of the same length: none
                 continue
             seen = per
-            blocks = num_kv_heads * sum(-(-r // per) for r in rounds)
-            waves = max(1.0, blocks / slots)
-            cost = (per + 2.0) * (math.ceil(waves) if waves < 4 else waves + 0.5) + 0.3 * s + (3.0 if s > 1 else 0.0)
-            if cost < best_cost:
-                best, best_cost = -s if s > 1 else 1, cost
-            if 1 < s <= 16 and s * pairs <= slots and cost - 2.5 < best_cost:
-                best, best_cost = s, cost - 2.5
+            blocks = num_kv_heads * sum([-(-r // per) * n for r, n in lengths])
+            if blocks > sms * per_sm:
+                cost = shared * ((total + ends_shared * blocks) / sms + tail * per * per_sm)
+            else:
+                cost = max((per + ends) * max(alone, shared * min(per_sm, -(-blocks // sms))), shared * total / sms)
+            joined = cost + 2.1 + 0.24 * s if s > 1 else cost
+            if joined < best_cost:
+                best, best_cost = -s if s > 1 else 1, joined
+            if 1 < s <= 16 and clustered * cost + 0.1 * s < best_cost and pairs <= self._clusters_8bit(head_dim, wide, s):
+                best, best_cost = s, clustered * cost + 0.1 * s
         return best
+
+    def _clusters_8bit(self, head_dim, wide, size) -> int:
+        """Clusters of that many blocks that the device runs at a time."""
+        key = ("8bit clusters", head_dim, wide, size)
+        count = self._parts_cache.get(key)
+        if count is None:
+            count = self._parts_cache[key] = self._get("attention_8bit", "q3_decode_clusters_8bit")(head_dim, int(wide), size)
+        return count
 
     def _decode_8bit(self, q, q_stride, H, G, D, pages, block_table, step, seq_list, num_seqs, max_len, slices, out, page_size, scale,
                      window, keep_first, longest):

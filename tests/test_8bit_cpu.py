@@ -68,6 +68,7 @@ def test_the_cache_of_tensors_has_the_layout_of_single_rows():
 def ops():
     table = Table()
     table._slices_cache = {}
+    table._clusters_8bit = lambda D, wide, size: 9 * 148 * table.DECODE_8BIT_BLOCKS_PER_SM[D] // (10 * size)  # (about what a device holds)
     return table
 
 
@@ -162,6 +163,7 @@ class Here(Table):
     def __init__(self):
         super().__init__()
         self._device_index, self._slices_cache, self.prefill_attention = torch.zeros(1).get_device(), {}, "tcgen05"
+        self._clusters_8bit = lambda *sizes: 0
 
     def paged_attention(self, *args, **kw):
         self.calls.append("paged_attention")
