@@ -11,6 +11,8 @@
 
 namespace {
 
+constexpr int STORE_THREADS = 512;  // of a block, at most
+
 struct Store {
   const float *q_w, *k_w, *cos_t, *sin_t;
   float eps;
@@ -18,7 +20,6 @@ struct Store {
   const int *positions, *kv_lens, *cu_seqlens, *block_table;
   int max_pages, num_pages, num_seqs, num_tokens, ps;
   int units;    // pages that get tokens, at most; 0: none are written
-  int single;   // every sequence brings one token: unit u is sequence u's
   int q_blocks;  // blocks that a token's queries take
   unsigned char* pages;
   int* error_word;
@@ -29,10 +30,11 @@ struct Store {
 struct Unit {
   int r0, r1, token;    // token: of row 0 (as if it were new as well)
   unsigned char* rec;   // null: nothing to write
-  __device__ __forceinline__ Unit(const Store& a, int u, int nkv, int kvh, long record) : r0(0), r1(0), token(0), rec(nullptr) {
+  // `single`: every sequence brings one token, unit u is sequence u's
+  __device__ __forceinline__ Unit(const Store& a, bool single, int u, int nkv, int kvh, long record) : r0(0), r1(0), token(0), rec(nullptr) {
     const int lane = threadIdx.x & 31;
     int seq = -1, i = 0, first = 0, len = 0, news = 0, cu = 0;
-    if (a.single) {
+    if (single) {
       seq = u, len = a.kv_lens[u], cu = a.cu_seqlens[u], news = a.cu_seqlens[u + 1] - cu;
       first = max(0, len - news), i = first / a.ps;
       if (news < 1 || len < 1) return;
@@ -150,9 +152,13 @@ __device__ __forceinline__ bool norm_and_turn(float (&v0)[8], float (&v1)[8], co
 // Head sizes 16, 32, 64, 128, 256 with the rotation over the whole head (or none): D / 16 threads per (token, head); thread c owns
 // channels [8c, 8c + 8) and [D/2 + 8c, D/2 + 8c + 8).  Blocks of the write come first (unit, then key and value heads), each as many rows at a
 // time as it has threads for; rows beyond that are made once more when the scale is known.  Then the queries' blocks.
-// KNOWN: the head size where the compiler knows it, else 0.
-template <typename T, int KNOWN>
-__global__ void store_8bit_vec_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, int nq, int nkv, int size, Store a) {
+// KNOWN: the head size where the compiler knows it, else 0.  SINGLE: every sequence brings one token.
+// The floor is the bytes of the projection and of the queries.  What bounds it is latency, loads one behind the other (a position, its angles), and
+// instructions: 3,258 tokens of 32 + 8 heads of 128 in bfloat16 take 21 us (3.5 TB/s), 14 of them the queries; 40 registers a thread, 48 warps an SM, are
+// worth two spilled ones (with 56: 23 us, with 32: 26).  Every value rounded by itself, without the hardware's conversion: 27.  Several tokens in
+// turn by a thread that keeps the weights and has the next one's values on their way, 80 registers: 27.
+template <typename T, int KNOWN, bool SINGLE>
+__global__ void __launch_bounds__(STORE_THREADS, SINGLE ? 2 : 3) store_8bit_vec_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, int nq, int nkv, int size, Store a) {
   const int D = KNOWN ? KNOWN : size, tph = D / 16, tph_shift = 31 - __clz(tph), half = D / 2, mask = q8_mask(D);
   const int tid = threadIdx.x, c = tid & (tph - 1);
   __shared__ uint32_t red[32];
@@ -183,7 +189,7 @@ __global__ void store_8bit_vec_kernel(const T* qkv, int row_stride, T* q_out, in
   }
   const int u = blockIdx.x / (2 * nkv), hd = blockIdx.x - u * 2 * nkv, is_v = hd >= nkv, kvh = hd - is_v * nkv;
   const Q8Page L(D, a.ps);
-  const Unit unit(a, u, nkv, kvh, L.record);
+  const Unit unit(a, SINGLE, u, nkv, kvh, L.record);
   if (!unit.rec) return;
   unsigned char* codes = unit.rec + (is_v ? L.values : 0);
   const int per = blockDim.x >> tph_shift, r_first = unit.r0 + (tid >> tph_shift);
@@ -212,10 +218,7 @@ __global__ void store_8bit_vec_kernel(const T* qkv, int row_stride, T* q_out, in
   const int passes = (unit.r1 - unit.r0 + per - 1) / per;
   for (int pass = 0; pass < passes; ++pass) {
     make(r_first + pass * per);
-    if (live) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = max(most, max(q8_finite(q8_rounded(v0[e])), q8_finite(q8_rounded(v1[e]))));
-    }
+    if (live) most = max(most, max(q8_most(v0), q8_most(v1)));
   }
   const int e = settle_scale(most, unit.r0, D, codes, reinterpret_cast<float*>(unit.rec + L.scales) + is_v, red);
   const float down = q8_power(-e);
@@ -224,8 +227,8 @@ __global__ void store_8bit_vec_kernel(const T* qkv, int row_stride, T* q_out, in
     if (passes > 1) make(row);
     if (!live) continue;
     unsigned char* to = codes + (long)row * D;
-    *reinterpret_cast<uint2*>(to + q8_at(8 * c, row, mask)) = make_uint2(q8_word(v0, down), q8_word(v0 + 4, down));
-    *reinterpret_cast<uint2*>(to + q8_at(half + 8 * c, row, mask)) = make_uint2(q8_word(v1, down), q8_word(v1 + 4, down));
+    *reinterpret_cast<uint2*>(to + q8_at(8 * c, row, mask)) = q8_words(v0, down);
+    *reinterpret_cast<uint2*>(to + q8_at(half + 8 * c, row, mask)) = q8_words(v1, down);
   }
 }
 
@@ -279,7 +282,7 @@ __global__ void store_8bit_kernel(const T* qkv, int row_stride, T* q_out, int q_
   }
   const int u = blockIdx.x / (2 * nkv), hd = blockIdx.x - u * 2 * nkv, is_v = hd >= nkv, kvh = hd - is_v * nkv;
   const Q8Page L(D, a.ps);
-  const Unit unit(a, u, nkv, kvh, L.record);
+  const Unit unit(a, false, u, nkv, kvh, L.record);
   if (!unit.rec) return;
   unsigned char* codes = unit.rec + (is_v ? L.values : 0);
   auto make_row = [&](int row) {
@@ -312,6 +315,8 @@ struct Unpack {
   int max_pages, num_seqs, max_len, least, window, keep_first, count, width;
   int* table_out;
 };
+
+__host__ __device__ __forceinline__ constexpr int unpack_rows(int D) { return 2048 / D; }  // of a page that a warp takes
 
 // Page `p` of the output (of a launch whose second axis is the sequences, without `cu_seqlens`).  Called by whole warps.
 struct UnpackPage {
@@ -376,62 +381,75 @@ struct UnpackPage {
   }
 };
 
-__device__ __forceinline__ void store_values(float* to, const float (&v)[8]) { store8(to, v); }
-__device__ __forceinline__ void store_values(bf16* to, const float (&v)[8]) { store8(to, v); }
+// What a lane writes at a time, 16 bytes: 8 values in bfloat16 (from 8 codes), 4 in float32.
+__device__ __forceinline__ void unpack_codes(float* to, const uint32_t (&code)[1], float scale) {
+  float v[4];
+  q8_floats(code[0], v);
+  *reinterpret_cast<float4*>(to) = make_float4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale);
+}
+__device__ __forceinline__ void unpack_codes(bf16* to, const uint32_t (&code)[2], float scale) {
+  float lo[4], hi[4];
+  q8_floats(code[0], lo);
+  q8_floats(code[1], hi);
+  const float v[8] = {lo[0] * scale, lo[1] * scale, lo[2] * scale, lo[3] * scale, hi[0] * scale, hi[1] * scale, hi[2] * scale, hi[3] * scale};
+  store8(to, v);
+}
 
-// A warp per (page, kv head), 8 channels a lane, so that what a warp writes at a time is one piece; all loads of a round (16 tokens of 128 channels:
-// 16 of 8 bytes a lane) are under way before the first is used.  What bounds it is the bytes written.  KNOWN: the head size where the compiler
-// knows it, else 0.
-template <typename T, int KNOWN> __global__ void __launch_bounds__(256) unpack_8bit_kernel(Unpack a, int size, T* __restrict__ k_out, T* __restrict__ v_out) {
-  const int D = KNOWN ? KNOWN : size, words = D / 8, mask = q8_mask(D);
-  constexpr int AT_ONCE = 8;
+// A warp per (page, kv head, keys or values, part of the rows: 2,048 channels), 16 bytes of the result a lane, so that what a warp writes at a time is one
+// piece; eight loads a lane are under way before the first is used.  What bounds it is the bytes written: 5,306 tokens of 8 heads of 128, padded to
+// 12,288, in 9.5 us.  (A warp for all of a page: 10.6, pages of 64 tokens 16; two pieces of 16 bytes side by side a lane, in float32: 33 us
+// for 20.)  KNOWN: the head size where the compiler knows it, else 0.
+template <typename T, int KNOWN> __global__ void __launch_bounds__(256) unpack_8bit_kernel(Unpack a, int size, int parts, T* __restrict__ k_out, T* __restrict__ v_out) {
+  constexpr int AT_ONCE = 8, CHANNELS = 16 / sizeof(T);
+  const int D = KNOWN ? KNOWN : size, words = D / CHANNELS, mask = q8_mask(D);
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const long item = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int kvh = (int)(item % a.nkv), p = (int)(item / a.nkv);
+  const uint32_t item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), half = item >> 1, pair = parts == 1 ? half : half / parts;
+  const int is_v = item & 1, part = (int)(half - pair * parts), p = (int)(pair / a.nkv), kvh = (int)(pair - p * a.nkv);
   if (p >= (a.cu_seqlens ? a.count : a.width)) return;
   const UnpackPage at_page(a, p);
   if (at_page.seq < 0) return;
   const int place = a.cu_seqlens ? p : blockIdx.y * a.width + p;
-  if (kvh == 0) at_page.name(a, place);
+  if (kvh == 0 && part == 0 && !is_v) at_page.name(a, place);
   int page;
-  const int rows = at_page.rows(a, &page);
+  const int row0 = part * unpack_rows(D), rows = at_page.rows(a, &page) - row0;  // those that count, from the part's first on
   const Q8Page L(D, a.ps);
   const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
-  const long out_base = ((long)place * a.nkv + kvh) * a.ps * D;
-  const float2 scale = rows > 0 ? *reinterpret_cast<const float2*>(rec + L.scales) : make_float2(0.f, 0.f);
-  const int total = 2 * a.ps * words, behind = a.ps * words;  // words of 8 channels: keys', then values', which lie behind them
-  for (int first = lane; first < total; first += 32 * AT_ONCE) {
-    uint2 code[AT_ONCE];
+  const unsigned char* from = rec + (is_v ? L.values : 0) + (long)row0 * D;
+  T* to = (is_v ? v_out : k_out) + (((long)place * a.nkv + kvh) * a.ps + row0) * D;
+  const float scale = rows > 0 ? reinterpret_cast<const float*>(rec + L.scales)[is_v] : 0.f;
+  const int count = min(unpack_rows(D), a.ps - row0) * words, live = rows * words;
+  for (int first = lane; first < count; first += 32 * AT_ONCE) {
+    uint32_t code[AT_ONCE][CHANNELS / 4];
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
-      const int at = first + 32 * u, in = at >= behind ? at - behind : at;
-      code[u] = make_uint2(0, 0);
-      if (at < total && in / words < rows) code[u] = *reinterpret_cast<const uint2*>(rec + 8l * at);
+      const int at = first + 32 * u;
+#pragma unroll
+      for (int e = 0; e < CHANNELS / 4; ++e) code[u][e] = 0;
+      if (at < count && at < live) {
+        if constexpr (CHANNELS == 8)
+          *reinterpret_cast<uint2*>(code[u]) = *reinterpret_cast<const uint2*>(from + CHANNELS * at);
+        else
+          code[u][0] = *reinterpret_cast<const uint32_t*>(from + CHANNELS * at);
+      }
     }
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
-      const int at = first + 32 * u, is_v = at >= behind, in = is_v ? at - behind : at, row = in / words;
-      if (at >= total) break;
-      const float s = row < rows ? (is_v ? scale.y : scale.x) : 0.f;
-      float lo[4], hi[4], v[8];
-      q8_floats(code[u].x, lo);
-      q8_floats(code[u].y, hi);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = lo[e] * s, v[4 + e] = hi[e] * s;
-      store_values((is_v ? v_out : k_out) + out_base + (long)row * D + q8_at(8 * (in - row * words), row, mask), v);
+      const int at = first + 32 * u, row = at / words;
+      if (at < count) unpack_codes(to + (long)row * D + q8_at(CHANNELS * (at - row * words), row0 + row, mask), code[u], at < live ? scale : 0.f);
     }
   }
 }
 
 template <typename T> cudaError_t launch_unpack(const Unpack& a, int D, T* k_out, T* v_out, cudaStream_t stream) {
-  const long items = (long)(a.cu_seqlens ? a.count : a.width) * a.nkv;
+  const int parts = (a.ps + unpack_rows(D) - 1) / unpack_rows(D);
+  const long items = 2L * (a.cu_seqlens ? a.count : a.width) * a.nkv * parts;
   const dim3 grid((unsigned)((items + 7) / 8), a.cu_seqlens ? 1 : a.num_seqs);
-  if (D == 64) return launch_pdl(unpack_8bit_kernel<T, 64>, grid, dim3(256), 0, stream, a, D, k_out, v_out);
-  if (D == 128) return launch_pdl(unpack_8bit_kernel<T, 128>, grid, dim3(256), 0, stream, a, D, k_out, v_out);
-  if (D == 256) return launch_pdl(unpack_8bit_kernel<T, 256>, grid, dim3(256), 0, stream, a, D, k_out, v_out);
-  return launch_pdl(unpack_8bit_kernel<T, 0>, grid, dim3(256), 0, stream, a, D, k_out, v_out);
+  if (D == 64) return launch_pdl(unpack_8bit_kernel<T, 64>, grid, dim3(256), 0, stream, a, D, parts, k_out, v_out);
+  if (D == 128) return launch_pdl(unpack_8bit_kernel<T, 128>, grid, dim3(256), 0, stream, a, D, parts, k_out, v_out);
+  if (D == 256) return launch_pdl(unpack_8bit_kernel<T, 256>, grid, dim3(256), 0, stream, a, D, parts, k_out, v_out);
+  return launch_pdl(unpack_8bit_kernel<T, 0>, grid, dim3(256), 0, stream, a, D, parts, k_out, v_out);
 }
 
 inline bool q8_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -453,32 +471,39 @@ Q3_EXPORT int q3_store_8bit(int dtype, const void* qkv, int row_stride, void* q_
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
   if (units > 0 && !q8_aligned(pages)) return Q3_ERR_UNSUPPORTED;
   Store a{q_w, k_w, cos_t, sin_t, eps, rot_half, max_pos, pairing, positions, kv_lens, cu_seqlens, block_table,
-          max_pages, num_pages, num_seqs, num_tokens, ps, units, single, 1, (unsigned char*)pages, error_word};
+          max_pages, num_pages, num_seqs, num_tokens, ps, units, 1, (unsigned char*)pages, error_word};
   const int tph = D / 16, rows = most_new < ps ? most_new : ps;
   const bool vec = (tph & (tph - 1)) == 0 && row_stride % 8 == 0 && q_stride % 8 == 0 && (!cos_t || 2 * rot_half == D) &&
                    q8_aligned(qkv) && q8_aligned(q_out) && q8_aligned(q_w) && q8_aligned(k_w) && q8_aligned(cos_t) && q8_aligned(sin_t);
   cudaError_t err;
   if (vec) {
     int threads = units > 0 ? (tph * rows + 31) / 32 * 32 : 128;
-    threads = threads > 512 ? 512 : threads;
+    threads = threads > STORE_THREADS ? STORE_THREADS : threads;
     a.q_blocks = (nq * tph + threads - 1) / threads;
     const long blocks = (long)units * 2 * nkv + (long)num_tokens * a.q_blocks;
     if (blocks > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
-    auto launch = [&](auto known) {
+    auto launch = [&](auto known, auto alone) {
       constexpr int K = decltype(known)::value;
-      err = dtype == Q3_DTYPE_F32 ? launch_pdl(store_8bit_vec_kernel<float, K>, dim3((unsigned)blocks), dim3(threads), 0, stream,
+      constexpr bool S = decltype(alone)::value;
+      err = dtype == Q3_DTYPE_F32 ? launch_pdl(store_8bit_vec_kernel<float, K, S>, dim3((unsigned)blocks), dim3(threads), 0, stream,
                                                (const float*)qkv, row_stride, (float*)q_out, q_stride, nq, nkv, D, a)
-                                  : launch_pdl(store_8bit_vec_kernel<bf16, K>, dim3((unsigned)blocks), dim3(threads), 0, stream,
+                                  : launch_pdl(store_8bit_vec_kernel<bf16, K, S>, dim3((unsigned)blocks), dim3(threads), 0, stream,
                                                (const bf16*)qkv, row_stride, (bf16*)q_out, q_stride, nq, nkv, D, a);
     };
-    if (D == 64)
-      launch(std::integral_constant<int, 64>());
-    else if (D == 128)
-      launch(std::integral_constant<int, 128>());
-    else if (D == 256)
-      launch(std::integral_constant<int, 256>());
+    auto launch_size = [&](auto alone) {
+      if (D == 64)
+        launch(std::integral_constant<int, 64>(), alone);
+      else if (D == 128)
+        launch(std::integral_constant<int, 128>(), alone);
+      else if (D == 256)
+        launch(std::integral_constant<int, 256>(), alone);
+      else
+        launch(std::integral_constant<int, 0>(), alone);
+    };
+    if (single)
+      launch_size(std::true_type());
     else
-      launch(std::integral_constant<int, 0>());
+      launch_size(std::false_type());
     return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
   }
   constexpr int WARPS = 4;
@@ -503,7 +528,7 @@ Q3_EXPORT int q3_unpack_8bit(int dtype, const void* pages, int num_pages, int nk
   if (cu_seqlens && (!table_out || least < 1 || keep_first < 0)) return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
   if ((!cu_seqlens && num_seqs > 65535) || !q8_aligned(pages) || !q8_aligned(k_out) || !q8_aligned(v_out)) return Q3_ERR_UNSUPPORTED;
-  if ((long)(cu_seqlens ? count : width) * nkv > 0x7fffffffL || 2L * ps * (D / 8) > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
+  if ((long)(cu_seqlens ? count : width) * 2 * nkv * ((ps + unpack_rows(D) - 1) / unpack_rows(D)) > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
   const Unpack a{(const unsigned char*)pages, num_pages, nkv, ps, block_table, kv_lens, cu_seqlens, max_pages, num_seqs, max_len, least, window,
                  keep_first, count, width, table_out};
   const cudaError_t err = dtype == Q3_DTYPE_F32 ? launch_unpack(a, D, (float*)k_out, (float*)v_out, stream)

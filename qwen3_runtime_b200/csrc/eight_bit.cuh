@@ -45,10 +45,42 @@ __device__ __forceinline__ int q8_exponent_of(float scale) {  // of a scale as i
 __device__ __forceinline__ uint32_t q8_code(float x, float down) {
   const uint32_t r = q8_rounded(x);
   const uint32_t c = r < Q8_INFINITE ? __float_as_uint(__fmul_rn(__fmul_rn(__uint_as_float(r), down), 0x1p-120f)) >> 20 : 0x7Fu;
-  return c | ((__float_as_uint(x) >> 24) & 0x80u);
+  return r < Q8_INFINITE ? c | ((__float_as_uint(x) >> 24) & 0x80u) : c;
 }
 __device__ __forceinline__ uint32_t q8_word(const float* x, float down) {  // four of them
   return q8_code(x[0], down) | (q8_code(x[1], down) << 8) | (q8_code(x[2], down) << 16) | (q8_code(x[3], down) << 24);
+}
+// The bits of the largest |R(x)| of eight values, of which those that are not finite are left out, for maxima.  (fmaxf leaves NaN out.)
+__device__ __forceinline__ uint32_t q8_most(const float (&x)[8]) {
+  float most = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+  uint32_t r = q8_rounded(most);
+  if (r >= Q8_INFINITE) {
+    r = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r = max(r, q8_finite(q8_rounded(x[e])));
+  }
+  return r;
+}
+// The codes of eight values.  Where none is infinite and none falls below the normal codes, where the cut is not a rounding, the conversion of the
+// hardware (to nearest, half ways to even; NaN 0x7F) gives them, two at a time.
+__device__ __forceinline__ uint2 q8_words(const float (&x)[8], float down) {
+  float y[8], most = 0.f, least = 448.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    y[e] = __fmul_rn(x[e], down);
+    most = fmaxf(most, fabsf(y[e]));
+    least = fminf(least, fabsf(y[e]));
+  }
+  if (least >= 0x1p-6f && most <= 464.f) {  // (464 lies halfway behind 448)
+    uint32_t two[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      asm("{\n\t.reg .b16 t;\n\tcvt.rn.satfinite.e4m3x2.f32 t, %1, %2;\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(two[e]) : "f"(y[2 * e + 1]), "f"(y[2 * e]));
+    return make_uint2(two[0] | (two[1] << 16), two[2] | (two[3] << 16));
+  }
+  return make_uint2(q8_word(x, down), q8_word(x + 4, down));
 }
 // Four codes under a scale that is larger: `shrink` is 2^-(growth).
 __device__ __forceinline__ uint32_t q8_rescaled(uint32_t w, float shrink) {
