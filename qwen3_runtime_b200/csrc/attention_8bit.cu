@@ -666,16 +666,15 @@ template <int D, int NT> int launch_decode(const Decode& a, int num_seqs, cudaSt
 }
 
 // ---- attention in general -----------------------------------------------------------------------------------------------------------------
-// float32, and bfloat16 tokens whose head size or group the tiles above do not take: a block of 256 threads takes a (token, kv head, up to 8
-// of its query heads); 64 keys at a time come to shared memory as they are stored, the next ones while these are worked on; four threads
-// make a key's scores, a warp a head's weights, a thread two channels' results.  Sums are float32 on the FMA pipes, in an order that
-// depends on the keys' places alone: tiles begin at multiples of 64, slices of 256 keys have a softmax of their own and are joined in
-// order, by the same block or, where the launch leaves SMs idle, by a second kernel from what one block a slice has left -- the same bits,
-// however a sequence is cut into steps and batched with others.  What bounds it is instructions.
-constexpr int GEN_THREADS = 256;
-constexpr int GEN_TILE = 64;
-constexpr int GEN_SLICE = 256;
-constexpr int GEN_HEADS = 8;
+// float32, and bfloat16 tokens whose head size or group the tiles above do not take: a block takes a (token, kv head, up to NH of its query heads) and
+// 256 keys at a time, each of its 8 warps 32 of them, with a softmax of their own: a lane makes a key's scores, channel by channel, from codes that it
+// reads itself, then takes two channels (or four, eight) of every value.  No barrier until the warps are joined.  Sums are float32 on the FMA pipes, in an
+// order that depends on the keys' places alone: a warp's 32 keys begin at a multiple of 32, what the warps and then the slices of 256 keys have is joined in
+// order, by the same block or, where the launch leaves SMs idle, by a second kernel from what one block a slice has left -- the same bits, however a
+// sequence is cut into steps and batched with others.  What bounds it is instructions, and for few tokens the chain of a slice.
+constexpr int GEN_WARPS = 8;
+constexpr int GEN_THREADS = 32 * GEN_WARPS;
+constexpr int GEN_SLICE = 32 * GEN_WARPS;
 
 struct General {
   const unsigned char* pages;
@@ -685,193 +684,212 @@ struct General {
   long q_stride;
   float scale_log2;
   float *mid_o, *mid_ml;  // slices > 0: [tokens][nq][slices][D] and [tokens][nq][slices][2]
-  int tiles_at;           // byte of shared memory
   // the last key that token t sees; -1: none (it belongs to no sequence, or its place lies outside the table), and its row is zero
   __device__ __forceinline__ int last_key(long t) const {
     const int seq = token_seq[t], place = places[t];
     return seq >= 0 && seq < num_seqs && place >= 0 && place / ps < max_pages ? place : -1;
   }
-  // the first key of the window of a token that sees keys up to `last`; and whether keys from .. to - 1 hold one that it sees
+  // the first key of the window of a token that sees keys up to `last`
   __device__ __forceinline__ int window_begin(int last) const { return window > 0 ? max(0, last - window + 1) : 0; }
-  __device__ __forceinline__ bool any_seen(int from, int to, int lo) const { return to > lo || from < keep_first; }
+  // Slices that hold a key which the token sees: 0 .. kept - 1, and those from kept + gap on.
+  __device__ __forceinline__ int kept_slices(int lo) const { return min((keep_first + GEN_SLICE - 1) / GEN_SLICE, lo / GEN_SLICE); }
 };
 
-// (m, l, o) <- its join with another's; o and b are unnormalised.  The fused steps are named, so that both kernels round alike.
-__device__ __forceinline__ void join_slices(float& m, float& l, float& o, float bm, float bl, float bo) {
-  const float top = fmaxf(m, bm), fa = exp2f(m - top), fb = exp2f(bm - top);
+// (m, l) <- its join with another slice's, and what results (unnormalised) are multiplied by: o <- o fa + bo fb.  The fused steps are named, so that
+// both kernels round alike.
+__device__ __forceinline__ void join_sums(float& m, float& l, float bm, float bl, float& fa, float& fb) {
+  const float top = fmaxf(m, bm);
+  fa = exp2f(m - top), fb = exp2f(bm - top);
   m = top;
   l = __fmaf_rn(l, fa, __fmul_rn(bl, fb));
-  o = __fmaf_rn(o, fa, __fmul_rn(bo, fb));
 }
-__host__ __device__ __forceinline__ int general_pitch(int D) { return D + 16; }  // bytes of a row in shared memory: the codes, the scale
+// As many neighbouring codes as `v` has places, from an address that is a multiple of that.
+__device__ __forceinline__ void read_codes(const unsigned char* at, float (&v)[2]) {
+  float y[4];
+  q8_floats(*reinterpret_cast<const uint16_t*>(at), y);
+  v[0] = y[0], v[1] = y[1];
+}
+__device__ __forceinline__ void read_codes(const unsigned char* at, float (&v)[4]) { q8_floats(*reinterpret_cast<const uint32_t*>(at), v); }
+__device__ __forceinline__ void read_codes(const unsigned char* at, float (&v)[8]) {
+  const uint2 w = *reinterpret_cast<const uint2*>(at);
+  float lo[4], hi[4];
+  q8_floats(w.x, lo);
+  q8_floats(w.y, hi);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+}
 
-template <typename T>
+// NH: heads of a block; CH: channels of a lane (heads of up to 32 CH channels).
+template <typename T, int NH, int CH>
 __global__ void __launch_bounds__(GEN_THREADS) general_8bit_kernel(General a, const T* __restrict__ q, T* __restrict__ out) {
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(16) float shared[];
   pdl_wait();
   pdl_launch_dependents();
-  const int R = a.nq / a.nkv, chunks = (R + GEN_HEADS - 1) / GEN_HEADS;
-  const int t = blockIdx.x, kvh = blockIdx.y / chunks, h0 = kvh * R + (blockIdx.y % chunks) * GEN_HEADS;
-  const int heads = min(GEN_HEADS, kvh * R + R - h0);
-  const int D = a.D, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, mask = q8_mask(D);
+  const int R = a.nq / a.nkv, chunks = (R + NH - 1) / NH, D = a.D, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, mask = q8_mask(D);
+  const int t = blockIdx.x, kvh = blockIdx.y / chunks, h0 = kvh * R + (blockIdx.y - kvh * chunks) * NH, heads = min(NH, kvh * R + R - h0);
   const Q8Page L(D, a.ps);
-  float* q_s = reinterpret_cast<float*>(smem);                   // [8][D]
-  float* x_s = q_s + GEN_HEADS * D;                              // [8][64] scores
-  float* p_s = x_s + GEN_HEADS * GEN_TILE;                       // [64][8] weights
-  float* f_s = p_s + GEN_HEADS * GEN_TILE;                       // [8]: what the results so far shrink by; then the slice's maximum and sum
-  float* v_s = f_s + 32;                                         // [groups of threads][8][D] at the end of a slice
-  unsigned char* k_s = smem + a.tiles_at;                        // two tiles: 64 rows of keys, then of values, each with its page's scale behind
-  const int pitch = general_pitch(D), bytes = 2 * GEN_TILE * pitch;
-  const int last = a.last_key(t), lo = a.window_begin(last);
+  float* q_s = shared;                                  // [NH][D]
+  float* o_s = q_s + NH * D;                            // [warps][NH][D]
+  float* ml_s = o_s + GEN_WARPS * NH * D;               // [warps][NH][2]: maxima and sums
+  float* f_s = ml_s + GEN_WARPS * NH * 2;               // [warps + 2][NH]: what the warps' results, the slices so far and this one are multiplied by
+  float2* p_s = reinterpret_cast<float2*>(f_s + (GEN_WARPS + 2) * NH) + warp * 32 * NH;  // [32][NH], this warp's weights, twice each
+  const int last = a.last_key(t), lo = a.window_begin(last), mine = CH * lane;  // this lane's first channel
   const int* bt = a.block_table + (long)(last >= 0 ? a.token_seq[t] : 0) * a.max_pages;
-  for (int i = tid; i < heads * D; i += GEN_THREADS) q_s[i] = to_f32(q[t * a.q_stride + (long)h0 * D + i]) * a.scale_log2;
-  // a thread owns channels c and c + 1 of the keys g, g + parts, g + 2 parts ... of each tile
-  const int parts = 2 * GEN_THREADS / D, c = 2 * (tid % (D / 2)), part = tid / (D / 2);
-  const bool owner = part < parts;
-  // two threads bring a row (64 of keys, then 64 of values), every other piece each, pieces put in order, a tile ahead of its use, into two
-  // buffers in turn; what is not there is zero
-  const int my_row = tid & (2 * GEN_TILE - 1), my_half = tid >> 7, my_v = my_row >= GEN_TILE;
-  auto fetch = [&](int base, int stop, int buffer) {
-    const int key = base + (my_row & (GEN_TILE - 1));
-    const unsigned char *codes = a.pages, *scale = a.pages;
-    int there = 0, swap = 0;
-    if (key < stop && (key >= lo || key < a.keep_first)) {
-      const int pi = key / a.ps, page = bt[pi];
-      if ((uint32_t)page < (uint32_t)a.num_pages) {
-        const int pr = key - pi * a.ps;
-        const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
-        codes = rec + (my_v ? L.values : 0) + (long)pr * D;
-        scale = rec + L.scales + 4 * my_v;
-        there = 1, swap = pr & mask;
-      }
-    }
-    const uint32_t dst = smem_addr(k_s) + buffer * bytes + my_row * pitch;
-    for (int p = my_half; p < D / 16; p += 2) cp_async16(dst + 16 * p, codes + 16 * (p ^ swap) * there, 16 * there);
-    if (my_half == 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst + D), "l"(scale), "r"(4 * there));
-    cp_async_commit();
-  };
-  float M[GEN_HEADS], S[GEN_HEADS], O[GEN_HEADS][2];
+  for (int i = tid; i < NH * D; i += GEN_THREADS) q_s[i] = i < heads * D ? to_f32(q[t * a.q_stride + (long)h0 * D + i]) * a.scale_log2 : 0.f;
+  __syncthreads();
+  // thread h keeps head h's joined maximum and sum; a thread the joined results of (head, channel) tid, tid + 256 ...
+  constexpr int OWN = NH * CH * 32 / GEN_THREADS;
+  float M = MINUS_BIG, S = 0.f, O[OWN];
 #pragma unroll
-  for (int h = 0; h < GEN_HEADS; ++h) M[h] = MINUS_BIG, S[h] = 0.f, O[h][0] = O[h][1] = 0.f;
-  const int slice0 = a.slices > 0 ? blockIdx.z : 0, slice1 = a.slices > 0 ? blockIdx.z : last / GEN_SLICE;
-  const int stop = min(last + 1, (slice1 + 1) * GEN_SLICE);
-  // the next tile at or behind `base` that has a key which the token sees (`stop` or beyond: none)
-  auto next_tile = [&](int base) { return base < stop && !a.any_seen(base, base + GEN_TILE, lo) ? max(base, lo / GEN_TILE * GEN_TILE) : base; };
-  int base = next_tile(slice0 * GEN_SLICE), buffer = 0;
-  fetch(base, stop, 0);
-  while (base < stop) {  // (last < 0: not once)
-    const int end = min(last + 1, (base / GEN_SLICE + 1) * GEN_SLICE);
-    float o[GEN_HEADS][2];
-#pragma unroll
-    for (int h = 0; h < GEN_HEADS; ++h) o[h][0] = o[h][1] = 0.f;
-    float m = MINUS_BIG, l = 0.f;  // warp h: of head h, the same in every lane
-    while (base < end) {
-      __syncthreads();
-      const int next = next_tile(base + GEN_TILE);
-      fetch(next, stop, buffer ^ 1);
-      cp_async_wait<1>();
-      __syncthreads();
-      const unsigned char* tile = k_s + buffer * bytes;
-      {  // four threads a key, each every fourth word of 8 channels in order, the four threads' sums in pairs
-        const int key = tid >> 2, sub = tid & 3;
-        const unsigned char* row = tile + key * pitch;
-        float x[GEN_HEADS];
-#pragma unroll
-        for (int h = 0; h < GEN_HEADS; ++h) x[h] = 0.f;
-        for (int w = sub; w < D / 8; w += 4) {
-          const uint2 code = *reinterpret_cast<const uint2*>(row + 8 * w);
-          float va[4], vb[4];
-          q8_floats(code.x, va);
-          q8_floats(code.y, vb);
-#pragma unroll
-          for (int h = 0; h < GEN_HEADS; ++h)
-            if (h < heads) {
-              const float4 qa = *reinterpret_cast<const float4*>(q_s + h * D + 8 * w), qb = *reinterpret_cast<const float4*>(q_s + h * D + 8 * w + 4);
-              x[h] = fmaf(qa.x, va[0], x[h]), x[h] = fmaf(qa.y, va[1], x[h]), x[h] = fmaf(qa.z, va[2], x[h]), x[h] = fmaf(qa.w, va[3], x[h]);
-              x[h] = fmaf(qb.x, vb[0], x[h]), x[h] = fmaf(qb.y, vb[1], x[h]), x[h] = fmaf(qb.z, vb[2], x[h]), x[h] = fmaf(qb.w, vb[3], x[h]);
-            }
-        }
-        const float scale = *reinterpret_cast<const float*>(row + D);
-        const int place = base + key;
-        const bool seen = place < end && (place >= lo || place < a.keep_first);
-#pragma unroll
-        for (int h = 0; h < GEN_HEADS; ++h) {
-          x[h] += __shfl_xor_sync(0xffffffffu, x[h], 1);
-          x[h] += __shfl_xor_sync(0xffffffffu, x[h], 2);
-          if (sub == (h & 3) && h < heads) x_s[h * GEN_TILE + key] = seen ? x[h] * scale : -INFINITY;
-        }
-      }
-      __syncthreads();
-      if (warp < heads) {
-        const float x0 = x_s[warp * GEN_TILE + lane], x1 = x_s[warp * GEN_TILE + 32 + lane];
-        const float top = fmaxf(m, warp_max(fmaxf(x0, x1))), f = exp2f(m - top);
-        const float p0 = exp2f(x0 - top), p1 = exp2f(x1 - top);
-        p_s[GEN_HEADS * lane + warp] = p0, p_s[GEN_HEADS * (lane + 32) + warp] = p1;
-        l = l * f + warp_sum(p0 + p1);
-        m = top;
-        if (lane == 0) f_s[warp] = f;
-      }
-      __syncthreads();
-      if (owner) {
-#pragma unroll
-        for (int h = 0; h < GEN_HEADS; ++h)
-          if (h < heads) o[h][0] *= f_s[h], o[h][1] *= f_s[h];
-        const unsigned char* rows = tile + GEN_TILE * pitch;
-        for (int key = part; key < GEN_TILE; key += parts) {
-          const unsigned char* row = rows + key * pitch;
-          const float scale = *reinterpret_cast<const float*>(row + D);
-          const uint32_t two = q8_halves(*reinterpret_cast<const uint16_t*>(row + c));
-          float v0, v1;
-          asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}" : "=f"(v0), "=f"(v1) : "r"(two));
-          v0 *= scale, v1 *= scale;
-          float w[GEN_HEADS];
-          *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(p_s + GEN_HEADS * key);
-          if (heads > 4) *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(p_s + GEN_HEADS * key + 4);
-#pragma unroll
-          for (int h = 0; h < GEN_HEADS; ++h)
-            if (h < heads) o[h][0] = fmaf(w[h], v0, o[h][0]), o[h][1] = fmaf(w[h], v1, o[h][1]);
-        }
-      }
-      base = next, buffer ^= 1;
-    }
-    // the threads' shares of a channel, in order; then the slice joins what came before it
-    __syncthreads();
-    if (owner) {
-#pragma unroll
-      for (int h = 0; h < GEN_HEADS; ++h)
-        if (h < heads) *reinterpret_cast<float2*>(v_s + (part * GEN_HEADS + h) * D + c) = make_float2(o[h][0], o[h][1]);
-    }
-    if (warp < heads && lane == 0) f_s[8 + 2 * warp] = m, f_s[9 + 2 * warp] = l;
-    __syncthreads();
-    if (owner && part == 0) {
-#pragma unroll
-      for (int h = 0; h < GEN_HEADS; ++h)
-        if (h < heads) {
-          float2 y = *reinterpret_cast<const float2*>(v_s + h * D + c);
-          for (int g = 1; g < parts; ++g) {
-            const float2 z = *reinterpret_cast<const float2*>(v_s + (g * GEN_HEADS + h) * D + c);
-            y.x += z.x, y.y += z.y;
-          }
-          float m0 = M[h], l0 = S[h];
-          join_slices(m0, l0, O[h][0], f_s[8 + 2 * h], f_s[9 + 2 * h], y.x);
-          join_slices(M[h], S[h], O[h][1], f_s[8 + 2 * h], f_s[9 + 2 * h], y.y);
-        }
-    }
+  for (int i = 0; i < OWN; ++i) O[i] = 0.f;
+  const int kept = a.kept_slices(lo), gap = lo / GEN_SLICE - kept, count = last < 0 ? 0 : last / GEN_SLICE + 1 - gap;
+  int first_slice = 0, stop_slice = count;  // of those that count
+  if (a.slices > 0) {
+    const int z = blockIdx.z;
+    first_slice = z < kept ? z : z - gap;
+    stop_slice = (z >= kept && z < kept + gap) || first_slice >= count ? first_slice : first_slice + 1;
   }
-  cp_async_wait<0>();  // (the tile behind the last one: zeros)
-  if (owner && part == 0) {
+  for (int s = first_slice; s < stop_slice; ++s) {
+    const int key = (s + (s >= kept ? gap : 0)) * GEN_SLICE + 32 * warp + lane;
+    const bool seen = key <= last && (key >= lo || key < a.keep_first);
+    // this lane's key: where its codes lie
+    const unsigned char* rec = nullptr;
+    int row = 0;
+    if (seen) {
+      const int pi = key / a.ps, page = bt[pi];
+      row = key - pi * a.ps;
+      if ((uint32_t)page < (uint32_t)a.num_pages) rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
+    }
+    const uint32_t there = __ballot_sync(0xffffffffu, rec != nullptr);
+    float m[NH], l[NH];
+    float2 o[NH][CH / 2];
 #pragma unroll
-    for (int h = 0; h < GEN_HEADS; ++h)
-      if (h < heads) {
-        if (a.slices > 0) {
-          const long at = ((long)t * a.nq + h0 + h) * a.slices + blockIdx.z;
-          a.mid_o[at * D + c] = O[h][0], a.mid_o[at * D + c + 1] = O[h][1];
-          if (c == 0) a.mid_ml[2 * at] = M[h], a.mid_ml[2 * at + 1] = S[h];
-        } else {
-          T* y = out + ((long)t * a.nq + h0 + h) * D + c;
-          y[0] = from_f32<T>(last >= 0 ? O[h][0] / S[h] : 0.f), y[1] = from_f32<T>(last >= 0 ? O[h][1] / S[h] : 0.f);
+    for (int h = 0; h < NH; ++h) {
+      m[h] = MINUS_BIG, l[h] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH / 2; ++c) o[h][c] = make_float2(0.f, 0.f);
+    }
+    if (there) {
+      float2 x[NH];  // sums over every second channel (two of them an instruction)
+#pragma unroll
+      for (int h = 0; h < NH; ++h) x[h] = make_float2(0.f, 0.f);
+      const unsigned char *codes = rec + (long)row * D, *values = codes + L.values;
+      float2 scale = make_float2(0.f, 0.f);
+      if (rec) {
+        scale = *reinterpret_cast<const float2*>(rec + L.scales);
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(values));
+        if (D > 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(values + 128));
+      }
+#pragma unroll 1
+      for (int piece0 = 0; piece0 < D / 16; piece0 += 4) {  // four loads at a time
+        uint4 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = make_uint4(0, 0, 0, 0);
+          if (rec && piece0 + i < D / 16) w[i] = *reinterpret_cast<const uint4*>(codes + 16 * ((piece0 + i) ^ (row & mask)));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (piece0 + i >= D / 16) break;
+          const uint32_t word[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          const float* y_at = q_s + 16 * (piece0 + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v[4];
+            q8_floats(word[e], v);
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+              const float4 y = *reinterpret_cast<const float4*>(y_at + h * D + 4 * e);
+              x[h] = __ffma2_rn(make_float2(y.x, y.y), make_float2(v[0], v[1]), x[h]);
+              x[h] = __ffma2_rn(make_float2(y.z, y.w), make_float2(v[2], v[3]), x[h]);
+            }
+          }
         }
       }
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const float y = rec ? (x[h].x + x[h].y) * scale.x : -INFINITY;
+        m[h] = fmaxf(MINUS_BIG, warp_max(y));
+        const float p = exp2f(y - m[h]), w = p * scale.y;  // (a power of two: what the values are to be multiplied by)
+        l[h] = warp_sum(p);
+        x[h] = make_float2(w, w);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < NH; h += 2) *reinterpret_cast<float4*>(p_s + lane * NH + h) = make_float4(x[h].x, x[h].y, x[h + 1].x, x[h + 1].y);
+      __syncwarp();
+      // where this lane's value row begins, a multiple of 16, and below that how its pieces are ordered
+      const unsigned long long where = reinterpret_cast<unsigned long long>(values) | (uint32_t)(row & mask);
+#pragma unroll 1
+      for (int k0 = 0; k0 < 32; k0 += 8) {
+        if (!(there >> k0 & 255u)) continue;
+        float v[8][CH];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const unsigned long long from = __shfl_sync(0xffffffffu, where, k0 + k);
+#pragma unroll
+          for (int c = 0; c < CH; ++c) v[k][c] = 0.f;
+          if ((there >> (k0 + k) & 1u) && mine < D) read_codes(reinterpret_cast<const unsigned char*>(from & ~15ull) + (mine ^ ((int)from << 4 & 0xF0)), v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float2 p[NH];
+#pragma unroll
+          for (int h = 0; h < NH; h += 2) *reinterpret_cast<float4*>(p + h) = *reinterpret_cast<const float4*>(p_s + (k0 + k) * NH + h);
+#pragma unroll
+          for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int c = 0; c < CH / 2; ++c) o[h][c] = __ffma2_rn(p[h], make_float2(v[k][2 * c], v[k][2 * c + 1]), o[h][c]);
+        }
+      }
+    }
+    // the warps' results, joined in order to what came before
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      if (lane == 0) *reinterpret_cast<float2*>(ml_s + 2 * (warp * NH + h)) = make_float2(m[h], l[h]);
+#pragma unroll
+      for (int c = 0; c < CH / 2; ++c)
+        if (mine < D) *reinterpret_cast<float2*>(o_s + (warp * NH + h) * D + mine + 2 * c) = o[h][c];
+    }
+    __syncthreads();
+    if (tid < NH) {
+      float top = MINUS_BIG, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < GEN_WARPS; ++w) top = fmaxf(top, ml_s[2 * (w * NH + tid)]);
+#pragma unroll
+      for (int w = 0; w < GEN_WARPS; ++w) {
+        const float f = exp2f(ml_s[2 * (w * NH + tid)] - top);
+        f_s[w * NH + tid] = f;
+        sum = __fmaf_rn(f, ml_s[2 * (w * NH + tid) + 1], sum);
+      }
+      join_sums(M, S, top, sum, f_s[GEN_WARPS * NH + tid], f_s[(GEN_WARPS + 1) * NH + tid]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int u = tid + GEN_THREADS * i, h = u / D;
+      if (u < NH * D) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < GEN_WARPS; ++w) sum = __fmaf_rn(f_s[w * NH + h], o_s[w * NH * D + u], sum);
+        O[i] = __fmaf_rn(O[i], f_s[GEN_WARPS * NH + h], __fmul_rn(sum, f_s[(GEN_WARPS + 1) * NH + h]));
+      }
+    }
+    __syncthreads();
+  }
+  if (tid < NH) ml_s[tid] = S;
+  if (a.slices > 0 && tid < heads) *reinterpret_cast<float2*>(a.mid_ml + 2 * (((long)t * a.nq + h0 + tid) * a.slices + blockIdx.z)) = make_float2(M, S);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const int u = tid + GEN_THREADS * i, h = u / D, c = u - h * D;
+    if (u >= heads * D) continue;
+    if (a.slices > 0) {
+      const long at = ((long)t * a.nq + h0 + h) * a.slices + blockIdx.z;
+      a.mid_o[at * D + c] = O[i];
+    } else {
+      out[((long)t * a.nq + h0 + h) * D + c] = from_f32<T>(last >= 0 ? O[i] / ml_s[h] : 0.f);
+    }
   }
 }
 
@@ -881,42 +899,51 @@ template <typename T> __global__ void general_8bit_merge_kernel(General a, T* __
   pdl_launch_dependents();
   const long at = blockIdx.x;
   const int last = a.last_key(at / a.nq), lo = a.window_begin(last);
-  const int stop = last >= 0 ? min(last / GEN_SLICE + 1, a.slices) : 0;
-  const int kept = min((a.keep_first + GEN_SLICE - 1) / GEN_SLICE, lo / GEN_SLICE), gap = lo / GEN_SLICE - kept;  // slices 0 .. kept - 1 and kept + gap ..
+  const int kept = a.kept_slices(lo), gap = lo / GEN_SLICE - kept, count = last < 0 ? 0 : min(last / GEN_SLICE + 1, a.slices) - gap;
   for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
     float M = MINUS_BIG, S = 0.f, O = 0.f;
-    for (int s0 = 0; s0 < stop - gap; s0 += 8) {  // eight slices' loads at a time
+    for (int s0 = 0; s0 < count; s0 += 8) {  // eight slices' loads at a time
       float m[8], l[8], o[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (s0 + u < stop - gap) {
+        if (s0 + u < count) {
           const long i = at * a.slices + s0 + u + (s0 + u >= kept ? gap : 0);
           m[u] = a.mid_ml[2 * i], l[u] = a.mid_ml[2 * i + 1], o[u] = a.mid_o[i * a.D + c];
         }
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (s0 + u < stop - gap) join_slices(M, S, O, m[u], l[u], o[u]);
+        if (s0 + u < count) {
+          float fa, fb;
+          join_sums(M, S, m[u], l[u], fa, fb);
+          O = __fmaf_rn(O, fa, __fmul_rn(o[u], fb));
+        }
     }
     out[at * a.D + c] = from_f32<T>(last >= 0 ? O / S : 0.f);
   }
 }
 
-template <typename T> int launch_general(General a, const T* q, T* out, int tokens, cudaStream_t stream) {
-  const int R = a.nq / a.nkv, chunks = (R + GEN_HEADS - 1) / GEN_HEADS, parts = 2 * GEN_THREADS / a.D;
-  const int tiles_at = ((GEN_HEADS * (a.D + 2 * GEN_TILE) + 32 + parts * GEN_HEADS * a.D) * 4 + 15) & ~15;
-  a.tiles_at = tiles_at;
-  const int smem = tiles_at + 2 * 2 * GEN_TILE * general_pitch(a.D);
+template <typename T, int NH, int CH> int launch_general_as(const General& a, const T* q, T* out, int tokens, cudaStream_t stream) {
+  const int chunks = (a.nq / a.nkv + NH - 1) / NH;
+  const int smem = 4 * (NH * a.D * (1 + GEN_WARPS) + NH * (GEN_WARPS * (2 + 1 + 64) + 2));
   static bool once[Q3_MAX_DEVICES];
   const int dev = q3_current_device();
   if (!once[dev]) {
-    if (cudaFuncSetAttribute(general_8bit_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024) != cudaSuccess) return Q3_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(general_8bit_kernel<T, NH, CH>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != cudaSuccess) return Q3_ERR_LAUNCH;
     once[dev] = true;
   }
-  cudaError_t err = launch_pdl(general_8bit_kernel<T>, dim3(tokens, a.nkv * chunks, a.slices > 0 ? a.slices : 1), dim3(GEN_THREADS), smem, stream,
+  cudaError_t err = launch_pdl(general_8bit_kernel<T, NH, CH>, dim3(tokens, a.nkv * chunks, a.slices > 0 ? a.slices : 1), dim3(GEN_THREADS), smem, stream,
                                a, q, out);
   if (err == cudaSuccess && a.slices > 0)
     err = launch_pdl(general_8bit_merge_kernel<T>, dim3((unsigned)((long)tokens * a.nq)), dim3(a.D <= 128 ? 128 : 256), 0, stream, a, out);
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
+}
+template <typename T> int launch_general(const General& a, const T* q, T* out, int tokens, cudaStream_t stream) {
+  if (a.nq / a.nkv <= 4) {
+    if (a.D <= 64) return launch_general_as<T, 4, 2>(a, q, out, tokens, stream);
+    return a.D <= 128 ? launch_general_as<T, 4, 4>(a, q, out, tokens, stream) : launch_general_as<T, 4, 8>(a, q, out, tokens, stream);
+  }
+  if (a.D <= 64) return launch_general_as<T, 8, 2>(a, q, out, tokens, stream);
+  return a.D <= 128 ? launch_general_as<T, 8, 4>(a, q, out, tokens, stream) : launch_general_as<T, 8, 8>(a, q, out, tokens, stream);
 }
 
 }  // namespace
@@ -962,7 +989,7 @@ Q3_EXPORT int q3_general_attention_8bit(int dtype, const void* q, long q_stride,
       slices < 0 || (slices > 0 && (!mid_o || !mid_ml)) || keep_first < 0)
     return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
-  if ((long)nkv * ((nq / nkv + GEN_HEADS - 1) / GEN_HEADS) > 65535 || slices > 65535 || (long)tokens * nq > 0x7fffffffL ||
+  if ((long)nkv * ((nq / nkv + 3) / 4) > 65535 || slices > 65535 || (long)tokens * nq > 0x7fffffffL ||
       (reinterpret_cast<uintptr_t>(pages) & 15))
     return Q3_ERR_UNSUPPORTED;
   General a{(const unsigned char*)pages, num_pages, block_table, token_seq, places, max_pages, num_seqs, nq, nkv, D, ps, window,
