@@ -2660,32 +2660,35 @@ class CudaOps:
         what = "paged_attention_8bit"
         D, G, H, dtype, shape, rows = head_dim, num_kv_heads, num_heads, out.dtype, q.shape, out.shape
         _, (table_rows, max_pages) = self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens, record_of=_eight_bit_record)
-        window, keep_first = int(window or 0), int(keep_first or 0)
-        if window < 0 or keep_first < 0 or window + keep_first > 1 << 30:
-            raise KernelError(f"{what}: a window and the first tokens are no fewer than none (got {window}, {keep_first})")
-        keep_first = keep_first if window else 0
+        if window or keep_first:
+            window, keep_first = int(window or 0), int(keep_first or 0)
+            if window < 0 or keep_first < 0 or window + keep_first > 1 << 30:
+                raise KernelError(f"{what}: a window and the first tokens are no fewer than none (got {window}, {keep_first})")
+            keep_first = keep_first if window else 0
+        else:
+            window = keep_first = 0
         if H < 1 or H % G or q.dtype != dtype or len(rows) != 2 or rows[1] != H * D or not out.is_contiguous():
             raise KernelError(f"{what}: out is dense [tokens, heads * head_dim] of the queries' type, heads a multiple of kv heads")
         T = rows[0]
         if (len(shape) != 2 or shape[0] < T or shape[1] < H * D or q_stride < H * D or T != step.num_tokens
                 or q.stride() != (q_stride if shape[0] > 1 else q.stride(0), 1)):
             raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step, q_stride apart")
-        longest = step.kv_longest
-        self._check_step_4bit(what, step.cu_seqlens, step.num_seqs + 1, q, out, longest)
+        longest, seqs, max_len = step.kv_longest, step.num_seqs, step.max_kv_len
+        self._check_step_4bit(what, step.cu_seqlens, seqs + 1, q, out, longest)
         room = max_pages * page_size
-        if step.max_kv_len > room or step.num_seqs > table_rows:
-            raise KernelError(f"{what}: {step.num_seqs} sequences of up to {step.max_kv_len} tokens do not fit a block table of "
-                              f"{table_rows} x {max_pages} pages")
-        max_len = min(step.captured_width * page_size, room) if step.captured_width else step.max_kv_len
-        fast = (dtype == torch.bfloat16 and D in (64, 128, 256) and H // G <= 16 and q_stride % 8 == 0 and q.data_ptr() % 16 == 0
-                and out.data_ptr() % 8 == 0)
+        if max_len > room or seqs > table_rows:
+            raise KernelError(f"{what}: {seqs} sequences of up to {max_len} tokens do not fit a block table of {table_rows} x {max_pages} pages")
+        if step.captured_width:
+            max_len = min(step.captured_width * page_size, room)
+        q_at, out_at = q.data_ptr(), out.data_ptr()
+        fast = dtype == torch.bfloat16 and D in (64, 128, 256) and H // G <= 16 and not (q_stride & 7 or q_at & 15 or out_at & 7)
         if fast and step.decode_only:
             if longest is not None and (longest.dtype != torch.int32 or longest.numel() < 1):
                 raise KernelError(f"{what}: kv_longest is one int32")
-            return self._decode_8bit(q, q_stride, H, G, D, pages, block_table, step, None, step.num_seqs, max_len,
-                                     decode_slices or self.decode_slices_8bit(step.host_kv_lens, G, D, window, H // G, keep_first), out,
+            return self._decode_8bit(q_at, q_stride, H, G, D, pages, block_table, step, None, seqs, max_len,
+                                     decode_slices or self.decode_slices_8bit(step.host_kv_lens, G, D, window, H // G, keep_first), out, out_at,
                                      page_size, scale, window, keep_first, longest)
-        aligned = q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0  # what the kernels for wide pages go by
+        aligned = not (q_at & 15 or out_at & 15)  # what the kernels for wide pages go by
         if dtype == torch.float32 or (step.decode_only and not fast) or not aligned:
             return self._general_8bit(q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window, keep_first)
         # portions of prompts (and single tokens beside them): their sequences' pages unpacked, the kernels for wide pages
@@ -2700,8 +2703,9 @@ class CudaOps:
         lens = list(step.host_kv_lens[:step.num_seqs]) if exact else [max_len] * step.num_seqs
         if split and step.num_single:
             own = [kv for b, kv in enumerate(lens) if cu[b + 1] - cu[b] == 1]
-            self._decode_8bit(q, q_stride, H, G, D, pages, block_table, step, singles, step.num_single, max(own),
-                              self.decode_slices_8bit(own, G, D, window, H // G, keep_first), out, page_size, scale, window, keep_first, None)
+            self._decode_8bit(q_at, q_stride, H, G, D, pages, block_table, step, singles, step.num_single, max(own),
+                              self.decode_slices_8bit(own, G, D, window, H // G, keep_first), out, out_at, page_size, scale, window, keep_first,
+                              None)
         counts = unpacked_pages_4bit(cu, lens, page_size, window, 2 if split else 1, exact, keep_first)
         total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * page_size * D)
         if total <= limit:
@@ -2722,18 +2726,20 @@ class CudaOps:
         self._check_here("paged_attention_8bit", step.token_seq, step.positions)
         slices, mid_o, mid_ml = -(-max_len // self.GENERAL_SLICE), None, None
         blocks = T * G * -(-(H // G) // 8)
-        # enough blocks without, or more to keep of the slices than 256 MB: each block goes through all slices (the same bits)
-        if slices < 2 or blocks >= 4 * self.SM_COUNT or T * H * slices * D > 1 << 26:
+        # few slices (a block takes less for another one than the second kernel and its scratch do), enough blocks without, or more to keep of the
+        # slices than 256 MB: each block goes through all slices (the same bits)
+        if slices < 3 or blocks >= 4 * self.SM_COUNT or T * H * slices * D > 1 << 26:
             slices = 0
         else:
-            mid_o = torch.empty((T, H, slices, D), dtype=torch.float32, device=out.device)
-            mid_ml = torch.empty((T, H, slices, 2), dtype=torch.float32, device=out.device)
+            mid = torch.empty(T * H * slices * (D + 2), dtype=torch.float32, device=out.device)
+            mid_o = mid.data_ptr()
+            mid_ml = mid_o + 4 * T * H * slices * D
             self.launches += 1
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out))
         self._call("attention_8bit", "q3_general_attention_8bit", "paged_attention_general_8bit", code, _ptr(q), q_stride, _ptr(pages),
                    pages.shape[0], _ptr(block_table), block_table.shape[1], block_table.shape[0], _ptr(step.token_seq),
-                   _ptr(step.positions), _ptr(out), _ptr(mid_o), _ptr(mid_ml), slices, T, H, G, D, page_size, float(scale), window, keep_first)
+                   _ptr(step.positions), _ptr(out), mid_o, mid_ml, slices, T, H, G, D, page_size, float(scale), window, keep_first)
         return out
 
     # Blocks of decode attention over 8-bit numbers that an SM holds, by head size; and what its cost model takes (see there), by head size and
@@ -2797,11 +2803,11 @@ class CudaOps:
             count = self._parts_cache[key] = self._get("attention_8bit", "q3_decode_clusters_8bit")(head_dim, int(wide), size)
         return count
 
-    def _decode_8bit(self, q, q_stride, H, G, D, pages, block_table, step, seq_list, num_seqs, max_len, slices, out, page_size, scale,
-                     window, keep_first, longest):
+    def _decode_8bit(self, q_at, q_stride, H, G, D, pages, block_table, step, seq_list, num_seqs, max_len, slices, out, out_at, page_size,
+                     scale, window, keep_first, longest):
         mid_o = mid_lse = None
-        joined, slices = slices < 0 or slices > 16, abs(slices)  # 16 blocks a cluster at most
-        if joined and slices > 1:
+        if slices < -1 or slices > 16:  # joined by a second kernel (16 blocks a cluster at most)
+            slices = abs(slices)
             mid = torch.empty(num_seqs * H * slices * (D + 1), dtype=torch.float32, device=out.device)
             mid_o = mid.data_ptr()
             mid_lse = mid_o + 4 * num_seqs * H * slices * D
@@ -2810,10 +2816,10 @@ class CudaOps:
             singles = [kv for b, kv in enumerate(step.host_kv_lens) if step.host_cu_seqlens[b + 1] - step.host_cu_seqlens[b] == 1]
             seen = sum(min(kv, window + keep_first) if window else kv for kv in singles)
             self._costs(seen * 2 * G * D + 4 * num_seqs * H * D, 4 * H * D * seen)
-        self._call("attention_8bit", "q3_decode_attention_8bit", "paged_attention_decode_8bit", q.data_ptr(), q_stride, pages.data_ptr(),
-                   pages.shape[0], block_table.data_ptr(), block_table.shape[1], step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(),
-                   _ptr(seq_list), out.data_ptr(), mid_o, mid_lse, num_seqs, H, G, D, page_size, float(scale), window, keep_first,
-                   slices, max_len, _ptr(longest), self._error_word(out.device).data_ptr())
+        self._call("attention_8bit", "q3_decode_attention_8bit", "paged_attention_decode_8bit", q_at, q_stride, pages.data_ptr(),
+                   pages.size(0), block_table.data_ptr(), block_table.size(1), step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(),
+                   _ptr(seq_list), out_at, mid_o, mid_lse, num_seqs, H, G, D, page_size, float(scale), window, keep_first,
+                   abs(slices), max_len, _ptr(longest), self._error_word(out.device).data_ptr())
         return out
 
     # ---- matrix products ----------------------------------------------------------------
