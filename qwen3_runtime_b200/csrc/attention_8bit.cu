@@ -214,15 +214,11 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_8bit_k
   bool behind = at >= sl.first;  // of the gap
   int at_page = (at + (behind ? sl.gap : 0)) / a.ps, at_row = at + (behind ? sl.gap : 0) - at_page * a.ps;
   const int go_pages = ROUND / a.ps, go_rows = ROUND - go_pages * a.ps;
-  auto look_up = [&]() { return at < end ? bt[at_page] : -1; };
-  int page = -1;
-  if (lane < (BULK ? TILES : STEP * TILES)) page = look_up();
+  auto look_up = [&]() { return lane < (BULK ? TILES : STEP * TILES) && at < end ? bt[at_page] : -1; };
+  int page = look_up();
   const uint32_t ring_at = smem_addr(ring) + (BULK ? lane : lane / STEP) * TILE, bar_at = smem_addr(&bars[warp][0]);
   auto load_step = [&](int stage) {  // the token looked up last; then the next is
-    if (lane >= (BULK ? TILES : STEP * TILES)) {
-      if (!BULK) cp_async_commit();
-      return;
-    }
+    if (BULK && lane >= TILES) return;
     const uint32_t dst = ring_at + stage * STAGE;
     const bool valid = (uint32_t)page < (uint32_t)a.num_pages;
     const unsigned char* rec = head + (unsigned long long)(uint32_t)(valid ? page : 0) * page_bytes;
@@ -243,14 +239,22 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_8bit_k
         }
       }
     } else {
-      const int to_row = lane & (STEP - 1), swap = (at_row ^ to_row) & H::MASK;  // pieces stand by the row in the page there, by the tile's here
-      const unsigned char* src = rec + (valid ? (long)at_row * D : 0);
+      // Neighbouring lanes bring neighbouring pieces of a row (every lane a row of its own: 32 lines a copy, half the speed).  A row's address comes from
+      // the lane that looked it up, with how its pieces are ordered (by the row in the page there, by the tile's here) and whether it exists below it.
+      constexpr int PIECES = D / 16, ROWS = 32 / PIECES;
+      const unsigned long long mine = reinterpret_cast<unsigned long long>(rec + (valid ? (long)at_row * D : 0)) | (uint32_t)((at_row ^ lane) & H::MASK) | (valid ? 8u : 0u);
+      const uint32_t to = smem_addr(ring) + stage * STAGE;
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        cp_async16(dst + to_row * D + 16 * c, src + 16 * (c ^ swap), valid ? 16 : 0);
-        cp_async16(dst + VALUES + to_row * D + 16 * c, src + L.values + 16 * (c ^ swap), valid ? 16 : 0);
+      for (int i = 0; i < STEP * TILES / ROWS; ++i) {
+        const int token = i * ROWS + lane / PIECES, piece = lane % PIECES;
+        const unsigned long long from = __shfl_sync(0xffffffffu, mine, token);
+        const unsigned char* src = reinterpret_cast<const unsigned char*>(from & ~15ull) + 16 * (piece ^ ((int)from & 7));
+        const uint32_t at_tile = to + token / STEP * TILE + token % STEP * D + 16 * piece;
+        cp_async16(at_tile, src, from & 8 ? 16 : 0);
+        cp_async16(at_tile + VALUES, src + L.values, from & 8 ? 16 : 0);
       }
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst + SCALES + 8 * to_row), "l"(rec + L.scales), "r"(valid ? 8 : 0));
+      if (lane < STEP * TILES)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst + SCALES + 8 * (lane & (STEP - 1))), "l"(rec + L.scales), "r"(valid ? 8 : 0));
       cp_async_commit();
     }
     at += ROUND, at_page += go_pages, at_row += go_rows;
