@@ -2,8 +2,9 @@
 // with accumulators in tensor memory; Q, K and V tiles arrive by TMA (128-byte swizzle).  bfloat16; four forms:
 //   PAGED    heads of 128 over the paged cache, straight from the QKV buffer and the pages (group size a divisor of 128,
 //            page size 8/16/32/64); options: a chunked mask, turned values, sinks;
-//   FIRST    the same under a window whose tokens see the sequence's first ones as well: the tiles of those come in front, and the ones
-//            between them and the window are left out;
+//   FIRST    over pages as well, for heads of 64 to 128 (columns that a head lacks are beyond the tensors' inner extent, and arrive as zeros) and any
+//            group (a block has as many rows as whole tokens give); optionally under a window, whose tokens may see the sequence's first ones too:
+//            the tiles of those come in front, and the ones between them and the window are left out;
 //   MAPS     differential attention: a head is two maps of 64 side by side in its 128 columns, over one value of 128;
 //            options: a chunked mask or a window;
 //   DENSE    keys of 192 = 128 of the head's own + 64 shared by the heads, values of 128, one key head per query head,
@@ -86,7 +87,7 @@ struct Params {
   const int* kv_base;             // DENSE: key j of sequence s is row kv_base[s] + j
   float lambda, eps, out_scale;   // MAPS
   int* error_word;
-  int keep_first;                 // FIRST: keys that every token sees, whatever its window
+  int keep_first, head_dim;       // FIRST: keys that every token sees, whatever its window; columns of a head
 };
 
 // 2^x in one instruction (exp2f adds range fix-ups around the same instruction; results
@@ -160,6 +161,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
   // heavy items first over the whole grid: all kv heads of the heaviest item, then the next ...
   const int kvh = blockIdx.x % nkv;
   const int G = nq / nkv;
+  const int block_m = MODE == FIRST ? BLOCK_M / G * G : BLOCK_M;  // rows of a block
   const uint32_t bar0 = smem_addr(&bars[0]);
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
@@ -171,7 +173,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
     for (int s = 0; s < p.num_seqs; ++s) {
       const int ql = cu_seqlens[s + 1] - cu_seqlens[s];
       if (ql <= 0 || (p.skip_single && ql == 1)) continue;
-      int nb = (ql * G + BLOCK_M - 1) / BLOCK_M;  // row blocks
+      int nb = (ql * G + block_m - 1) / block_m;  // row blocks
       if (MODE != MAPS) nb = (nb + 1) / 2;        // pairs of them
       if (w < acc + nb) {
         found = s;
@@ -220,7 +222,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
     int row0[2], p_max[2], tiles[2];
     // under a chunked mask or a window the item's first visible key is that of its first row; tiles count from the tile
     // it is in
-    const int p_first = base_pos + (MODE == MAPS ? 1 : 2) * s_item[1] * BLOCK_M / G;
+    const int p_first = base_pos + (MODE == MAPS ? 1 : 2) * s_item[1] * block_m / G;
     const int k_lo = chunk > 0 ? p_first / chunk * chunk : (window > 0 ? max(0, p_first - window + 1) : 0);
     const int tile0 = k_lo / BLOCK_N;
     // FIRST: tiles 0 .. firsts - 1 and those from tile0 on; `skip` of them lie between
@@ -229,9 +231,9 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
     auto tile_at = [&](int j) { return MODE == FIRST ? j + (j >= firsts ? skip : 0) : tile0 + j; };
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      row0[x] = (MODE == MAPS ? s_item[1] : 2 * s_item[1] + x) * BLOCK_M;
+      row0[x] = (MODE == MAPS ? s_item[1] : 2 * s_item[1] + x) * block_m;
       const bool live = row0[x] < rows;
-      const int last_row = min(rows, row0[x] + BLOCK_M) - 1;
+      const int last_row = min(rows, row0[x] + block_m) - 1;
       p_max[x] = live ? base_pos + last_row / G : -1;
       tiles[x] = live ? p_max[x] / BLOCK_N + 1 - skip : 0;
     }
@@ -244,8 +246,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       const int part = warp;  // keys: 0, 1; values: 2, 3
       const int half = part & 1;
       if (part == 3 && lane == 0) {
-        constexpr int BOXES = MODE == MAPS ? 1 : DK / 64;  // of a block; MAPS: map x is columns 64 x .. of the head
-        mbar_expect_tx(bar(BAR_Q), (tiles[1] ? 2 : 1) * BOXES * HALF_Q);
+        const int BOXES = MODE == MAPS ? 1 : MODE == FIRST ? (p.head_dim + 63) / 64 : DK / 64;  // of a block; MAPS: map x is columns 64 x .. of the head
+        mbar_expect_tx(bar(BAR_Q), (tiles[1] ? 2 : 1) * BOXES * (MODE == FIRST ? block_m * 128 : HALF_Q));
         for (int x = 0; x < 2; ++x) {
           if (!tiles[x]) continue;
           for (int c = 0; c < BOXES; ++c) {
@@ -276,8 +278,9 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         const int page = next;
         const uint32_t dst = dst0 + st * stage_bytes;
         uint32_t bytes = HALF_KV + (MODE == DENSE && part == 1 ? HALF_KV : 0);
+        const bool wanted = MODE != FIRST || 64 * half < p.head_dim;  // (heads of up to 64 have no second half)
         if (MODE != DENSE) {
-          bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * (uint32_t)ps * 128u;
+          bytes = wanted ? __popc(__ballot_sync(0xffffffffu, page >= 0)) * (uint32_t)ps * 128u : 0;
           next = page_of(j + 1);
         }
         if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, phase, &abort_flag))) break;
@@ -294,7 +297,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         } else {
           for (int u = 0; u < pages_per_tile; ++u) {
             const int pg = __shfl_sync(0xffffffffu, page, u);
-            if (lane == 0 && pg >= 0) tma_load_2d(dst + u * ps * 128, map, full + 8 * st, half * 64, (pg * nkv + kvh) * ps);
+            if (lane == 0 && pg >= 0 && wanted) tma_load_2d(dst + u * ps * 128, map, full + 8 * st, half * 64, (pg * nkv + kvh) * ps);
           }
         }
         if (++st == KV_STAGES) st = 0, phase ^= 1;
@@ -334,7 +337,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
 #pragma unroll
               for (int k = 0; k < (MODE == MAPS ? 64 : DK) / 16; ++k) {
                 const uint32_t half = (k >> 2), sub = (k & 3) * 2;  // 4 steps of 32 bytes per 64 columns
-                umma_bf16(tmem_x, umma_desc(q_addr + half * HALF_Q) + sub,
+                if (MODE != FIRST || 16 * k < p.head_dim) umma_bf16(tmem_x, umma_desc(q_addr + half * HALF_Q) + sub,
                      umma_desc(k_addr + (MODE == MAPS ? x : half) * HALF_KV) + sub, idesc, k > 0 ? 1u : 0u);
               }
               umma_commit(bar(BAR_S_FULL + x));    // S_j is in TMEM
@@ -347,7 +350,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
           if (++st == KV_STAGES) st = 0, phase ^= 1;
         }
       } else {
-        constexpr uint32_t idesc = umma_idesc(BLOCK_M, D, 1);  // PV: N = 128, V MN-major
+        // PV: N = 128 (64 for smaller heads), V MN-major
+        const uint32_t idesc = MODE == FIRST && p.head_dim <= 64 ? umma_idesc(BLOCK_M, 64, 1) : umma_idesc(BLOCK_M, D, 1);
         bool ok = true;
         for (int j = 0; j < all && ok; ++j) {
           ok = (j >= mine || wait_all(BAR_P_FULL + x, j & 1)) && wait_all(BAR_V_FULL + st, phase);  // P_j written, O at rest
@@ -380,7 +384,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       const int quarter = warp & 3;
       const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
       const int R = row0[x] + r;
-      const bool row_ok = R < rows;
+      const bool row_ok = R < rows && (MODE != FIRST || r < block_m);
       const int pos = row_ok ? base_pos + R / G : -1;
       // the row's first visible key
       const int lo = !row_ok ? 0 : (chunk > 0 ? pos / chunk * chunk : (window > 0 ? max(0, pos - window + 1) : 0));
@@ -495,7 +499,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         return true;
       };
       // tiles that every row of the block sees as a whole: from the last row's first key on, up to the first row's position
-      const int row_first = row0[x], row_last = min(rows, row0[x] + BLOCK_M) - 1;
+      const int row_first = row0[x], row_last = min(rows, row0[x] + block_m) - 1;
       const int pos_first = base_pos + row_first / G, pos_last = base_pos + row_last / G;
       const int lo_last = chunk > 0 ? pos_last / chunk * chunk : (window > 0 ? max(0, pos_last - window + 1) : 0);
       // (What rows that are none see in a last block has no say: nothing of theirs is stored.  A last block that goes through tiles with
@@ -572,7 +576,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         if (p.sinks && row_ok) l_run += exp2f(p.sinks[kvh * G + R % G] * LOG2_E - m_ref * scale_log2);
         const float inv = 1.f / l_run;
         const float* turns = MODE == PAGED ? p.turns : nullptr;
-        bf16* dst = row_ok ? p.out + ((long)(tok0 + R / G) * nq + kvh * G + R % G) * D : nullptr;
+        const int cols = MODE == FIRST ? p.head_dim : D;
+        bf16* dst = row_ok ? p.out + ((long)(tok0 + R / G) * nq + kvh * G + R % G) * cols : nullptr;
         if (turns) {  // turned values: the sum is turned back, element c with element c + D / 2
           const float* cs = row_ok ? turns + (long)(tok0 + R / G) * D : nullptr;  // cos (D / 2), sin (D / 2)
 #pragma unroll 1
@@ -600,7 +605,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
           }
         }
 #pragma unroll 1
-        for (int c0 = 0; c0 < D && !turns; c0 += 32) {
+        for (int c0 = 0; c0 < cols && !turns; c0 += 32) {
           uint32_t ov[32];
           tmem_load32(o_addr + c0, ov);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -610,7 +615,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
               float v8[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) v8[e] = __uint_as_float(ov[c + e]) * inv;
-              store8(dst + c0 + c, v8);
+              if (MODE != FIRST || c0 + c < cols) store8(dst + c0 + c, v8);
             }
           }
         }
@@ -692,23 +697,26 @@ Q3_EXPORT int q3_paged_attention_prefill_tc(const void* q, int q_stride, int num
   return launch<PAGED>(tq, tk, tv, tq, p, stream);
 }
 
-// The same under a window: a token sees the last `window` keys up to itself, and the sequence's first `keep_first`.
+// The same for heads of 64 to 128 (a multiple of 16) and groups of up to 128, num_work = sum over served sequences of ceil(ceil(q_len / (128 / group)) / 2),
+// 128 / group in whole tokens; window > 0: a token sees the last `window` keys up to itself, and the sequence's first `keep_first`.
 Q3_EXPORT int q3_window_attention_prefill_tc(const void* q, int q_stride, int num_tokens, const void* kpages, const void* vpages,
                                              long num_rows_kv, const int* block_table, int max_pages, const int* kv_lens,
                                              const int* cu_seqlens, void* out, int num_seqs, int num_work, int nq, int nkv, int head_dim,
                                              int ps, float scale, int skip_single, int window, int keep_first, int* error_word,
                                              cudaStream_t stream) {
-  if (!q || !kpages || !vpages || !block_table || !kv_lens || !cu_seqlens || !out || window < 1 || keep_first < 0) return Q3_ERR_ARGUMENT;
+  if (!q || !kpages || !vpages || !block_table || !kv_lens || !cu_seqlens || !out || window < 0 || keep_first < 0) return Q3_ERR_ARGUMENT;
   if (nq < 1 || nkv < 1 || nq % nkv) return Q3_ERR_ARGUMENT;
-  if (head_dim != D || !paged_ok(q, q_stride, kpages, vpages, nq, nkv, ps) || ((uintptr_t)out & 15)) return Q3_ERR_UNSUPPORTED;
+  if (head_dim < 64 || head_dim > D || head_dim % 16 || nq / nkv > BLOCK_M || (ps != 8 && ps != 16 && ps != 32 && ps != 64) || q_stride % 8 || nkv > 65535 ||
+      (((uintptr_t)q | (uintptr_t)kpages | (uintptr_t)vpages | (uintptr_t)out) & 15))
+    return Q3_ERR_UNSUPPORTED;
   if (num_work == 0) return Q3_OK;
   CUtensorMap tq, tk, tv;
-  if (!q_map(&tq, q, D, nq, num_tokens, q_stride, nq / nkv) ||
-      !q3_bf16_map(&tk, kpages, num_rows_kv, D, D, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
-      !q3_bf16_map(&tv, vpages, num_rows_kv, D, D, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
+  if (!q_map(&tq, q, head_dim, nq, num_tokens, q_stride, nq / nkv) ||
+      !q3_bf16_map(&tk, kpages, num_rows_kv, head_dim, head_dim, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
+      !q3_bf16_map(&tv, vpages, num_rows_kv, head_dim, head_dim, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
     return Q3_ERR_LAUNCH;
   const Params p = {block_table, max_pages, kv_lens, cu_seqlens, (bf16*)out, num_seqs, num_work, nq, nkv, ps, scale * LOG2_E, skip_single, 0,
-                    window, nullptr, nullptr, nullptr, 0.f, 0.f, 0.f, error_word, keep_first};
+                    window, nullptr, nullptr, nullptr, 0.f, 0.f, 0.f, error_word, keep_first, head_dim};
   return launch<FIRST>(tq, tk, tv, tq, p, stream);
 }
 

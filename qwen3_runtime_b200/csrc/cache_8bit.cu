@@ -307,12 +307,12 @@ __global__ void store_8bit_kernel(const T* qkv, int row_stride, T* q_out, int q_
 // it too.  With it, the attention over prompts reads the pages: only sequences that bring at least `least` tokens count, and of each only the
 // pages that a new token sees (with a window those of the first `keep_first` tokens, and those from the first that the first new token's window
 // reaches); they lie one after the other, `count` pages in all, and `table_out` [num_seqs][width] says where (entries that nobody asks for name a
-// page of the same sequence, never none).
+// page of the same sequence, never none).  The pages that are written are as large as the cache's, or of 16 tokens where the attention does not take those.
 struct Unpack {
   const unsigned char* pages;
   int num_pages, nkv, ps;
   const int *block_table, *kv_lens, *cu_seqlens;
-  int max_pages, num_seqs, max_len, least, window, keep_first, count, width;
+  int max_pages, num_seqs, max_len, least, window, keep_first, count, width, out_ps;  // out_ps: tokens of a page that is written
   int* table_out;
 };
 
@@ -334,9 +334,9 @@ struct UnpackPage {
       if (base + lane < a.num_seqs) {
         const int tokens = a.cu_seqlens[base + lane + 1] - a.cu_seqlens[base + lane], len = min(a.kv_lens[base + lane], a.max_len);
         if (tokens >= a.least && len > 0) {
-          if (a.window > 0) from_page = max(0, len - tokens - a.window + 1) / a.ps;
-          first_pages = min(from_page, (a.keep_first + a.ps - 1) / a.ps);
-          pages = (len + a.ps - 1) / a.ps;
+          if (a.window > 0) from_page = max(0, len - tokens - a.window + 1) / a.out_ps;
+          first_pages = min(from_page, (a.keep_first + a.out_ps - 1) / a.out_ps);
+          pages = (len + a.out_ps - 1) / a.out_ps;
         }
       }
       const int n = pages - from_page + first_pages;
@@ -442,7 +442,55 @@ template <typename T, int KNOWN> __global__ void __launch_bounds__(256) unpack_8
   }
 }
 
+// Into pages of 16 tokens, whatever the cache's: a warp per (page that is written, kv head, keys or values), a lane of the first 16 looks a token up.
+constexpr int OTHER_PAGE = 16;
+template <typename T> __global__ void __launch_bounds__(256) unpack_8bit_other_kernel(Unpack a, int D, T* __restrict__ k_out, T* __restrict__ v_out) {
+  constexpr int CHANNELS = 16 / sizeof(T);
+  const int words = D / CHANNELS, mask = q8_mask(D);
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const uint32_t item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), half = item >> 1;
+  const int is_v = item & 1, p = (int)(half / a.nkv), kvh = (int)(half - (uint32_t)p * a.nkv);
+  const UnpackPage at_page(a, p);
+  if (at_page.seq < 0) return;
+  if (kvh == 0 && !is_v) at_page.name(a, p);
+  const Q8Page L(D, a.ps);
+  // where this lane's token lies, a multiple of 16, and below that how its pieces are ordered; 0: nowhere
+  unsigned long long where = 0;
+  float scale = 0.f;
+  const int key = at_page.i * OTHER_PAGE + lane, in_page = key / a.ps;
+  if (lane < OTHER_PAGE && key < min(a.kv_lens[at_page.seq], a.max_len) && in_page < a.max_pages) {
+    const int page = a.block_table[(long)at_page.seq * a.max_pages + in_page], row = key - in_page * a.ps;
+    if (page >= 0 && page < a.num_pages) {
+      const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
+      scale = reinterpret_cast<const float*>(rec + L.scales)[is_v];
+      where = reinterpret_cast<unsigned long long>(rec + (is_v ? L.values : 0) + (long)row * D) | (uint32_t)(row & mask);
+    }
+  }
+  T* to = (is_v ? v_out : k_out) + ((long)p * a.nkv + kvh) * OTHER_PAGE * D;
+#pragma unroll 4
+  for (int at = lane; at < OTHER_PAGE * words; at += 32) {  // (a whole number of warps)
+    const int row = at / words, channel = CHANNELS * (at - row * words);
+    const unsigned long long from = __shfl_sync(0xffffffffu, where, row);
+    const float s = __shfl_sync(0xffffffffu, scale, row);
+    uint32_t code[CHANNELS / 4];
+#pragma unroll
+    for (int e = 0; e < CHANNELS / 4; ++e) code[e] = 0;
+    if (from) {
+      const unsigned char* c = reinterpret_cast<const unsigned char*>(from & ~15ull) + q8_at(channel, (int)from & 15, 15);
+      if constexpr (CHANNELS == 8)
+        *reinterpret_cast<uint2*>(code) = *reinterpret_cast<const uint2*>(c);
+      else
+        code[0] = *reinterpret_cast<const uint32_t*>(c);
+    }
+    unpack_codes(to + (long)row * D + channel, code, s);
+  }
+}
+
 template <typename T> cudaError_t launch_unpack(const Unpack& a, int D, T* k_out, T* v_out, cudaStream_t stream) {
+  if (a.out_ps != a.ps)
+    return launch_pdl(unpack_8bit_other_kernel<T>, dim3((unsigned)((2L * a.count * a.nkv + 7) / 8)), dim3(256), 0, stream, a, D, k_out, v_out);
   const int parts = (a.ps + unpack_rows(D) - 1) / unpack_rows(D);
   const long items = 2L * (a.cu_seqlens ? a.count : a.width) * a.nkv * parts;
   const dim3 grid((unsigned)((items + 7) / 8), a.cu_seqlens ? 1 : a.num_seqs);
@@ -519,18 +567,19 @@ Q3_EXPORT int q3_store_8bit(int dtype, const void* qkv, int row_stride, void* q_
   return q3_launch_status();
 }
 
-// `cu_seqlens` null: num_seqs * width pages are written; else `count` pages (struct Unpack).
+// `cu_seqlens` null: num_seqs * width pages are written, as large as the cache's; else `count` pages of out_ps tokens (struct Unpack).
 Q3_EXPORT int q3_unpack_8bit(int dtype, const void* pages, int num_pages, int nkv, int D, int ps, const int* block_table, int max_pages,
                              const int* kv_lens, int num_seqs, int max_len, const int* cu_seqlens, int least, int window, int keep_first,
-                             int count, int width, void* k_out, void* v_out, int* table_out, cudaStream_t stream) {
+                             int count, int width, int out_ps, void* k_out, void* v_out, int* table_out, cudaStream_t stream) {
   if (num_seqs < 1 || width < 1 || (cu_seqlens && count < 1)) return Q3_OK;
   if (!pages || !block_table || !kv_lens || !k_out || !v_out || nkv < 1 || max_pages < 1 || !q8_sizes_ok(D, ps)) return Q3_ERR_ARGUMENT;
   if (cu_seqlens && (!table_out || least < 1 || keep_first < 0)) return Q3_ERR_ARGUMENT;
+  if (out_ps != ps && (!cu_seqlens || out_ps != OTHER_PAGE)) return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
   if ((!cu_seqlens && num_seqs > 65535) || !q8_aligned(pages) || !q8_aligned(k_out) || !q8_aligned(v_out)) return Q3_ERR_UNSUPPORTED;
   if ((long)(cu_seqlens ? count : width) * 2 * nkv * ((ps + unpack_rows(D) - 1) / unpack_rows(D)) > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
   const Unpack a{(const unsigned char*)pages, num_pages, nkv, ps, block_table, kv_lens, cu_seqlens, max_pages, num_seqs, max_len, least, window,
-                 keep_first, count, width, table_out};
+                 keep_first, count, width, out_ps, table_out};
   const cudaError_t err = dtype == Q3_DTYPE_F32 ? launch_unpack(a, D, (float*)k_out, (float*)v_out, stream)
                                                 : launch_unpack(a, D, (bf16*)k_out, (bf16*)v_out, stream);
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;

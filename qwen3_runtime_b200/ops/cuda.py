@@ -262,7 +262,7 @@ _SIGNATURES = {
                           c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int,
                           c_int, c_int, c_int, c_int, c_void_p, c_void_p],
         "q3_unpack_8bit": [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
-                           c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+                           c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     },
     "attention_8bit": {
         "q3_decode_attention_8bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -271,6 +271,10 @@ _SIGNATURES = {
         "q3_decode_clusters_8bit": [c_int, c_int, c_int],
         "q3_general_attention_8bit": [c_int, c_void_p, c_long, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                       c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
+    },
+    "prompts_8bit": {
+        "q3_prompts_attention_8bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p],
     },
     "gemm_f32": {
         "q3_gemm_f32": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
@@ -2326,10 +2330,9 @@ class CudaOps:
     # more by itself is taken alone).
     UNPACK_BYTES = 1 << 30
 
-    def _prompts_4bit(self, q, q_stride, H, G, D, pages, block_table, step, first, end, count, longest, split, out, page_size, scale, window,
-                      keep_first=None):
+    def _prompts_4bit(self, q, q_stride, H, G, D, pages, block_table, step, first, end, count, longest, split, out, page_size, scale, window):
         """Attention of the step's sequences ``first .. end - 1``, whose ``count`` pages are unpacked for it (none of those has more than
-        ``longest`` keys).  ``keep_first``: a number for a cache in 8 bits, None for one in 4."""
+        ``longest`` keys)."""
         cu, t0, t1 = step.host_cu_seqlens, step.host_cu_seqlens[first], step.host_cu_seqlens[end]
         part = type(step).__new__(type(step))
         part.__dict__.update(step.__dict__)  # (copy.copy takes five times as long)
@@ -2350,26 +2353,14 @@ class CudaOps:
         width = -(-longest // page_size)
         table = torch.empty((part.num_seqs, width), dtype=torch.int32, device=out.device)
         if self.timing is not None:
-            self._costs(2 * k.numel() * k.element_size() + count * pages.shape[-1] * G)
-        bits, kept = ("4bit", ()) if keep_first is None else ("8bit", (keep_first,))
-        self._call(f"cache_{bits}", f"q3_unpack_{bits}", f"unpack_{bits}", _dtype_code(k.dtype), _ptr(pages), pages.shape[0], G, D, page_size,
+            self._costs(2 * k.numel() * k.element_size() + count * G * four_bit_page_bytes(D, page_size))
+        self._call("cache_4bit", "q3_unpack_4bit", "unpack_4bit", _dtype_code(k.dtype), _ptr(pages), pages.shape[0], G, D, page_size,
                    _ptr(block_table), block_table.shape[1], _ptr(part.kv_lens), part.num_seqs, longest, _ptr(part.cu_seqlens),
-                   2 if split else 1, int(window or 0), *kept, count, width, k.data_ptr(), v.data_ptr(), _ptr(table))
-        if (keep_first is not None and window and split and D == 128 and 128 % (H // G) == 0 and page_size in (8, 16, 32, 64)
-                and self.prefill_attention == "tcgen05"):
-            news = [b - a for a, b in zip(part.host_cu_seqlens, part.host_cu_seqlens[1:])]
-            pairs = sum(-(-(-(-n * H // G // 128)) // 2) for n in news if n > 1)  # two blocks of 128 rows an item
-            if self.timing is not None:
-                self._costs(*self._attention_cost(part, H, G, D, out, prompts=True))
-            self._call("attention_prefill_tc", "q3_window_attention_prefill_tc", "paged_attention_prefill_window", q.data_ptr(), q_stride,
-                       q.shape[0], k.data_ptr(), v.data_ptr(), count * G * page_size, table.data_ptr(), width, part.kv_lens.data_ptr(),
-                       part.cu_seqlens.data_ptr(), out.data_ptr(), part.num_seqs, pairs, H, G, D, page_size, float(scale), 1, window,
-                       keep_first, self._error_word(out.device).data_ptr())
-            return
+                   2 if split else 1, int(window or 0), count, width, k.data_ptr(), v.data_ptr(), _ptr(table))
         # the wide kernels number a token by its place: kv_lens and cu_seqlens say it, or for the general kernel `positions`
         self.paged_attention(q, q_stride, num_heads=H, num_kv_heads=G, head_dim=D, k_pages=k, v_pages=v, block_table=table,
                              token_seq=part.token_seq, positions=part.positions, out=out, page_size=page_size, scale=scale,
-                             window=window, keep_first=keep_first, step=part)
+                             window=window, step=part)
 
     GENERAL_SLICE = 256  # keys with a softmax of their own (csrc/attention_4bit.cu)
 
@@ -2643,8 +2634,8 @@ class CudaOps:
         if self.timing is not None:
             self._costs(2 * k.numel() * k.element_size() + B * n * num_kv_heads * eight_bit_page_bytes(head_dim, page_size))
         self._call("cache_8bit", "q3_unpack_8bit", what, _dtype_code(dtype), pages.data_ptr(), pages.shape[0], num_kv_heads, head_dim,
-                   page_size, block_table.data_ptr(), width, _ptr(kv_lens), B, int(max_kv_len), None, 0, 0, 0, 0, n, k.data_ptr(), v.data_ptr(),
-                   None)
+                   page_size, block_table.data_ptr(), width, _ptr(kv_lens), B, int(max_kv_len), None, 0, 0, 0, 0, n, page_size, k.data_ptr(),
+                   v.data_ptr(), None)
         return k, v
 
     def paged_attention_8bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, block_table, out, page_size, scale, step,
@@ -2652,11 +2643,12 @@ class CudaOps:
         """:meth:`paged_attention` over a cache in 8 bits; ``window``: a token sees that many tokens up to itself; ``keep_first``: with a window,
         the sequence's first tokens as well.  A sequence's tokens are the first ``kv_lens`` places of its cache and the step's tokens the last
         of them; ``step.positions`` are places here.  Single tokens of bfloat16 heads of 64, 128 or 256 (up to 16 query heads a kv head)
-        read the codes as they are, on the tensor cores; float32, single tokens of other sizes, and rows that do not begin at 16
-        bytes, on the FMA pipes (csrc/attention_8bit.cu).  bfloat16 portions of prompts have their sequences' pages unpacked once (exactly; at
-        most ``UNPACK_BYTES`` at a time, or one sequence) and go through the kernels for wide pages; so do the single tokens beside them,
-        but for heads of 64 and 128, whose codes are read as they are there too.  A table entry that is no page is read nowhere; the rows
-        of a sequence that sees such a token are undefined, the others are not."""
+        read the codes as they are, on the tensor cores; float32, other single tokens of up to 8 query heads a kv head, and rows that do not
+        begin at 16 bytes, on the FMA pipes (csrc/attention_8bit.cu).  bfloat16 portions of prompts read the codes as well, turned to
+        bfloat16 on the way (csrc/prompts_8bit.cu); longer ones of heads of 64 to 128 have their sequences' pages unpacked once (at most
+        ``UNPACK_BYTES`` at a time, or one sequence) and go through the tcgen05 kernel.  Both are exact up to the weights, which are rounded to
+        bfloat16.  A table entry that is no page is read nowhere; the rows of a sequence that sees such a token are undefined, the others
+        are not."""
         what = "paged_attention_8bit"
         D, G, H, dtype, shape, rows = head_dim, num_kv_heads, num_heads, out.dtype, q.shape, out.shape
         _, (table_rows, max_pages) = self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens, record_of=_eight_bit_record)
@@ -2688,34 +2680,117 @@ class CudaOps:
             return self._decode_8bit(q_at, q_stride, H, G, D, pages, block_table, step, None, seqs, max_len,
                                      decode_slices or self.decode_slices_8bit(step.host_kv_lens, G, D, window, H // G, keep_first), out, out_at,
                                      page_size, scale, window, keep_first, longest)
-        aligned = not (q_at & 15 or out_at & 15)  # what the kernels for wide pages go by
-        if dtype == torch.float32 or (step.decode_only and not fast) or not aligned:
+        # (single tokens of up to 8 query heads a kv head that the decode kernel does not take: eight behind 4,096, 20 heads over 4 of 80, take the
+        # general form 30 us and the one for prompts, whose blocks have 128 rows, 41; 40 over 2 of 128 51 and 39)
+        if _dtype_code(dtype) == 0 or q_stride & 7 or q_at & 15 or out_at & 3 or (step.decode_only and not fast and H // G <= 8):
             return self._general_8bit(q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window, keep_first)
-        # portions of prompts (and single tokens beside them): their sequences' pages unpacked, the kernels for wide pages
-        split = fast and D != 256  # prompts apart from single tokens, which are decoded as they are
+        cu = step.host_cu_seqlens
+        if len(cu) <= seqs:
+            raise KernelError(f"{what}: host_cu_seqlens are the sequences' first tokens and the number of all")
+        if not fast:
+            return self._prompts_8bit(q_at, q_stride, H, G, D, pages, block_table, step, 1, max_len, out, page_size, scale, window, keep_first)
+        # portions of prompts, and single tokens beside them, which are decoded as they are
         singles = step.single_seqs
         if (singles is None and step.num_single) or (singles is not None and (
                 singles.dtype != torch.int32 or singles.numel() < step.num_single or not singles.is_contiguous())):
             raise KernelError(f"{what}: single_seqs is dense int32, one per sequence that brings one token")
         self._check_here(what, singles)
-        cu = step.host_cu_seqlens
-        exact = not step.captured_width and len(step.host_kv_lens) >= step.num_seqs  # (else the lengths are those of the moment, up to max_len)
-        lens = list(step.host_kv_lens[:step.num_seqs]) if exact else [max_len] * step.num_seqs
-        if split and step.num_single:
+        exact = not step.captured_width and len(step.host_kv_lens) >= seqs  # (else the lengths are those of the moment, up to max_len)
+        lens = list(step.host_kv_lens[:seqs]) if exact else [max_len] * seqs
+        if step.num_single:
             own = [kv for b, kv in enumerate(lens) if cu[b + 1] - cu[b] == 1]
             self._decode_8bit(q_at, q_stride, H, G, D, pages, block_table, step, singles, step.num_single, max(own),
                               self.decode_slices_8bit(own, G, D, window, H // G, keep_first), out, out_at, page_size, scale, window, keep_first,
                               None)
-        counts = unpacked_pages_4bit(cu, lens, page_size, window, 2 if split else 1, exact, keep_first)
-        total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * page_size * D)
+        if not (64 <= D <= 128 and out_at & 15 == 0 and self._prompts_unpacked(cu, lens, H // G, G, D, window, keep_first)):
+            return self._prompts_8bit(q_at, q_stride, H, G, D, pages, block_table, step, 2, max_len, out, page_size, scale, window, keep_first)
+        wide = page_size if page_size in (8, 16, 32, 64) else 16  # tokens of a page that is unpacked
+        counts = unpacked_pages_4bit(cu, lens, wide, window, 2, exact, keep_first)
+        total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * wide * D)
         if total <= limit:
             runs = [(0, len(counts), total)] if total else []
         else:
             runs = [(first, end, sum(counts[first:end])) for first, end in runs_within(counts, limit)]
         for first, end, count in runs:
             most = max([n for n, c in zip(lens[first:end], counts[first:end]) if c])
-            self._prompts_4bit(q, q_stride, H, G, D, pages, block_table, step, first, end, count, most, split, out, page_size, scale, window,
-                               keep_first)
+            self._prompts_tc_8bit(q, q_stride, H, G, D, pages, block_table, step, first, end, count, most, out, page_size, wide, scale, window,
+                                  keep_first)
+        return out
+
+    def _prompts_unpacked(self, cu, lens, R, G, D, window, keep_first) -> bool:
+        """Whether a step's portions are faster unpacked and on the tcgen05 kernel than straight over the codes.  Times in us, fitted to both at 150
+        random steps (one to eight portions of 2 to 1,000 tokens behind up to 8,000, 1 to 8 kv heads of 64, 96 and 128, groups of 2 to 16, windows) on a
+        B200: the choice is 1.5 % slower than the better one on average, 33 % at worst.  Straight, a block of 128 rows takes a tile of 64 keys of
+        128 channels in 4.1 of an SM, in 2.6 if it is by itself, and slices cost their joining; unpacked, the longest sequence's tiles take 0.66 each, one
+        after the other (a machine full of blocks hardly more at these sizes), and unpacking the bytes it moves."""
+        work = chain = read = items = most = 0
+        for b, kv in enumerate(lens):
+            n = cu[b + 1] - cu[b]
+            if n < 2:
+                continue
+            rows, most = -(-n * R // 128), max(most, n)
+            seen = min(kv, window + n + keep_first) if window else kv  # keys that any of its tokens sees
+            work += rows * ((min(seen, window + keep_first) if window else kv - n / 2) / 64 + 1)  # tiles of its blocks
+            chain = max(chain, (min(seen, window + 256 // R + keep_first) if window else kv) / 64 + 1)
+            read += seen
+            items += rows
+        if not items:
+            return False
+        splits = self._prompt_splits(items * G, D, window, keep_first, most, max(lens))
+        size = max(D, 64) / 128
+        straight = 5.7 + max(4.1 * work * G * size / self.SM_COUNT, 2.6 * chain * size / splits) + (5 + 0.67 * splits if splits > 1 else 0)
+        return 10.6 + 3.7e-6 * read * G * D + max(0.66 * chain, 0.08 * work * G / self.SM_COUNT) < straight
+
+    def _prompt_splits(self, blocks, D, window, keep_first, most_new, max_len) -> int:
+        """Slices of the tiles of ``blocks`` blocks of rows: as many blocks as run at a time, each at least four tiles of 64 keys."""
+        tiles = -(-(min(max_len, window + most_new + keep_first) if window else max_len) // 64)
+        return max(1, min(self.SM_COUNT * (2 if D <= 64 else 1) // blocks, tiles // 4, 32))
+
+    def _prompts_tc_8bit(self, q, q_stride, H, G, D, pages, block_table, step, first, end, count, longest, out, page_size, wide, scale, window,
+                         keep_first):
+        """Attention of the portions of the step's sequences ``first .. end - 1``, whose ``count`` pages of ``wide`` tokens are unpacked for it (none of
+        those has more than ``longest`` keys)."""
+        cu, kv_lens, seqs = step.cu_seqlens, step.kv_lens, end - first
+        news = [b - a for a, b in zip(step.host_cu_seqlens[first:end], step.host_cu_seqlens[first + 1:end + 1])]
+        if seqs != step.num_seqs:  # these sequences alone
+            cu, kv_lens, block_table = cu[first:end + 1], kv_lens[first:end], block_table[first:end]
+        k = torch.empty((2, count, G, wide, D), dtype=out.dtype, device=out.device)
+        v_at = k.data_ptr() + k.numel()  # (half of its bytes)
+        width = -(-longest // wide)
+        table = torch.empty((seqs, width), dtype=torch.int32, device=out.device)
+        if self.timing is not None:
+            self._costs(k.numel() * k.element_size() + count * wide * 2 * G * D)
+        self._call("cache_8bit", "q3_unpack_8bit", "unpack_8bit", _dtype_code(out.dtype), pages.data_ptr(), pages.size(0), G, D, page_size,
+                   block_table.data_ptr(), block_table.size(1), kv_lens.data_ptr(), seqs, longest, cu.data_ptr(), 2, window, keep_first, count,
+                   width, wide, k.data_ptr(), v_at, table.data_ptr())
+        per = 128 // (H // G)  # tokens of a block of rows
+        pairs = sum([-(-(-(-n // per)) // 2) for n in news if n > 1])  # two blocks an item
+        if self.timing is not None:
+            self._costs(*self._attention_cost(step, H, G, D, out, prompts=True))
+        self._call("attention_prefill_tc", "q3_window_attention_prefill_tc", "paged_attention_prefill_8bit", q.data_ptr(), q_stride, q.size(0),
+                   k.data_ptr(), v_at, count * G * wide, table.data_ptr(), width, kv_lens.data_ptr(), cu.data_ptr(), out.data_ptr(), seqs, pairs,
+                   H, G, D, wide, float(scale), 1, window, keep_first, self._error_word(out.device).data_ptr())
+
+    def _prompts_8bit(self, q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first):
+        """Attention of the sequences that bring at least ``least`` tokens, straight over the codes (csrc/prompts_8bit.cu)."""
+        T, R, cu = step.num_tokens, H // G, step.host_cu_seqlens
+        news = [n for n in [b - a for a, b in zip(cu, cu[1:step.num_seqs + 1])] if n >= least]
+        items = sum([-(-n * R // 128) for n in news])
+        if not items:
+            return out
+        splits = self._prompt_splits(items * G, D, window, keep_first, max(news), max_len)
+        splits = max(1, min(splits, (1 << 26) // (T * H * D)))  # (no more to keep of the slices than 256 MB)
+        mid_o = mid_ml = None
+        if splits > 1:
+            mid = torch.empty(T * H * splits * (D + 2), dtype=torch.float32, device=out.device)
+            mid_o = mid.data_ptr()
+            mid_ml = mid_o + 4 * T * H * splits * D
+            self.launches += 1
+        if self.timing is not None:
+            self._costs(*self._attention_cost(step, H, G, D, out, prompts=None if least < 2 else True))
+        self._call("prompts_8bit", "q3_prompts_attention_8bit", "paged_attention_prompts_8bit", q_at, q_stride, pages.data_ptr(), pages.size(0),
+                   block_table.data_ptr(), block_table.size(1), step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(), out.data_ptr(), mid_o, mid_ml,
+                   splits, items, least, T, step.num_seqs, H, G, D, page_size, float(scale), window, keep_first, max_len)
         return out
 
     def _general_8bit(self, q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window, keep_first):

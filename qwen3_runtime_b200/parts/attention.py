@@ -88,6 +88,8 @@ class PagedAttention(Part):
         groups = ["rope_kv", "attention_generic", *product_groups(self.ctx), *self.position.kernel_groups()]
         if self.bits:
             groups += [f"cache_{self.bits}bit", f"attention_{self.bits}bit"]
+        if self.bits == 8 and self.ctx.dtype == torch.bfloat16:  # (what the specialised kernels over wide pages are for a cache in 16 bits)
+            return [*groups, "prompts_8bit", *(["attention_prefill_tc"] if 64 <= self.head_dim <= 128 else [])]
         if self.ctx.dtype == torch.bfloat16:
             # the specialised attention kernels that this head size can reach (ops.paged_attention)
             group = self.num_heads // self.num_kv_heads
@@ -95,7 +97,7 @@ class PagedAttention(Part):
                 groups.append("attention_decode")
             if self.head_dim in (64, 128) and group <= 16:
                 groups.append("attention_prefill")
-            if self.head_dim == 128 and (not self.window or self.bits == 8) and 128 % group == 0:
+            if self.head_dim == 128 and not self.window and 128 % group == 0:
                 groups.append("attention_prefill_tc")
         return groups
 

@@ -169,8 +169,11 @@ class Here(Table):
         self.calls.append("paged_attention")
 
 
-def call(new=(1, 1), kw={}, **change):
+def call(new=(1, 1), kw={}, unpacked=None, **change):
+    """The launches of an attention call; ``unpacked``: how portions are decided on (None: by their cost)."""
     ops, args = Here(), attention_args(new=new, **kw)
+    if unpacked is not None:
+        ops._prompts_unpacked = lambda *sizes: unpacked
     for name, value in change.items():
         setattr(args["step"], name, value)
     ops.paged_attention_8bit(args.pop("q"), args.pop("q_stride"), **args)
@@ -199,14 +202,29 @@ def test_tensors_on_another_device_are_refused():
 
 def test_which_kernels_attention_takes():
     f32, wide = dict(dtype=torch.float32), dict(H=34, G=2)
-    assert call() == call(kv_longest=None, single_seqs=None) == ["q3_decode_attention_8bit"]
-    assert call(kw=f32) == call((2, 3), f32) == call(kw=dict(D=80)) == call(kw=wide) == ["q3_general_attention_8bit"]
-    assert call((2, 3)) == call((2, 3), wide) == call((2, 1), wide) == ["q3_unpack_8bit", "paged_attention"]
-    assert call((2, 1)) == ["q3_decode_attention_8bit", "q3_unpack_8bit", "paged_attention"]
-    assert call((2, 1), dict(window=4, keep_first=1)) == ["q3_decode_attention_8bit", "q3_unpack_8bit", "q3_window_attention_prefill_tc"]
-    assert call((2, 1), dict(window=4, page=20, keep_first=1)) == ["q3_decode_attention_8bit", "q3_unpack_8bit", "paged_attention"]
-    assert call((2, 1), dict(window=4, D=64)) == ["q3_decode_attention_8bit", "q3_unpack_8bit", "paged_attention"]
-    assert call((2, 1), dict(D=256)) == ["q3_unpack_8bit", "paged_attention"]
+    decode, straight, general = "q3_decode_attention_8bit", "q3_prompts_attention_8bit", "q3_general_attention_8bit"
+    unpacked = ["q3_unpack_8bit", "q3_window_attention_prefill_tc"]
+    assert call() == call(kv_longest=None, single_seqs=None) == [decode]
+    assert call(kw=f32) == call((2, 3), f32) == [general]
+    assert call(kw=dict(D=80)) == call(kw=dict(D=80, H=16)) == [general] and call(kw=dict(D=80, H=18)) == [straight]
+    assert call(kw=wide) == call((2, 3), wide) == call((2, 1), wide) == call((2, 1), dict(D=80)) == [straight]
+    odd = dict(H=1, G=1, q=torch.zeros((3, 132), dtype=torch.bfloat16), q_stride=132)  # rows that do not begin at 16 bytes
+    assert call((2, 1), odd) == [general]
+    for kw in (dict(), dict(window=4, keep_first=1), dict(D=64), dict(page=20), dict(H=10)):
+        assert call((2, 1), kw, True) == [decode, *unpacked] and call((2, 3), kw, True) == unpacked
+        assert call((2, 1), kw, False) == [decode, straight] and call((2, 3), kw, False) == call((2, 3), kw) == [straight]
+    assert call((2, 1), dict(D=256), True) == [decode, straight] and call((2, 1), dict(D=80), True) == call((2, 1), dict(D=48), True) == [straight]
+
+
+def test_which_portions_are_unpacked():
+    """Long ones; few rows behind a long context are not, nor prompts of a few tokens."""
+    ops = Here()
+    ops.SM_COUNT = 148
+    cases = lambda news, kvs, D=128, window=0, first=0, group=4: ops._prompts_unpacked(  # noqa: E731
+        [sum(news[:b]) for b in range(len(news) + 1)], kvs, group, 8, D, window, first)
+    assert cases([2048], [2048]) and cases([512, 1, 700], [512, 9000, 900]) and cases([2048], [2048], 64) and cases([256], [4256])
+    assert not cases([16], [16]) and not cases([64], [16064]) and not cases([2, 1, 3], [1000, 5, 1003]) and not cases([1, 1], [9, 9])
+    assert cases([2048], [9000], window=1024, first=4) and not cases([16], [30000])
 
 
 def test_unpacking_more_than_the_table_holds_is_refused(ops):
