@@ -233,11 +233,11 @@ __global__ void __launch_bounds__(STORE_THREADS, SINGLE ? 2 : 3) store_8bit_vec_
 }
 
 // Any other size, rotation or alignment: a warp per (token, head) of the queries, a block per (unit, head) of the write, its rows a warp each.
-template <typename T, int WARPS>
-__global__ void store_8bit_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, int nq, int nkv, int D, Store a) {
-  extern __shared__ float stage[];  // WARPS * 2 * D
+template <typename T>
+__global__ void __launch_bounds__(STORE_THREADS) store_8bit_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, int nq, int nkv, int D, Store a) {
+  extern __shared__ float stage[];  // warps * 2 * D
   __shared__ uint32_t red[32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   float *xs = stage + warp * 2 * D, *ys = xs + D;
   // ys gets the head that x names; false: its position lies outside the tables
   auto make = [&](const T* x, const float* w, int p, bool turn) {
@@ -272,7 +272,7 @@ __global__ void store_8bit_kernel(const T* qkv, int row_stride, T* q_out, int q_
   };
   const int write_blocks = a.units * 2 * nkv;
   if ((int)blockIdx.x >= write_blocks) {
-    const long item = (long)(blockIdx.x - write_blocks) * WARPS + warp;
+    const long item = (long)(blockIdx.x - write_blocks) * warps + warp;
     if (item >= (long)a.num_tokens * nq) return;
     const int t = (int)(item / nq), hi = (int)(item - (long)t * nq);
     if (!make(qkv + (long)t * row_stride + (long)hi * D, a.q_w, a.positions[t], true)) return;
@@ -291,13 +291,13 @@ __global__ void store_8bit_kernel(const T* qkv, int row_stride, T* q_out, int q_
            make(qkv + (long)t * row_stride + (long)(nq + hd) * D, is_v ? nullptr : a.k_w, a.positions[t], !is_v);
   };
   uint32_t most = 0;
-  for (int row = unit.r0 + warp; row < unit.r1; row += WARPS)
+  for (int row = unit.r0 + warp; row < unit.r1; row += warps)
     if (make_row(row))
       for (int d = lane; d < D; d += 32) most = max(most, q8_finite(q8_rounded(ys[d])));
   const int e = settle_scale(most, unit.r0, D, codes, reinterpret_cast<float*>(unit.rec + L.scales) + is_v, red);
   const float down = q8_power(-e);
   const int mask = q8_mask(D);
-  for (int row = unit.r0 + warp; row < unit.r1; row += WARPS)
+  for (int row = unit.r0 + warp; row < unit.r1; row += warps)
     if (make_row(row))
       for (int d = 4 * lane; d < D; d += 128) *reinterpret_cast<uint32_t*>(codes + (long)row * D + q8_at(d, row, mask)) = q8_word(ys + d, down);
 }
@@ -554,16 +554,16 @@ Q3_EXPORT int q3_store_8bit(int dtype, const void* qkv, int row_stride, void* q_
       launch_size(std::false_type());
     return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
   }
-  constexpr int WARPS = 4;
-  const long blocks = (long)units * 2 * nkv + ((long)num_tokens * nq + WARPS - 1) / WARPS;
+  // (a page's rows are its warps', one after the other: 475 tokens of 20 + 4 heads of 80 in pages of 64, with their unpacking 49 us with 4 warps, 20 with 16; single
+  // tokens leave all but one idle)
+  const int warps = units > 0 && rows > 4 ? STORE_THREADS / 32 : 4;
+  const long blocks = (long)units * 2 * nkv + ((long)num_tokens * nq + warps - 1) / warps;
   if (blocks > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
-  const size_t smem = (size_t)WARPS * 2 * D * sizeof(float);
+  const size_t smem = (size_t)warps * 2 * D * sizeof(float);
   if (dtype == Q3_DTYPE_F32)
-    store_8bit_kernel<float, WARPS><<<(unsigned)blocks, WARPS * 32, smem, stream>>>((const float*)qkv, row_stride, (float*)q_out, q_stride, nq,
-                                                                                  nkv, D, a);
+    store_8bit_kernel<float><<<(unsigned)blocks, warps * 32, smem, stream>>>((const float*)qkv, row_stride, (float*)q_out, q_stride, nq, nkv, D, a);
   else
-    store_8bit_kernel<bf16, WARPS><<<(unsigned)blocks, WARPS * 32, smem, stream>>>((const bf16*)qkv, row_stride, (bf16*)q_out, q_stride, nq, nkv,
-                                                                                 D, a);
+    store_8bit_kernel<bf16><<<(unsigned)blocks, warps * 32, smem, stream>>>((const bf16*)qkv, row_stride, (bf16*)q_out, q_stride, nq, nkv, D, a);
   return q3_launch_status();
 }
 
