@@ -2648,7 +2648,8 @@ class CudaOps:
         bfloat16 on the way (csrc/prompts_8bit.cu); longer ones of heads of 64 to 128 have their sequences' pages unpacked once (at most
         ``UNPACK_BYTES`` at a time, or one sequence) and go through the tcgen05 kernel.  Both are exact up to the weights, which are rounded to
         bfloat16.  A table entry that is no page is read nowhere; the rows of a sequence that sees such a token are undefined, the others
-        are not."""
+        are not.  A key that is no number makes the rows none that see it; a value, its channel of them, and of its portion's other rows too (their weight
+        for it is zero)."""
         what = "paged_attention_8bit"
         D, G, H, dtype, shape, rows = head_dim, num_kv_heads, num_heads, out.dtype, q.shape, out.shape
         _, (table_rows, max_pages) = self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens, record_of=_eight_bit_record)
@@ -2687,25 +2688,23 @@ class CudaOps:
         cu = step.host_cu_seqlens
         if len(cu) <= seqs:
             raise KernelError(f"{what}: host_cu_seqlens are the sequences' first tokens and the number of all")
-        if not fast:
-            return self._prompts_8bit(q_at, q_stride, H, G, D, pages, block_table, step, 1, max_len, out, page_size, scale, window, keep_first)
-        # portions of prompts, and single tokens beside them, which are decoded as they are
-        singles = step.single_seqs
-        if (singles is None and step.num_single) or (singles is not None and (
-                singles.dtype != torch.int32 or singles.numel() < step.num_single or not singles.is_contiguous())):
+        singles, least = step.single_seqs, 2 if fast else 1  # (portions of prompts; single tokens beside them are decoded as they are, if they can be)
+        if fast and ((singles is None and step.num_single) or (singles is not None and (
+                singles.dtype != torch.int32 or singles.numel() < step.num_single or not singles.is_contiguous()))):
             raise KernelError(f"{what}: single_seqs is dense int32, one per sequence that brings one token")
         self._check_here(what, singles)
         exact = not step.captured_width and len(step.host_kv_lens) >= seqs  # (else the lengths are those of the moment, up to max_len)
         lens = list(step.host_kv_lens[:seqs]) if exact else [max_len] * seqs
-        if step.num_single:
+        if fast and step.num_single:
             own = [kv for b, kv in enumerate(lens) if cu[b + 1] - cu[b] == 1]
             self._decode_8bit(q_at, q_stride, H, G, D, pages, block_table, step, singles, step.num_single, max(own),
                               self.decode_slices_8bit(own, G, D, window, H // G, keep_first), out, out_at, page_size, scale, window, keep_first,
                               None)
-        if not (64 <= D <= 128 and out_at & 15 == 0 and self._prompts_unpacked(cu, lens, H // G, G, D, window, keep_first)):
-            return self._prompts_8bit(q_at, q_stride, H, G, D, pages, block_table, step, 2, max_len, out, page_size, scale, window, keep_first)
+        if not (64 <= D <= 128 and H // G <= 128 and out_at & 15 == 0 and not step.decode_only
+                and self._prompts_unpacked(cu, lens, H // G, G, D, window, keep_first, least)):
+            return self._prompts_8bit(q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first)
         wide = page_size if page_size in (8, 16, 32, 64) else 16  # tokens of a page that is unpacked
-        counts = unpacked_pages_4bit(cu, lens, wide, window, 2, exact, keep_first)
+        counts = unpacked_pages_4bit(cu, lens, wide, window, least, exact, keep_first)
         total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * wide * D)
         if total <= limit:
             runs = [(0, len(counts), total)] if total else []
@@ -2713,11 +2712,11 @@ class CudaOps:
             runs = [(first, end, sum(counts[first:end])) for first, end in runs_within(counts, limit)]
         for first, end, count in runs:
             most = max([n for n, c in zip(lens[first:end], counts[first:end]) if c])
-            self._prompts_tc_8bit(q, q_stride, H, G, D, pages, block_table, step, first, end, count, most, out, page_size, wide, scale, window,
-                                  keep_first)
+            self._prompts_tc_8bit(q, q_stride, H, G, D, pages, block_table, step, least, first, end, count, most, out, page_size, wide, scale,
+                                  window, keep_first)
         return out
 
-    def _prompts_unpacked(self, cu, lens, R, G, D, window, keep_first) -> bool:
+    def _prompts_unpacked(self, cu, lens, R, G, D, window, keep_first, least=2) -> bool:
         """Whether a step's portions are faster unpacked and on the tcgen05 kernel than straight over the codes.  Times in us, fitted to both at 150
         random steps (one to eight portions of 2 to 1,000 tokens behind up to 8,000, 1 to 8 kv heads of 64, 96 and 128, groups of 2 to 16, windows) on a
         B200: the choice is 1.5 % slower than the better one on average, 33 % at worst.  Straight, a block of 128 rows takes a tile of 64 keys of
@@ -2726,7 +2725,7 @@ class CudaOps:
         work = chain = read = items = most = 0
         for b, kv in enumerate(lens):
             n = cu[b + 1] - cu[b]
-            if n < 2:
+            if n < least:
                 continue
             rows, most = -(-n * R // 128), max(most, n)
             seen = min(kv, window + n + keep_first) if window else kv  # keys that any of its tokens sees
@@ -2746,10 +2745,10 @@ class CudaOps:
         tiles = -(-(min(max_len, window + most_new + keep_first) if window else max_len) // 64)
         return max(1, min(self.SM_COUNT * (2 if D <= 64 else 1) // blocks, tiles // 4, 32))
 
-    def _prompts_tc_8bit(self, q, q_stride, H, G, D, pages, block_table, step, first, end, count, longest, out, page_size, wide, scale, window,
-                         keep_first):
-        """Attention of the portions of the step's sequences ``first .. end - 1``, whose ``count`` pages of ``wide`` tokens are unpacked for it (none of
-        those has more than ``longest`` keys)."""
+    def _prompts_tc_8bit(self, q, q_stride, H, G, D, pages, block_table, step, least, first, end, count, longest, out, page_size, wide, scale,
+                         window, keep_first):
+        """Attention of those of the step's sequences ``first .. end - 1`` that bring at least ``least`` tokens, whose ``count`` pages of ``wide`` tokens
+        are unpacked for it (none of those has more than ``longest`` keys)."""
         cu, kv_lens, seqs = step.cu_seqlens, step.kv_lens, end - first
         news = [b - a for a, b in zip(step.host_cu_seqlens[first:end], step.host_cu_seqlens[first + 1:end + 1])]
         if seqs != step.num_seqs:  # these sequences alone
@@ -2761,15 +2760,15 @@ class CudaOps:
         if self.timing is not None:
             self._costs(k.numel() * k.element_size() + count * wide * 2 * G * D)
         self._call("cache_8bit", "q3_unpack_8bit", "unpack_8bit", _dtype_code(out.dtype), pages.data_ptr(), pages.size(0), G, D, page_size,
-                   block_table.data_ptr(), block_table.size(1), kv_lens.data_ptr(), seqs, longest, cu.data_ptr(), 2, window, keep_first, count,
+                   block_table.data_ptr(), block_table.size(1), kv_lens.data_ptr(), seqs, longest, cu.data_ptr(), least, window, keep_first, count,
                    width, wide, k.data_ptr(), v_at, table.data_ptr())
         per = 128 // (H // G)  # tokens of a block of rows
-        pairs = sum([-(-(-(-n // per)) // 2) for n in news if n > 1])  # two blocks an item
+        pairs = sum([-(-(-(-n // per)) // 2) for n in news if n >= least])  # two blocks an item
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out, prompts=True))
         self._call("attention_prefill_tc", "q3_window_attention_prefill_tc", "paged_attention_prefill_8bit", q.data_ptr(), q_stride, q.size(0),
                    k.data_ptr(), v_at, count * G * wide, table.data_ptr(), width, kv_lens.data_ptr(), cu.data_ptr(), out.data_ptr(), seqs, pairs,
-                   H, G, D, wide, float(scale), 1, window, keep_first, self._error_word(out.device).data_ptr())
+                   H, G, D, wide, float(scale), least - 1, window, keep_first, self._error_word(out.device).data_ptr())
 
     def _prompts_8bit(self, q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first):
         """Attention of the sequences that bring at least ``least`` tokens, straight over the codes (csrc/prompts_8bit.cu)."""

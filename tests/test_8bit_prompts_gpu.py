@@ -1,0 +1,139 @@
+"""Attention of prompts over a cache in 8 bits, straight over the codes and over unpacked pages, each where the other would be chosen too; and single
+tokens that take the way of prompts.  The bounds are those of tests/test_8bit_gpu.py."""
+
+import math
+
+import pytest
+import torch
+
+import plain_8bit as p8
+from test_8bit_gpu import BF16, attend, check_rows, i32, ops, queries, sizes  # noqa: F401 (ops: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=[True, False], ids=["unpacked", "straight"])
+def form(request, ops, monkeypatch):  # noqa: F811
+    """Whichever form the rule on times would choose; ``used`` collects the entry points that ran."""
+    used, call = [], ops._call
+    monkeypatch.setattr(ops, "_prompts_unpacked", lambda *sizes: request.param, raising=False)
+    monkeypatch.setattr(ops, "_call", lambda group, name, *args: (used.append(name), call(group, name, *args))[1], raising=False)
+    return request.param, used
+
+
+def check_form(form, D):
+    unpacked, used = form
+    names = set(used) - {"q3_decode_attention_8bit"}
+    assert names == ({"q3_unpack_8bit", "q3_window_attention_prefill_tc"} if unpacked and 64 <= D <= 128 else {"q3_prompts_attention_8bit"})
+
+
+@pytest.mark.parametrize("window,keep_first", [(None, 0), (1, 0), (40, 6), (70, 200)])
+@pytest.mark.parametrize("H,G,D,page", [(8, 8, 64, 5), (6, 2, 64, 8), (5, 1, 80, 16), (20, 4, 80, 24), (10, 1, 96, 32), (14, 2, 112, 1), (40, 2, 128, 16),
+                                        (8, 2, 128, 100), (12, 4, 128, 64), (128, 1, 64, 16), (16, 2, 256, 7), (6, 1, 32, 3), (3, 3, 208, 16)])
+def test_portions(ops, form, H, G, D, page, window, keep_first):  # noqa: F811
+    """Portions with and without tokens before them, that end inside a tile, a page and a block of rows; single tokens between them."""
+    new, lens = [33, 1, 70, 2, 1, 5], [33, 90, 210, 64, 1, 130]
+    c = p8.Cache(lens, G, D, page, seed=D + G)
+    q = queries(sum(new), H, D, H)
+    got = attend(ops, c, q, new, lens, H, D ** -0.5, window=window, keep_first=keep_first)
+    check_rows(got, q.view(-1, H, D), c, new, lens, D ** -0.5, window=window, keep_first=keep_first, wide=True)
+    check_form(form, D)
+
+
+@pytest.mark.parametrize("H,G,D", [(20, 4, 80), (40, 2, 128), (8, 2, 128), (2, 1, 256)])
+def test_a_long_prompt_of_many_slices(ops, form, H, G, D):  # noqa: F811
+    """One portion behind thousands of tokens: slices whose joining has many parts."""
+    new, lens = [37], [4021]
+    c = p8.Cache(lens, G, D, 16, seed=3)
+    q = queries(37, H, D, 2)
+    got = attend(ops, c, q, new, lens, H, D ** -0.5)
+    check_rows(got, q.view(-1, H, D), c, new, lens, D ** -0.5, wide=True)
+    check_form(form, D)
+
+
+@pytest.mark.parametrize("H,G,D", [(10, 2, 80), (40, 2, 128)])
+def test_turns_of_sequences(ops, form, H, G, D):  # noqa: F811
+    """More sequences than are unpacked at a time, single tokens among them: the same results."""
+    new, lens, page = [9, 1, 30, 2, 17], [100, 70, 30, 64, 90], 24
+    c = p8.Cache(lens, G, D, page, seed=9)
+    q = queries(sum(new), H, D, 4)
+    whole = attend(ops, c, q, new, lens, H, D ** -0.5)
+    check_rows(whole, q.view(-1, H, D), c, new, lens, D ** -0.5, wide=True)
+    ops.UNPACK_BYTES = 8 * 4 * G * 16 * D
+    try:
+        assert torch.equal(attend(ops, c, q, new, lens, H, D ** -0.5), whole)
+    finally:
+        del ops.UNPACK_BYTES
+
+
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_what_is_not_finite_stays_with_its_sequence_and_head(ops, form, D):  # noqa: F811
+    """A key or value that is no number: tokens that see it are none; other heads and sequences are untouched, and so are, by a key, the
+    tokens before it and, by a value, other channels."""
+    def mutate(b, k, v):
+        if b == 1:
+            k[0, 30, 3] = math.nan
+            v[1, 31, D - 2] = math.inf
+
+    H, G, new, lens = 6, 3, [20, 20, 20], [40, 40, 40]
+    c = p8.Cache(lens, G, D, 16, seed=1, mutate=mutate)
+    q = queries(60, H, D, 5)
+    got = attend(ops, c, q, new, lens, H, D ** -0.5)
+    assert bool(got[:20].isfinite().all()) and bool(got[40:].isfinite().all()) and bool(got[:, 4:].isfinite().all())
+    assert bool(got[30:40, :2].isnan().all()) and bool(got[20:30, :2].isfinite().all()), "a key: tokens that see it, and no others"
+    assert bool(got[31:40, 2:4, D - 2].isnan().all())
+    got[20:40, 2:4, D - 2] = 0
+    assert bool(got[20:40, 2:4].isfinite().all()), "a value: its channel"
+
+
+@pytest.mark.parametrize("H,G,D,page", [(10, 1, 80, 16), (20, 2, 96, 5), (40, 2, 128, 16), (20, 4, 80, 16)])
+def test_captured_single_tokens(ops, H, G, D, page):  # noqa: F811
+    """Steps of single tokens that the decode kernel does not take, captured, replayed with lengths that grow."""
+    width, lens = 400 // page, [3, 150, 17]
+    c = p8.Cache([400] * 3, G, D, page, seed=7, width=width)
+    pages, table = c.pages.cuda(), c.table.cuda()
+    q = torch.zeros((3, H * D), dtype=BF16, device="cuda")
+    out = torch.zeros_like(q)
+    step = p8.step_of([1] * 3, lens, page, captured_width=width)
+
+    def run(to, by):
+        ops.paged_attention_8bit(q, H * D, num_heads=H, pages=pages, block_table=table, out=to, scale=D ** -0.5, step=by, **sizes(c))
+
+    run(out, step)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(out, step)
+    for turn in range(1, 200, 33):
+        now = [n + turn for n in lens]
+        rows = queries(3, H, D, turn)
+        q.copy_(rows)
+        step.kv_lens.copy_(i32(now))
+        step.positions.copy_(i32([n - 1 for n in now]))
+        graph.replay()
+        torch.cuda.synchronize()
+        sub = p8.Cache([], G, D, page)
+        sub.kv = [x[:, :, :n] for x, n in zip(c.kv, now)]
+        sub.scales = [s[:, :, : -(-n // page)] for s, n in zip(c.scales, now)]
+        check_rows(out.cpu().view(3, H, D), rows.view(-1, H, D), sub, [1] * 3, now, D ** -0.5, wide=True)
+
+
+def test_portions_on_another_stream(ops, form):  # noqa: F811
+    """Two steps of portions under way together: each with pages and slices of its own."""
+    H, G, D = 10, 2, 128
+    made = []
+    for i, (new, lens) in enumerate((([40, 3], [900, 300]), ([7, 90, 1], [40, 700, 60]))):
+        c = p8.Cache(lens, G, D, 16, seed=i)
+        q = queries(sum(new), H, D, i)
+        made.append((c, q.cuda(), c.pages.cuda(), c.table.cuda(), p8.step_of(new, lens, 16), torch.cuda.Stream(), attend(ops, c, q, new, lens, H, D ** -0.5)))
+    outs = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, (c, q, pages, table, step, stream, _want) in enumerate(made):
+            with torch.cuda.stream(stream):
+                out = torch.empty_like(q)
+                ops.paged_attention_8bit(q, H * D, num_heads=H, pages=pages, block_table=table, out=out, scale=D ** -0.5, step=step, **sizes(c))
+                outs[i].append(out)
+    torch.cuda.synchronize()
+    for got, (*_, want) in zip(outs, made):
+        assert all(torch.equal(x.cpu().view(want.shape), want) for x in got)
