@@ -2611,15 +2611,15 @@ class CudaOps:
             if step.num_tokens != step.num_seqs:
                 raise KernelError(f"{what}: a step of single tokens has as many tokens as sequences")
             return step.num_seqs, 1
-        found = step.extras.get(("written_pages", page_size))
-        if found is None:
-            cu = step.host_cu_seqlens
+        cu = step.host_cu_seqlens
+        found = step.extras.get(("written_pages", page_size))  # (every layer asks)
+        if found is None or found[0] != cu:
             if len(cu) <= step.num_seqs or cu[0] != 0 or cu[step.num_seqs] != step.num_tokens:
                 raise KernelError(f"{what}: host_cu_seqlens are the sequences' first tokens and the number of all")
             news = [cu[b + 1] - cu[b] for b in range(step.num_seqs)]
             units = sum((n + page_size - 2) // page_size + 1 for n in news if n > 0)
-            found = step.extras[("written_pages", page_size)] = (units, max([1, *news]))
-        return found
+            found = step.extras[("written_pages", page_size)] = (cu[:], (units, max([1, *news])))
+        return found[1]
 
     def unpack_8bit(self, pages, *, num_kv_heads, head_dim, page_size, block_table, kv_lens, max_kv_len, dtype):
         """Keys and values of the sequences' first ``max_kv_len`` tokens as wide pages ``[sequences * n, kv heads, page_size, head_dim]``

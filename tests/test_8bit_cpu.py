@@ -131,6 +131,18 @@ def test_pages_that_a_step_writes():
         assert step.decode_only or CudaOps._written_pages("x", step, page) is CudaOps._written_pages("x", step, page)
 
 
+def test_a_step_that_is_filled_anew_is_counted_anew():
+    step = p8.step_of([3, 1], [3, 40], 16, device="cpu")
+    assert CudaOps._written_pages("x", step, 16) == (3, 3)
+    step.host_cu_seqlens[1:] = [1, 4]
+    assert CudaOps._written_pages("x", step, 16) == (3, 3)
+    step.host_cu_seqlens[1:] = [40, 41]
+    step.num_tokens = 41
+    assert CudaOps._written_pages("x", step, 16) == (5, 40)
+    step.host_cu_seqlens = [0, 1, 41]
+    assert CudaOps._written_pages("x", step, 16) == (5, 40)
+
+
 def attention_args(new=(1, 1), lens=(20, 3), H=4, G=2, D=128, page=16, dtype=torch.bfloat16, **kw):
     step = p8.step_of(list(new), list(lens), page, device="cpu")
     T = sum(new)
