@@ -105,6 +105,10 @@ template <int D> __device__ __forceinline__ void take_query(uint32_t (&b)[Head<D
 //   BULK   page sizes that are a multiple of 16: a tile is 16 tokens of one page, brought by one bulk copy (16 tokens a page) or three
 //          that a lane asks for, and has one scale.  Rows behind the slice's end come along and are masked.
 //   else   any page size: cp.async token by token, each with its scales; what is not there is zero.
+// What bounds it is reading the codes: eight tokens behind 17,000 to 32,768, 64 heads over 8 of 128, 85 us, 5.9 TB/s while it runs (pages of 16 bits 163);
+// issue 0.34 a clock, a warp waits for results of mma.sync and for copies about alike.  Smaller launches lose to the blocks' beginnings and ends: eight
+// behind 4,096, 32 heads over 8, 17 us for 10 of reading; one behind 512, 5 us, a chain of lookups, copies and a join.  No more, measured at both: rings of
+// 2 or 4 stages, 1 or 4 tiles a step, 3 blocks an SM, two accumulators for the scores, values read before the softmax.
 constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int STEP = 16;  // keys of a tile
@@ -675,7 +679,9 @@ template <int D, int NT> int launch_decode(const Decode& a, int num_seqs, cudaSt
 // reads itself, then takes two channels (or four, eight) of every value.  No barrier until the warps are joined.  Sums are float32 on the FMA pipes, in an
 // order that depends on the keys' places alone: a warp's 32 keys begin at a multiple of 32, what the warps and then the slices of 256 keys have is joined in
 // order, by the same block or, where the launch leaves SMs idle, by a second kernel from what one block a slice has left -- the same bits, however a
-// sequence is cut into steps and batched with others.  What bounds it is instructions, and for few tokens the chain of a slice.
+// sequence is cut into steps and batched with others.  What bounds it is instructions, and for few tokens the chain of a slice: 21 float32 tokens behind up
+// to 320, 16 heads over 4 of 64, 10 us (0.17 issued a clock; with barriers between the tiles of a slice 17); eight behind 4,096, 32 over 8 of 128, 52; a prompt of 512 158
+// (keys' pieces by neighbouring lanes, each line once: 185).
 constexpr int GEN_WARPS = 8;
 constexpr int GEN_THREADS = 32 * GEN_WARPS;
 constexpr int GEN_SLICE = 32 * GEN_WARPS;
