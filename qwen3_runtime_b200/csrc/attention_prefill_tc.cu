@@ -89,6 +89,7 @@ struct Params {
   float lambda, eps, out_scale;   // MAPS
   int* error_word;
   int keep_first, head_dim;       // FIRST: keys that every token sees, whatever its window; columns of a head
+  const int4* items;              // FIRST: what the blocks take, see q3_window_attention_prefill_tc
 };
 
 // 2^x in one instruction (exp2f adds range fix-ups around the same instruction; results
@@ -171,7 +172,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
     // heavy work (late rows of long prompts) first: walk the work list from its end
     int acc = 0, found = -1, rb = 0;
     const int w = p.num_work - 1 - (int)(blockIdx.x / nkv);
-    for (int s = 0; s < p.num_seqs; ++s) {
+    for (int s = 0; MODE != FIRST && s < p.num_seqs; ++s) {
       const int ql = cu_seqlens[s + 1] - cu_seqlens[s];
       if (ql <= 0 || (p.skip_single && ql == 1)) continue;
       int nb = (ql * G + block_m - 1) / block_m;  // row blocks
@@ -211,19 +212,26 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_base_s;
-  const int seq = s_item[0];
+  int4 what = make_int4(s_item[1], 0, 0, 0), where = make_int4(0, 0, 0, 0);
+  int seq = s_item[0];
+  if (MODE == FIRST) {  // (the kernel before may still have been at work on its last pages)
+    pdl_wait();
+    what = p.items[2 * (blockIdx.x / nkv)], where = p.items[2 * (blockIdx.x / nkv) + 1];
+    seq = what.x < 0 ? -1 : 0;
+  }
 
   if (seq >= 0) {
-    const int tok0 = cu_seqlens[seq];
-    const int q_len = cu_seqlens[seq + 1] - tok0;
-    const int kv_len = p.kv_lens[seq];
+    const int item = what.x;
+    const int tok0 = MODE == FIRST ? what.y : cu_seqlens[seq];
+    const int q_len = MODE == FIRST ? what.z : cu_seqlens[seq + 1] - tok0;
+    const int kv_len = MODE == FIRST ? what.w : p.kv_lens[seq];
     const int rows = q_len * G;
     const int base_pos = kv_len - q_len;
     // row blocks A and B of this item; B may not exist (odd number of blocks)
     int row0[2], p_max[2], tiles[2];
     // under a chunked mask or a window the item's first visible key is that of its first row; tiles count from the tile
     // it is in
-    const int p_first = base_pos + (MODE == MAPS ? 1 : 2) * s_item[1] * block_m / G;
+    const int p_first = base_pos + (MODE == MAPS ? 1 : 2) * item * block_m / G;
     const int k_lo = chunk > 0 ? p_first / chunk * chunk : (window > 0 ? max(0, p_first - window + 1) : 0);
     const int tile0 = k_lo / BLOCK_N;
     // FIRST: tiles 0 .. firsts - 1 and those from tile0 on; `skip` of them lie between
@@ -232,7 +240,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
     auto tile_at = [&](int j) { return MODE == FIRST ? j + (j >= firsts ? skip : 0) : tile0 + j; };
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      row0[x] = (MODE == MAPS ? s_item[1] : 2 * s_item[1] + x) * block_m;
+      row0[x] = (MODE == MAPS ? item : 2 * item + x) * block_m;
       const bool live = row0[x] < rows;
       const int last_row = min(rows, row0[x] + block_m) - 1;
       p_max[x] = live ? base_pos + last_row / G : -1;
@@ -240,7 +248,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
     }
     const int num_tiles = max(tiles[0], tiles[1]);  // B lies after A, so this is B's count when B exists
     const int p_last = max(p_max[0], p_max[1]);
-    const int* bt = MODE == DENSE ? nullptr : block_table + (long)seq * max_pages;
+    const int* bt = MODE == DENSE || MODE == FIRST ? nullptr : block_table + (long)seq * max_pages;
     const int pages_per_tile = MODE == DENSE ? 0 : BLOCK_N / ps;
 
     if (warp < 4) {  // ---- TMA producers: keys and values, 64 columns each ----
@@ -268,8 +276,12 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       const CUtensorMap* map = MODE == DENSE || part < 2 ? &tmap_k : &tmap_v;
       auto page_of = [&](int j) -> int {  // pages of tile j that exist in the block table (the rest of the tile is masked)
         const int pi = tile_at(j) * pages_per_tile + lane;
+        if (MODE == FIRST) {  // pages lie in order, without those between the first tokens' and the first window's
+          const bool in = lane < pages_per_tile && j < num_tiles && pi * ps <= p_last && ((pi + 1) * ps > k_lo || pi * ps < keep);
+          return in ? where.x + (pi < where.y ? pi : pi - where.z + where.y) : -1;
+        }
         const bool in = lane < pages_per_tile && j < num_tiles && pi < max_pages && pi * ps <= p_last &&
-                        ((pi + 1) * ps > k_lo || (MODE == FIRST && pi * ps < keep));
+                        (pi + 1) * ps > k_lo;
         return in ? bt[pi] : -1;
       };
       int next = MODE == DENSE ? 0 : page_of(0);
@@ -644,7 +656,10 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
       return Q3_ERR_LAUNCH;
     configured = true;
   }
-  prefill_attention_tc_kernel<MODE><<<dim3((unsigned)p.num_work * p.nkv), THREADS, Sizes<MODE>::SMEM, stream>>>(tq, tk, tv, tr, p);
+  const dim3 grid((unsigned)p.num_work * p.nkv);
+  if (MODE == FIRST)
+    return launch_pdl(prefill_attention_tc_kernel<MODE>, grid, dim3(THREADS), Sizes<MODE>::SMEM, stream, tq, tk, tv, tr, p) == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
+  prefill_attention_tc_kernel<MODE><<<grid, THREADS, Sizes<MODE>::SMEM, stream>>>(tq, tk, tv, tr, p);
   return q3_launch_status();
 }
 
@@ -698,17 +713,17 @@ Q3_EXPORT int q3_paged_attention_prefill_tc(const void* q, int q_stride, int num
   return launch<PAGED>(tq, tk, tv, tq, p, stream);
 }
 
-// The same for heads of 64 to 128 (a multiple of 16) and groups of up to 128, num_work = sum over served sequences of ceil(ceil(q_len / (128 / group)) / 2),
-// 128 / group in whole tokens; window > 0: a token sees the last `window` keys up to itself, and the sequence's first `keep_first`.
+// The same for heads of 64 to 128 (a multiple of 16) and groups of up to 128, over pages that lie in a sequence's order; window > 0: a token sees the last
+// `window` keys up to itself, and the sequence's first `keep_first`.  `items` [num_work][2], 16-byte aligned, what the blocks take, in that order:
+// {item of its sequence, of 2 (128 / group) tokens, 128 / group in whole ones (-1: nothing); the sequence's first token; its tokens; its length},
+// {its first page; k; s}: the sequence's pages 0 .. k - 1 and s, s + 1, .. are there, one after the other.
 Q3_EXPORT int q3_window_attention_prefill_tc(const void* q, int q_stride, int num_tokens, const void* kpages, const void* vpages,
-                                             long num_rows_kv, const int* block_table, int max_pages, const int* kv_lens,
-                                             const int* cu_seqlens, void* out, int num_seqs, int num_work, int nq, int nkv, int head_dim,
-                                             int ps, float scale, int skip_single, int window, int keep_first, int* error_word,
-                                             cudaStream_t stream) {
-  if (!q || !kpages || !vpages || !block_table || !kv_lens || !cu_seqlens || !out || window < 0 || keep_first < 0) return Q3_ERR_ARGUMENT;
+                                             long num_rows_kv, const void* items, void* out, int num_work, int nq, int nkv, int head_dim,
+                                             int ps, float scale, int window, int keep_first, int* error_word, cudaStream_t stream) {
+  if (!q || !kpages || !vpages || !items || !out || window < 0 || keep_first < 0) return Q3_ERR_ARGUMENT;
   if (nq < 1 || nkv < 1 || nq % nkv) return Q3_ERR_ARGUMENT;
   if (head_dim < 64 || head_dim > D || head_dim % 16 || nq / nkv > BLOCK_M || (ps != 8 && ps != 16 && ps != 32 && ps != 64) || q_stride % 8 || nkv > 65535 ||
-      (((uintptr_t)q | (uintptr_t)kpages | (uintptr_t)vpages | (uintptr_t)out) & 15))
+      (((uintptr_t)q | (uintptr_t)kpages | (uintptr_t)vpages | (uintptr_t)out | (uintptr_t)items) & 15))
     return Q3_ERR_UNSUPPORTED;
   if (num_work == 0) return Q3_OK;
   CUtensorMap tq, tk, tv;
@@ -716,8 +731,8 @@ Q3_EXPORT int q3_window_attention_prefill_tc(const void* q, int q_stride, int nu
       !q3_bf16_map(&tk, kpages, num_rows_kv, head_dim, head_dim, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
       !q3_bf16_map(&tv, vpages, num_rows_kv, head_dim, head_dim, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
     return Q3_ERR_LAUNCH;
-  const Params p = {block_table, max_pages, kv_lens, cu_seqlens, (bf16*)out, num_seqs, num_work, nq, nkv, ps, scale * LOG2_E, skip_single, 0,
-                    window, nullptr, nullptr, nullptr, 0.f, 0.f, 0.f, error_word, keep_first, head_dim};
+  const Params p = {nullptr, 0, nullptr, nullptr, (bf16*)out, 0, num_work, nq, nkv, ps, scale * LOG2_E, 0, 0,
+                    window, nullptr, nullptr, nullptr, 0.f, 0.f, 0.f, error_word, keep_first, head_dim, (const int4*)items};
   return launch<FIRST>(tq, tk, tv, tq, p, stream);
 }
 

@@ -306,23 +306,89 @@ __global__ void __launch_bounds__(STORE_THREADS) store_8bit_kernel(const T* qkv,
 // Two forms.  Without `cu_seqlens`, sequence z's page i goes to page z * width + i, rows behind its last token are zero, and whole pages behind
 // it too.  With it, the attention over prompts reads the pages: only sequences that bring at least `least` tokens count, and of each only the
 // pages that a new token sees (with a window those of the first `keep_first` tokens, and those from the first that the first new token's window
-// reaches); they lie one after the other, `count` pages in all, and `table_out` [num_seqs][width] says where (entries that nobody asks for name a
-// page of the same sequence, never none).  The pages that are written are as large as the cache's, or of 16 tokens where the attention does not take those.
+// reaches); they lie one after the other, `count` pages in all.  The pages that are written are as large as the cache's, or of 16 tokens where the attention
+// does not take those.  Warps of their own then write what that attention works through: `items`, of `item_tokens` tokens of a sequence each.
 struct Unpack {
   const unsigned char* pages;
   int num_pages, nkv, ps;
   const int *block_table, *kv_lens, *cu_seqlens;
   int max_pages, num_seqs, max_len, least, window, keep_first, count, width, out_ps;  // out_ps: tokens of a page that is written
-  int* table_out;
+  int item_tokens, num_items;
+  int4* items;  // [num_items][2], see write_item
 };
+
+// What sequence s brings: tokens (0: it does not count), length, and its pages that are written: 0 .. kept - 1 and skip .. last.
+struct UnpackSequence {
+  int tokens = 0, len = 0, kept = 0, skip = 0, pages = 0;
+  __device__ __forceinline__ UnpackSequence(const Unpack& a, int s) {
+    if (s >= a.num_seqs) return;
+    const int news = a.cu_seqlens[s + 1] - a.cu_seqlens[s];
+    len = min(a.kv_lens[s], a.max_len);
+    if (news < a.least) return;
+    tokens = news;
+    if (len <= 0) return;
+    if (a.window > 0) skip = max(0, len - tokens - a.window + 1) / a.out_ps;
+    kept = min(skip, (a.keep_first + a.out_ps - 1) / a.out_ps);
+    pages = (len + a.out_ps - 1) / a.out_ps - skip + kept;
+  }
+};
+__device__ __forceinline__ int warp_prefix(int n) {  // the sum up to and with this lane's
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, n, o);
+    if ((threadIdx.x & 31) >= o) n += y;
+  }
+  return n;
+}
+
+// Item `w` of the attention, as {place in its sequence, the sequence's first token, its tokens, its length}, {its first page that is written, kept, skip}; place
+// -1: none.  Items stand by how many keys they see, in units of a tile, the heaviest first, so that the last blocks of the launch are short: where
+// 1,500 + 701 + 1,000 tokens stand behind one another the attention takes ITEMS_NOW us, in the order of the sequences ITEMS_THEN.  An item's place follows from how many of each
+// sequence see more, which is a division, as they grow evenly.  By a warp.
+__device__ __forceinline__ void write_item(const Unpack& a, int w) {
+  const int lane = threadIdx.x & 31, T = a.item_tokens;
+  const int most = a.window > 0 ? a.window + a.keep_first + T : 0x7fffffff;  // keys that an item sees, roughly
+  int seq = -1, i = 0, before = 0, pages = 0;
+  int4 what = make_int4(-1, 0, 0, 0), where = make_int4(0, 0, 0, 0);
+  for (int base = 0, left = w; base < a.num_seqs && seq < 0; base += 32) {
+    const UnpackSequence s(a, base + lane);
+    const int n = (s.tokens + T - 1) / T, sum = warp_prefix(n), page_sum = warp_prefix(s.pages);
+    const uint32_t reach = __ballot_sync(0xffffffffu, sum > left);
+    if (reach) {
+      const int from = __ffs(reach) - 1;
+      seq = base + from;
+      i = left - __shfl_sync(0xffffffffu, sum - n, from);
+      what = make_int4(i, a.cu_seqlens[seq], __shfl_sync(0xffffffffu, s.tokens, from), __shfl_sync(0xffffffffu, s.len, from));
+      where = make_int4(pages + __shfl_sync(0xffffffffu, page_sum - s.pages, from), __shfl_sync(0xffffffffu, s.kept, from),
+                        __shfl_sync(0xffffffffu, s.skip, from), 0);
+    } else {
+      left -= __shfl_sync(0xffffffffu, sum, 31);
+      pages += __shfl_sync(0xffffffffu, page_sum, 31);
+    }
+  }
+  int at = w;  // (places behind the last item say so)
+  if (seq >= 0) {
+    const int tiles = min(max(0, what.w - what.z) + (i + 1) * T, most) >> 6;
+    for (int base = 0; base < a.num_seqs; base += 32) {
+      const UnpackSequence s(a, base + lane);
+      const int n = (s.tokens + T - 1) / T, first = max(0, s.len - s.tokens);
+      auto items_of = [&](int t) {  // how many of this sequence's see at least t tiles: the last ones
+        return t > most >> 6 ? 0 : n - min(n, max(0, (max(0, 64 * t - first) + T - 1) / T - 1));
+      };
+      const int more = items_of(tiles + 1);
+      before += more + (base + lane < seq ? items_of(tiles) - more : 0) + (base + lane == seq ? n - more - 1 - i : 0);
+    }
+    at = __reduce_add_sync(0xffffffffu, before);
+  }
+  if (lane == 0 && at < a.num_items) a.items[2 * at] = what, a.items[2 * at + 1] = where;
+}
 
 __host__ __device__ __forceinline__ constexpr int unpack_rows(int D) { return 2048 / D; }  // of a page that a warp takes
 
 // Page `p` of the output (of a launch whose second axis is the sequences, without `cu_seqlens`).  Called by whole warps.
 struct UnpackPage {
-  int seq, i;             // the sequence (-1: none) and its page
-  int kept, skip, last;   // its pages that count: 0 .. kept - 1 and skip .. last
-  __device__ __forceinline__ UnpackPage(const Unpack& a, int p) : seq(-1), i(0), kept(0), skip(0), last(a.width - 1) {
+  int seq, i;  // the sequence (-1: none) and its page
+  __device__ __forceinline__ UnpackPage(const Unpack& a, int p) : seq(-1), i(0) {
     if (!a.cu_seqlens) {
       seq = blockIdx.y, i = p;
       return;
@@ -330,45 +396,19 @@ struct UnpackPage {
     if (p >= a.count) return;
     const int lane = threadIdx.x & 31;
     for (int base = 0; base < a.num_seqs; base += 32) {
-      int from_page = 0, first_pages = 0, pages = 0;
-      if (base + lane < a.num_seqs) {
-        const int tokens = a.cu_seqlens[base + lane + 1] - a.cu_seqlens[base + lane], len = min(a.kv_lens[base + lane], a.max_len);
-        if (tokens >= a.least && len > 0) {
-          if (a.window > 0) from_page = max(0, len - tokens - a.window + 1) / a.out_ps;
-          first_pages = min(from_page, (a.keep_first + a.out_ps - 1) / a.out_ps);
-          pages = (len + a.out_ps - 1) / a.out_ps;
-        }
-      }
-      const int n = pages - from_page + first_pages;
-      int sum = n;  // pages up to and with this lane's sequence
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += y;
-      }
+      const UnpackSequence s(a, base + lane);
+      const int sum = warp_prefix(s.pages);
       const uint32_t reach = __ballot_sync(0xffffffffu, sum > p);
       if (reach) {
         const int from = __ffs(reach) - 1;
         seq = base + from;
-        kept = __shfl_sync(0xffffffffu, first_pages, from), skip = __shfl_sync(0xffffffffu, from_page, from);
-        last = __shfl_sync(0xffffffffu, pages, from) - 1;
-        i = p - (__shfl_sync(0xffffffffu, sum, from) - __shfl_sync(0xffffffffu, n, from));
+        const int kept = __shfl_sync(0xffffffffu, s.kept, from), skip = __shfl_sync(0xffffffffu, s.skip, from);
+        i = p - __shfl_sync(0xffffffffu, sum - s.pages, from);
         if (i >= kept) i += skip - kept;
         return;
       }
       p -= __shfl_sync(0xffffffffu, sum, 31);
     }
-  }
-  // what the table says of this page, of those that are left out in front of it and of those behind the last; by one warp a page
-  __device__ __forceinline__ void name(const Unpack& a, int p) const {
-    if (!a.table_out) return;
-    int* row = a.table_out + (long)seq * a.width;
-    const int lane = threadIdx.x & 31;
-    if (lane == 0 && i < a.width) row[i] = p;
-    if (i == skip)
-      for (int j = kept + lane; j < min(skip, a.width); j += 32) row[j] = p;
-    if (i == last)
-      for (int j = last + 1 + lane; j < a.width; j += 32) row[j] = p;
   }
   // where its bytes lie, and how many rows of it count
   __device__ __forceinline__ int rows(const Unpack& a, int* page) const {
@@ -405,13 +445,18 @@ template <typename T, int KNOWN> __global__ void __launch_bounds__(256) unpack_8
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const uint32_t item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), half = item >> 1, pair = parts == 1 ? half : half / parts;
+  uint32_t item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (item < a.num_items) {
+    write_item(a, item);
+    return;
+  }
+  item -= a.num_items;
+  const uint32_t half = item >> 1, pair = parts == 1 ? half : half / parts;
   const int is_v = item & 1, part = (int)(half - pair * parts), p = (int)(pair / a.nkv), kvh = (int)(pair - p * a.nkv);
   if (p >= (a.cu_seqlens ? a.count : a.width)) return;
   const UnpackPage at_page(a, p);
   if (at_page.seq < 0) return;
   const int place = a.cu_seqlens ? p : blockIdx.y * a.width + p;
-  if (kvh == 0 && part == 0 && !is_v) at_page.name(a, place);
   int page;
   const int row0 = part * unpack_rows(D), rows = at_page.rows(a, &page) - row0;  // those that count, from the part's first on
   const Q8Page L(D, a.ps);
@@ -450,11 +495,16 @@ template <typename T> __global__ void __launch_bounds__(256) unpack_8bit_other_k
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const uint32_t item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), half = item >> 1;
+  uint32_t item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (item < a.num_items) {
+    write_item(a, item);
+    return;
+  }
+  item -= a.num_items;
+  const uint32_t half = item >> 1;
   const int is_v = item & 1, p = (int)(half / a.nkv), kvh = (int)(half - (uint32_t)p * a.nkv);
   const UnpackPage at_page(a, p);
   if (at_page.seq < 0) return;
-  if (kvh == 0 && !is_v) at_page.name(a, p);
   const Q8Page L(D, a.ps);
   // where this lane's token lies, a multiple of 16, and below that how its pieces are ordered; 0: nowhere
   unsigned long long where = 0;
@@ -490,9 +540,9 @@ template <typename T> __global__ void __launch_bounds__(256) unpack_8bit_other_k
 
 template <typename T> cudaError_t launch_unpack(const Unpack& a, int D, T* k_out, T* v_out, cudaStream_t stream) {
   if (a.out_ps != a.ps)
-    return launch_pdl(unpack_8bit_other_kernel<T>, dim3((unsigned)((2L * a.count * a.nkv + 7) / 8)), dim3(256), 0, stream, a, D, k_out, v_out);
+    return launch_pdl(unpack_8bit_other_kernel<T>, dim3((unsigned)((2L * a.count * a.nkv + a.num_items + 7) / 8)), dim3(256), 0, stream, a, D, k_out, v_out);
   const int parts = (a.ps + unpack_rows(D) - 1) / unpack_rows(D);
-  const long items = 2L * (a.cu_seqlens ? a.count : a.width) * a.nkv * parts;
+  const long items = 2L * (a.cu_seqlens ? a.count : a.width) * a.nkv * parts + a.num_items;
   const dim3 grid((unsigned)((items + 7) / 8), a.cu_seqlens ? 1 : a.num_seqs);
   if (D == 64) return launch_pdl(unpack_8bit_kernel<T, 64>, grid, dim3(256), 0, stream, a, D, parts, k_out, v_out);
   if (D == 128) return launch_pdl(unpack_8bit_kernel<T, 128>, grid, dim3(256), 0, stream, a, D, parts, k_out, v_out);
@@ -567,19 +617,22 @@ Q3_EXPORT int q3_store_8bit(int dtype, const void* qkv, int row_stride, void* q_
   return q3_launch_status();
 }
 
-// `cu_seqlens` null: num_seqs * width pages are written, as large as the cache's; else `count` pages of out_ps tokens (struct Unpack).
+// `cu_seqlens` null: num_seqs * width pages are written, as large as the cache's; else `count` pages of out_ps tokens and `num_items` items (struct Unpack).
 Q3_EXPORT int q3_unpack_8bit(int dtype, const void* pages, int num_pages, int nkv, int D, int ps, const int* block_table, int max_pages,
                              const int* kv_lens, int num_seqs, int max_len, const int* cu_seqlens, int least, int window, int keep_first,
-                             int count, int width, int out_ps, void* k_out, void* v_out, int* table_out, cudaStream_t stream) {
-  if (num_seqs < 1 || width < 1 || (cu_seqlens && count < 1)) return Q3_OK;
+                             int count, int width, int out_ps, void* k_out, void* v_out, int item_tokens, int num_items, void* items,
+                             cudaStream_t stream) {
+  if (num_seqs < 1 || (cu_seqlens ? count : width) < 1) return Q3_OK;
   if (!pages || !block_table || !kv_lens || !k_out || !v_out || nkv < 1 || max_pages < 1 || !q8_sizes_ok(D, ps)) return Q3_ERR_ARGUMENT;
-  if (cu_seqlens && (!table_out || least < 1 || keep_first < 0)) return Q3_ERR_ARGUMENT;
+  if (cu_seqlens ? !items || item_tokens < 1 || num_items < 0 || least < 1 || keep_first < 0 || window + (long)keep_first > 1 << 30 || !q8_aligned(items)
+                 : num_items != 0)
+    return Q3_ERR_ARGUMENT;
   if (out_ps != ps && (!cu_seqlens || out_ps != OTHER_PAGE)) return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
   if ((!cu_seqlens && num_seqs > 65535) || !q8_aligned(pages) || !q8_aligned(k_out) || !q8_aligned(v_out)) return Q3_ERR_UNSUPPORTED;
-  if ((long)(cu_seqlens ? count : width) * 2 * nkv * ((ps + unpack_rows(D) - 1) / unpack_rows(D)) > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
+  if ((long)(cu_seqlens ? count : width) * 2 * nkv * ((ps + unpack_rows(D) - 1) / unpack_rows(D)) + num_items > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
   const Unpack a{(const unsigned char*)pages, num_pages, nkv, ps, block_table, kv_lens, cu_seqlens, max_pages, num_seqs, max_len, least, window,
-                 keep_first, count, width, out_ps, table_out};
+                 keep_first, count, width, out_ps, item_tokens, num_items, (int4*)items};
   const cudaError_t err = dtype == Q3_DTYPE_F32 ? launch_unpack(a, D, (float*)k_out, (float*)v_out, stream)
                                                 : launch_unpack(a, D, (bf16*)k_out, (bf16*)v_out, stream);
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;

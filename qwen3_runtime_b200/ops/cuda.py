@@ -220,9 +220,8 @@ _SIGNATURES = {
         "q3_paged_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, ctypes.c_long, c_void_p, c_int,
                                           c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                                           c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
-        "q3_window_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_long, c_void_p, c_int, c_void_p, c_void_p,
-                                           c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p,
-                                           c_void_p],
+        "q3_window_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_int, c_int, c_int,
+                                           c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p],
         "q3_diff_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_long, c_void_p, c_int, c_void_p,
                                          c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
                                          c_float, c_float, c_float, c_void_p, c_void_p],
@@ -262,7 +261,7 @@ _SIGNATURES = {
                           c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int,
                           c_int, c_int, c_int, c_int, c_void_p, c_void_p],
         "q3_unpack_8bit": [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
-                           c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+                           c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p],
     },
     "attention_8bit": {
         "q3_decode_attention_8bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -2635,7 +2634,7 @@ class CudaOps:
             self._costs(2 * k.numel() * k.element_size() + B * n * num_kv_heads * eight_bit_page_bytes(head_dim, page_size))
         self._call("cache_8bit", "q3_unpack_8bit", what, _dtype_code(dtype), pages.data_ptr(), pages.shape[0], num_kv_heads, head_dim,
                    page_size, block_table.data_ptr(), width, _ptr(kv_lens), B, int(max_kv_len), None, 0, 0, 0, 0, n, page_size, k.data_ptr(),
-                   v.data_ptr(), None)
+                   v.data_ptr(), 0, 0, None)
         return k, v
 
     def paged_attention_8bit(self, q, q_stride, *, num_heads, num_kv_heads, head_dim, pages, block_table, out, page_size, scale, step,
@@ -2753,22 +2752,21 @@ class CudaOps:
         news = [b - a for a, b in zip(step.host_cu_seqlens[first:end], step.host_cu_seqlens[first + 1:end + 1])]
         if seqs != step.num_seqs:  # these sequences alone
             cu, kv_lens, block_table = cu[first:end + 1], kv_lens[first:end], block_table[first:end]
+        per = 2 * (128 // (H // G))  # tokens of an item: two blocks of rows
+        num_items = sum([-(-n // per) for n in news if n >= least])
         k = torch.empty((2, count, G, wide, D), dtype=out.dtype, device=out.device)
         v_at = k.data_ptr() + k.numel()  # (half of its bytes)
-        width = -(-longest // wide)
-        table = torch.empty((seqs, width), dtype=torch.int32, device=out.device)
+        items = torch.empty((num_items, 8), dtype=torch.int32, device=out.device)
         if self.timing is not None:
             self._costs(k.numel() * k.element_size() + count * wide * 2 * G * D)
         self._call("cache_8bit", "q3_unpack_8bit", "unpack_8bit", _dtype_code(out.dtype), pages.data_ptr(), pages.size(0), G, D, page_size,
-                   block_table.data_ptr(), block_table.size(1), kv_lens.data_ptr(), seqs, longest, cu.data_ptr(), least, window, keep_first, count,
-                   width, wide, k.data_ptr(), v_at, table.data_ptr())
-        per = 128 // (H // G)  # tokens of a block of rows
-        pairs = sum([-(-(-(-n // per)) // 2) for n in news if n >= least])  # two blocks an item
+                   block_table.data_ptr(), block_table.size(1), kv_lens.data_ptr(), seqs, longest, cu.data_ptr(), least, window, keep_first, count, 0,
+                   wide, k.data_ptr(), v_at, per, num_items, items.data_ptr())
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out, prompts=True))
         self._call("attention_prefill_tc", "q3_window_attention_prefill_tc", "paged_attention_prefill_8bit", q.data_ptr(), q_stride, q.size(0),
-                   k.data_ptr(), v_at, count * G * wide, table.data_ptr(), width, kv_lens.data_ptr(), cu.data_ptr(), out.data_ptr(), seqs, pairs,
-                   H, G, D, wide, float(scale), least - 1, window, keep_first, self._error_word(out.device).data_ptr())
+                   k.data_ptr(), v_at, count * G * wide, items.data_ptr(), out.data_ptr(), num_items, H, G, D, wide, float(scale), window, keep_first,
+                   self._error_word(out.device).data_ptr())
 
     def _prompts_8bit(self, q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first):
         """Attention of the sequences that bring at least ``least`` tokens, straight over the codes (csrc/prompts_8bit.cu)."""

@@ -51,10 +51,9 @@ def test_prompts_under_a_window():
     q = t8.queries(270, H, D, 1)
     step, dev, out = p8.step_of(new, lens, page), q.cuda(), torch.zeros((270, H * D), dtype=torch.bfloat16, device="cuda")
     k, v = ops.unpack_8bit(c.pages.cuda(), block_table=c.table.cuda(), kv_lens=step.kv_lens, max_kv_len=400, dtype=torch.bfloat16, **t8.sizes(c))
-    table = torch.arange(2 * 25, dtype=torch.int32, device="cuda").view(2, 25)
-    pairs = sum(-(-(-(-n * H // G // 128)) // 2) for n in new)
+    items = t8.i32([[i, 70 * b, new[b], lens[b], 25 * b, 0, 0, 0] for b in range(2) for i in range(-(-new[b] // 64))])
     launch = _build("attention_prefill_tc", "q3_window_attention_prefill_tc")
-    assert run(launch, dev.data_ptr(), H * D, 270, k.data_ptr(), v.data_ptr(), 50 * G * page, table.data_ptr(), 25, step.kv_lens.data_ptr(),
-               step.cu_seqlens.data_ptr(), out.data_ptr(), 2, pairs, H, G, D, page, D ** -0.5, 1, 100, 20) == 2
+    assert run(launch, dev.data_ptr(), H * D, 270, k.data_ptr(), v.data_ptr(), 50 * G * page, items.data_ptr(),
+               out.data_ptr(), len(items), H, G, D, page, D ** -0.5, 100, 20) == 2
     got = t8.attend(ops, c, q, new, lens, H, D ** -0.5, window=100, keep_first=20)  # the ordinary build afterwards
     t8.check_rows(got, q.view(270, H, D), c, new, lens, D ** -0.5, window=100, keep_first=20, wide=True)
