@@ -1,11 +1,7 @@
 // Causal attention of prompt portions on the 5th-generation tensor cores: S = Q K^T and O += P V are tcgen05.mma
-// with accumulators in tensor memory; Q, K and V tiles arrive by TMA (128-byte swizzle).  bfloat16; four forms:
+// with accumulators in tensor memory; Q, K and V tiles arrive by TMA (128-byte swizzle).  bfloat16; three forms:
 //   PAGED    heads of 128 over the paged cache, straight from the QKV buffer and the pages (group size a divisor of 128,
 //            page size 8/16/32/64); options: a chunked mask, turned values, sinks;
-//   FIRST    over pages as well, for heads of 64 to 128 (columns that a head lacks are beyond the tensors' inner extent, and arrive as zeros) and any
-//            group (a block has as many rows as whole tokens give); optionally under a window, whose tokens may see the sequence's first ones too:
-//            the tiles of those come in front, and the ones between them and the window are left out;
-//            700 + 2,048 + 500 tokens, 32 heads over 8 under a window of 1,024: 63 us (on mma.sync 200), the longest chain of tiles on an SM 54 of them;
 //   MAPS     differential attention: a head is two maps of 64 side by side in its 128 columns, over one value of 128;
 //            options: a chunked mask or a window;
 //   DENSE    keys of 192 = 128 of the head's own + 64 shared by the heads, values of 128, one key head per query head,
@@ -56,7 +52,7 @@
 
 namespace {
 
-enum { PAGED = 0, MAPS = 1, DENSE = 2, FIRST = 3 };
+enum { PAGED = 0, MAPS = 1, DENSE = 2 };
 constexpr int D = 128;  // value size, and query/key size of PAGED and of both maps together
 constexpr int BLOCK_M = 128;
 constexpr int BLOCK_N = 64;
@@ -88,8 +84,6 @@ struct Params {
   const int* kv_base;             // DENSE: key j of sequence s is row kv_base[s] + j
   float lambda, eps, out_scale;   // MAPS
   int* error_word;
-  int keep_first, head_dim;       // FIRST: keys that every token sees, whatever its window; columns of a head
-  const int4* items;              // FIRST: what the blocks take, see q3_window_attention_prefill_tc
 };
 
 // 2^x in one instruction (exp2f adds range fix-ups around the same instruction; results
@@ -163,7 +157,6 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
   // heavy items first over the whole grid: all kv heads of the heaviest item, then the next ...
   const int kvh = blockIdx.x % nkv;
   const int G = nq / nkv;
-  const int block_m = MODE == FIRST ? BLOCK_M / G * G : BLOCK_M;  // rows of a block
   const uint32_t bar0 = smem_addr(&bars[0]);
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
@@ -172,10 +165,10 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
     // heavy work (late rows of long prompts) first: walk the work list from its end
     int acc = 0, found = -1, rb = 0;
     const int w = p.num_work - 1 - (int)(blockIdx.x / nkv);
-    for (int s = 0; MODE != FIRST && s < p.num_seqs; ++s) {
+    for (int s = 0; s < p.num_seqs; ++s) {
       const int ql = cu_seqlens[s + 1] - cu_seqlens[s];
       if (ql <= 0 || (p.skip_single && ql == 1)) continue;
-      int nb = (ql * G + block_m - 1) / block_m;  // row blocks
+      int nb = (ql * G + BLOCK_M - 1) / BLOCK_M;  // row blocks
       if (MODE != MAPS) nb = (nb + 1) / 2;        // pairs of them
       if (w < acc + nb) {
         found = s;
@@ -212,51 +205,40 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_base_s;
-  int4 what = make_int4(s_item[1], 0, 0, 0), where = make_int4(0, 0, 0, 0);
-  int seq = s_item[0];
-  if (MODE == FIRST) {  // (the kernel before may still have been at work on its last pages)
-    pdl_wait();
-    what = p.items[2 * (blockIdx.x / nkv)], where = p.items[2 * (blockIdx.x / nkv) + 1];
-    seq = what.x < 0 ? -1 : 0;
-  }
+  const int seq = s_item[0];
 
   if (seq >= 0) {
-    const int item = what.x;
-    const int tok0 = MODE == FIRST ? what.y : cu_seqlens[seq];
-    const int q_len = MODE == FIRST ? what.z : cu_seqlens[seq + 1] - tok0;
-    const int kv_len = MODE == FIRST ? what.w : p.kv_lens[seq];
+    const int tok0 = cu_seqlens[seq];
+    const int q_len = cu_seqlens[seq + 1] - tok0;
+    const int kv_len = p.kv_lens[seq];
     const int rows = q_len * G;
     const int base_pos = kv_len - q_len;
     // row blocks A and B of this item; B may not exist (odd number of blocks)
     int row0[2], p_max[2], tiles[2];
     // under a chunked mask or a window the item's first visible key is that of its first row; tiles count from the tile
     // it is in
-    const int p_first = base_pos + (MODE == MAPS ? 1 : 2) * item * block_m / G;
+    const int p_first = base_pos + (MODE == MAPS ? 1 : 2) * s_item[1] * BLOCK_M / G;
     const int k_lo = chunk > 0 ? p_first / chunk * chunk : (window > 0 ? max(0, p_first - window + 1) : 0);
     const int tile0 = k_lo / BLOCK_N;
-    // FIRST: tiles 0 .. firsts - 1 and those from tile0 on; `skip` of them lie between
-    const int keep = MODE == FIRST ? p.keep_first : 0;
-    const int firsts = MODE == FIRST ? min((keep + BLOCK_N - 1) / BLOCK_N, tile0) : 0, skip = tile0 - firsts;
-    auto tile_at = [&](int j) { return MODE == FIRST ? j + (j >= firsts ? skip : 0) : tile0 + j; };
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      row0[x] = (MODE == MAPS ? item : 2 * item + x) * block_m;
+      row0[x] = (MODE == MAPS ? s_item[1] : 2 * s_item[1] + x) * BLOCK_M;
       const bool live = row0[x] < rows;
-      const int last_row = min(rows, row0[x] + block_m) - 1;
+      const int last_row = min(rows, row0[x] + BLOCK_M) - 1;
       p_max[x] = live ? base_pos + last_row / G : -1;
-      tiles[x] = live ? p_max[x] / BLOCK_N + 1 - skip : 0;
+      tiles[x] = live ? p_max[x] / BLOCK_N + 1 - tile0 : 0;
     }
     const int num_tiles = max(tiles[0], tiles[1]);  // B lies after A, so this is B's count when B exists
     const int p_last = max(p_max[0], p_max[1]);
-    const int* bt = MODE == DENSE || MODE == FIRST ? nullptr : block_table + (long)seq * max_pages;
+    const int* bt = MODE == DENSE ? nullptr : block_table + (long)seq * max_pages;
     const int pages_per_tile = MODE == DENSE ? 0 : BLOCK_N / ps;
 
     if (warp < 4) {  // ---- TMA producers: keys and values, 64 columns each ----
       const int part = warp;  // keys: 0, 1; values: 2, 3
       const int half = part & 1;
       if (part == 3 && lane == 0) {
-        const int BOXES = MODE == MAPS ? 1 : MODE == FIRST ? (p.head_dim + 63) / 64 : DK / 64;  // of a block; MAPS: map x is columns 64 x .. of the head
-        mbar_expect_tx(bar(BAR_Q), (tiles[1] ? 2 : 1) * BOXES * (MODE == FIRST ? block_m * 128 : HALF_Q));
+        constexpr int BOXES = MODE == MAPS ? 1 : DK / 64;  // of a block; MAPS: map x is columns 64 x .. of the head
+        mbar_expect_tx(bar(BAR_Q), (tiles[1] ? 2 : 1) * BOXES * HALF_Q);
         for (int x = 0; x < 2; ++x) {
           if (!tiles[x]) continue;
           for (int c = 0; c < BOXES; ++c) {
@@ -275,13 +257,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       const uint32_t dst0 = smem_addr(part < 2 ? k_s : v_s) + half * HALF_KV;
       const CUtensorMap* map = MODE == DENSE || part < 2 ? &tmap_k : &tmap_v;
       auto page_of = [&](int j) -> int {  // pages of tile j that exist in the block table (the rest of the tile is masked)
-        const int pi = tile_at(j) * pages_per_tile + lane;
-        if (MODE == FIRST) {  // pages lie in order, without those between the first tokens' and the first window's
-          const bool in = lane < pages_per_tile && j < num_tiles && pi * ps <= p_last && ((pi + 1) * ps > k_lo || pi * ps < keep);
-          return in ? where.x + (pi < where.y ? pi : pi - where.z + where.y) : -1;
-        }
-        const bool in = lane < pages_per_tile && j < num_tiles && pi < max_pages && pi * ps <= p_last &&
-                        (pi + 1) * ps > k_lo;
+        const int pi = (tile0 + j) * pages_per_tile + lane;
+        const bool in = lane < pages_per_tile && j < num_tiles && pi < max_pages && pi * ps <= p_last && (pi + 1) * ps > k_lo;
         return in ? bt[pi] : -1;
       };
       int next = MODE == DENSE ? 0 : page_of(0);
@@ -291,9 +268,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         const int page = next;
         const uint32_t dst = dst0 + st * stage_bytes;
         uint32_t bytes = HALF_KV + (MODE == DENSE && part == 1 ? HALF_KV : 0);
-        const bool wanted = MODE != FIRST || 64 * half < p.head_dim;  // (heads of up to 64 have no second half)
         if (MODE != DENSE) {
-          bytes = wanted ? __popc(__ballot_sync(0xffffffffu, page >= 0)) * (uint32_t)ps * 128u : 0;
+          bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * (uint32_t)ps * 128u;
           next = page_of(j + 1);
         }
         if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, phase, &abort_flag))) break;
@@ -310,7 +286,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         } else {
           for (int u = 0; u < pages_per_tile; ++u) {
             const int pg = __shfl_sync(0xffffffffu, page, u);
-            if (lane == 0 && pg >= 0 && wanted) tma_load_2d(dst + u * ps * 128, map, full + 8 * st, half * 64, (pg * nkv + kvh) * ps);
+            if (lane == 0 && pg >= 0) tma_load_2d(dst + u * ps * 128, map, full + 8 * st, half * 64, (pg * nkv + kvh) * ps);
           }
         }
         if (++st == KV_STAGES) st = 0, phase ^= 1;
@@ -350,7 +326,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
 #pragma unroll
               for (int k = 0; k < (MODE == MAPS ? 64 : DK) / 16; ++k) {
                 const uint32_t half = (k >> 2), sub = (k & 3) * 2;  // 4 steps of 32 bytes per 64 columns
-                if (MODE != FIRST || 16 * k < p.head_dim) umma_bf16(tmem_x, umma_desc(q_addr + half * HALF_Q) + sub,
+                umma_bf16(tmem_x, umma_desc(q_addr + half * HALF_Q) + sub,
                      umma_desc(k_addr + (MODE == MAPS ? x : half) * HALF_KV) + sub, idesc, k > 0 ? 1u : 0u);
               }
               umma_commit(bar(BAR_S_FULL + x));    // S_j is in TMEM
@@ -363,8 +339,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
           if (++st == KV_STAGES) st = 0, phase ^= 1;
         }
       } else {
-        // PV: N = 128 (64 for smaller heads), V MN-major
-        const uint32_t idesc = MODE == FIRST && p.head_dim <= 64 ? umma_idesc(BLOCK_M, 64, 1) : umma_idesc(BLOCK_M, D, 1);
+        constexpr uint32_t idesc = umma_idesc(BLOCK_M, D, 1);  // PV: N = 128, V MN-major
         bool ok = true;
         for (int j = 0; j < all && ok; ++j) {
           ok = (j >= mine || wait_all(BAR_P_FULL + x, j & 1)) && wait_all(BAR_V_FULL + st, phase);  // P_j written, O at rest
@@ -397,7 +372,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       const int quarter = warp & 3;
       const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
       const int R = row0[x] + r;
-      const bool row_ok = R < rows && (MODE != FIRST || r < block_m);
+      const bool row_ok = R < rows;
       const int pos = row_ok ? base_pos + R / G : -1;
       // the row's first visible key
       const int lo = !row_ok ? 0 : (chunk > 0 ? pos / chunk * chunk : (window > 0 ? max(0, pos - window + 1) : 0));
@@ -416,7 +391,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       // are scheduled as one run of instructions.
       auto step = [&](int j, auto edge) -> bool {
         constexpr bool EDGE = decltype(edge)::value;
-        const int key0 = tile_at(j) * BLOCK_N;
+        const int key0 = (tile0 + j) * BLOCK_N;
         if (!wait(bar(BAR_S_FULL + x), j & 1, &abort_flag)) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t sa[32], sb[32];
@@ -437,8 +412,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
           if (key0 < lo) {  // keys of an earlier chunk, or before the window
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
-              if (key0 + c < lo && (MODE != FIRST || key0 + c >= keep)) sa[c] = 0xff800000u;
-              if (key0 + 32 + c < lo && (MODE != FIRST || key0 + 32 + c >= keep)) sb[c] = 0xff800000u;
+              if (key0 + c < lo) sa[c] = 0xff800000u;
+              if (key0 + 32 + c < lo) sb[c] = 0xff800000u;
             }
           }
         }
@@ -498,7 +473,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
             const int vst = j % KV_STAGES;
             if (!wait(bar(BAR_V_FULL + vst), (j / KV_STAGES) & 1, &abort_flag)) return false;
             const int vrow = r & 63, half = r >> 6;
-            if (key0 + vrow > p_last || (key0 + vrow < k_lo && (MODE != FIRST || key0 + vrow >= keep))) {
+            if (key0 + vrow > p_last || key0 + vrow < k_lo) {
               uint4* dst = reinterpret_cast<uint4*>(v_s + vst * V_BYTES + half * HALF_KV + vrow * 128);
 #pragma unroll
               for (int ch = 0; ch < 8; ++ch) dst[ch] = make_uint4(0, 0, 0, 0);
@@ -512,15 +487,15 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         return true;
       };
       // tiles that every row of the block sees as a whole: from the last row's first key on, up to the first row's position
-      const int row_first = row0[x], row_last = min(rows, row0[x] + block_m) - 1;
+      const int row_first = row0[x], row_last = min(rows, row0[x] + BLOCK_M) - 1;
       const int pos_first = base_pos + row_first / G, pos_last = base_pos + row_last / G;
       const int lo_last = chunk > 0 ? pos_last / chunk * chunk : (window > 0 ? max(0, pos_last - window + 1) : 0);
       // (What rows that are none see in a last block has no say: nothing of theirs is stored.  A last block that goes through tiles with
       // masks only is the longest of its sequence: 32 heads over 8, 500 tokens behind 3000, 78 us; so 64.)
       int whole0 = 1, whole1 = 0;  // such tiles behind the first one
       if (row0[x] < rows) {
-        whole0 = max(1, (max(lo_last, k_lo) + BLOCK_N - 1) / BLOCK_N - skip);
-        whole1 = min(my_tiles, (pos_first + 1) / BLOCK_N - skip);
+        whole0 = max(1, (max(lo_last, k_lo) + BLOCK_N - 1) / BLOCK_N - tile0);
+        whole1 = min(my_tiles, (pos_first + 1) / BLOCK_N - tile0);
       }
       bool ok = true;
       for (int j = 0; j < my_tiles && ok; ++j) {
@@ -589,8 +564,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         if (p.sinks && row_ok) l_run += exp2f(p.sinks[kvh * G + R % G] * LOG2_E - m_ref * scale_log2);
         const float inv = 1.f / l_run;
         const float* turns = MODE == PAGED ? p.turns : nullptr;
-        const int cols = MODE == FIRST ? p.head_dim : D;
-        bf16* dst = row_ok ? p.out + ((long)(tok0 + R / G) * nq + kvh * G + R % G) * cols : nullptr;
+        bf16* dst = row_ok ? p.out + ((long)(tok0 + R / G) * nq + kvh * G + R % G) * D : nullptr;
         if (turns) {  // turned values: the sum is turned back, element c with element c + D / 2
           const float* cs = row_ok ? turns + (long)(tok0 + R / G) * D : nullptr;  // cos (D / 2), sin (D / 2)
 #pragma unroll 1
@@ -618,7 +592,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
           }
         }
 #pragma unroll 1
-        for (int c0 = 0; c0 < cols && !turns; c0 += 32) {
+        for (int c0 = 0; c0 < D && !turns; c0 += 32) {
           uint32_t ov[32];
           tmem_load32(o_addr + c0, ov);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -628,7 +602,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
               float v8[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) v8[e] = __uint_as_float(ov[c + e]) * inv;
-              if (MODE != FIRST || c0 + c < cols) store8(dst + c0 + c, v8);
+              store8(dst + c0 + c, v8);
             }
           }
         }
@@ -656,10 +630,7 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
       return Q3_ERR_LAUNCH;
     configured = true;
   }
-  const dim3 grid((unsigned)p.num_work * p.nkv);
-  if (MODE == FIRST)
-    return launch_pdl(prefill_attention_tc_kernel<MODE>, grid, dim3(THREADS), Sizes<MODE>::SMEM, stream, tq, tk, tv, tr, p) == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
-  prefill_attention_tc_kernel<MODE><<<grid, THREADS, Sizes<MODE>::SMEM, stream>>>(tq, tk, tv, tr, p);
+  prefill_attention_tc_kernel<MODE><<<dim3((unsigned)p.num_work * p.nkv), THREADS, Sizes<MODE>::SMEM, stream>>>(tq, tk, tv, tr, p);
   return q3_launch_status();
 }
 
@@ -711,29 +682,6 @@ Q3_EXPORT int q3_paged_attention_prefill_tc(const void* q, int q_stride, int num
   const Params p = {block_table, max_pages, kv_lens, cu_seqlens, (bf16*)out, num_seqs, num_work, nq, nkv, ps,
                     scale * LOG2_E, skip_single, chunk, 0, turns, sinks, nullptr, 0.f, 0.f, 0.f, error_word};
   return launch<PAGED>(tq, tk, tv, tq, p, stream);
-}
-
-// The same for heads of 64 to 128 (a multiple of 16) and groups of up to 128, over pages that lie in a sequence's order; window > 0: a token sees the last
-// `window` keys up to itself, and the sequence's first `keep_first`.  `items` [num_work][2], 16-byte aligned, what the blocks take, in that order:
-// {item of its sequence, of 2 (128 / group) tokens, 128 / group in whole ones (-1: nothing); the sequence's first token; its tokens; its length},
-// {its first page; k; s}: the sequence's pages 0 .. k - 1 and s, s + 1, .. are there, one after the other.
-Q3_EXPORT int q3_window_attention_prefill_tc(const void* q, int q_stride, int num_tokens, const void* kpages, const void* vpages,
-                                             long num_rows_kv, const void* items, void* out, int num_work, int nq, int nkv, int head_dim,
-                                             int ps, float scale, int window, int keep_first, int* error_word, cudaStream_t stream) {
-  if (!q || !kpages || !vpages || !items || !out || window < 0 || keep_first < 0) return Q3_ERR_ARGUMENT;
-  if (nq < 1 || nkv < 1 || nq % nkv) return Q3_ERR_ARGUMENT;
-  if (head_dim < 64 || head_dim > D || head_dim % 16 || nq / nkv > BLOCK_M || (ps != 8 && ps != 16 && ps != 32 && ps != 64) || q_stride % 8 || nkv > 65535 ||
-      (((uintptr_t)q | (uintptr_t)kpages | (uintptr_t)vpages | (uintptr_t)out | (uintptr_t)items) & 15))
-    return Q3_ERR_UNSUPPORTED;
-  if (num_work == 0) return Q3_OK;
-  CUtensorMap tq, tk, tv;
-  if (!q_map(&tq, q, head_dim, nq, num_tokens, q_stride, nq / nkv) ||
-      !q3_bf16_map(&tk, kpages, num_rows_kv, head_dim, head_dim, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
-      !q3_bf16_map(&tv, vpages, num_rows_kv, head_dim, head_dim, ps, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
-    return Q3_ERR_LAUNCH;
-  const Params p = {nullptr, 0, nullptr, nullptr, (bf16*)out, 0, num_work, nq, nkv, ps, scale * LOG2_E, 0, 0,
-                    window, nullptr, nullptr, nullptr, 0.f, 0.f, 0.f, error_word, keep_first, head_dim, (const int4*)items};
-  return launch<FIRST>(tq, tk, tv, tq, p, stream);
 }
 
 // Differential attention of every sequence of the step: query head h is [map 1 (64) | map 2 (64)] at column h * 128, key

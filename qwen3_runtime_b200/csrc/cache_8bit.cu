@@ -306,20 +306,21 @@ __global__ void __launch_bounds__(STORE_THREADS) store_8bit_kernel(const T* qkv,
 // Two forms.  Without `cu_seqlens`, sequence z's page i goes to page z * width + i, rows behind its last token are zero, and whole pages behind
 // it too.  With it, the attention over prompts reads the pages: only sequences that bring at least `least` tokens count, and of each only the
 // pages that a new token sees (with a window those of the first `keep_first` tokens, and those from the first that the first new token's window
-// reaches); they lie one after the other, `count` pages in all.  The pages that are written are as large as the cache's, or of 16 tokens where the attention
-// does not take those.  Warps of their own then write what that attention works through: `items`, of `item_tokens` tokens of a sequence each.
+// reaches); they lie one after the other, `count` tiles of 64 tokens, in which rows behind a sequence's last token are left as they are.  Warps of their own
+// write what that attention works through: `items`, of `item_tokens` tokens of a sequence each.
 struct Unpack {
   const unsigned char* pages;
   int num_pages, nkv, ps;
   const int *block_table, *kv_lens, *cu_seqlens;
-  int max_pages, num_seqs, max_len, least, window, keep_first, count, width, out_ps;  // out_ps: tokens of a page that is written
+  int max_pages, num_seqs, max_len, least, window, keep_first, count, width;
   int item_tokens, num_items;
-  int4* items;  // [num_items][2], see write_item
+  int4* items;  // [num_items + 1][2], see write_item
 };
+constexpr int TILE = 64;  // tokens
 
-// What sequence s brings: tokens (0: it does not count), length, and its pages that are written: 0 .. kept - 1 and skip .. last.
+// What sequence s brings: tokens (0: it does not count), length, and its tiles that are written: 0 .. kept - 1 and skip, skip + 1 ..
 struct UnpackSequence {
-  int tokens = 0, len = 0, kept = 0, skip = 0, pages = 0;
+  int tokens = 0, len = 0, kept = 0, skip = 0, tiles = 0;
   __device__ __forceinline__ UnpackSequence(const Unpack& a, int s) {
     if (s >= a.num_seqs) return;
     const int news = a.cu_seqlens[s + 1] - a.cu_seqlens[s];
@@ -327,9 +328,9 @@ struct UnpackSequence {
     if (news < a.least) return;
     tokens = news;
     if (len <= 0) return;
-    if (a.window > 0) skip = max(0, len - tokens - a.window + 1) / a.out_ps;
-    kept = min(skip, (a.keep_first + a.out_ps - 1) / a.out_ps);
-    pages = (len + a.out_ps - 1) / a.out_ps - skip + kept;
+    if (a.window > 0) skip = max(0, len - tokens - a.window + 1) / TILE;
+    kept = min(skip, (a.keep_first + TILE - 1) / TILE);
+    tiles = (len + TILE - 1) / TILE - skip + kept;
   }
 };
 __device__ __forceinline__ int warp_prefix(int n) {  // the sum up to and with this lane's
@@ -341,29 +342,29 @@ __device__ __forceinline__ int warp_prefix(int n) {  // the sum up to and with t
   return n;
 }
 
-// Item `w` of the attention, as {place in its sequence, the sequence's first token, its tokens, its length}, {its first page that is written, kept, skip}; place
-// -1: none.  Items stand by how many keys they see, in units of a tile, the heaviest first, so that the last blocks of the launch are short: where
+// Item `w` of the attention, as {place in its sequence, the sequence's first token, its tokens, its length}, {its first tile that is written, kept, skip}; place
+// -1: none.  The number behind the last item is zero: blocks of the attention count on it.  Items stand by how many keys they see, in units of a tile, the heaviest first, so that the last blocks of the launch are short: where
 // 1,500 + 701 + 1,000 tokens stand behind one another the attention takes ITEMS_NOW us, in the order of the sequences ITEMS_THEN.  An item's place follows from how many of each
 // sequence see more, which is a division, as they grow evenly.  By a warp.
 __device__ __forceinline__ void write_item(const Unpack& a, int w) {
   const int lane = threadIdx.x & 31, T = a.item_tokens;
   const int most = a.window > 0 ? a.window + a.keep_first + T : 0x7fffffff;  // keys that an item sees, roughly
-  int seq = -1, i = 0, before = 0, pages = 0;
+  int seq = -1, i = 0, before = 0, tiles_before = 0;
   int4 what = make_int4(-1, 0, 0, 0), where = make_int4(0, 0, 0, 0);
   for (int base = 0, left = w; base < a.num_seqs && seq < 0; base += 32) {
     const UnpackSequence s(a, base + lane);
-    const int n = (s.tokens + T - 1) / T, sum = warp_prefix(n), page_sum = warp_prefix(s.pages);
+    const int n = (s.tokens + T - 1) / T, sum = warp_prefix(n), tile_sum = warp_prefix(s.tiles);
     const uint32_t reach = __ballot_sync(0xffffffffu, sum > left);
     if (reach) {
       const int from = __ffs(reach) - 1;
       seq = base + from;
       i = left - __shfl_sync(0xffffffffu, sum - n, from);
       what = make_int4(i, a.cu_seqlens[seq], __shfl_sync(0xffffffffu, s.tokens, from), __shfl_sync(0xffffffffu, s.len, from));
-      where = make_int4(pages + __shfl_sync(0xffffffffu, page_sum - s.pages, from), __shfl_sync(0xffffffffu, s.kept, from),
+      where = make_int4(tiles_before + __shfl_sync(0xffffffffu, tile_sum - s.tiles, from), __shfl_sync(0xffffffffu, s.kept, from),
                         __shfl_sync(0xffffffffu, s.skip, from), 0);
     } else {
       left -= __shfl_sync(0xffffffffu, sum, 31);
-      pages += __shfl_sync(0xffffffffu, page_sum, 31);
+      tiles_before += __shfl_sync(0xffffffffu, tile_sum, 31);
     }
   }
   int at = w;  // (places behind the last item say so)
@@ -381,13 +382,14 @@ __device__ __forceinline__ void write_item(const Unpack& a, int w) {
     at = __reduce_add_sync(0xffffffffu, before);
   }
   if (lane == 0 && at < a.num_items) a.items[2 * at] = what, a.items[2 * at + 1] = where;
+  if (lane == 0 && w == 0) a.items[2 * a.num_items] = make_int4(0, 0, 0, 0);
 }
 
 __host__ __device__ __forceinline__ constexpr int unpack_rows(int D) { return 2048 / D; }  // of a page that a warp takes
 
-// Page `p` of the output (of a launch whose second axis is the sequences, without `cu_seqlens`).  Called by whole warps.
+// Page `p` of the output (of a launch whose second axis is the sequences), or with `cu_seqlens` tile `p`.  Called by whole warps.
 struct UnpackPage {
-  int seq, i;  // the sequence (-1: none) and its page
+  int seq, i;  // the sequence (-1: none) and its page (tile)
   __device__ __forceinline__ UnpackPage(const Unpack& a, int p) : seq(-1), i(0) {
     if (!a.cu_seqlens) {
       seq = blockIdx.y, i = p;
@@ -397,13 +399,13 @@ struct UnpackPage {
     const int lane = threadIdx.x & 31;
     for (int base = 0; base < a.num_seqs; base += 32) {
       const UnpackSequence s(a, base + lane);
-      const int sum = warp_prefix(s.pages);
+      const int sum = warp_prefix(s.tiles);
       const uint32_t reach = __ballot_sync(0xffffffffu, sum > p);
       if (reach) {
         const int from = __ffs(reach) - 1;
         seq = base + from;
         const int kept = __shfl_sync(0xffffffffu, s.kept, from), skip = __shfl_sync(0xffffffffu, s.skip, from);
-        i = p - __shfl_sync(0xffffffffu, sum - s.pages, from);
+        i = p - __shfl_sync(0xffffffffu, sum - s.tiles, from);
         if (i >= kept) i += skip - kept;
         return;
       }
@@ -452,17 +454,20 @@ template <typename T, int KNOWN> __global__ void __launch_bounds__(256) unpack_8
   }
   item -= a.num_items;
   const uint32_t half = item >> 1, pair = parts == 1 ? half : half / parts;
-  const int is_v = item & 1, part = (int)(half - pair * parts), p = (int)(pair / a.nkv), kvh = (int)(pair - p * a.nkv);
+  const int is_v = item & 1, part = (int)(half - pair * parts), kvh = (int)(pair % a.nkv), in_all = (int)(pair / a.nkv);
+  const int per_tile = a.cu_seqlens ? TILE / a.ps : 1, p = in_all / per_tile, in_tile = in_all - p * per_tile;  // (the page size divides a tile)
   if (p >= (a.cu_seqlens ? a.count : a.width)) return;
-  const UnpackPage at_page(a, p);
+  UnpackPage at_page(a, p);
   if (at_page.seq < 0) return;
+  at_page.i = at_page.i * per_tile + in_tile;
+  if (a.cu_seqlens && at_page.i * a.ps >= min(a.kv_lens[at_page.seq], a.max_len)) return;
   const int place = a.cu_seqlens ? p : blockIdx.y * a.width + p;
   int page;
   const int row0 = part * unpack_rows(D), rows = at_page.rows(a, &page) - row0;  // those that count, from the part's first on
   const Q8Page L(D, a.ps);
   const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
   const unsigned char* from = rec + (is_v ? L.values : 0) + (long)row0 * D;
-  T* to = (is_v ? v_out : k_out) + (((long)place * a.nkv + kvh) * a.ps + row0) * D;
+  T* to = (is_v ? v_out : k_out) + (((long)place * a.nkv + kvh) * per_tile * a.ps + in_tile * a.ps + row0) * D;
   const float scale = rows > 0 ? reinterpret_cast<const float*>(rec + L.scales)[is_v] : 0.f;
   const int count = min(unpack_rows(D), a.ps - row0) * words, live = rows * words;
   for (int first = lane; first < count; first += 32 * AT_ONCE) {
@@ -487,8 +492,8 @@ template <typename T, int KNOWN> __global__ void __launch_bounds__(256) unpack_8
   }
 }
 
-// Into pages of 16 tokens, whatever the cache's: a warp per (page that is written, kv head, keys or values), a lane of the first 16 looks a token up.
-constexpr int OTHER_PAGE = 16;
+// Into tiles, whatever the pages' size: a warp per (quarter of a tile, kv head, keys or values), a lane of the first 16 looks a token up.
+constexpr int QUARTER = TILE / 4;
 template <typename T> __global__ void __launch_bounds__(256) unpack_8bit_other_kernel(Unpack a, int D, T* __restrict__ k_out, T* __restrict__ v_out) {
   constexpr int CHANNELS = 16 / sizeof(T);
   const int words = D / CHANNELS, mask = q8_mask(D);
@@ -502,15 +507,15 @@ template <typename T> __global__ void __launch_bounds__(256) unpack_8bit_other_k
   }
   item -= a.num_items;
   const uint32_t half = item >> 1;
-  const int is_v = item & 1, p = (int)(half / a.nkv), kvh = (int)(half - (uint32_t)p * a.nkv);
+  const int is_v = item & 1, quarter = (int)(half / a.nkv), p = quarter / 4, kvh = (int)(half - (uint32_t)quarter * a.nkv);
   const UnpackPage at_page(a, p);
   if (at_page.seq < 0) return;
   const Q8Page L(D, a.ps);
   // where this lane's token lies, a multiple of 16, and below that how its pieces are ordered; 0: nowhere
   unsigned long long where = 0;
   float scale = 0.f;
-  const int key = at_page.i * OTHER_PAGE + lane, in_page = key / a.ps;
-  if (lane < OTHER_PAGE && key < min(a.kv_lens[at_page.seq], a.max_len) && in_page < a.max_pages) {
+  const int key = at_page.i * TILE + quarter % 4 * QUARTER + lane, in_page = key / a.ps;
+  if (lane < QUARTER && key < min(a.kv_lens[at_page.seq], a.max_len) && in_page < a.max_pages) {
     const int page = a.block_table[(long)at_page.seq * a.max_pages + in_page], row = key - in_page * a.ps;
     if (page >= 0 && page < a.num_pages) {
       const unsigned char* rec = a.pages + ((long)page * a.nkv + kvh) * L.record;
@@ -518,9 +523,9 @@ template <typename T> __global__ void __launch_bounds__(256) unpack_8bit_other_k
       where = reinterpret_cast<unsigned long long>(rec + (is_v ? L.values : 0) + (long)row * D) | (uint32_t)(row & mask);
     }
   }
-  T* to = (is_v ? v_out : k_out) + ((long)p * a.nkv + kvh) * OTHER_PAGE * D;
+  T* to = (is_v ? v_out : k_out) + (((long)p * a.nkv + kvh) * TILE + quarter % 4 * QUARTER) * D;
 #pragma unroll 4
-  for (int at = lane; at < OTHER_PAGE * words; at += 32) {  // (a whole number of warps)
+  for (int at = lane; at < QUARTER * words; at += 32) {  // (a whole number of warps)
     const int row = at / words, channel = CHANNELS * (at - row * words);
     const unsigned long long from = __shfl_sync(0xffffffffu, where, row);
     const float s = __shfl_sync(0xffffffffu, scale, row);
@@ -539,10 +544,10 @@ template <typename T> __global__ void __launch_bounds__(256) unpack_8bit_other_k
 }
 
 template <typename T> cudaError_t launch_unpack(const Unpack& a, int D, T* k_out, T* v_out, cudaStream_t stream) {
-  if (a.out_ps != a.ps)
-    return launch_pdl(unpack_8bit_other_kernel<T>, dim3((unsigned)((2L * a.count * a.nkv + a.num_items + 7) / 8)), dim3(256), 0, stream, a, D, k_out, v_out);
+  if (a.cu_seqlens && TILE % a.ps)
+    return launch_pdl(unpack_8bit_other_kernel<T>, dim3((unsigned)((8L * a.count * a.nkv + a.num_items + 7) / 8)), dim3(256), 0, stream, a, D, k_out, v_out);
   const int parts = (a.ps + unpack_rows(D) - 1) / unpack_rows(D);
-  const long items = 2L * (a.cu_seqlens ? a.count : a.width) * a.nkv * parts + a.num_items;
+  const long items = 2L * (a.cu_seqlens ? a.count * (TILE / a.ps) : a.width) * a.nkv * parts + a.num_items;
   const dim3 grid((unsigned)((items + 7) / 8), a.cu_seqlens ? 1 : a.num_seqs);
   if (D == 64) return launch_pdl(unpack_8bit_kernel<T, 64>, grid, dim3(256), 0, stream, a, D, parts, k_out, v_out);
   if (D == 128) return launch_pdl(unpack_8bit_kernel<T, 128>, grid, dim3(256), 0, stream, a, D, parts, k_out, v_out);
@@ -617,22 +622,21 @@ Q3_EXPORT int q3_store_8bit(int dtype, const void* qkv, int row_stride, void* q_
   return q3_launch_status();
 }
 
-// `cu_seqlens` null: num_seqs * width pages are written, as large as the cache's; else `count` pages of out_ps tokens and `num_items` items (struct Unpack).
+// `cu_seqlens` null: num_seqs * width pages are written, as large as the cache's; else `count` tiles of 64 tokens and `num_items` items (struct Unpack).
 Q3_EXPORT int q3_unpack_8bit(int dtype, const void* pages, int num_pages, int nkv, int D, int ps, const int* block_table, int max_pages,
                              const int* kv_lens, int num_seqs, int max_len, const int* cu_seqlens, int least, int window, int keep_first,
-                             int count, int width, int out_ps, void* k_out, void* v_out, int item_tokens, int num_items, void* items,
+                             int count, int width, void* k_out, void* v_out, int item_tokens, int num_items, void* items,
                              cudaStream_t stream) {
   if (num_seqs < 1 || (cu_seqlens ? count : width) < 1) return Q3_OK;
   if (!pages || !block_table || !kv_lens || !k_out || !v_out || nkv < 1 || max_pages < 1 || !q8_sizes_ok(D, ps)) return Q3_ERR_ARGUMENT;
   if (cu_seqlens ? !items || item_tokens < 1 || num_items < 0 || least < 1 || keep_first < 0 || window + (long)keep_first > 1 << 30 || !q8_aligned(items)
                  : num_items != 0)
     return Q3_ERR_ARGUMENT;
-  if (out_ps != ps && (!cu_seqlens || out_ps != OTHER_PAGE)) return Q3_ERR_ARGUMENT;
   if (dtype != Q3_DTYPE_F32 && dtype != Q3_DTYPE_BF16) return Q3_ERR_ARGUMENT;
   if ((!cu_seqlens && num_seqs > 65535) || !q8_aligned(pages) || !q8_aligned(k_out) || !q8_aligned(v_out)) return Q3_ERR_UNSUPPORTED;
-  if ((long)(cu_seqlens ? count : width) * 2 * nkv * ((ps + unpack_rows(D) - 1) / unpack_rows(D)) + num_items > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
+  if ((long)(cu_seqlens ? (long)count * (TILE % ps ? 4 : TILE / ps) : width) * 2 * nkv * ((ps + unpack_rows(D) - 1) / unpack_rows(D)) + num_items > 0x7fffffffL) return Q3_ERR_UNSUPPORTED;
   const Unpack a{(const unsigned char*)pages, num_pages, nkv, ps, block_table, kv_lens, cu_seqlens, max_pages, num_seqs, max_len, least, window,
-                 keep_first, count, width, out_ps, item_tokens, num_items, (int4*)items};
+                 keep_first, count, width, item_tokens, num_items, (int4*)items};
   const cudaError_t err = dtype == Q3_DTYPE_F32 ? launch_unpack(a, D, (float*)k_out, (float*)v_out, stream)
                                                 : launch_unpack(a, D, (bf16*)k_out, (bf16*)v_out, stream);
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;

@@ -220,8 +220,6 @@ _SIGNATURES = {
         "q3_paged_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, ctypes.c_long, c_void_p, c_int,
                                           c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                                           c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
-        "q3_window_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_int, c_int, c_int,
-                                           c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p],
         "q3_diff_attention_prefill_tc": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_long, c_void_p, c_int, c_void_p,
                                          c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
                                          c_float, c_float, c_float, c_void_p, c_void_p],
@@ -261,7 +259,11 @@ _SIGNATURES = {
                           c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int,
                           c_int, c_int, c_int, c_int, c_void_p, c_void_p],
         "q3_unpack_8bit": [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
-                           c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p],
+                           c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p],
+    },
+    "prompts_tiles_8bit": {
+        "q3_prompts_tiles_8bit": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float,
+                                  c_int, c_int, c_void_p, c_void_p],
     },
     "attention_8bit": {
         "q3_decode_attention_8bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -2633,7 +2635,7 @@ class CudaOps:
         if self.timing is not None:
             self._costs(2 * k.numel() * k.element_size() + B * n * num_kv_heads * eight_bit_page_bytes(head_dim, page_size))
         self._call("cache_8bit", "q3_unpack_8bit", what, _dtype_code(dtype), pages.data_ptr(), pages.shape[0], num_kv_heads, head_dim,
-                   page_size, block_table.data_ptr(), width, _ptr(kv_lens), B, int(max_kv_len), None, 0, 0, 0, 0, n, page_size, k.data_ptr(),
+                   page_size, block_table.data_ptr(), width, _ptr(kv_lens), B, int(max_kv_len), None, 0, 0, 0, 0, n, k.data_ptr(),
                    v.data_ptr(), 0, 0, None)
         return k, v
 
@@ -2645,7 +2647,7 @@ class CudaOps:
         read the codes as they are, on the tensor cores; float32, other single tokens of up to 8 query heads a kv head, and rows that do not
         begin at 16 bytes, on the FMA pipes (csrc/attention_8bit.cu).  bfloat16 portions of prompts read the codes as well, turned to
         bfloat16 on the way (csrc/prompts_8bit.cu); longer ones of heads of 64 to 128 have their sequences' pages unpacked once (at most
-        ``UNPACK_BYTES`` at a time, or one sequence) and go through the tcgen05 kernel.  Both are exact up to the weights, which are rounded to
+        ``UNPACK_BYTES`` at a time, or one sequence) and go through the tcgen05 kernel (csrc/prompts_tiles_8bit.cu).  Both are exact up to the weights, which are rounded to
         bfloat16.  A table entry that is no page is read nowhere; the rows of a sequence that sees such a token are undefined, the others
         are not.  A key that is no number makes the rows none that see it; a value, its channel of them, and of its portion's other rows too (their weight
         for it is zero)."""
@@ -2702,16 +2704,15 @@ class CudaOps:
         if not (64 <= D <= 128 and H // G <= 128 and out_at & 15 == 0 and not step.decode_only
                 and self._prompts_unpacked(cu, lens, H // G, G, D, window, keep_first, least)):
             return self._prompts_8bit(q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first)
-        wide = page_size if page_size in (8, 16, 32, 64) else 16  # tokens of a page that is unpacked
-        counts = unpacked_pages_4bit(cu, lens, wide, window, least, exact, keep_first)
-        total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * wide * D)
+        counts = unpacked_pages_4bit(cu, lens, 64, window, least, exact, keep_first)  # tiles of 64 tokens
+        total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * 64 * D)
         if total <= limit:
             runs = [(0, len(counts), total)] if total else []
         else:
             runs = [(first, end, sum(counts[first:end])) for first, end in runs_within(counts, limit)]
         for first, end, count in runs:
             most = max([n for n, c in zip(lens[first:end], counts[first:end]) if c])
-            self._prompts_tc_8bit(q, q_stride, H, G, D, pages, block_table, step, least, first, end, count, most, out, page_size, wide, scale,
+            self._prompts_tc_8bit(q, q_stride, H, G, D, pages, block_table, step, least, first, end, count, most, out, page_size, scale,
                                   window, keep_first)
         return out
 
@@ -2744,9 +2745,9 @@ class CudaOps:
         tiles = -(-(min(max_len, window + most_new + keep_first) if window else max_len) // 64)
         return max(1, min(self.SM_COUNT * (2 if D <= 64 else 1) // blocks, tiles // 4, 32))
 
-    def _prompts_tc_8bit(self, q, q_stride, H, G, D, pages, block_table, step, least, first, end, count, longest, out, page_size, wide, scale,
+    def _prompts_tc_8bit(self, q, q_stride, H, G, D, pages, block_table, step, least, first, end, count, longest, out, page_size, scale,
                          window, keep_first):
-        """Attention of those of the step's sequences ``first .. end - 1`` that bring at least ``least`` tokens, whose ``count`` pages of ``wide`` tokens
+        """Attention of those of the step's sequences ``first .. end - 1`` that bring at least ``least`` tokens, whose ``count`` tiles of 64 tokens
         are unpacked for it (none of those has more than ``longest`` keys)."""
         cu, kv_lens, seqs = step.cu_seqlens, step.kv_lens, end - first
         news = [b - a for a, b in zip(step.host_cu_seqlens[first:end], step.host_cu_seqlens[first + 1:end + 1])]
@@ -2754,19 +2755,18 @@ class CudaOps:
             cu, kv_lens, block_table = cu[first:end + 1], kv_lens[first:end], block_table[first:end]
         per = 2 * (128 // (H // G))  # tokens of an item: two blocks of rows
         num_items = sum([-(-n // per) for n in news if n >= least])
-        k = torch.empty((2, count, G, wide, D), dtype=out.dtype, device=out.device)
+        k = torch.empty((2, count, G, 64, D), dtype=out.dtype, device=out.device)
         v_at = k.data_ptr() + k.numel()  # (half of its bytes)
-        items = torch.empty((num_items, 8), dtype=torch.int32, device=out.device)
+        items = torch.empty((num_items + 1, 8), dtype=torch.int32, device=out.device)
         if self.timing is not None:
-            self._costs(k.numel() * k.element_size() + count * wide * 2 * G * D)
+            self._costs(k.numel() * k.element_size() + count * 64 * 2 * G * D)
         self._call("cache_8bit", "q3_unpack_8bit", "unpack_8bit", _dtype_code(out.dtype), pages.data_ptr(), pages.size(0), G, D, page_size,
                    block_table.data_ptr(), block_table.size(1), kv_lens.data_ptr(), seqs, longest, cu.data_ptr(), least, window, keep_first, count, 0,
-                   wide, k.data_ptr(), v_at, per, num_items, items.data_ptr())
+                   k.data_ptr(), v_at, per, num_items, items.data_ptr())
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out, prompts=True))
-        self._call("attention_prefill_tc", "q3_window_attention_prefill_tc", "paged_attention_prefill_8bit", q.data_ptr(), q_stride, q.size(0),
-                   k.data_ptr(), v_at, count * G * wide, items.data_ptr(), out.data_ptr(), num_items, H, G, D, wide, float(scale), window, keep_first,
-                   self._error_word(out.device).data_ptr())
+        self._call("prompts_tiles_8bit", "q3_prompts_tiles_8bit", "paged_attention_tiles_8bit", q.data_ptr(), q_stride, q.size(0), k.data_ptr(), v_at,
+                   count, items.data_ptr(), num_items, out.data_ptr(), H, G, D, float(scale), window, keep_first, self._error_word(out.device).data_ptr())
 
     def _prompts_8bit(self, q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first):
         """Attention of the sequences that bring at least ``least`` tokens, straight over the codes (csrc/prompts_8bit.cu)."""

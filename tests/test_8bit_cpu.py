@@ -215,7 +215,7 @@ def test_tensors_on_another_device_are_refused():
 def test_which_kernels_attention_takes():
     f32, wide = dict(dtype=torch.float32), dict(H=34, G=2)
     decode, straight, general = "q3_decode_attention_8bit", "q3_prompts_attention_8bit", "q3_general_attention_8bit"
-    unpacked = ["q3_unpack_8bit", "q3_window_attention_prefill_tc"]
+    unpacked = ["q3_unpack_8bit", "q3_prompts_tiles_8bit"]
     assert call() == call(kv_longest=None, single_seqs=None) == [decode]
     assert call(kw=f32) == call((2, 3), f32) == [general]
     assert call(kw=dict(D=80)) == call(kw=dict(D=80, H=16)) == [general] and call(kw=dict(D=80, H=18)) == [straight]

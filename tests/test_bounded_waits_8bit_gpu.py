@@ -50,10 +50,10 @@ def test_prompts_under_a_window():
     c = p8.Cache(lens, G, D, page, seed=3)
     q = t8.queries(270, H, D, 1)
     step, dev, out = p8.step_of(new, lens, page), q.cuda(), torch.zeros((270, H * D), dtype=torch.bfloat16, device="cuda")
-    k, v = ops.unpack_8bit(c.pages.cuda(), block_table=c.table.cuda(), kv_lens=step.kv_lens, max_kv_len=400, dtype=torch.bfloat16, **t8.sizes(c))
-    items = t8.i32([[i, 70 * b, new[b], lens[b], 25 * b, 0, 0, 0] for b in range(2) for i in range(-(-new[b] // 64))])
-    launch = _build("attention_prefill_tc", "q3_window_attention_prefill_tc")
-    assert run(launch, dev.data_ptr(), H * D, 270, k.data_ptr(), v.data_ptr(), 50 * G * page, items.data_ptr(),
-               out.data_ptr(), len(items), H, G, D, page, D ** -0.5, 100, 20) == 2
+    k = torch.zeros((14, G, 64, D), dtype=torch.bfloat16, device="cuda")
+    v, items = k.clone(), t8.i32([*([i, 70 * b, new[b], lens[b], 7 * b, 0, 0, 0] for b in range(2) for i in range(-(-new[b] // 64))), [0] * 8])
+    launch = _build("prompts_tiles_8bit", "q3_prompts_tiles_8bit")
+    assert run(launch, dev.data_ptr(), H * D, 270, k.data_ptr(), v.data_ptr(), 14, items.data_ptr(), len(items) - 1, out.data_ptr(), H, G, D,
+               D ** -0.5, 100, 20) == 2
     got = t8.attend(ops, c, q, new, lens, H, D ** -0.5, window=100, keep_first=20)  # the ordinary build afterwards
     t8.check_rows(got, q.view(270, H, D), c, new, lens, D ** -0.5, window=100, keep_first=20, wide=True)
