@@ -2717,11 +2717,11 @@ class CudaOps:
         return out
 
     def _prompts_unpacked(self, cu, lens, R, G, D, window, keep_first, least=2) -> bool:
-        """Whether a step's portions are faster unpacked and on the tcgen05 kernel than straight over the codes.  Times in us, fitted to both at 150
-        random steps (one to eight portions of 2 to 1,000 tokens behind up to 8,000, 1 to 8 kv heads of 64, 96 and 128, groups of 2 to 16, windows) on a
-        B200: the choice is 1.5 % slower than the better one on average, 33 % at worst.  Straight, a block of 128 rows takes a tile of 64 keys of
-        128 channels in 4.1 of an SM, in 2.6 if it is by itself, and slices cost their joining; unpacked, the longest sequence's tiles take 0.66 each, one
-        after the other (a machine full of blocks hardly more at these sizes), and unpacking the bytes it moves."""
+        """Whether a step's portions are faster unpacked and on the tcgen05 kernel than straight over the codes.  Times in us, fitted to both at 220
+        random steps (one to eight portions of 2 to 1,000 tokens behind up to 8,000, 1 to 8 kv heads of 64 to 128, groups of 2 to 20, windows) on a
+        B200: the choice is 1.6 % slower than the better one on average, 63 % at worst.  Straight, a block of 128 rows takes a tile of 64 keys of
+        128 channels in 4 of an SM, in 2.6 if it is by itself, and slices cost their joining; unpacked, the longest sequence's tiles take 0.7 each, one
+        after the other, or all tiles 0.87 of an SM, and unpacking the bytes it moves."""
         work = chain = read = items = most = 0
         for b, kv in enumerate(lens):
             n = cu[b + 1] - cu[b]
@@ -2737,8 +2737,8 @@ class CudaOps:
             return False
         splits = self._prompt_splits(items * G, D, window, keep_first, most, max(lens))
         size = max(D, 64) / 128
-        straight = 5.7 + max(4.1 * work * G * size / self.SM_COUNT, 2.6 * chain * size / splits) + (5 + 0.67 * splits if splits > 1 else 0)
-        return 10.6 + 3.7e-6 * read * G * D + max(0.66 * chain, 0.08 * work * G / self.SM_COUNT) < straight
+        straight = 5.9 + max(4.0 * work * G * size / self.SM_COUNT, 2.6 * chain * size / splits) + (5.3 + 0.57 * splits if splits > 1 else 0)
+        return 10.8 + 1.5e-6 * read * G * D + max(0.7 * chain, 0.87 * work * G / self.SM_COUNT) < straight
 
     def _prompt_splits(self, blocks, D, window, keep_first, most_new, max_len) -> int:
         """Slices of the tiles of ``blocks`` blocks of rows: as many blocks as run at a time, each at least four tiles of 64 keys."""
