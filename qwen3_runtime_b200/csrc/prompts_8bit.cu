@@ -14,10 +14,10 @@
 // behind 4,000, 32 over 8 of 128: 39 (64); behind 16,000 91 (230).  Slices for more balance than idle SMs ask for, four blocks an SM: 84 for 89 with heads of 64, 230 for 192 with 256.
 #include "eight_bit.cuh"
 #include "mma_tiles.cuh"
+#include "prompt_slices.cuh"
 
 namespace {
 
-constexpr float MINUS_BIG = -3.402823466e+38f;  // the maximum of a row that has seen nothing: a hidden key's score, -inf, weighs 2^(-inf - MINUS_BIG) = 0
 constexpr int WARPS = 8, THREADS = 32 * WARPS, ROWS = 16 * WARPS;
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2^x to 2 units in the last place; below 2^-126 zero
@@ -34,7 +34,7 @@ struct Prompts {
   const int *block_table, *kv_lens, *cu_seqlens;
   int max_pages, num_seqs;
   bf16* out;
-  float *mid_o, *mid_ml;  // splits > 1: [tokens][nq][splits][D] and [tokens][nq][splits][2] (a maximum, and a sum that is 0 where there is nothing)
+  float *mid_o, *mid_ml;  // splits > 1: see PromptSlices
   int splits, items, least, nq, nkv, D, ps, shift, window, keep_first, max_len;  // shift: log2 of the page size, or -1
   float scale_log2;
 };
@@ -272,42 +272,6 @@ template <int KD> __global__ void __launch_bounds__(THREADS, KD <= 4 ? 2 : 1) pr
   }
 }
 
-// A warp per (token of a sequence that counts, head): joins the slices in order.
-__global__ void __launch_bounds__(128) prompts_8bit_merge_kernel(Prompts a, int tokens) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (at >= (long)tokens * a.nq) return;
-  const int t = (int)(at / a.nq);
-  // the token's sequence: whether it counts
-  bool mine = false;
-  for (int base = 0; base < a.num_seqs; base += 32) {
-    const int b = base + lane;
-    const bool in = b < a.num_seqs && a.cu_seqlens[b] <= t && t < a.cu_seqlens[b + 1] && a.cu_seqlens[b + 1] - a.cu_seqlens[b] >= a.least;
-    mine = mine || __any_sync(0xffffffffu, in);
-  }
-  if (!mine) return;
-  float top = MINUS_BIG;
-  for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.mid_ml[2 * (at * a.splits + s)]);
-  top = warp_max(top);
-  float den = 0.f, y[8] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.mid_ml + 2 * (at * a.splits + s));
-    if (ml.x == MINUS_BIG) continue;
-    const float f = exp2_fast(ml.x - top);
-    den += f * ml.y;
-    const float* o = a.mid_o + (at * a.splits + s) * a.D;
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-      if (lane + 32 * c < a.D) y[c] += f * o[lane + 32 * c];
-  }
-  const float inv = top == MINUS_BIG ? 0.f : 1.f / den;
-#pragma unroll
-  for (int c = 0; c < 8; ++c)
-    if (lane + 32 * c < a.D) a.out[at * a.D + lane + 32 * c] = __float2bfloat16_rn(y[c] * inv);
-}
-
 template <int KD> int launch_prompts(const Prompts& a, int tokens, cudaStream_t stream) {
   static bool once[Q3_MAX_DEVICES];
   const int dev = q3_current_device();
@@ -317,7 +281,7 @@ template <int KD> int launch_prompts(const Prompts& a, int tokens, cudaStream_t 
   }
   cudaError_t err = launch_pdl(prompts_8bit_kernel<KD>, dim3(a.items, a.nkv, a.splits), dim3(THREADS), Sizes<KD>::SMEM, stream, a);
   if (err == cudaSuccess && a.splits > 1)
-    err = launch_pdl(prompts_8bit_merge_kernel, dim3((unsigned)(((long)tokens * a.nq + 3) / 4)), dim3(128), 0, stream, a, tokens);
+    err = merge_prompts({a.mid_o, a.mid_ml, a.out, a.cu_seqlens, a.num_seqs, a.least, tokens, a.nq, a.D, a.splits}, stream);
   return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
 }
 

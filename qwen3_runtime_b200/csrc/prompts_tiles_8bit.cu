@@ -7,6 +7,8 @@
 //   * An item is a sequence's 2 x 128 rows (A and B; as many as whole tokens give) for one kv head.  Blocks stay: one an SM takes item after item from a
 //     list that begins with the heaviest (csrc/cache_8bit.cu writes it), the next one when the keys of the present one are all asked for.  Then the next
 //     item's queries, keys and first product come while the softmax ends the present one and writes its rows.
+//   * Where items would leave SMs idle (a portion behind a long context), each one's tiles are cut into slices, items of their own; a second kernel joins
+//     what they leave.
 //
 // What bounds it: 0.96 us a tile of both blocks (the softmax, as there), and what an item costs beside its tiles.  With a block of the launch for each item that
 // was 6.5 us (1.1 between two blocks, 0.5 for the item, 2.8 until the first scores, 2 to 2.6 at the end), now the end's.  us, with the unpacking, in blocks that
@@ -21,6 +23,7 @@
 #include <type_traits>
 
 #include "async_tiles.cuh"
+#include "prompt_slices.cuh"
 
 namespace {
 
@@ -43,6 +46,8 @@ struct Params {
   int num_items, nq, nkv, group, per, magic, head_dim, window, keep_first;  // per: tokens of a block; magic: 2^16 / group, rounded up
   float scale_log2;
   int* error_word;
+  int splits;
+  float *mid_o, *mid_ml;  // splits > 1: see PromptSlices
 };
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x; below 2^-126 zero, which is what a weight that small is worth
@@ -82,11 +87,11 @@ __device__ __forceinline__ void arrive_if(bool yes, uint32_t bar) {
       : "memory");
 }
 
-// An item, as all roles see it.  Its tokens are its sequence's tokens first .. ; tile j of its keys is tile `at(j)` of the sequence.
+// An item, as all roles see it.  Its tokens are its sequence's tokens first .. ; tile j of its keys (of this slice, its tile j + j0) is tile `at(j)` of the sequence.
 struct Item {
-  int kvh, tok0, q_len, base_pos, first, k_lo, p_last, firsts, skip, p_max[2], tiles[2], num_tiles, place, kept, gap;
+  int kvh, slice, tok0, q_len, base_pos, first, k_lo, p_last, firsts, skip, p_max[2], tiles[2], j0, num_tiles, place, kept, gap;
   __device__ __forceinline__ Item(const Params& p, const int4& what, const int4& where) {
-    kvh = where.w, tok0 = what.y, q_len = what.z, base_pos = what.w - what.z, first = 2 * p.per * what.x;
+    kvh = where.w & 0xffff, slice = where.w >> 16, tok0 = what.y, q_len = what.z, base_pos = what.w - what.z, first = 2 * p.per * what.x;
     k_lo = p.window > 0 ? max(0, base_pos + first - p.window + 1) : 0;
     const int tile0 = k_lo / BLOCK_N;
     firsts = min((p.keep_first + BLOCK_N - 1) / BLOCK_N, tile0), skip = tile0 - firsts;
@@ -96,11 +101,16 @@ struct Item {
       p_max[x] = begin < q_len ? base_pos + end - 1 : -1;
       tiles[x] = p_max[x] >= 0 ? p_max[x] / BLOCK_N + 1 - skip : 0;
     }
-    num_tiles = max(tiles[0], tiles[1]), p_last = max(p_max[0], p_max[1]);
+    num_tiles = max(tiles[0], tiles[1]), p_last = max(p_max[0], p_max[1]), j0 = 0;
+    if (p.splits > 1) {
+      const int per = (num_tiles + p.splits - 1) / p.splits;
+      j0 = slice * per;
+      tiles[0] = max(0, min(tiles[0] - j0, per)), tiles[1] = max(0, min(tiles[1] - j0, per)), num_tiles = max(tiles[0], tiles[1]);
+    }
     place = where.x, kept = where.y, gap = where.z - where.y;
   }
   __device__ __forceinline__ int tiles_of(int x) const { return x ? tiles[1] : tiles[0]; }  // (an index would put them into local memory)
-  __device__ __forceinline__ int at(int j) const { return j + (j >= firsts ? skip : 0); }
+  __device__ __forceinline__ int at(int j) const { return j + j0 + (j + j0 >= firsts ? skip : 0); }
   __device__ __forceinline__ int row(const Params& p, int j) const {  // of the unpacked tiles, as rows
     const int t = at(j);
     return ((place + t - (t < kept ? 0 : gap)) * p.nkv + kvh) * BLOCK_N;
@@ -171,15 +181,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
   };
 
   if (warp == 0) {  // ---- items, and their keys
-    const int units = p.num_items * p.nkv;  // item by item, the kv heads of each
+    const int each = p.nkv * p.splits, units = p.num_items * each;  // item by item, the slices of each, the kv heads of each
     int unit = blockIdx.x, c = 0;
     bool ok = true;
     for (;; ++n) {
       what = make_int4(-1, 0, 0, 0), where = make_int4(0, 0, 0, 0);
       if (unit < units) {  // (an item that is none: the list's end)
-        const int item = unit / p.nkv;
+        const int item = unit / each, rest = unit - item * each, slice = rest / p.nkv;
         what = p.items[2 * item], where = p.items[2 * item + 1];
-        where.w = unit - item * p.nkv;
+        where.w = rest - slice * p.nkv + (slice << 16);
       }
       const int slot = n & 1;
       ok = __all_sync(0xffffffffu, mbar_wait(bar(ITEM_EMPTY + slot), ((n >> 1) & 1) ^ 1, &abort_flag));
@@ -431,8 +441,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
       int whole0 = 1, whole1 = 0;  // such tiles behind the first one
       if (my_tiles) {
         const int lo_last = p.window > 0 ? max(0, (x ? it.p_max[1] : it.p_max[0]) - p.window + 1) : 0;
-        whole0 = max(1, (max(lo_last, it.k_lo) + BLOCK_N - 1) / BLOCK_N - it.skip);
-        whole1 = min(my_tiles, (it.base_pos + it.first + x * p.per + 1) / BLOCK_N - it.skip);
+        whole0 = max(1, (max(lo_last, it.k_lo) + BLOCK_N - 1) / BLOCK_N - it.skip - it.j0);
+        whole1 = min(my_tiles, (it.base_pos + it.first + x * p.per + 1) / BLOCK_N - it.skip - it.j0);
       }
       for (int j = 0; j < my_tiles && ok; ++j) {
         if (j < whole0 || j >= whole1) {
@@ -445,13 +455,37 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
       c += my_tiles, tiles_before += it.num_tiles;
       if (ok && my_tiles) ok = wait(bar(PV_FULL + x), (c - 1) & 1, &abort_flag);
       ok = __all_sync(0xffffffffu, ok);
+      const long at = (long)(it.tok0 + tok) * p.nq + it.kvh * p.group + head, at_slice = at * p.splits + it.slice;
+      if (ok && p.splits > 1 && row_ok)
+        *reinterpret_cast<float2*>(p.mid_ml + 2 * at_slice) = m_ref == -INFINITY ? make_float2(MINUS_BIG, 0.f) : make_float2(fmaxf(m_ref * scale_log2, -3e38f), l_run);
       if (!ok || !my_tiles) continue;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      // Out by way of shared memory, 64 columns at a time, so that a warp writes whole rows.
-      const float inv = 1.f / l_run;
+      // Out by way of shared memory, 128 bytes of a row at a time, so that a warp writes whole rows.
       unsigned char* mine = out_s + x * STAGE_OUT + quarter * 32 * 128;
-      const unsigned long long dst =
-          row_ok ? reinterpret_cast<unsigned long long>(p.out + ((long)(it.tok0 + tok) * p.nq + it.kvh * p.group + head) * p.head_dim) : 0;
+      if (p.splits > 1) {  // as it is, for the kernel that joins the slices
+        const unsigned long long dst = row_ok ? reinterpret_cast<unsigned long long>(p.mid_o + at_slice * p.head_dim) : 0;
+#pragma unroll 1
+        for (int c0 = 0; c0 < p.head_dim; c0 += 32) {
+          uint32_t ov[32];
+          tmem_load32(o_addr + c0, ov);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch)
+            *reinterpret_cast<uint4*>(mine + lane * 128 + 16 * (ch ^ (lane & 7))) = make_uint4(ov[4 * ch], ov[4 * ch + 1], ov[4 * ch + 2], ov[4 * ch + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row = 4 * i + (lane >> 3), piece = lane & 7;
+            float* to = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, dst, row));
+            if (to && c0 + 4 * piece < p.head_dim) *reinterpret_cast<uint4*>(to + c0 + 4 * piece) = *reinterpret_cast<const uint4*>(mine + row * 128 + 16 * (piece ^ (row & 7)));
+          }
+          __syncwarp();
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        continue;
+      }
+      const float inv = 1.f / l_run;
+      const unsigned long long dst = row_ok ? reinterpret_cast<unsigned long long>(p.out + at * p.head_dim) : 0;
 #pragma unroll 1
       for (int c0 = 0; c0 < p.head_dim; c0 += 64) {
         uint32_t ov[2][32];
@@ -509,14 +543,18 @@ bool q_map(CUtensorMap* map, const void* q, int cols, int nq, long num_tokens, l
 
 // q [num_tokens, *] bfloat16, head h at column h * head_dim.  k, v [tiles][nkv][64][head_dim].  `items` [num_items + 1][2]: the blocks' work in the order in
 // which it is taken, as csrc/cache_8bit.cu writes it; the last one's first number is zero, and counts.  out [num_tokens, nq * head_dim]: the rows of the items.
-// window > 0: a token sees the last `window` keys up to itself, and the sequence's first `keep_first`.  error_word: set to 2 if a wait expired.
+// window > 0: a token sees the last `window` keys up to itself, and the sequence's first `keep_first`.  splits > 1: each item in so many slices, with
+// mid_o and mid_ml (PromptSlices) as scratch and the sequences that the items are of.  error_word: set to 2 if a wait expired.
 Q3_EXPORT int q3_prompts_tiles_8bit(const void* q, int q_stride, int num_tokens, const void* k, const void* v, int tiles, void* items, int num_items, void* out,
-                                    int nq, int nkv, int head_dim, float scale, int window, int keep_first, int* error_word, cudaStream_t stream) {
+                                    int nq, int nkv, int head_dim, float scale, int window, int keep_first, int splits, float* mid_o, float* mid_ml,
+                                    const int* cu_seqlens, int num_seqs, int least, int* error_word, cudaStream_t stream) {
   if (num_items < 1 || tiles < 1 || num_tokens < 1) return Q3_OK;
-  if (!q || !k || !v || !items || !out || nq < 1 || nkv < 1 || nq % nkv || window < 0 || keep_first < 0) return Q3_ERR_ARGUMENT;
+  if (!q || !k || !v || !items || !out || nq < 1 || nkv < 1 || nq % nkv || window < 0 || keep_first < 0 || splits < 1 ||
+      (splits > 1 && (!mid_o || !mid_ml || !cu_seqlens || num_seqs < 1 || least < 1)))
+    return Q3_ERR_ARGUMENT;
   const int group = nq / nkv;
   if (head_dim < 64 || head_dim > 128 || head_dim % 16 || group > BLOCK_M || q_stride % 8 || (long)tiles * nkv * BLOCK_N > 0x7fffffffL ||
-      (long)num_items * nkv > 0x3fffffffL || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)items) & 15))
+      nkv > 0xffff || splits > 0x7fff || (long)num_items * nkv * splits > 0x3fffffffL || (long)num_tokens * nq > 0x7fffffffL || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)items) & 15))
     return Q3_ERR_UNSUPPORTED;
   CUtensorMap tq, tk, tv;
   const long rows = (long)tiles * nkv * BLOCK_N;
@@ -532,7 +570,9 @@ Q3_EXPORT int q3_prompts_tiles_8bit(const void* q, int q_stride, int num_tokens,
       return Q3_ERR_LAUNCH;
   }
   const Params p = {(int4*)items, (bf16*)out, num_items, nq, nkv, group, BLOCK_M / group, (65536 + group - 1) / group, head_dim, window, window > 0 ? keep_first : 0,
-                    scale * LOG2_E, error_word};
-  const int units = num_items * nkv, blocks = units < sms_of[dev] ? units : sms_of[dev];
-  return launch_pdl(prompts_tiles_kernel, dim3(blocks), dim3(THREADS), SMEM, stream, tq, tk, tv, p) == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
+                    scale * LOG2_E, error_word, splits, mid_o, mid_ml};
+  const int units = num_items * nkv * splits, blocks = units < sms_of[dev] ? units : sms_of[dev];
+  cudaError_t err = launch_pdl(prompts_tiles_kernel, dim3(blocks), dim3(THREADS), SMEM, stream, tq, tk, tv, p);
+  if (err == cudaSuccess && splits > 1) err = merge_prompts({mid_o, mid_ml, (bf16*)out, cu_seqlens, num_seqs, least, num_tokens, nq, head_dim, splits}, stream);
+  return err == cudaSuccess ? Q3_OK : Q3_ERR_LAUNCH;
 }

@@ -263,7 +263,7 @@ _SIGNATURES = {
     },
     "prompts_tiles_8bit": {
         "q3_prompts_tiles_8bit": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float,
-                                  c_int, c_int, c_void_p, c_void_p],
+                                  c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p],
     },
     "attention_8bit": {
         "q3_decode_attention_8bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -2745,6 +2745,21 @@ class CudaOps:
         tiles = -(-(min(max_len, window + most_new + keep_first) if window else max_len) // 64)
         return max(1, min(self.SM_COUNT * (2 if D <= 64 else 1) // blocks, tiles // 4, 32))
 
+    def _tile_splits(self, items, longest, most_new, window, keep_first) -> int:
+        """The same for the tcgen05 kernel: its blocks, one an SM, each at least eight tiles."""
+        tiles = -(-(min(longest, window + most_new + keep_first) if window else longest) // 64)
+        return max(1, min(self.SM_COUNT // items, tiles // 8, 16))
+
+    def _slices_of_prompts(self, rows, D, splits, device):
+        """``splits``, fewer where there would be more to keep of the slices than 256 MB; scratch for them (to be held until the launch), and where the
+        results, and the maxima and sums, of so many slices of ``rows`` lie in it."""
+        splits = max(1, min(splits, (1 << 26) // (rows * D)))
+        if splits == 1:
+            return 1, None, None, None
+        mid = torch.empty(rows * splits * (D + 2), dtype=torch.float32, device=device)
+        self.launches += 1
+        return splits, mid, mid.data_ptr(), mid.data_ptr() + 4 * rows * splits * D
+
     def _prompts_tc_8bit(self, q, q_stride, H, G, D, pages, block_table, step, least, first, end, count, longest, out, page_size, scale,
                          window, keep_first):
         """Attention of those of the step's sequences ``first .. end - 1`` that bring at least ``least`` tokens, whose ``count`` tiles of 64 tokens
@@ -2758,6 +2773,8 @@ class CudaOps:
         k = torch.empty((2, count, G, 64, D), dtype=out.dtype, device=out.device)
         v_at = k.data_ptr() + k.numel()  # (half of its bytes)
         items = torch.empty((num_items + 1, 8), dtype=torch.int32, device=out.device)
+        splits = self._tile_splits(num_items * G, longest, max(news), window, keep_first)
+        splits, mid, mid_o, mid_ml = self._slices_of_prompts(q.size(0) * H, D, splits, out.device)
         if self.timing is not None:
             self._costs(k.numel() * k.element_size() + count * 64 * 2 * G * D)
         self._call("cache_8bit", "q3_unpack_8bit", "unpack_8bit", _dtype_code(out.dtype), pages.data_ptr(), pages.size(0), G, D, page_size,
@@ -2766,7 +2783,8 @@ class CudaOps:
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out, prompts=True))
         self._call("prompts_tiles_8bit", "q3_prompts_tiles_8bit", "paged_attention_tiles_8bit", q.data_ptr(), q_stride, q.size(0), k.data_ptr(), v_at,
-                   count, items.data_ptr(), num_items, out.data_ptr(), H, G, D, float(scale), window, keep_first, self._error_word(out.device).data_ptr())
+                   count, items.data_ptr(), num_items, out.data_ptr(), H, G, D, float(scale), window, keep_first, splits, mid_o, mid_ml, cu.data_ptr(), seqs,
+                   least, self._error_word(out.device).data_ptr())
 
     def _prompts_8bit(self, q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first):
         """Attention of the sequences that bring at least ``least`` tokens, straight over the codes (csrc/prompts_8bit.cu)."""
@@ -2776,13 +2794,7 @@ class CudaOps:
         if not items:
             return out
         splits = self._prompt_splits(items * G, D, window, keep_first, max(news), max_len)
-        splits = max(1, min(splits, (1 << 26) // (T * H * D)))  # (no more to keep of the slices than 256 MB)
-        mid_o = mid_ml = None
-        if splits > 1:
-            mid = torch.empty(T * H * splits * (D + 2), dtype=torch.float32, device=out.device)
-            mid_o = mid.data_ptr()
-            mid_ml = mid_o + 4 * T * H * splits * D
-            self.launches += 1
+        splits, mid, mid_o, mid_ml = self._slices_of_prompts(T * H, D, splits, out.device)
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out, prompts=None if least < 2 else True))
         self._call("prompts_8bit", "q3_prompts_attention_8bit", "paged_attention_prompts_8bit", q_at, q_stride, pages.data_ptr(), pages.size(0),

@@ -54,6 +54,6 @@ def test_prompts_under_a_window():
     v, items = k.clone(), t8.i32([*([i, 70 * b, new[b], lens[b], 7 * b, 0, 0, 0] for b in range(2) for i in range(-(-new[b] // 64))), [0] * 8])
     launch = _build("prompts_tiles_8bit", "q3_prompts_tiles_8bit")
     assert run(launch, dev.data_ptr(), H * D, 270, k.data_ptr(), v.data_ptr(), 14, items.data_ptr(), len(items) - 1, out.data_ptr(), H, G, D,
-               D ** -0.5, 100, 20) == 2
+               D ** -0.5, 100, 20, 1, None, None, None, 2, 1) == 2
     got = t8.attend(ops, c, q, new, lens, H, D ** -0.5, window=100, keep_first=20)  # the ordinary build afterwards
     t8.check_rows(got, q.view(270, H, D), c, new, lens, D ** -0.5, window=100, keep_first=20, wide=True)
