@@ -2717,12 +2717,12 @@ class CudaOps:
         return out
 
     def _prompts_unpacked(self, cu, lens, R, G, D, window, keep_first, least=2) -> bool:
-        """Whether a step's portions are faster unpacked and on the tcgen05 kernel than straight over the codes.  Times in us, fitted to both at 220
-        random steps (one to eight portions of 2 to 1,000 tokens behind up to 8,000, 1 to 8 kv heads of 64 to 128, groups of 2 to 20, windows) on a
-        B200: the choice is 1.6 % slower than the better one on average, 63 % at worst.  Straight, a block of 128 rows takes a tile of 64 keys of
-        128 channels in 4 of an SM, in 2.6 if it is by itself, and slices cost their joining; unpacked, the longest sequence's tiles take 0.7 each, one
-        after the other, or all tiles 0.87 of an SM, and unpacking the bytes it moves."""
-        work = chain = read = items = most = 0
+        """Whether a step's portions are faster unpacked and on the tcgen05 kernel than straight over the codes.  Times in us, fitted to both at 300
+        random steps (one to eight portions of 2 to 1,000 tokens behind up to 30,000, 1 to 8 kv heads of 64 to 128, groups of 2 to 20, windows) on a
+        B200: the choice is 1.4 % slower than the better one on average, 44 % at worst.  Straight, a block of 128 rows takes a tile of 64 keys of
+        128 channels in 4.2 of an SM, in 2.6 if it is by itself, and slices cost their joining; unpacked, the longest sequence's tiles take 0.74 each, one
+        after the other, or all tiles 0.65 of an SM, slices their joining, and unpacking the bytes it moves."""
+        work = chain = read = items = pairs = most = 0
         for b, kv in enumerate(lens):
             n = cu[b + 1] - cu[b]
             if n < least:
@@ -2733,12 +2733,15 @@ class CudaOps:
             chain = max(chain, (min(seen, window + 256 // R + keep_first) if window else kv) / 64 + 1)
             read += seen
             items += rows
+            pairs += -(-n // (2 * (128 // R)))
         if not items:
             return False
         splits = self._prompt_splits(items * G, D, window, keep_first, most, max(lens))
         size = max(D, 64) / 128
-        straight = 5.9 + max(4.0 * work * G * size / self.SM_COUNT, 2.6 * chain * size / splits) + (5.3 + 0.57 * splits if splits > 1 else 0)
-        return 10.8 + 1.5e-6 * read * G * D + max(0.7 * chain, 0.87 * work * G / self.SM_COUNT) < straight
+        straight = 6.4 + max(4.2 * work * G * size / self.SM_COUNT, 2.6 * chain * size / splits) + (5.7 + 0.2 * splits if splits > 1 else 0)
+        splits = self._tile_splits(pairs * G, max(lens), most, window, keep_first)
+        unpacked = max(0.74 * chain / splits, 0.65 * work * G / self.SM_COUNT) + (4.6 + 0.33 * splits if splits > 1 else 0)
+        return 9 + 2.5 * D / 128 + 1.3e-6 * read * G * D + unpacked < straight
 
     def _prompt_splits(self, blocks, D, window, keep_first, most_new, max_len) -> int:
         """Slices of the tiles of ``blocks`` blocks of rows: as many blocks as run at a time, each at least four tiles of 64 keys."""

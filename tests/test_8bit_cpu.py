@@ -231,14 +231,27 @@ def test_which_kernels_attention_takes():
 
 
 def test_which_portions_are_unpacked():
-    """Long ones; few rows behind a long context are not, nor prompts of a few tokens."""
+    """Long ones and those behind long contexts; prompts of a few tokens are not."""
     ops = Here()
     ops.SM_COUNT = 148
     cases = lambda news, kvs, D=128, window=0, first=0, group=4: ops._prompts_unpacked(  # noqa: E731
         [sum(news[:b]) for b in range(len(news) + 1)], kvs, group, 8, D, window, first)
-    assert cases([2048], [2048]) and cases([512, 1, 700], [512, 9000, 900]) and cases([2048], [2048], 64) and cases([256], [4256])
-    assert not cases([16], [16]) and not cases([64], [16064]) and not cases([2, 1, 3], [1000, 5, 1003]) and not cases([1, 1], [9, 9])
-    assert cases([2048], [9000], window=1024, first=4) and not cases([16], [30000])
+    assert cases([2048], [2048]) and cases([512, 1, 700], [512, 9000, 900]) and cases([2048], [2048], 64) and cases([256], [4256]) and cases([64], [16064])
+    assert not cases([16], [16]) and not cases([2, 1, 3], [1000, 5, 1003]) and not cases([1, 1], [9, 9])
+    assert cases([2048], [9000], window=1024, first=4)
+
+
+def test_slices_of_prompts():
+    """No more items than SMs by slices, each of at least eight tiles (a block of 128 rows: four); no more to keep of them than 256 MB."""
+    ops = Here()
+    ops.SM_COUNT = 148
+    assert [ops._tile_splits(n, 16384, 64, 0, 0) for n in (1, 8, 74, 75, 148, 500)] == [16, 16, 2, 1, 1, 1]
+    assert [ops._tile_splits(8, n, 64, 0, 0) for n in (1, 64, 1000, 1024, 3000)] == [1, 1, 2, 2, 5]
+    assert ops._tile_splits(8, 16384, 64, 1000, 24) == 2 and ops._prompt_splits(8, 128, 1000, 24, 64, 16384) == 4
+    assert [ops._prompt_splits(8, D, 0, 0, 64, 16384) for D in (64, 128)] == [32, 18]
+    splits, mid, o, ml = ops._slices_of_prompts(2048, 128, 400, "cpu")
+    assert splits == 256 and mid.numel() == 2048 * 256 * 130 and o == mid.data_ptr() and ml == o + 4 * 2048 * 256 * 128
+    assert ops._slices_of_prompts(1 << 20, 128, 7, "cpu") == (1, None, None, None)
 
 
 def test_unpacking_more_than_the_table_holds_is_refused(ops):

@@ -40,14 +40,15 @@ def test_portions(ops, form, H, G, D, page, window, keep_first):  # noqa: F811
     check_form(form, D)
 
 
-@pytest.mark.parametrize("H,G,D", [(20, 4, 80), (40, 2, 128), (8, 2, 128), (2, 1, 256)])
-def test_a_long_prompt_of_many_slices(ops, form, H, G, D):  # noqa: F811
-    """One portion behind thousands of tokens: slices whose joining has many parts."""
-    new, lens = [37], [4021]
+@pytest.mark.parametrize("window,keep_first", [(None, 0), (2000, 70)])
+@pytest.mark.parametrize("new,lens", [([37], [4021]), ([5, 37, 1, 60, 3], [40, 3021, 900, 64, 1500])])
+@pytest.mark.parametrize("H,G,D", [(20, 4, 80), (40, 2, 128), (8, 2, 128), (6, 3, 64), (2, 1, 256)])
+def test_portions_behind_long_contexts(ops, form, H, G, D, new, lens, window, keep_first):  # noqa: F811
+    """One portion behind thousands of tokens, by itself and among others that have a key for the first of its slices alone."""
     c = p8.Cache(lens, G, D, 16, seed=3)
-    q = queries(37, H, D, 2)
-    got = attend(ops, c, q, new, lens, H, D ** -0.5)
-    check_rows(got, q.view(-1, H, D), c, new, lens, D ** -0.5, wide=True)
+    q = queries(sum(new), H, D, 2)
+    got = attend(ops, c, q, new, lens, H, D ** -0.5, window=window, keep_first=keep_first)
+    check_rows(got, q.view(-1, H, D), c, new, lens, D ** -0.5, window=window, keep_first=keep_first, wide=True)
     check_form(form, D)
 
 
