@@ -11,7 +11,8 @@
 //
 // What bounds it is mma.sync, which takes an SM's quarter some 27 cycles here for 16 x 8 x 16, and for few rows the chain of a tile.  us, a prompt of 2,048:
 // 16 heads over 8 of 64 89 (tcgen05: 34), 32 over 8 of 128 200 (43), 20 over 4 of 80 112 (38), 40 over 2 of 128 210 (63), 16 over 2 of 256 192; 64 tokens
-// behind 4,000, 32 over 8 of 128: 39 (64); behind 16,000 91 (230).  Slices for more balance than idle SMs ask for, four blocks an SM: 84 for 89 with heads of 64, 230 for 192 with 256.
+// behind 4,000, 32 over 8 of 128: 38 (29); behind 16,000 89 (54).  Slices for more balance than idle SMs ask for, four blocks an SM: 84 for 89 with heads
+// of 64, 230 for 192 with 256.
 #include "eight_bit.cuh"
 #include "mma_tiles.cuh"
 #include "prompt_slices.cuh"

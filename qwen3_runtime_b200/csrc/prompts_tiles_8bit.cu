@@ -13,7 +13,8 @@
 // What bounds it: 0.96 us a tile of both blocks (the softmax, as there), and what an item costs beside its tiles.  With a block of the launch for each item that
 // was 6.5 us (1.1 between two blocks, 0.5 for the item, 2.8 until the first scores, 2 to 2.6 at the end), now the end's.  us, with the unpacking, in blocks that
 // stay and one for each item: 32 heads over 8 of 128, 1,500 + 701 + 1,000 (behind 2,048) tokens and a single one 78, 87; 700 + 2,048 + 500 (behind 5,000) under
-// a window of 1,024 59, 67 (straight over the codes 210); a prompt of 2,048 43, 47.
+// a window of 1,024 59, 67 (straight over the codes 210); a prompt of 2,048 43, 47.  In
+// slices and without: 64 tokens behind 4,000 29, 64; behind 16,000 54, 230.
 //
 // Warps:  0 takes items and brings keys, 1 values, 2 queries;  4..7 and 8..11 softmax of block A and B, one thread per row;  12, 13 issue S = Q K^T,
 // 14, 15 O += P V.  An item passes through a ring of two places in shared memory.  What runs on from item to item are the rings' places and the numbers of

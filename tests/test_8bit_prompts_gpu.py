@@ -138,3 +138,39 @@ def test_portions_on_another_stream(ops, form):  # noqa: F811
     torch.cuda.synchronize()
     for got, (*_, want) in zip(outs, made):
         assert all(torch.equal(x.cpu().view(want.shape), want) for x in got)
+
+
+@pytest.mark.parametrize("window,keep_first", [(None, 0), (300, 20)])
+def test_captured_portions(ops, form, window, keep_first):  # noqa: F811
+    """A step of portions, captured, replayed with lengths that grow to all that its pages hold: what is counted from the lengths holds for any."""
+    H, G, D, page, new = 10, 2, 128, 16, [40, 1, 7]
+    width, lens = 2048 // page, [60, 90, 7]
+    c = p8.Cache([2048] * 3, G, D, page, seed=8, width=width)
+    pages, table = c.pages.cuda(), c.table.cuda()
+    q = torch.zeros((48, H * D), dtype=BF16, device="cuda")
+    out = torch.zeros_like(q)
+    step = p8.step_of(new, lens, page, captured_width=width)
+
+    def run():
+        ops.paged_attention_8bit(q, H * D, num_heads=H, pages=pages, block_table=table, out=out, scale=D ** -0.5, step=step, window=window,
+                                 keep_first=keep_first, **sizes(c))
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for more in (0, 1, 63, 800, 1958):
+        now = [min(2048, n + more) for n in lens]
+        rows = queries(48, H, D, more)
+        q.copy_(rows)
+        step.kv_lens.copy_(i32(now))
+        step.positions.copy_(i32([L - n + i for n, L in zip(new, now) for i in range(n)]))
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.raise_if_kernel_error()
+        sub = p8.Cache([], G, D, page)
+        sub.kv = [x[:, :, :n] for x, n in zip(c.kv, now)]
+        sub.scales = [s[:, :, : -(-n // page)] for s, n in zip(c.scales, now)]
+        check_rows(out.cpu().view(48, H, D), rows.view(-1, H, D), sub, new, now, D ** -0.5, window=window, keep_first=keep_first, wide=True)
