@@ -261,10 +261,9 @@ _SIGNATURES = {
         "q3_unpack_8bit": [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
                            c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p],
     },
-    "prompts_tiles_8bit": {
-        "q3_prompts_tiles_8bit": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float,
-                                  c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p],
-    },
+    **{name: {f"q3_{name}": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float,
+                             c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]}
+       for name in ("prompts_tiles_8bit", "prompts_tiles_wide_8bit")},
     "attention_8bit": {
         "q3_decode_attention_8bit": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int,
@@ -2646,8 +2645,8 @@ class CudaOps:
         of them; ``step.positions`` are places here.  Single tokens of bfloat16 heads of 64, 128 or 256 (up to 16 query heads a kv head)
         read the codes as they are, on the tensor cores; float32, other single tokens of up to 8 query heads a kv head, and rows that do not
         begin at 16 bytes, on the FMA pipes (csrc/attention_8bit.cu).  bfloat16 portions of prompts read the codes as well, turned to
-        bfloat16 on the way (csrc/prompts_8bit.cu); longer ones of heads of 64 to 128 have their sequences' pages unpacked once (at most
-        ``UNPACK_BYTES`` at a time, or one sequence) and go through the tcgen05 kernel (csrc/prompts_tiles_8bit.cu).  Both are exact up to the weights, which are rounded to
+        bfloat16 on the way (csrc/prompts_8bit.cu); longer ones of heads of 64 and more have their sequences' pages unpacked once (at most
+        ``UNPACK_BYTES`` at a time, or one sequence) and go through the tcgen05 kernel (csrc/prompts_tiles.cuh).  Both are exact up to the weights, which are rounded to
         bfloat16.  A table entry that is no page is read nowhere; the rows of a sequence that sees such a token are undefined, the others
         are not.  A key that is no number makes the rows none that see it; a value, its channel of them, and of its portion's other rows too (their weight
         for it is zero)."""
@@ -2701,7 +2700,7 @@ class CudaOps:
             self._decode_8bit(q_at, q_stride, H, G, D, pages, block_table, step, singles, step.num_single, max(own),
                               self.decode_slices_8bit(own, G, D, window, H // G, keep_first), out, out_at, page_size, scale, window, keep_first,
                               None)
-        if not (64 <= D <= 128 and H // G <= 128 and out_at & 15 == 0 and not step.decode_only
+        if not (64 <= D <= 256 and H // G <= 128 and out_at & 15 == 0 and not step.decode_only
                 and self._prompts_unpacked(cu, lens, H // G, G, D, window, keep_first, least)):
             return self._prompts_8bit(q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first)
         counts = unpacked_pages_4bit(cu, lens, 64, window, least, exact, keep_first)  # tiles of 64 tokens
@@ -2717,11 +2716,11 @@ class CudaOps:
         return out
 
     def _prompts_unpacked(self, cu, lens, R, G, D, window, keep_first, least=2) -> bool:
-        """Whether a step's portions are faster unpacked and on the tcgen05 kernel than straight over the codes.  Times in us, fitted to both at 300
-        random steps (one to eight portions of 2 to 1,000 tokens behind up to 30,000, 1 to 8 kv heads of 64 to 128, groups of 2 to 20, windows) on a
-        B200: the choice is 1.4 % slower than the better one on average, 44 % at worst.  Straight, a block of 128 rows takes a tile of 64 keys of
-        128 channels in 4.2 of an SM, in 2.6 if it is by itself, and slices cost their joining; unpacked, the longest sequence's tiles take 0.74 each, one
-        after the other, or all tiles 0.65 of an SM, slices their joining, and unpacking the bytes it moves."""
+        """Whether a step's portions are faster unpacked and on the tcgen05 kernel than straight over the codes.  Times in us, fitted to both at 400
+        random steps (one to eight portions of 2 to 1,000 tokens behind up to 30,000, 1 to 8 kv heads of 64 to 256, groups of 2 to 20, windows) on a
+        B200: the choice is 1.1 % slower than the better one on average, 47 % at worst.  Straight, a block of 128 rows takes a tile of 64 keys of
+        128 channels in 3.8 of an SM, in 2.75 if it is by itself, and slices cost their joining; unpacked, the longest sequence's tiles take 0.77 each, one
+        after the other, or all tiles 0.71 of an SM, slices their joining, and unpacking the bytes it moves."""
         work = chain = read = items = pairs = most = 0
         for b, kv in enumerate(lens):
             n = cu[b + 1] - cu[b]
@@ -2733,15 +2732,15 @@ class CudaOps:
             chain = max(chain, (min(seen, window + 256 // R + keep_first) if window else kv) / 64 + 1)
             read += seen
             items += rows
-            pairs += -(-n // (2 * (128 // R)))
+            pairs += -(-n // ((2 if D <= 128 else 1) * (128 // R)))
         if not items:
             return False
         splits = self._prompt_splits(items * G, D, window, keep_first, most, max(lens))
         size = max(D, 64) / 128
-        straight = 6.4 + max(4.2 * work * G * size / self.SM_COUNT, 2.6 * chain * size / splits) + (5.7 + 0.2 * splits if splits > 1 else 0)
+        straight = 6.1 + max(3.8 * work * G * size / self.SM_COUNT, 2.75 * chain * size / splits) + (5.5 + 0.38 * splits if splits > 1 else 0)
         splits = self._tile_splits(pairs * G, max(lens), most, window, keep_first)
-        unpacked = max(0.74 * chain / splits, 0.65 * work * G / self.SM_COUNT) + (4.6 + 0.33 * splits if splits > 1 else 0)
-        return 9 + 2.5 * D / 128 + 1.3e-6 * read * G * D + unpacked < straight
+        unpacked = max(0.77 * chain / splits, 0.71 * work * G / self.SM_COUNT) + (4 + 0.27 * splits if splits > 1 else 0)
+        return 10.3 + 1.4 * D / 128 + 1.2e-6 * read * G * D + unpacked < straight
 
     def _prompt_splits(self, blocks, D, window, keep_first, most_new, max_len) -> int:
         """Slices of the tiles of ``blocks`` blocks of rows: as many blocks as run at a time, each at least four tiles of 64 keys."""
@@ -2771,7 +2770,7 @@ class CudaOps:
         news = [b - a for a, b in zip(step.host_cu_seqlens[first:end], step.host_cu_seqlens[first + 1:end + 1])]
         if seqs != step.num_seqs:  # these sequences alone
             cu, kv_lens, block_table = cu[first:end + 1], kv_lens[first:end], block_table[first:end]
-        per = 2 * (128 // (H // G))  # tokens of an item: two blocks of rows
+        per = (2 if D <= 128 else 1) * (128 // (H // G))  # tokens of an item: two blocks of rows, one of heads of more than 128
         num_items = sum([-(-n // per) for n in news if n >= least])
         k = torch.empty((2, count, G, 64, D), dtype=out.dtype, device=out.device)
         v_at = k.data_ptr() + k.numel()  # (half of its bytes)
@@ -2785,7 +2784,8 @@ class CudaOps:
                    k.data_ptr(), v_at, per, num_items, items.data_ptr())
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out, prompts=True))
-        self._call("prompts_tiles_8bit", "q3_prompts_tiles_8bit", "paged_attention_tiles_8bit", q.data_ptr(), q_stride, q.size(0), k.data_ptr(), v_at,
+        group = "prompts_tiles_8bit" if D <= 128 else "prompts_tiles_wide_8bit"
+        self._call(group, "q3_" + group, "paged_attention_tiles_8bit", q.data_ptr(), q_stride, q.size(0), k.data_ptr(), v_at,
                    count, items.data_ptr(), num_items, out.data_ptr(), H, G, D, float(scale), window, keep_first, splits, mid_o, mid_ml, cu.data_ptr(), seqs,
                    least, self._error_word(out.device).data_ptr())
 

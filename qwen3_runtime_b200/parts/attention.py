@@ -89,7 +89,7 @@ class PagedAttention(Part):
         if self.bits:
             groups += [f"cache_{self.bits}bit", f"attention_{self.bits}bit"]
         if self.bits == 8 and self.ctx.dtype == torch.bfloat16:  # (what the specialised kernels over wide pages are for a cache in 16 bits)
-            return [*groups, "prompts_8bit", *(["prompts_tiles_8bit"] if 64 <= self.head_dim <= 128 else [])]
+            return [*groups, "prompts_8bit", *([f"prompts_tiles{'_wide' if self.head_dim > 128 else ''}_8bit"] if self.head_dim >= 64 else [])]
         if self.ctx.dtype == torch.bfloat16:
             # the specialised attention kernels that this head size can reach (ops.paged_attention)
             group = self.num_heads // self.num_kv_heads

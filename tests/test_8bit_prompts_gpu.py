@@ -24,7 +24,7 @@ def form(request, ops, monkeypatch):  # noqa: F811
 def check_form(form, D):
     unpacked, used = form
     names = set(used) - {"q3_decode_attention_8bit"}
-    assert names == ({"q3_unpack_8bit", "q3_prompts_tiles_8bit"} if unpacked and 64 <= D <= 128 else {"q3_prompts_attention_8bit"})
+    assert names == ({"q3_unpack_8bit", f"q3_prompts_tiles{'_wide' if D > 128 else ''}_8bit"} if unpacked and D >= 64 else {"q3_prompts_attention_8bit"})
 
 
 @pytest.mark.parametrize("window,keep_first", [(None, 0), (1, 0), (40, 6), (70, 200)])
