@@ -1,6 +1,6 @@
 // Attention of portions of prompts (and of single tokens that the decode kernel does not take) straight over a cache in 8 bits, in bfloat16: any head
 // size that is a multiple of 16 up to 256, any group, page size and window, with or without the sequence's first tokens.  (Longer portions of
-// heads of 64 to 128 go to the tcgen05 kernel, unpacked once: an n^2 product of their size is bound by the tensor cores.)
+// heads of 64 and more go to the tcgen05 kernel, unpacked once: an n^2 product of their size is bound by the tensor cores.)
 //
 // Rows are the (token, head of the group) pairs of a sequence and kv head, token by token; a block takes 128 of them, 16 a warp, and goes through the
 // keys in tiles of 64 (32 for heads of more than 128), which all warps share: a thread has its pieces of the next tile's codes on their way in
@@ -10,7 +10,7 @@
 // tiles are cut into slices, joined by a second kernel.
 //
 // What bounds it is mma.sync, which takes an SM's quarter some 27 cycles here for 16 x 8 x 16, and for few rows the chain of a tile.  us, a prompt of 2,048:
-// 16 heads over 8 of 64 89 (tcgen05: 34), 32 over 8 of 128 200 (43), 20 over 4 of 80 112 (38), 40 over 2 of 128 210 (63), 16 over 2 of 256 192; 64 tokens
+// 16 heads over 8 of 64 89 (tcgen05: 34), 32 over 8 of 128 200 (43), 20 over 4 of 80 112 (38), 40 over 2 of 128 210 (63), 16 over 2 of 256 192 (42); 64 tokens
 // behind 4,000, 32 over 8 of 128: 38 (29); behind 16,000 89 (54).  Slices for more balance than idle SMs ask for, four blocks an SM: 84 for 89 with heads
 // of 64, 230 for 192 with 256.
 #include "eight_bit.cuh"

@@ -3,24 +3,24 @@
 // optionally under a window, whose tokens may see the sequence's first ones as well.  The products, the softmax and their order are those of
 // attention_prefill_tc.cu, whose head comment has the reasons and what was tried; what differs is how blocks get their work:
 //
-//   * Keys and values lie in tiles of 64 tokens, in a sequence's order, so a tile's place follows from the item alone, and a half of it is one TMA box.
-//   * An item is a sequence's 2 x 128 rows (A and B; as many as whole tokens give) for one kv head; WIDE, heads of more than 128, whose results take half of the
-//     tensor memory, one block of rows, with scores in two places by turns, so that the next product does not wait for the softmax.  Blocks stay: one an SM takes item after item from a
-//     list that begins with the heaviest (csrc/cache_8bit.cu writes it), the next one when the keys of the present one are all asked for.  Then the next
-//     item's queries, keys and first product come while the softmax ends the present one and writes its rows.
+//   * Keys and values lie in tiles of 64 tokens, in a sequence's order, so a tile's place follows from the item alone, and 64 columns of it are one TMA box.
+//   * An item is a sequence's 2 x 128 rows (A and B; as many as whole tokens give) for one kv head.  WIDE, heads of more than 128, whose results take half of
+//     the tensor memory: one block of rows, with scores in two places by turns, so that the next product does not wait for the softmax.
+//   * Blocks stay: one an SM takes item after item from a list that begins with the heaviest (csrc/cache_8bit.cu writes it), the next one when the keys of the
+//     present one are all asked for.  Then the next item's queries, keys and first product come while the softmax ends the present one and writes its rows.
 //   * Where items would leave SMs idle (a portion behind a long context), each one's tiles are cut into slices, items of their own; a second kernel joins
 //     what they leave.
 //
 // What bounds it: 0.96 us a tile of both blocks (the softmax, as there), and what an item costs beside its tiles.  With a block of the launch for each item that
-// was 6.5 us (1.1 between two blocks, 0.5 for the item, 2.8 until the first scores, 2 to 2.6 at the end), now the end's.  us, with the unpacking, in blocks that
-// stay and one for each item: 32 heads over 8 of 128, 1,500 + 701 + 1,000 (behind 2,048) tokens and a single one 78, 87; 700 + 2,048 + 500 (behind 5,000) under
-// a window of 1,024 59, 67 (straight over the codes 210); a prompt of 2,048 43, 47.  In
-// slices and without: 64 tokens behind 4,000 29, 64; behind 16,000 54, 230.
+// was 6.5 us (1.1 between two blocks, 0.5 for the item, 2.8 until the first scores, 2 to 2.6 at the end), now the end's.  us, with the unpacking, 32 heads over
+// 8 of 128, in blocks that stay and one for each item: 1,500 + 701 + 1,000 (behind 2,048) tokens and a single one 78, 87; 700 + 2,048 + 500 (behind 5,000) under
+// a window of 1,024 59, 67 (straight over the codes 210); a prompt of 2,048 43, 47.  In slices and without: 64 tokens behind 4,000 29, 64; behind 16,000 54,
+// 230.  WIDE, 16 heads over 2 of 256, and straight over the codes: a prompt of 2,048 42, 192; the first of the above 78, 387.
 //
 // Warps:  0 takes items and brings keys, 1 values, 2 queries;  4..7 and 8..11 softmax of block A and B, one thread per row;  12, 13 issue S = Q K^T,
-// 14, 15 O += P V (WIDE: 4..7, 12 and 14).  An item passes through a ring of two places in shared memory.  What runs on from item to item are the rings' places and the numbers of
-// scores and weights so far, whose last bits are the barriers' phases.  Tensor memory as there: per block S [0,64), P_0 and P_1 [64,128), O [128,256); WIDE:
-// S_0 and S_1 [0,128), P_0 and P_1 [128,192), O [256,512).
+// 14, 15 O += P V (WIDE: 4..7, 12 and 14).  An item passes through a ring of two places in shared memory.  What runs on from item to item are the rings' places
+// and the numbers of scores and weights so far, whose last bits are the barriers' phases.  Tensor memory as there: per block S [0,64), P_0 and P_1 [64,128),
+// O [128,256); WIDE: S_0 and S_1 [0,128), P_0 and P_1 [128,192), O [256,512).
 // Every wait is bounded; on expiry the block raises its abort flag and the error word, waits for its copies and products in flight, frees its tensor memory
 // and returns.
 #pragma once
@@ -523,14 +523,13 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
           *reinterpret_cast<uint4*>(mine + lane * 128 + 16 * (ch ^ (lane & 7))) = make_uint4(y[0], y[1], y[2], y[3]);
         }
         __syncwarp();
-        const int pieces = min(8, (p.head_dim - c0) / 8), row_step = 32 / pieces, piece_step = 32 - row_step * pieces;
-        int row = lane / pieces, piece = lane - row * pieces;
-#pragma unroll 4
-        for (int i = 0; i < pieces; ++i) {
+        const int piece = lane & 7;
+        const bool there = c0 + 8 * piece < p.head_dim;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = 4 * i + (lane >> 3);
           bf16* to = reinterpret_cast<bf16*>(__shfl_sync(0xffffffffu, dst, row));
-          if (to) *reinterpret_cast<uint4*>(to + c0 + 8 * piece) = *reinterpret_cast<const uint4*>(mine + row * 128 + 16 * (piece ^ (row & 7)));
-          row += row_step, piece += piece_step;
-          if (piece >= pieces) piece -= pieces, ++row;
+          if (to && there) *reinterpret_cast<uint4*>(to + c0 + 8 * piece) = *reinterpret_cast<const uint4*>(mine + row * 128 + 16 * (piece ^ (row & 7)));
         }
         __syncwarp();
       }

@@ -42,17 +42,19 @@ def test_decode_attention(splits):
     t8.check_rows(got, q.view(2, 8, D), c, [1, 1], lens, D ** -0.5)
 
 
-def test_prompts_under_a_window():
+@pytest.mark.parametrize("D", [128, 256])
+def test_prompts_under_a_window(D):
     from qwen3_runtime_b200.ops.cuda import CudaOps
 
     ops = CudaOps()
-    H, G, D, page, new, lens = 8, 2, 128, 16, [70, 200], [400, 200]
+    H, G, page, new, lens = 8, 2, 16, [70, 200], [400, 200]
+    per, group = (64, "prompts_tiles_8bit") if D == 128 else (32, "prompts_tiles_wide_8bit")
     c = p8.Cache(lens, G, D, page, seed=3)
     q = t8.queries(270, H, D, 1)
     step, dev, out = p8.step_of(new, lens, page), q.cuda(), torch.zeros((270, H * D), dtype=torch.bfloat16, device="cuda")
     k = torch.zeros((14, G, 64, D), dtype=torch.bfloat16, device="cuda")
-    v, items = k.clone(), t8.i32([*([i, 70 * b, new[b], lens[b], 7 * b, 0, 0, 0] for b in range(2) for i in range(-(-new[b] // 64))), [0] * 8])
-    launch = _build("prompts_tiles_8bit", "q3_prompts_tiles_8bit")
+    v, items = k.clone(), t8.i32([*([i, 70 * b, new[b], lens[b], 7 * b, 0, 0, 0] for b in range(2) for i in range(-(-new[b] // per))), [0] * 8])
+    launch = _build(group, "q3_" + group)
     assert run(launch, dev.data_ptr(), H * D, 270, k.data_ptr(), v.data_ptr(), 14, items.data_ptr(), len(items) - 1, out.data_ptr(), H, G, D,
                D ** -0.5, 100, 20, 1, None, None, None, 2, 1) == 2
     got = t8.attend(ops, c, q, new, lens, H, D ** -0.5, window=100, keep_first=20)  # the ordinary build afterwards
