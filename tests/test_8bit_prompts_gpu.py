@@ -29,10 +29,11 @@ def check_form(form, D):
 
 @pytest.mark.parametrize("window,keep_first", [(None, 0), (1, 0), (40, 6), (70, 200)])
 @pytest.mark.parametrize("H,G,D,page", [(8, 8, 64, 5), (6, 2, 64, 8), (5, 1, 80, 16), (20, 4, 80, 24), (10, 1, 96, 32), (14, 2, 112, 1), (40, 2, 128, 16),
-                                        (8, 2, 128, 100), (12, 4, 128, 64), (128, 1, 64, 16), (16, 2, 256, 7), (6, 1, 32, 3), (3, 3, 208, 16)])
+                                        (8, 2, 128, 100), (12, 4, 128, 64), (128, 1, 64, 16), (100, 1, 128, 16), (70, 1, 144, 8), (16, 2, 256, 7), (6, 1, 32, 3), (3, 3, 208, 16)])
 def test_portions(ops, form, H, G, D, page, window, keep_first):  # noqa: F811
-    """Portions with and without tokens before them, that end inside a tile, a page and a block of rows; single tokens between them."""
-    new, lens = [33, 1, 70, 2, 1, 5], [33, 90, 210, 64, 1, 130]
+    """Portions with and without tokens before them, that end inside a tile, a page and a block of rows; single tokens and sequences that bring none
+    between them."""
+    new, lens = [0, 33, 1, 70, 0, 2, 1, 5, 0], [20, 33, 90, 210, 0, 64, 1, 130, 300]
     c = p8.Cache(lens, G, D, page, seed=D + G)
     q = queries(sum(new), H, D, H)
     got = attend(ops, c, q, new, lens, H, D ** -0.5, window=window, keep_first=keep_first)
