@@ -105,10 +105,12 @@ template <int D> __device__ __forceinline__ void take_query(uint32_t (&b)[Head<D
 //   BULK   page sizes that are a multiple of 16: a tile is 16 tokens of one page, brought by one bulk copy (16 tokens a page) or three
 //          that a lane asks for, and has one scale.  Rows behind the slice's end come along and are masked.
 //   else   any page size: cp.async token by token, each with its scales; what is not there is zero.
-// What bounds it is reading the codes: eight tokens behind 17,000 to 32,768, 64 heads over 8 of 128, 85 us, 5.9 TB/s while it runs (pages of 16 bits 163);
-// issue 0.34 a clock, a warp waits for results of mma.sync and for copies about alike.  Smaller launches lose to the blocks' beginnings and ends: eight
-// behind 4,096, 32 heads over 8, 17 us for 10 of reading; one behind 512, 5 us, a chain of lookups, copies and a join.  No more, measured at both: rings of
-// 2 or 4 stages, 1 or 4 tiles a step, 3 blocks an SM, two accumulators for the scores, values read before the softmax.
+// What bounds it is reading the codes: eight tokens behind 17,000 to 32,768, 64 heads over 8 of 128, 79 us, 6.2 TB/s (pages of 16 bits 163); issue 0.34 a
+// clock, a warp waits for results of mma.sync and for copies about alike.  Smaller launches lose to the blocks' beginnings and ends: eight behind 4,096, 32
+// heads over 8, 16.5 us for 10 of reading; one behind 512, 5 us, a chain of lookups, copies and a join.  No more, measured at both: rings of 2 or 4 stages, 1
+// or 4 tiles a step, 3 blocks an SM, two accumulators for the scores, values read before the softmax.  Slower: all pairs' steps behind one another, as many for
+// each warp of a launch that fills the device, its ring filled across the pairs' borders, the parts joined by a second kernel: 88, 22.5, and 48 sequences of
+// 65 to 3,966 44 for 42 -- a warp's every page is another place to read from, 1,184 of them, and the second kernel has many parts to join.
 constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int STEP = 16;  // keys of a tile
@@ -155,14 +157,20 @@ struct Decode {
 // lies in one page): places count the tiles of the first ones, `first` keys of them, and then those from lo on; key = place + gap from `first`
 // on.  Slices are cut by places.  Places per slice, the same for all sequences of the launch: the longest sequence's over the slices
 // asked for, in whole rounds of the block.  A shorter sequence has fewer slices.
-template <int ROUND> struct Slice {
-  int kv_len, lo, first, gap, begin, end, per, places;
-  __device__ __forceinline__ Slice(const Decode& a, int seq, int split) {
+struct Seen {
+  int kv_len, lo, first, gap, places;
+  __device__ __forceinline__ Seen(const Decode& a, int seq) {
     kv_len = min(a.kv_lens[seq], a.max_len);
     lo = a.window > 0 ? max(0, kv_len - a.window) : 0;
     const int tiles = (a.keep_first + STEP - 1) & ~(STEP - 1), begins = lo & ~(STEP - 1);
     first = min(tiles, begins), gap = begins - first;
-    places = kv_len - gap;
+    places = max(0, kv_len - gap);
+  }
+};
+template <int ROUND> struct Slice : Seen {
+  int begin, end, per;
+  __device__ __forceinline__ Slice(const Decode& a, int seq, int split) : Seen(a, seq) {
+    const int tiles = (a.keep_first + STEP - 1) & ~(STEP - 1);
     int longest = a.longest ? min(*a.longest, a.max_len) : a.max_len;
     if (a.window > 0) longest = min(longest, a.window + STEP - 1 + tiles);
     per = max(ROUND, ((longest + a.splits - 1) / a.splits + ROUND - 1) / ROUND * ROUND);
@@ -172,133 +180,29 @@ template <int ROUND> struct Slice {
   __device__ __forceinline__ int count(const Decode& a) const { return min(a.splits, max(0, places + per - 1) / per); }  // slices that have keys
 };
 
-template <int D, int NT> constexpr int decode_blocks() { return D == 64 ? 4 : 2; }
-
-template <int D, int NT, bool BULK, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_8bit_kernel(Decode a) {
+// What a warp holds of the queries of one kv head and sequence, and of their attention so far.
+template <int D, int NT, bool BULK> struct Taker {
   using H = Head<D>;
-  constexpr int TILES = H::TILES, ROUND = STEP * TILES * WARPS, QS = 8 * NT, PITCH = D + 4;
-  constexpr int VALUES = STEP * D, SCALES = 2 * VALUES;       // of a tile: keys, values, scales (one pair, or a pair of rows)
-  constexpr int TILE = SCALES + (BULK ? 16 : 8 * STEP), STAGE = TILES * TILE;
-  constexpr int MT = D / 16;                                  // products for the results of 16 keys
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t bars[WARPS][STAGES];
-  const int split = blockIdx.x, kvh = blockIdx.y, slot = blockIdx.z;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, l = lane & 3;
-  const int R = a.nq / a.nkv;
-  if (BULK) {
-    if (lane == 0) {
-#pragma unroll
-      for (int i = 0; i < STAGES; ++i) mbar_init(smem_addr(&bars[warp][i]), TILES);
-      mbar_init_fence();
-    }
-    __syncwarp();
-  }
-  pdl_wait();
-  const int seq = a.seq_list ? a.seq_list[slot] : slot;
-  const int tok = a.cu_seqlens[seq];
-  const Slice<ROUND> sl(a, seq, split);
-  const int begin = sl.begin, end = sl.end;
-  const long out_row = (long)tok * a.nq + kvh * R;
-  if (!CLUSTER && begin >= end) {
-    pdl_launch_dependents();
-    if (a.splits == 1)  // no key at all
-      for (int i = tid; i < R * D; i += THREADS) a.out[out_row * D + i] = __float2bfloat16_rn(0.f);
-    return;
-  }
-  const Q8Page L(D, a.ps);
-  const int* bt = a.block_table + (long)seq * a.max_pages;
-  unsigned char* ring = smem + warp * STAGES * STAGE;
-
-  // The token that this lane copies (BULK: the first lanes, a tile's first), as page of the sequence and row, moved on by a round at a time and
-  // over the gap once.  Its page is looked up a step before the copy, whose address waits for it.
-  const unsigned char* head = a.pages + kvh * L.record;
-  const uint32_t page_bytes = (uint32_t)(a.nkv * L.record);
-  int at = begin + warp * STEP * TILES + (BULK ? STEP * lane : lane);
-  bool behind = at >= sl.first;  // of the gap
-  int at_page = (at + (behind ? sl.gap : 0)) / a.ps, at_row = at + (behind ? sl.gap : 0) - at_page * a.ps;
-  const int go_pages = ROUND / a.ps, go_rows = ROUND - go_pages * a.ps;
-  auto look_up = [&]() { return lane < (BULK ? TILES : STEP * TILES) && at < end ? bt[at_page] : -1; };
-  int page = look_up();
-  const uint32_t ring_at = smem_addr(ring) + (BULK ? lane : lane / STEP) * TILE, bar_at = smem_addr(&bars[warp][0]);
-  auto load_step = [&](int stage) {  // the token looked up last; then the next is
-    if (BULK && lane >= TILES) return;
-    const uint32_t dst = ring_at + stage * STAGE;
-    const bool valid = (uint32_t)page < (uint32_t)a.num_pages;
-    const unsigned char* rec = head + (unsigned long long)(uint32_t)(valid ? page : 0) * page_bytes;
-    if (BULK) {  // each lane arrives once, with the bytes that it asks for
-      const uint32_t bar = bar_at + 8 * stage;
-      mbar_expect_tx(bar, valid ? TILE : 0);
-#ifdef Q3_TEST_WITHHOLD_A_BOX  // (a test build leaves the second tiles out: the stages never fill, a wait runs out)
-      if (valid && lane == 0) {
-#else
-      if (valid) {
-#endif
-        if (a.ps == STEP) {
-          bulk_copy(dst, rec, TILE, bar);
-        } else {
-          bulk_copy(dst, rec + (long)at_row * D, VALUES, bar);
-          bulk_copy(dst + VALUES, rec + L.values + (long)at_row * D, VALUES, bar);
-          bulk_copy(dst + SCALES, rec + L.scales, 16, bar);
-        }
-      }
-    } else {
-      // Neighbouring lanes bring neighbouring pieces of a row (every lane a row of its own: 32 lines a copy, half the speed).  A row's address comes from
-      // the lane that looked it up, with how its pieces are ordered (by the row in the page there, by the tile's here) and whether it exists below it.
-      constexpr int PIECES = D / 16, ROWS = 32 / PIECES;
-      const unsigned long long mine = reinterpret_cast<unsigned long long>(rec + (valid ? (long)at_row * D : 0)) | (uint32_t)((at_row ^ lane) & H::MASK) | (valid ? 8u : 0u);
-      const uint32_t to = smem_addr(ring) + stage * STAGE;
-#pragma unroll
-      for (int i = 0; i < STEP * TILES / ROWS; ++i) {
-        const int token = i * ROWS + lane / PIECES, piece = lane % PIECES;
-        const unsigned long long from = __shfl_sync(0xffffffffu, mine, token);
-        const unsigned char* src = reinterpret_cast<const unsigned char*>(from & ~15ull) + 16 * (piece ^ ((int)from & 7));
-        const uint32_t at_tile = to + token / STEP * TILE + token % STEP * D + 16 * piece;
-        cp_async16(at_tile, src, from & 8 ? 16 : 0);
-        cp_async16(at_tile + VALUES, src + L.values, from & 8 ? 16 : 0);
-      }
-      if (lane < STEP * TILES)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst + SCALES + 8 * (lane & (STEP - 1))), "l"(rec + L.scales), "r"(valid ? 8 : 0));
-      cp_async_commit();
-    }
-    at += ROUND, at_page += go_pages, at_row += go_rows;
-    if (at_row >= a.ps) at_row -= a.ps, ++at_page;
-    if (!behind && at >= sl.first) {
-      behind = true;
-      const int key = at + sl.gap;
-      at_page = key / a.ps, at_row = key - at_page * a.ps;
-    }
-    page = look_up();
-  };
-  // the queries' rows are on their way together with the first pages
-  uint4 raw[NT][H::PIECES][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-    fetch_query<D>(raw[n], 8 * n + r < R ? a.q + (long)tok * a.q_stride + (long)(kvh * R + 8 * n + r) * D : nullptr, lane);
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) load_step(i);
-
+  static constexpr int TILES = H::TILES, MT = D / 16, VALUES = STEP * D, SCALES = 2 * VALUES, TILE = SCALES + (BULK ? 16 : 8 * STEP);
+  int lane, r, l, k_row, k_swap;
   uint32_t q[NT][H::PIECES][4][2];
   float undo[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) take_query<D>(q[n], undo[n], raw[n], a.scale_log2, lane);
   // o: 2^(6 - M) times the results so far; sum: of 2^(x - m), this lane's share.  m and M are the same in all lanes of a column.
   float o[NT][MT][4], m[NT][2], M[NT][2], sum[NT][2];
+  __device__ __forceinline__ Taker(int lane) : lane(lane), r(lane >> 2), l(lane & 3), k_row((lane >> 2) * D), k_swap((lane >> 2) & H::MASK) {}
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = M[n][0] = M[n][1] = MINUS_BIG;
-    sum[n][0] = sum[n][1] = 0.f;
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = M[n][0] = M[n][1] = MINUS_BIG;
+      sum[n][0] = sum[n][1] = 0.f;
 #pragma unroll
-    for (int j = 0; j < MT; ++j)
+      for (int j = 0; j < MT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][j][e] = 0.f;
+        for (int e = 0; e < 4; ++e) o[n][j][e] = 0.f;
+    }
   }
-  const int k_row = r * D, k_swap = r & H::MASK;
-  int stage = 0;
-  uint32_t parity = 0;
-  // WHOLE: every key of the step is visible
-  auto take = [&](auto whole_tiles, const unsigned char* st, int base) {
-    constexpr bool WHOLE = decltype(whole_tiles)::value;
+  // The keys of one step, at places base .. of which those in front of `end` count.  WHOLE: every one of them is visible.
+  template <bool WHOLE> __device__ __forceinline__ void take(const Decode& a, const unsigned char* st, int base, const Seen& sl, int end) {
     float x[TILES][NT][4], up[TILES][2];  // up: log2 of the values' scales of rows r and r + 8
     bool in[TILES][2];
     int key0[TILES];
@@ -448,7 +352,141 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_8bit_k
         }
       }
     }
+  }
+  // column c of tile n, from here, as its sum (all lanes of a column) and, by `put`, four channels at a time of 2^-m times the results
+  template <typename Put> __device__ __forceinline__ float finished(int n, int c, Put put) const {
+    float total = sum[n][c];
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    const float back = exp2_fast((M[n][c] - m[n][c]) - 6.f);
+#pragma unroll
+    for (int i = 0; i < MT / 2; ++i) {  // channels 4 i .. 4 i + 3 of this lane's, which are pieces r and r + 8 of the head (D = 64: half of one)
+      const int channel = D == 64 ? 8 * r + 4 * i : 16 * (r + 8 * (i / 4)) + 4 * (i % 4);
+      put(channel, make_float4(o[n][2 * i][c] * back, o[n][2 * i][c + 2] * back, o[n][2 * i + 1][c] * back, o[n][2 * i + 1][c + 2] * back));
+    }
+    return total;
+  }
+};
+
+// The copies of a step into a stage, by a warp: `rec` and `at_row` are of the token that this lane has looked up (BULK: the first lanes, a tile's first token),
+// `valid` that there is one.
+template <int D, bool BULK>
+__device__ __forceinline__ void copy_step(const Decode& a, const Q8Page& L, uint32_t dst, uint32_t stage_at, uint32_t bar, const unsigned char* rec, int at_row,
+                                          bool valid, int lane) {
+  using H = Head<D>;
+  constexpr int TILES = H::TILES, VALUES = STEP * D, SCALES = 2 * VALUES, TILE = SCALES + (BULK ? 16 : 8 * STEP);
+  if (BULK) {  // each lane arrives once, with the bytes that it asks for
+    if (lane >= TILES) return;
+    mbar_expect_tx(bar, valid ? TILE : 0);
+#ifdef Q3_TEST_WITHHOLD_A_BOX  // (a test build leaves the second tiles out: the stages never fill, a wait runs out)
+    if (valid && lane == 0) {
+#else
+    if (valid) {
+#endif
+      if (a.ps == STEP) {
+        bulk_copy(dst, rec, TILE, bar);
+      } else {
+        bulk_copy(dst, rec + (long)at_row * D, VALUES, bar);
+        bulk_copy(dst + VALUES, rec + L.values + (long)at_row * D, VALUES, bar);
+        bulk_copy(dst + SCALES, rec + L.scales, 16, bar);
+      }
+    }
+  } else {
+    // Neighbouring lanes bring neighbouring pieces of a row (every lane a row of its own: 32 lines a copy, half the speed).  A row's address comes from
+    // the lane that looked it up, with how its pieces are ordered (by the row in the page there, by the tile's here) and whether it exists below it.
+    constexpr int PIECES = D / 16, ROWS = 32 / PIECES;
+    const unsigned long long mine = reinterpret_cast<unsigned long long>(rec + (valid ? (long)at_row * D : 0)) | (uint32_t)((at_row ^ lane) & H::MASK) | (valid ? 8u : 0u);
+#pragma unroll
+    for (int i = 0; i < STEP * TILES / ROWS; ++i) {
+      const int token = i * ROWS + lane / PIECES, piece = lane % PIECES;
+      const unsigned long long from = __shfl_sync(0xffffffffu, mine, token);
+      const unsigned char* src = reinterpret_cast<const unsigned char*>(from & ~15ull) + 16 * (piece ^ ((int)from & 7));
+      const uint32_t at_tile = stage_at + token / STEP * TILE + token % STEP * D + 16 * piece;
+      cp_async16(at_tile, src, from & 8 ? 16 : 0);
+      cp_async16(at_tile + VALUES, src + L.values, from & 8 ? 16 : 0);
+    }
+    if (lane < STEP * TILES)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst + SCALES + 8 * (lane & (STEP - 1))), "l"(rec + L.scales), "r"(valid ? 8 : 0));
+    cp_async_commit();
+  }
+}
+
+template <int D, int NT> constexpr int decode_blocks() { return D == 64 ? 4 : 2; }
+
+template <int D, int NT, bool BULK, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_8bit_kernel(Decode a) {
+  using H = Head<D>;
+  constexpr int TILES = H::TILES, ROUND = STEP * TILES * WARPS, QS = 8 * NT, PITCH = D + 4;
+  constexpr int VALUES = STEP * D, SCALES = 2 * VALUES;       // of a tile: keys, values, scales (one pair, or a pair of rows)
+  constexpr int TILE = SCALES + (BULK ? 16 : 8 * STEP), STAGE = TILES * TILE;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) uint64_t bars[WARPS][STAGES];
+  const int split = blockIdx.x, kvh = blockIdx.y, slot = blockIdx.z;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, l = lane & 3;
+  const int R = a.nq / a.nkv;
+  if (BULK) {
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i) mbar_init(smem_addr(&bars[warp][i]), TILES);
+      mbar_init_fence();
+    }
+    __syncwarp();
+  }
+  pdl_wait();
+  const int seq = a.seq_list ? a.seq_list[slot] : slot;
+  const int tok = a.cu_seqlens[seq];
+  const Slice<ROUND> sl(a, seq, split);
+  const int begin = sl.begin, end = sl.end;
+  const long out_row = (long)tok * a.nq + kvh * R;
+  if (!CLUSTER && begin >= end) {
+    pdl_launch_dependents();
+    if (a.splits == 1)  // no key at all
+      for (int i = tid; i < R * D; i += THREADS) a.out[out_row * D + i] = __float2bfloat16_rn(0.f);
+    return;
+  }
+  const Q8Page L(D, a.ps);
+  const int* bt = a.block_table + (long)seq * a.max_pages;
+  unsigned char* ring = smem + warp * STAGES * STAGE;
+
+  // The token that this lane copies (BULK: the first lanes, a tile's first), as page of the sequence and row, moved on by a round at a time and
+  // over the gap once.  Its page is looked up a step before the copy, whose address waits for it.
+  const unsigned char* head = a.pages + kvh * L.record;
+  const uint32_t page_bytes = (uint32_t)(a.nkv * L.record);
+  int at = begin + warp * STEP * TILES + (BULK ? STEP * lane : lane);
+  bool behind = at >= sl.first;  // of the gap
+  int at_page = (at + (behind ? sl.gap : 0)) / a.ps, at_row = at + (behind ? sl.gap : 0) - at_page * a.ps;
+  const int go_pages = ROUND / a.ps, go_rows = ROUND - go_pages * a.ps;
+  auto look_up = [&]() { return lane < (BULK ? TILES : STEP * TILES) && at < end ? bt[at_page] : -1; };
+  int page = look_up();
+  const uint32_t ring_at = smem_addr(ring) + (BULK ? lane : lane / STEP) * TILE, bar_at = smem_addr(&bars[warp][0]);
+  auto load_step = [&](int stage) {  // the token looked up last; then the next is
+    const uint32_t dst = ring_at + stage * STAGE;
+    const bool valid = (uint32_t)page < (uint32_t)a.num_pages;
+    const unsigned char* rec = head + (unsigned long long)(uint32_t)(valid ? page : 0) * page_bytes;
+    copy_step<D, BULK>(a, L, dst, smem_addr(ring) + stage * STAGE, bar_at + 8 * stage, rec, at_row, valid, lane);
+    at += ROUND, at_page += go_pages, at_row += go_rows;
+    if (at_row >= a.ps) at_row -= a.ps, ++at_page;
+    if (!behind && at >= sl.first) {
+      behind = true;
+      const int key = at + sl.gap;
+      at_page = key / a.ps, at_row = key - at_page * a.ps;
+    }
+    page = look_up();
   };
+  // the queries' rows are on their way together with the first pages
+  uint4 raw[NT][H::PIECES][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    fetch_query<D>(raw[n], 8 * n + r < R ? a.q + (long)tok * a.q_stride + (long)(kvh * R + 8 * n + r) * D : nullptr, lane);
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) load_step(i);
+
+  Taker<D, NT, BULK> mine(lane);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) take_query<D>(mine.q[n], mine.undo[n], raw[n], a.scale_log2, lane);
+  mine.clear();
+  int stage = 0;
+  uint32_t parity = 0;
   for (int base = begin + warp * STEP * TILES; base < end; base += ROUND) {
     if (BULK) {
       if (!__all_sync(0xffffffffu, mbar_try_wait(bar_at + 8 * stage, parity)) && !wait_for_tiles(bar_at + 8 * stage, parity, a.error_word)) {
@@ -461,9 +499,9 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_8bit_k
     __syncwarp();
     const unsigned char* st = ring + stage * STAGE;
     if (base + STEP * TILES <= end && base >= sl.first && base + sl.gap >= sl.lo)  // (of one mind over the warp)
-      take(std::true_type(), st, base);
+      mine.template take<true>(a, st, base, sl, end);
     else
-      take(std::false_type(), st, base);
+      mine.template take<false>(a, st, base, sl, end);
     __syncwarp();
     load_step(stage ? stage - 1 : STAGES - 1);
     if (++stage == STAGES) stage = 0, parity ^= 1;
@@ -481,20 +519,11 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_8bit_k
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int h = 8 * n + 2 * l + c;
-      float total = sum[n][c];
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-      if (r == 0) {
-        ml[(warp * QS + h) * 2] = m[n][c];
-        ml[(warp * QS + h) * 2 + 1] = total;
-      }
       float* row = ow + (warp * QS + h) * PITCH;
-      const float back = exp2_fast((M[n][c] - m[n][c]) - 6.f);
-#pragma unroll
-      for (int i = 0; i < MT / 2; ++i) {  // channels 4 i .. 4 i + 3 of this lane's, which are pieces r and r + 8 of the head (D = 64: half of one)
-        const int channel = D == 64 ? 8 * r + 4 * i : 16 * (r + 8 * (i / 4)) + 4 * (i % 4);
-        *reinterpret_cast<float4*>(row + channel) =
-            make_float4(o[n][2 * i][c] * back, o[n][2 * i][c + 2] * back, o[n][2 * i + 1][c] * back, o[n][2 * i + 1][c + 2] * back);
+      const float total = mine.finished(n, c, [&](int channel, float4 v) { *reinterpret_cast<float4*>(row + channel) = v; });
+      if (r == 0) {
+        ml[(warp * QS + h) * 2] = mine.m[n][c];
+        ml[(warp * QS + h) * 2 + 1] = total;
       }
     }
   }

@@ -2833,9 +2833,9 @@ class CudaOps:
     # whether a kv head has more than 8 query heads.
     DECODE_8BIT_BLOCKS_PER_SM = {64: 4, 128: 2, 256: 2}
     DECODE_8BIT_COSTS = {
-        (64, False): (0.81, 0.33, 2.6, 1.8, 0.45, 1.16), (64, True): (0.92, 0.56, 0.3, 1.2, 0.0, 1.09),
-        (128, False): (0.89, 0.57, 2.9, 2.8, 0.62, 1.14), (128, True): (1.11, 0.70, 4.0, 4.0, 0.56, 1.08),
-        (256, False): (0.86, 0.54, 5.2, 5.1, 0.86, 1.08), (256, True): (1.13, 0.75, 0.0, 5.5, 0.0, 1.06),
+        (64, False): (0.70, 0.28, 4.2, 2.3, 0.63, 1.31), (64, True): (1.09, 0.47, 0.0, 1.0, 0.0, 1.23),
+        (128, False): (0.79, 0.50, 5.3, 4.6, 0.71, 0.99), (128, True): (0.95, 0.60, 0.0, 3.4, 0.43, 1.11),
+        (256, False): (0.77, 0.49, 0.0, 3.6, 0.72, 1.01), (256, True): (1.14, 0.70, 0.0, 3.8, 0.53, 0.91),
     }
 
     def decode_slices_8bit(self, kv_lens, num_kv_heads, head_dim, window=None, group=1, keep_first=0) -> int:
@@ -2854,7 +2854,7 @@ class CudaOps:
 
     def _decode_slices_8bit(self, rounds, num_kv_heads, head_dim, wide) -> int:
         """Times in us, fitted to a sweep of 1 to 64 slices over 212 batches of 1 to 128 sequences of 20 to 131,072 tokens (7 head counts and sizes) on
-        a B200: the choice is 2 to 5 % slower than the best one on average (heads of 64 in wide groups 8 %), 26 % at worst.  A round of keys takes
+        a B200: the choice is 1 to 5 % slower than the best one on average, 30 % at worst.  A round of keys takes
         a block `alone` on its SM, and `shared` for every block there; a block's beginning and end as much as `ends` rounds, of which an SM
         notices `ends_shared` where other blocks go on meanwhile; the last blocks end apart by a share `tail` of their length.  A second kernel
         joins slices in 2.1 and more; clusters do so for less, but take `clustered` times as long, and all have to run at once."""
