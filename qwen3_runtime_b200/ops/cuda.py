@@ -2652,7 +2652,8 @@ class CudaOps:
         for it is zero)."""
         what = "paged_attention_8bit"
         D, G, H, dtype, shape, rows = head_dim, num_kv_heads, num_heads, out.dtype, q.shape, out.shape
-        _, (table_rows, max_pages) = self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens, record_of=_eight_bit_record)
+        (num_pages, *_), (table_rows, max_pages) = self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens,
+                                                                    record_of=_eight_bit_record)
         if window or keep_first:
             window, keep_first = int(window or 0), int(keep_first or 0)
             if window < 0 or keep_first < 0 or window + keep_first > 1 << 30:
@@ -2674,17 +2675,18 @@ class CudaOps:
         if step.captured_width:
             max_len = min(step.captured_width * page_size, room)
         q_at, out_at = q.data_ptr(), out.data_ptr()
+        held = (pages.data_ptr(), num_pages, block_table.data_ptr(), max_pages)
         fast = dtype == torch.bfloat16 and D in (64, 128, 256) and H // G <= 16 and not (q_stride & 7 or q_at & 15 or out_at & 7)
         if fast and step.decode_only:
             if longest is not None and (longest.dtype != torch.int32 or longest.numel() < 1):
                 raise KernelError(f"{what}: kv_longest is one int32")
-            return self._decode_8bit(q_at, q_stride, H, G, D, pages, block_table, step, None, seqs, max_len,
+            return self._decode_8bit(q_at, q_stride, H, G, D, held, step, None, seqs, max_len,
                                      decode_slices or self.decode_slices_8bit(step.host_kv_lens, G, D, window, H // G, keep_first), out, out_at,
                                      page_size, scale, window, keep_first, longest)
         # (single tokens of up to 8 query heads a kv head that the decode kernel does not take: eight behind 4,096, 20 heads over 4 of 80, take the
         # general form 30 us and the one for prompts, whose blocks have 128 rows, 41; 40 over 2 of 128 51 and 39)
         if _dtype_code(dtype) == 0 or q_stride & 7 or q_at & 15 or out_at & 3 or (step.decode_only and not fast and H // G <= 8):
-            return self._general_8bit(q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window, keep_first)
+            return self._general_8bit(q_at, q_stride, H, G, D, held, table_rows, step, max_len, out, page_size, scale, window, keep_first)
         cu = step.host_cu_seqlens
         if len(cu) <= seqs:
             raise KernelError(f"{what}: host_cu_seqlens are the sequences' first tokens and the number of all")
@@ -2697,12 +2699,12 @@ class CudaOps:
         lens = list(step.host_kv_lens[:seqs]) if exact else [max_len] * seqs
         if fast and step.num_single:
             own = [kv for b, kv in enumerate(lens) if cu[b + 1] - cu[b] == 1]
-            self._decode_8bit(q_at, q_stride, H, G, D, pages, block_table, step, singles, step.num_single, max(own),
+            self._decode_8bit(q_at, q_stride, H, G, D, held, step, singles, step.num_single, max(own),
                               self.decode_slices_8bit(own, G, D, window, H // G, keep_first), out, out_at, page_size, scale, window, keep_first,
                               None)
         if not (64 <= D <= 256 and H // G <= 128 and out_at & 15 == 0 and not step.decode_only
                 and self._prompts_unpacked(cu, lens, H // G, G, D, window, keep_first, least)):
-            return self._prompts_8bit(q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first)
+            return self._prompts_8bit(q_at, q_stride, H, G, D, held, step, least, max_len, out, page_size, scale, window, keep_first)
         counts = unpacked_pages_4bit(cu, lens, 64, window, least, exact, keep_first)  # tiles of 64 tokens
         total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * 64 * D)
         if total <= limit:
@@ -2711,8 +2713,8 @@ class CudaOps:
             runs = [(first, end, sum(counts[first:end])) for first, end in runs_within(counts, limit)]
         for first, end, count in runs:
             most = max([n for n, c in zip(lens[first:end], counts[first:end]) if c])
-            self._prompts_tc_8bit(q, q_stride, H, G, D, pages, block_table, step, least, first, end, count, most, out, page_size, scale,
-                                  window, keep_first)
+            self._prompts_tc_8bit(q_at, q_stride, shape[0], H, G, D, held, step, least, first, end, count, most, out, out_at, page_size, scale, window,
+                                  keep_first)
         return out
 
     def _prompts_unpacked(self, cu, lens, R, G, D, window, keep_first, least=2) -> bool:
@@ -2752,44 +2754,37 @@ class CudaOps:
         tiles = -(-(min(longest, window + most_new + keep_first) if window else longest) // 64)
         return max(1, min(self.SM_COUNT // items, tiles // 8, 16))
 
-    def _slices_of_prompts(self, rows, D, splits, device):
-        """``splits``, fewer where there would be more to keep of the slices than 256 MB; scratch for them (to be held until the launch), and where the
-        results, and the maxima and sums, of so many slices of ``rows`` lie in it."""
-        splits = max(1, min(splits, (1 << 26) // (rows * D)))
-        if splits == 1:
-            return 1, None, None, None
-        mid = torch.empty(rows * splits * (D + 2), dtype=torch.float32, device=device)
-        self.launches += 1
-        return splits, mid, mid.data_ptr(), mid.data_ptr() + 4 * rows * splits * D
-
-    def _prompts_tc_8bit(self, q, q_stride, H, G, D, pages, block_table, step, least, first, end, count, longest, out, page_size, scale,
-                         window, keep_first):
+    def _prompts_tc_8bit(self, q_at, q_stride, q_rows, H, G, D, held, step, least, first, end, count, longest, out, out_at, page_size, scale, window,
+                         keep_first):
         """Attention of those of the step's sequences ``first .. end - 1`` that bring at least ``least`` tokens, whose ``count`` tiles of 64 tokens
         are unpacked for it (none of those has more than ``longest`` keys)."""
-        cu, kv_lens, seqs = step.cu_seqlens, step.kv_lens, end - first
+        pages_at, num_pages, table_at, width = held
+        cu_at, lens_at, seqs = step.cu_seqlens.data_ptr() + 4 * first, step.kv_lens.data_ptr() + 4 * first, end - first
         news = [b - a for a, b in zip(step.host_cu_seqlens[first:end], step.host_cu_seqlens[first + 1:end + 1])]
-        if seqs != step.num_seqs:  # these sequences alone
-            cu, kv_lens, block_table = cu[first:end + 1], kv_lens[first:end], block_table[first:end]
         per = (2 if D <= 128 else 1) * (128 // (H // G))  # tokens of an item: two blocks of rows, one of heads of more than 128
         num_items = sum([-(-n // per) for n in news if n >= least])
-        k = torch.empty((2, count, G, 64, D), dtype=out.dtype, device=out.device)
-        v_at = k.data_ptr() + k.numel()  # (half of its bytes)
-        items = torch.empty((num_items + 1, 8), dtype=torch.int32, device=out.device)
-        splits = self._tile_splits(num_items * G, longest, max(news), window, keep_first)
-        splits, mid, mid_o, mid_ml = self._slices_of_prompts(q.size(0) * H, D, splits, out.device)
+        splits, rows = self._tile_splits(num_items * G, longest, max(news), window, keep_first), q_rows * H
+        splits = max(1, min(splits, (1 << 26) // (rows * D)))  # (no more to keep of the slices than 256 MB)
+        # keys, values, the items and the number behind them, what is kept of the slices: one after the other (each allocation costs the host 2.5 us)
+        half, listed = 128 * count * G * D, 32 * (num_items + 1)
+        scratch = torch.empty(2 * half + listed + (4 * rows * splits * (D + 2) if splits > 1 else 0), dtype=torch.uint8, device=out.device)
+        k_at = scratch.data_ptr()
+        items_at, mid_o, mid_ml = k_at + 2 * half, None, None
+        if splits > 1:
+            mid_o = items_at + listed
+            mid_ml = mid_o + 4 * rows * splits * D
+            self.launches += 1
         if self.timing is not None:
-            self._costs(k.numel() * k.element_size() + count * 64 * 2 * G * D)
-        self._call("cache_8bit", "q3_unpack_8bit", "unpack_8bit", _dtype_code(out.dtype), pages.data_ptr(), pages.size(0), G, D, page_size,
-                   block_table.data_ptr(), block_table.size(1), kv_lens.data_ptr(), seqs, longest, cu.data_ptr(), least, window, keep_first, count, 0,
-                   k.data_ptr(), v_at, per, num_items, items.data_ptr())
+            self._costs(2 * half + count * 64 * 2 * G * D)
+        self._call("cache_8bit", "q3_unpack_8bit", "unpack_8bit", _dtype_code(out.dtype), pages_at, num_pages, G, D, page_size,
+                   table_at + 4 * first * width, width, lens_at, seqs, longest, cu_at, least, window, keep_first, count, 0, k_at, k_at + half, per, num_items, items_at)
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out, prompts=True))
         group = "prompts_tiles_8bit" if D <= 128 else "prompts_tiles_wide_8bit"
-        self._call(group, "q3_" + group, "paged_attention_tiles_8bit", q.data_ptr(), q_stride, q.size(0), k.data_ptr(), v_at,
-                   count, items.data_ptr(), num_items, out.data_ptr(), H, G, D, float(scale), window, keep_first, splits, mid_o, mid_ml, cu.data_ptr(), seqs,
-                   least, self._error_word(out.device).data_ptr())
+        self._call(group, "q3_" + group, "paged_attention_tiles_8bit", q_at, q_stride, q_rows, k_at, k_at + half, count, items_at, num_items, out_at, H, G,
+                   D, float(scale), window, keep_first, splits, mid_o, mid_ml, cu_at, seqs, least, self._error_word(out.device).data_ptr())
 
-    def _prompts_8bit(self, q_at, q_stride, H, G, D, pages, block_table, step, least, max_len, out, page_size, scale, window, keep_first):
+    def _prompts_8bit(self, q_at, q_stride, H, G, D, held, step, least, max_len, out, page_size, scale, window, keep_first):
         """Attention of the sequences that bring at least ``least`` tokens, straight over the codes (csrc/prompts_8bit.cu)."""
         T, R, cu = step.num_tokens, H // G, step.host_cu_seqlens
         news = [n for n in [b - a for a, b in zip(cu, cu[1:step.num_seqs + 1])] if n >= least]
@@ -2797,15 +2792,20 @@ class CudaOps:
         if not items:
             return out
         splits = self._prompt_splits(items * G, D, window, keep_first, max(news), max_len)
-        splits, mid, mid_o, mid_ml = self._slices_of_prompts(T * H, D, splits, out.device)
+        splits = max(1, min(splits, (1 << 26) // (T * H * D)))  # (no more to keep of the slices than 256 MB)
+        mid_o = mid_ml = None
+        if splits > 1:
+            mid = torch.empty(T * H * splits * (D + 2), dtype=torch.float32, device=out.device)
+            mid_o = mid.data_ptr()
+            mid_ml = mid_o + 4 * T * H * splits * D
+            self.launches += 1
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out, prompts=None if least < 2 else True))
-        self._call("prompts_8bit", "q3_prompts_attention_8bit", "paged_attention_prompts_8bit", q_at, q_stride, pages.data_ptr(), pages.size(0),
-                   block_table.data_ptr(), block_table.size(1), step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(), out.data_ptr(), mid_o, mid_ml,
-                   splits, items, least, T, step.num_seqs, H, G, D, page_size, float(scale), window, keep_first, max_len)
+        self._call("prompts_8bit", "q3_prompts_attention_8bit", "paged_attention_prompts_8bit", q_at, q_stride, *held,
+                   step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(), out.data_ptr(), mid_o, mid_ml, splits, items, least, T, step.num_seqs, H, G, D, page_size, float(scale), window, keep_first, max_len)
         return out
 
-    def _general_8bit(self, q, q_stride, H, G, D, pages, block_table, step, max_len, out, page_size, scale, window, keep_first):
+    def _general_8bit(self, q_at, q_stride, H, G, D, held, table_rows, step, max_len, out, page_size, scale, window, keep_first):
         code, T = _dtype_code(out.dtype), out.size(0)
         for t in (step.token_seq, step.positions):
             if t.dtype != torch.int32 or t.numel() < T or not t.is_contiguous():
@@ -2824,9 +2824,8 @@ class CudaOps:
             self.launches += 1
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out))
-        self._call("attention_8bit", "q3_general_attention_8bit", "paged_attention_general_8bit", code, _ptr(q), q_stride, _ptr(pages),
-                   pages.shape[0], _ptr(block_table), block_table.shape[1], block_table.shape[0], _ptr(step.token_seq),
-                   _ptr(step.positions), _ptr(out), mid_o, mid_ml, slices, T, H, G, D, page_size, float(scale), window, keep_first)
+        self._call("attention_8bit", "q3_general_attention_8bit", "paged_attention_general_8bit", code, q_at, q_stride, *held, table_rows,
+                   _ptr(step.token_seq), _ptr(step.positions), _ptr(out), mid_o, mid_ml, slices, T, H, G, D, page_size, float(scale), window, keep_first)
         return out
 
     # Blocks of decode attention over 8-bit numbers that an SM holds, by head size; and what its cost model takes (see there), by head size and
@@ -2890,8 +2889,8 @@ class CudaOps:
             count = self._parts_cache[key] = self._get("attention_8bit", "q3_decode_clusters_8bit")(head_dim, int(wide), size)
         return count
 
-    def _decode_8bit(self, q_at, q_stride, H, G, D, pages, block_table, step, seq_list, num_seqs, max_len, slices, out, out_at, page_size,
-                     scale, window, keep_first, longest):
+    def _decode_8bit(self, q_at, q_stride, H, G, D, held, step, seq_list, num_seqs, max_len, slices, out, out_at, page_size, scale, window, keep_first,
+                     longest):
         mid_o = mid_lse = None
         if slices < -1 or slices > 16:  # joined by a second kernel (16 blocks a cluster at most)
             slices = abs(slices)
@@ -2903,9 +2902,8 @@ class CudaOps:
             singles = [kv for b, kv in enumerate(step.host_kv_lens) if step.host_cu_seqlens[b + 1] - step.host_cu_seqlens[b] == 1]
             seen = sum(min(kv, window + keep_first) if window else kv for kv in singles)
             self._costs(seen * 2 * G * D + 4 * num_seqs * H * D, 4 * H * D * seen)
-        self._call("attention_8bit", "q3_decode_attention_8bit", "paged_attention_decode_8bit", q_at, q_stride, pages.data_ptr(),
-                   pages.size(0), block_table.data_ptr(), block_table.size(1), step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(),
-                   _ptr(seq_list), out_at, mid_o, mid_lse, num_seqs, H, G, D, page_size, float(scale), window, keep_first,
+        self._call("attention_8bit", "q3_decode_attention_8bit", "paged_attention_decode_8bit", q_at, q_stride, *held,
+                   step.kv_lens.data_ptr(), step.cu_seqlens.data_ptr(), _ptr(seq_list), out_at, mid_o, mid_lse, num_seqs, H, G, D, page_size, float(scale), window, keep_first,
                    abs(slices), max_len, _ptr(longest), self._error_word(out.device).data_ptr())
         return out
 
