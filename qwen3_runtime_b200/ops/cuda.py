@@ -2702,7 +2702,8 @@ class CudaOps:
             self._decode_8bit(q_at, q_stride, H, G, D, held, step, singles, step.num_single, max(own),
                               self.decode_slices_8bit(own, G, D, window, H // G, keep_first), out, out_at, page_size, scale, window, keep_first,
                               None)
-        if not (64 <= D <= 256 and H // G <= 128 and out_at & 15 == 0 and not step.decode_only
+        # (the tcgen05 kernel looks for a row's largest score before it is scaled)
+        if not (64 <= D <= 256 and H // G <= 128 and out_at & 15 == 0 and scale > 0 and not step.decode_only
                 and self._prompts_unpacked(cu, lens, H // G, G, D, window, keep_first, least)):
             return self._prompts_8bit(q_at, q_stride, H, G, D, held, step, least, max_len, out, page_size, scale, window, keep_first)
         counts = unpacked_pages_4bit(cu, lens, 64, window, least, exact, keep_first)  # tiles of 64 tokens
@@ -2777,7 +2778,8 @@ class CudaOps:
         if self.timing is not None:
             self._costs(2 * half + count * 64 * 2 * G * D)
         self._call("cache_8bit", "q3_unpack_8bit", "unpack_8bit", _dtype_code(out.dtype), pages_at, num_pages, G, D, page_size,
-                   table_at + 4 * first * width, width, lens_at, seqs, longest, cu_at, least, window, keep_first, count, 0, k_at, k_at + half, per, num_items, items_at)
+                   table_at + 4 * first * width, width, lens_at, seqs, longest, cu_at, least, window, keep_first, count, 0, k_at, k_at + half, per,
+                   num_items, items_at)
         if self.timing is not None:
             self._costs(*self._attention_cost(step, H, G, D, out, prompts=True))
         group = "prompts_tiles_8bit" if D <= 128 else "prompts_tiles_wide_8bit"

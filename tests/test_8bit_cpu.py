@@ -227,6 +227,7 @@ def test_which_kernels_attention_takes():
         assert call((2, 1), kw, False) == [decode, straight] and call((2, 3), kw, False) == call((2, 3), kw) == [straight]
     assert call((2, 1), dict(D=256), True) == [decode, "q3_unpack_8bit", "q3_prompts_tiles_wide_8bit"] and call((2, 1), dict(D=48), True) == [straight]
     assert call((2, 1), dict(D=80), True) == call((2, 1), wide, True) == unpacked
+    assert call((2, 3), dict(scale=0.0), True) == call((2, 3), dict(scale=-1.0), True) == [straight]
     assert call((1, 1), dict(D=80, H=18), True) == call((2, 1), dict(H=129, G=1), True) == [straight]
 
 

@@ -55,7 +55,7 @@ def attend(ops, c, q, new, lens, H, scale, *, window=None, keep_first=0, slices=
 def score_error(row, k, scale, dtype):
     """Bound of a score's error ``[H]``: D additions of float32 to sums of |q k|, whatever their order."""
     D = row.shape[-1]
-    return scale * 2.0 ** (-22 if dtype == F32 else -23) * (D + 8) * row.double().abs().sum(-1) * k.abs().amax()
+    return abs(scale) * 2.0 ** (-22 if dtype == F32 else -23) * (D + 8) * row.double().abs().sum(-1) * k.abs().amax()
 
 
 def check_rows(got, q, c, new, lens, scale, window=None, keep_first=0, wide=False, dtype=BF16):
@@ -703,6 +703,17 @@ def test_captured_steps(ops, dtype, window, keep_first):
             else:  # (slices are cut by the same lengths)
                 assert torch.equal(s["out"], want)
             s["lens"] = now
+
+
+@pytest.mark.parametrize("dtype,H,G,D", [(BF16, 8, 2, 128), (BF16, 20, 4, 80), (BF16, 4, 2, 256), (F32, 4, 2, 64)])
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
+@pytest.mark.parametrize("new", [[1, 1], [700, 1]])
+def test_any_scale(ops, dtype, H, G, D, scale, new):
+    lens = [900, 300]
+    c = p8.Cache(lens, G, D, 16, seed=6)
+    q = queries(sum(new), H, D, 3, dtype)
+    got = attend(ops, c, q, new, lens, H, scale, dtype=dtype)
+    check_rows(got, q.view(-1, H, D), c, new, lens, scale, wide=True, dtype=dtype)
 
 
 def test_steps_of_nothing(ops):
