@@ -7,7 +7,8 @@
 //   mbar_wait(bar, parity, &abort_flag)            the block has a shared abort flag: on expiry the
 //                                                  waiter raises it and returns false; every role
 //                                                  that sees it leaves its loop, the block frees
-//                                                  what it holds and reports through an error word;
+//                                                  what it holds and reports through an error word
+//                                                  (mbar_wait_warp: by a whole warp);
 //   mbar_wait_report(bar, parity, error_word, c)   no flag: on expiry the waiter writes code c to
 //                                                  the error word and carries on, so that barriers
 //                                                  which other threads still count on are not
@@ -72,6 +73,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
   }
   return true;
+}
+// The same by a whole warp, whose lanes leave it of one mind.  What follows is theirs together (__syncwarp, loads and stores of tensor memory
+// by all 32 lanes): where some give up and others still see the barrier complete, the ones would go on without the others.  One instruction, a
+// vote and a branch that is not taken where the barrier is complete, or becomes so while the instruction holds the warp; the rest is out of line.
+__device__ __noinline__ inline bool mbar_wait_warp_on(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
+  return mbar_wait_warp_on(bar, parity, abort_flag);
 }
 // the same for a barrier on which other blocks of the cluster arrive
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {

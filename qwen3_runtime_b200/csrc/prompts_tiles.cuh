@@ -21,8 +21,8 @@
 // 14, 15 O += P V (WIDE: 4..7, 12 and 14).  An item passes through a ring of two places in shared memory.  What runs on from item to item are the rings' places
 // and the numbers of scores and weights so far, whose last bits are the barriers' phases.  Tensor memory as there: per block S [0,64), P_0 and P_1 [64,128),
 // O [128,256); WIDE: S_0 and S_1 [0,128), P_0 and P_1 [128,192), O [256,512).
-// Every wait is bounded; on expiry the block raises its abort flag and the error word, waits for its copies and products in flight, frees its tensor memory
-// and returns.
+// Every wait is bounded and, where a whole warp goes on behind it, of one mind; on expiry the block raises its abort flag and the error word, waits for its
+// copies and products in flight, frees its tensor memory and returns.
 #pragma once
 #include <type_traits>
 
@@ -68,13 +68,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-// A wait that is one instruction and a branch that is not taken where the barrier is complete; the rest is out of line.
-__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag) { return mbar_wait(bar, parity, abort_flag); }
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
-  return wait_on(bar, parity, abort_flag);
-}
-// a row's accumulators in tensor memory times `corr`; rare, and out of line for the same reason
+// a row's accumulators in tensor memory times `corr`; rare, and out of line: branches are what the softmax warps stumble over
 __device__ __noinline__ void rescale_rows(uint32_t o_addr, float corr, int cols) {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -367,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
       auto step = [&](int j, auto edge) -> bool {
         constexpr bool EDGE = decltype(edge)::value;
         const int key0 = it.at(j) * BLOCK_N, buffer = (c + j) & 1, place = WIDE ? buffer : x;
-        if (!wait(bar(S_FULL + place), WIDE ? ((c + j) >> 1) & 1 : buffer, &abort_flag)) return false;
+        if (!mbar_wait_warp(bar(S_FULL + place), WIDE ? ((c + j) >> 1) & 1 : buffer, &abort_flag)) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t sa[32], sb[32];
         const uint32_t s_addr = lane_base + (WIDE ? buffer * BLOCK_N : 0);
@@ -431,7 +425,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
         // The product before must be finished before these weights are signalled: it keeps the barrier from running a phase ahead of the waiters, the
         // next weights go where the ones before were, and O must be at rest if it has to be rescaled.  (The last item's was waited for at its end.)
         if (!EDGE || j > 0) {
-          if (!wait(bar(PV_FULL + x), buffer ^ 1, &abort_flag)) return false;
+          if (!mbar_wait_warp(bar(PV_FULL + x), buffer ^ 1, &abort_flag)) return false;
           if (__builtin_expect(moved, 0)) rescale_rows(o_addr, m_ref == m_old ? 1.f : exp2f((m_old - m_ref) * scale_log2), 64 * Z::PARTS);
         }
         // Keys behind the item's last position, and those between the first tokens and its window, are nobody's, and their values may be what is no
@@ -439,7 +433,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
         if constexpr (EDGE) {
           if (key0 + BLOCK_N - 1 > it.p_last || key0 < it.k_lo) {
             const int tile = tiles_before + j, st = tile % STAGES;
-            if (!wait(bar(V_FULL + st), (tile / STAGES) & 1, &abort_flag)) return false;
+            if (!mbar_wait_warp(bar(V_FULL + st), (tile / STAGES) & 1, &abort_flag)) return false;
             const int key = key0 + (r & 63);
             if (key > it.p_last || (key < it.k_lo && key >= keep)) {
 #pragma unroll
@@ -473,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
         }
       }
       c += my_tiles, tiles_before += it.num_tiles;
-      if (ok && my_tiles) ok = wait(bar(PV_FULL + x), (c - 1) & 1, &abort_flag);
+      if (ok && my_tiles) ok = mbar_wait_warp(bar(PV_FULL + x), (c - 1) & 1, &abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       const long at = (long)(it.tok0 + tok) * p.nq + it.kvh * p.group + head, at_slice = at * p.splits + it.slice;
       if (ok && p.splits > 1 && row_ok)
