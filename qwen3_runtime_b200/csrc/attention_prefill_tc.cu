@@ -98,16 +98,8 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// A wait that is one instruction and a branch that is not taken where the barrier is complete, or becomes so while the
-// instruction holds the warp; the rest is out of line.  (Branches are what the softmax warps stumble over.)
-__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  return mbar_wait(bar, parity, abort_flag);
-}
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
-  return wait_on(bar, parity, abort_flag);
-}
-// a row's D accumulators in tensor memory times `corr`; rare, and out of line for the same reason
+// a row's D accumulators in tensor memory times `corr`; rare, and out of line: branches are
+// what the softmax warps stumble over
 __device__ __noinline__ void rescale_rows(uint32_t o_addr, float corr) {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -392,7 +384,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
       auto step = [&](int j, auto edge) -> bool {
         constexpr bool EDGE = decltype(edge)::value;
         const int key0 = (tile0 + j) * BLOCK_N;
-        if (!wait(bar(BAR_S_FULL + x), j & 1, &abort_flag)) return false;
+        if (!mbar_wait_warp(bar(BAR_S_FULL + x), j & 1, &abort_flag)) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t sa[32], sb[32];
         tmem_load32(lane_base, sa);
@@ -460,7 +452,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         // PV_(j-1) must be finished before P_j is signalled: it keeps this barrier from running a phase ahead of the waiters,
         // P_(j+1) goes where P_(j-1) was, and O must be at rest if it has to be rescaled
         if (!EDGE || j > 0) {
-          if (!wait(bar(BAR_PV_FULL + x), (j - 1) & 1, &abort_flag)) return false;
+          if (!mbar_wait_warp(bar(BAR_PV_FULL + x), (j - 1) & 1, &abort_flag)) return false;
           if (__builtin_expect(moved, 0)) {
             rescale_rows(o_addr, m_ref == m_old ? 1.f : exp2f((m_old - m_ref) * scale_log2));
           }
@@ -471,7 +463,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
         if constexpr (EDGE) {
           if (key0 + BLOCK_N - 1 > p_last || key0 < k_lo) {
             const int vst = j % KV_STAGES;
-            if (!wait(bar(BAR_V_FULL + vst), (j / KV_STAGES) & 1, &abort_flag)) return false;
+            if (!mbar_wait_warp(bar(BAR_V_FULL + vst), (j / KV_STAGES) & 1, &abort_flag)) return false;
             const int vrow = r & 63, half = r >> 6;
             if (key0 + vrow > p_last || key0 + vrow < k_lo) {
               uint4* dst = reinterpret_cast<uint4*>(v_s + vst * V_BYTES + half * HALF_KV + vrow * 128);
@@ -506,7 +498,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __
           ok = j-- == whole1;
         }
       }
-      if (ok && my_tiles) ok = wait(bar(BAR_PV_FULL + x), (my_tiles - 1) & 1, &abort_flag);
+      if (ok && my_tiles) ok = mbar_wait_warp(bar(BAR_PV_FULL + x), (my_tiles - 1) & 1, &abort_flag);
       __syncwarp();
       if constexpr (MODE == MAPS) {
         // out = o / sqrt(mean(o^2) + eps) * out_scale, o = O_A / l_A - lambda O_B / l_B.  A row's 128 values pass from

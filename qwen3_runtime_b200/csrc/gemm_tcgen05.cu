@@ -178,7 +178,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       const int m0 = (tile % tiles_m) * BM, n0 = (tile / tiles_m) * BN;  // token tiles fastest: a weight tile stays in L2
       const int buf = i & 1;
       const int row = m0 + quarter * 32 + lane;
-      ok = mbar_wait(acc_full0 + 8 * buf, (i >> 1) & 1, &abort_flag);
+      ok = mbar_wait_warp(acc_full0 + 8 * buf, (i >> 1) & 1, &abort_flag);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t lane_addr = tmem_base + buf * ACC_COLS + ((uint32_t)(quarter * 32) << 16);
@@ -361,7 +361,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
       const int m0 = (tile % tiles_m) * (2 * BM) + rank * BM, n0 = (tile / tiles_m) * TILE_N;
       const int buf = i & 1;
       const int row = m0 + quarter * 32 + lane;
-      ok = mbar_wait(acc_full0 + 8 * buf, (i >> 1) & 1, &abort_flag);
+      ok = mbar_wait_warp(acc_full0 + 8 * buf, (i >> 1) & 1, &abort_flag);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t lane_addr = tmem_base + buf * ACC_COLS + ((uint32_t)(quarter * 32) << 16);
@@ -518,7 +518,7 @@ gemm_tcgen05_pair_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
     for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++i) {
       const int m0 = (tile % tiles_m) * (2 * BM) + rank * BM, n0 = (tile / tiles_m) * WIDE;
       const int row = m0 + quarter * 32 + lane;
-      ok = mbar_wait(acc_full, i & 1, &abort_flag);
+      ok = mbar_wait_warp(acc_full, i & 1, &abort_flag);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);

@@ -23,8 +23,14 @@ def test_the_warp_s_wait_votes_on_both_ways_out():
     assert body.count("return") == 3 and VOTED + "wait(" in body and VOTED + "try_wait(" in body
 
 
-@pytest.mark.parametrize("name", ["prompts_tiles.cuh"])
+@pytest.mark.parametrize("name", ["prompts_tiles.cuh", "attention_prefill_tc.cu"])
 def test_every_wait_is_a_warp_s(name):
     found = waits(name)
     assert found and all(VOTED in line or "mbar_wait_warp(" in line for line in found), [
         line for line in found if VOTED not in line and "mbar_wait_warp(" not in line]
+
+
+def test_the_products_epilogues_wait_as_warps():
+    """(The other waits of this source are single threads'.)"""
+    found = [line for line in waits("gemm_tcgen05.cu") if "(acc_full" in line]
+    assert len(found) == 3 and all("mbar_wait_warp(" in line for line in found), found
