@@ -257,9 +257,9 @@ template <int KD> __global__ void __launch_bounds__(THREADS, KD <= 4 ? 2 : 1) pr
     const long at = (long)(tok0 + row / G) * a.nq + kvh * G + row % G;
     if (a.splits > 1) {
       float* to = a.mid_o + (at * a.splits + blockIdx.z) * D;
-      const bool none = m[h] == MINUS_BIG;
-      if ((lane & 3) == 0) *reinterpret_cast<float2*>(a.mid_ml + 2 * (at * a.splits + blockIdx.z)) = make_float2(m[h], none ? 0.f : l[h]);
-      if (none) continue;
+      const bool seen = sees_tiles(j0, j1, firsts, skip, KEYS, pos[h], lo[h], keep);
+      if ((lane & 3) == 0) *reinterpret_cast<float2*>(a.mid_ml + 2 * (at * a.splits + blockIdx.z)) = make_float2(m[h], seen ? l[h] : NOTHING_SEEN);
+      if (!seen) continue;
 #pragma unroll
       for (int c = 0; c < 2 * KD; ++c)
         if (8 * c < D) *reinterpret_cast<float2*>(to + 8 * c + 2 * (lane & 3)) = make_float2(o[c][2 * h], o[c][2 * h + 1]);

@@ -470,8 +470,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
       if (ok && my_tiles) ok = mbar_wait_warp(bar(PV_FULL + x), (c - 1) & 1, &abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       const long at = (long)(it.tok0 + tok) * p.nq + it.kvh * p.group + head, at_slice = at * p.splits + it.slice;
-      if (ok && p.splits > 1 && row_ok)
-        *reinterpret_cast<float2*>(p.mid_ml + 2 * at_slice) = m_ref == -INFINITY ? make_float2(MINUS_BIG, 0.f) : make_float2(fmaxf(m_ref * scale_log2, -3e38f), l_run);
+      if (ok && p.splits > 1 && row_ok) {
+        const bool seen = sees_tiles(it.j0, it.j0 + my_tiles, it.firsts, it.skip, BLOCK_N, pos, lo, keep);
+        *reinterpret_cast<float2*>(p.mid_ml + 2 * at_slice) = make_float2(m_ref == -INFINITY ? MINUS_BIG : fmaxf(m_ref * scale_log2, -3e38f), seen ? l_run : NOTHING_SEEN);
+      }
       if (!ok || !my_tiles) continue;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // Out by way of shared memory, 128 bytes of a row at a time, so that a warp writes whole rows.

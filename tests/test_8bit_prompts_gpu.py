@@ -175,3 +175,75 @@ def test_captured_portions(ops, form, window, keep_first):  # noqa: F811
         sub.kv = [x[:, :, :n] for x, n in zip(c.kv, now)]
         sub.scales = [s[:, :, : -(-n // page)] for s, n in zip(c.scales, now)]
         check_rows(out.cpu().view(48, H, D), rows.view(-1, H, D), sub, new, now, D ** -0.5, window=window, keep_first=keep_first, wide=True)
+
+
+@pytest.fixture
+def sliced(ops, monkeypatch):  # noqa: F811
+    """Into how many slices the launches' tiles were cut."""
+    found = []
+    for name in ("_prompt_splits", "_tile_splits"):
+        call = getattr(ops, name)
+        monkeypatch.setattr(ops, name, lambda *args, call=call: (found.append(call(*args)), found[-1])[1], raising=False)
+    return found
+
+
+SLICED = pytest.mark.parametrize("H,G,D", [(20, 4, 80), (40, 2, 128), (8, 2, 128), (6, 3, 64), (2, 1, 256)])
+
+
+@SLICED
+@pytest.mark.parametrize("window,keep_first", [(None, 0), (2000, 70)])
+def test_rows_that_are_no_numbers_in_slices(ops, form, sliced, H, G, D, window, keep_first):  # noqa: F811
+    """A query that is none, of which one number is none, or infinite: its rows are none, all others the same bits as without it."""
+    new, lens = [37, 2], [4021, 900]
+    c = p8.Cache(lens, G, D, 16, seed=3)
+    clean = queries(39, H, D, 2)
+    q = clean.clone().view(39, H, D)
+    q[3, H - 1] = math.nan
+    q[20, 0, D - 1] = math.nan
+    q[21, 1, 5] = math.inf
+    q[38, 0, 0] = math.nan
+    args = (new, lens, H, D ** -0.5)
+    want = attend(ops, c, clean, *args, window=window, keep_first=keep_first)
+    got = attend(ops, c, q.view(39, -1), *args, window=window, keep_first=keep_first)
+    assert min(sliced) >= 1 and max(sliced) > 1
+    bad = torch.zeros((39, H), dtype=torch.bool)
+    bad[[3, 20, 21, 38], [H - 1, 0, 1, 0]] = True
+    assert bool(got[bad].isnan().all())
+    assert torch.equal(got[~bad], want[~bad]) and bool(want.isfinite().all())
+
+
+@SLICED
+@pytest.mark.parametrize("first,end", [(0, 4000), (1500, 2700), (64, 65)])
+def test_keys_that_are_no_numbers_throughout_slices(ops, form, sliced, H, G, D, first, end):  # noqa: F811
+    """Rows that see such a key are none, whatever part of their keys it is; other heads, and rows whose window begins behind it, are as ever."""
+    def mutate(b, k, v):
+        k[0, first:end] = math.nan
+
+    new, lens, R = [37], [4021], H // G
+    c, plain = p8.Cache(lens, G, D, 16, seed=3, mutate=mutate), p8.Cache(lens, G, D, 16, seed=3)
+    q = queries(37, H, D, 2)
+    for window, keep_first, hidden in ((None, 0, 0), (4000, 40, 0), (4021 - 20 - first, 0, 20)):
+        got = attend(ops, c, q, new, lens, H, D ** -0.5, window=window, keep_first=keep_first)
+        want = attend(ops, plain, q, new, lens, H, D ** -0.5, window=window, keep_first=keep_first)
+        assert torch.equal(got[:, R:], want[:, R:]) and bool(want.isfinite().all())
+        # the last row that sees the last of these keys through its window
+        sees = [window is None or max(0, lens[0] - 37 + i - window + 1) < end or first < keep_first for i in range(37)]
+        assert all(bool(got[i, :R].isnan().all()) for i in range(37) if sees[i])
+        assert all(torch.equal(got[i, :R], want[i, :R]) for i in range(37) if not sees[i])
+    assert max(sliced) > 1
+
+
+@SLICED
+@pytest.mark.parametrize("lens", [[30], [4021]])
+def test_rows_whose_scores_are_all_minus_infinity(ops, form, H, G, D, lens):  # noqa: F811
+    """No weight can be made of them: none, in one slice and in many."""
+    def mutate(b, k, v):
+        k[:, :, 7] = -1.0
+
+    c = p8.Cache(lens, G, D, 16, seed=4, mutate=mutate)
+    q = queries(20, H, D, 3).view(20, H, D)
+    q[4, 0, 7] = math.inf
+    got = attend(ops, c, q.view(20, -1), [20], lens, H, D ** -0.5)
+    assert bool(got[4, 0].isnan().all())
+    got[4, 0] = 0
+    assert bool(got.isfinite().all())
