@@ -265,10 +265,11 @@ template <int KD> __global__ void __launch_bounds__(THREADS, KD <= 4 ? 2 : 1) pr
         if (8 * c < D) *reinterpret_cast<float2*>(to + 8 * c + 2 * (lane & 3)) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
     } else {
       bf16* to = a.out + at * D;
-      const float inv = pos[h] >= 0 ? 1.f / l[h] : 0.f;  // (a token without a key: zero)
+      const float inv = 1.f / l[h];
+      const uint32_t there = pos[h] >= 0 ? 0xffffffffu : 0u;  // (a token without a key: zero)
 #pragma unroll
       for (int c = 0; c < 2 * KD; ++c)
-        if (8 * c < D) *reinterpret_cast<uint32_t*>(to + 8 * c + 2 * (lane & 3)) = pack_bf16(o[c][2 * h] * inv, o[c][2 * h + 1] * inv);
+        if (8 * c < D) *reinterpret_cast<uint32_t*>(to + 8 * c + 2 * (lane & 3)) = pack_bf16(o[c][2 * h] * inv, o[c][2 * h + 1] * inv) & there;
     }
   }
 }

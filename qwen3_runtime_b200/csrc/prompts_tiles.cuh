@@ -474,7 +474,12 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
         const bool seen = sees_tiles(it.j0, it.j0 + my_tiles, it.firsts, it.skip, BLOCK_N, pos, lo, keep);
         *reinterpret_cast<float2*>(p.mid_ml + 2 * at_slice) = make_float2(m_ref == -INFINITY ? MINUS_BIG : fmaxf(m_ref * scale_log2, -3e38f), seen ? l_run : NOTHING_SEEN);
       }
-      if (!ok || !my_tiles) continue;
+      if (!ok) continue;
+      if (!my_tiles) {  // rows without a key: zero (slices are joined to that)
+        if (p.splits == 1 && row_ok)
+          for (int col = 0; col < p.head_dim; col += 8) *reinterpret_cast<uint4*>(p.out + at * p.head_dim + col) = make_uint4(0, 0, 0, 0);
+        continue;
+      }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // Out by way of shared memory, 128 bytes of a row at a time, so that a warp writes whole rows.
       unsigned char* mine = out_s + x * STAGE_OUT + quarter * 32 * 128;
@@ -501,6 +506,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
         continue;
       }
       const float inv = 1.f / l_run;
+      const uint32_t there = pos >= 0 ? 0xffffffffu : 0u;  // (a token in front of its sequence's first key: zero)
       const unsigned long long dst = row_ok ? reinterpret_cast<unsigned long long>(p.out + at * p.head_dim) : 0;
 #pragma unroll 1
       for (int c0 = 0; c0 < p.head_dim; c0 += 64) {
@@ -514,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompts_tiles_kernel(const __grid_
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int i = 8 * (ch & 3) + 2 * e;
-            y[e] = pack2(__uint_as_float(ov[ch >> 2][i]) * inv, __uint_as_float(ov[ch >> 2][i + 1]) * inv);
+            y[e] = pack2(__uint_as_float(ov[ch >> 2][i]) * inv, __uint_as_float(ov[ch >> 2][i + 1]) * inv) & there;
           }
           *reinterpret_cast<uint4*>(mine + lane * 128 + 16 * (ch ^ (lane & 7))) = make_uint4(y[0], y[1], y[2], y[3]);
         }

@@ -2647,8 +2647,8 @@ class CudaOps:
         begin at 16 bytes, on the FMA pipes (csrc/attention_8bit.cu).  bfloat16 portions of prompts read the codes as well, turned to
         bfloat16 on the way (csrc/prompts_8bit.cu); longer ones of heads of 64 and more have their sequences' pages unpacked once (at most
         ``UNPACK_BYTES`` at a time, or one sequence) and go through the tcgen05 kernel (csrc/prompts_tiles.cuh).  Both are exact up to the weights, which are rounded to
-        bfloat16.  A table entry that is no page is read nowhere; the rows of a sequence that sees such a token are undefined, the others
-        are not.  A key that is no number makes the rows none that see it; a value, its channel of them, and of its portion's other rows too (their weight
+        bfloat16.  A token without a key (of a sequence that holds fewer tokens than the step says that it brings) gets zeros.  A table entry
+        that is no page is read nowhere; the rows of a sequence that sees such a token are undefined, the others are not.  A key that is no number makes the rows none that see it; a value, its channel of them, and of its portion's other rows too (their weight
         for it is zero)."""
         what = "paged_attention_8bit"
         D, G, H, dtype, shape, rows = head_dim, num_kv_heads, num_heads, out.dtype, q.shape, out.shape
@@ -2708,8 +2708,10 @@ class CudaOps:
             return self._prompts_8bit(q_at, q_stride, H, G, D, held, step, least, max_len, out, page_size, scale, window, keep_first)
         counts = unpacked_pages_4bit(cu, lens, 64, window, least, exact, keep_first)  # tiles of 64 tokens
         total, limit = sum(counts), self.UNPACK_BYTES // (4 * G * 64 * D)
+        if not total:  # (no key at all: nothing to unpack, and rows that are zero)
+            return self._prompts_8bit(q_at, q_stride, H, G, D, held, step, least, max_len, out, page_size, scale, window, keep_first)
         if total <= limit:
-            runs = [(0, len(counts), total)] if total else []
+            runs = [(0, len(counts), total)]
         else:
             runs = [(first, end, sum(counts[first:end])) for first, end in runs_within(counts, limit)]
         for first, end, count in runs:

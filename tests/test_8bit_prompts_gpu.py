@@ -247,3 +247,27 @@ def test_rows_whose_scores_are_all_minus_infinity(ops, form, H, G, D, lens):  # 
     assert bool(got[4, 0].isnan().all())
     got[4, 0] = 0
     assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("window,keep_first", [(None, 0), (30, 6)])
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (40, 2, 128), (6, 3, 64), (20, 4, 80), (4, 2, 256), (6, 1, 32)])
+@pytest.mark.parametrize("new,lens", [([70, 5, 40, 1], [20, 0, 300, 0]), ([100], [40]), ([130, 2], [1, 2]), ([40, 3], [0, 0]),
+                                      ([70, 40, 1], [20, 4000, 0])])
+def test_sequences_that_hold_fewer_tokens_than_they_bring(ops, form, H, G, D, new, lens, window, keep_first):  # noqa: F811
+    """Tokens in front of a sequence's first key get zeros, those with keys what they always get; with values that are no numbers as well."""
+    c = p8.Cache(lens, G, D, 16, seed=D)
+    q = queries(sum(new), H, D, H)
+    got = attend(ops, c, q, new, lens, H, D ** -0.5, window=window, keep_first=keep_first)
+    there, at = torch.zeros(sum(new), dtype=torch.bool), 0
+    for n, L in zip(new, lens):
+        there[at + n - min(n, L):at + n] = True
+        at += n
+    assert bool((got[~there] == 0).all())
+    check_rows(got[there], q.view(-1, H, D)[there], c, [min(n, L) for n, L in zip(new, lens)], lens, D ** -0.5, window=window, keep_first=keep_first,
+               wide=True)
+
+    def mutate(b, k, v):
+        v[0, :1] = math.nan
+
+    bad = p8.Cache(lens, G, D, 16, seed=D, mutate=mutate)
+    assert bool((attend(ops, bad, q, new, lens, H, D ** -0.5, window=window, keep_first=keep_first)[~there] == 0).all())
