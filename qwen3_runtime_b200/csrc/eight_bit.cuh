@@ -63,8 +63,9 @@ __device__ __forceinline__ uint32_t q8_most(const float (&x)[8]) {
   }
   return r;
 }
-// The codes of eight values.  Where none is infinite and none falls below the normal codes, where the cut is not a rounding, the conversion of the
-// hardware (to nearest, half ways to even; NaN 0x7F) gives them, two at a time.
+// The codes of eight values.  Where none is infinite or rounds to it (from 1.9375 * 2^127 on, which lies within 448 scales of the largest scale alone) and
+// none falls below the normal codes, where the cut is not a rounding, the conversion of the hardware (to nearest, half ways to even; NaN 0x7F) gives
+// them, two at a time.
 __device__ __forceinline__ uint2 q8_words(const float (&x)[8], float down) {
   float y[8], most = 0.f, least = 448.f;
 #pragma unroll
@@ -73,7 +74,7 @@ __device__ __forceinline__ uint2 q8_words(const float (&x)[8], float down) {
     most = fmaxf(most, fabsf(y[e]));
     least = fminf(least, fabsf(y[e]));
   }
-  if (least >= 0x1p-6f && most <= 464.f) {  // (464 lies halfway behind 448)
+  if (least >= 0x1p-6f && most <= 464.f && most < __fmul_rn(0x1.Fp127f, down)) {  // (464 lies halfway behind 448)
     uint32_t two[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)

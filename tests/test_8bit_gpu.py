@@ -211,6 +211,34 @@ def test_what_is_not_finite_becomes_nan_and_nothing_else(ops, bad):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [128, 64, 256, 48])
+def test_numbers_that_round_beyond_float32_under_the_largest_scale(ops, D, dtype):
+    """3.2e38 rounds to 1.875 * 2^127 and makes the scale 2^120, under which 3.4e38 (bfloat16: 3.39e38), which rounds beyond float32, is no more than 256
+    scales: not a number like elsewhere, also among large numbers; by the same bytes at every size, in the step that makes the scale and later."""
+    G, page, T = 2, 8, 5
+    g = torch.Generator().manual_seed(D)
+    qkv = (torch.rand((T, (1 + 2 * G) * D), generator=g) + 0.5) * 1e37
+    qkv[0, 2 * D + 3], qkv[2, D + 9] = 3.2e38, -3.2e38
+    for row, col in ((0, 2 * D + 1), (1, D + 1), (2, 2 * D + 17), (3, D + 10), (4, 2 * D + 30), (4, 3 * D + 30)):
+        qkv[row, col] = 3.4e38 if dtype == F32 else 3.39e38
+    qkv[4, D + 5] = -3.39e38
+    qkv = qkv.to(dtype)
+    want = torch.zeros((1, G, p8.page_bytes(D, page)), dtype=torch.uint8)
+    rows = p8.four_bits(qkv[:, D:].float().view(T, 2, G, D).permute(1, 2, 0, 3))
+    assert int(rows.isnan().sum()) == 7 and p8.scale_exponent(rows[0, 1]) == 120
+    for which in range(2):
+        for h in range(G):
+            p8.write_rows(want, 0, h, page, which, rows[which, h])
+    for cuts in ([5], [3, 1, 1]):
+        pages, at = torch.zeros_like(want).cuda(), 0
+        for n in cuts:
+            ops.qk_norm_rope_store_8bit(qkv[at:at + n].cuda(), num_heads=1, num_kv_heads=G, head_dim=D, q_weight=None, k_weight=None, eps=0.0, cos=None,
+                                        sin=None, step=p8.step_of([n], [at + n], page), block_table=i32([[0]]), pages=pages, page_size=page)
+            at += n
+        assert torch.equal(pages.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("D,rot,pairing", [(128, 128, "half"), (64, 64, "interleaved"), (256, 256, "half"), (128, 64, "half"), (80, 80, "half"),
                                            (48, 32, "interleaved"), (32, 32, "half")])
 def test_norm_and_rotation_are_those_of_the_wide_cache(ops, dtype, D, rot, pairing):
