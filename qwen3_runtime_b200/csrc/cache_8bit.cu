@@ -90,7 +90,7 @@ __device__ __forceinline__ int settle_scale(uint32_t most, int r0, int D, unsign
     const int old = q8_exponent_of(held);
     if (e > old) {
       const float shrink = e - old > 120 ? 0.f : q8_power(old - e);
-      for (int at = 16 * threadIdx.x; at < r0 * D; at += 16 * blockDim.x) {
+      for (uint32_t at = 16 * threadIdx.x; at < (uint32_t)(r0 * D); at += 16 * blockDim.x) {  // (a page's codes may end just in front of 2^31)
         uint4 w = *reinterpret_cast<const uint4*>(codes + at);
         w.x = q8_rescaled(w.x, shrink), w.y = q8_rescaled(w.y, shrink), w.z = q8_rescaled(w.z, shrink), w.w = q8_rescaled(w.w, shrink);
         *reinterpret_cast<uint4*>(codes + at) = w;

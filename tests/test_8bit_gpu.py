@@ -401,6 +401,25 @@ def test_a_long_cache(ops):
     check_rows(got, q.view(-1, 4, 128), c, [1, 1], lens, 128 ** -0.5, window=7000, keep_first=2000)
 
 
+def test_a_page_as_large_as_they_come(ops):
+    """Codes that end just in front of 2^31: those that were there are cut to the last, and no others."""
+    D, page, new = 256, (1 << 23) - 1, 5
+    pages = torch.full((1, 1, p8.page_bytes(D, page)), 0x38, dtype=torch.uint8, device="cuda")  # ones
+    pages[0, 0, 2 * page * D:2 * page * D + 8] = torch.tensor([1.0, 1.0]).view(torch.uint8).cuda()
+    x = torch.full((new, 3 * D + 1), 2.0, device="cuda")[:, : 3 * D]  # (rows that do not begin at 16 bytes: the form for all sizes)
+    x[:, ::D] = 1000.0  # rounds to 1024: under a scale of 4
+    ops.qk_norm_rope_store_8bit(x, num_heads=1, num_kv_heads=1, head_dim=D, q_weight=None, k_weight=None, eps=0.0, cos=None, sin=None,
+                                step=p8.step_of([new], [page], page), block_table=i32([[0]]), pages=pages, page_size=page)
+    ops.raise_if_kernel_error()
+    assert pages[0, 0, 2 * page * D:2 * page * D + 8].cpu().view(torch.float32).tolist() == [4.0, 4.0]
+    for codes in pages[0, 0, : 2 * page * D].view(2, page, D):
+        assert bool((codes[: page - new] == 0x28).all()), "a quarter"
+        for row in range(page - new, page):
+            want = torch.full((D,), 0x30, dtype=torch.uint8)
+            want[p8.channel_at(D, row)[0]] = 0x78
+            assert torch.equal(codes[row].cpu(), want)
+
+
 def test_offsets_beyond_32_bits(ops):
     """Pages whose bytes lie more than 2^31 (and 2^32) behind the first."""
     G, D, page = 8, 128, 16
