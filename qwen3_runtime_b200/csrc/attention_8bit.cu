@@ -546,7 +546,8 @@ __global__ void __launch_bounds__(THREADS, decode_blocks<D, NT>()) decode_8bit_k
       if (d == 0) part[QS * D + 2 * h] = top, part[QS * D + 2 * h + 1] = den;
     } else if (a.splits > 1) {
       const long where = ((long)slot * a.nq + kvh * R + h) * a.splits + split;
-      *reinterpret_cast<float4*>(a.mid_o + where * D + d) = make_float4(y[0] / den, y[1] / den, y[2] / den, y[3] / den);
+      const float by = den == 0.f ? 1.f : den;  // (all of the slice's scores beyond float32's range below: nothing beside other slices', and 2^-infinity of it)
+      *reinterpret_cast<float4*>(a.mid_o + where * D + d) = make_float4(y[0] / by, y[1] / by, y[2] / by, y[3] / by);
       if (d == 0) a.mid_lse[where] = top + log2f(den);
     } else {
       uint2 packed;

@@ -535,6 +535,30 @@ def test_scores_beyond_all_measure(ops, sign):
                 assert float((got[0, h].double() - want[0, h]).abs().max()) <= U * float(want[0, h].abs().max()) * 2
 
 
+@pytest.mark.parametrize("first,end", [(0, 200), (200, 300), (128, 256), (0, 300)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scores_beyond_float32_in_one_slice(ops, dtype, first, end):
+    """Products below -3.4e38 weigh nothing beside others, wherever slices end; where there are no others, the row is none."""
+    H, G, D, lens = 4, 2, 128, [300]
+
+    def mutate(b, k, v):
+        k[:, :, 0] = 0
+        k[:, first:end, 0] = -1e30
+
+    c = p8.Cache(lens, G, D, 16, seed=4, mutate=mutate)
+    q = torch.zeros((1, H, D), dtype=dtype)  # (the other tokens weigh alike: beside 1e30 a row's other numbers are rounded away)
+    q[0, :, 0] = 1e30
+    for slices in (1, 2, -2, 3, -3):
+        got = attend(ops, c, q.view(1, -1), [1], lens, H, D ** -0.5, slices=slices, dtype=dtype)
+        if end - first == 300:
+            assert bool(got.isnan().all())
+            continue
+        keep = [j for j in range(300) if not first <= j < end]
+        sub = p8.Cache([], G, D, 16)
+        sub.kv, sub.scales = [c.kv[0][:, :, keep]], [torch.ones((2, G, 19), dtype=torch.float64)]
+        check_rows(got, torch.zeros_like(q), sub, [1], [len(keep)], D ** -0.5, dtype=dtype)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("H,G,D,page,window,keep_first", [
     (8, 2, 128, 16, None, 0), (8, 2, 64, 8, None, 0), (8, 2, 128, 16, 20, 0), (8, 2, 128, 16, 20, 7), (4, 2, 256, 16, None, 0), (4, 2, 256, 16, 30, 20),
