@@ -2553,6 +2553,9 @@ class CudaOps:
                    int(first), int(recent), cap, _ptr(spill), _ptr(lists))
 
     # ---- a cache in 8 bits (csrc/eight_bit.cuh says how a page is laid out and how values are rounded) ----------------------
+    FARTHEST_ROWS = (1 << 31) - 1  # elements between rows that the kernels are handed
+    LONGEST_8BIT = 1 << 30  # tokens of a sequence that attention looks at, at most (a table may have room for more; places and a window's sums are 32 bits)
+
     def qk_norm_rope_store_8bit(self, qkv, *, num_heads, num_kv_heads, head_dim, q_weight, k_weight, eps, cos, sin, step, block_table, pages,
                                 page_size, write_kv=True, pairing="half", q_out=None):
         """:meth:`qk_norm_rope_store` for a cache in 8 bits: per-head q/k norm, rotation by ``step.positions``, and the write of k and v into
@@ -2576,6 +2579,8 @@ class CudaOps:
             shape, stride = q_out.shape, q_out.stride()
             if (q_out.dtype != dtype or len(shape) != 2 or shape[0] != T or shape[1] < num_heads * D or (T and stride[1] != 1)):
                 raise KernelError(f"{what}: queries go to [tokens, heads * head_dim] of the projection's type, unit-stride rows")
+        if T > 1 and max(q_stride, stride[0]) > self.FARTHEST_ROWS:
+            raise KernelError(f"{what}: rows lie 2^31 - 1 elements apart at most (got {q_stride} and {stride[0]})")
         positions = step.positions
         if positions.dtype != torch.int32 or positions.numel() < T or not positions.is_contiguous():
             raise KernelError(f"{what}: positions are dense int32, one per token")
@@ -2627,7 +2632,7 @@ class CudaOps:
         what = "unpack_8bit"
         _, (B, width) = self._check_4bit(what, pages, num_kv_heads, head_dim, page_size, block_table, kv_lens, record_of=_eight_bit_record)
         n = -(-int(max_kv_len) // page_size)
-        if n > width or max_kv_len < 0:
+        if n > width or not 0 <= max_kv_len <= self.LONGEST_8BIT:
             raise KernelError(f"{what}: max_kv_len={max_kv_len} does not fit a block table of {width} pages")
         k = torch.empty((B * n, num_kv_heads, page_size, head_dim), dtype=dtype, device=pages.device)
         v = torch.empty_like(k)
@@ -2667,9 +2672,11 @@ class CudaOps:
         if (len(shape) != 2 or shape[0] < T or shape[1] < H * D or q_stride < H * D or T != step.num_tokens
                 or q.stride() != (q_stride if shape[0] > 1 else q.stride(0), 1)):
             raise KernelError(f"{what}: queries are the first heads * head_dim columns of a row per token of the step, q_stride apart")
+        if T > 1 and q_stride > self.FARTHEST_ROWS:
+            raise KernelError(f"{what}: rows lie 2^31 - 1 elements apart at most (got {q_stride})")
         longest, seqs, max_len = step.kv_longest, step.num_seqs, step.max_kv_len
         self._check_step_4bit(what, step.cu_seqlens, seqs + 1, q, out, longest)
-        room = max_pages * page_size
+        room = min(max_pages * page_size, self.LONGEST_8BIT)
         if max_len > room or seqs > table_rows:
             raise KernelError(f"{what}: {seqs} sequences of up to {max_len} tokens do not fit a block table of {table_rows} x {max_pages} pages")
         if step.captured_width:

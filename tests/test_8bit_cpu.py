@@ -167,6 +167,44 @@ def test_attention_that_is_refused(ops, change, match):
     assert not ops.calls
 
 
+def far(T, columns, stride=1 << 31, dtype=torch.bfloat16):
+    """Rows so far apart, without their memory."""
+    return torch.empty_strided((T, columns), (stride, 1), dtype=dtype, device="meta")
+
+
+def test_rows_and_sequences_beyond_32_bits_are_refused(ops):
+    """What the kernels get of them are 32 bits: others would be somewhere else."""
+    for change in (dict(qkv=far(3, 1024)), dict(q_out=far(3, 512, dtype=torch.float32))):
+        args = store_args(**change)
+        with pytest.raises(KernelError, match="elements apart"):
+            ops.qk_norm_rope_store_8bit(args.pop("qkv"), **args)
+    args = attention_args(q=far(2, 512), q_stride=1 << 31)
+    with pytest.raises(KernelError, match="elements apart"):
+        ops.paged_attention_8bit(args.pop("q"), args.pop("q_stride"), **args)
+    assert not ops.calls
+    for T in (1, 2):  # (a single row lies nowhere else)
+        near = far(T, 1024, (1 << 31) - T)
+        args = store_args(new=(1,) * T, lens=(20,) * T, qkv=near, block_table=i32([[0, 1], [2, 3]][:T]))
+        ops.qk_norm_rope_store_8bit(args.pop("qkv"), **args)
+    args = store_args(new=(1,), lens=(20,), qkv=far(1, 1024))
+    ops.qk_norm_rope_store_8bit(args.pop("qkv"), **args)
+    assert ops.calls == ["q3_store_8bit"] * 3
+    wide = torch.empty((2, 1 << 27), dtype=torch.int32, device="meta")  # room for 2^31 tokens
+    args = attention_args(block_table=wide)
+    args["step"].max_kv_len = (1 << 30) + 1
+    with pytest.raises(KernelError, match="do not fit"):
+        ops.paged_attention_8bit(args.pop("q"), args.pop("q_stride"), **args)
+    with pytest.raises(KernelError, match="does not fit"):
+        ops.unpack_8bit(cache(), num_kv_heads=2, head_dim=128, page_size=16, block_table=wide, kv_lens=i32([1, 1]), max_kv_len=(1 << 30) + 1,
+                        dtype=torch.float32)
+    seen, taken = [], attention_args(block_table=wide)
+    taken["step"].captured_width = 1 << 27
+    call = ops._call
+    ops._call = lambda group, name, *sizes: (seen.append(sizes), call(group, name, *sizes))
+    ops.paged_attention_8bit(taken.pop("q"), taken.pop("q_stride"), **taken)
+    assert 1 << 30 in seen[0] and 1 << 31 not in seen[0], "a captured step looks as far as it can"
+
+
 class Here(Table):
     """A table whose own device is the CPU."""
 
