@@ -2676,6 +2676,8 @@ class CudaOps:
             raise KernelError(f"{what}: rows lie 2^31 - 1 elements apart at most (got {q_stride})")
         longest, seqs, max_len = step.kv_longest, step.num_seqs, step.max_kv_len
         self._check_step_4bit(what, step.cu_seqlens, seqs + 1, q, out, longest)
+        if step.decode_only and T != seqs:
+            raise KernelError(f"{what}: a step of single tokens has as many tokens as sequences (got {T} and {seqs})")
         room = min(max_pages * page_size, self.LONGEST_8BIT)
         if max_len > room or seqs > table_rows:
             raise KernelError(f"{what}: {seqs} sequences of up to {max_len} tokens do not fit a block table of {table_rows} x {max_pages} pages")

@@ -235,6 +235,7 @@ def call(new=(1, 1), kw={}, unpacked=None, **change):
     (dict(kv_lens=elsewhere([20, 3])), "launches on"), (dict(cu_seqlens=torch.tensor([0, 1, 2])), "cu_seqlens"), (dict(cu_seqlens=i32([0, 1])), "cu_seqlens"),
     (dict(cu_seqlens=elsewhere([0, 1, 2])), "launches on"),
     (dict(new=(1, 2), single_seqs=torch.tensor([0])), "single_seqs"), (dict(new=(1, 2), single_seqs=i32([])), "single_seqs"),
+    (dict(new=(1, 2), decode_only=True), "single tokens"), (dict(new=(2, 1), kw=dict(D=80), decode_only=True), "single tokens"),
     (dict(new=(1, 2), single_seqs=None), "single_seqs"), (dict(new=(1, 2), single_seqs=elsewhere([0])), "launches on"),
     (dict(kw=dict(dtype=torch.float32), token_seq=i32([0])), "token_seq"), (dict(kw=dict(dtype=torch.float32), positions=torch.tensor([0, 1])), "positions")])
 def test_what_attention_reads_of_a_step(change, match):
