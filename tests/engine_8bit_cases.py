@@ -43,3 +43,33 @@ def case_generation(tmp_path, name, dtype, ops, device, graphs=(False,)):
                 assert got == alone, (graph, kw)
             assert [len(x) for x in got] == [12] * 4 and eng.cache.num_free_pages == eng.cache.num_pages
     return alone
+
+
+def trace_of_pages(requests, page):
+    """Portions of one to three whole pages (a request's last one ends where it ends), every request in every step while it lasts."""
+    steps, at = [], dict.fromkeys(requests, 0)
+    while at:
+        entries, end = [], []
+        for i, rid in enumerate(list(at)):
+            tokens = requests[rid]
+            n = min(len(tokens) - at[rid], page * (1 + (len(steps) + i) % 3))
+            entries.append({"id": rid, "tokens": tokens[at[rid]:at[rid] + n], "want": list(range(n))})
+            at[rid] += n
+            if at[rid] == len(tokens):
+                end.append(rid)
+                del at[rid]
+        steps.append({"step": len(steps), "entries": entries, "end": end})
+    return steps
+
+
+def case_portions_of_pages(tmp_path, name, ops, device, lengths=(40, 25, 9, 33)):
+    """float32: portions that end where pages end give the bits of whole prompts, whatever their company.  A page's tokens then come together, and
+    what makes schedules differ (``case_schedules_agree``) has no place.  (Not for the CPU, where a row of PyTorch's products depends on how many there are.)"""
+    reqs = requests_of(name, lengths)
+    want = run_trace(engine(tmp_path, name, "float32", ops, device), trace_whole(reqs))
+    eng = engine(tmp_path, name, "float32", ops, device)
+    eng.runner.storage.poison_pages(0, list(range(64)))
+    got = run_trace(eng, trace_of_pages(reqs, TINY[name]["page_size"]))
+    assert got.keys() == want.keys()
+    for key, row in got.items():
+        assert bool((row == want[key]).all()), key

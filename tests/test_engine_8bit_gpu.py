@@ -27,6 +27,11 @@ def test_schedules_agree_also_with_the_plain_statements(tmp_path, ops, name):
             assert float((got[key] - row).abs().max()) <= 0.03 * float(row.abs().max())
 
 
+@pytest.mark.parametrize("name", ["A", "B", "C", "D", "E"])
+def test_portions_of_pages_are_the_whole_prompts_bit_for_bit(tmp_path, ops, name):
+    ec.case_portions_of_pages(tmp_path, name, ops, "cuda")
+
+
 @pytest.mark.parametrize("name", ["A", "C", "D", "E"])
 def test_generation_in_float32(tmp_path, ops, name):
     ec.case_generation(tmp_path, name, "float32", ops, "cuda", graphs=(False, True))
