@@ -105,8 +105,8 @@ template <int D> __device__ __forceinline__ void take_query(uint32_t (&b)[Head<D
 //   BULK   page sizes that are a multiple of 16: a tile is 16 tokens of one page, brought by one bulk copy (16 tokens a page) or three
 //          that a lane asks for, and has one scale.  Rows behind the slice's end come along and are masked.
 //   else   any page size: cp.async token by token, each with its scales; what is not there is zero.
-// What bounds it is reading the codes: eight tokens behind 17,000 to 32,768, 64 heads over 8 of 128, 79 us, 6.2 TB/s (pages of 16 bits 163); issue 0.34 a
-// clock, a warp waits for results of mma.sync and for copies about alike.  Smaller launches lose to the blocks' beginnings and ends: eight behind 4,096, 32
+// What bounds it is reading the codes: eight tokens behind 17,000 to 32,768, 64 heads over 8 of 128, 81 to 85 us over other pages each time, 5.8 to 6.0 TB/s, 78
+// over the same two sets again and again (pages of 16 bits 162); issue 0.34 a clock, a warp waits for results of mma.sync and for copies about alike.  Smaller launches lose to the blocks' beginnings and ends: eight behind 4,096, 32
 // heads over 8, 16.5 us for 10 of reading; one behind 512, 5 us, a chain of lookups, copies and a join.  No more, measured at both: rings of 2 or 4 stages, 1
 // or 4 tiles a step, 3 blocks an SM, two accumulators for the scores, values read before the softmax.  Slower: all pairs' steps behind one another, as many for
 // each warp of a launch that fills the device, its ring filled across the pairs' borders, the parts joined by a second kernel: 88, 22.5, and 48 sequences of

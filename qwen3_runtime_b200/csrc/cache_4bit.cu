@@ -46,9 +46,10 @@ __device__ __forceinline__ bool store_place(const Store& a, int t, int nkv, int 
 // ahead of the squares' sum (26), three heads a thread (41), blocks of 64 to 256 threads (24 to 28).
 //
 // A key near the border between two numbers falls on either side by float32's last bit.  So that it falls where element-wise float32
-// operations put it that anybody can repeat, heads of 128 and 256 sum their squares in a stated order, four neighbours at a time and then
-// by halves, and products and sums are rounded one by one (with fused products and another order 14 keys of 59 million fell elsewhere).
+// operations put it that anybody can repeat, heads of 128 and 256 sum their squares in a stated order, and products and sums are rounded one by
+// one (quad_of_squares and turn_rounded of rotary.cuh; with fused products and another order 14 keys of 59 million fell elsewhere).
 // Heads of 16, 32 and 64 add fused squares, as the general form below does.
+
 __device__ __forceinline__ float least_or_nan(float x, float y) {
   float z;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));

@@ -10,8 +10,8 @@
 // tiles are cut into slices, joined by a second kernel.
 //
 // What bounds it is mma.sync, which takes an SM's quarter some 27 cycles here for 16 x 8 x 16, and for few rows the chain of a tile.  us, a prompt of 2,048:
-// 16 heads over 8 of 64 89 (tcgen05: 34), 32 over 8 of 128 200 (43), 20 over 4 of 80 112 (38), 40 over 2 of 128 210 (63), 16 over 2 of 256 192 (42); 64 tokens
-// behind 4,000, 32 over 8 of 128: 38 (29); behind 16,000 89 (54).  Slices for more balance than idle SMs ask for, four blocks an SM: 84 for 89 with heads
+// 16 heads over 8 of 64 90 (tcgen05: 35), 32 over 8 of 128 203 (42), 20 over 4 of 80 110 (42), 40 over 2 of 128 213 (64), 16 over 2 of 256 186 (40); 64 tokens
+// behind 4,000, 32 over 8 of 128: 37 (28); behind 16,000 91 (52: there the tensor pipe is busy in 0.39 of the clocks, instructions wait for one another).  Slices for more balance than idle SMs ask for, four blocks an SM: 84 for 89 with heads
 // of 64, 230 for 192 with 256.
 #include "eight_bit.cuh"
 #include "mma_tiles.cuh"

@@ -11,11 +11,12 @@
 //   * Where items would leave SMs idle (a portion behind a long context), each one's tiles are cut into slices, items of their own; a second kernel joins
 //     what they leave.
 //
-// What bounds it: 0.96 us a tile of both blocks (the softmax, as there), and what an item costs beside its tiles.  With a block of the launch for each item that
+// What bounds it: 0.96 us a tile of both blocks (the softmax, as there: the tensor pipe is busy in 0.51 of the clocks, WIDE 0.58, the exponentials' in 0.41 and
+// 0.24, and warps wait for tensor memory most), and what an item costs beside its tiles.  With a block of the launch for each item that
 // was 6.5 us (1.1 between two blocks, 0.5 for the item, 2.8 until the first scores, 2 to 2.6 at the end), now the end's.  us, with the unpacking, 32 heads over
-// 8 of 128, in blocks that stay and one for each item: 1,500 + 701 + 1,000 (behind 2,048) tokens and a single one 78, 87; 700 + 2,048 + 500 (behind 5,000) under
-// a window of 1,024 59, 67 (straight over the codes 210); a prompt of 2,048 43, 47.  In slices and without: 64 tokens behind 4,000 29, 64; behind 16,000 54,
-// 230.  WIDE, 16 heads over 2 of 256, and straight over the codes: a prompt of 2,048 42, 192; the first of the above 78, 387.
+// 8 of 128, in blocks that stay and one for each item: 1,500 + 701 + 1,000 (behind 2,048) tokens and a single one 79, 87; 700 + 2,048 + 500 (behind 5,000) under
+// a window of 1,024 59, 67 (straight over the codes 230); a prompt of 2,048 42, 47.  In slices and without: 64 tokens behind 4,000 28, 64; behind 16,000 52,
+// 230.  WIDE, 16 heads over 2 of 256, and straight over the codes: a prompt of 2,048 40, 186; the first of the above 77, 387.
 //
 // Warps:  0 takes items and brings keys, 1 values, 2 queries;  4..7 and 8..11 softmax of block A and B, one thread per row;  12, 13 issue S = Q K^T,
 // 14, 15 O += P V (WIDE: 4..7, 12 and 14).  An item passes through a ring of two places in shared memory.  What runs on from item to item are the rings' places

@@ -511,7 +511,7 @@ def chunk_segment(cu, H, D, Dv, sms, seg) -> int:
 
 
 def unpacked_pages_4bit(cu, kv_lens, page_size, window=None, least=1, exact=True, keep_first=0) -> list:
-    """Pages that attention over prompts reads of each sequence of a step (tokens ``cu[b]`` to ``cu[b + 1] - 1``, ``kv_lens[b]`` keys): from
+    """Pages that attention over prompts reads of each sequence of a step over a cache in 4 bits, or tiles in 8 (tokens ``cu[b]`` to ``cu[b + 1] - 1``, ``kv_lens[b]`` keys): from
     the first that its first new token's window reaches to the last, and those of its first ``keep_first`` tokens; none of a sequence that brings fewer than ``least`` tokens.  Not
     ``exact``: as many as any shorter length asks for, too."""
     counts = []
@@ -2561,7 +2561,9 @@ class CudaOps:
         """:meth:`qk_norm_rope_store` for a cache in 8 bits: per-head q/k norm, rotation by ``step.positions``, and the write of k and v into
         ``pages`` (uint8 ``[pages, kv heads, eight_bit_page_bytes(head_dim, page_size)]``).  A sequence's new tokens are the last of its
         ``step.kv_lens`` places, so what its last page held before is known: it goes on under a scale that grows when it has to (a page that
-        gets its first token starts anew).  A page belongs to one sequence; tokens whose place or page lies outside the table or
+        gets its first token starts anew).  The same rows leave the same bytes however they are cut into steps; but numbers below 2^-6 of the scale
+        are cut, by less than 2^-9 of it, so what attention reads of a page depends on the tokens that are in it by then, later ones of the same portion among
+        them.  A page belongs to one sequence and stands in its table once; tokens whose place or page lies outside the table or
         the pages are written nowhere.  Queries go to ``q_out`` ``[T, num_heads * head_dim]``, or are changed in place."""
         what = "qk_norm_rope_store_8bit"
         D, dtype, shape, stride = head_dim, qkv.dtype, qkv.shape, qkv.stride()
@@ -2653,8 +2655,8 @@ class CudaOps:
         bfloat16 on the way (csrc/prompts_8bit.cu); longer ones of heads of 64 and more have their sequences' pages unpacked once (at most
         ``UNPACK_BYTES`` at a time, or one sequence) and go through the tcgen05 kernel (csrc/prompts_tiles.cuh).  Both are exact up to the weights, which are rounded to
         bfloat16.  A token without a key (of a sequence that holds fewer tokens than the step says that it brings) gets zeros.  A table entry
-        that is no page is read nowhere; the rows of a sequence that sees such a token are undefined, the others are not.  A key that is no number makes the rows none that see it; a value, its channel of them, and of its portion's other rows too (their weight
-        for it is zero)."""
+        that is no page is read nowhere; the rows of a sequence that sees such a token are undefined, the others are not.  A key that is no number makes the rows none that see it, a query its own rows; a value, its channel of them, and of its portion's other
+        rows too (their weight for it is zero)."""
         what = "paged_attention_8bit"
         D, G, H, dtype, shape, rows = head_dim, num_kv_heads, num_heads, out.dtype, q.shape, out.shape
         (num_pages, *_), (table_rows, max_pages) = self._check_4bit(what, pages, G, D, page_size, block_table, step.kv_lens,
