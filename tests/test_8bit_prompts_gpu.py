@@ -271,3 +271,40 @@ def test_sequences_that_hold_fewer_tokens_than_they_bring(ops, form, H, G, D, ne
 
     bad = p8.Cache(lens, G, D, 16, seed=D, mutate=mutate)
     assert bool((attend(ops, bad, q, new, lens, H, D ** -0.5, window=window, keep_first=keep_first)[~there] == 0).all())
+
+
+@pytest.mark.parametrize("H,G,D", [(10, 2, 128), (4, 2, 256)])
+def test_captured_portions_of_sequences_that_hold_fewer_tokens(ops, form, H, G, D):  # noqa: F811
+    """What is captured for sequences that hold their tokens holds for ones that do not: those in front of the first key get zeros."""
+    page, new = 16, [40, 1, 70]
+    width, full = 1024 // page, [60, 90, 700]
+    c = p8.Cache([1024] * 3, G, D, page, seed=8, width=width)
+    pages, table = c.pages.cuda(), c.table.cuda()
+    q = queries(111, H, D, 5)
+    dev, out = q.cuda(), torch.zeros((111, H * D), dtype=BF16, device="cuda")
+    step = p8.step_of(new, full, page, captured_width=width)
+
+    def run():
+        ops.paged_attention_8bit(dev, H * D, num_heads=H, pages=pages, block_table=table, out=out, scale=D ** -0.5, step=step, **sizes(c))
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for now in (full, [0, 0, 0], [39, 1, 20], [0, 90, 1024], [1, 0, 69]):
+        step.kv_lens.copy_(i32(now))
+        step.positions.copy_(i32([L - n + i for n, L in zip(new, now) for i in range(n)]))
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.raise_if_kernel_error()
+        got, there, at = out.cpu().view(111, H, D), torch.zeros(111, dtype=torch.bool), 0
+        for n, L in zip(new, now):
+            there[at + n - min(n, L):at + n] = True
+            at += n
+        assert bool((got[~there] == 0).all())
+        sub = p8.Cache([], G, D, page)
+        sub.kv = [x[:, :, :n] for x, n in zip(c.kv, now)]
+        sub.scales = [s[:, :, : -(-n // page)] for s, n in zip(c.scales, now)]
+        check_rows(got[there], q.view(-1, H, D)[there], sub, [min(n, L) for n, L in zip(new, now)], now, D ** -0.5, wide=True)
